@@ -524,6 +524,121 @@ int me_mask_media(const void *ids, int ids_dtype, int64_t n, int64_t width, int6
                   const void *media_ids, int media_dtype, int32_t n_media, int32_t *ids_out,
                   uint8_t *keep_out, void *stream);
 
+/* ---- losses over logits ---------------------------------------------------------------
+ * The reference trains with cross-entropy over the vocabulary (micro_engram/train/head.py);
+ * these are the losses that follow it. Common arguments:
+ *
+ *   logits      [n, vocab] of dtype (ME_BF16 / ME_F32): row r starts at element
+ *               (r / rows_per_batch) * batch_stride + (r % rows_per_batch) * row_stride, its
+ *               values next to each other; rows may start at any element. vocab <= 2,097,152.
+ *   targets     [n] token ids of targets_dtype (ME_I32 / ME_I64). A row whose target is
+ *               ignore_index or outside [0, vocab) does not count: it is not read, its values
+ *               are 0 and its gradient is zeros.
+ *   temperature logits are divided by it (1e-6..1e6)
+ *   row_stats   [n, 2] fp32, coef [n] fp32: what the gradient needs of each row
+ *   grad        [n, vocab] of the logits' dtype, contiguous
+ *   upstream    device scalar, the loss's own gradient (NULL: 1). With done_for_one != 0,
+ *               grad already holds the gradient for an upstream of 1, and nothing is written
+ *               if it is 1.
+ *   sequences   seq_offsets [n_seqs + 1] of offsets_dtype (rows seq_offsets[s] up to
+ *               seq_offsets[s + 1]; clamped to 0..n; rows of no sequence do not count), or
+ *               NULL: n_seqs sequences of seq_len rows each
+ *   workspace   me_loss_workspace_size(n, vocab, pairs or 0) bytes, 256-byte aligned
+ */
+#define ME_REDUCE_MEAN 0     /* over the rows that count */
+#define ME_REDUCE_SUM 1
+#define ME_REDUCE_SEQUENCE 2 /* mean of the sequences' means */
+#define ME_PAIR_SIGMOID 0
+#define ME_PAIR_IPO 1
+#define ME_PAIR_HINGE 2
+
+int me_loss_workspace_size(int64_t n, int64_t vocab, int64_t pairs, size_t *bytes);
+
+/*
+ * me_token_logps -- logps[r] = log softmax(logits[r] / temperature)[targets[r]], fp32.
+ * row_stats nullable (no gradient wanted).
+ */
+int me_token_logps(const void *logits, int dtype, int64_t n, int64_t vocab, int64_t rows_per_batch,
+                   int64_t batch_stride, int64_t row_stride, const void *targets, int targets_dtype,
+                   int64_t ignore_index, double temperature, float *logps, float *row_stats,
+                   void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * me_token_logps_backward -- grad[r][j] = c (1[j = targets[r]] - softmax(logits[r] / temperature)[j])
+ * with c = coef[r] * coef_scale * upstream: the gradient of me_token_logps (coef = the
+ * log-probabilities' gradient, coef_scale = 1 / temperature), and from the coef that they
+ * leave of me_preference and me_policy (coef_scale = 1).
+ */
+int me_token_logps_backward(const void *logits, int dtype, int64_t n, int64_t vocab,
+                            int64_t rows_per_batch, int64_t batch_stride, int64_t row_stride,
+                            const void *targets, int targets_dtype, int64_t ignore_index,
+                            double temperature, const float *row_stats, const float *coef,
+                            double coef_scale, const float *upstream, int done_for_one, void *grad,
+                            void *stream);
+
+/*
+ * me_preference -- mean over pairs of a loss of h = D(chosen) - D(rejected), D of a sequence the
+ * sum (normalized != 0: the mean) of logp - ref_logps over its rows that count. Sequences 0 ..
+ * pairs - 1 are the chosen ones, pairs .. 2 pairs - 1 the rejected ones.
+ *   kind  ME_PAIR_SIGMOID: -(1 - smoothing) log sigmoid(beta h) - smoothing log sigmoid(-beta h);
+ *         ME_PAIR_IPO: (h - 1 / (2 beta))^2; ME_PAIR_HINGE: max(0, 1 - beta h)
+ *   chosen, rejected  [pairs] fp32: beta D
+ * Gradient: me_token_logps_backward. No pairs: loss 0.
+ */
+int me_preference(const void *logits, int dtype, int64_t n, int64_t vocab, int64_t rows_per_batch,
+                  int64_t batch_stride, int64_t row_stride, const void *targets, int targets_dtype,
+                  int64_t ignore_index, const float *ref_logps, const void *seq_offsets,
+                  int offsets_dtype, int64_t pairs, int64_t seq_len, int kind, double beta,
+                  double smoothing, int normalized, float *loss, float *chosen, float *rejected,
+                  float *row_stats, float *coef, void *workspace, size_t workspace_bytes,
+                  void *stream);
+
+/*
+ * me_policy -- scale * sum over rows of weight * L, weight by `reduction`,
+ *   L = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(d) - d - 1),
+ *   r = exp(logp - old_logps), d = ref_logps - logp (ref_logps NULL: no KL term).
+ *   advantages  [n], or with adv_per_seq != 0 [n_seqs]
+ *   logps       [n] fp32; out_stats [2] fp32: means over the rows that count of the KL term and
+ *               of the clipped rows
+ *   grad        nullable: the gradient for an upstream of 1 (any other:
+ *               me_token_logps_backward with done_for_one)
+ */
+int me_policy(const void *logits, int dtype, int64_t n, int64_t vocab, int64_t rows_per_batch,
+              int64_t batch_stride, int64_t row_stride, const void *targets, int targets_dtype,
+              int64_t ignore_index, const float *old_logps, const float *advantages,
+              int adv_per_seq, const float *ref_logps, const void *seq_offsets, int offsets_dtype,
+              int64_t n_seqs, int64_t seq_len, double clip_low, double clip_high, double kl_coef,
+              double temperature, double scale, int reduction, float *loss, float *logps,
+              float *out_stats, float *row_stats, float *coef, void *grad, void *workspace,
+              size_t workspace_bytes, void *stream);
+
+/*
+ * me_distill -- scale * sum over rows of weight * temperature^2 * KL(teacher | softmax(logits /
+ * temperature)), the teacher given by its `top` (<= 1024) highest logits of each row.
+ *   teacher_ids [n, top] of ids_dtype; entries outside [0, vocab) are left out (a row of only
+ *               such does not count), entries with the same id add up
+ *   teacher     [n, top] of teacher_dtype (ME_BF16 / ME_F32): the teacher's logits there
+ *   teacher_lse NULL: the teacher is its softmax over the entries. Else [n] fp32: log of the sum
+ *               over the whole vocabulary of exp(teacher logit / temperature); all tokens
+ *               that are no entry are then one class more, of the probability that is left
+ *   mask        nullable [n]: rows with 0 do not count
+ *   reduction   ME_REDUCE_MEAN or ME_REDUCE_SUM
+ *   fix         [n, top] fp32: the gradient at the entries before the row's factor
+ *   grad        nullable: the gradient for an upstream of 1 (any other: me_distill_backward)
+ */
+int me_distill(const void *logits, int dtype, int64_t n, int64_t vocab, int64_t rows_per_batch,
+               int64_t batch_stride, int64_t row_stride, const void *teacher_ids, int ids_dtype,
+               const void *teacher, int teacher_dtype, int64_t top, const float *teacher_lse,
+               const uint8_t *mask, double temperature, double scale, int reduction, float *loss,
+               float *row_stats, float *coef, float *fix, void *grad, void *workspace,
+               size_t workspace_bytes, void *stream);
+
+int me_distill_backward(const void *logits, int dtype, int64_t n, int64_t vocab,
+                        int64_t rows_per_batch, int64_t batch_stride, int64_t row_stride,
+                        const void *teacher_ids, int ids_dtype, int64_t top, double temperature,
+                        const float *row_stats, const float *coef, const float *fix,
+                        const float *upstream, int done_for_one, void *grad, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -17,6 +17,11 @@ ME_I32, ME_I64, ME_F32, ME_BF16, ME_U8 = 1, 2, 3, 4, 5
 ME_GATE_SCALAR, ME_GATE_SCALAR_SQRT = 0, 1
 ME_MAX_TABLES, ME_MAX_ORDER = 64, 8
 
+ME_REDUCE_MEAN, ME_REDUCE_SUM, ME_REDUCE_SEQUENCE = 0, 1, 2
+ME_PAIR_SIGMOID, ME_PAIR_IPO, ME_PAIR_HINGE = 0, 1, 2
+
+_LOGITS = [c_ptr, c_int, c_i64, c_i64, c_i64, c_i64, c_i64]  # logits..row_stride
+_TARGETS = [c_ptr, c_int, c_i64]  # targets, dtype, ignore_index
 _HASH_COMMON = [c_ptr, c_i64, c_ptr, c_i32, c_i32, c_ptr, c_ptr, c_i64]  # canon..pad_id
 # name -> argtypes; every function returns int (ME_OK or a negative error code)
 SIGNATURES = {
@@ -68,6 +73,19 @@ SIGNATURES = {
                            c_ptr, c_int, c_ptr, c_int, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64,
                            c_ptr, c_int, c_i32, c_ptr, c_ptr],
     "me_mask_media": [c_ptr, c_int, c_i64, c_i64, c_i64, c_ptr, c_int, c_i32, c_ptr, c_ptr, c_ptr],
+    "me_loss_workspace_size": [c_i64, c_i64, c_i64, ctypes.POINTER(c_size)],
+    "me_token_logps": [*_LOGITS, *_TARGETS, c_double, c_ptr, c_ptr, c_ptr, c_size, c_ptr],
+    "me_token_logps_backward": [*_LOGITS, *_TARGETS, c_double, c_ptr, c_ptr, c_double, c_ptr, c_int, c_ptr,
+                                c_ptr],
+    "me_preference": [*_LOGITS, *_TARGETS, c_ptr, c_ptr, c_int, c_i64, c_i64, c_int, c_double, c_double,
+                      c_int, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_size, c_ptr],
+    "me_policy": [*_LOGITS, *_TARGETS, c_ptr, c_ptr, c_int, c_ptr, c_ptr, c_int, c_i64, c_i64, c_double,
+                  c_double, c_double, c_double, c_double, c_int, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr,
+                  c_ptr, c_size, c_ptr],
+    "me_distill": [*_LOGITS, c_ptr, c_int, c_ptr, c_int, c_i64, c_ptr, c_ptr, c_double, c_double, c_int,
+                   c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_size, c_ptr],
+    "me_distill_backward": [*_LOGITS, c_ptr, c_int, c_i64, c_double, c_ptr, c_ptr, c_ptr, c_ptr, c_int, c_ptr,
+                            c_ptr],
 }
 
 _lock = threading.Lock()

@@ -1,0 +1,570 @@
+"""The losses over logits on the GPU against float64 (loss_reference.py, which also derives the tolerances):
+sizes from one token and one row up, odd vocabularies, strided views, rows that do not count and hold NaN
+or infinities, rows at the type's lowest value, empty sequences, repeated and missing teacher entries,
+gradients by formula and by differences, an upstream gradient other than 1."""
+import math
+
+import pytest
+import torch
+
+import loss_reference as ref64
+from loss_reference import HALF_ULP, REL
+from micro_engram_fork_amd import losses, loss_ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+DTYPES = [torch.bfloat16, torch.float32]
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _logits(n, vocab, dtype, seed, scale=2.0):
+    """CPU logits in dtype, a raised token in each row."""
+    g = _gen(seed)
+    x = torch.randn(n, vocab, generator=g) * scale
+    hot = torch.randint(0, vocab, (n, 1), generator=g)
+    x.scatter_(1, hot, math.log(vocab) + 2 + torch.randn(n, 1, generator=g))
+    return x.to(dtype), hot.squeeze(1)
+
+
+def _close(got, want, tol, what):
+    got, want = got.detach().double().cpu(), want.detach().double()
+    assert got.shape == want.shape, what
+    bad = ~((got - want).abs() <= tol) & ~(got.isnan() & want.isnan()) & ~(got == want)
+    assert not bool(bad.any()), f"{what}: off by {float((got - want).abs()[bad].max()):.3g}, {int(bad.sum())} values"
+
+
+def _grad_tol(coef, probs, targets, dtype, want):
+    """coef [n] (magnitudes), probs [n, vocab] of the softmax."""
+    base = probs.clone()
+    base.scatter_add_(1, targets.clamp(0, probs.shape[1] - 1)[:, None], torch.ones(len(targets), 1, dtype=probs.dtype))
+    return coef.abs()[:, None] * base * REL + want.abs() * HALF_ULP[dtype] + 1e-37
+
+
+def _probs(logits64, temperature=1.0):
+    return torch.softmax(torch.nan_to_num(logits64, nan=0.0) / temperature, dim=-1)
+
+
+# --------------------------------------------------------------------------- log-probabilities
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,vocab", [(1, 1), (3, 2), (5, 7), (2, 8), (3, 9), (4, 255), (70, 1000), (3, 2047), (2, 2048),
+                                     (2, 2049), (5, 32_003), (1, 262_144), (3, 131_075)])
+def test_token_logps_and_gradient(dtype, n, vocab):
+    x, hot = _logits(n, vocab, dtype, n * 7 + vocab)
+    targets = hot.clone()
+    if n > 2:
+        targets[1] = -100
+        targets[2] = (int(hot[2]) + 1) % vocab
+    weights = torch.randn(n, generator=_gen(5))
+    temp = 0.8
+    leaf = x.double().requires_grad_()
+    want = ref64.token_logps(leaf, targets, temp)
+    want_grad, = torch.autograd.grad((want * weights.double()).sum(), leaf)
+    xg = x.to(DEV).requires_grad_()
+    got = losses.token_logps(xg, targets.to(DEV), temperature=temp)
+    grad, = torch.autograd.grad(got, xg, weights.to(DEV))
+    _close(got, want, REL + 1e-6 * want.detach().abs(), "logps")
+    ok = ref64.counted(targets, vocab)
+    _close(grad, want_grad, _grad_tol(weights.double() * ok / temp, _probs(x.double(), temp), targets, dtype, want_grad), "grad")
+    with torch.no_grad():
+        assert torch.equal(losses.token_logps(xg, targets.to(DEV).int(), temperature=temp), got)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("layout", ["shift", "padded", "both", "four_dims", "transposed", "expanded", "offset"])
+def test_layouts_equal_contiguous_rows(dtype, layout):
+    b, t, vocab = 3, 5, 1003
+    x, hot = _logits(b * (t + 1), vocab, dtype, 3)
+    base = x.to(DEV).view(b, t + 1, vocab)
+    if layout == "shift":
+        view = base[:, :-1]
+    elif layout in ("padded", "both"):
+        wide = torch.full((b, t + 1, vocab + 13), float("nan"), dtype=dtype, device=DEV)
+        wide[..., :vocab] = base
+        view = wide[:, 1:, :vocab] if layout == "both" else wide[..., :vocab]
+    elif layout == "four_dims":
+        view = base.view(1, b, t + 1, vocab).expand(2, b, t + 1, vocab)[:, :, 1:]
+    elif layout == "transposed":
+        view = base.transpose(0, 1)
+    elif layout == "expanded":
+        view = base[:, :1].expand(b, 4, vocab)
+    else:
+        flat = torch.empty(base.numel() + 1, dtype=dtype, device=DEV)
+        flat[1:] = base.reshape(-1)
+        view = flat[1:].view(base.shape)
+    targets = torch.randint(0, vocab, view.shape[:-1], generator=_gen(9)).to(DEV)
+    weights = torch.randn(view.shape[:-1], generator=_gen(4)).to(DEV)
+    results = []
+    for logits in (view, view.contiguous().clone()):
+        logits = logits.detach().requires_grad_()
+        out = losses.token_logps(logits, targets)
+        grad, = torch.autograd.grad(out, logits, weights)
+        results.append((out, grad))
+    assert torch.equal(results[0][0], results[1][0]) and torch.equal(results[0][1], results[1][1])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_values_in_rows_that_do_not_count_reach_nothing(dtype):
+    vocab = 515
+    x, hot = _logits(6, vocab, dtype, 11)
+    targets = torch.tensor([int(hot[0]), -100, 7, vocab, -1, int(hot[5])])
+    bad = x.clone()
+    bad[1], bad[3], bad[4] = float("nan"), float("inf"), -float("inf")
+    bad[2, 100:] = -float("inf")  # tokens ruled out
+    bad[5, 3] = torch.finfo(dtype).min
+    xg = bad.to(DEV).requires_grad_()
+    got = losses.token_logps(xg, targets.to(DEV), ignore_index=-100)
+    grad, = torch.autograd.grad(got.sum(), xg)
+    clean = torch.where(ref64.counted(targets, vocab)[:, None], bad.double(), torch.zeros_like(bad.double()))
+    want = ref64.token_logps(clean, targets)
+    _close(got, want, REL + 1e-6 * want.abs(), "logps")
+    assert bool(torch.isfinite(grad).all())
+    for r in (1, 3, 4):
+        assert int(grad[r].count_nonzero()) == 0 and float(got[r]) == 0.0
+    assert int(grad[2, 100:].count_nonzero()) == 0
+    # the ignored index may be a token
+    other = losses.token_logps(xg, targets.to(DEV), ignore_index=7)
+    assert float(other[2]) == 0.0 and float(other[0]) == float(got[0])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_of_the_lowest_value_and_of_infinities(dtype):
+    vocab = 300
+    x = torch.zeros(4, vocab, dtype=dtype)
+    x[0] = torch.finfo(dtype).min
+    x[1] = torch.finfo(dtype).max
+    x[2] = -float("inf")
+    x[3, 5] = float("inf")
+    xg = x.to(DEV).requires_grad_()
+    out = losses.token_logps(xg, torch.tensor([3, 4, 5, 6], device=DEV))
+    grad, = torch.autograd.grad(out.sum(), xg)
+    assert out[:2].tolist() == pytest.approx([-math.log(vocab)] * 2, rel=1e-6)
+    assert bool(out[2:].isnan().all())
+    assert float(grad[0, 0]) == pytest.approx(-1 / vocab, rel=2.0 ** -8)
+    assert float(grad[1, 4]) == pytest.approx(1 - 1 / vocab, rel=2.0 ** -8)
+
+
+def test_large_row_offsets():
+    # row starts past 2^32 elements of the tensor (a view: the memory between the rows is not touched)
+    vocab, rows = 1024, 3
+    stride = (1 << 31) + 8
+    base = torch.empty((rows - 1) * stride + vocab, dtype=torch.bfloat16, device=DEV)
+    view = base.as_strided((rows, vocab), (stride, 1))
+    x, hot = _logits(rows, vocab, torch.bfloat16, 2)
+    view.copy_(x.to(DEV))
+    assert torch.equal(losses.token_logps(view, hot.to(DEV)), losses.token_logps(x.to(DEV), hot.to(DEV)))
+
+
+@pytest.mark.parametrize("shape", [(0, 10), (2, 0, 10)])
+def test_no_rows(shape):
+    x = torch.zeros(shape, device=DEV, requires_grad=True)
+    targets = torch.zeros(shape[:-1], dtype=torch.long, device=DEV)
+    out = losses.token_logps(x, targets)
+    grad, = torch.autograd.grad(out.sum(), x)
+    assert out.shape == targets.shape and grad.shape == x.shape
+    rows = torch.zeros(shape[:-1], device=DEV)
+    loss, logps, stats = losses.policy_loss(x, targets, rows, rows)
+    assert float(loss) == 0 and logps.shape == targets.shape and stats.tolist() == [0, 0]
+    assert torch.autograd.grad(loss, x)[0].shape == x.shape
+    top = torch.zeros((*shape[:-1], 3), dtype=torch.long, device=DEV)
+    assert float(losses.distill_loss(x, top, top.float())) == 0
+    if len(shape) == 3:
+        loss, chosen, rejected = losses.preference_loss(x, targets, rows)
+        assert float(loss) == pytest.approx(math.log(2)) and chosen.tolist() == [0] and rejected.tolist() == [0]
+
+
+# ---------------------------------------------------------------------------------- preference
+def _preference_case(pairs, longest, vocab, dtype, seed, empty=False):
+    g = _gen(seed)
+    lengths = torch.randint(1, longest + 1, (2 * pairs,), generator=g)
+    if empty:
+        lengths[0] = 0
+        lengths[-1] = 0
+    offsets = [0, *lengths.cumsum(0).tolist()]
+    n = offsets[-1]
+    x, targets = _logits(n, vocab, dtype, seed + 1)
+    targets[torch.rand(n, generator=g) < 0.2] = -100
+    ref = ref64.token_logps(x.double(), targets) + 0.3 * torch.randn(n, generator=g)
+    return x, targets, ref.float(), offsets
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind,smoothing,normalized", [("sigmoid", 0.0, False), ("sigmoid", 0.2, True), ("ipo", 0.0, True),
+                                                       ("ipo", 0.0, False), ("hinge", 0.0, False)])
+@pytest.mark.parametrize("pairs,longest,vocab,empty", [(1, 1, 40, False), (2, 9, 1001, True), (17, 70, 130, False)])
+def test_preference(dtype, kind, smoothing, normalized, pairs, longest, vocab, empty):
+    x, targets, ref, offsets = _preference_case(pairs, longest, vocab, dtype, pairs + longest, empty)
+    n, beta = len(targets), 0.5
+    leaf = x.double().requires_grad_()
+    want = ref64.preference(leaf, targets, ref, offsets, beta, kind, smoothing, normalized)
+    want_grad, = torch.autograd.grad(want[0], leaf)
+    xg = x.to(DEV).requires_grad_()
+    got = losses.preference_loss(xg, targets.to(DEV), ref.to(DEV), cu_seqlens=torch.tensor(offsets, device=DEV), beta=beta,
+                                 loss_type=kind, label_smoothing=smoothing, length_normalized=normalized)
+    grad, = torch.autograd.grad(got[0], xg)
+    # D: up to `longest` log-probabilities off by REL and one rounding of D itself
+    off = REL * (1 if normalized else longest) + 2e-7 * float(torch.cat(want[1:]).abs().max() / beta + 1)
+    h = float((want[1] - want[2]).abs().max()) / beta
+    slope = {"sigmoid": beta, "ipo": 2 * (h + 1 / beta), "hinge": beta}[kind]
+    _close(got[1], want[1], beta * off, "chosen")
+    _close(got[2], want[2], beta * off, "rejected")
+    _close(got[0], want[0], 2 * slope * off + 1e-6 * want[0].abs() + 1e-7, "loss")
+    # the gradient's factor: its own derivative by h times the error of h
+    bend = {"sigmoid": beta * beta / 4, "ipo": 2.0, "hinge": 0.0}[kind]
+    seq = ref64.sequence_of(n, offsets)
+    ok = ref64.counted(targets, vocab)
+    factor = torch.full((n,), (2 * off * bend / slope + REL) * slope / pairs, dtype=torch.float64) * ok
+    tol = _grad_tol(factor / REL + slope / pairs * ok, _probs(x.double()), targets, dtype, want_grad)
+    _close(grad, want_grad, tol, "grad")
+    assert int(grad.cpu()[~ok].count_nonzero()) == 0 and int((seq < 0).sum()) == 0
+
+
+def test_preference_dense_rows_equal_packed_ones():
+    x, targets, ref, _ = _preference_case(4, 1, 300, torch.bfloat16, 3)
+    x, hot = _logits(8 * 6, 300, torch.bfloat16, 4)
+    ref = torch.randn(48, generator=_gen(1))
+    a = losses.preference_loss(x.to(DEV).view(8, 6, 300), hot.to(DEV).view(8, 6), ref.to(DEV).view(8, 6))
+    b = losses.preference_loss(x.to(DEV), hot.to(DEV), ref.to(DEV), cu_seqlens=torch.arange(0, 49, 6, device=DEV, dtype=torch.int32))
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_preference_offsets_outside_the_rows_and_rows_of_no_sequence():
+    # offsets are clamped to the rows; rows before the first and after the last take no gradient
+    x, hot = _logits(12, 65, torch.float32, 8)
+    ref = torch.randn(12, generator=_gen(1)).to(DEV)
+    xg = x.to(DEV).requires_grad_()
+    got = losses.preference_loss(xg, hot.to(DEV), ref, cu_seqlens=torch.tensor([2, 7, 10], device=DEV))
+    grad, = torch.autograd.grad(got[0], xg)
+    assert int(grad[:2].count_nonzero()) == 0 and int(grad[10:].count_nonzero()) == 0
+    assert bool((grad[2:10].abs().sum(1) > 0).all())
+    wide = losses.preference_loss(xg, hot.to(DEV), ref, cu_seqlens=torch.tensor([-5, 7, 99], device=DEV))
+    same = losses.preference_loss(xg, hot.to(DEV), ref, cu_seqlens=torch.tensor([0, 7, 12], device=DEV))
+    assert torch.equal(wide[0], same[0])
+
+
+# -------------------------------------------------------------------------------------- policy
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("reduction,reference,per_seq,packed", [("token", True, True, False), ("sequence", False, True, True),
+                                                                ("sequence", True, False, False), ("sum", True, False, True),
+                                                                ("token", False, False, True)])
+@pytest.mark.parametrize("b,t,vocab", [(1, 1, 33), (3, 7, 515), (5, 60, 131), (2, 3, 70_001)])
+def test_policy(dtype, reduction, reference, per_seq, packed, b, t, vocab):
+    n = b * t
+    g = _gen(n + vocab)
+    x, targets = _logits(n, vocab, dtype, n)
+    if n > 1:
+        targets[torch.rand(n, generator=g) < 0.3] = -100
+    temp, lo, hi, kl, scale = 1.3, 0.2, 0.25, 0.1, 0.5
+    ok = ref64.counted(targets, vocab)
+    now = ref64.token_logps(x.double(), targets, temp)
+    old = (now + 0.3 * torch.randn(n, generator=g)).float()
+    refl = (now + 0.2 * torch.randn(n, generator=g)).float() if reference else None
+    offsets = [0, *sorted(torch.randint(0, n + 1, (b - 1,), generator=g).tolist()), n] if packed else list(range(0, n + 1, t))
+    seq = ref64.sequence_of(n, offsets)
+    adv = torch.randn(b if per_seq else n, generator=g)
+    adv_rows = (adv[seq] if per_seq else adv).double()
+    # a ratio next to a bound may fall on its other side: moved away
+    ratio = torch.exp(now - old.double())
+    near = ((ratio - (1 - lo)).abs() < 1e-3) | ((ratio - (1 + hi)).abs() < 1e-3)
+    old[near] += 0.01
+    weight = ref64.row_weights(ok, seq, reduction)
+    leaf = x.double().requires_grad_()
+    loss, logps, stats = ref64.policy(leaf, targets, old, adv_rows, refl, weight, ok, lo, hi, kl if reference else 0.0, temp)
+    want_grad, = torch.autograd.grad(loss * scale, leaf)
+    coef = (torch.exp(now - old.double()) * adv_rows.abs() + (kl * 3 if reference else 0)) * weight * scale / temp
+    shape = (n,) if packed else (b, t)
+    args = dict(old_logps=old.to(DEV).view(shape), ref_logps=None if refl is None else refl.to(DEV).view(shape),
+                advantages=adv.to(DEV) if per_seq else adv.to(DEV).view(shape), clip_low=lo, clip_high=hi,
+                cu_seqlens=torch.tensor(offsets, device=DEV, dtype=torch.int32) if packed else None,
+                kl_coef=kl if reference else 0.0, temperature=temp, scale=scale, reduction=reduction)
+    xg = x.to(DEV).view(*shape, vocab).requires_grad_()
+    tg = targets.to(DEV).view(shape)
+    got = losses.policy_loss(xg, tg, **args)
+    grad, = torch.autograd.grad(got[0], xg)
+    tol = float((coef * temp * 4 * REL).sum()) + 1e-6 * float(loss.abs()) + 1e-8
+    _close(got[0], loss.detach() * scale, tol, "loss")
+    _close(got[1].view(-1), logps, REL + 1e-6 * logps.detach().abs(), "logps")
+    _close(got[2], stats, 4 * REL, "stats")
+    # the factor holds exp of an error of REL: 3 REL covers it and the roundings of its few products
+    _close(grad.view(n, vocab), want_grad, 4 * _grad_tol(coef, _probs(x.double(), temp), targets, dtype, want_grad / 4), "grad")
+    with torch.no_grad():
+        again = losses.policy_loss(xg, tg, **args)
+    assert torch.equal(again[0], got[0]) and torch.equal(again[1], got[1]) and torch.equal(again[2], got[2])
+
+
+def test_policy_rows_of_no_sequence_and_empty_batches():
+    x, hot = _logits(9, 77, torch.float32, 8)
+    old = ref64.token_logps(x.double(), hot).float().to(DEV)
+    xg = x.to(DEV).requires_grad_()
+    cu = torch.tensor([2, 2, 6], device=DEV)
+    loss, logps, stats = losses.policy_loss(xg, hot.to(DEV), old, torch.tensor([5.0, 2.0], device=DEV), cu_seqlens=cu)
+    grad, = torch.autograd.grad(loss, xg)
+    assert float(loss) == pytest.approx(-2.0, rel=1e-5)
+    assert int(grad[:2].count_nonzero()) == 0 and int(grad[6:].count_nonzero()) == 0
+    assert bool((grad[2:6].abs().sum(1) > 0).all())
+    for reduction in ("token", "sequence", "sum"):  # nothing counts
+        loss, _, stats = losses.policy_loss(xg, torch.full_like(hot, -100).to(DEV), old, torch.ones(9, device=DEV),
+                                            reduction=reduction)
+        grad, = torch.autograd.grad(loss, xg)
+        assert float(loss) == 0 and stats.tolist() == [0, 0] and int(grad.count_nonzero()) == 0
+
+
+def test_policy_of_the_sampling_policy_itself():
+    # ratios of 1: the loss is minus the mean advantage, and no KL
+    x, hot = _logits(40, 500, torch.bfloat16, 6)
+    xg = x.to(DEV)
+    old = losses.token_logps(xg, hot.to(DEV))
+    adv = torch.randn(40, generator=_gen(2)).to(DEV)
+    loss, logps, stats = losses.policy_loss(xg, hot.to(DEV), old, adv, ref_logps=old, kl_coef=0.5)
+    assert torch.equal(logps, old) and stats.tolist() == [0, 0]
+    assert float(loss) == pytest.approx(-float(adv.double().mean()), abs=1e-7)
+
+
+# -------------------------------------------------------------------------------- distillation
+def _teacher(n, vocab, top, seed, missing=False, repeated=False):
+    g = _gen(seed)
+    ids = torch.stack([torch.randperm(vocab, generator=g)[:top] for _ in range(n)])
+    teacher = torch.randn(n, top, generator=g) * 2 + 8
+    if repeated and top > 2:
+        ids[:, -1] = ids[:, 0]
+    if missing:
+        ids[0, top // 2:] = -1
+        ids[-1] = vocab + 3
+    return ids, teacher
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("n,vocab,top,missing,repeated", [(1, 2, 1, False, False), (3, 9, 4, True, True), (5, 1003, 64, False, True),
+                                                          (70, 130, 7, True, False), (2, 5000, 1024, False, True),
+                                                          (2, 140_001, 100, False, False)])
+def test_distill(dtype, rest, n, vocab, top, missing, repeated):
+    x, hot = _logits(n, vocab, dtype, n + vocab)
+    ids, teacher = _teacher(n, vocab, top, vocab, missing, repeated)
+    teacher = teacher.to(dtype)
+    mask = torch.ones(n, dtype=torch.bool)
+    if n > 2:
+        mask[1] = False
+        x[1] = float("nan")
+    temp = 1.7
+    g = _gen(3)
+    lse = None
+    if rest:
+        lse = torch.where((ids >= 0) & (ids < vocab), teacher.double() / temp, -torch.inf).logsumexp(1)
+        lse = (lse + 0.05 + 0.3 * torch.rand(n, generator=g)).nan_to_num(0, 0, 0).float()
+    ok = mask & ((ids >= 0) & (ids < vocab)).any(1)
+    weight = ref64.row_weights(ok, torch.zeros(n, dtype=torch.long), "mean")
+    leaf = torch.where(mask[:, None], x.double(), torch.zeros_like(x.double())).requires_grad_()
+    want = ref64.distill(leaf, ids, teacher, lse, ok, weight, temp)
+    want_grad, = torch.autograd.grad(want, leaf)
+    xg = x.to(DEV).requires_grad_()
+    got = losses.distill_loss(xg, ids.to(DEV), teacher.to(DEV), teacher_lse=None if lse is None else lse.to(DEV),
+                              mask=mask.to(DEV), temperature=temp)
+    grad, = torch.autograd.grad(got, xg)
+    # log q is off by REL, log p by the teacher's own roundings (|t| / T <= 12: 3e-6)
+    _close(got, want, temp ** 2 * 3 * REL + 1e-6 * want.detach().abs(), "loss")
+    # at entries q - p of errors REL each; elsewhere a factor of two probabilities, each with REL (left = 1 - sum p loses
+    # up to 2^-24 top / left, left > 0.04 here)
+    q = _probs(leaf.detach(), temp)
+    p = torch.zeros_like(q)
+    for r in range(n):
+        use = (ids[r] >= 0) & (ids[r] < vocab)
+        if bool(use.any()):
+            t = teacher[r].double()[use] / temp
+            p[r].index_add_(0, ids[r][use], torch.softmax(t, 0) if lse is None else torch.exp(t - lse[r].double()))
+    share = 1 + (1 / torch.where(p > 0, 0.0, q).sum(1, keepdim=True).clamp(min=1e-3) if rest else 0.0)
+    tol = weight[:, None] * temp * (q * share * 3 + 2 * p) * REL + want_grad.abs() * HALF_ULP[dtype] + 1e-37
+    _close(grad, want_grad, tol, "grad")
+    assert int(grad.cpu()[~ok].count_nonzero()) == 0
+    with torch.no_grad():
+        again = losses.distill_loss(xg, ids.int().to(DEV), teacher.to(DEV), teacher_lse=None if lse is None else lse.to(DEV),
+                                    mask=mask.to(DEV), temperature=temp)
+    assert torch.equal(again, got)
+
+
+def test_distill_sum_scale_and_nothing_counted():
+    x, _ = _logits(6, 99, torch.float32, 1)
+    ids, teacher = _teacher(6, 99, 5, 2)
+    xg, ids, teacher = x.to(DEV).requires_grad_(), ids.to(DEV), teacher.to(DEV)
+    mean = losses.distill_loss(xg, ids, teacher)
+    total = losses.distill_loss(xg, ids, teacher, reduction="sum", scale=0.25)
+    assert float(total) == pytest.approx(float(mean) * 6 * 0.25, rel=1e-6)
+    none = losses.distill_loss(xg, ids, teacher, mask=torch.zeros(6, dtype=torch.bool, device=DEV))
+    grad, = torch.autograd.grad(none, xg)
+    assert float(none) == 0 and int(grad.count_nonzero()) == 0
+    ids.fill_(-1)
+    assert float(losses.distill_loss(xg, ids, teacher)) == 0
+
+
+def test_distill_entries_that_hold_nearly_everything():
+    # the student's other tokens are 60 below its entries: their share is far under fp32's 2^-24 of the sum, and its
+    # logarithm and the gradient there must still be those of float64
+    vocab, top = 400, 3
+    x = torch.randn(2, vocab, generator=_gen(0))
+    ids = torch.tensor([[3, 100, 399], [0, 1, 2]])
+    x.scatter_(1, ids, 60 + torch.randn(2, top, generator=_gen(1)))
+    teacher = torch.tensor([[3.0, 2.0, 1.0], [1.0, 1.0, 1.0]])
+    lse = teacher.logsumexp(1) + 0.2
+    leaf = x.double().requires_grad_()
+    want = ref64.distill(leaf, ids, teacher, lse, torch.ones(2, dtype=torch.bool), torch.full((2,), 0.5).double(), 1.0)
+    want_grad, = torch.autograd.grad(want, leaf)
+    xg = x.to(DEV).requires_grad_()
+    got = losses.distill_loss(xg, ids.to(DEV), teacher.to(DEV), teacher_lse=lse.to(DEV))
+    grad, = torch.autograd.grad(got, xg)
+    _close(got, want, 3 * REL + 1e-6 * want.detach().abs(), "loss")
+    _close(grad, want_grad, 3 * REL * want_grad.abs() + REL * 0.5 * torch.softmax(x.double(), -1) + 1e-7, "grad")
+
+
+# ----------------------------------------------------------------------- autograd and the device
+def _losses_of(x, seed=3):
+    """name -> function of logits [6, vocab] giving a scalar."""
+    n, vocab = x.shape
+    g = _gen(seed)
+    targets = torch.randint(0, vocab, (n,), generator=g).to(DEV)
+    now = losses.token_logps(x.detach(), targets)
+    near = lambda s: now + (s * torch.randn(n, generator=g)).to(DEV)  # noqa: E731
+    ids, teacher = _teacher(n, vocab, 5, seed)
+    ids, teacher = ids.to(DEV), teacher.to(DEV)
+    lse = teacher.logsumexp(-1) + 0.3
+    old, ref, ref2 = near(0.05), near(0.1), near(0.3)
+    adv = torch.randn(n, generator=g).to(DEV)
+    cu = torch.tensor([0, 2, 3, 4, n], device=DEV)
+    return {
+        "logps": lambda z: losses.token_logps(z, targets, temperature=0.9).sum(),
+        "preference": lambda z: losses.preference_loss(z, targets, ref2, cu_seqlens=cu, beta=0.7)[0],
+        "policy": lambda z: losses.policy_loss(z, targets, old, adv, ref_logps=ref, kl_coef=0.3, clip_low=0.5, clip_high=0.5)[0],
+        "distill": lambda z: losses.distill_loss(z, ids, teacher, temperature=1.2),
+        "distill_rest": lambda z: losses.distill_loss(z, ids, teacher, teacher_lse=lse),
+    }
+
+
+@pytest.mark.parametrize("name", ["logps", "preference", "policy", "distill", "distill_rest"])
+def test_gradient_against_differences(name):
+    x = torch.randn(6, 50, generator=_gen(8)).to(DEV)
+    f = _losses_of(x)[name]
+    xg = x.clone().requires_grad_()
+    grad, = torch.autograd.grad(f(xg), xg)
+    step = 1e-2
+    for k in range(4):
+        v = torch.randn(6, 50, generator=_gen(20 + k)).to(DEV)
+        with torch.no_grad():
+            slope = (float(f(x + step * v)) - float(f(x - step * v))) / (2 * step)
+        # truncation: third derivatives of order one times step^2 / 6 times |v|^3 over the rows; roundings 1e-6 / step
+        assert slope == pytest.approx(float((grad * v).sum()), abs=5e-3, rel=5e-3)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [53, 9001])
+@pytest.mark.parametrize("name", ["logps", "preference", "policy", "distill", "distill_rest"])
+def test_upstream_gradients_and_repeated_backwards(name, vocab, dtype):
+    x = (torch.randn(6, vocab, generator=_gen(8)) * 2).to(dtype).to(DEV)
+    f = _losses_of(x)[name]
+    xg = x.clone().requires_grad_()
+    one, = torch.autograd.grad(f(xg), xg)
+    tripled, = torch.autograd.grad(f(xg), xg, torch.tensor(3.0, device=DEV))
+    tol = one.double().abs().cpu() * 3 * HALF_ULP[dtype] * 2 + 1e-9
+    _close(tripled, one.double().cpu() * 3, tol, "upstream of 3")
+    zero, = torch.autograd.grad(f(xg), xg, torch.tensor(0.0, device=DEV))
+    assert int(zero.count_nonzero()) == 0
+    loss = f(xg)
+    first, = torch.autograd.grad(loss, xg, torch.tensor(3.0, device=DEV), retain_graph=True)
+    kept = first.clone()
+    second, = torch.autograd.grad(loss, xg, retain_graph=True)
+    third, = torch.autograd.grad(loss, xg, torch.tensor(3.0, device=DEV))
+    assert torch.equal(second, one) and torch.equal(third, tripled)
+    assert torch.equal(first, kept) and torch.equal(first, tripled)
+    # two uses of the same logits add up
+    y = x.float().clone().requires_grad_()
+    (both,) = torch.autograd.grad(f(y) + f(y), y)
+    single, = torch.autograd.grad(f(y), y)
+    _close(both, 2 * single.double().cpu(), 1e-6 * single.double().abs().cpu() + 1e-12, "twice")
+
+
+@pytest.mark.parametrize("name", ["logps", "preference", "policy", "distill", "distill_rest"])
+def test_same_bits_every_time_and_on_another_stream(name):
+    x = (torch.randn(6, 40_001, generator=_gen(8)) * 2).bfloat16().to(DEV)
+    f = _losses_of(x)[name]
+    want = None
+    side = torch.cuda.Stream()
+    for k in range(6):
+        xg = x.clone().requires_grad_()
+        if k % 2:
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                loss = f(xg)
+                grad, = torch.autograd.grad(loss, xg)
+            torch.cuda.current_stream().wait_stream(side)
+        else:
+            loss = f(xg)
+            grad, = torch.autograd.grad(loss, xg)
+        torch.cuda.synchronize()
+        if want is None:
+            want = loss.clone(), grad.clone()
+        assert torch.equal(loss, want[0]) and torch.equal(grad, want[1])
+
+
+def test_changed_logits_are_noticed():
+    x = torch.randn(6, 50, device=DEV)
+    f = _losses_of(x)["policy"]
+    leaf = x.clone().requires_grad_()
+    y = leaf * 1.0
+    loss = f(y)
+    with torch.no_grad():
+        y.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+def test_half_of_the_inputs_in_other_dtypes():
+    x = torch.randn(6, 50, device=DEV)
+    t = torch.randint(0, 50, (6,), device=DEV)
+    old = losses.token_logps(x, t)
+    a = losses.policy_loss(x, t, old.bfloat16().float(), torch.ones(6, device=DEV))
+    b = losses.policy_loss(x, t.int(), old.bfloat16(), torch.ones(6, device=DEV, dtype=torch.float64))
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_captured_graph_replays_like_eager():
+    # a server's next-token log-probabilities, and a whole training loss, replayed on changing inputs
+    n, vocab = 4, 262_144
+    x = torch.empty(n, vocab, dtype=torch.bfloat16, device=DEV)
+    t = torch.zeros(n, dtype=torch.long, device=DEV)
+    old, adv = torch.zeros(n, device=DEV), torch.ones(n, device=DEV)
+    xs, hots = zip(*[_logits(n, vocab, torch.bfloat16, 50 + k) for k in range(3)])
+
+    def step():
+        res = loss_ops.policy(x, t, old, adv, False, old, None, 1, n, 0.2, 0.2, 0.1, 1.0, 1.0, 0, -100, True)
+        return losses.token_logps(x, t), res[0], res[5]
+
+    x.copy_(xs[0])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for k in (0, 1, 2, 1):
+        x.copy_(xs[k])
+        t.copy_(hots[k])
+        old.copy_(torch.full((n,), -1.0 - k))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step()
+        assert all(torch.equal(a, b) for a, b in zip(held, want))
+
+
+def test_compiled_losses_equal_eager_ones():
+    x = (torch.randn(6, 500, generator=_gen(8)) * 2).bfloat16().to(DEV)
+    for name, f in _losses_of(x).items():
+        def both(z, f=f):
+            return f(z)
+        a, b = x.clone().requires_grad_(), x.clone().requires_grad_()
+        want, got = f(a), torch.compile(both, backend="aot_eager", fullgraph=True)(b)
+        assert torch.equal(got, want), name
+        ga, = torch.autograd.grad(want, a)
+        gb, = torch.autograd.grad(got, b)
+        _close(gb, ga.double().cpu(), 2.0 ** -8 * ga.double().abs().cpu() + 1e-12, name)
