@@ -107,12 +107,23 @@ struct Raw8<float> {
     f32x4_v lo, hi;
 };
 
+template <bool kNt>
 __device__ __forceinline__ void load_raw(const uint16_t *p, Raw8<uint16_t> &r) {
-    r.w = *reinterpret_cast<const __attribute__((address_space(1))) u32x4_e2 *>(as_global(p));
+    const auto q = reinterpret_cast<const __attribute__((address_space(1))) u32x4_e2 *>(as_global(p));
+    if constexpr (kNt) r.w = __builtin_nontemporal_load(q);
+    else r.w = *q;
 }
+template <bool kNt>
 __device__ __forceinline__ void load_raw(const float *p, Raw8<float> &r) {
-    r.lo = *reinterpret_cast<const __attribute__((address_space(1))) f32x4_e4 *>(as_global(p));
-    r.hi = *reinterpret_cast<const __attribute__((address_space(1))) f32x4_e4 *>(as_global(p + 4));
+    const auto q = reinterpret_cast<const __attribute__((address_space(1))) f32x4_e4 *>(as_global(p));
+    const auto h = reinterpret_cast<const __attribute__((address_space(1))) f32x4_e4 *>(as_global(p + 4));
+    if constexpr (kNt) {
+        r.lo = __builtin_nontemporal_load(q);
+        r.hi = __builtin_nontemporal_load(h);
+    } else {
+        r.lo = *q;
+        r.hi = *h;
+    }
 }
 __device__ __forceinline__ void widen(const Raw8<uint16_t> &r, float (&v)[8]) {
 #pragma unroll
@@ -154,7 +165,8 @@ __device__ __forceinline__ void store8(float *p, const float (&v)[8]) {
 }
 
 // ------------------------------------------------------------------------------------------ (m, s) pairs
-// m: largest logit seen (x, not scaled), s: sum of exp2((x - m) k) with k = log2(e) / temperature.
+// m: the logit that exponents are taken from (the largest one seen, or a guess near it), s: sum of exp2((x - m) k) with
+// k = log2(e) / temperature.
 struct MaxSum {
     float m, s;
 };
@@ -167,6 +179,36 @@ __device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b, float k) {
     if (m == -kInf) return {m, a.s + b.s};  // nothing but minus infinity so far (a NaN stays in s)
     return {m, a.s * exp2_of(a.m, m, k) + b.s * exp2_of(b.m, m, k)};
 }
+
+// The usual way to the sum: m is a guess (the logit of the row's own token, or of a teacher's entry, which no other
+// exceeds by more than e^60 in a model that is any good), so nothing is compared or rescaled and each logit takes one
+// multiply-add, one exponential and one addition. What the guess cannot serve shows in the sum (and in m itself), and
+// is then added up again by add_values, whose m is the running maximum: sums over 2^100 or NaN, where a wrong guess would
+// lose digits also those under 2^-60, and guesses so large that m k could overflow.
+struct Guess {
+    float m, mk;
+    bool fits;
+};
+
+__device__ __forceinline__ Guess guess_of(float m, float k) { return {m, m * k, fabsf(m) <= 1e30f}; }
+
+__device__ __forceinline__ float guessed_exp(float x, const Guess &g, float k) {
+    return __builtin_amdgcn_exp2f(__builtin_fmaf(x, k, -g.mk));
+}
+
+// m k is rounded once; this takes that rounding out of a sum
+__device__ __forceinline__ float without_rounding(float s, const Guess &g, float k) {
+    return s * __builtin_amdgcn_exp2f(-__builtin_fmaf(g.m, k, -g.mk));
+}
+
+__device__ __forceinline__ float sum8(const float (&v)[8], const Guess &g, float k) {
+    float e[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = guessed_exp(v[i], g, k);
+    return ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+}
+
+constexpr float kLargestSum = 0x1p100f, kSmallestSum = 0x1p-60f;
 
 template <int N>
 __device__ __forceinline__ void add_values(MaxSum &a, const float (&v)[N], float k) {
@@ -328,8 +370,15 @@ __global__ __launch_bounds__(kThreads) void stats_kernel(const StatsArgs a) {
         __syncthreads();
     }
     const T *x = static_cast<const T *>(a.logits.x) + a.logits.offset(row);
-    MaxSum acc = {-kInf, 0.0f};
-    const auto take = [&](float (&v)[8], int32_t j) {
+    float near = kInf;  // no guess
+    if (a.tokens.targets != nullptr) {
+        near = load1(x + a.tokens.token(row, vocab));
+    } else {
+        const int32_t id = teacher_id(a.ids, a.ids64, row * a.top, vocab);
+        if (id >= 0) near = load1(x + id);
+    }
+    const Guess guess = guess_of(near, a.k);
+    const auto leave_out = [&](float (&v)[8], int32_t j) {
         if constexpr (kLeaveOut) {
             const int32_t at = j - from;
             const uint32_t bits = (left_out[at >> 5] >> (at & 31)) & 0xff;
@@ -339,40 +388,62 @@ __global__ __launch_bounds__(kThreads) void stats_kernel(const StatsArgs a) {
                     if (bits >> e & 1) v[e] = -kInf;
             }
         }
-        add_values<8>(acc, v, a.k);
     };
     const int32_t whole = (to - from) / 8;  // spans are multiples of 8: only the row's end has a rest
-    int32_t c = tid;
-    for (; c + 3 * kThreads < whole; c += 4 * kThreads) {
-        Raw8<T> raw[4];
+    const auto sweep = [&](auto take) {
+        int32_t c = tid;
+        for (; c + 3 * kThreads < whole; c += 4 * kThreads) {
+            Raw8<T> raw[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) load_raw(x + from + 8 * (c + u * kThreads), raw[u]);
+            for (int u = 0; u < 4; ++u) load_raw<true>(x + from + 8 * (c + u * kThreads), raw[u]);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
+            for (int u = 0; u < 4; ++u) {
+                float v[8];
+                widen(raw[u], v);
+                leave_out(v, from + 8 * (c + u * kThreads));
+                take(v);
+            }
+        }
+        for (; c < whole; c += kThreads) {
+            Raw8<T> raw;
+            load_raw<true>(x + from + 8 * c, raw);
             float v[8];
-            widen(raw[u], v);
-            take(v, from + 8 * (c + u * kThreads));
+            widen(raw, v);
+            leave_out(v, from + 8 * c);
+            take(v);
+        }
+        if (from + 8 * whole < to && tid == whole % kThreads) {
+            float v[8];
+            load8_tail(x, from + 8 * whole, vocab, v);
+            leave_out(v, from + 8 * whole);
+            take(v);
+        }
+    };
+    __shared__ float sums[kThreads / 64];
+    __shared__ MaxSum joined[kThreads / 64];
+    if (guess.fits) {
+        float sum = 0.0f;
+        sweep([&](float (&v)[8]) { sum += sum8(v, guess, a.k); });
+        sum = wave_sum(sum);
+        if constexpr (kThreads > 64) {
+            if ((tid & 63) == 0) sums[tid >> 6] = sum;
+            __syncthreads();
+            sum = sums[0];
+            for (int w = 1; w < kThreads / 64; ++w) sum += sums[w];
+        }
+        if (sum < kLargestSum && (!kLeaveOut || sum > kSmallestSum)) {
+            if (tid == 0) a.part[blockIdx.x] = {guess.m, without_rounding(sum, guess, a.k)};
+            return;
         }
     }
-    for (; c < whole; c += kThreads) {
-        Raw8<T> raw;
-        load_raw(x + from + 8 * c, raw);
-        float v[8];
-        widen(raw, v);
-        take(v, from + 8 * c);
-    }
-    if (from + 8 * whole < to && tid == whole % kThreads) {
-        float v[8];
-        load8_tail(x, from + 8 * whole, vocab, v);
-        take(v, from + 8 * whole);
-    }
+    MaxSum acc = {-kInf, 0.0f};
+    sweep([&](float (&v)[8]) { add_values<8>(acc, v, a.k); });
     acc = wave_join(acc, a.k);
     if constexpr (kThreads > 64) {
-        __shared__ MaxSum waves[kThreads / 64];
-        if ((tid & 63) == 0) waves[tid >> 6] = acc;
+        if ((tid & 63) == 0) joined[tid >> 6] = acc;
         __syncthreads();
         if (tid == 0) {
-            for (int w = 1; w < kThreads / 64; ++w) acc = join(acc, waves[w], a.k);
+            for (int w = 1; w < kThreads / 64; ++w) acc = join(acc, joined[w], a.k);
         }
     }
     if (tid == 0) a.part[blockIdx.x] = acc;
@@ -747,7 +818,7 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(const GradArgs a) {
     for (; i + 3 * kThreads < whole; i += 4 * kThreads) {
         Raw8<T> raw[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) load_raw(x + from + 8 * (i + u * kThreads), raw[u]);
+        for (int u = 0; u < 4; ++u) load_raw<false>(x + from + 8 * (i + u * kThreads), raw[u]);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             const int32_t j = from + 8 * (i + u * kThreads);
@@ -760,7 +831,7 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(const GradArgs a) {
     for (; i < whole; i += kThreads) {
         const int32_t j = from + 8 * i;
         Raw8<T> raw;
-        load_raw(x + j, raw);
+        load_raw<false>(x + j, raw);
         float v[8], d[8];
         widen(raw, v);
         values(v, j, d);
