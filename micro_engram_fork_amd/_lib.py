@@ -73,7 +73,7 @@ SIGNATURES = {
                            c_ptr, c_int, c_ptr, c_int, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64,
                            c_ptr, c_int, c_i32, c_ptr, c_ptr],
     "me_mask_media": [c_ptr, c_int, c_i64, c_i64, c_i64, c_ptr, c_int, c_i32, c_ptr, c_ptr, c_ptr],
-    "me_loss_workspace_size": [c_i64, c_i64, c_i64, ctypes.POINTER(c_size)],
+    "me_loss_workspace_size": [c_i64, c_i64, c_i64, c_i64, ctypes.POINTER(c_size)],
     "me_token_logps": [*_LOGITS, *_TARGETS, c_double, c_ptr, c_ptr, c_ptr, c_size, c_ptr],
     "me_token_logps_backward": [*_LOGITS, *_TARGETS, c_double, c_ptr, c_ptr, c_double, c_ptr, c_int, c_ptr,
                                 c_ptr],

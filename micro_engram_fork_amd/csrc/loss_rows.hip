@@ -1,0 +1,342 @@
+// The policy and distillation losses with their gradient from one read of the logits: a workgroup keeps a row on its
+// CU, in registers and for the longest rows in LDS too, between adding up its exponentials and writing its gradient.
+//
+// Bound by HBM: 2 bytes read and 2 written per bf16 logit, where two sweeps (losses.hip) move 6. A CU has 512 KB of
+// registers and 160 KB of LDS: a row of 262,144 bf16 logits is 512 KB, of which 1024 threads hold 22 16-byte slots each in
+// registers (88 of the 128 that 16 wavefronts leave a thread) and 9 in LDS; what is beyond is read a second time. A row's
+// slots are all requested before the first is used, so the whole row is in flight at once.
+#include "loss_common.h"
+
+namespace me {
+
+using namespace loss;
+
+namespace {
+
+constexpr int64_t kPassRows = 128;  // rows from which
+constexpr bool kNtLoads = true;
+constexpr int kPassTop = 512;  // teacher entries the kernels' LDS has room for
+
+// The logit at an index that all threads share.
+__device__ __forceinline__ float scalar_logit(const uint16_t *x, int32_t j) {
+    return __uint_as_float(constant_bytes(x + j) << 16);
+}
+__device__ __forceinline__ float scalar_logit(const float *x, int32_t j) { return constant(x + j); }
+
+template <typename T, int kThreads, int kRegs, int kLds, Op kOp, bool kRest>
+__global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *grad) {
+    constexpr bool kDist = kOp == kDistill;
+    constexpr int kWaves = kThreads / 64;
+    constexpr bool kKeepExp = sizeof(T) == 4;  // fp32 slots take the exponentials in place: the gradient needs no second one
+    __shared__ Raw8<T> held[kLds > 0 ? kLds : 1][kThreads];
+    __shared__ __attribute__((aligned(16))) uint8_t entry_space[kDist ? kPassTop * kEntryBytes : 16];
+    __shared__ float sums[kWaves];
+    const int64_t r = blockIdx.x;
+    const int32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int32_t vocab = a.logits.vocab, whole = vocab / 8, slots = (whole + kThreads - 1) / kThreads, rest = vocab - 8 * whole;
+    T *g = static_cast<T *>(grad) + r * vocab;
+    if (constant(a.weights.weight + r) == 0.0f) {
+        const float zeros[8] = {};
+        for (int32_t i = tid; i < whole; i += kThreads) store8(g + 8 * i, zeros);
+        if (tid < rest) store1(g + 8 * whole + tid, 0.0f);
+        if (tid == 0) {
+            a.stats[r] = {0.0f, 0.0f};
+            a.coef[r] = 0.0f;
+            if constexpr (!kDist) a.logps[r] = 0.0f;
+            for (int c = 0; c < 3; ++c) a.sums[3 * r + c] = 0;
+        }
+        if constexpr (kDist)
+            for (int32_t i = tid; i < a.top; i += kThreads) a.fix[r * a.top + i] = 0.0f;
+        return;
+    }
+    const T *x = static_cast<const T *>(a.logits.x) + a.logits.offset(r);
+
+    // All loads of the row are issued before the first is used, and none of them under a condition: a slot past the row's
+    // end loads the last chunk again. (Loads return in the order of their issue; after one that may or may not have been
+    // issued the compiler can only wait for all.) The entries of a row come before its logits for the same reason.
+    constexpr int kPer = kDist ? (kPassTop + kThreads - 1) / kThreads : 1;  // entries of a thread
+    const Entries e = entries_at(entry_space, a.top);
+    int32_t entry_id[kPer];
+    float entry_p[kPer], entry_x[kPer];
+    if constexpr (kDist) {
+#pragma unroll
+        for (int u = 0; u < kPer; ++u) {
+            const int32_t i = min(tid + u * kThreads, a.top - 1);
+            entry_id[u] = *as_global(a.entry_id + r * a.top + i);
+            entry_p[u] = *as_global(a.fix + r * a.top + i);
+            entry_x[u] = *as_global(a.entry_x + r * a.top + i);
+        }
+    }
+    const float last = load1(x + min(8 * whole + tid, vocab - 1));
+    // slot s of a thread: the 8 logits of chunk s * kThreads + tid
+    const auto load_slot = [&](int32_t s, Raw8<T> &raw) {
+        load_raw<kNtLoads>(x + 8 * static_cast<int64_t>(min(s * kThreads + tid, whole - 1)), raw);
+    };
+    Raw8<T> q[kRegs];
+#pragma unroll
+    for (int c = 0; c < kRegs; ++c) load_slot(c, q[c]);
+
+    const float weight = row_weight(a.weights, r);
+    int32_t t = -1;
+    float xt;
+    Sampled sampled = {};
+    if constexpr (kDist) {
+        xt = constant(a.near + r);
+    } else {
+        t = a.tokens.token(r, vocab);
+        xt = scalar_logit(x, t);
+        sampled = sampled_row(a, r);
+    }
+    const Guess guess = guess_of(xt, a.k);
+
+    uint64_t marks = 0;  // slots of this wavefront that hold an entry's token
+    if constexpr (kDist) {
+#pragma unroll
+        for (int u = 0; u < kPer; ++u) {
+            const int32_t i = tid + u * kThreads;
+            if (i < a.top) {
+                e.id[i] = entry_id[u];
+                e.p[i] = entry_p[u];
+                e.x[i] = entry_x[u];
+            }
+        }
+        if constexpr (kWaves > 1) __syncthreads();
+        else wave_lds_order();
+        for (int32_t i0 = 0; i0 < a.top; i0 += 64) {
+            const int32_t i = i0 + lane, c = i < a.top ? e.id[i] >> 3 : -1, s = c / kThreads;
+            uint64_t hits = __ballot(c >= 0 && c < whole && (c % kThreads) >> 6 == wave);
+            while (hits != 0) {
+                const int src = __builtin_ctzll(hits);
+                hits &= hits - 1;
+                marks |= 1ull << __builtin_amdgcn_readlane(s, src);
+            }
+        }
+    }
+    float tail = tid < rest ? last : -kInf;
+    // v at the entries' tokens in slot s of this wavefront becomes coef times their `value`, or minus infinity
+    float coef = 0.0f;
+    const auto at_entries = [&](int32_t s, float (&v)[8], const float *value) {
+        const int32_t first = s * kThreads + wave * 64;
+        for (int32_t i0 = 0; i0 < a.top; i0 += 64) {
+            const int32_t i = i0 + lane, id = i < a.top ? e.id[i] : -1;
+            const int32_t rel = (id >> 3) - first;
+            const float mine = value != nullptr && i < a.top ? coef * value[i] : -kInf;
+            uint64_t hits = __ballot(id >= 0 && rel >= 0 && rel < 64);
+            while (hits != 0) {
+                const int src = __builtin_ctzll(hits);
+                hits &= hits - 1;
+                const int32_t token = __builtin_amdgcn_readlane(id, src);
+                const float val = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(mine), src));
+#pragma unroll
+                for (int w = 0; w < 8; ++w)
+                    if (lane == (token >> 3) - first && w == (token & 7)) v[w] = val;
+            }
+        }
+    };
+
+    // ---- sum of exponentials
+    float sum = 0.0f;
+    const auto add_slot = [&](int32_t s, Raw8<T> &raw) {
+        float v[8];
+        widen(raw, v);
+        if ((s + 1) * kThreads > whole && s * kThreads + tid >= whole) {
+#pragma unroll
+            for (int w = 0; w < 8; ++w) v[w] = -kInf;
+        }
+        if constexpr (kRest) {
+            if (marks >> s & 1) at_entries(s, v, nullptr);
+        }
+#pragma unroll
+        for (int w = 0; w < 8; ++w) v[w] = guessed_exp(v[w], guess, a.k);
+        if constexpr (kKeepExp) keep_raw(raw, v);
+        sum += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+    };
+#pragma unroll
+    for (int c = 0; c < kLds; ++c) {  // these make room for the slots past the registers' own
+        if (c < slots) {
+            add_slot(c, q[c]);
+            held[c][tid] = q[c];
+        }
+        load_slot(kRegs + c, q[c]);
+    }
+#pragma unroll
+    for (int c = kLds; c < kRegs; ++c)
+        if (c < slots) add_slot(c, q[c]);
+#pragma unroll
+    for (int c = 0; c < kLds; ++c)
+        if (kRegs + c < slots) add_slot(kRegs + c, q[c]);
+    for (int32_t s = kRegs + kLds; s < slots; ++s) {
+        Raw8<T> raw;
+        load_slot(s, raw);
+        add_slot(s, raw);
+    }
+    if constexpr (kRest) {
+        if (tid < rest)
+            for (int32_t i = 0; i < a.top; ++i)
+                if (e.id[i] == 8 * whole + tid) tail = -kInf;
+    }
+    sum = wave_sum(sum + guessed_exp(tail, guess, a.k));
+    if constexpr (kWaves > 1) {
+        if (lane == 0) sums[wave] = sum;
+        __syncthreads();
+        sum = sums[0];
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) sum += sums[w];
+    }
+    MaxSum row = {guess.m, without_rounding(sum, guess, a.k)};
+    const bool guessed = guess.fits && sum < kLargestSum && (!kRest || sum > kSmallestSum);
+    if (!guessed) {  // again, with the running maximum
+        row = {-kInf, 0.0f};
+        for (int32_t j = 8 * tid; j < vocab; j += 8 * kThreads) {
+            float v[8];
+            load8_tail(x, j, vocab, v);
+            if constexpr (kRest) {
+                for (int32_t i = 0; i < a.top; ++i) {
+#pragma unroll
+                    for (int w = 0; w < 8; ++w)
+                        if (e.id[i] == j + w) v[w] = -kInf;
+                }
+            }
+            add_values<8>(row, v, a.k);
+        }
+        row = wave_join(row, a.k);
+        if constexpr (kWaves > 1) {
+            __shared__ MaxSum joined[kWaves];
+            if (lane == 0) joined[wave] = row;
+            __syncthreads();
+            row = joined[0];
+            for (int w = 1; w < kWaves; ++w) row = join(row, joined[w], a.k);
+        }
+    }
+
+    // ---- the loss and the gradient's factors
+    float factor, ref = row.m;
+    if constexpr (kDist) {  // every wavefront the same, so that none waits for another
+        float2 stats;
+        const float loss = distill_finish(a, r, row, e, stats, wave == 0);
+        coef = a.scale * weight * a.temp;
+        factor = coef * stats.y;
+        ref = stats.x;
+        if (tid == 0) {
+            a.stats[r] = stats;
+            a.coef[r] = coef;
+            a.sums[3 * r] = static_cast<double>(loss) * weight;
+        }
+    } else {
+        const float logp = (xt - row.m) * a.inv_temp - logf(row.s), inv_s = 1.0f / row.s;
+        float loss, slope, kl;
+        bool clipped;
+        policy_terms(a, sampled, logp, loss, slope, kl, clipped);
+        coef = a.scale * weight * slope * a.inv_temp;
+        factor = -coef * inv_s;
+        if (tid == 0) {
+            a.stats[r] = {row.m, inv_s};
+            a.coef[r] = coef;
+            a.logps[r] = logp;
+            a.sums[3 * r] = static_cast<double>(loss) * weight;
+            a.sums[3 * r + 1] = kl;
+            a.sums[3 * r + 2] = clipped;
+        }
+    }
+
+    // ---- gradient
+    if (grad == nullptr) return;
+    if (!guessed) {
+        for (int32_t j = 8 * tid; j < vocab; j += 8 * kThreads) {
+            for (int w = 0; w < 8 && j + w < vocab; ++w) {
+                float d = factor * exp2_of(load1(x + j + w), ref, a.k);
+                if constexpr (kDist) {
+                    for (int32_t i = 0; i < a.top; ++i)
+                        if (e.id[i] == j + w) d = coef * e.raw[i];
+                } else {
+                    if (j + w == t) d += coef;
+                }
+                store1(g + j + w, d);
+            }
+        }
+        return;
+    }
+    // exponentials are those of `sum`; the rounding of m k that row.s is without goes into the factor
+    factor = without_rounding(factor, guess, a.k);
+    const int32_t t_slot = kDist || t >= 8 * whole ? -1 : (t >> 3) / kThreads, t_thread = kDist ? -1 : (t >> 3) % kThreads;
+    const auto put_slot = [&](int32_t s, const Raw8<T> &raw) {
+        float d[8];
+        widen(raw, d);
+#pragma unroll
+        for (int w = 0; w < 8; ++w) {
+            if constexpr (!kKeepExp) d[w] = guessed_exp(d[w], guess, a.k);
+            d[w] *= factor;
+        }
+        if constexpr (kDist) {
+            if (marks >> s & 1) at_entries(s, d, e.raw);
+        } else if (s == t_slot) {
+#pragma unroll
+            for (int w = 0; w < 8; ++w)
+                if (tid == t_thread && w == (t & 7)) d[w] += coef;
+        }
+        const int32_t c = s * kThreads + tid;
+        if (c < whole) store8(g + 8 * static_cast<int64_t>(c), d);
+    };
+#pragma unroll
+    for (int c = kLds; c < kRegs; ++c)
+        if (c < slots) put_slot(c, q[c]);
+#pragma unroll
+    for (int c = 0; c < kLds; ++c)
+        if (kRegs + c < slots) put_slot(kRegs + c, q[c]);
+#pragma unroll
+    for (int c = 0; c < kLds; ++c)
+        if (c < slots) put_slot(c, held[c][tid]);
+    for (int32_t s = kRegs + kLds; s < slots; ++s) {
+        Raw8<T> raw;
+        load_slot(s, raw);
+        if constexpr (kKeepExp) {
+            float v[8];
+            widen(raw, v);
+#pragma unroll
+            for (int w = 0; w < 8; ++w) v[w] = guessed_exp(v[w], guess, a.k);
+            keep_raw(raw, v);
+        }
+        put_slot(s, raw);
+    }
+    if (tid < rest) {
+        const int32_t j = 8 * whole + tid;
+        float d = factor * guessed_exp(tail, guess, a.k) + (j == t ? coef : 0.0f);
+        if constexpr (kDist) {
+            for (int32_t i = 0; i < a.top; ++i)
+                if (e.id[i] == j) d = coef * e.raw[i];
+        }
+        store1(g + j, d);
+    }
+}
+
+template <typename T, int kThreads, int kRegs, int kLds>
+void launch_pass_of(Op op, const RowArgs &a, void *grad, hipStream_t s) {
+    const unsigned n = static_cast<unsigned>(a.logits.n);
+    if (op == kPolicy) pass_kernel<T, kThreads, kRegs, kLds, kPolicy, false><<<n, kThreads, 0, s>>>(a, grad);
+    else if (a.teacher_lse != nullptr) pass_kernel<T, kThreads, kRegs, kLds, kDistill, true><<<n, kThreads, 0, s>>>(a, grad);
+    else pass_kernel<T, kThreads, kRegs, kLds, kDistill, false><<<n, kThreads, 0, s>>>(a, grad);
+}
+
+}  // namespace
+
+bool takes_row_pass(int64_t n, int64_t vocab, int dtype, int64_t top) {
+    if (n == 0 || vocab < 64 || top > kPassTop) return false;
+    return vocab <= (dtype == ME_BF16 ? 327680 : 163840) && n >= kPassRows;
+}
+
+void launch_row_pass(Op op, const RowArgs &a, int dtype, void *grad, hipStream_t s) {
+    const int32_t v = a.logits.vocab;
+    if (dtype == ME_BF16) {
+        if (v <= 8192) launch_pass_of<uint16_t, 64, 16, 0>(op, a, grad, s);
+        else if (v <= 32768) launch_pass_of<uint16_t, 256, 16, 0>(op, a, grad, s);
+        else if (v <= 131072) launch_pass_of<uint16_t, 1024, 16, 0>(op, a, grad, s);
+        else launch_pass_of<uint16_t, 1024, 22, 9>(op, a, grad, s);
+    } else {
+        if (v <= 4096) launch_pass_of<float, 64, 8, 0>(op, a, grad, s);
+        else if (v <= 16384) launch_pass_of<float, 256, 8, 0>(op, a, grad, s);
+        else if (v <= 65536) launch_pass_of<float, 1024, 8, 0>(op, a, grad, s);
+        else launch_pass_of<float, 1024, 11, 4>(op, a, grad, s);
+    }
+}
+
+}  // namespace me

@@ -16,291 +16,54 @@
 //
 // Rows that do not count (a target that is ignored or no token, a mask) are not read at all: what they hold cannot
 // reach the loss, and their gradient is zeros.
-#include "me_common.h"
-
-#include <cmath>
-#include <cstring>
+#include "loss_common.h"
 
 namespace me {
+
+using namespace loss;
+
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
-constexpr float kInf = __builtin_huge_valf();
-constexpr int kMaxSplits = 64;      // parts of a row whose (m, s) one wavefront joins, a lane each
-constexpr int kMaxSpan = 32768;     // logits of one part
-constexpr int kMaxTop = 1024;       // teacher entries of a row
-
-// Where the logits are: row r at x + (r / rows_per_batch) * batch_stride + (r % rows_per_batch) * row_stride elements.
-struct Logits {
-    const void *x;
-    int64_t n, rows_per_batch, batch_stride, row_stride;
-    int32_t vocab;
-
-    __device__ __forceinline__ int64_t offset(int64_t r) const {
-        const int64_t b = r / rows_per_batch;
-        return b * batch_stride + (r - b * rows_per_batch) * row_stride;
-    }
-};
-
-// The tokens of the rows, and which rows count: a target in [0, vocab) that is not the ignored one, a mask that is set.
-struct Tokens {
-    const void *targets;  // [n] int32 / int64, or null
-    const uint8_t *mask;  // [n], or null
-    int64_t ignore;
-    int is64;
-
-    __device__ __forceinline__ int64_t at(int64_t r) const {
-        return is64 ? static_cast<const int64_t *>(targets)[r] : static_cast<const int32_t *>(targets)[r];
-    }
-    // the row's token, or -1 where the row does not count
-    __device__ __forceinline__ int32_t token(int64_t r, int32_t vocab) const {
-        const int64_t t = at(r);
-        return t >= 0 && t < vocab && t != ignore ? static_cast<int32_t>(t) : -1;
-    }
-    __device__ __forceinline__ bool counts(int64_t r, int32_t vocab) const {
-        if (mask != nullptr && mask[r] == 0) return false;
-        return targets == nullptr || token(r, vocab) >= 0;
-    }
-};
-
-// Sequences of the rows: offsets [n_seqs + 1] (packed), or all of one length (offsets null). Offsets are clamped to
-// the rows there are, so that no value of theirs reads or writes outside.
-struct Seqs {
-    const void *offsets;
-    int64_t n_seqs, length, n;
-    int is64;
-
-    __device__ __forceinline__ int64_t begin(int64_t s) const {
-        if (offsets == nullptr) return s * length;
-        const int64_t v = is64 ? static_cast<const int64_t *>(offsets)[s] : static_cast<const int32_t *>(offsets)[s];
-        return v < 0 ? 0 : v > n ? n : v;
-    }
-    // the sequence that holds row r, -1 if none does
-    __device__ __forceinline__ int64_t of(int64_t r) const {
-        if (offsets == nullptr) return length > 0 && r / length < n_seqs ? r / length : -1;
-        int64_t lo = 0, hi = n_seqs;  // the last s with begin(s) <= r
-        if (n_seqs == 0 || begin(0) > r) return -1;
-        while (hi - lo > 1) {
-            const int64_t mid = (lo + hi) / 2;
-            if (begin(mid) <= r) lo = mid;
-            else hi = mid;
+// The weight of a row: 1 over the rows that count (kMean), 1 (kSum), or 1 over the row's sequence's counting rows and the
+// sequences that have any (kSequence); 0 for a row that does not count. One workgroup: it runs beside the rows' own ones.
+template <typename I>
+__device__ int64_t count_rows(const WeightArgs &a) {
+    const bool of_ids = a.ids != nullptr;
+    const I *key = static_cast<const I *>(of_ids ? a.ids : a.tokens.targets);
+    const int64_t stride = of_ids ? a.top : 1, ignore = of_ids ? -1 : a.tokens.ignore;
+    int64_t total = 0;
+    for (int64_t r0 = threadIdx.x; r0 < a.n; r0 += 8 * static_cast<int64_t>(blockDim.x)) {
+        I v[8];
+        uint8_t in[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {  // eight loads in flight
+            const int64_t r = r0 + u * static_cast<int64_t>(blockDim.x), at = r < a.n ? r : a.n - 1;
+            v[u] = key[at * stride];
+            in[u] = a.tokens.mask != nullptr ? a.tokens.mask[at] : 1;
         }
-        return r < begin(lo + 1) ? lo : -1;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const int64_t r = r0 + u * static_cast<int64_t>(blockDim.x);
+            bool counts = r < a.n && in[u] != 0;
+            if (counts && !(v[u] >= 0 && v[u] < a.vocab && v[u] != ignore)) counts = of_ids && row_counts(a, r);
+            total += counts;
+            if (r < a.n) a.weight[r] = counts ? 1.0f : 0.0f;
+        }
     }
-};
-
-// ------------------------------------------------------------------------------------------ row access
-// Rows may start at any element (an odd vocabulary, a view without its padding), so the 16-byte accesses are declared
-// to need the element's alignment only; gfx950 takes them at any address.
-typedef uint32_t u32x4_e2 __attribute__((ext_vector_type(4), aligned(2)));
-typedef float f32x4_e4 __attribute__((ext_vector_type(4), aligned(4)));
-
-template <typename T>
-struct Raw8;  // 8 logits as loaded
-template <>
-struct Raw8<uint16_t> {
-    u32x4_v w;
-};
-template <>
-struct Raw8<float> {
-    f32x4_v lo, hi;
-};
-
-template <bool kNt>
-__device__ __forceinline__ void load_raw(const uint16_t *p, Raw8<uint16_t> &r) {
-    const auto q = reinterpret_cast<const __attribute__((address_space(1))) u32x4_e2 *>(as_global(p));
-    if constexpr (kNt) r.w = __builtin_nontemporal_load(q);
-    else r.w = *q;
-}
-template <bool kNt>
-__device__ __forceinline__ void load_raw(const float *p, Raw8<float> &r) {
-    const auto q = reinterpret_cast<const __attribute__((address_space(1))) f32x4_e4 *>(as_global(p));
-    const auto h = reinterpret_cast<const __attribute__((address_space(1))) f32x4_e4 *>(as_global(p + 4));
-    if constexpr (kNt) {
-        r.lo = __builtin_nontemporal_load(q);
-        r.hi = __builtin_nontemporal_load(h);
-    } else {
-        r.lo = *q;
-        r.hi = *h;
-    }
-}
-__device__ __forceinline__ void widen(const Raw8<uint16_t> &r, float (&v)[8]) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        v[2 * e] = __uint_as_float(r.w[e] << 16);
-        v[2 * e + 1] = __uint_as_float(r.w[e] & 0xffff0000u);
-    }
-}
-__device__ __forceinline__ void widen(const Raw8<float> &r, float (&v)[8]) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        v[e] = r.lo[e];
-        v[4 + e] = r.hi[e];
-    }
-}
-__device__ __forceinline__ float load1(const uint16_t *p) { return bf16_bits_to_float(*as_global(p)); }
-__device__ __forceinline__ float load1(const float *p) { return *as_global(p); }
-
-// 8 logits from element j, minus infinity past the end of the row
-template <typename T>
-__device__ __forceinline__ void load8_tail(const T *row, int32_t j, int32_t vocab, float (&v)[8]) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = j + e < vocab ? load1(row + j + e) : -kInf;
+    return total;
 }
 
-__device__ __forceinline__ void store1(uint16_t *p, float f) { *as_global(p) = float_to_bf16_bits_rne(f); }
-__device__ __forceinline__ void store1(float *p, float f) { *as_global(p) = f; }
-__device__ __forceinline__ void store8(uint16_t *p, const float (&v)[8]) {
-    u32x4_v w;
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-        w[e] = static_cast<uint32_t>(float_to_bf16_bits_rne(v[2 * e])) |
-               (static_cast<uint32_t>(float_to_bf16_bits_rne(v[2 * e + 1])) << 16);
-    *reinterpret_cast<__attribute__((address_space(1))) u32x4_e2 *>(as_global(p)) = w;
-}
-__device__ __forceinline__ void store8(float *p, const float (&v)[8]) {
-    *reinterpret_cast<__attribute__((address_space(1))) f32x4_e4 *>(as_global(p)) = f32x4_v{v[0], v[1], v[2], v[3]};
-    *reinterpret_cast<__attribute__((address_space(1))) f32x4_e4 *>(as_global(p + 4)) = f32x4_v{v[4], v[5], v[6], v[7]};
-}
-
-// ------------------------------------------------------------------------------------------ (m, s) pairs
-// m: the logit that exponents are taken from (the largest one seen, or a guess near it), s: sum of exp2((x - m) k) with
-// k = log2(e) / temperature.
-struct MaxSum {
-    float m, s;
-};
-
-// exp2((x - m) k); v_exp_f32 is within one unit in the last place and takes minus infinity to 0
-__device__ __forceinline__ float exp2_of(float x, float m, float k) { return __builtin_amdgcn_exp2f((x - m) * k); }
-
-__device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b, float k) {
-    const float m = fmaxf(a.m, b.m);
-    if (m == -kInf) return {m, a.s + b.s};  // nothing but minus infinity so far (a NaN stays in s)
-    return {m, a.s * exp2_of(a.m, m, k) + b.s * exp2_of(b.m, m, k)};
-}
-
-// The usual way to the sum: m is a guess (the logit of the row's own token, or of a teacher's entry, which no other
-// exceeds by more than e^60 in a model that is any good), so nothing is compared or rescaled and each logit takes one
-// multiply-add, one exponential and one addition. What the guess cannot serve shows in the sum (and in m itself), and
-// is then added up again by add_values, whose m is the running maximum: sums over 2^100 or NaN, where a wrong guess would
-// lose digits also those under 2^-60, and guesses so large that m k could overflow.
-struct Guess {
-    float m, mk;
-    bool fits;
-};
-
-__device__ __forceinline__ Guess guess_of(float m, float k) { return {m, m * k, fabsf(m) <= 1e30f}; }
-
-__device__ __forceinline__ float guessed_exp(float x, const Guess &g, float k) {
-    return __builtin_amdgcn_exp2f(__builtin_fmaf(x, k, -g.mk));
-}
-
-// m k is rounded once; this takes that rounding out of a sum
-__device__ __forceinline__ float without_rounding(float s, const Guess &g, float k) {
-    return s * __builtin_amdgcn_exp2f(-__builtin_fmaf(g.m, k, -g.mk));
-}
-
-__device__ __forceinline__ float sum8(const float (&v)[8], const Guess &g, float k) {
-    float e[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = guessed_exp(v[i], g, k);
-    return ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
-}
-
-constexpr float kLargestSum = 0x1p100f, kSmallestSum = 0x1p-60f;
-
-template <int N>
-__device__ __forceinline__ void add_values(MaxSum &a, const float (&v)[N], float k) {
-    float top = v[0];
-#pragma unroll
-    for (int e = 1; e < N; ++e) top = fmaxf(top, v[e]);
-    const float m = fmaxf(a.m, top);
-    const float ref = m == -kInf ? 0.0f : m;
-    float part[N];
-#pragma unroll
-    for (int e = 0; e < N; ++e) part[e] = exp2_of(v[e], ref, k);
-#pragma unroll
-    for (int w = N / 2; w > 0; w /= 2) {
-#pragma unroll
-        for (int e = 0; e < w; ++e) part[e] += part[e + w];
-    }
-    a.s = a.s * exp2_of(a.m, ref, k) + part[0];
-    a.m = m;
-}
-
-__device__ __forceinline__ MaxSum wave_join(MaxSum a, float k) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) a = join(a, {__shfl_xor(a.m, off), __shfl_xor(a.s, off)}, k);
-    return a;
-}
-
-template <typename T>
-__device__ __forceinline__ T wave_sum(T v) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off);
-    return v;
-}
-
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off));
-    return v;
-}
-
-// Sum of v over the workgroup's wavefronts, in their order; every thread gets it. `slots`: one per wavefront.
-template <typename T>
-__device__ T block_sum(T v, T *slots) {
-    v = wave_sum(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) slots[threadIdx.x >> 6] = v;
-    __syncthreads();
-    T sum = 0;
-    for (int w = 0; w < static_cast<int>(blockDim.x >> 6); ++w) sum += slots[w];
-    return sum;
-}
-
-// ------------------------------------------------------------------------------------------ weights of the rows
-enum Reduction { kMean = 0, kSum = 1, kSequence = 2 };
-
-struct WeightArgs {
-    Tokens tokens;
-    Seqs seqs;         // read where use_seqs: rows of no sequence do not count
-    const void *ids;   // teacher ids [n, top] or null: a row without one in the vocabulary does not count
-    float *weight;     // [n]; null: this workgroup is not launched
-    float *counted;    // [1]: how many rows count
-    int64_t n;
-    int32_t vocab, top;
-    int ids64, use_seqs, reduction;
-};
-
-__device__ __forceinline__ int32_t teacher_id(const void *ids, int is64, int64_t at, int32_t vocab) {
-    const int64_t v = is64 ? static_cast<const int64_t *>(ids)[at] : static_cast<const int32_t *>(ids)[at];
-    return v >= 0 && v < vocab ? static_cast<int32_t>(v) : -1;
-}
-
-__device__ __forceinline__ bool row_counts(const WeightArgs &a, int64_t r) {
-    if (!a.tokens.counts(r, a.vocab)) return false;
-    if (a.ids != nullptr) {
-        for (int32_t i = 0; i < a.top; ++i)  // the first entry is one almost always
-            if (teacher_id(a.ids, a.ids64, r * a.top + i, a.vocab) >= 0) return true;
-        return false;
-    }
-    return true;
-}
-
-// weight [n]: 1 over the rows that count (kMean), 1 (kSum), or 1 over the row's sequence's counting rows and the
-// sequences that have any (kSequence); 0 for the others. One workgroup: it runs beside the rows' own ones.
 __device__ void make_weights(const WeightArgs &a) {
     __shared__ double slots[16];
     const int tid = threadIdx.x, threads = blockDim.x;
     int64_t total = 0;
     if (!a.use_seqs) {
-        for (int64_t r = tid; r < a.n; r += threads) total += row_counts(a, r);
+        total = (a.ids != nullptr ? a.ids64 : a.tokens.is64) ? count_rows<int64_t>(a) : count_rows<int32_t>(a);
         total = static_cast<int64_t>(block_sum(static_cast<double>(total), slots));
-        const float w = a.reduction == kSum ? 1.0f : 1.0f / static_cast<float>(total > 0 ? total : 1);
-        for (int64_t r = tid; r < a.n; r += threads) a.weight[r] = row_counts(a, r) ? w : 0.0f;
-        if (tid == 0) *a.counted = static_cast<float>(total);
+        if (tid == 0) {
+            a.counted[0] = static_cast<float>(total);
+            a.counted[1] = a.reduction == kSum ? 1.0f : 1.0f / static_cast<float>(total > 0 ? total : 1);
+        }
         return;
     }
     for (int64_t r = tid; r < a.n; r += threads) a.weight[r] = 0.0f;
@@ -449,155 +212,16 @@ __global__ __launch_bounds__(kThreads) void stats_kernel(const StatsArgs a) {
     if (tid == 0) a.part[blockIdx.x] = acc;
 }
 
-// ------------------------------------------------------------------------------------------ per-row values
-enum Op { kLogps, kPreference, kPolicy, kDistill };
-
-struct RowArgs {
-    Logits logits;
-    Tokens tokens;
-    Seqs seqs;
-    const MaxSum *part;    // [n, splits]
-    const float *weight;   // [n] (policy, distillation)
-    const float *counted;  // [1]
-    float2 *stats;         // [n] (m, 1 / s): what the gradient needs (distillation: (m, a), see distill_row)
-    float *logps;          // [n] (nullable)
-    float *coef;           // [n] (nullable): the gradient's factor of the row
-    float *gap;            // [n] preference: log-probability above the reference's
-    const float *old_logps, *ref_logps, *advantages;
-    const void *ids, *teacher;
-    const float *teacher_lse;
-    float *fix;            // [n, top]: the gradient at the teacher's tokens before the row's factor
-    double *sums;          // [gridDim, 3]
-    float *loss, *out_stats;
-    float k, inv_temp, temp, scale, clip_low, clip_high, kl_coef;
-    int32_t splits, top;
-    int ids64, teacher_bf16, adv_per_seq;
-};
-
-struct RowSums {
-    double loss = 0, kl = 0, clipped = 0;
-};
-
-__device__ __forceinline__ float row_logit(const Logits &l, int64_t off, int32_t j, bool bf16) {
-    return bf16 ? load1(static_cast<const uint16_t *>(l.x) + off + j) : load1(static_cast<const float *>(l.x) + off + j);
-}
-
-// exp(d) - 1 - d without the cancellation of small d
-__device__ __forceinline__ float exp_excess(float d) { return expm1f(d) - d; }
-
-// The policy loss of one row and its derivative by the log-probability, both before the row's weight.
-__device__ __forceinline__ void policy_terms(const RowArgs &a, int64_t r, float logp, float &loss, float &slope, float &kl,
-                                             bool &clipped) {
-    const float adv = a.advantages[a.adv_per_seq ? a.seqs.of(r) : r];
-    const float ratio = expf(logp - a.old_logps[r]);
-    const float held = fminf(fmaxf(ratio, 1.0f - a.clip_low), 1.0f + a.clip_high);
-    const float free_term = ratio * adv, held_term = held * adv;
-    clipped = free_term > held_term;
-    loss = -(clipped ? held_term : free_term);
-    slope = clipped ? 0.0f : -free_term;
-    kl = 0.0f;
-    if (a.ref_logps != nullptr) {
-        const float d = a.ref_logps[r] - logp;
-        kl = exp_excess(d);
-        loss += a.kl_coef * kl;
-        slope -= a.kl_coef * expm1f(d);
-    }
-}
-
-// Teacher entry i of row r, scaled; minus infinity where its id is no token.
-__device__ __forceinline__ float teacher_at(const RowArgs &a, int64_t r, int32_t i) {
-    const int64_t at = r * a.top + i;
-    return (a.teacher_bf16 ? load1(static_cast<const uint16_t *>(a.teacher) + at)
-                           : load1(static_cast<const float *>(a.teacher) + at)) * a.inv_temp;
-}
-
-// One row of the distillation loss by one wavefront, lane i of it for the teacher's entries i, i + 64, ... `seen` are
-// the (m, s) of the row: of all its tokens, or (teacher_lse given) of those that are no entry. Entries with the same id are one token
-// whose probabilities add up; the first of them stands for all in the sums. Leaves (m, a) in stats so that the
-// gradient at a token that is no entry is  weight T a exp2((x - m) k), and in fix the factors at the entries.
-__device__ float distill_row(const RowArgs &a, int64_t r, int64_t off, bool bf16, MaxSum seen, int32_t *id, float *prob) {
-    const int lane = threadIdx.x & 63;
-    const bool rest = a.teacher_lse != nullptr;
-    float top = -kInf;
-    for (int32_t i = lane; i < a.top; i += 64) {
-        id[i] = teacher_id(a.ids, a.ids64, r * a.top + i, a.logits.vocab);
-        prob[i] = id[i] >= 0 ? teacher_at(a, r, i) : -kInf;
-        top = fmaxf(top, prob[i]);
-    }
-    top = wave_max(top);
-    float sum = 0.0f, log_norm;  // log of what the entries' exponentials are divided by
-    if (rest) {
-        log_norm = a.teacher_lse[r];
-    } else {
-        for (int32_t i = lane; i < a.top; i += 64) sum += id[i] >= 0 ? expf(prob[i] - top) : 0.0f;
-        sum = wave_sum(sum);
-        log_norm = logf(sum);
-    }
-    const float ref = rest ? 0.0f : top;
-    for (int32_t i = lane; i < a.top; i += 64) {
-        if (id[i] < 0) prob[i] = 0.0f;
-        else prob[i] = rest ? expf(prob[i] - log_norm) : expf(prob[i] - ref) / sum;
-    }
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    // the row's (m, s) over all tokens
-    MaxSum all = seen;
-    if (rest) {
-        MaxSum mine = {-kInf, 0.0f};
-        for (int32_t i = lane; i < a.top; i += 64) {
-            bool first = id[i] >= 0;
-            for (int32_t j = 0; j < i && first; ++j) first = id[j] != id[i];
-            if (first) mine = join(mine, {row_logit(a.logits, off, id[i], bf16), 1.0f}, a.k);
-        }
-        all = join(seen, wave_join(mine, a.k), a.k);
-    }
-    const float log_s = logf(all.s), inv_s = 1.0f / all.s;
-    float loss = 0.0f, mass = 0.0f;
-    for (int32_t i = lane; i < a.top; i += 64) {
-        if (id[i] < 0) {
-            a.fix[r * a.top + i] = 0.0f;
-            continue;
-        }
-        float p = 0.0f;
-        bool first = true;
-        for (int32_t j = 0; j < a.top; ++j) {
-            if (id[j] == id[i]) {
-                p += prob[j];
-                first = first && j >= i;
-            }
-        }
-        const float z = (row_logit(a.logits, off, id[i], bf16) - all.m) * a.inv_temp;
-        a.fix[r * a.top + i] = expf(z) * inv_s - p;
-        if (first) {
-            mass += p;
-            if (p > 0.0f || p != p) loss += p * (logf(p) - (z - log_s));
-        }
-    }
-    loss = wave_sum(loss);
-    float2 st = {all.m, inv_s};
-    if (rest) {
-        mass = wave_sum(mass);
-        const float left = mass < 1.0f ? 1.0f - mass : mass == mass ? 0.0f : mass;
-        // probability of the other tokens, as a logarithm: it does not vanish where the entries hold nearly all
-        const float log_other = seen.m == -kInf ? -kInf : (seen.m - all.m) * a.inv_temp + logf(seen.s) - log_s;
-        if (left > 0.0f || left != left) loss += left * (logf(left) - log_other);
-        st = seen.m == -kInf ? float2{0.0f, 0.0f} : float2{seen.m, (expf(log_other) - left) / seen.s};
-    }
-    if (lane == 0) a.stats[r] = st;
-    return loss * (a.temp * a.temp);
-}
-
 // A wavefront per row: joins the parts' (m, s), then the loss's own few values.
 template <Op kOp, bool kBf16>
 __global__ __launch_bounds__(kOp == kDistill ? 256 : 1024) void row_kernel(const RowArgs a) {
     constexpr int kWaves = kOp == kDistill ? 4 : 16;
-    __shared__ int32_t id_all[kOp == kDistill ? kWaves * kMaxTop : 1];
-    __shared__ float prob_all[kOp == kDistill ? kWaves * kMaxTop : 1];
+    extern __shared__ __attribute__((aligned(16))) uint8_t entry_space[];  // distillation: kEntryBytes * top per wavefront
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     RowSums sums;
     for (int64_t r = static_cast<int64_t>(blockIdx.x) * kWaves + wave; r < a.logits.n; r += static_cast<int64_t>(gridDim.x) * kWaves) {
         const int32_t t = kOp == kDistill ? 0 : a.tokens.token(r, a.logits.vocab);
-        const float weight = a.weight != nullptr ? a.weight[r] : 1.0f;
+        const float weight = kOp >= kPolicy ? row_weight(a.weights, r) : 1.0f;
         if (t < 0 || (kOp >= kPolicy && weight == 0.0f)) {
             if (lane == 0) {
                 if (a.logps != nullptr) a.logps[r] = 0.0f;
@@ -614,13 +238,16 @@ __global__ __launch_bounds__(kOp == kDistill ? 256 : 1024) void row_kernel(const
         if (lane < a.splits) row = a.part[r * a.splits + lane];
         row = wave_join(row, a.k);
         if constexpr (kOp == kDistill) {
-            const float loss = distill_row(a, r, off, kBf16, row, id_all + wave * kMaxTop, prob_all + wave * kMaxTop);
+            const Entries e = entries_at(entry_space + wave * kEntryBytes * a.top, a.top);
+            distill_entries(a, r, off, kBf16, e);
+            float2 stats;
+            const float loss = distill_finish(a, r, row, e, stats, true);
             if (lane == 0) {
+                a.stats[r] = stats;
                 a.coef[r] = a.scale * weight * a.temp;
                 sums.loss += static_cast<double>(loss) * weight;
             }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
+            wave_lds_order();
         } else if (lane == 0) {
             const float logp = (row_logit(a.logits, off, t, kBf16) - row.m) * a.inv_temp - logf(row.s);
             if (a.stats != nullptr) a.stats[r] = {row.m, 1.0f / row.s};
@@ -631,7 +258,7 @@ __global__ __launch_bounds__(kOp == kDistill ? 256 : 1024) void row_kernel(const
             } else if constexpr (kOp == kPolicy) {
                 float loss, slope, kl;
                 bool clipped;
-                policy_terms(a, r, logp, loss, slope, kl, clipped);
+                policy_terms(a, sampled_row(a, r), logp, loss, slope, kl, clipped);
                 a.coef[r] = a.scale * weight * slope * a.inv_temp;
                 sums.loss += static_cast<double>(loss) * weight;
                 sums.kl += kl;
@@ -650,7 +277,7 @@ __global__ __launch_bounds__(kOp == kDistill ? 256 : 1024) void row_kernel(const
             } else {
                 *a.loss = static_cast<float>(loss * a.scale);
                 if (a.out_stats != nullptr) {
-                    const float n = fmaxf(*a.counted, 1.0f);
+                    const float n = fmaxf(*a.weights.counted, 1.0f);
                     a.out_stats[0] = static_cast<float>(kl / n);
                     a.out_stats[1] = static_cast<float>(clipped / n);
                 }
@@ -659,14 +286,42 @@ __global__ __launch_bounds__(kOp == kDistill ? 256 : 1024) void row_kernel(const
     }
 }
 
-// Adds the workgroups' sums in a fixed order.
-__global__ __launch_bounds__(256) void total_kernel(const double *sums, int64_t count, const float *counted, float scale,
+// The weights alone, before a kernel that needs them.
+__global__ __launch_bounds__(1024) void weights_kernel(const WeightArgs a) { make_weights(a); }
+
+// The teacher's entries of every row for the one-read kernel, a wavefront per row; the last workgroup makes the weights.
+template <bool kBf16>
+__global__ __launch_bounds__(256) void entries_kernel(const RowArgs a) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t entry_space[];
+    if (blockIdx.x == gridDim.x - 1) {
+        make_weights(a.weights);
+        return;
+    }
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t r = static_cast<int64_t>(blockIdx.x) * 4 + wave;
+    if (r >= a.logits.n || !row_counts(a.weights, r)) return;
+    const Entries e = entries_at(entry_space + wave * kEntryBytes * a.top, a.top);
+    distill_entries(a, r, a.logits.offset(r), kBf16, e);
+    float near = -kInf;
+    for (int32_t i = lane; i < a.top; i += 64) {
+        near = fmaxf(near, e.x[i]);
+        a.fix[r * a.top + i] = e.p[i];
+        a.entry_x[r * a.top + i] = e.x[i];
+        a.entry_id[r * a.top + i] = e.id[i];
+    }
+    near = wave_max(near);
+    if (lane == 0) a.near[r] = near;
+}
+
+// Adds the workgroups' or rows' sums in a fixed order.
+__global__ __launch_bounds__(1024) void total_kernel(const double *sums, int64_t count, const float *counted, float scale,
                                                     float *loss, float *out_stats) {
-    __shared__ double slots[4];
+    __shared__ double slots[16];
     double v[3] = {0, 0, 0};
-    for (int64_t i = threadIdx.x; i < count; i += 256)
-        for (int c = 0; c < 3; ++c) v[c] += sums[3 * i + c];
-    for (int c = 0; c < 3; ++c) v[c] = block_sum(v[c], slots);
+    const int parts = out_stats != nullptr ? 3 : 1;
+    for (int64_t i = threadIdx.x; i < count; i += 1024)
+        for (int c = 0; c < parts; ++c) v[c] += sums[3 * i + c];
+    for (int c = 0; c < parts; ++c) v[c] = block_sum(v[c], slots);
     if (threadIdx.x == 0) {
         *loss = static_cast<float>(v[0] * scale);
         if (out_stats != nullptr) {
@@ -877,12 +532,13 @@ int64_t row_blocks(Op op, int64_t n) {
 // Workspace: parts, weights, row sums, counted.
 struct Space {
     MaxSum *part;
-    float *weight, *counted, *gap;
+    float *weight, *counted, *gap, *entry_x;
+    int32_t *entry_id;
     double *sums;
     size_t bytes;
 };
 
-Space carve(void *base, int64_t n, int64_t vocab, int64_t pairs) {
+Space carve(void *base, int64_t n, int64_t vocab, int64_t pairs, int64_t top = 0) {
     const Split s = split_of(n, vocab);
     uint8_t *p = static_cast<uint8_t *>(base);
     size_t at = 0;
@@ -895,11 +551,19 @@ Space carve(void *base, int64_t n, int64_t vocab, int64_t pairs) {
     w.part = reinterpret_cast<MaxSum *>(take(static_cast<size_t>(n) * s.splits * sizeof(MaxSum)));
     w.weight = reinterpret_cast<float *>(take(static_cast<size_t>(n) * sizeof(float)));
     w.gap = reinterpret_cast<float *>(take(static_cast<size_t>(n) * sizeof(float)));
-    const int64_t most = pairs > 2048 ? pairs : 2048;
+    const int64_t most = pairs > n ? pairs : n > 2048 ? n : 2048;
     w.sums = reinterpret_cast<double *>(take(static_cast<size_t>(most) * 3 * sizeof(double)));
-    w.counted = reinterpret_cast<float *>(take(sizeof(float)));
+    w.counted = reinterpret_cast<float *>(take(2 * sizeof(float)));
+    w.entry_x = reinterpret_cast<float *>(take(static_cast<size_t>(n) * top * sizeof(float)));
+    w.entry_id = reinterpret_cast<int32_t *>(take(static_cast<size_t>(n) * top * sizeof(int32_t)));
     w.bytes = at;
     return w;
+}
+
+// rows_per_batch past the rows there are makes one batch of them; one that is not positive stays 0 for the check.
+Logits logits_of(const void *x, int64_t n, int64_t rows_per_batch, int64_t batch_stride, int64_t row_stride, int64_t vocab) {
+    const uint32_t per = rows_per_batch < 1 ? 0u : static_cast<uint32_t>(rows_per_batch < INT32_MAX ? rows_per_batch : INT32_MAX);
+    return {x, n, per, batch_stride, row_stride, static_cast<int32_t>(vocab)};
 }
 
 int check_logits(const char *what, const Logits &l, int dtype) {
@@ -937,14 +601,18 @@ int check_seqs(const char *what, const void *offsets, int dtype, int64_t n_seqs,
 
 template <typename T, int kThreads>
 void launch_stats_of(const StatsArgs &a, bool left_out, hipStream_t s) {
-    const unsigned blocks = static_cast<unsigned>(a.logits.n * a.splits + (a.weights.weight != nullptr ? 1 : 0));
+    const unsigned blocks = static_cast<unsigned>(a.logits.n * a.splits + (a.weights.counted != nullptr ? 1 : 0));
     if (blocks == 0) return;
     if (left_out) stats_kernel<T, kThreads, true><<<blocks, kThreads, 0, s>>>(a);
     else stats_kernel<T, kThreads, false><<<blocks, kThreads, 0, s>>>(a);
 }
 
-void launch_stats(const StatsArgs &a, int dtype, bool left_out, hipStream_t s) {
+void launch_stats(StatsArgs a, int dtype, bool left_out, hipStream_t s) {
     const bool small = a.logits.vocab <= 2048;
+    if (small && a.weights.counted != nullptr) {  // many rows may be counted: not by a workgroup of one wavefront
+        weights_kernel<<<1, 1024, 0, s>>>(a.weights);
+        a.weights.counted = nullptr;
+    }
     if (dtype == ME_BF16) {
         if (small) launch_stats_of<uint16_t, 64>(a, left_out, s);
         else launch_stats_of<uint16_t, 256>(a, left_out, s);
@@ -958,10 +626,11 @@ template <Op kOp>
 void launch_rows(const RowArgs &a, int dtype, hipStream_t s) {
     const unsigned blocks = static_cast<unsigned>(row_blocks(kOp, a.logits.n));
     const int threads = kOp == kDistill ? 256 : 1024;
-    if (dtype == ME_BF16) row_kernel<kOp, true><<<blocks, threads, 0, s>>>(a);
-    else row_kernel<kOp, false><<<blocks, threads, 0, s>>>(a);
+    const size_t lds = kOp == kDistill ? size_t{4} * kEntryBytes * a.top : 0;
+    if (dtype == ME_BF16) row_kernel<kOp, true><<<blocks, threads, lds, s>>>(a);
+    else row_kernel<kOp, false><<<blocks, threads, lds, s>>>(a);
     if (kOp >= kPolicy && blocks > 1)
-        total_kernel<<<1, 256, 0, s>>>(a.sums, blocks, a.counted, a.scale, a.loss, a.out_stats);
+        total_kernel<<<1, 1024, 0, s>>>(a.sums, blocks, a.weights.counted, a.scale, a.loss, a.out_stats);
 }
 
 void launch_grad(const GradArgs &a, int dtype, hipStream_t s) {
@@ -977,12 +646,6 @@ void launch_grad(const GradArgs &a, int dtype, hipStream_t s) {
     }
 }
 
-#define ME_TRY(call)                     \
-    do {                                 \
-        const int st_ = (call);          \
-        if (st_ != ME_OK) return st_;    \
-    } while (0)
-
 int check_space(const char *what, const Space &w, const void *workspace, size_t bytes) {
     if (workspace == nullptr || bytes < w.bytes) {
         set_error("%s: workspace of %zu bytes, %zu needed", what, workspace == nullptr ? size_t{0} : bytes, w.bytes);
@@ -996,11 +659,12 @@ int check_space(const char *what, const Space &w, const void *workspace, size_t 
 
 using namespace me;
 
-extern "C" int me_loss_workspace_size(int64_t n, int64_t vocab, int64_t pairs, size_t *bytes) {
+extern "C" int me_loss_workspace_size(int64_t n, int64_t vocab, int64_t pairs, int64_t top, size_t *bytes) {
     ME_CHECK_ARG(bytes != nullptr, "me_loss_workspace_size: bytes is null");
-    ME_CHECK_ARG(n >= 0 && n <= INT32_MAX && pairs >= 0 && pairs <= INT32_MAX, "me_loss_workspace_size: size out of range");
+    ME_CHECK_ARG(n >= 0 && n <= INT32_MAX && pairs >= 0 && pairs <= INT32_MAX && top >= 0 && top <= kMaxTop,
+                 "me_loss_workspace_size: size out of range");
     ME_CHECK_ARG(vocab >= 1 && vocab <= kMaxSpan * kMaxSplits, "me_loss_workspace_size: vocab must be in 1..%d", kMaxSpan * kMaxSplits);
-    *bytes = carve(nullptr, n, vocab, pairs).bytes;
+    *bytes = carve(nullptr, n, vocab, pairs, top).bytes;
     return ME_OK;
 }
 
@@ -1010,7 +674,7 @@ extern "C" int me_token_logps(const void *logits, int dtype, int64_t n, int64_t 
                               void *workspace, size_t workspace_bytes, void *stream) {
     const char *what = "me_token_logps";
     ME_CHECK_ARG(vocab >= 1 && vocab <= kMaxSpan * kMaxSplits, "%s: vocab must be in 1..%d", what, kMaxSpan * kMaxSplits);
-    const Logits l = {logits, n, rows_per_batch, batch_stride, row_stride, static_cast<int32_t>(vocab)};
+    const Logits l = logits_of(logits, n, rows_per_batch, batch_stride, row_stride, vocab);
     ME_TRY(check_logits(what, l, dtype));
     ME_TRY(check_temperature(what, temperature));
     ME_TRY(check_tokens(what, targets, targets_dtype, n));
@@ -1048,7 +712,7 @@ extern "C" int me_token_logps_backward(const void *logits, int dtype, int64_t n,
                                        void *grad, void *stream) {
     const char *what = "me_token_logps_backward";
     ME_CHECK_ARG(vocab >= 1 && vocab <= kMaxSpan * kMaxSplits, "%s: vocab must be in 1..%d", what, kMaxSpan * kMaxSplits);
-    const Logits l = {logits, n, rows_per_batch, batch_stride, row_stride, static_cast<int32_t>(vocab)};
+    const Logits l = logits_of(logits, n, rows_per_batch, batch_stride, row_stride, vocab);
     ME_TRY(check_logits(what, l, dtype));
     ME_TRY(check_temperature(what, temperature));
     ME_TRY(check_tokens(what, targets, targets_dtype, n));
@@ -1079,7 +743,7 @@ extern "C" int me_preference(const void *logits, int dtype, int64_t n, int64_t v
                              void *workspace, size_t workspace_bytes, void *stream) {
     const char *what = "me_preference";
     ME_CHECK_ARG(vocab >= 1 && vocab <= kMaxSpan * kMaxSplits, "%s: vocab must be in 1..%d", what, kMaxSpan * kMaxSplits);
-    const Logits l = {logits, n, rows_per_batch, batch_stride, row_stride, static_cast<int32_t>(vocab)};
+    const Logits l = logits_of(logits, n, rows_per_batch, batch_stride, row_stride, vocab);
     ME_TRY(check_logits(what, l, dtype));
     ME_TRY(check_tokens(what, targets, targets_dtype, n));
     ME_CHECK_ARG(pairs >= 0 && pairs < INT32_MAX / 2, "%s: pairs out of range", what);
@@ -1137,7 +801,7 @@ extern "C" int me_preference(const void *logits, int dtype, int64_t n, int64_t v
     } else {
         const int64_t blocks = ceil_div(pairs, 4) < 2048 ? ceil_div(pairs, 4) : 2048;
         pair_kernel<<<static_cast<unsigned>(blocks), 256, 0, s>>>(p);
-        total_kernel<<<1, 256, 0, s>>>(w.sums, blocks, nullptr, 1.0f / static_cast<float>(pairs), loss, nullptr);
+        total_kernel<<<1, 1024, 0, s>>>(w.sums, blocks, nullptr, 1.0f / static_cast<float>(pairs), loss, nullptr);
     }
     return check_launch(what);
 }
@@ -1151,7 +815,7 @@ extern "C" int me_policy(const void *logits, int dtype, int64_t n, int64_t vocab
                          float *coef, void *grad, void *workspace, size_t workspace_bytes, void *stream) {
     const char *what = "me_policy";
     ME_CHECK_ARG(vocab >= 1 && vocab <= kMaxSpan * kMaxSplits, "%s: vocab must be in 1..%d", what, kMaxSpan * kMaxSplits);
-    const Logits l = {logits, n, rows_per_batch, batch_stride, row_stride, static_cast<int32_t>(vocab)};
+    const Logits l = logits_of(logits, n, rows_per_batch, batch_stride, row_stride, vocab);
     ME_TRY(check_logits(what, l, dtype));
     ME_TRY(check_temperature(what, temperature));
     ME_TRY(check_tokens(what, targets, targets_dtype, n));
@@ -1182,14 +846,15 @@ extern "C" int me_policy(const void *logits, int dtype, int64_t n, int64_t vocab
     st.weights.vocab = l.vocab;
     st.weights.use_seqs = seq_offsets != nullptr || reduction == kSequence;
     st.weights.reduction = reduction;
-    launch_stats(st, dtype, false, s);
+    const bool pass = grad != nullptr && takes_row_pass(n, vocab, dtype, 0);
+    if (pass) weights_kernel<<<1, 1024, 0, s>>>(st.weights);
+    else launch_stats(st, dtype, false, s);
     RowArgs r = {};
     r.logits = l;
     r.tokens = st.tokens;
     r.seqs = seqs;
     r.part = w.part;
-    r.weight = w.weight;
-    r.counted = w.counted;
+    r.weights = st.weights;
     r.stats = reinterpret_cast<float2 *>(row_stats);
     r.logps = logps;
     r.coef = coef;
@@ -1207,6 +872,11 @@ extern "C" int me_policy(const void *logits, int dtype, int64_t n, int64_t vocab
     r.kl_coef = static_cast<float>(kl_coef);
     r.splits = sp.splits;
     r.adv_per_seq = adv_per_seq;
+    if (pass) {
+        launch_row_pass(kPolicy, r, dtype, grad, s);
+        total_kernel<<<1, 1024, 0, s>>>(w.sums, n, w.counted, r.scale, loss, out_stats);
+        return check_launch(what);
+    }
     launch_rows<kPolicy>(r, dtype, s);
     if (grad != nullptr) {
         GradArgs g = {};
@@ -1232,7 +902,7 @@ extern "C" int me_distill(const void *logits, int dtype, int64_t n, int64_t voca
                           size_t workspace_bytes, void *stream) {
     const char *what = "me_distill";
     ME_CHECK_ARG(vocab >= 1 && vocab <= kMaxSpan * kMaxSplits, "%s: vocab must be in 1..%d", what, kMaxSpan * kMaxSplits);
-    const Logits l = {logits, n, rows_per_batch, batch_stride, row_stride, static_cast<int32_t>(vocab)};
+    const Logits l = logits_of(logits, n, rows_per_batch, batch_stride, row_stride, vocab);
     ME_TRY(check_logits(what, l, dtype));
     ME_TRY(check_temperature(what, temperature));
     ME_CHECK_ARG(ids_dtype == ME_I32 || ids_dtype == ME_I64, "%s: teacher ids must be int32 or int64", what);
@@ -1243,7 +913,7 @@ extern "C" int me_distill(const void *logits, int dtype, int64_t n, int64_t voca
     ME_CHECK_ARG(loss != nullptr, "%s: null output", what);
     ME_CHECK_ARG(n == 0 || (teacher_ids != nullptr && teacher != nullptr && row_stats != nullptr && coef != nullptr &&
                             fix != nullptr), "%s: null pointer", what);
-    const Space w = carve(workspace, n, vocab, 0);
+    const Space w = carve(workspace, n, vocab, 0, top);
     ME_TRY(check_space(what, w, workspace, workspace_bytes));
     const hipStream_t s = as_stream(stream);
     const Split sp = split_of(n, vocab);
@@ -1266,13 +936,13 @@ extern "C" int me_distill(const void *logits, int dtype, int64_t n, int64_t voca
     st.weights.n = n;
     st.weights.vocab = l.vocab;
     st.weights.reduction = reduction;
-    launch_stats(st, dtype, teacher_lse != nullptr, s);
+    const bool pass = grad != nullptr && takes_row_pass(n, vocab, dtype, top);
+    if (!pass) launch_stats(st, dtype, teacher_lse != nullptr, s);
     RowArgs r = {};
     r.logits = l;
     r.tokens = st.tokens;
     r.part = w.part;
-    r.weight = w.weight;
-    r.counted = w.counted;
+    r.weights = st.weights;
     r.stats = reinterpret_cast<float2 *>(row_stats);
     r.coef = coef;
     r.ids = teacher_ids;
@@ -1289,6 +959,18 @@ extern "C" int me_distill(const void *logits, int dtype, int64_t n, int64_t voca
     r.temp = static_cast<float>(temperature);
     r.scale = static_cast<float>(scale);
     r.splits = sp.splits;
+    if (pass) {
+        r.near = w.gap;
+        r.entry_x = w.entry_x;
+        r.entry_id = w.entry_id;
+        const unsigned blocks = static_cast<unsigned>(ceil_div(n, 4) + 1);
+        const size_t lds = size_t{4} * kEntryBytes * top;
+        if (dtype == ME_BF16) entries_kernel<true><<<blocks, 256, lds, s>>>(r);
+        else entries_kernel<false><<<blocks, 256, lds, s>>>(r);
+        launch_row_pass(kDistill, r, dtype, grad, s);
+        total_kernel<<<1, 1024, 0, s>>>(w.sums, n, nullptr, r.scale, loss, nullptr);
+        return check_launch(what);
+    }
     launch_rows<kDistill>(r, dtype, s);
     if (grad != nullptr) {
         GradArgs g = {};
@@ -1315,7 +997,7 @@ extern "C" int me_distill_backward(const void *logits, int dtype, int64_t n, int
                                    const float *fix, const float *upstream, int done_for_one, void *grad, void *stream) {
     const char *what = "me_distill_backward";
     ME_CHECK_ARG(vocab >= 1 && vocab <= kMaxSpan * kMaxSplits, "%s: vocab must be in 1..%d", what, kMaxSpan * kMaxSplits);
-    const Logits l = {logits, n, rows_per_batch, batch_stride, row_stride, static_cast<int32_t>(vocab)};
+    const Logits l = logits_of(logits, n, rows_per_batch, batch_stride, row_stride, vocab);
     ME_TRY(check_logits(what, l, dtype));
     ME_TRY(check_temperature(what, temperature));
     ME_CHECK_ARG(ids_dtype == ME_I32 || ids_dtype == ME_I64, "%s: teacher ids must be int32 or int64", what);

@@ -13,14 +13,14 @@ from .ops import _custom_op, _p, dtype_code, require_gpu, stream_of
 
 
 @functools.lru_cache(maxsize=256)
-def workspace_bytes(n, vocab, pairs=0):
+def workspace_bytes(n, vocab, pairs=0, top=0):
     size = ctypes.c_size_t(0)
-    call("me_loss_workspace_size", n, vocab, pairs, ctypes.byref(size))
+    call("me_loss_workspace_size", n, vocab, pairs, top, ctypes.byref(size))
     return size.value
 
 
-def _workspace(n, vocab, dev, pairs=0):
-    ws = torch.empty(workspace_bytes(n, vocab, pairs), dtype=torch.uint8, device=dev)
+def _workspace(n, vocab, dev, pairs=0, top=0):
+    ws = torch.empty(workspace_bytes(n, vocab, pairs, top), dtype=torch.uint8, device=dev)
     return ws, ws.data_ptr(), ws.numel()
 
 
@@ -199,7 +199,7 @@ def distill(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: tor
     top = ids.shape[-1]
     loss, stats, coef, fix = _f32(dev=dev), _f32(n, 2, dev=dev), _f32(n, dev=dev), _f32(n, top, dev=dev)
     grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev) if with_grad else None
-    ws, ptr, size = _workspace(n, vocab, dev)
+    ws, ptr, size = _workspace(n, vocab, dev, 0, top)
     call("me_distill", *rows, ids.data_ptr(), _int_code(ids, "teacher_ids"), teacher.data_ptr(),
          dtype_code(teacher), top, _p(teacher_lse), _p(mask), temperature, scale, reduction, loss.data_ptr(),
          stats.data_ptr(), coef.data_ptr(), fix.data_ptr(), _p(grad), ptr, size, stream_of(dev))
