@@ -14,7 +14,6 @@ using namespace loss;
 namespace {
 
 constexpr int64_t kPassRows = 128;  // rows from which
-constexpr bool kNtLoads = true;
 constexpr int kPassTop = 512;  // teacher entries the kernels' LDS has room for
 
 // The logit at an index that all threads share.
@@ -70,7 +69,7 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *g
     const float last = load1(x + min(8 * whole + tid, vocab - 1));
     // slot s of a thread: the 8 logits of chunk s * kThreads + tid
     const auto load_slot = [&](int32_t s, Raw8<T> &raw) {
-        load_raw<kNtLoads>(x + 8 * static_cast<int64_t>(min(s * kThreads + tid, whole - 1)), raw);
+        load_raw<false>(x + 8 * static_cast<int64_t>(min(s * kThreads + tid, whole - 1)), raw);
     };
     Raw8<T> q[kRegs];
 #pragma unroll

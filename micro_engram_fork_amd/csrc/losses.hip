@@ -609,7 +609,7 @@ void launch_stats_of(const StatsArgs &a, bool left_out, hipStream_t s) {
 
 void launch_stats(StatsArgs a, int dtype, bool left_out, hipStream_t s) {
     const bool small = a.logits.vocab <= 2048;
-    if (small && a.weights.counted != nullptr) {  // many rows may be counted: not by a workgroup of one wavefront
+    if (small && a.weights.counted != nullptr && a.logits.n > 1024) {  // too many for a workgroup of one wavefront
         weights_kernel<<<1, 1024, 0, s>>>(a.weights);
         a.weights.counted = nullptr;
     }

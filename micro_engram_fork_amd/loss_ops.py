@@ -9,7 +9,7 @@ from typing import List, Optional
 import torch
 
 from ._lib import ME_I32, ME_I64, call
-from .ops import _custom_op, _p, dtype_code, require_gpu, stream_of
+from .ops import _custom_op, _direct_call, _p, dtype_code, require_gpu, stream_of
 
 
 @functools.lru_cache(maxsize=256)
@@ -33,14 +33,13 @@ def row_layout(logits):
         logits = logits.contiguous()
     lead = logits.dim() - 1
     n = logits.numel() // vocab if vocab else 0
+    rows = logits
     if lead > 2:
         try:
             rows = logits.view(-1, logits.shape[-2], vocab)
         except RuntimeError:
             logits = logits.contiguous()
             rows = logits.view(-1, logits.shape[-2], vocab)
-    else:
-        rows = logits
     if lead == 0:
         per, batch_stride, row_stride = 1, 0, 0
     elif lead == 1:
@@ -50,26 +49,50 @@ def row_layout(logits):
     return logits, (logits.data_ptr(), dtype_code(logits), n, vocab, per, batch_stride, row_stride)
 
 
+def is_plain(*tensors):
+    """Whether a call on these tensors runs the kernels at once (no tracing, no fake tensors)."""
+    return _direct_call(tensors, None)
+
+
 def _int_code(t, what):
-    if t.dtype not in (torch.int32, torch.int64):
-        raise TypeError(f"[micro_engram] {what} must be int32 or int64, got {t.dtype}")
-    return ME_I32 if t.dtype == torch.int32 else ME_I64
+    if t.dtype is torch.int64:
+        return ME_I64
+    if t.dtype is torch.int32:
+        return ME_I32
+    raise TypeError(f"[micro_engram] {what} must be int32 or int64, got {t.dtype}")
+
+
+def _contiguous(t):
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _targets(targets, ignore_index):
-    targets = targets.contiguous()
+    targets = _contiguous(targets)
     return targets, (targets.data_ptr(), _int_code(targets, "targets"), ignore_index)
 
 
 def _offsets(offsets):
     if offsets is None:
         return None, (None, 0)
-    offsets = offsets.contiguous()
+    offsets = _contiguous(offsets)
     return offsets, (offsets.data_ptr(), _int_code(offsets, "cu_seqlens"))
 
 
-def _f32(*shape, dev):
+def _f32(shape, dev):
     return torch.empty(shape, dtype=torch.float32, device=dev)
+
+
+# What a backward needs of n rows is one fp32 buffer: (m, 1 / s) pairs [n, 2], factors [n], and for
+# distillation the values at the teacher's entries [n, top].
+def _saved(n, dev, top=0):
+    """(buffer, addresses of its parts)."""
+    saved = _f32(n * (3 + top), dev)
+    return saved, *_saved_parts(saved, n)
+
+
+def _saved_parts(saved, n):
+    at = saved.data_ptr()
+    return at, at + 8 * n, at + 12 * n
 
 
 # ------------------------------------------------------------------------- log-probabilities
@@ -82,8 +105,8 @@ def token_logps(logits: torch.Tensor, targets: torch.Tensor, ignore_index: int, 
     logits, rows = row_layout(logits)
     targets, toks = _targets(targets, ignore_index)
     n, vocab = rows[2], rows[3]
-    out = _f32(*targets.shape, dev=dev)
-    stats = _f32(n, 2, dev=dev) if with_stats else None
+    out = _f32(targets.shape, dev)
+    stats = _f32((n, 2), dev) if with_stats else None
     ws, ptr, size = _workspace(n, vocab, dev)
     call("me_token_logps", *rows, *toks, temperature, out.data_ptr(), _p(stats), ptr, size, stream_of(dev))
     return [out, stats] if with_stats else [out]
@@ -95,35 +118,73 @@ def _(logits, targets, ignore_index, temperature, with_stats):
     return [out, logits.new_empty((targets.numel(), 2), dtype=torch.float32)] if with_stats else [out]
 
 
-def _token_logps_backward(grad, logits, targets, stats, coef, upstream, ignore_index, temperature, coef_scale,
-                          done_for_one):
-    dev = require_gpu(logits, targets, stats, coef, upstream)
+def _token_logps_backward(logits, targets, stats, coef, upstream, ignore_index, temperature, coef_scale):
+    """stats, coef: addresses."""
+    grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
     logits, rows = row_layout(logits)
     targets, toks = _targets(targets, ignore_index)
-    call("me_token_logps_backward", *rows, *toks, temperature, stats.data_ptr(), coef.data_ptr(), coef_scale,
-         _p(upstream), int(done_for_one), grad.data_ptr(), stream_of(dev))
+    call("me_token_logps_backward", *rows, *toks, temperature, stats, coef, coef_scale, _p(upstream),
+         0, grad.data_ptr(), stream_of(logits.device))
     return grad
 
 
 @_custom_op("token_logps_backward")
 def token_logps_backward(logits: torch.Tensor, targets: torch.Tensor, stats: torch.Tensor, coef: torch.Tensor,
-                         upstream: Optional[torch.Tensor], ignore_index: int, temperature: float,
-                         coef_scale: float) -> torch.Tensor:
-    """The logits' gradient coef * coef_scale * upstream * (1[j = target] - probability of j)."""
-    grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    return _token_logps_backward(grad, logits, targets, stats, coef, upstream, ignore_index, temperature,
-                                 coef_scale, False)
+                         ignore_index: int, temperature: float) -> torch.Tensor:
+    """The logits' gradient coef / temperature * (1[j = target] - probability of j)."""
+    require_gpu(logits, targets, stats, coef)
+    return _token_logps_backward(logits, targets, stats.data_ptr(), coef.data_ptr(), None, ignore_index, temperature,
+                                 1.0 / temperature)
 
 
 @token_logps_backward.register_fake
-def _(logits, targets, stats, coef, upstream, ignore_index, temperature, coef_scale):
+def _(logits, targets, stats, coef, ignore_index, temperature):
     return logits.new_empty(logits.shape)
 
 
-def token_grad_for(grad, upstream, logits, targets, stats, coef, ignore_index, temperature):
-    """`grad`, the gradient for an upstream of 1, made the one for `upstream`: in place, and only where
-    that is not 1 (the kernel looks, not the host)."""
-    return _token_logps_backward(grad, logits, targets, stats, coef, upstream, ignore_index, temperature, 1.0, True)
+@_custom_op("saved_token_backward")
+def saved_token_backward(logits: torch.Tensor, targets: torch.Tensor, saved: torch.Tensor, upstream: torch.Tensor,
+                         ignore_index: int, temperature: float) -> torch.Tensor:
+    """The logits' gradient from what preference and policy leave of their rows, times upstream (fp32)."""
+    require_gpu(logits, targets, saved, upstream)
+    stats, coef, _ = _saved_parts(saved, targets.numel())
+    return _token_logps_backward(logits, targets, stats, coef, upstream, ignore_index, temperature, 1.0)
+
+
+@saved_token_backward.register_fake
+def _(logits, targets, saved, upstream, ignore_index, temperature):
+    return logits.new_empty(logits.shape)
+
+
+# A gradient that the forward has written already is right for an upstream of 1. These give what makes
+# it the one for another upstream: a call whose arguments the forward has at hand, so that the backward,
+# which autograd runs in a thread of its own, has little left to do.
+class Rescale:
+    """rescale(upstream): `grad` in place, and only where upstream (fp32, on the device) is not 1: the kernel
+    looks, not the host."""
+    __slots__ = ("name", "args", "grad", "kept")
+
+    def __init__(self, name, args, grad, *kept):
+        self.name, self.args, self.grad, self.kept = name, args, grad, kept
+
+    def __call__(self, upstream):
+        call(self.name, *self.args, upstream.data_ptr(), 1, self.grad.data_ptr(), stream_of(self.grad.device))
+        return self.grad
+
+
+def token_rescale(grad, logits, targets, saved, ignore_index, temperature):
+    logits, rows = row_layout(logits)
+    targets, toks = _targets(targets, ignore_index)
+    stats, coef, _ = _saved_parts(saved, rows[2])
+    return Rescale("me_token_logps_backward", (*rows, *toks, temperature, stats, coef, 1.0), grad, logits, targets,
+                   saved)
+
+
+def distill_rescale(grad, logits, teacher_ids, saved, temperature):
+    logits, rows = row_layout(logits)
+    ids = _contiguous(teacher_ids)
+    return Rescale("me_distill_backward", (*rows, ids.data_ptr(), _int_code(ids, "teacher_ids"), ids.shape[-1],
+                                           temperature, *_saved_parts(saved, rows[2])), grad, logits, ids, saved)
 
 
 # -------------------------------------------------------------------------------- preference
@@ -131,25 +192,25 @@ def token_grad_for(grad, upstream, logits, targets, stats, coef, ignore_index, t
 def preference(logits: torch.Tensor, targets: torch.Tensor, ref_logps: torch.Tensor,
                offsets: Optional[torch.Tensor], pairs: int, seq_len: int, kind: int, beta: float,
                smoothing: float, normalized: bool, ignore_index: int) -> List[torch.Tensor]:
-    """[loss, chosen [pairs], rejected [pairs], row stats [n, 2], coef [n]], all fp32."""
+    """[loss, chosen [pairs], rejected [pairs], saved [3 n]], all fp32."""
     dev = require_gpu(logits, targets, ref_logps, offsets)
     logits, rows = row_layout(logits)
     targets, toks = _targets(targets, ignore_index)
     offsets, seqs = _offsets(offsets)
     n, vocab = rows[2], rows[3]
-    loss, chosen, rejected = _f32(dev=dev), _f32(pairs, dev=dev), _f32(pairs, dev=dev)
-    stats, coef = _f32(n, 2, dev=dev), _f32(n, dev=dev)
+    loss, chosen, rejected = _f32((), dev), _f32((pairs,), dev), _f32((pairs,), dev)
+    saved, stats, coef, _ = _saved(n, dev)
     ws, ptr, size = _workspace(n, vocab, dev, pairs)
     call("me_preference", *rows, *toks, ref_logps.data_ptr(), *seqs, pairs, seq_len, kind, beta, smoothing,
-         int(normalized), loss.data_ptr(), chosen.data_ptr(), rejected.data_ptr(), stats.data_ptr(),
-         coef.data_ptr(), ptr, size, stream_of(dev))
-    return [loss, chosen, rejected, stats, coef]
+         int(normalized), loss.data_ptr(), chosen.data_ptr(), rejected.data_ptr(), stats, coef, ptr, size,
+         stream_of(dev))
+    return [loss, chosen, rejected, saved]
 
 
 @preference.register_fake
 def _(logits, targets, ref_logps, offsets, pairs, seq_len, kind, beta, smoothing, normalized, ignore_index):
     n, new = targets.numel(), functools.partial(logits.new_empty, dtype=torch.float32)
-    return [new(()), new((pairs,)), new((pairs,)), new((n, 2)), new((n,))]
+    return [new(()), new((pairs,)), new((pairs,)), new((3 * n,))]
 
 
 # ------------------------------------------------------------------------------------ policy
@@ -158,22 +219,21 @@ def policy(logits: torch.Tensor, targets: torch.Tensor, old_logps: torch.Tensor,
            adv_per_seq: bool, ref_logps: Optional[torch.Tensor], offsets: Optional[torch.Tensor], n_seqs: int,
            seq_len: int, clip_low: float, clip_high: float, kl_coef: float, temperature: float, scale: float,
            reduction: int, ignore_index: int, with_grad: bool) -> List[torch.Tensor]:
-    """[loss, log-probabilities of targets' shape, (mean KL, clipped share), row stats [n, 2], coef [n]],
-    all fp32, plus the logits' gradient for an upstream of 1 when with_grad."""
+    """[loss, log-probabilities of targets' shape, (mean KL, clipped share), saved [3 n]], all fp32, plus
+    the logits' gradient for an upstream of 1 when with_grad."""
     dev = require_gpu(logits, targets, old_logps, advantages, ref_logps, offsets)
     logits, rows = row_layout(logits)
     targets, toks = _targets(targets, ignore_index)
     offsets, seqs = _offsets(offsets)
     n, vocab = rows[2], rows[3]
-    loss, logps, out_stats = _f32(dev=dev), _f32(*targets.shape, dev=dev), _f32(2, dev=dev)
-    stats, coef = _f32(n, 2, dev=dev), _f32(n, dev=dev)
+    loss, logps, out_stats = _f32((), dev), _f32(targets.shape, dev), _f32((2,), dev)
+    saved, stats, coef, _ = _saved(n, dev)
     grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev) if with_grad else None
     ws, ptr, size = _workspace(n, vocab, dev)
     call("me_policy", *rows, *toks, old_logps.data_ptr(), advantages.data_ptr(), int(adv_per_seq), _p(ref_logps),
          *seqs, n_seqs, seq_len, clip_low, clip_high, kl_coef, temperature, scale, reduction, loss.data_ptr(),
-         logps.data_ptr(), out_stats.data_ptr(), stats.data_ptr(), coef.data_ptr(), _p(grad), ptr, size,
-         stream_of(dev))
-    res = [loss, logps, out_stats, stats, coef]
+         logps.data_ptr(), out_stats.data_ptr(), stats, coef, _p(grad), ptr, size, stream_of(dev))
+    res = [loss, logps, out_stats, saved]
     return [*res, grad] if with_grad else res
 
 
@@ -181,7 +241,7 @@ def policy(logits: torch.Tensor, targets: torch.Tensor, old_logps: torch.Tensor,
 def _(logits, targets, old_logps, advantages, adv_per_seq, ref_logps, offsets, n_seqs, seq_len, clip_low,
       clip_high, kl_coef, temperature, scale, reduction, ignore_index, with_grad):
     n, new = targets.numel(), functools.partial(logits.new_empty, dtype=torch.float32)
-    res = [new(()), new(targets.shape), new((2,)), new((n, 2)), new((n,))]
+    res = [new(()), new(targets.shape), new((2,)), new((3 * n,))]
     return [*res, logits.new_empty(logits.shape)] if with_grad else res
 
 
@@ -190,53 +250,43 @@ def _(logits, targets, old_logps, advantages, adv_per_seq, ref_logps, offsets, n
 def distill(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor,
             teacher_lse: Optional[torch.Tensor], mask: Optional[torch.Tensor], temperature: float, scale: float,
             reduction: int, with_grad: bool) -> List[torch.Tensor]:
-    """[loss, row stats [n, 2], coef [n], fix [n, top]], all fp32, plus the logits' gradient for an
-    upstream of 1 when with_grad."""
+    """[loss, saved [(3 + top) n]], fp32, plus the logits' gradient for an upstream of 1 when with_grad."""
     dev = require_gpu(logits, teacher_ids, teacher_logits, teacher_lse, mask)
     logits, rows = row_layout(logits)
     n, vocab = rows[2], rows[3]
-    ids, teacher = teacher_ids.contiguous(), teacher_logits.contiguous()
+    ids, teacher = _contiguous(teacher_ids), _contiguous(teacher_logits)
     top = ids.shape[-1]
-    loss, stats, coef, fix = _f32(dev=dev), _f32(n, 2, dev=dev), _f32(n, dev=dev), _f32(n, top, dev=dev)
+    loss = _f32((), dev)
+    saved, stats, coef, fix = _saved(n, dev, top)
     grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev) if with_grad else None
     ws, ptr, size = _workspace(n, vocab, dev, 0, top)
     call("me_distill", *rows, ids.data_ptr(), _int_code(ids, "teacher_ids"), teacher.data_ptr(),
          dtype_code(teacher), top, _p(teacher_lse), _p(mask), temperature, scale, reduction, loss.data_ptr(),
-         stats.data_ptr(), coef.data_ptr(), fix.data_ptr(), _p(grad), ptr, size, stream_of(dev))
-    res = [loss, stats, coef, fix]
-    return [*res, grad] if with_grad else res
+         stats, coef, fix, _p(grad), ptr, size, stream_of(dev))
+    return [loss, saved, grad] if with_grad else [loss, saved]
 
 
 @distill.register_fake
 def _(logits, teacher_ids, teacher_logits, teacher_lse, mask, temperature, scale, reduction, with_grad):
     top = teacher_ids.shape[-1]
     n, new = teacher_ids.numel() // top, functools.partial(logits.new_empty, dtype=torch.float32)
-    res = [new(()), new((n, 2)), new((n,)), new((n, top))]
+    res = [new(()), new((n * (3 + top),))]
     return [*res, logits.new_empty(logits.shape)] if with_grad else res
 
 
-def _distill_backward(grad, logits, teacher_ids, stats, coef, fix, upstream, temperature, done_for_one):
-    dev = require_gpu(logits, teacher_ids, stats, coef, fix, upstream)
+@_custom_op("distill_backward")
+def distill_backward(logits: torch.Tensor, teacher_ids: torch.Tensor, saved: torch.Tensor, upstream: torch.Tensor,
+                     temperature: float) -> torch.Tensor:
+    """The logits' gradient from what distill leaves of its rows, times upstream (fp32)."""
+    require_gpu(logits, teacher_ids, saved, upstream)
+    grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
     logits, rows = row_layout(logits)
-    ids = teacher_ids.contiguous()
+    ids = _contiguous(teacher_ids)
     call("me_distill_backward", *rows, ids.data_ptr(), _int_code(ids, "teacher_ids"), ids.shape[-1], temperature,
-         stats.data_ptr(), coef.data_ptr(), fix.data_ptr(), _p(upstream), int(done_for_one), grad.data_ptr(),
-         stream_of(dev))
+         *_saved_parts(saved, rows[2]), upstream.data_ptr(), 0, grad.data_ptr(), stream_of(logits.device))
     return grad
 
 
-@_custom_op("distill_backward")
-def distill_backward(logits: torch.Tensor, teacher_ids: torch.Tensor, stats: torch.Tensor, coef: torch.Tensor,
-                     fix: torch.Tensor, upstream: Optional[torch.Tensor], temperature: float) -> torch.Tensor:
-    grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    return _distill_backward(grad, logits, teacher_ids, stats, coef, fix, upstream, temperature, False)
-
-
 @distill_backward.register_fake
-def _(logits, teacher_ids, stats, coef, fix, upstream, temperature):
+def _(logits, teacher_ids, saved, upstream, temperature):
     return logits.new_empty(logits.shape)
-
-
-def distill_grad_for(grad, upstream, logits, teacher_ids, stats, coef, fix, temperature):
-    """As token_grad_for."""
-    return _distill_backward(grad, logits, teacher_ids, stats, coef, fix, upstream, temperature, True)

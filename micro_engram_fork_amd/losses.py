@@ -21,6 +21,7 @@ gradients they write it in the forward and keep it for the backward, for an upst
 The backward looks (on the device) whether that held, and computes the gradient again from the
 logits if not: give a factor such as 1 / accumulation steps as `scale`, where it costs nothing.
 """
+import functools
 import math
 
 import torch
@@ -77,6 +78,8 @@ def _per_row(values, shape, what):
     """fp32 contiguous values of the rows, without their history."""
     if tuple(values.shape) != tuple(shape):
         raise ValueError(f"[micro_engram] {what} {tuple(values.shape)} do not match the rows {tuple(shape)}")
+    if values.dtype is torch.float32 and not values.requires_grad and values.is_contiguous():
+        return values
     if not values.is_floating_point():
         raise TypeError(f"[micro_engram] {what} must be floating point, got {values.dtype}")
     return values.detach().float().contiguous()
@@ -94,6 +97,21 @@ def _sequences(targets, cu_seqlens):
     return cu_seqlens.numel() - 1, 0
 
 
+def _no_second_derivatives(backward):
+    """once_differentiable, whose bookkeeping is needed only where a graph of the backward is made."""
+    guarded = once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        return (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
+    return run
+
+
+def _upstream(grad):
+    """The loss's own gradient as the kernels read it."""
+    return grad if grad.dtype is torch.float32 and grad.is_contiguous() else grad.float().contiguous()
+
+
 def _wants_grad(logits):
     return torch.is_grad_enabled() and logits.requires_grad
 
@@ -108,13 +126,12 @@ class _TokenLogps(torch.autograd.Function):
         return logps
 
     @staticmethod
-    @once_differentiable
+    @_no_second_derivatives
     def backward(ctx, grad):
         logits, targets, stats = ctx.saved_tensors
         ignore_index, temperature = ctx.consts
-        coef = grad.float().contiguous()
-        return loss_ops.token_logps_backward(logits.detach(), targets, stats, coef, None, ignore_index,
-                                             temperature, 1.0 / temperature), None, None, None
+        return loss_ops.token_logps_backward(logits.detach(), targets, stats, _upstream(grad), ignore_index,
+                                             temperature), None, None, None
 
 
 def token_logps(logits, targets, temperature=1.0, ignore_index=IGNORE_INDEX):
@@ -130,26 +147,22 @@ def token_logps(logits, targets, temperature=1.0, ignore_index=IGNORE_INDEX):
 # -------------------------------------------------------------------------------- preference
 class _Preference(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, targets, ref_logps, offsets, pairs, seq_len, kind, beta, smoothing, normalized,
-                ignore_index):
-        loss, chosen, rejected, stats, coef = loss_ops.preference(
-            logits.detach(), targets, ref_logps, offsets, pairs, seq_len, kind, beta, smoothing, normalized,
-            ignore_index)
-        ctx.save_for_backward(logits, targets, stats, coef)
-        ctx.ignore_index = ignore_index
+    def forward(ctx, logits, targets, args):  # one tuple, as in _Policy
+        loss, chosen, rejected, saved = loss_ops.preference(logits.detach(), targets, *args)
+        ctx.save_for_backward(logits, targets, saved)
+        ctx.ignore_index = args[-1]
         ctx.mark_non_differentiable(chosen, rejected)
         ctx.set_materialize_grads(False)
         return loss, chosen, rejected
 
     @staticmethod
-    @once_differentiable
+    @_no_second_derivatives
     def backward(ctx, upstream, _chosen, _rejected):
         if upstream is None:
-            return (None,) * 11
-        logits, targets, stats, coef = ctx.saved_tensors
-        grad = loss_ops.token_logps_backward(logits.detach(), targets, stats, coef, upstream.float().contiguous(),
-                                             ctx.ignore_index, 1.0, 1.0)
-        return (grad, *(None,) * 10)
+            return None, None, None
+        logits, targets, saved = ctx.saved_tensors
+        grad = loss_ops.saved_token_backward(logits.detach(), targets, saved, _upstream(upstream), ctx.ignore_index, 1.0)
+        return grad, None, None
 
 
 def preference_loss(logits, targets, ref_logps, cu_seqlens=None, beta=0.1, loss_type="sigmoid",
@@ -179,40 +192,39 @@ def preference_loss(logits, targets, ref_logps, cu_seqlens=None, beta=0.1, loss_
     if n_seqs % 2:
         raise ValueError(f"[micro_engram] {n_seqs} sequences are no pairs")
     ref = _per_row(ref_logps, targets.shape, "ref_logps")
-    args = (targets, ref, cu_seqlens, n_seqs // 2, seq_len, kind, beta, smoothing, bool(length_normalized),
-            int(ignore_index))
+    args = (ref, cu_seqlens, n_seqs // 2, seq_len, kind, beta, smoothing, bool(length_normalized), int(ignore_index))
     if _wants_grad(logits):
-        return _Preference.apply(logits, *args)
-    return tuple(loss_ops.preference(logits.detach(), *args)[:3])
+        return _Preference.apply(logits, targets, args)
+    return tuple(loss_ops.preference(logits.detach(), targets, *args)[:3])
 
 
 # ------------------------------------------------------------------------------------ policy
+# These take everything but their first two tensors as one tuple: apply() costs host time for each argument, and a
+# small batch's training step is bound by the rate at which the host issues it.
 class _Policy(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, targets, *args):
-        # under torch.compile the gradient is the backward's: the kept one is overwritten in place
-        early = not torch.compiler.is_compiling()
-        loss, logps, out_stats, stats, coef, *grad = loss_ops.policy(logits.detach(), targets, *args, early)
-        ctx.save_for_backward(logits, targets, stats, coef)
-        ctx.grad = grad[0] if early else None
+    def forward(ctx, logits, targets, args):
+        early = loss_ops.is_plain(logits, targets)  # traced: the gradient is the backward's, nothing in place
+        loss, logps, out_stats, saved, *grad = loss_ops.policy(logits.detach(), targets, *args, early)
         ctx.consts = args[-1], args[-4]  # ignore_index, temperature
+        ctx.rescale = loss_ops.token_rescale(grad[0], logits.detach(), targets, saved, *ctx.consts) if early else None
+        ctx.save_for_backward(logits, targets, saved)
         ctx.mark_non_differentiable(logps, out_stats)
         ctx.set_materialize_grads(False)
         return loss, logps, out_stats
 
     @staticmethod
-    @once_differentiable
+    @_no_second_derivatives
     def backward(ctx, upstream, _logps, _stats):
         if upstream is None:
-            return (None,) * 16
-        logits, targets, stats, coef = ctx.saved_tensors
-        upstream, consts = upstream.float().contiguous(), ctx.consts
-        grad, ctx.grad = ctx.grad, None  # handed out once: a second backward computes its own
-        if grad is not None:
-            grad = loss_ops.token_grad_for(grad, upstream, logits.detach(), targets, stats, coef, *consts)
+            return None, None, None
+        logits, targets, saved = ctx.saved_tensors  # looks whether they are still as they were
+        rescale, ctx.rescale = ctx.rescale, None  # the gradient is handed out once: a second backward computes its own
+        if rescale is not None:
+            grad = rescale(_upstream(upstream))
         else:
-            grad = loss_ops.token_logps_backward(logits.detach(), targets, stats, coef, upstream, *consts, 1.0)
-        return (grad, *(None,) * 15)
+            grad = loss_ops.saved_token_backward(logits.detach(), targets, saved, _upstream(upstream), *ctx.consts)
+        return grad, None, None
 
 
 def policy_loss(logits, targets, old_logps, advantages, ref_logps=None, cu_seqlens=None, clip_low=0.2,
@@ -250,32 +262,32 @@ def policy_loss(logits, targets, old_logps, advantages, ref_logps=None, cu_seqle
     args = (old, adv, per_seq, ref, cu_seqlens, n_seqs, seq_len, clip_low, clip_high, kl_coef, temperature, scale,
             how, int(ignore_index))
     if _wants_grad(logits):
-        return _Policy.apply(logits, targets, *args)
+        return _Policy.apply(logits, targets, args)
     return tuple(loss_ops.policy(logits.detach(), targets, *args, False)[:3])
 
 
 # ------------------------------------------------------------------------------ distillation
 class _Distill(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, teacher_ids, *args):
-        early = not torch.compiler.is_compiling()  # as in _Policy
-        loss, stats, coef, fix, *grad = loss_ops.distill(logits.detach(), teacher_ids, *args, early)
-        ctx.save_for_backward(logits, teacher_ids, stats, coef, fix)
-        ctx.grad = grad[0] if early else None
+    def forward(ctx, logits, teacher_ids, args):
+        early = loss_ops.is_plain(logits, teacher_ids)  # as in _Policy
+        loss, saved, *grad = loss_ops.distill(logits.detach(), teacher_ids, *args, early)
         ctx.temperature = args[3]
+        ctx.rescale = (loss_ops.distill_rescale(grad[0], logits.detach(), teacher_ids, saved, ctx.temperature)
+                       if early else None)
+        ctx.save_for_backward(logits, teacher_ids, saved)
         return loss
 
     @staticmethod
-    @once_differentiable
+    @_no_second_derivatives
     def backward(ctx, upstream):
-        logits, teacher_ids, *rows = ctx.saved_tensors
-        upstream = upstream.float().contiguous()
-        grad, ctx.grad = ctx.grad, None  # handed out once: a second backward computes its own
-        if grad is not None:
-            grad = loss_ops.distill_grad_for(grad, upstream, logits.detach(), teacher_ids, *rows, ctx.temperature)
+        logits, teacher_ids, saved = ctx.saved_tensors
+        rescale, ctx.rescale = ctx.rescale, None
+        if rescale is not None:
+            grad = rescale(_upstream(upstream))
         else:
-            grad = loss_ops.distill_backward(logits.detach(), teacher_ids, *rows, upstream, ctx.temperature)
-        return (grad, *(None,) * 7)
+            grad = loss_ops.distill_backward(logits.detach(), teacher_ids, saved, _upstream(upstream), ctx.temperature)
+        return grad, None, None
 
 
 def distill_loss(logits, teacher_ids, teacher_logits, teacher_lse=None, mask=None, temperature=1.0, scale=1.0,
@@ -315,7 +327,7 @@ def distill_loss(logits, teacher_ids, teacher_logits, teacher_lse=None, mask=Non
         if tuple(mask.shape) != lead or mask.dtype not in (torch.bool, torch.uint8):
             raise ValueError(f"[micro_engram] mask must be bool {lead}, got {mask.dtype} {tuple(mask.shape)}")
         mask = mask.contiguous()
-    args = (teacher_ids, teacher_logits.detach(), lse, mask, temperature, scale, how)
+    args = (teacher_logits.detach(), lse, mask, temperature, scale, how)
     if _wants_grad(logits):
-        return _Distill.apply(logits, *args)
-    return loss_ops.distill(logits.detach(), *args, False)[0]
+        return _Distill.apply(logits, teacher_ids, args)
+    return loss_ops.distill(logits.detach(), teacher_ids, *args, False)[0]

@@ -538,7 +538,7 @@ def test_captured_graph_replays_like_eager():
 
     def step():
         res = loss_ops.policy(x, t, old, adv, False, old, None, 1, n, 0.2, 0.2, 0.1, 1.0, 1.0, 0, -100, True)
-        return losses.token_logps(x, t), res[0], res[5]
+        return losses.token_logps(x, t), res[0], res[4]
 
     x.copy_(xs[0])
     side = torch.cuda.Stream()
