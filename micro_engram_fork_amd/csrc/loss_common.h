@@ -95,77 +95,82 @@ struct Seqs {
 typedef uint32_t u32x4_e2 __attribute__((ext_vector_type(4), aligned(2)));
 typedef float f32x4_e4 __attribute__((ext_vector_type(4), aligned(4)));
 
+// A row is worked on in units of 16 bytes, one per thread and load: neighbouring lanes then read neighbouring units.
 template <typename T>
-struct Raw8;  // 8 logits as loaded
+constexpr int kVec = 16 / sizeof(T);
+
+template <typename T>
+struct Raw;  // a unit as loaded
 template <>
-struct Raw8<uint16_t> {
+struct Raw<uint16_t> {
     u32x4_v w;
 };
 template <>
-struct Raw8<float> {
-    f32x4_v lo, hi;
+struct Raw<float> {
+    f32x4_v w;
 };
 
-template <bool kNt>
-__device__ __forceinline__ void load_raw(const uint16_t *p, Raw8<uint16_t> &r) {
+// kStream: past the caches (non-temporal), for rows that are read or written once
+template <bool kStream>
+__device__ __forceinline__ void load_raw(const uint16_t *p, Raw<uint16_t> &r) {
     const auto q = reinterpret_cast<const __attribute__((address_space(1))) u32x4_e2 *>(as_global(p));
-    if constexpr (kNt) r.w = __builtin_nontemporal_load(q);
+    if constexpr (kStream) r.w = __builtin_nontemporal_load(q);
     else r.w = *q;
 }
-template <bool kNt>
-__device__ __forceinline__ void load_raw(const float *p, Raw8<float> &r) {
+template <bool kStream>
+__device__ __forceinline__ void load_raw(const float *p, Raw<float> &r) {
     const auto q = reinterpret_cast<const __attribute__((address_space(1))) f32x4_e4 *>(as_global(p));
-    const auto h = reinterpret_cast<const __attribute__((address_space(1))) f32x4_e4 *>(as_global(p + 4));
-    if constexpr (kNt) {
-        r.lo = __builtin_nontemporal_load(q);
-        r.hi = __builtin_nontemporal_load(h);
-    } else {
-        r.lo = *q;
-        r.hi = *h;
-    }
+    if constexpr (kStream) r.w = __builtin_nontemporal_load(q);
+    else r.w = *q;
 }
-__device__ __forceinline__ void widen(const Raw8<uint16_t> &r, float (&v)[8]) {
+__device__ __forceinline__ void widen(const Raw<uint16_t> &r, float (&v)[8]) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         v[2 * e] = __uint_as_float(r.w[e] << 16);
         v[2 * e + 1] = __uint_as_float(r.w[e] & 0xffff0000u);
     }
 }
-__device__ __forceinline__ void widen(const Raw8<float> &r, float (&v)[8]) {
+__device__ __forceinline__ void widen(const Raw<float> &r, float (&v)[4]) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        v[e] = r.lo[e];
-        v[4 + e] = r.hi[e];
-    }
+    for (int e = 0; e < 4; ++e) v[e] = r.w[e];
 }
 // values back into the form of loaded fp32 logits
-__device__ __forceinline__ void keep_raw(Raw8<float> &r, const float (&v)[8]) {
-    r.lo = f32x4_v{v[0], v[1], v[2], v[3]};
-    r.hi = f32x4_v{v[4], v[5], v[6], v[7]};
-}
+__device__ __forceinline__ void keep_raw(Raw<float> &r, const float (&v)[4]) { r.w = f32x4_v{v[0], v[1], v[2], v[3]}; }
 __device__ __forceinline__ float load1(const uint16_t *p) { return bf16_bits_to_float(*as_global(p)); }
 __device__ __forceinline__ float load1(const float *p) { return *as_global(p); }
 
-// 8 logits from element j, minus infinity past the end of the row
-template <typename T>
-__device__ __forceinline__ void load8_tail(const T *row, int32_t j, int32_t vocab, float (&v)[8]) {
+// N logits from element j, minus infinity past the end of the row
+template <typename T, int N>
+__device__ __forceinline__ void load_tail(const T *row, int32_t j, int32_t vocab, float (&v)[N]) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = j + e < vocab ? load1(row + j + e) : -kInf;
+    for (int e = 0; e < N; ++e) v[e] = j + e < vocab ? load1(row + j + e) : -kInf;
 }
 
 __device__ __forceinline__ void store1(uint16_t *p, float f) { *as_global(p) = float_to_bf16_bits_rne(f); }
 __device__ __forceinline__ void store1(float *p, float f) { *as_global(p) = f; }
-__device__ __forceinline__ void store8(uint16_t *p, const float (&v)[8]) {
+template <bool kStream>
+__device__ __forceinline__ void store_unit(uint16_t *p, const float (&v)[8]) {
     u32x4_v w;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
         w[e] = static_cast<uint32_t>(float_to_bf16_bits_rne(v[2 * e])) |
                (static_cast<uint32_t>(float_to_bf16_bits_rne(v[2 * e + 1])) << 16);
-    *reinterpret_cast<__attribute__((address_space(1))) u32x4_e2 *>(as_global(p)) = w;
+    const auto q = reinterpret_cast<__attribute__((address_space(1))) u32x4_e2 *>(as_global(p));
+    if constexpr (kStream) __builtin_nontemporal_store(u32x4_e2(w), q);
+    else *q = w;
 }
-__device__ __forceinline__ void store8(float *p, const float (&v)[8]) {
-    *reinterpret_cast<__attribute__((address_space(1))) f32x4_e4 *>(as_global(p)) = f32x4_v{v[0], v[1], v[2], v[3]};
-    *reinterpret_cast<__attribute__((address_space(1))) f32x4_e4 *>(as_global(p + 4)) = f32x4_v{v[4], v[5], v[6], v[7]};
+template <bool kStream>
+__device__ __forceinline__ void store_unit(float *p, const float (&v)[4]) {
+    const auto q = reinterpret_cast<__attribute__((address_space(1))) f32x4_e4 *>(as_global(p));
+    const f32x4_v w = {v[0], v[1], v[2], v[3]};
+    if constexpr (kStream) __builtin_nontemporal_store(f32x4_e4(w), q);
+    else *q = w;
+}
+
+template <int N>
+__device__ __forceinline__ float tree_sum(const float (&e)[N]) {
+    if constexpr (N == 4) return (e[0] + e[1]) + (e[2] + e[3]);
+    else return ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
 }
 
 // ------------------------------------------------------------------------------------------ (m, s) pairs
@@ -205,11 +210,12 @@ __device__ __forceinline__ float without_rounding(float s, const Guess &g, float
     return s * __builtin_amdgcn_exp2f(-__builtin_fmaf(g.m, k, -g.mk));
 }
 
-__device__ __forceinline__ float sum8(const float (&v)[8], const Guess &g, float k) {
-    float e[8];
+template <int N>
+__device__ __forceinline__ float guessed_sum(const float (&v)[N], const Guess &g, float k) {
+    float e[N];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = guessed_exp(v[i], g, k);
-    return ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+    for (int i = 0; i < N; ++i) e[i] = guessed_exp(v[i], g, k);
+    return tree_sum(e);
 }
 
 constexpr float kLargestSum = 0x1p100f, kSmallestSum = 0x1p-60f;
@@ -224,12 +230,7 @@ __device__ __forceinline__ void add_values(MaxSum &a, const float (&v)[N], float
     float part[N];
 #pragma unroll
     for (int e = 0; e < N; ++e) part[e] = exp2_of(v[e], ref, k);
-#pragma unroll
-    for (int w = N / 2; w > 0; w /= 2) {
-#pragma unroll
-        for (int e = 0; e < w; ++e) part[e] += part[e + w];
-    }
-    a.s = a.s * exp2_of(a.m, ref, k) + part[0];
+    a.s = a.s * exp2_of(a.m, ref, k) + tree_sum(part);
     a.m = m;
 }
 
@@ -493,7 +494,7 @@ static __device__ float distill_finish(const RowArgs &a, int64_t r, MaxSum seen,
 
 }  // namespace loss
 
-// loss_rows.hip: whether rows of this size and number take its one-read kernels, and their launch
+// loss_rows.hip: whether rows of this size and number take its one-read kernels, and their launch (stream_rows: past the caches)
 bool takes_row_pass(int64_t n, int64_t vocab, int dtype, int64_t top);
-void launch_row_pass(loss::Op op, const loss::RowArgs &a, int dtype, void *grad, hipStream_t s);
+void launch_row_pass(loss::Op op, const loss::RowArgs &a, int dtype, void *grad, bool stream_rows, hipStream_t s);
 }  // namespace me

@@ -22,22 +22,23 @@ __device__ __forceinline__ float scalar_logit(const uint16_t *x, int32_t j) {
 }
 __device__ __forceinline__ float scalar_logit(const float *x, int32_t j) { return constant(x + j); }
 
-template <typename T, int kThreads, int kRegs, int kLds, Op kOp, bool kRest>
+template <typename T, int kThreads, int kRegs, int kLds, bool kStream, Op kOp, bool kRest>
 __global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *grad) {
+    constexpr int N = kVec<T>;
     constexpr bool kDist = kOp == kDistill;
     constexpr int kWaves = kThreads / 64;
     constexpr bool kKeepExp = sizeof(T) == 4;  // fp32 slots take the exponentials in place: the gradient needs no second one
-    __shared__ Raw8<T> held[kLds > 0 ? kLds : 1][kThreads];
+    __shared__ Raw<T> held[kLds > 0 ? kLds : 1][kThreads];
     __shared__ __attribute__((aligned(16))) uint8_t entry_space[kDist ? kPassTop * kEntryBytes : 16];
     __shared__ float sums[kWaves];
     const int64_t r = blockIdx.x;
     const int32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int32_t vocab = a.logits.vocab, whole = vocab / 8, slots = (whole + kThreads - 1) / kThreads, rest = vocab - 8 * whole;
+    const int32_t vocab = a.logits.vocab, whole = vocab / N, slots = (whole + kThreads - 1) / kThreads, rest = vocab - N * whole;
     T *g = static_cast<T *>(grad) + r * vocab;
     if (constant(a.weights.weight + r) == 0.0f) {
-        const float zeros[8] = {};
-        for (int32_t i = tid; i < whole; i += kThreads) store8(g + 8 * i, zeros);
-        if (tid < rest) store1(g + 8 * whole + tid, 0.0f);
+        const float zeros[N] = {};
+        for (int32_t i = tid; i < whole; i += kThreads) store_unit<kStream>(g + N * i, zeros);
+        if (tid < rest) store1(g + N * whole + tid, 0.0f);
         if (tid == 0) {
             a.stats[r] = {0.0f, 0.0f};
             a.coef[r] = 0.0f;
@@ -51,7 +52,7 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *g
     const T *x = static_cast<const T *>(a.logits.x) + a.logits.offset(r);
 
     // All loads of the row are issued before the first is used, and none of them under a condition: a slot past the row's
-    // end loads the last chunk again. (Loads return in the order of their issue; after one that may or may not have been
+    // end loads the last unit again. (Loads return in the order of their issue; after one that may or may not have been
     // issued the compiler can only wait for all.) The entries of a row come before its logits for the same reason.
     constexpr int kPer = kDist ? (kPassTop + kThreads - 1) / kThreads : 1;  // entries of a thread
     const Entries e = entries_at(entry_space, a.top);
@@ -66,12 +67,12 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *g
             entry_x[u] = *as_global(a.entry_x + r * a.top + i);
         }
     }
-    const float last = load1(x + min(8 * whole + tid, vocab - 1));
-    // slot s of a thread: the 8 logits of chunk s * kThreads + tid
-    const auto load_slot = [&](int32_t s, Raw8<T> &raw) {
-        load_raw<false>(x + 8 * static_cast<int64_t>(min(s * kThreads + tid, whole - 1)), raw);
+    const float last = load1(x + min(N * whole + tid, vocab - 1));
+    // slot s of a thread: unit s * kThreads + tid
+    const auto load_slot = [&](int32_t s, Raw<T> &raw) {
+        load_raw<kStream>(x + N * static_cast<int64_t>(min(s * kThreads + tid, whole - 1)), raw);
     };
-    Raw8<T> q[kRegs];
+    Raw<T> q[kRegs];
 #pragma unroll
     for (int c = 0; c < kRegs; ++c) load_slot(c, q[c]);
 
@@ -102,7 +103,7 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *g
         if constexpr (kWaves > 1) __syncthreads();
         else wave_lds_order();
         for (int32_t i0 = 0; i0 < a.top; i0 += 64) {
-            const int32_t i = i0 + lane, c = i < a.top ? e.id[i] >> 3 : -1, s = c / kThreads;
+            const int32_t i = i0 + lane, c = i < a.top ? e.id[i] / N : -1, s = c / kThreads;
             uint64_t hits = __ballot(c >= 0 && c < whole && (c % kThreads) >> 6 == wave);
             while (hits != 0) {
                 const int src = __builtin_ctzll(hits);
@@ -114,11 +115,11 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *g
     float tail = tid < rest ? last : -kInf;
     // v at the entries' tokens in slot s of this wavefront becomes coef times their `value`, or minus infinity
     float coef = 0.0f;
-    const auto at_entries = [&](int32_t s, float (&v)[8], const float *value) {
+    const auto at_entries = [&](int32_t s, float (&v)[N], const float *value) {
         const int32_t first = s * kThreads + wave * 64;
         for (int32_t i0 = 0; i0 < a.top; i0 += 64) {
             const int32_t i = i0 + lane, id = i < a.top ? e.id[i] : -1;
-            const int32_t rel = (id >> 3) - first;
+            const int32_t rel = (id / N) - first;
             const float mine = value != nullptr && i < a.top ? coef * value[i] : -kInf;
             uint64_t hits = __ballot(id >= 0 && rel >= 0 && rel < 64);
             while (hits != 0) {
@@ -127,28 +128,28 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *g
                 const int32_t token = __builtin_amdgcn_readlane(id, src);
                 const float val = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(mine), src));
 #pragma unroll
-                for (int w = 0; w < 8; ++w)
-                    if (lane == (token >> 3) - first && w == (token & 7)) v[w] = val;
+                for (int w = 0; w < N; ++w)
+                    if (lane == (token / N) - first && w == (token % N)) v[w] = val;
             }
         }
     };
 
     // ---- sum of exponentials
     float sum = 0.0f;
-    const auto add_slot = [&](int32_t s, Raw8<T> &raw) {
-        float v[8];
+    const auto add_slot = [&](int32_t s, Raw<T> &raw) {
+        float v[N];
         widen(raw, v);
         if ((s + 1) * kThreads > whole && s * kThreads + tid >= whole) {
 #pragma unroll
-            for (int w = 0; w < 8; ++w) v[w] = -kInf;
+            for (int w = 0; w < N; ++w) v[w] = -kInf;
         }
         if constexpr (kRest) {
             if (marks >> s & 1) at_entries(s, v, nullptr);
         }
 #pragma unroll
-        for (int w = 0; w < 8; ++w) v[w] = guessed_exp(v[w], guess, a.k);
+        for (int w = 0; w < N; ++w) v[w] = guessed_exp(v[w], guess, a.k);
         if constexpr (kKeepExp) keep_raw(raw, v);
-        sum += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+        sum += tree_sum(v);
     };
 #pragma unroll
     for (int c = 0; c < kLds; ++c) {  // these make room for the slots past the registers' own
@@ -165,14 +166,14 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *g
     for (int c = 0; c < kLds; ++c)
         if (kRegs + c < slots) add_slot(kRegs + c, q[c]);
     for (int32_t s = kRegs + kLds; s < slots; ++s) {
-        Raw8<T> raw;
+        Raw<T> raw;
         load_slot(s, raw);
         add_slot(s, raw);
     }
     if constexpr (kRest) {
         if (tid < rest)
             for (int32_t i = 0; i < a.top; ++i)
-                if (e.id[i] == 8 * whole + tid) tail = -kInf;
+                if (e.id[i] == N * whole + tid) tail = -kInf;
     }
     sum = wave_sum(sum + guessed_exp(tail, guess, a.k));
     if constexpr (kWaves > 1) {
@@ -186,17 +187,17 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *g
     const bool guessed = guess.fits && sum < kLargestSum && (!kRest || sum > kSmallestSum);
     if (!guessed) {  // again, with the running maximum
         row = {-kInf, 0.0f};
-        for (int32_t j = 8 * tid; j < vocab; j += 8 * kThreads) {
-            float v[8];
-            load8_tail(x, j, vocab, v);
+        for (int32_t j = N * tid; j < vocab; j += N * kThreads) {
+            float v[N];
+            load_tail(x, j, vocab, v);
             if constexpr (kRest) {
                 for (int32_t i = 0; i < a.top; ++i) {
 #pragma unroll
-                    for (int w = 0; w < 8; ++w)
+                    for (int w = 0; w < N; ++w)
                         if (e.id[i] == j + w) v[w] = -kInf;
                 }
             }
-            add_values<8>(row, v, a.k);
+            add_values(row, v, a.k);
         }
         row = wave_join(row, a.k);
         if constexpr (kWaves > 1) {
@@ -241,8 +242,8 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *g
     // ---- gradient
     if (grad == nullptr) return;
     if (!guessed) {
-        for (int32_t j = 8 * tid; j < vocab; j += 8 * kThreads) {
-            for (int w = 0; w < 8 && j + w < vocab; ++w) {
+        for (int32_t j = N * tid; j < vocab; j += N * kThreads) {
+            for (int w = 0; w < N && j + w < vocab; ++w) {
                 float d = factor * exp2_of(load1(x + j + w), ref, a.k);
                 if constexpr (kDist) {
                     for (int32_t i = 0; i < a.top; ++i)
@@ -257,12 +258,12 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *g
     }
     // exponentials are those of `sum`; the rounding of m k that row.s is without goes into the factor
     factor = without_rounding(factor, guess, a.k);
-    const int32_t t_slot = kDist || t >= 8 * whole ? -1 : (t >> 3) / kThreads, t_thread = kDist ? -1 : (t >> 3) % kThreads;
-    const auto put_slot = [&](int32_t s, const Raw8<T> &raw) {
-        float d[8];
+    const int32_t t_slot = kDist || t >= N * whole ? -1 : (t / N) / kThreads, t_thread = kDist ? -1 : (t / N) % kThreads;
+    const auto put_slot = [&](int32_t s, const Raw<T> &raw) {
+        float d[N];
         widen(raw, d);
 #pragma unroll
-        for (int w = 0; w < 8; ++w) {
+        for (int w = 0; w < N; ++w) {
             if constexpr (!kKeepExp) d[w] = guessed_exp(d[w], guess, a.k);
             d[w] *= factor;
         }
@@ -270,11 +271,11 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *g
             if (marks >> s & 1) at_entries(s, d, e.raw);
         } else if (s == t_slot) {
 #pragma unroll
-            for (int w = 0; w < 8; ++w)
-                if (tid == t_thread && w == (t & 7)) d[w] += coef;
+            for (int w = 0; w < N; ++w)
+                if (tid == t_thread && w == (t % N)) d[w] += coef;
         }
         const int32_t c = s * kThreads + tid;
-        if (c < whole) store8(g + 8 * static_cast<int64_t>(c), d);
+        if (c < whole) store_unit<kStream>(g + N * static_cast<int64_t>(c), d);
     };
 #pragma unroll
     for (int c = kLds; c < kRegs; ++c)
@@ -286,19 +287,19 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *g
     for (int c = 0; c < kLds; ++c)
         if (c < slots) put_slot(c, held[c][tid]);
     for (int32_t s = kRegs + kLds; s < slots; ++s) {
-        Raw8<T> raw;
+        Raw<T> raw;
         load_slot(s, raw);
         if constexpr (kKeepExp) {
-            float v[8];
+            float v[N];
             widen(raw, v);
 #pragma unroll
-            for (int w = 0; w < 8; ++w) v[w] = guessed_exp(v[w], guess, a.k);
+            for (int w = 0; w < N; ++w) v[w] = guessed_exp(v[w], guess, a.k);
             keep_raw(raw, v);
         }
         put_slot(s, raw);
     }
     if (tid < rest) {
-        const int32_t j = 8 * whole + tid;
+        const int32_t j = N * whole + tid;
         float d = factor * guessed_exp(tail, guess, a.k) + (j == t ? coef : 0.0f);
         if constexpr (kDist) {
             for (int32_t i = 0; i < a.top; ++i)
@@ -308,12 +309,23 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *g
     }
 }
 
-template <typename T, int kThreads, int kRegs, int kLds>
+template <typename T, int kThreads, int kRegs, int kLds, bool kStream = false>
 void launch_pass_of(Op op, const RowArgs &a, void *grad, hipStream_t s) {
     const unsigned n = static_cast<unsigned>(a.logits.n);
-    if (op == kPolicy) pass_kernel<T, kThreads, kRegs, kLds, kPolicy, false><<<n, kThreads, 0, s>>>(a, grad);
-    else if (a.teacher_lse != nullptr) pass_kernel<T, kThreads, kRegs, kLds, kDistill, true><<<n, kThreads, 0, s>>>(a, grad);
-    else pass_kernel<T, kThreads, kRegs, kLds, kDistill, false><<<n, kThreads, 0, s>>>(a, grad);
+    if (op == kPolicy) pass_kernel<T, kThreads, kRegs, kLds, kStream, kPolicy, false><<<n, kThreads, 0, s>>>(a, grad);
+    else if (a.teacher_lse != nullptr) pass_kernel<T, kThreads, kRegs, kLds, kStream, kDistill, true><<<n, kThreads, 0, s>>>(a, grad);
+    else pass_kernel<T, kThreads, kRegs, kLds, kStream, kDistill, false><<<n, kThreads, 0, s>>>(a, grad);
+}
+
+template <typename T>
+void launch_pass(Op op, const RowArgs &a, void *grad, bool stream_rows, hipStream_t s) {
+    const int32_t units = a.logits.vocab / kVec<T>;
+    if (units <= 64 * 16) launch_pass_of<T, 64, 16, 0>(op, a, grad, s);
+    else if (units <= 256 * 16) launch_pass_of<T, 256, 16, 0>(op, a, grad, s);
+    else if (units <= 1024 * 16) launch_pass_of<T, 1024, 16, 0>(op, a, grad, s);
+    else if (units <= 1024 * 22) launch_pass_of<T, 1024, 22, 0>(op, a, grad, s);
+    else if (stream_rows) launch_pass_of<T, 1024, 22, 9, true>(op, a, grad, s);
+    else launch_pass_of<T, 1024, 22, 9>(op, a, grad, s);
 }
 
 }  // namespace
@@ -323,19 +335,9 @@ bool takes_row_pass(int64_t n, int64_t vocab, int dtype, int64_t top) {
     return vocab <= (dtype == ME_BF16 ? 327680 : 163840) && n >= kPassRows;
 }
 
-void launch_row_pass(Op op, const RowArgs &a, int dtype, void *grad, hipStream_t s) {
-    const int32_t v = a.logits.vocab;
-    if (dtype == ME_BF16) {
-        if (v <= 8192) launch_pass_of<uint16_t, 64, 16, 0>(op, a, grad, s);
-        else if (v <= 32768) launch_pass_of<uint16_t, 256, 16, 0>(op, a, grad, s);
-        else if (v <= 131072) launch_pass_of<uint16_t, 1024, 16, 0>(op, a, grad, s);
-        else launch_pass_of<uint16_t, 1024, 22, 9>(op, a, grad, s);
-    } else {
-        if (v <= 4096) launch_pass_of<float, 64, 8, 0>(op, a, grad, s);
-        else if (v <= 16384) launch_pass_of<float, 256, 8, 0>(op, a, grad, s);
-        else if (v <= 65536) launch_pass_of<float, 1024, 8, 0>(op, a, grad, s);
-        else launch_pass_of<float, 1024, 11, 4>(op, a, grad, s);
-    }
+void launch_row_pass(Op op, const RowArgs &a, int dtype, void *grad, bool stream_rows, hipStream_t s) {
+    if (dtype == ME_BF16) launch_pass<uint16_t>(op, a, grad, stream_rows, s);
+    else launch_pass<float>(op, a, grad, stream_rows, s);
 }
 
 }  // namespace me

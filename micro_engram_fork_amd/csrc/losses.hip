@@ -141,44 +141,46 @@ __global__ __launch_bounds__(kThreads) void stats_kernel(const StatsArgs a) {
         if (id >= 0) near = load1(x + id);
     }
     const Guess guess = guess_of(near, a.k);
-    const auto leave_out = [&](float (&v)[8], int32_t j) {
+    constexpr int N = kVec<T>;
+    const auto leave_out = [&](float (&v)[N], int32_t j) {
         if constexpr (kLeaveOut) {
             const int32_t at = j - from;
-            const uint32_t bits = (left_out[at >> 5] >> (at & 31)) & 0xff;
+            const uint32_t bits = (left_out[at >> 5] >> (at & 31)) & ((1u << N) - 1);
             if (bits != 0) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
+                for (int e = 0; e < N; ++e)
                     if (bits >> e & 1) v[e] = -kInf;
             }
         }
     };
-    const int32_t whole = (to - from) / 8;  // spans are multiples of 8: only the row's end has a rest
+    const int32_t whole = (to - from) / N;  // spans are whole units: only the row's end has a rest
+    constexpr int kUnroll = sizeof(T) == 2 ? 4 : 8;  // loads in flight per thread
     const auto sweep = [&](auto take) {
         int32_t c = tid;
-        for (; c + 3 * kThreads < whole; c += 4 * kThreads) {
-            Raw8<T> raw[4];
+        for (; c + (kUnroll - 1) * kThreads < whole; c += kUnroll * kThreads) {
+            Raw<T> raw[kUnroll];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) load_raw<true>(x + from + 8 * (c + u * kThreads), raw[u]);
+            for (int u = 0; u < kUnroll; ++u) load_raw<true>(x + from + N * (c + u * kThreads), raw[u]);
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                float v[8];
+            for (int u = 0; u < kUnroll; ++u) {
+                float v[N];
                 widen(raw[u], v);
-                leave_out(v, from + 8 * (c + u * kThreads));
+                leave_out(v, from + N * (c + u * kThreads));
                 take(v);
             }
         }
         for (; c < whole; c += kThreads) {
-            Raw8<T> raw;
-            load_raw<true>(x + from + 8 * c, raw);
-            float v[8];
+            Raw<T> raw;
+            load_raw<true>(x + from + N * c, raw);
+            float v[N];
             widen(raw, v);
-            leave_out(v, from + 8 * c);
+            leave_out(v, from + N * c);
             take(v);
         }
-        if (from + 8 * whole < to && tid == whole % kThreads) {
-            float v[8];
-            load8_tail(x, from + 8 * whole, vocab, v);
-            leave_out(v, from + 8 * whole);
+        if (from + N * whole < to && tid == whole % kThreads) {
+            float v[N];
+            load_tail(x, from + N * whole, vocab, v);
+            leave_out(v, from + N * whole);
             take(v);
         }
     };
@@ -186,7 +188,7 @@ __global__ __launch_bounds__(kThreads) void stats_kernel(const StatsArgs a) {
     __shared__ MaxSum joined[kThreads / 64];
     if (guess.fits) {
         float sum = 0.0f;
-        sweep([&](float (&v)[8]) { sum += sum8(v, guess, a.k); });
+        sweep([&](float (&v)[N]) { sum += guessed_sum(v, guess, a.k); });
         sum = wave_sum(sum);
         if constexpr (kThreads > 64) {
             if ((tid & 63) == 0) sums[tid >> 6] = sum;
@@ -200,7 +202,7 @@ __global__ __launch_bounds__(kThreads) void stats_kernel(const StatsArgs a) {
         }
     }
     MaxSum acc = {-kInf, 0.0f};
-    sweep([&](float (&v)[8]) { add_values<8>(acc, v, a.k); });
+    sweep([&](float (&v)[N]) { add_values(acc, v, a.k); });
     acc = wave_join(acc, a.k);
     if constexpr (kThreads > 64) {
         if ((tid & 63) == 0) joined[tid >> 6] = acc;
@@ -438,8 +440,9 @@ struct GradArgs {
 
 // One part of a row per workgroup: streams the logits once more and writes the gradient; a copy's bytes, and bound
 // by them. Rows whose factor is 0 are filled without being read.
-template <typename T, int kThreads>
+template <typename T, int kThreads, bool kStream>
 __global__ __launch_bounds__(kThreads) void grad_kernel(const GradArgs a) {
+    constexpr int N = kVec<T>;
     const float up = a.upstream != nullptr ? *a.upstream : 1.0f;
     if (a.done_for_one && up == 1.0f) return;
     const int64_t row = blockIdx.x / a.splits;
@@ -448,52 +451,53 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(const GradArgs a) {
     const bool distill = a.tokens.targets == nullptr;
     const int32_t t = distill ? -1 : a.tokens.token(row, vocab);
     const int32_t from = part * a.span, to = min(vocab, from + a.span);
-    const int32_t whole = (to - from) / 8;
+    const int32_t whole = (to - from) / N;
     T *g = static_cast<T *>(a.grad) + row * vocab;
     const float c = (distill || t >= 0) ? a.coef[row] * up * a.extra : 0.0f;
     if (c == 0.0f) {
-        const float zeros[8] = {};
-        for (int32_t i = tid; i < whole; i += kThreads) store8(g + from + 8 * i, zeros);
-        if (tid < to - from - 8 * whole) store1(g + from + 8 * whole + tid, 0.0f);
+        const float zeros[N] = {};
+        for (int32_t i = tid; i < whole; i += kThreads) store_unit<kStream>(g + from + N * i, zeros);
+        if (tid < to - from - N * whole) store1(g + from + N * whole + tid, 0.0f);
         return;
     }
     const float2 st = a.stats[row];
     const float factor = distill ? c * st.y : -c * st.y;
     const T *x = static_cast<const T *>(a.logits.x) + a.logits.offset(row);
-    const auto values = [&](const float (&v)[8], int32_t j, float (&d)[8]) {
+    const auto values = [&](const float (&v)[N], int32_t j, float (&d)[N]) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) d[e] = factor * exp2_of(v[e], st.x, a.k);
-        if (t >= j && t < j + 8) {
+        for (int e = 0; e < N; ++e) d[e] = factor * exp2_of(v[e], st.x, a.k);
+        if (t >= j && t < j + N) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
+            for (int e = 0; e < N; ++e)
                 if (j + e == t) d[e] += c;
         }
     };
+    constexpr int kUnroll = sizeof(T) == 2 ? 4 : 8;  // loads in flight per thread
     int32_t i = tid;
-    for (; i + 3 * kThreads < whole; i += 4 * kThreads) {
-        Raw8<T> raw[4];
+    for (; i + (kUnroll - 1) * kThreads < whole; i += kUnroll * kThreads) {
+        Raw<T> raw[kUnroll];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) load_raw<false>(x + from + 8 * (i + u * kThreads), raw[u]);
+        for (int u = 0; u < kUnroll; ++u) load_raw<kStream>(x + from + N * (i + u * kThreads), raw[u]);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int32_t j = from + 8 * (i + u * kThreads);
-            float v[8], d[8];
+        for (int u = 0; u < kUnroll; ++u) {
+            const int32_t j = from + N * (i + u * kThreads);
+            float v[N], d[N];
             widen(raw[u], v);
             values(v, j, d);
-            store8(g + j, d);
+            store_unit<kStream>(g + j, d);
         }
     }
     for (; i < whole; i += kThreads) {
-        const int32_t j = from + 8 * i;
-        Raw8<T> raw;
-        load_raw<false>(x + j, raw);
-        float v[8], d[8];
+        const int32_t j = from + N * i;
+        Raw<T> raw;
+        load_raw<kStream>(x + j, raw);
+        float v[N], d[N];
         widen(raw, v);
         values(v, j, d);
-        store8(g + j, d);
+        store_unit<kStream>(g + j, d);
     }
-    if (tid < to - from - 8 * whole) {
-        const int32_t j = from + 8 * whole + tid;
+    if (tid < to - from - N * whole) {
+        const int32_t j = from + N * whole + tid;
         store1(g + j, factor * exp2_of(load1(x + j), st.x, a.k) + (j == t ? c : 0.0f));
     }
     if (distill) {  // the teacher's tokens of this part, over what the sweep has stored there
@@ -622,6 +626,15 @@ void launch_stats(StatsArgs a, int dtype, bool left_out, hipStream_t s) {
     }
 }
 
+// Logits and gradient go past the caches where every unit of both is 16-byte aligned and they are too large for the
+// last-level cache of 256 MB. (Unaligned units share cache lines, which the caches put together.)
+bool streams(const Logits &l, const void *grad, int dtype) {
+    const int64_t size = static_cast<int64_t>(dtype_size(dtype)), unit = 16 / size;
+    const bool aligned = reinterpret_cast<uint64_t>(l.x) % 16 == 0 && reinterpret_cast<uint64_t>(grad) % 16 == 0 &&
+                         l.vocab % unit == 0 && l.row_stride % unit == 0 && l.batch_stride % unit == 0;
+    return aligned && l.n * l.vocab * size > int64_t{256} << 20;
+}
+
 template <Op kOp>
 void launch_rows(const RowArgs &a, int dtype, hipStream_t s) {
     const unsigned blocks = static_cast<unsigned>(row_blocks(kOp, a.logits.n));
@@ -633,16 +646,22 @@ void launch_rows(const RowArgs &a, int dtype, hipStream_t s) {
         total_kernel<<<1, 1024, 0, s>>>(a.sums, blocks, a.weights.counted, a.scale, a.loss, a.out_stats);
 }
 
-void launch_grad(const GradArgs &a, int dtype, hipStream_t s) {
+template <typename T, int kThreads>
+void launch_grad_of(const GradArgs &a, bool stream_out, hipStream_t s) {
     const unsigned blocks = static_cast<unsigned>(a.logits.n * a.splits);
-    if (blocks == 0) return;
-    const bool small = a.logits.vocab <= 2048;
+    if (stream_out) grad_kernel<T, kThreads, true><<<blocks, kThreads, 0, s>>>(a);
+    else grad_kernel<T, kThreads, false><<<blocks, kThreads, 0, s>>>(a);
+}
+
+void launch_grad(const GradArgs &a, int dtype, hipStream_t s) {
+    if (a.logits.n == 0) return;
+    const bool small = a.logits.vocab <= 2048, out = streams(a.logits, a.grad, dtype);
     if (dtype == ME_BF16) {
-        if (small) grad_kernel<uint16_t, 64><<<blocks, 64, 0, s>>>(a);
-        else grad_kernel<uint16_t, 256><<<blocks, 256, 0, s>>>(a);
+        if (small) launch_grad_of<uint16_t, 64>(a, out, s);
+        else launch_grad_of<uint16_t, 256>(a, out, s);
     } else {
-        if (small) grad_kernel<float, 64><<<blocks, 64, 0, s>>>(a);
-        else grad_kernel<float, 256><<<blocks, 256, 0, s>>>(a);
+        if (small) launch_grad_of<float, 64>(a, out, s);
+        else launch_grad_of<float, 256>(a, out, s);
     }
 }
 
@@ -873,7 +892,7 @@ extern "C" int me_policy(const void *logits, int dtype, int64_t n, int64_t vocab
     r.splits = sp.splits;
     r.adv_per_seq = adv_per_seq;
     if (pass) {
-        launch_row_pass(kPolicy, r, dtype, grad, s);
+        launch_row_pass(kPolicy, r, dtype, grad, streams(l, grad, dtype), s);
         total_kernel<<<1, 1024, 0, s>>>(w.sums, n, w.counted, r.scale, loss, out_stats);
         return check_launch(what);
     }
@@ -967,7 +986,7 @@ extern "C" int me_distill(const void *logits, int dtype, int64_t n, int64_t voca
         const size_t lds = size_t{4} * kEntryBytes * top;
         if (dtype == ME_BF16) entries_kernel<true><<<blocks, 256, lds, s>>>(r);
         else entries_kernel<false><<<blocks, 256, lds, s>>>(r);
-        launch_row_pass(kDistill, r, dtype, grad, s);
+        launch_row_pass(kDistill, r, dtype, grad, streams(l, grad, dtype), s);
         total_kernel<<<1, 1024, 0, s>>>(w.sums, n, nullptr, r.scale, loss, nullptr);
         return check_launch(what);
     }
