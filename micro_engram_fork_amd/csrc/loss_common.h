@@ -386,12 +386,16 @@ struct Entries {
 
 constexpr int kEntryBytes = 16;
 
+// Each array has room for a multiple of 4 entries, so that the ids can be read four at a time.
+__host__ __device__ __forceinline__ int32_t entry_room(int32_t top) { return (top + 3) / 4 * 4; }
+
 __device__ __forceinline__ Entries entries_at(void *lds, int32_t top) {
+    const int32_t room = entry_room(top);
     Entries e;
     e.id = static_cast<int32_t *>(lds);
-    e.x = reinterpret_cast<float *>(e.id + top);
-    e.p = e.x + top;
-    e.raw = e.p + top;
+    e.x = reinterpret_cast<float *>(e.id + room);
+    e.p = e.x + room;
+    e.raw = e.p + room;
     return e;
 }
 
@@ -424,15 +428,22 @@ static __device__ void distill_entries(const RowArgs &a, int64_t r, int64_t off,
         sum += w;
     }
     const float norm = rest ? 1.0f : wave_sum(sum);
+    if (lane < entry_room(a.top) - a.top) e.id[a.top + lane] = -1;
     wave_lds_order();
     for (int32_t i = lane; i < a.top; i += 64) {
         const int32_t id = e.id[i];
-        float p = 0.0f;
+        float p = e.raw[i];
         bool first = true;
-        for (int32_t j = 0; j < a.top; ++j) {
-            if (e.id[j] == id) {
-                p += e.raw[j];
-                first = first && j >= i;
+        if (id >= 0) {
+            for (int32_t j0 = 0; j0 < a.top; j0 += 4) {  // entries of the same token, which there hardly ever are
+                const int4 four = *reinterpret_cast<const int4 *>(e.id + j0);
+                if (four.x == id || four.y == id || four.z == id || four.w == id) {
+                    for (int32_t j = j0; j < j0 + 4; ++j) {
+                        if (j == i || e.id[j] != id) continue;
+                        p += e.raw[j];
+                        first = first && j > i;
+                    }
+                }
             }
         }
         p = id >= 0 ? p / norm : 0.0f;
@@ -495,6 +506,6 @@ static __device__ float distill_finish(const RowArgs &a, int64_t r, MaxSum seen,
 }  // namespace loss
 
 // loss_rows.hip: whether rows of this size and number take its one-read kernels, and their launch (stream_rows: past the caches)
-bool takes_row_pass(int64_t n, int64_t vocab, int dtype, int64_t top);
+bool takes_row_pass(int64_t n, int64_t vocab, int dtype, int64_t top, bool with_grad);
 void launch_row_pass(loss::Op op, const loss::RowArgs &a, int dtype, void *grad, bool stream_rows, hipStream_t s);
 }  // namespace me

@@ -13,7 +13,7 @@ using namespace loss;
 
 namespace {
 
-constexpr int64_t kPassRows = 128;  // rows from which
+constexpr int64_t kForwardUnits = 4096;
 constexpr int kPassTop = 512;  // teacher entries the kernels' LDS has room for
 
 // The logit at an index that all threads share.
@@ -25,25 +25,31 @@ __device__ __forceinline__ float scalar_logit(const float *x, int32_t j) { retur
 template <typename T, int kThreads, int kRegs, int kLds, bool kStream, Op kOp, bool kRest>
 __global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *grad) {
     constexpr int N = kVec<T>;
-    constexpr bool kDist = kOp == kDistill;
+    constexpr bool kDist = kOp == kDistill, kWeighted = kOp >= kPolicy;
     constexpr int kWaves = kThreads / 64;
     constexpr bool kKeepExp = sizeof(T) == 4;  // fp32 slots take the exponentials in place: the gradient needs no second one
     __shared__ Raw<T> held[kLds > 0 ? kLds : 1][kThreads];
     __shared__ __attribute__((aligned(16))) uint8_t entry_space[kDist ? kPassTop * kEntryBytes : 16];
+    constexpr bool kBits = kRest && kLds == 0;
+    __shared__ uint32_t left_out[kBits ? (kThreads * kRegs * N + 8 + 31) / 32 : 1];
     __shared__ float sums[kWaves];
     const int64_t r = blockIdx.x;
     const int32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int32_t vocab = a.logits.vocab, whole = vocab / N, slots = (whole + kThreads - 1) / kThreads, rest = vocab - N * whole;
     T *g = static_cast<T *>(grad) + r * vocab;
-    if (constant(a.weights.weight + r) == 0.0f) {
-        const float zeros[N] = {};
-        for (int32_t i = tid; i < whole; i += kThreads) store_unit<kStream>(g + N * i, zeros);
-        if (tid < rest) store1(g + N * whole + tid, 0.0f);
+    if (kWeighted ? constant(a.weights.weight + r) == 0.0f : a.tokens.token(r, vocab) < 0) {
+        if (grad != nullptr) {
+            const float zeros[N] = {};
+            for (int32_t i = tid; i < whole; i += kThreads) store_unit<kStream>(g + N * i, zeros);
+            if (tid < rest) store1(g + N * whole + tid, 0.0f);
+        }
         if (tid == 0) {
-            a.stats[r] = {0.0f, 0.0f};
-            a.coef[r] = 0.0f;
-            if constexpr (!kDist) a.logps[r] = 0.0f;
-            for (int c = 0; c < 3; ++c) a.sums[3 * r + c] = 0;
+            if (a.stats != nullptr) a.stats[r] = {0.0f, 0.0f};
+            if (a.coef != nullptr) a.coef[r] = 0.0f;
+            if (a.logps != nullptr) a.logps[r] = 0.0f;
+            if (a.gap != nullptr) a.gap[r] = 0.0f;
+            if constexpr (kWeighted)
+                for (int c = 0; c < 3; ++c) a.sums[3 * r + c] = 0;
         }
         if constexpr (kDist)
             for (int32_t i = tid; i < a.top; i += kThreads) a.fix[r * a.top + i] = 0.0f;
@@ -61,6 +67,7 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *g
     if constexpr (kDist) {
 #pragma unroll
         for (int u = 0; u < kPer; ++u) {
+            if (u > 0 && u * kThreads >= a.top) break;
             const int32_t i = min(tid + u * kThreads, a.top - 1);
             entry_id[u] = *as_global(a.entry_id + r * a.top + i);
             entry_p[u] = *as_global(a.fix + r * a.top + i);
@@ -76,7 +83,7 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *g
 #pragma unroll
     for (int c = 0; c < kRegs; ++c) load_slot(c, q[c]);
 
-    const float weight = row_weight(a.weights, r);
+    const float weight = kWeighted ? row_weight(a.weights, r) : 1.0f;
     int32_t t = -1;
     float xt;
     Sampled sampled = {};
@@ -85,11 +92,19 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *g
     } else {
         t = a.tokens.token(r, vocab);
         xt = scalar_logit(x, t);
-        sampled = sampled_row(a, r);
+        if constexpr (kOp == kPolicy) sampled = sampled_row(a, r);
+        else if constexpr (kOp == kPreference) sampled.ref_logp = constant(a.ref_logps + r);
     }
     const Guess guess = guess_of(xt, a.k);
 
-    uint64_t marks = 0;  // slots of this wavefront that hold an entry's token
+    // Where entries are to be left out of the sum: a bit for each token, or where the LDS is taken by logits, a mark for each
+    // slot of a wavefront that holds one (few do: such rows are long).
+    uint64_t marks = 0;
+    if constexpr (kBits) {
+        for (int32_t i = tid; i < (vocab + 31) / 32; i += kThreads) left_out[i] = 0;
+        if constexpr (kWaves > 1) __syncthreads();
+        else wave_lds_order();
+    }
     if constexpr (kDist) {
 #pragma unroll
         for (int u = 0; u < kPer; ++u) {
@@ -98,13 +113,17 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *g
                 e.id[i] = entry_id[u];
                 e.p[i] = entry_p[u];
                 e.x[i] = entry_x[u];
+                if constexpr (kBits)
+                    if (entry_id[u] >= 0) atomicOr(&left_out[entry_id[u] >> 5], 1u << (entry_id[u] & 31));
             }
         }
         if constexpr (kWaves > 1) __syncthreads();
         else wave_lds_order();
+    }
+    if constexpr (kRest && !kBits) {
         for (int32_t i0 = 0; i0 < a.top; i0 += 64) {
             const int32_t i = i0 + lane, c = i < a.top ? e.id[i] / N : -1, s = c / kThreads;
-            uint64_t hits = __ballot(c >= 0 && c < whole && (c % kThreads) >> 6 == wave);
+            uint64_t hits = __ballot(i < a.top && e.id[i] >= 0 && c < whole && (c % kThreads) >> 6 == wave);
             while (hits != 0) {
                 const int src = __builtin_ctzll(hits);
                 hits &= hits - 1;
@@ -113,23 +132,28 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *g
         }
     }
     float tail = tid < rest ? last : -kInf;
-    // v at the entries' tokens in slot s of this wavefront becomes coef times their `value`, or minus infinity
-    float coef = 0.0f;
-    const auto at_entries = [&](int32_t s, float (&v)[N], const float *value) {
-        const int32_t first = s * kThreads + wave * 64;
-        for (int32_t i0 = 0; i0 < a.top; i0 += 64) {
-            const int32_t i = i0 + lane, id = i < a.top ? e.id[i] : -1;
-            const int32_t rel = (id / N) - first;
-            const float mine = value != nullptr && i < a.top ? coef * value[i] : -kInf;
-            uint64_t hits = __ballot(id >= 0 && rel >= 0 && rel < 64);
-            while (hits != 0) {
-                const int src = __builtin_ctzll(hits);
-                hits &= hits - 1;
-                const int32_t token = __builtin_amdgcn_readlane(id, src);
-                const float val = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(mine), src));
+    const auto leave_out = [&](int32_t s, float (&v)[N]) {
+        if constexpr (kBits) {
+            const int32_t j = N * min(s * kThreads + tid, whole - 1);
+            const uint32_t bits = left_out[j >> 5] >> (j & 31);
+            if (__any((bits & ((1u << N) - 1)) != 0)) {
 #pragma unroll
                 for (int w = 0; w < N; ++w)
-                    if (lane == (token / N) - first && w == (token % N)) v[w] = val;
+                    if (bits >> w & 1) v[w] = -kInf;
+            }
+        } else if (marks >> s & 1) {
+            const int32_t first = s * kThreads + wave * 64;
+            for (int32_t i0 = 0; i0 < a.top; i0 += 64) {
+                const int32_t i = i0 + lane, id = i < a.top ? e.id[i] : -1, rel = id / N - first;
+                uint64_t hits = __ballot(id >= 0 && rel >= 0 && rel < 64);
+                while (hits != 0) {
+                    const int src = __builtin_ctzll(hits);
+                    hits &= hits - 1;
+                    const int32_t token = __builtin_amdgcn_readlane(id, src);
+#pragma unroll
+                    for (int w = 0; w < N; ++w)
+                        if (lane == token / N - first && w == token % N) v[w] = -kInf;
+                }
             }
         }
     };
@@ -143,9 +167,7 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *g
 #pragma unroll
             for (int w = 0; w < N; ++w) v[w] = -kInf;
         }
-        if constexpr (kRest) {
-            if (marks >> s & 1) at_entries(s, v, nullptr);
-        }
+        if constexpr (kRest) leave_out(s, v);
 #pragma unroll
         for (int w = 0; w < N; ++w) v[w] = guessed_exp(v[w], guess, a.k);
         if constexpr (kKeepExp) keep_raw(raw, v);
@@ -192,9 +214,12 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *g
             load_tail(x, j, vocab, v);
             if constexpr (kRest) {
                 for (int32_t i = 0; i < a.top; ++i) {
+                    const int32_t w0 = e.id[i] - j;
+                    if (w0 >= 0 && w0 < N) {
 #pragma unroll
-                    for (int w = 0; w < N; ++w)
-                        if (e.id[i] == j + w) v[w] = -kInf;
+                        for (int w = 0; w < N; ++w)
+                            if (w == w0) v[w] = -kInf;
+                    }
                 }
             }
             add_values(row, v, a.k);
@@ -210,7 +235,7 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *g
     }
 
     // ---- the loss and the gradient's factors
-    float factor, ref = row.m;
+    float coef, factor, ref = row.m;
     if constexpr (kDist) {  // every wavefront the same, so that none waits for another
         float2 stats;
         const float loss = distill_finish(a, r, row, e, stats, wave == 0);
@@ -224,35 +249,43 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *g
         }
     } else {
         const float logp = (xt - row.m) * a.inv_temp - logf(row.s), inv_s = 1.0f / row.s;
-        float loss, slope, kl;
-        bool clipped;
-        policy_terms(a, sampled, logp, loss, slope, kl, clipped);
-        coef = a.scale * weight * slope * a.inv_temp;
-        factor = -coef * inv_s;
         if (tid == 0) {
-            a.stats[r] = {row.m, inv_s};
-            a.coef[r] = coef;
-            a.logps[r] = logp;
-            a.sums[3 * r] = static_cast<double>(loss) * weight;
-            a.sums[3 * r + 1] = kl;
-            a.sums[3 * r + 2] = clipped;
+            if (a.stats != nullptr) a.stats[r] = {row.m, inv_s};
+            if (a.logps != nullptr) a.logps[r] = logp;
+        }
+        if constexpr (kOp == kPolicy) {
+            float loss, slope, kl;
+            bool clipped;
+            policy_terms(a, sampled, logp, loss, slope, kl, clipped);
+            coef = a.scale * weight * slope * a.inv_temp;
+            factor = -coef * inv_s;
+            if (tid == 0) {
+                a.coef[r] = coef;
+                a.sums[3 * r] = static_cast<double>(loss) * weight;
+                a.sums[3 * r + 1] = kl;
+                a.sums[3 * r + 2] = clipped;
+            }
+        } else {
+            if constexpr (kOp == kPreference) {
+                if (tid == 0) {
+                    a.gap[r] = logp - sampled.ref_logp;
+                    a.coef[r] = 0.0f;
+                }
+            }
+            return;  // the gradient waits for other rows or for the caller
         }
     }
 
     // ---- gradient
     if (grad == nullptr) return;
+    if (grad == nullptr) return;
     if (!guessed) {
-        for (int32_t j = N * tid; j < vocab; j += N * kThreads) {
-            for (int w = 0; w < N && j + w < vocab; ++w) {
-                float d = factor * exp2_of(load1(x + j + w), ref, a.k);
-                if constexpr (kDist) {
-                    for (int32_t i = 0; i < a.top; ++i)
-                        if (e.id[i] == j + w) d = coef * e.raw[i];
-                } else {
-                    if (j + w == t) d += coef;
-                }
-                store1(g + j + w, d);
-            }
+        for (int32_t j = tid; j < vocab; j += kThreads)
+            store1(g + j, factor * exp2_of(load1(x + j), ref, a.k) + (!kDist && j == t ? coef : 0.0f));
+        if constexpr (kDist) {
+            __syncthreads();
+            for (int32_t i = tid; i < a.top; i += kThreads)
+                if (e.id[i] >= 0) store1(g + e.id[i], coef * e.raw[i]);
         }
         return;
     }
@@ -267,12 +300,12 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *g
             if constexpr (!kKeepExp) d[w] = guessed_exp(d[w], guess, a.k);
             d[w] *= factor;
         }
-        if constexpr (kDist) {
-            if (marks >> s & 1) at_entries(s, d, e.raw);
-        } else if (s == t_slot) {
+        if constexpr (!kDist) {
+            if (s == t_slot) {
 #pragma unroll
-            for (int w = 0; w < N; ++w)
-                if (tid == t_thread && w == (t % N)) d[w] += coef;
+                for (int w = 0; w < N; ++w)
+                    if (tid == t_thread && w == (t % N)) d[w] += coef;
+            }
         }
         const int32_t c = s * kThreads + tid;
         if (c < whole) store_unit<kStream>(g + N * static_cast<int64_t>(c), d);
@@ -300,21 +333,28 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *g
     }
     if (tid < rest) {
         const int32_t j = N * whole + tid;
-        float d = factor * guessed_exp(tail, guess, a.k) + (j == t ? coef : 0.0f);
-        if constexpr (kDist) {
-            for (int32_t i = 0; i < a.top; ++i)
-                if (e.id[i] == j) d = coef * e.raw[i];
-        }
-        store1(g + j, d);
+        store1(g + j, factor * guessed_exp(tail, guess, a.k) + (j == t ? coef : 0.0f));
+    }
+    if constexpr (kDist) {  // the entries over what the sweep has stored there
+        __syncthreads();
+        for (int32_t i = tid; i < a.top; i += kThreads)
+            if (e.id[i] >= 0) store1(g + e.id[i], coef * e.raw[i]);
     }
 }
 
 template <typename T, int kThreads, int kRegs, int kLds, bool kStream = false>
 void launch_pass_of(Op op, const RowArgs &a, void *grad, hipStream_t s) {
     const unsigned n = static_cast<unsigned>(a.logits.n);
+    if constexpr (kThreads < 1024) {  // (kForwardUnits)
+        if (op == kLogps) return pass_kernel<T, kThreads, kRegs, kLds, kStream, kLogps, false><<<n, kThreads, 0, s>>>(a, nullptr);
+        if (op == kPreference)
+            return pass_kernel<T, kThreads, kRegs, kLds, kStream, kPreference, false><<<n, kThreads, 0, s>>>(a, nullptr);
+    }
     if (op == kPolicy) pass_kernel<T, kThreads, kRegs, kLds, kStream, kPolicy, false><<<n, kThreads, 0, s>>>(a, grad);
-    else if (a.teacher_lse != nullptr) pass_kernel<T, kThreads, kRegs, kLds, kStream, kDistill, true><<<n, kThreads, 0, s>>>(a, grad);
-    else pass_kernel<T, kThreads, kRegs, kLds, kStream, kDistill, false><<<n, kThreads, 0, s>>>(a, grad);
+    else if constexpr (kRegs <= 16 || kLds > 0) {  // (registers for the other tokens as a class are there in these only)
+        if (a.teacher_lse != nullptr) pass_kernel<T, kThreads, kRegs, kLds, kStream, kDistill, true><<<n, kThreads, 0, s>>>(a, grad);
+        else pass_kernel<T, kThreads, kRegs, kLds, kStream, kDistill, false><<<n, kThreads, 0, s>>>(a, grad);
+    } else pass_kernel<T, kThreads, kRegs, kLds, kStream, kDistill, false><<<n, kThreads, 0, s>>>(a, grad);
 }
 
 template <typename T>
@@ -323,16 +363,23 @@ void launch_pass(Op op, const RowArgs &a, void *grad, bool stream_rows, hipStrea
     if (units <= 64 * 16) launch_pass_of<T, 64, 16, 0>(op, a, grad, s);
     else if (units <= 256 * 16) launch_pass_of<T, 256, 16, 0>(op, a, grad, s);
     else if (units <= 1024 * 16) launch_pass_of<T, 1024, 16, 0>(op, a, grad, s);
-    else if (units <= 1024 * 22) launch_pass_of<T, 1024, 22, 0>(op, a, grad, s);
+    else if (units <= 1024 * 22 && a.teacher_lse == nullptr) launch_pass_of<T, 1024, 22, 0>(op, a, grad, s);
     else if (stream_rows) launch_pass_of<T, 1024, 22, 9, true>(op, a, grad, s);
     else launch_pass_of<T, 1024, 22, 9>(op, a, grad, s);
 }
 
 }  // namespace
 
-bool takes_row_pass(int64_t n, int64_t vocab, int dtype, int64_t top) {
+// Rows from which one read wins, measured as kernel times (policy / distillation with 64 entries and the rest class, two
+// sweeps over one read): at 32,768 units (262,144 bf16 logits) 64 rows 0.79 / 0.76, 128 rows 1.06 / 0.90, 256 rows 1.19 /
+// 1.11; 8192 units 32 rows 1.01 / 0.95, 64 rows 1.18 / 1.02; 4000 units 16 rows 0.85 / 1.01, 32 rows 1.16; 1000 units 16
+// rows 1.03 / 1.10; 125 units 8 rows 1.08. Without a gradient there is nothing to read twice, and the parts of many
+// workgroups read faster than a CU's one row (8192 rows of 262,144: 500 us against 615); short rows keep their kernel there,
+// for fewer launches.
+bool takes_row_pass(int64_t n, int64_t vocab, int dtype, int64_t top, bool with_grad) {
     if (n == 0 || vocab < 64 || top > kPassTop) return false;
-    return vocab <= (dtype == ME_BF16 ? 327680 : 163840) && n >= kPassRows;
+    const int64_t units = vocab / (dtype == ME_BF16 ? 8 : 4);
+    return units <= (with_grad ? 1024 * 40 : kForwardUnits) && n * 192 >= units;
 }
 
 void launch_row_pass(Op op, const RowArgs &a, int dtype, void *grad, bool stream_rows, hipStream_t s) {

@@ -240,7 +240,7 @@ __global__ __launch_bounds__(kOp == kDistill ? 256 : 1024) void row_kernel(const
         if (lane < a.splits) row = a.part[r * a.splits + lane];
         row = wave_join(row, a.k);
         if constexpr (kOp == kDistill) {
-            const Entries e = entries_at(entry_space + wave * kEntryBytes * a.top, a.top);
+            const Entries e = entries_at(entry_space + wave * kEntryBytes * entry_room(a.top), a.top);
             distill_entries(a, r, off, kBf16, e);
             float2 stats;
             const float loss = distill_finish(a, r, row, e, stats, true);
@@ -302,7 +302,7 @@ __global__ __launch_bounds__(256) void entries_kernel(const RowArgs a) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t r = static_cast<int64_t>(blockIdx.x) * 4 + wave;
     if (r >= a.logits.n || !row_counts(a.weights, r)) return;
-    const Entries e = entries_at(entry_space + wave * kEntryBytes * a.top, a.top);
+    const Entries e = entries_at(entry_space + wave * kEntryBytes * entry_room(a.top), a.top);
     distill_entries(a, r, a.logits.offset(r), kBf16, e);
     float near = -kInf;
     for (int32_t i = lane; i < a.top; i += 64) {
@@ -639,7 +639,7 @@ template <Op kOp>
 void launch_rows(const RowArgs &a, int dtype, hipStream_t s) {
     const unsigned blocks = static_cast<unsigned>(row_blocks(kOp, a.logits.n));
     const int threads = kOp == kDistill ? 256 : 1024;
-    const size_t lds = kOp == kDistill ? size_t{4} * kEntryBytes * a.top : 0;
+    const size_t lds = kOp == kDistill ? size_t{4} * kEntryBytes * entry_room(a.top) : 0;
     if (dtype == ME_BF16) row_kernel<kOp, true><<<blocks, threads, lds, s>>>(a);
     else row_kernel<kOp, false><<<blocks, threads, lds, s>>>(a);
     if (kOp >= kPolicy && blocks > 1)
@@ -710,7 +710,8 @@ extern "C" int me_token_logps(const void *logits, int dtype, int64_t n, int64_t 
     st.k = static_cast<float>(1.4426950408889634 / temperature);
     st.splits = sp.splits;
     st.span = sp.span;
-    launch_stats(st, dtype, false, s);
+    const bool pass = takes_row_pass(n, vocab, dtype, 0, false);
+    if (!pass) launch_stats(st, dtype, false, s);
     RowArgs r = {};
     r.logits = l;
     r.tokens = st.tokens;
@@ -720,7 +721,8 @@ extern "C" int me_token_logps(const void *logits, int dtype, int64_t n, int64_t 
     r.k = st.k;
     r.inv_temp = static_cast<float>(1.0 / temperature);
     r.splits = sp.splits;
-    launch_rows<kLogps>(r, dtype, s);
+    if (pass) launch_row_pass(kLogps, r, dtype, nullptr, false, s);
+    else launch_rows<kLogps>(r, dtype, s);
     return check_launch(what);
 }
 
@@ -786,7 +788,8 @@ extern "C" int me_preference(const void *logits, int dtype, int64_t n, int64_t v
         st.k = kLog2e;
         st.splits = sp.splits;
         st.span = sp.span;
-        launch_stats(st, dtype, false, s);
+        const bool pass = takes_row_pass(n, vocab, dtype, 0, false);
+        if (!pass) launch_stats(st, dtype, false, s);
         RowArgs r = {};
         r.logits = l;
         r.tokens = tokens;
@@ -798,7 +801,8 @@ extern "C" int me_preference(const void *logits, int dtype, int64_t n, int64_t v
         r.k = kLog2e;
         r.inv_temp = 1.0f;
         r.splits = sp.splits;
-        launch_rows<kPreference>(r, dtype, s);
+        if (pass) launch_row_pass(kPreference, r, dtype, nullptr, false, s);
+        else launch_rows<kPreference>(r, dtype, s);
     }
     PairArgs p = {};
     p.tokens = tokens;
@@ -865,7 +869,7 @@ extern "C" int me_policy(const void *logits, int dtype, int64_t n, int64_t vocab
     st.weights.vocab = l.vocab;
     st.weights.use_seqs = seq_offsets != nullptr || reduction == kSequence;
     st.weights.reduction = reduction;
-    const bool pass = grad != nullptr && takes_row_pass(n, vocab, dtype, 0);
+    const bool pass = takes_row_pass(n, vocab, dtype, 0, grad != nullptr);
     if (pass) weights_kernel<<<1, 1024, 0, s>>>(st.weights);
     else launch_stats(st, dtype, false, s);
     RowArgs r = {};
@@ -955,7 +959,7 @@ extern "C" int me_distill(const void *logits, int dtype, int64_t n, int64_t voca
     st.weights.n = n;
     st.weights.vocab = l.vocab;
     st.weights.reduction = reduction;
-    const bool pass = grad != nullptr && takes_row_pass(n, vocab, dtype, top);
+    const bool pass = takes_row_pass(n, vocab, dtype, top, grad != nullptr);
     if (!pass) launch_stats(st, dtype, teacher_lse != nullptr, s);
     RowArgs r = {};
     r.logits = l;
@@ -983,7 +987,7 @@ extern "C" int me_distill(const void *logits, int dtype, int64_t n, int64_t voca
         r.entry_x = w.entry_x;
         r.entry_id = w.entry_id;
         const unsigned blocks = static_cast<unsigned>(ceil_div(n, 4) + 1);
-        const size_t lds = size_t{4} * kEntryBytes * top;
+        const size_t lds = size_t{4} * kEntryBytes * entry_room(r.top);
         if (dtype == ME_BF16) entries_kernel<true><<<blocks, 256, lds, s>>>(r);
         else entries_kernel<false><<<blocks, 256, lds, s>>>(r);
         launch_row_pass(kDistill, r, dtype, grad, streams(l, grad, dtype), s);
