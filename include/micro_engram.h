@@ -535,7 +535,7 @@ int me_mask_media(const void *ids, int ids_dtype, int64_t n, int64_t width, int6
  *               ignore_index or outside [0, vocab) does not count: it is not read, its values
  *               are 0 and its gradient is zeros.
  *   temperature logits are divided by it (1e-6..1e6)
- *   row_stats   [n, 2] fp32, coef [n] fp32: what the gradient needs of each row
+ *   row_stats   [n, 4] fp32 (16-byte aligned), coef [n] fp32: what the gradient needs of each row
  *   grad        [n, vocab] of the logits' dtype, contiguous
  *   upstream    device scalar, the loss's own gradient (NULL: 1). With done_for_one != 0,
  *               grad already holds the gradient for an upstream of 1, and nothing is written

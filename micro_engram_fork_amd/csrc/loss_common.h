@@ -309,7 +309,8 @@ struct RowArgs {
     Seqs seqs;
     const MaxSum *part;    // [n, splits]
     WeightArgs weights;    // policy, distillation
-    float2 *stats;         // [n] (m, 1 / s): what the gradient needs (distillation: (m, a), see distill_row)
+    float4 *stats;         // [n] (m, 1 / s, 1 - q of the token, -): what the gradient needs (distillation: (m, a, -, -), see
+                           // distill_finish)
     float *logps;          // [n] (nullable)
     float *coef;           // [n] (nullable): the gradient's factor of the row
     float *gap;            // [n] preference: log-probability above the reference's
@@ -336,6 +337,24 @@ __device__ __forceinline__ float row_logit(const Logits &l, int64_t off, int32_t
 
 // exp(d) - 1 - d without the cancellation of small d
 __device__ __forceinline__ float exp_excess(float d) { return expm1f(d) - d; }
+
+// A row's token against all others. `others` is the (m, s) of these alone, so that a log-probability near 0 and the 1 - q of
+// the gradient there keep their digits: log(1 + u) for the others' weight u over the token's.
+struct TokenTerms {
+    float logp, rest;  // rest: 1 - q
+    MaxSum all;        // (m, s) of the whole row
+};
+
+__device__ __forceinline__ TokenTerms token_terms(float xt, MaxSum others, float k, float inv_temp) {
+    TokenTerms v;
+    const float d = (others.m - xt) * inv_temp;
+    if (d > 0.0f) v.logp = -(d + logf(others.s + expf(-d)));
+    else v.logp = -log1pf(others.s * expf(d));
+    if (xt == kInf) v.logp = __builtin_nanf("");  // infinity over infinity
+    v.rest = -expm1f(v.logp);
+    v.all = join(others, {xt, 1.0f}, k);
+    return v;
+}
 
 // What the policy loss takes of a row besides its log-probability.
 struct Sampled {
@@ -455,7 +474,7 @@ static __device__ void distill_entries(const RowArgs &a, int64_t r, int64_t off,
 // The loss of row r before its weight, by the wavefront that filled the entries. `seen` are the (m, s) of the row: of all its
 // tokens, or (teacher_lse given) of those that are no entry. Leaves in stats (m, a) such that the gradient at a token that
 // is no entry is  weight T a exp2((x - m) k), and in raw and fix the gradient at the entries over weight T.
-static __device__ float distill_finish(const RowArgs &a, int64_t r, MaxSum seen, const Entries &e, float2 &stats, bool write) {
+static __device__ float distill_finish(const RowArgs &a, int64_t r, MaxSum seen, const Entries &e, float4 &stats, bool write) {
     const int lane = threadIdx.x & 63;
     const bool rest = a.teacher_lse != nullptr;
     MaxSum all = seen;  // the row's (m, s) over all tokens
@@ -482,14 +501,15 @@ static __device__ float distill_finish(const RowArgs &a, int64_t r, MaxSum seen,
         if (write) a.fix[r * a.top + i] = fix;
     }
     loss = wave_sum(loss);
-    stats = {all.m, inv_s};
+    stats = {all.m, inv_s, 0.0f, 0.0f};
     if (rest) {
         mass = wave_sum(mass);
         const float left = mass < 1.0f ? 1.0f - mass : mass == mass ? 0.0f : mass;
         // probability of the other tokens, as a logarithm: it does not vanish where the entries hold nearly all
         const float log_other = seen.m == -kInf ? -kInf : (seen.m - all.m) * a.inv_temp + logf(seen.s) - log_s;
         if (!(left <= 0.0f)) loss += left * (logf(left) - log_other);
-        stats = seen.m == -kInf ? float2{0.0f, 0.0f} : float2{seen.m, (expf(log_other) - left) / seen.s};
+        stats = seen.m == -kInf ? float4{0.0f, 0.0f, 0.0f, 0.0f}
+                                : float4{seen.m, (expf(log_other) - left) / seen.s, 0.0f, 0.0f};
     }
     wave_lds_order();
     return loss * (a.temp * a.temp);

@@ -44,7 +44,7 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *g
             if (tid < rest) store1(g + N * whole + tid, 0.0f);
         }
         if (tid == 0) {
-            if (a.stats != nullptr) a.stats[r] = {0.0f, 0.0f};
+            if (a.stats != nullptr) a.stats[r] = {0.0f, 0.0f, 0.0f, 0.0f};
             if (a.coef != nullptr) a.coef[r] = 0.0f;
             if (a.logps != nullptr) a.logps[r] = 0.0f;
             if (a.gap != nullptr) a.gap[r] = 0.0f;
@@ -96,6 +96,7 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *g
         else if constexpr (kOp == kPreference) sampled.ref_logp = constant(a.ref_logps + r);
     }
     const Guess guess = guess_of(xt, a.k);
+    const int32_t t_slot = kDist || t >= N * whole ? -1 : (t / N) / kThreads, t_thread = kDist ? -1 : (t / N) % kThreads;
 
     // Where entries are to be left out of the sum: a bit for each token, or where the LDS is taken by logits, a mark for each
     // slot of a wavefront that holds one (few do: such rows are long).
@@ -168,6 +169,13 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *g
             for (int w = 0; w < N; ++w) v[w] = -kInf;
         }
         if constexpr (kRest) leave_out(s, v);
+        if constexpr (!kDist) {  // the row's own token is added by token_terms
+            if (s == t_slot) {
+#pragma unroll
+                for (int w = 0; w < N; ++w)
+                    if (tid == t_thread && w == t % N) v[w] = -kInf;
+            }
+        }
 #pragma unroll
         for (int w = 0; w < N; ++w) v[w] = guessed_exp(v[w], guess, a.k);
         if constexpr (kKeepExp) keep_raw(raw, v);
@@ -197,6 +205,7 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *g
             for (int32_t i = 0; i < a.top; ++i)
                 if (e.id[i] == N * whole + tid) tail = -kInf;
     }
+    if (!kDist && N * whole + tid == t) tail = -kInf;
     sum = wave_sum(sum + guessed_exp(tail, guess, a.k));
     if constexpr (kWaves > 1) {
         if (lane == 0) sums[wave] = sum;
@@ -222,6 +231,11 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *g
                     }
                 }
             }
+            if constexpr (!kDist) {
+#pragma unroll
+                for (int w = 0; w < N; ++w)
+                    if (j + w == t) v[w] = -kInf;
+            }
             add_values(row, v, a.k);
         }
         row = wave_join(row, a.k);
@@ -235,9 +249,9 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *g
     }
 
     // ---- the loss and the gradient's factors
-    float coef, factor, ref = row.m;
+    float coef, factor, ref, at_token = 0.0f;
     if constexpr (kDist) {  // every wavefront the same, so that none waits for another
-        float2 stats;
+        float4 stats;
         const float loss = distill_finish(a, r, row, e, stats, wave == 0);
         coef = a.scale * weight * a.temp;
         factor = coef * stats.y;
@@ -248,9 +262,11 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *g
             a.sums[3 * r] = static_cast<double>(loss) * weight;
         }
     } else {
-        const float logp = (xt - row.m) * a.inv_temp - logf(row.s), inv_s = 1.0f / row.s;
+        const TokenTerms token = token_terms(xt, row, a.k, a.inv_temp);
+        const float logp = token.logp, inv_s = 1.0f / token.all.s;
+        ref = token.all.m;
         if (tid == 0) {
-            if (a.stats != nullptr) a.stats[r] = {row.m, inv_s};
+            if (a.stats != nullptr) a.stats[r] = {ref, inv_s, token.rest, 0.0f};
             if (a.logps != nullptr) a.logps[r] = logp;
         }
         if constexpr (kOp == kPolicy) {
@@ -259,6 +275,7 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *g
             policy_terms(a, sampled, logp, loss, slope, kl, clipped);
             coef = a.scale * weight * slope * a.inv_temp;
             factor = -coef * inv_s;
+            at_token = coef * token.rest;
             if (tid == 0) {
                 a.coef[r] = coef;
                 a.sums[3 * r] = static_cast<double>(loss) * weight;
@@ -281,7 +298,7 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *g
     if (grad == nullptr) return;
     if (!guessed) {
         for (int32_t j = tid; j < vocab; j += kThreads)
-            store1(g + j, factor * exp2_of(load1(x + j), ref, a.k) + (!kDist && j == t ? coef : 0.0f));
+            store1(g + j, !kDist && j == t ? at_token : factor * exp2_of(load1(x + j), ref, a.k));
         if constexpr (kDist) {
             __syncthreads();
             for (int32_t i = tid; i < a.top; i += kThreads)
@@ -291,7 +308,6 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *g
     }
     // exponentials are those of `sum`; the rounding of m k that row.s is without goes into the factor
     factor = without_rounding(factor, guess, a.k);
-    const int32_t t_slot = kDist || t >= N * whole ? -1 : (t / N) / kThreads, t_thread = kDist ? -1 : (t / N) % kThreads;
     const auto put_slot = [&](int32_t s, const Raw<T> &raw) {
         float d[N];
         widen(raw, d);
@@ -304,7 +320,7 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *g
             if (s == t_slot) {
 #pragma unroll
                 for (int w = 0; w < N; ++w)
-                    if (tid == t_thread && w == (t % N)) d[w] += coef;
+                    if (tid == t_thread && w == t % N) d[w] = at_token;
             }
         }
         const int32_t c = s * kThreads + tid;
@@ -333,7 +349,7 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *g
     }
     if (tid < rest) {
         const int32_t j = N * whole + tid;
-        store1(g + j, factor * guessed_exp(tail, guess, a.k) + (j == t ? coef : 0.0f));
+        store1(g + j, !kDist && j == t ? at_token : factor * guessed_exp(tail, guess, a.k));
     }
     if constexpr (kDist) {  // the entries over what the sweep has stored there
         __syncthreads();

@@ -108,7 +108,7 @@ struct StatsArgs {
     int ids64;
 };
 
-// (m, s) of one part of a row per workgroup: bound by the bytes of the logits. Four 16-byte loads per thread are in
+// (m, s) of one part of a row, of all tokens but the row's own, per workgroup: bound by the bytes of the logits. Four 16-byte loads per thread are in
 // flight before the first is used. The workgroup past the last part makes the rows' weights meanwhile.
 template <typename T, int kThreads, bool kLeaveOut>
 __global__ __launch_bounds__(kThreads) void stats_kernel(const StatsArgs a) {
@@ -134,8 +134,10 @@ __global__ __launch_bounds__(kThreads) void stats_kernel(const StatsArgs a) {
     }
     const T *x = static_cast<const T *>(a.logits.x) + a.logits.offset(row);
     float near = kInf;  // no guess
+    int32_t t = -1;
     if (a.tokens.targets != nullptr) {
-        near = load1(x + a.tokens.token(row, vocab));
+        t = a.tokens.token(row, vocab);
+        near = load1(x + t);
     } else {
         const int32_t id = teacher_id(a.ids, a.ids64, row * a.top, vocab);
         if (id >= 0) near = load1(x + id);
@@ -150,6 +152,13 @@ __global__ __launch_bounds__(kThreads) void stats_kernel(const StatsArgs a) {
 #pragma unroll
                 for (int e = 0; e < N; ++e)
                     if (bits >> e & 1) v[e] = -kInf;
+            }
+        } else {
+            const uint32_t own = static_cast<uint32_t>(t - j);  // the row's own token is added by token_terms
+            if (own < N) {
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                    if (e == static_cast<int>(own)) v[e] = -kInf;
             }
         }
     };
@@ -229,7 +238,7 @@ __global__ __launch_bounds__(kOp == kDistill ? 256 : 1024) void row_kernel(const
                 if (a.logps != nullptr) a.logps[r] = 0.0f;
                 if (a.coef != nullptr) a.coef[r] = 0.0f;
                 if (a.gap != nullptr) a.gap[r] = 0.0f;
-                if (a.stats != nullptr) a.stats[r] = {0.0f, 0.0f};
+                if (a.stats != nullptr) a.stats[r] = {0.0f, 0.0f, 0.0f, 0.0f};
             }
             if (kOp == kDistill && a.fix != nullptr)
                 for (int32_t i = lane; i < a.top; i += 64) a.fix[r * a.top + i] = 0.0f;
@@ -242,7 +251,7 @@ __global__ __launch_bounds__(kOp == kDistill ? 256 : 1024) void row_kernel(const
         if constexpr (kOp == kDistill) {
             const Entries e = entries_at(entry_space + wave * kEntryBytes * entry_room(a.top), a.top);
             distill_entries(a, r, off, kBf16, e);
-            float2 stats;
+            float4 stats;
             const float loss = distill_finish(a, r, row, e, stats, true);
             if (lane == 0) {
                 a.stats[r] = stats;
@@ -251,8 +260,9 @@ __global__ __launch_bounds__(kOp == kDistill ? 256 : 1024) void row_kernel(const
             }
             wave_lds_order();
         } else if (lane == 0) {
-            const float logp = (row_logit(a.logits, off, t, kBf16) - row.m) * a.inv_temp - logf(row.s);
-            if (a.stats != nullptr) a.stats[r] = {row.m, 1.0f / row.s};
+            const TokenTerms token = token_terms(row_logit(a.logits, off, t, kBf16), row, a.k, a.inv_temp);
+            const float logp = token.logp;
+            if (a.stats != nullptr) a.stats[r] = {token.all.m, 1.0f / token.all.s, token.rest, 0.0f};
             if (a.logps != nullptr) a.logps[r] = logp;
             if constexpr (kOp == kPreference) {
                 a.gap[r] = logp - a.ref_logps[r];
@@ -427,7 +437,7 @@ __global__ __launch_bounds__(1024) void pair_kernel(const PairArgs a) {
 struct GradArgs {
     Logits logits;
     Tokens tokens;          // targets null: distillation
-    const float2 *stats;    // [n] (m, a)
+    const float4 *stats;    // [n]
     const float *coef;      // [n]
     const float *upstream;  // [1] (nullable: 1)
     const void *ids;
@@ -460,8 +470,8 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(const GradArgs a) {
         if (tid < to - from - N * whole) store1(g + from + N * whole + tid, 0.0f);
         return;
     }
-    const float2 st = a.stats[row];
-    const float factor = distill ? c * st.y : -c * st.y;
+    const float4 st = a.stats[row];
+    const float factor = distill ? c * st.y : -c * st.y, at_token = c * st.z;
     const T *x = static_cast<const T *>(a.logits.x) + a.logits.offset(row);
     const auto values = [&](const float (&v)[N], int32_t j, float (&d)[N]) {
 #pragma unroll
@@ -469,7 +479,7 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(const GradArgs a) {
         if (t >= j && t < j + N) {
 #pragma unroll
             for (int e = 0; e < N; ++e)
-                if (j + e == t) d[e] += c;
+                if (j + e == t) d[e] = at_token;
         }
     };
     constexpr int kUnroll = sizeof(T) == 2 ? 4 : 8;  // loads in flight per thread
@@ -498,7 +508,7 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(const GradArgs a) {
     }
     if (tid < to - from - N * whole) {
         const int32_t j = from + N * whole + tid;
-        store1(g + j, factor * exp2_of(load1(x + j), st.x, a.k) + (j == t ? c : 0.0f));
+        store1(g + j, j == t ? at_token : factor * exp2_of(load1(x + j), st.x, a.k));
     }
     if (distill) {  // the teacher's tokens of this part, over what the sweep has stored there
         __builtin_amdgcn_s_waitcnt(0);
@@ -716,7 +726,7 @@ extern "C" int me_token_logps(const void *logits, int dtype, int64_t n, int64_t 
     r.logits = l;
     r.tokens = st.tokens;
     r.part = w.part;
-    r.stats = reinterpret_cast<float2 *>(row_stats);
+    r.stats = reinterpret_cast<float4 *>(row_stats);
     r.logps = logps;
     r.k = st.k;
     r.inv_temp = static_cast<float>(1.0 / temperature);
@@ -743,7 +753,7 @@ extern "C" int me_token_logps_backward(const void *logits, int dtype, int64_t n,
     GradArgs g = {};
     g.logits = l;
     g.tokens = {targets, nullptr, ignore_index, targets_dtype == ME_I64};
-    g.stats = reinterpret_cast<const float2 *>(row_stats);
+    g.stats = reinterpret_cast<const float4 *>(row_stats);
     g.coef = coef;
     g.upstream = upstream;
     g.grad = grad;
@@ -794,7 +804,7 @@ extern "C" int me_preference(const void *logits, int dtype, int64_t n, int64_t v
         r.logits = l;
         r.tokens = tokens;
         r.part = w.part;
-        r.stats = reinterpret_cast<float2 *>(row_stats);
+        r.stats = reinterpret_cast<float4 *>(row_stats);
         r.coef = coef;
         r.gap = w.gap;
         r.ref_logps = ref_logps;
@@ -878,7 +888,7 @@ extern "C" int me_policy(const void *logits, int dtype, int64_t n, int64_t vocab
     r.seqs = seqs;
     r.part = w.part;
     r.weights = st.weights;
-    r.stats = reinterpret_cast<float2 *>(row_stats);
+    r.stats = reinterpret_cast<float4 *>(row_stats);
     r.logps = logps;
     r.coef = coef;
     r.old_logps = old_logps;
@@ -966,7 +976,7 @@ extern "C" int me_distill(const void *logits, int dtype, int64_t n, int64_t voca
     r.tokens = st.tokens;
     r.part = w.part;
     r.weights = st.weights;
-    r.stats = reinterpret_cast<float2 *>(row_stats);
+    r.stats = reinterpret_cast<float4 *>(row_stats);
     r.coef = coef;
     r.ids = teacher_ids;
     r.ids64 = st.ids64;
@@ -1031,7 +1041,7 @@ extern "C" int me_distill_backward(const void *logits, int dtype, int64_t n, int
     const Split sp = split_of(n, vocab);
     GradArgs g = {};
     g.logits = l;
-    g.stats = reinterpret_cast<const float2 *>(row_stats);
+    g.stats = reinterpret_cast<const float4 *>(row_stats);
     g.coef = coef;
     g.upstream = upstream;
     g.ids = teacher_ids;

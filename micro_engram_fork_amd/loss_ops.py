@@ -82,31 +82,31 @@ def _f32(shape, dev):
     return torch.empty(shape, dtype=torch.float32, device=dev)
 
 
-# What a backward needs of n rows is one fp32 buffer: (m, 1 / s) pairs [n, 2], factors [n], and for
+# What a backward needs of n rows is one fp32 buffer: statistics [n, 4], factors [n], and for
 # distillation the values at the teacher's entries [n, top].
 def _saved(n, dev, top=0):
     """(buffer, addresses of its parts)."""
-    saved = _f32(n * (3 + top), dev)
+    saved = _f32(n * (5 + top), dev)
     return saved, *_saved_parts(saved, n)
 
 
 def _saved_parts(saved, n):
     at = saved.data_ptr()
-    return at, at + 8 * n, at + 12 * n
+    return at, at + 16 * n, at + 20 * n
 
 
 # ------------------------------------------------------------------------- log-probabilities
 @_custom_op("token_logps")
 def token_logps(logits: torch.Tensor, targets: torch.Tensor, ignore_index: int, temperature: float,
                 with_stats: bool) -> List[torch.Tensor]:
-    """[log-probabilities fp32 of targets' shape], plus row stats [n, 2] (what the backward needs)
+    """[log-probabilities fp32 of targets' shape], plus row stats [n, 4] (what the backward needs)
     when with_stats."""
     dev = require_gpu(logits, targets)
     logits, rows = row_layout(logits)
     targets, toks = _targets(targets, ignore_index)
     n, vocab = rows[2], rows[3]
     out = _f32(targets.shape, dev)
-    stats = _f32((n, 2), dev) if with_stats else None
+    stats = _f32((n, 4), dev) if with_stats else None
     ws, ptr, size = _workspace(n, vocab, dev)
     call("me_token_logps", *rows, *toks, temperature, out.data_ptr(), _p(stats), ptr, size, stream_of(dev))
     return [out, stats] if with_stats else [out]
@@ -115,7 +115,7 @@ def token_logps(logits: torch.Tensor, targets: torch.Tensor, ignore_index: int, 
 @token_logps.register_fake
 def _(logits, targets, ignore_index, temperature, with_stats):
     out = logits.new_empty(targets.shape, dtype=torch.float32)
-    return [out, logits.new_empty((targets.numel(), 2), dtype=torch.float32)] if with_stats else [out]
+    return [out, logits.new_empty((targets.numel(), 4), dtype=torch.float32)] if with_stats else [out]
 
 
 def _token_logps_backward(logits, targets, stats, coef, upstream, ignore_index, temperature, coef_scale):
@@ -192,7 +192,7 @@ def distill_rescale(grad, logits, teacher_ids, saved, temperature):
 def preference(logits: torch.Tensor, targets: torch.Tensor, ref_logps: torch.Tensor,
                offsets: Optional[torch.Tensor], pairs: int, seq_len: int, kind: int, beta: float,
                smoothing: float, normalized: bool, ignore_index: int) -> List[torch.Tensor]:
-    """[loss, chosen [pairs], rejected [pairs], saved [3 n]], all fp32."""
+    """[loss, chosen [pairs], rejected [pairs], saved [5 n]], all fp32."""
     dev = require_gpu(logits, targets, ref_logps, offsets)
     logits, rows = row_layout(logits)
     targets, toks = _targets(targets, ignore_index)
@@ -210,7 +210,7 @@ def preference(logits: torch.Tensor, targets: torch.Tensor, ref_logps: torch.Ten
 @preference.register_fake
 def _(logits, targets, ref_logps, offsets, pairs, seq_len, kind, beta, smoothing, normalized, ignore_index):
     n, new = targets.numel(), functools.partial(logits.new_empty, dtype=torch.float32)
-    return [new(()), new((pairs,)), new((pairs,)), new((3 * n,))]
+    return [new(()), new((pairs,)), new((pairs,)), new((5 * n,))]
 
 
 # ------------------------------------------------------------------------------------ policy
@@ -219,7 +219,7 @@ def policy(logits: torch.Tensor, targets: torch.Tensor, old_logps: torch.Tensor,
            adv_per_seq: bool, ref_logps: Optional[torch.Tensor], offsets: Optional[torch.Tensor], n_seqs: int,
            seq_len: int, clip_low: float, clip_high: float, kl_coef: float, temperature: float, scale: float,
            reduction: int, ignore_index: int, with_grad: bool) -> List[torch.Tensor]:
-    """[loss, log-probabilities of targets' shape, (mean KL, clipped share), saved [3 n]], all fp32, plus
+    """[loss, log-probabilities of targets' shape, (mean KL, clipped share), saved [5 n]], all fp32, plus
     the logits' gradient for an upstream of 1 when with_grad."""
     dev = require_gpu(logits, targets, old_logps, advantages, ref_logps, offsets)
     logits, rows = row_layout(logits)
@@ -241,7 +241,7 @@ def policy(logits: torch.Tensor, targets: torch.Tensor, old_logps: torch.Tensor,
 def _(logits, targets, old_logps, advantages, adv_per_seq, ref_logps, offsets, n_seqs, seq_len, clip_low,
       clip_high, kl_coef, temperature, scale, reduction, ignore_index, with_grad):
     n, new = targets.numel(), functools.partial(logits.new_empty, dtype=torch.float32)
-    res = [new(()), new(targets.shape), new((2,)), new((3 * n,))]
+    res = [new(()), new(targets.shape), new((2,)), new((5 * n,))]
     return [*res, logits.new_empty(logits.shape)] if with_grad else res
 
 
@@ -250,7 +250,7 @@ def _(logits, targets, old_logps, advantages, adv_per_seq, ref_logps, offsets, n
 def distill(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor,
             teacher_lse: Optional[torch.Tensor], mask: Optional[torch.Tensor], temperature: float, scale: float,
             reduction: int, with_grad: bool) -> List[torch.Tensor]:
-    """[loss, saved [(3 + top) n]], fp32, plus the logits' gradient for an upstream of 1 when with_grad."""
+    """[loss, saved [(5 + top) n]], fp32, plus the logits' gradient for an upstream of 1 when with_grad."""
     dev = require_gpu(logits, teacher_ids, teacher_logits, teacher_lse, mask)
     logits, rows = row_layout(logits)
     n, vocab = rows[2], rows[3]
@@ -270,7 +270,7 @@ def distill(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: tor
 def _(logits, teacher_ids, teacher_logits, teacher_lse, mask, temperature, scale, reduction, with_grad):
     top = teacher_ids.shape[-1]
     n, new = teacher_ids.numel() // top, functools.partial(logits.new_empty, dtype=torch.float32)
-    res = [new(()), new((n * (3 + top),))]
+    res = [new(()), new((n * (5 + top),))]
     return [*res, logits.new_empty(logits.shape)] if with_grad else res
 
 

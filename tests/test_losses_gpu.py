@@ -570,3 +570,30 @@ def test_compiled_losses_equal_eager_ones():
         ga, = torch.autograd.grad(want, a)
         gb, = torch.autograd.grad(got, b)
         _close(gb, ga.double().cpu(), 2.0 ** -8 * ga.double().abs().cpu() + 1e-12, name)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [40, 32_003, 262_144])
+def test_tokens_that_are_nearly_certain_keep_their_digits(dtype, vocab):
+    # log-probabilities down to -1e-12: relative errors like those of any other, in the gradient too. The others' weight u has
+    # REL; log(1 + u) and 1 - q follow it
+    n = 12
+    x = torch.randn(n, vocab, generator=_gen(1))
+    targets = torch.randint(0, vocab, (n,), generator=_gen(2))
+    x.scatter_(1, targets[:, None], (math.log(vocab) + 2.0 * torch.arange(1, n + 1))[:, None])
+    x = x.to(dtype)
+    leaf = x.double().requires_grad_()
+    others = leaf.scatter(1, targets[:, None], -torch.inf).logsumexp(1)
+    want = -torch.log1p(torch.exp(others - leaf.gather(1, targets[:, None]).squeeze(1)))
+    want_grad, = torch.autograd.grad(want.sum(), leaf)
+    xg = x.to(DEV).requires_grad_()
+    got = losses.token_logps(xg, targets.to(DEV))
+    grad, = torch.autograd.grad(got.sum(), xg)
+    _close(got, want, REL * want.detach().abs(), "logps")
+    _close(grad, want_grad, (REL + HALF_ULP[dtype]) * want_grad.abs(), "grad")
+    old, adv = (want.detach() - 0.1).float().to(DEV), torch.ones(n, device=DEV)
+    loss, logps, _ = losses.policy_loss(xg, targets.to(DEV), old, adv)
+    grad, = torch.autograd.grad(loss, xg)
+    _close(logps, want, REL * want.detach().abs(), "policy logps")
+    ratio = torch.exp(want.detach() - old.double().cpu())
+    _close(grad, -want_grad * ratio[:, None] / n, (2 * REL + HALF_ULP[dtype]) * (want_grad * ratio[:, None] / n).abs(), "policy grad")
