@@ -583,7 +583,8 @@ int me_token_logps_backward(const void *logits, int dtype, int64_t n, int64_t vo
  *   kind  ME_PAIR_SIGMOID: -(1 - smoothing) log sigmoid(beta h) - smoothing log sigmoid(-beta h);
  *         ME_PAIR_IPO: (h - 1 / (2 beta))^2; ME_PAIR_HINGE: max(0, 1 - beta h)
  *   chosen, rejected  [pairs] fp32: beta D
- * Gradient: me_token_logps_backward. No pairs: loss 0.
+ * Gradient: me_token_logps_backward; row_stats and coef both NULL where none is wanted. No
+ * pairs: loss 0.
  */
 int me_preference(const void *logits, int dtype, int64_t n, int64_t vocab, int64_t rows_per_batch,
                   int64_t batch_stride, int64_t row_stride, const void *targets, int targets_dtype,

@@ -286,7 +286,7 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *g
             if constexpr (kOp == kPreference) {
                 if (tid == 0) {
                     a.gap[r] = logp - sampled.ref_logp;
-                    a.coef[r] = 0.0f;
+                    if (a.coef != nullptr) a.coef[r] = 0.0f;
                 }
             }
             return;  // the gradient waits for other rows or for the caller
@@ -361,7 +361,7 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *g
 template <typename T, int kThreads, int kRegs, int kLds, bool kStream = false>
 void launch_pass_of(Op op, const RowArgs &a, void *grad, hipStream_t s) {
     const unsigned n = static_cast<unsigned>(a.logits.n);
-    if constexpr (kThreads < 1024) {  // (kForwardUnits)
+    if constexpr (kThreads <= 256) {  // (kForwardUnits)
         if (op == kLogps) return pass_kernel<T, kThreads, kRegs, kLds, kStream, kLogps, false><<<n, kThreads, 0, s>>>(a, nullptr);
         if (op == kPreference)
             return pass_kernel<T, kThreads, kRegs, kLds, kStream, kPreference, false><<<n, kThreads, 0, s>>>(a, nullptr);
@@ -378,6 +378,7 @@ void launch_pass(Op op, const RowArgs &a, void *grad, bool stream_rows, hipStrea
     const int32_t units = a.logits.vocab / kVec<T>;
     if (units <= 64 * 16) launch_pass_of<T, 64, 16, 0>(op, a, grad, s);
     else if (units <= 256 * 16) launch_pass_of<T, 256, 16, 0>(op, a, grad, s);
+    else if (units <= 512 * 16) launch_pass_of<T, 512, 16, 0>(op, a, grad, s);
     else if (units <= 1024 * 16) launch_pass_of<T, 1024, 16, 0>(op, a, grad, s);
     else if (units <= 1024 * 22 && a.teacher_lse == nullptr) launch_pass_of<T, 1024, 22, 0>(op, a, grad, s);
     else if (stream_rows) launch_pass_of<T, 1024, 22, 9, true>(op, a, grad, s);

@@ -144,9 +144,12 @@ __global__ __launch_bounds__(kThreads) void stats_kernel(const StatsArgs a) {
     }
     const Guess guess = guess_of(near, a.k);
     constexpr int N = kVec<T>;
-    const auto leave_out = [&](float (&v)[N], int32_t j) {
+    // v: the unit of unit number `first` + lane of this part, whose logits the sum leaves out where they are entries' or the
+    // row's own token's (which token_terms adds). Only the wavefront that holds the token looks at single lanes for it.
+    const int32_t lane = tid & 63;
+    const auto leave_out = [&](float (&v)[N], int32_t first) {
         if constexpr (kLeaveOut) {
-            const int32_t at = j - from;
+            const int32_t at = N * (first + lane);
             const uint32_t bits = (left_out[at >> 5] >> (at & 31)) & ((1u << N) - 1);
             if (bits != 0) {
 #pragma unroll
@@ -154,42 +157,44 @@ __global__ __launch_bounds__(kThreads) void stats_kernel(const StatsArgs a) {
                     if (bits >> e & 1) v[e] = -kInf;
             }
         } else {
-            const uint32_t own = static_cast<uint32_t>(t - j);  // the row's own token is added by token_terms
-            if (own < N) {
+            const uint32_t ahead = static_cast<uint32_t>(t - from - N * first);
+            if (ahead < 64 * N) {
 #pragma unroll
                 for (int e = 0; e < N; ++e)
-                    if (e == static_cast<int>(own)) v[e] = -kInf;
+                    if (static_cast<uint32_t>(N * lane + e) == ahead) v[e] = -kInf;
             }
         }
     };
     const int32_t whole = (to - from) / N;  // spans are whole units: only the row's end has a rest
     constexpr int kUnroll = sizeof(T) == 2 ? 4 : 8;  // loads in flight per thread
     const auto sweep = [&](auto take) {
-        int32_t c = tid;
-        for (; c + (kUnroll - 1) * kThreads < whole; c += kUnroll * kThreads) {
+        int32_t first = __builtin_amdgcn_readfirstlane(tid & ~63);  // unit of this wavefront's first lane
+        for (; first + 63 + (kUnroll - 1) * kThreads < whole; first += kUnroll * kThreads) {
             Raw<T> raw[kUnroll];
 #pragma unroll
-            for (int u = 0; u < kUnroll; ++u) load_raw<true>(x + from + N * (c + u * kThreads), raw[u]);
+            for (int u = 0; u < kUnroll; ++u) load_raw<true>(x + from + N * (first + lane + u * kThreads), raw[u]);
 #pragma unroll
             for (int u = 0; u < kUnroll; ++u) {
                 float v[N];
                 widen(raw[u], v);
-                leave_out(v, from + N * (c + u * kThreads));
+                leave_out(v, first + u * kThreads);
                 take(v);
             }
         }
-        for (; c < whole; c += kThreads) {
-            Raw<T> raw;
-            load_raw<true>(x + from + N * c, raw);
-            float v[N];
-            widen(raw, v);
-            leave_out(v, from + N * c);
-            take(v);
+        for (; first < whole; first += kThreads) {
+            if (first + lane < whole) {
+                Raw<T> raw;
+                load_raw<true>(x + from + N * (first + lane), raw);
+                float v[N];
+                widen(raw, v);
+                leave_out(v, first);
+                take(v);
+            }
         }
         if (from + N * whole < to && tid == whole % kThreads) {
             float v[N];
             load_tail(x, from + N * whole, vocab, v);
-            leave_out(v, from + N * whole);
+            leave_out(v, whole - lane);
             take(v);
         }
     };
@@ -266,7 +271,7 @@ __global__ __launch_bounds__(kOp == kDistill ? 256 : 1024) void row_kernel(const
             if (a.logps != nullptr) a.logps[r] = logp;
             if constexpr (kOp == kPreference) {
                 a.gap[r] = logp - a.ref_logps[r];
-                a.coef[r] = 0.0f;
+                if (a.coef != nullptr) a.coef[r] = 0.0f;
             } else if constexpr (kOp == kPolicy) {
                 float loss, slope, kl;
                 bool clipped;
@@ -351,7 +356,7 @@ struct PairArgs {
     Tokens tokens;
     Seqs seqs;             // 2 * pairs sequences: the chosen ones, then the rejected ones
     const float *gap;      // [n]
-    float *coef;           // [n]
+    float *coef;           // [n] (nullable)
     float *chosen, *rejected, *loss;
     double *sums;          // [pairs]
     int64_t pairs;
@@ -364,7 +369,9 @@ struct PairArgs {
 __device__ __forceinline__ float softplus_neg(float x) { return fmaxf(-x, 0.0f) + log1pf(expf(-fabsf(x))); }
 
 // One pair by one wavefront: both sequences' sums, the loss, and the factors of their rows' gradients. Returns the loss.
+// Eight rows per lane are requested at a time: the sums are bound by the loads' latency.
 __device__ double pair_terms(const PairArgs &a, int64_t p) {
+    constexpr int kFlight = 8;
     const int lane = threadIdx.x & 63;
     float d[2];
     int64_t from[2], to[2];
@@ -375,9 +382,21 @@ __device__ double pair_terms(const PairArgs &a, int64_t p) {
         to[side] = a.seqs.begin(s + 1);
         double sum = 0;  // up to thousands of terms of either sign
         int64_t count = 0;
-        for (int64_t r = from[side] + lane; r < to[side]; r += 64) {
-            sum += a.gap[r];
-            if (a.normalized) count += a.tokens.token(r, a.vocab) >= 0;
+        for (int64_t r0 = from[side] + lane; r0 < to[side]; r0 += 64 * kFlight) {
+            float v[kFlight];
+            bool in[kFlight];
+#pragma unroll
+            for (int u = 0; u < kFlight; ++u) {
+                const int64_t r = r0 + 64 * u < to[side] ? r0 + 64 * u : to[side] - 1;
+                v[u] = a.gap[r];
+                in[u] = a.normalized && a.tokens.token(r, a.vocab) >= 0;
+            }
+#pragma unroll
+            for (int u = 0; u < kFlight; ++u) {
+                if (r0 + 64 * u >= to[side]) break;
+                sum += v[u];
+                count += in[u];
+            }
         }
         sum = wave_sum(sum);
         count = wave_sum(count);
@@ -401,10 +420,17 @@ __device__ double pair_terms(const PairArgs &a, int64_t p) {
         slope = x < 1.0f ? -a.beta : 0.0f;
     }
     slope /= static_cast<float>(a.pairs);
-    for (int side = 0; side < 2; ++side) {
+    for (int side = 0; a.coef != nullptr && side < 2; ++side) {
         const float c = (side == 0 ? slope : -slope) * inv_len[side];
-        for (int64_t r = from[side] + lane; r < to[side]; r += 64)
-            if (a.tokens.token(r, a.vocab) >= 0) a.coef[r] = c;
+        for (int64_t r0 = from[side] + lane; r0 < to[side]; r0 += 64 * kFlight) {
+            int32_t t[kFlight];
+#pragma unroll
+            for (int u = 0; u < kFlight; ++u)
+                t[u] = a.tokens.token(r0 + 64 * u < to[side] ? r0 + 64 * u : to[side] - 1, a.vocab);
+#pragma unroll
+            for (int u = 0; u < kFlight; ++u)
+                if (r0 + 64 * u < to[side] && t[u] >= 0) a.coef[r0 + 64 * u] = c;
+        }
     }
     if (lane == 0) {
         a.chosen[p] = a.beta * d[0];
@@ -783,7 +809,7 @@ extern "C" int me_preference(const void *logits, int dtype, int64_t n, int64_t v
     ME_CHECK_ARG(beta > 0 && beta <= 1e6, "%s: beta must be positive", what);
     ME_CHECK_ARG(smoothing >= 0 && smoothing <= 1, "%s: smoothing must be in 0..1", what);
     ME_CHECK_ARG(loss != nullptr && (pairs == 0 || (chosen != nullptr && rejected != nullptr)), "%s: null output", what);
-    ME_CHECK_ARG(n == 0 || (ref_logps != nullptr && coef != nullptr), "%s: null pointer", what);
+    ME_CHECK_ARG(n == 0 || (ref_logps != nullptr && (coef != nullptr) == (row_stats != nullptr)), "%s: null pointer", what);
     const Space w = carve(workspace, n, vocab, pairs);
     ME_TRY(check_space(what, w, workspace, workspace_bytes));
     const hipStream_t s = as_stream(stream);

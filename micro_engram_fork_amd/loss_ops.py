@@ -191,26 +191,29 @@ def distill_rescale(grad, logits, teacher_ids, saved, temperature):
 @_custom_op("preference")
 def preference(logits: torch.Tensor, targets: torch.Tensor, ref_logps: torch.Tensor,
                offsets: Optional[torch.Tensor], pairs: int, seq_len: int, kind: int, beta: float,
-               smoothing: float, normalized: bool, ignore_index: int) -> List[torch.Tensor]:
-    """[loss, chosen [pairs], rejected [pairs], saved [5 n]], all fp32."""
+               smoothing: float, normalized: bool, ignore_index: int, with_saved: bool) -> List[torch.Tensor]:
+    """[loss, chosen [pairs], rejected [pairs]], plus saved [5 n] (what the backward needs) when
+    with_saved, all fp32."""
     dev = require_gpu(logits, targets, ref_logps, offsets)
     logits, rows = row_layout(logits)
     targets, toks = _targets(targets, ignore_index)
     offsets, seqs = _offsets(offsets)
     n, vocab = rows[2], rows[3]
     loss, chosen, rejected = _f32((), dev), _f32((pairs,), dev), _f32((pairs,), dev)
-    saved, stats, coef, _ = _saved(n, dev)
+    saved, stats, coef, _ = _saved(n, dev) if with_saved else (None,) * 4
     ws, ptr, size = _workspace(n, vocab, dev, pairs)
     call("me_preference", *rows, *toks, ref_logps.data_ptr(), *seqs, pairs, seq_len, kind, beta, smoothing,
          int(normalized), loss.data_ptr(), chosen.data_ptr(), rejected.data_ptr(), stats, coef, ptr, size,
          stream_of(dev))
-    return [loss, chosen, rejected, saved]
+    return [loss, chosen, rejected, saved] if with_saved else [loss, chosen, rejected]
 
 
 @preference.register_fake
-def _(logits, targets, ref_logps, offsets, pairs, seq_len, kind, beta, smoothing, normalized, ignore_index):
+def _(logits, targets, ref_logps, offsets, pairs, seq_len, kind, beta, smoothing, normalized, ignore_index,
+      with_saved):
     n, new = targets.numel(), functools.partial(logits.new_empty, dtype=torch.float32)
-    return [new(()), new((pairs,)), new((pairs,)), new((5 * n,))]
+    res = [new(()), new((pairs,)), new((pairs,))]
+    return [*res, new((5 * n,))] if with_saved else res
 
 
 # ------------------------------------------------------------------------------------ policy

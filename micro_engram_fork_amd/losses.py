@@ -148,7 +148,7 @@ def token_logps(logits, targets, temperature=1.0, ignore_index=IGNORE_INDEX):
 class _Preference(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, args):  # one tuple, as in _Policy
-        loss, chosen, rejected, saved = loss_ops.preference(logits.detach(), targets, *args)
+        loss, chosen, rejected, saved = loss_ops.preference(logits.detach(), targets, *args, True)
         ctx.save_for_backward(logits, targets, saved)
         ctx.ignore_index = args[-1]
         ctx.mark_non_differentiable(chosen, rejected)
@@ -195,7 +195,7 @@ def preference_loss(logits, targets, ref_logps, cu_seqlens=None, beta=0.1, loss_
     args = (ref, cu_seqlens, n_seqs // 2, seq_len, kind, beta, smoothing, bool(length_normalized), int(ignore_index))
     if _wants_grad(logits):
         return _Preference.apply(logits, targets, args)
-    return tuple(loss_ops.preference(logits.detach(), targets, *args)[:3])
+    return tuple(loss_ops.preference(logits.detach(), targets, *args, False))
 
 
 # ------------------------------------------------------------------------------------ policy
