@@ -277,8 +277,8 @@ struct WeightArgs {
     Tokens tokens;
     Seqs seqs;         // read where use_seqs: rows of no sequence do not count
     const void *ids;   // teacher ids [n, top] or null: a row without one in the vocabulary does not count
-    float *weight;     // [n]: 0 where a row does not count; else its weight, or 1 where all have that of counted[1]
-    float *counted;    // [2]: how many rows count, the weight of all of these (not with use_seqs); null: nothing is weighted
+    float *weight;     // [n]: 0 where a row does not count; else its share of its sequence (kSequence), or 1
+    float *counted;    // [2]: how many rows count, and the factor on weight; null: nothing is weighted
     int64_t n;
     int32_t vocab, top;
     int ids64, use_seqs, reduction;
@@ -296,8 +296,7 @@ __device__ __forceinline__ bool row_counts(const WeightArgs &a, int64_t r) {
 
 // The weight of row r once make_weights has run: 0 where it does not count.
 __device__ __forceinline__ float row_weight(const WeightArgs &a, int64_t r) {
-    const float w = constant(a.weight + r);
-    return a.use_seqs || w == 0.0f ? w : constant(a.counted + 1);
+    return constant(a.weight + r) * constant(a.counted + 1);
 }
 
 // ------------------------------------------------------------------------------------------ per-row values
@@ -365,7 +364,7 @@ __device__ __forceinline__ Sampled sampled_row(const RowArgs &a, int64_t r) {
     Sampled v;
     v.old_logp = constant(a.old_logps + r);
     v.ref_logp = a.ref_logps != nullptr ? constant(a.ref_logps + r) : 0.0f;
-    v.advantage = constant(a.advantages + (a.adv_per_seq ? a.seqs.of(r) : r));
+    v.advantage = constant(a.advantages + (a.adv_per_seq ? max(a.seqs.of(r), int64_t{0}) : r));
     return v;
 }
 

@@ -66,34 +66,45 @@ __device__ void make_weights(const WeightArgs &a) {
         }
         return;
     }
-    for (int64_t r = tid; r < a.n; r += threads) a.weight[r] = 0.0f;
-    __syncthreads();
+    if (a.seqs.offsets != nullptr) {  // rows of no sequence
+        for (int64_t r = tid; r < a.n; r += threads) a.weight[r] = 0.0f;
+        __syncthreads();
+    }
     int64_t filled = 0;  // sequences with a counting row, seen by each wavefront's first lane
     const int lane = tid & 63, wave = tid >> 6, waves = threads >> 6;
+    constexpr int kFlight = 8;
     for (int64_t s = wave; s < a.seqs.n_seqs; s += waves) {
         const int64_t from = a.seqs.begin(s), to = a.seqs.begin(s + 1);
         int64_t mine = 0;
-        for (int64_t r = from + lane; r < to; r += 64) mine += row_counts(a, r);
+        for (int64_t r0 = from + lane; r0 < to; r0 += 64 * kFlight) {
+            int32_t t[kFlight];
+#pragma unroll
+            for (int u = 0; u < kFlight; ++u) t[u] = a.tokens.token(min(r0 + 64 * u, to - 1), a.vocab);
+#pragma unroll
+            for (int u = 0; u < kFlight; ++u) mine += r0 + 64 * u < to && t[u] >= 0;
+        }
         mine = wave_sum(mine);
         if (lane == 0) {
             filled += mine > 0;
             total += mine;
         }
-        if (a.reduction == kSequence && mine > 0) {
-            for (int64_t r = from + lane; r < to; r += 64)
-                if (row_counts(a, r)) a.weight[r] = 1.0f / static_cast<float>(mine);
-        } else if (mine > 0) {
-            for (int64_t r = from + lane; r < to; r += 64)
-                if (row_counts(a, r)) a.weight[r] = 1.0f;
+        const float w = a.reduction == kSequence && mine > 0 ? 1.0f / static_cast<float>(mine) : 1.0f;
+        for (int64_t r0 = from + lane; r0 < to; r0 += 64 * kFlight) {
+            int32_t t[kFlight];
+#pragma unroll
+            for (int u = 0; u < kFlight; ++u) t[u] = a.tokens.token(min(r0 + 64 * u, to - 1), a.vocab);
+#pragma unroll
+            for (int u = 0; u < kFlight; ++u)
+                if (r0 + 64 * u < to) a.weight[r0 + 64 * u] = t[u] >= 0 ? w : 0.0f;
         }
     }
     const double all = block_sum(static_cast<double>(total), slots);
     const double some = block_sum(static_cast<double>(filled), slots);
-    if (tid == 0) *a.counted = static_cast<float>(all);
-    if (a.reduction == kSum) return;
-    const double by = a.reduction == kSequence ? some : all;
-    const float scale = 1.0f / static_cast<float>(by > 0 ? by : 1);
-    for (int64_t r = tid; r < a.n; r += threads) a.weight[r] *= scale;
+    if (tid == 0) {
+        const double by = a.reduction == kSequence ? some : all;
+        a.counted[0] = static_cast<float>(all);
+        a.counted[1] = a.reduction == kSum ? 1.0f : 1.0f / static_cast<float>(by > 0 ? by : 1);
+    }
 }
 
 // ------------------------------------------------------------------------------------------ statistics of row parts
@@ -477,12 +488,8 @@ struct GradArgs {
 // One part of a row per workgroup: streams the logits once more and writes the gradient; a copy's bytes, and bound
 // by them. Rows whose factor is 0 are filled without being read.
 template <typename T, int kThreads, bool kStream>
-__global__ __launch_bounds__(kThreads) void grad_kernel(const GradArgs a) {
+__device__ __forceinline__ void grad_part(const GradArgs &a, float up, int64_t row, int32_t part) {
     constexpr int N = kVec<T>;
-    const float up = a.upstream != nullptr ? *a.upstream : 1.0f;
-    if (a.done_for_one && up == 1.0f) return;
-    const int64_t row = blockIdx.x / a.splits;
-    const int32_t part = static_cast<int32_t>(blockIdx.x - row * a.splits);
     const int32_t vocab = a.logits.vocab, tid = threadIdx.x;
     const bool distill = a.tokens.targets == nullptr;
     const int32_t t = distill ? -1 : a.tokens.token(row, vocab);
@@ -543,6 +550,17 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(const GradArgs a) {
             const int32_t id = teacher_id(a.ids, a.ids64, row * a.top + e, vocab);
             if (id >= from && id < to) store1(g + id, c * a.fix[row * a.top + e]);
         }
+    }
+}
+
+template <typename T, int kThreads, bool kStream>
+__global__ __launch_bounds__(kThreads) void grad_kernel(const GradArgs a) {
+    const float up = a.upstream != nullptr ? *a.upstream : 1.0f;
+    if (a.done_for_one && up == 1.0f) return;
+    const int64_t parts = a.logits.n * a.splits;
+    for (int64_t p = blockIdx.x; p < parts; p += gridDim.x) {
+        const int64_t row = p / a.splits;
+        grad_part<T, kThreads, kStream>(a, up, row, static_cast<int32_t>(p - row * a.splits));
     }
 }
 
@@ -684,7 +702,10 @@ void launch_rows(const RowArgs &a, int dtype, hipStream_t s) {
 
 template <typename T, int kThreads>
 void launch_grad_of(const GradArgs &a, bool stream_out, hipStream_t s) {
-    const unsigned blocks = static_cast<unsigned>(a.logits.n * a.splits);
+    // a workgroup per part; where most likely nothing is left to do, no more than fill the GPU twice (65,536 workgroups that
+    // end at once take 15 us, 4096 take 3)
+    const int64_t parts = a.logits.n * a.splits;
+    const unsigned blocks = static_cast<unsigned>(a.done_for_one && parts > 4096 ? 4096 : parts);
     if (stream_out) grad_kernel<T, kThreads, true><<<blocks, kThreads, 0, s>>>(a);
     else grad_kernel<T, kThreads, false><<<blocks, kThreads, 0, s>>>(a);
 }
