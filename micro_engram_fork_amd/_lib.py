@@ -126,10 +126,9 @@ def load():
 
 def call(name, *args):
     """Calls entry point `name`; raises EngramLibError with the library's message on failure."""
-    lib = load()
-    status = getattr(lib, name)(*args)
+    status = getattr(_lib or load(), name)(*args)
     if status != 0:
-        msg = lib.me_last_error().decode(errors="replace")
+        msg = _lib.me_last_error().decode(errors="replace")
         raise EngramLibError(f"[micro_engram] {name} failed ({status}): {msg}")
 
 

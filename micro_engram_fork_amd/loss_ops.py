@@ -96,11 +96,8 @@ def _saved_parts(saved, n):
 
 
 # ------------------------------------------------------------------------- log-probabilities
-@_custom_op("token_logps")
-def token_logps(logits: torch.Tensor, targets: torch.Tensor, ignore_index: int, temperature: float,
-                with_stats: bool) -> List[torch.Tensor]:
-    """[log-probabilities fp32 of targets' shape], plus row stats [n, 4] (what the backward needs)
-    when with_stats."""
+def run_token_logps(logits, targets, ignore_index, temperature, with_stats):
+    """([log-probabilities, stats or None], arguments of the rows and tokens with the tensors that hold them)."""
     dev = require_gpu(logits, targets)
     logits, rows = row_layout(logits)
     targets, toks = _targets(targets, ignore_index)
@@ -109,7 +106,16 @@ def token_logps(logits: torch.Tensor, targets: torch.Tensor, ignore_index: int, 
     stats = _f32((n, 4), dev) if with_stats else None
     ws, ptr, size = _workspace(n, vocab, dev)
     call("me_token_logps", *rows, *toks, temperature, out.data_ptr(), _p(stats), ptr, size, stream_of(dev))
-    return [out, stats] if with_stats else [out]
+    return [out, stats], ((*rows, *toks), logits, targets)
+
+
+@_custom_op("token_logps")
+def token_logps(logits: torch.Tensor, targets: torch.Tensor, ignore_index: int, temperature: float,
+                with_stats: bool) -> List[torch.Tensor]:
+    """[log-probabilities fp32 of targets' shape], plus row stats [n, 4] (what the backward needs)
+    when with_stats."""
+    res, _ = run_token_logps(logits, targets, ignore_index, temperature, with_stats)
+    return res if with_stats else res[:1]
 
 
 @token_logps.register_fake
@@ -156,44 +162,58 @@ def _(logits, targets, saved, upstream, ignore_index, temperature):
     return logits.new_empty(logits.shape)
 
 
-# A gradient that the forward has written already is right for an upstream of 1. These give what makes
-# it the one for another upstream: a call whose arguments the forward has at hand, so that the backward,
-# which autograd runs in a thread of its own, has little left to do.
-class Rescale:
-    """rescale(upstream): `grad` in place, and only where upstream (fp32, on the device) is not 1: the kernel
-    looks, not the host."""
-    __slots__ = ("name", "args", "grad", "kept")
+# A backward's call, made ready in the forward, which has the arguments at hand: autograd runs the backward in a thread
+# of its own, where everything takes longer. Not for traced calls.
+class Backward:
+    """backward(upstream): the logits' gradient by the entry point `name` with `args` up to its upstream argument.
+    grad: the gradient for an upstream of 1, which the forward has written already; it is made the one for
+    `upstream` in place, and only where that is not 1 (the kernel looks, not the host). None: a new one.
+    kept: tensors behind the addresses in args."""
+    __slots__ = ("name", "args", "like", "grad", "kept")
 
-    def __init__(self, name, args, grad, *kept):
-        self.name, self.args, self.grad, self.kept = name, args, grad, kept
+    def __init__(self, name, args, like, grad, kept):
+        self.name, self.args, self.like, self.grad, self.kept = name, args, like, grad, kept
 
     def __call__(self, upstream):
-        call(self.name, *self.args, upstream.data_ptr(), 1, self.grad.data_ptr(), stream_of(self.grad.device))
-        return self.grad
+        grad, done = self.grad, 1
+        if grad is None:
+            grad, done = torch.empty(self.like.shape, dtype=self.like.dtype, device=self.like.device), 0
+        call(self.name, *self.args, upstream.data_ptr(), done, grad.data_ptr(), stream_of(grad.device))
+        return grad
 
 
-def token_rescale(grad, logits, targets, saved, ignore_index, temperature):
-    logits, rows = row_layout(logits)
-    targets, toks = _targets(targets, ignore_index)
-    stats, coef, _ = _saved_parts(saved, rows[2])
-    return Rescale("me_token_logps_backward", (*rows, *toks, temperature, stats, coef, 1.0), grad, logits, targets,
-                   saved)
+class LogpsBackward:
+    """As Backward, for token_logps, whose upstream is a factor for each row."""
+    __slots__ = ("args", "scale", "like", "kept")
+
+    def __init__(self, held, temperature, stats):
+        args, self.like, targets = held
+        self.args, self.scale, self.kept = (*args, temperature, stats.data_ptr()), 1.0 / temperature, (targets, stats)
+
+    def __call__(self, upstream):
+        grad = torch.empty(self.like.shape, dtype=self.like.dtype, device=self.like.device)
+        call("me_token_logps_backward", *self.args, upstream.data_ptr(), self.scale, None, 0, grad.data_ptr(),
+             stream_of(grad.device))
+        return grad
 
 
-def distill_rescale(grad, logits, teacher_ids, saved, temperature):
-    logits, rows = row_layout(logits)
-    ids = _contiguous(teacher_ids)
-    return Rescale("me_distill_backward", (*rows, ids.data_ptr(), _int_code(ids, "teacher_ids"), ids.shape[-1],
-                                           temperature, *_saved_parts(saved, rows[2])), grad, logits, ids, saved)
+def token_backward(held, temperature, saved, grad=None):
+    """Backward of preference and policy. held: as run_policy gives it."""
+    args, logits, targets = held
+    stats, coef, _ = _saved_parts(saved, args[2])
+    return Backward("me_token_logps_backward", (*args, temperature, stats, coef, 1.0), logits, grad, (targets, saved))
+
+
+def distill_backward_of(held, temperature, saved, grad):
+    args, logits, ids = held
+    return Backward("me_distill_backward", (*args, temperature, *_saved_parts(saved, args[2])), logits, grad,
+                    (ids, saved))
 
 
 # -------------------------------------------------------------------------------- preference
-@_custom_op("preference")
-def preference(logits: torch.Tensor, targets: torch.Tensor, ref_logps: torch.Tensor,
-               offsets: Optional[torch.Tensor], pairs: int, seq_len: int, kind: int, beta: float,
-               smoothing: float, normalized: bool, ignore_index: int, with_saved: bool) -> List[torch.Tensor]:
-    """[loss, chosen [pairs], rejected [pairs]], plus saved [5 n] (what the backward needs) when
-    with_saved, all fp32."""
+def run_preference(logits, targets, ref_logps, offsets, pairs, seq_len, kind, beta, smoothing, normalized,
+                   ignore_index, with_saved):
+    """([loss, chosen, rejected, saved or None], held as of run_token_logps)."""
     dev = require_gpu(logits, targets, ref_logps, offsets)
     logits, rows = row_layout(logits)
     targets, toks = _targets(targets, ignore_index)
@@ -205,7 +225,18 @@ def preference(logits: torch.Tensor, targets: torch.Tensor, ref_logps: torch.Ten
     call("me_preference", *rows, *toks, ref_logps.data_ptr(), *seqs, pairs, seq_len, kind, beta, smoothing,
          int(normalized), loss.data_ptr(), chosen.data_ptr(), rejected.data_ptr(), stats, coef, ptr, size,
          stream_of(dev))
-    return [loss, chosen, rejected, saved] if with_saved else [loss, chosen, rejected]
+    return [loss, chosen, rejected, saved], ((*rows, *toks), logits, targets)
+
+
+@_custom_op("preference")
+def preference(logits: torch.Tensor, targets: torch.Tensor, ref_logps: torch.Tensor,
+               offsets: Optional[torch.Tensor], pairs: int, seq_len: int, kind: int, beta: float,
+               smoothing: float, normalized: bool, ignore_index: int, with_saved: bool) -> List[torch.Tensor]:
+    """[loss, chosen [pairs], rejected [pairs]], plus saved [5 n] (what the backward needs) when
+    with_saved, all fp32."""
+    res, _ = run_preference(logits, targets, ref_logps, offsets, pairs, seq_len, kind, beta, smoothing, normalized,
+                            ignore_index, with_saved)
+    return res if with_saved else res[:3]
 
 
 @preference.register_fake
@@ -217,13 +248,9 @@ def _(logits, targets, ref_logps, offsets, pairs, seq_len, kind, beta, smoothing
 
 
 # ------------------------------------------------------------------------------------ policy
-@_custom_op("policy")
-def policy(logits: torch.Tensor, targets: torch.Tensor, old_logps: torch.Tensor, advantages: torch.Tensor,
-           adv_per_seq: bool, ref_logps: Optional[torch.Tensor], offsets: Optional[torch.Tensor], n_seqs: int,
-           seq_len: int, clip_low: float, clip_high: float, kl_coef: float, temperature: float, scale: float,
-           reduction: int, ignore_index: int, with_grad: bool) -> List[torch.Tensor]:
-    """[loss, log-probabilities of targets' shape, (mean KL, clipped share), saved [5 n]], all fp32, plus
-    the logits' gradient for an upstream of 1 when with_grad."""
+def run_policy(logits, targets, old_logps, advantages, adv_per_seq, ref_logps, offsets, n_seqs, seq_len, clip_low,
+               clip_high, kl_coef, temperature, scale, reduction, ignore_index, with_grad):
+    """([loss, log-probabilities, stats, saved, gradient or None], held as of run_token_logps)."""
     dev = require_gpu(logits, targets, old_logps, advantages, ref_logps, offsets)
     logits, rows = row_layout(logits)
     targets, toks = _targets(targets, ignore_index)
@@ -236,8 +263,19 @@ def policy(logits: torch.Tensor, targets: torch.Tensor, old_logps: torch.Tensor,
     call("me_policy", *rows, *toks, old_logps.data_ptr(), advantages.data_ptr(), int(adv_per_seq), _p(ref_logps),
          *seqs, n_seqs, seq_len, clip_low, clip_high, kl_coef, temperature, scale, reduction, loss.data_ptr(),
          logps.data_ptr(), out_stats.data_ptr(), stats, coef, _p(grad), ptr, size, stream_of(dev))
-    res = [loss, logps, out_stats, saved]
-    return [*res, grad] if with_grad else res
+    return [loss, logps, out_stats, saved, grad], ((*rows, *toks), logits, targets)
+
+
+@_custom_op("policy")
+def policy(logits: torch.Tensor, targets: torch.Tensor, old_logps: torch.Tensor, advantages: torch.Tensor,
+           adv_per_seq: bool, ref_logps: Optional[torch.Tensor], offsets: Optional[torch.Tensor], n_seqs: int,
+           seq_len: int, clip_low: float, clip_high: float, kl_coef: float, temperature: float, scale: float,
+           reduction: int, ignore_index: int, with_grad: bool) -> List[torch.Tensor]:
+    """[loss, log-probabilities of targets' shape, (mean KL, clipped share), saved [5 n]], all fp32, plus
+    the logits' gradient for an upstream of 1 when with_grad."""
+    res, _ = run_policy(logits, targets, old_logps, advantages, adv_per_seq, ref_logps, offsets, n_seqs, seq_len,
+                        clip_low, clip_high, kl_coef, temperature, scale, reduction, ignore_index, with_grad)
+    return res if with_grad else res[:4]
 
 
 @policy.register_fake
@@ -249,11 +287,8 @@ def _(logits, targets, old_logps, advantages, adv_per_seq, ref_logps, offsets, n
 
 
 # ------------------------------------------------------------------------------ distillation
-@_custom_op("distill")
-def distill(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor,
-            teacher_lse: Optional[torch.Tensor], mask: Optional[torch.Tensor], temperature: float, scale: float,
-            reduction: int, with_grad: bool) -> List[torch.Tensor]:
-    """[loss, saved [(5 + top) n]], fp32, plus the logits' gradient for an upstream of 1 when with_grad."""
+def run_distill(logits, teacher_ids, teacher_logits, teacher_lse, mask, temperature, scale, reduction, with_grad):
+    """([loss, saved, gradient or None], held: the arguments of the rows and ids with their tensors)."""
     dev = require_gpu(logits, teacher_ids, teacher_logits, teacher_lse, mask)
     logits, rows = row_layout(logits)
     n, vocab = rows[2], rows[3]
@@ -263,10 +298,20 @@ def distill(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: tor
     saved, stats, coef, fix = _saved(n, dev, top)
     grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev) if with_grad else None
     ws, ptr, size = _workspace(n, vocab, dev, 0, top)
-    call("me_distill", *rows, ids.data_ptr(), _int_code(ids, "teacher_ids"), teacher.data_ptr(),
-         dtype_code(teacher), top, _p(teacher_lse), _p(mask), temperature, scale, reduction, loss.data_ptr(),
-         stats, coef, fix, _p(grad), ptr, size, stream_of(dev))
-    return [loss, saved, grad] if with_grad else [loss, saved]
+    id_args = ids.data_ptr(), _int_code(ids, "teacher_ids")
+    call("me_distill", *rows, *id_args, teacher.data_ptr(), dtype_code(teacher), top, _p(teacher_lse), _p(mask),
+         temperature, scale, reduction, loss.data_ptr(), stats, coef, fix, _p(grad), ptr, size, stream_of(dev))
+    return [loss, saved, grad], ((*rows, *id_args, top), logits, ids)
+
+
+@_custom_op("distill")
+def distill(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor,
+            teacher_lse: Optional[torch.Tensor], mask: Optional[torch.Tensor], temperature: float, scale: float,
+            reduction: int, with_grad: bool) -> List[torch.Tensor]:
+    """[loss, saved [(5 + top) n]], fp32, plus the logits' gradient for an upstream of 1 when with_grad."""
+    res, _ = run_distill(logits, teacher_ids, teacher_logits, teacher_lse, mask, temperature, scale, reduction,
+                         with_grad)
+    return res if with_grad else res[:2]
 
 
 @distill.register_fake

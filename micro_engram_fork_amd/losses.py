@@ -49,7 +49,7 @@ def _check_logits(logits):
 
 def _check_targets(logits, targets):
     _check_logits(logits)
-    if tuple(targets.shape) != tuple(logits.shape[:-1]):
+    if targets.shape != logits.shape[:-1]:
         raise ValueError(f"[micro_engram] targets {tuple(targets.shape)} do not match the logits' rows "
                          f"{tuple(logits.shape[:-1])}")
     if targets.dtype not in (torch.int32, torch.int64):
@@ -57,6 +57,8 @@ def _check_targets(logits, targets):
 
 
 def _check_number(value, what, low=0.0, high=math.inf, open_low=False):
+    if type(value) is float and low < value < high:
+        return value
     value = float(value)
     if not (low < value if open_low else low <= value) or not value <= high or math.isinf(value):
         raise ValueError(f"[micro_engram] {what} of {value} is out of range")
@@ -76,7 +78,7 @@ def _choice(table, value, what):
 
 def _per_row(values, shape, what):
     """fp32 contiguous values of the rows, without their history."""
-    if tuple(values.shape) != tuple(shape):
+    if values.shape != shape:
         raise ValueError(f"[micro_engram] {what} {tuple(values.shape)} do not match the rows {tuple(shape)}")
     if values.dtype is torch.float32 and not values.requires_grad and values.is_contiguous():
         return values
@@ -117,21 +119,29 @@ def _wants_grad(logits):
 
 
 # ------------------------------------------------------------------------- log-probabilities
+# The Functions take everything but their first two tensors as one tuple: apply() costs host time for each argument,
+# and a small batch's training step is bound by the rate at which the host issues it. For plain tensors the
+# backward's call is made ready in the forward (ctx.run, used once: a second backward makes its own).
 class _TokenLogps(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, targets, ignore_index, temperature):
-        logps, stats = loss_ops.token_logps(logits.detach(), targets, ignore_index, temperature, True)
+    def forward(ctx, logits, targets, args):
+        ctx.run = None
+        if loss_ops.is_plain(logits, targets):
+            (logps, stats), held = loss_ops.run_token_logps(logits.detach(), targets, *args, True)
+            ctx.run = loss_ops.LogpsBackward(held, args[1], stats)
+        else:
+            logps, stats = loss_ops.token_logps(logits.detach(), targets, *args, True)
         ctx.save_for_backward(logits, targets, stats)
-        ctx.consts = ignore_index, temperature
+        ctx.consts = args
         return logps
 
     @staticmethod
     @_no_second_derivatives
     def backward(ctx, grad):
-        logits, targets, stats = ctx.saved_tensors
-        ignore_index, temperature = ctx.consts
-        return loss_ops.token_logps_backward(logits.detach(), targets, stats, _upstream(grad), ignore_index,
-                                             temperature), None, None, None
+        logits, targets, stats = ctx.saved_tensors  # looks whether they are still as they were
+        if ctx.run is not None:
+            return ctx.run(_upstream(grad)), None, None
+        return loss_ops.token_logps_backward(logits.detach(), targets, stats, _upstream(grad), *ctx.consts), None, None
 
 
 def token_logps(logits, targets, temperature=1.0, ignore_index=IGNORE_INDEX):
@@ -140,15 +150,20 @@ def token_logps(logits, targets, temperature=1.0, ignore_index=IGNORE_INDEX):
     _check_targets(logits, targets)
     temperature, ignore_index = _check_temperature(temperature), int(ignore_index)
     if _wants_grad(logits):
-        return _TokenLogps.apply(logits, targets, ignore_index, temperature)
+        return _TokenLogps.apply(logits, targets, (ignore_index, temperature))
     return loss_ops.token_logps(logits.detach(), targets, ignore_index, temperature, False)[0]
 
 
 # -------------------------------------------------------------------------------- preference
 class _Preference(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, targets, args):  # one tuple, as in _Policy
-        loss, chosen, rejected, saved = loss_ops.preference(logits.detach(), targets, *args, True)
+    def forward(ctx, logits, targets, args):
+        ctx.run = None
+        if loss_ops.is_plain(logits, targets):
+            (loss, chosen, rejected, saved), held = loss_ops.run_preference(logits.detach(), targets, *args, True)
+            ctx.run = loss_ops.token_backward(held, 1.0, saved)
+        else:
+            loss, chosen, rejected, saved = loss_ops.preference(logits.detach(), targets, *args, True)
         ctx.save_for_backward(logits, targets, saved)
         ctx.ignore_index = args[-1]
         ctx.mark_non_differentiable(chosen, rejected)
@@ -161,8 +176,10 @@ class _Preference(torch.autograd.Function):
         if upstream is None:
             return None, None, None
         logits, targets, saved = ctx.saved_tensors
-        grad = loss_ops.saved_token_backward(logits.detach(), targets, saved, _upstream(upstream), ctx.ignore_index, 1.0)
-        return grad, None, None
+        if ctx.run is not None:
+            return ctx.run(_upstream(upstream)), None, None
+        return loss_ops.saved_token_backward(logits.detach(), targets, saved, _upstream(upstream), ctx.ignore_index,
+                                             1.0), None, None
 
 
 def preference_loss(logits, targets, ref_logps, cu_seqlens=None, beta=0.1, loss_type="sigmoid",
@@ -199,15 +216,16 @@ def preference_loss(logits, targets, ref_logps, cu_seqlens=None, beta=0.1, loss_
 
 
 # ------------------------------------------------------------------------------------ policy
-# These take everything but their first two tensors as one tuple: apply() costs host time for each argument, and a
-# small batch's training step is bound by the rate at which the host issues it.
 class _Policy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, args):
-        early = loss_ops.is_plain(logits, targets)  # traced: the gradient is the backward's, nothing in place
-        loss, logps, out_stats, saved, *grad = loss_ops.policy(logits.detach(), targets, *args, early)
         ctx.consts = args[-1], args[-4]  # ignore_index, temperature
-        ctx.rescale = loss_ops.token_rescale(grad[0], logits.detach(), targets, saved, *ctx.consts) if early else None
+        ctx.run = None
+        if loss_ops.is_plain(logits, targets):
+            (loss, logps, out_stats, saved, grad), held = loss_ops.run_policy(logits.detach(), targets, *args, True)
+            ctx.run = loss_ops.token_backward(held, args[-4], saved, grad)
+        else:  # traced: the gradient is the backward's, nothing is written in place
+            loss, logps, out_stats, saved = loss_ops.policy(logits.detach(), targets, *args, False)
         ctx.save_for_backward(logits, targets, saved)
         ctx.mark_non_differentiable(logps, out_stats)
         ctx.set_materialize_grads(False)
@@ -218,13 +236,11 @@ class _Policy(torch.autograd.Function):
     def backward(ctx, upstream, _logps, _stats):
         if upstream is None:
             return None, None, None
-        logits, targets, saved = ctx.saved_tensors  # looks whether they are still as they were
-        rescale, ctx.rescale = ctx.rescale, None  # the gradient is handed out once: a second backward computes its own
-        if rescale is not None:
-            grad = rescale(_upstream(upstream))
-        else:
-            grad = loss_ops.saved_token_backward(logits.detach(), targets, saved, _upstream(upstream), *ctx.consts)
-        return grad, None, None
+        logits, targets, saved = ctx.saved_tensors
+        run, ctx.run = ctx.run, None  # its gradient is handed out once
+        if run is not None:
+            return run(_upstream(upstream)), None, None
+        return loss_ops.saved_token_backward(logits.detach(), targets, saved, _upstream(upstream), *ctx.consts), None, None
 
 
 def policy_loss(logits, targets, old_logps, advantages, ref_logps=None, cu_seqlens=None, clip_low=0.2,
@@ -254,7 +270,7 @@ def policy_loss(logits, targets, old_logps, advantages, ref_logps=None, cu_seqle
     n_seqs, seq_len = _sequences(targets, cu_seqlens)
     old = _per_row(old_logps, targets.shape, "old_logps")
     ref = None if ref_logps is None else _per_row(ref_logps, targets.shape, "ref_logps")
-    per_seq = tuple(advantages.shape) != tuple(targets.shape)
+    per_seq = advantages.shape != targets.shape
     if per_seq and tuple(advantages.shape) not in ((n_seqs,), (*targets.shape[:-1], 1)):
         raise ValueError(f"[micro_engram] advantages {tuple(advantages.shape)} are neither the rows' "
                          f"{tuple(targets.shape)} nor one for each of {n_seqs} sequences")
@@ -270,11 +286,13 @@ def policy_loss(logits, targets, old_logps, advantages, ref_logps=None, cu_seqle
 class _Distill(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, teacher_ids, args):
-        early = loss_ops.is_plain(logits, teacher_ids)  # as in _Policy
-        loss, saved, *grad = loss_ops.distill(logits.detach(), teacher_ids, *args, early)
         ctx.temperature = args[3]
-        ctx.rescale = (loss_ops.distill_rescale(grad[0], logits.detach(), teacher_ids, saved, ctx.temperature)
-                       if early else None)
+        ctx.run = None
+        if loss_ops.is_plain(logits, teacher_ids):
+            (loss, saved, grad), held = loss_ops.run_distill(logits.detach(), teacher_ids, *args, True)
+            ctx.run = loss_ops.distill_backward_of(held, ctx.temperature, saved, grad)
+        else:
+            loss, saved = loss_ops.distill(logits.detach(), teacher_ids, *args, False)
         ctx.save_for_backward(logits, teacher_ids, saved)
         return loss
 
@@ -282,12 +300,10 @@ class _Distill(torch.autograd.Function):
     @_no_second_derivatives
     def backward(ctx, upstream):
         logits, teacher_ids, saved = ctx.saved_tensors
-        rescale, ctx.rescale = ctx.rescale, None
-        if rescale is not None:
-            grad = rescale(_upstream(upstream))
-        else:
-            grad = loss_ops.distill_backward(logits.detach(), teacher_ids, saved, _upstream(upstream), ctx.temperature)
-        return grad, None, None
+        run, ctx.run = ctx.run, None
+        if run is not None:
+            return run(_upstream(upstream)), None, None
+        return loss_ops.distill_backward(logits.detach(), teacher_ids, saved, _upstream(upstream), ctx.temperature), None, None
 
 
 def distill_loss(logits, teacher_ids, teacher_logits, teacher_lse=None, mask=None, temperature=1.0, scale=1.0,
