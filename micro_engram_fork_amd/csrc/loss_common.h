@@ -22,6 +22,10 @@ template <typename T>
 __device__ __forceinline__ T constant(const T *p) {
     return *reinterpret_cast<const __attribute__((address_space(4))) T *>(reinterpret_cast<uint64_t>(p));
 }
+// element i of an int64 or int32 array
+__device__ __forceinline__ int64_t constant_index(const void *p, int is64, int64_t i) {
+    return is64 ? constant(static_cast<const int64_t *>(p) + i) : constant(static_cast<const int32_t *>(p) + i);
+}
 // 1- and 2-byte values by way of the whole 4 bytes that hold them
 __device__ __forceinline__ uint32_t constant_bytes(const void *p) {
     const uint64_t at = reinterpret_cast<uint64_t>(p);
@@ -50,7 +54,7 @@ struct Tokens {
     int is64;
 
     __device__ __forceinline__ int64_t at(int64_t r) const {
-        return is64 ? constant(static_cast<const int64_t *>(targets) + r) : constant(static_cast<const int32_t *>(targets) + r);
+        return constant_index(targets, is64, r);
     }
     // the row's token, or -1 where the row does not count
     __device__ __forceinline__ int32_t token(int64_t r, int32_t vocab) const {
@@ -72,7 +76,7 @@ struct Seqs {
 
     __device__ __forceinline__ int64_t begin(int64_t s) const {
         if (offsets == nullptr) return s * length;
-        const int64_t v = is64 ? constant(static_cast<const int64_t *>(offsets) + s) : constant(static_cast<const int32_t *>(offsets) + s);
+        const int64_t v = constant_index(offsets, is64, s);
         return v < 0 ? 0 : v > n ? n : v;
     }
     // the sequence that holds row r, -1 if none does
@@ -192,14 +196,15 @@ __device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b, float k) {
 // The usual way to the sum: m is a guess (the logit of the row's own token, or of a teacher's entry, which no other
 // exceeds by more than e^60 in a model that is any good), so nothing is compared or rescaled and each logit takes one
 // multiply-add, one exponential and one addition. What the guess cannot serve shows in the sum (and in m itself), and
-// is then added up again by add_values, whose m is the running maximum: sums over 2^100 or NaN, where a wrong guess would
-// lose digits also those under 2^-60, and guesses so large that m k could overflow.
+// is then added up again by add_values, whose m is the running maximum: sums over 2^100 or NaN, where a wrong guess
+// would lose digits also those under 2^-60, and guesses so large that the rounding of m k (2^-5 at 1e6), which
+// without_rounding takes out, would come near a factor.
 struct Guess {
     float m, mk;
     bool fits;
 };
 
-__device__ __forceinline__ Guess guess_of(float m, float k) { return {m, m * k, fabsf(m) <= 1e30f}; }
+__device__ __forceinline__ Guess guess_of(float m, float k) { return {m, m * k, fabsf(m * k) <= 1e6f}; }
 
 __device__ __forceinline__ float guessed_exp(float x, const Guess &g, float k) {
     return __builtin_amdgcn_exp2f(__builtin_fmaf(x, k, -g.mk));
@@ -266,7 +271,7 @@ __device__ __forceinline__ T block_sum(T v, T *slots) {
 }
 
 __device__ __forceinline__ int32_t teacher_id(const void *ids, int is64, int64_t at, int32_t vocab) {
-    const int64_t v = is64 ? constant(static_cast<const int64_t *>(ids) + at) : constant(static_cast<const int32_t *>(ids) + at);
+    const int64_t v = constant_index(ids, is64, at);
     return v >= 0 && v < vocab ? static_cast<int32_t>(v) : -1;
 }
 
@@ -308,8 +313,8 @@ struct RowArgs {
     Seqs seqs;
     const MaxSum *part;    // [n, splits]
     WeightArgs weights;    // policy, distillation
-    float4 *stats;         // [n] (m, 1 / s, 1 - q of the token, -): what the gradient needs (distillation: (m, a, -, -), see
-                           // distill_finish)
+    float4 *stats;         // [n] what the gradient needs: (m, 1 / s, 1 - q of the token, -), for distillation
+                           // (m, a, -, -) as of distill_finish
     float *logps;          // [n] (nullable)
     float *coef;           // [n] (nullable): the gradient's factor of the row
     float *gap;            // [n] preference: log-probability above the reference's
@@ -317,8 +322,8 @@ struct RowArgs {
     const void *ids, *teacher;
     const float *teacher_lse;
     float *fix;            // [n, top]: the gradient at the teacher's tokens before the row's factor
-    int32_t *entry_id;     // for the one-read kernel: [n, top] the entries' tokens and the logits there, [n] the largest
-    float *entry_x, *near; // of these; the tokens' probabilities are in fix until it writes that
+    int32_t *entry_id;     // for the one-read kernel: [n, top] the entries' tokens and the logits there, [n] the
+    float *entry_x, *near; // largest of these; the tokens' probabilities are in fix until it writes that
     double *sums;          // [gridDim, 3]
     float *loss, *out_stats;
     float k, inv_temp, temp, scale, clip_low, clip_high, kl_coef;
@@ -337,8 +342,8 @@ __device__ __forceinline__ float row_logit(const Logits &l, int64_t off, int32_t
 // exp(d) - 1 - d without the cancellation of small d
 __device__ __forceinline__ float exp_excess(float d) { return expm1f(d) - d; }
 
-// A row's token against all others. `others` is the (m, s) of these alone, so that a log-probability near 0 and the 1 - q of
-// the gradient there keep their digits: log(1 + u) for the others' weight u over the token's.
+// A row's token against all others. `others` is the (m, s) of these alone, so that a log-probability near 0 and the
+// 1 - q of the gradient there keep their digits: log(1 + u) for the others' weight u over the token's.
 struct TokenTerms {
     float logp, rest;  // rest: 1 - q
     MaxSum all;        // (m, s) of the whole row
@@ -393,8 +398,9 @@ __device__ __forceinline__ float teacher_at(const RowArgs &a, int64_t r, int32_t
                            : load1(static_cast<const float *>(a.teacher) + at)) * a.inv_temp;
 }
 
-// A row's teacher entries, in LDS. p: the probability of the entry's token, which adds up the entries of one token; its sign
-// bit is set on all of these but the first, which stands for the token in sums. Ids that are no token are -1, with p = 0.
+// A row's teacher entries, in LDS. p: the probability of the entry's token, which adds up the entries of one token;
+// its sign bit is set on all of these but the first, which stands for the token in sums. Ids that are no token are -1,
+// with p = 0.
 struct Entries {
     int32_t *id;
     float *x;     // the row's logit at the token
@@ -470,10 +476,11 @@ static __device__ void distill_entries(const RowArgs &a, int64_t r, int64_t off,
     wave_lds_order();
 }
 
-// The loss of row r before its weight, by the wavefront that filled the entries. `seen` are the (m, s) of the row: of all its
-// tokens, or (teacher_lse given) of those that are no entry. Leaves in stats (m, a) such that the gradient at a token that
-// is no entry is  weight T a exp2((x - m) k), and in raw and fix the gradient at the entries over weight T.
-static __device__ float distill_finish(const RowArgs &a, int64_t r, MaxSum seen, const Entries &e, float4 &stats, bool write) {
+// The loss of row r before its weight, by a wavefront. `seen` are the (m, s) of the row: of all its tokens, or
+// (teacher_lse given) of those that are no entry. Leaves in stats (m, a) such that the gradient at a token that is no
+// entry is  weight T a exp2((x - m) k), and in raw (and where `write`, fix) the gradient at the entries over weight T.
+static __device__ float distill_finish(const RowArgs &a, int64_t r, MaxSum seen, const Entries &e, float4 &stats,
+                                       bool write) {
     const int lane = threadIdx.x & 63;
     const bool rest = a.teacher_lse != nullptr;
     MaxSum all = seen;  // the row's (m, s) over all tokens
@@ -524,7 +531,8 @@ static __device__ float distill_finish(const RowArgs &a, int64_t r, MaxSum seen,
 
 }  // namespace loss
 
-// loss_rows.hip: whether rows of this size and number take its one-read kernels, and their launch (stream_rows: past the caches)
+// loss_rows.hip: whether rows of this size and number take its one-read kernels, and their launch (stream_rows: past
+// the caches)
 bool takes_row_pass(int64_t n, int64_t vocab, int dtype, int64_t top, bool with_grad);
 void launch_row_pass(loss::Op op, const loss::RowArgs &a, int dtype, void *grad, bool stream_rows, hipStream_t s);
 }  // namespace me

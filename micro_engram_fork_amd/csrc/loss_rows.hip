@@ -2,9 +2,13 @@
 // CU, in registers and for the longest rows in LDS too, between adding up its exponentials and writing its gradient.
 //
 // Bound by HBM: 2 bytes read and 2 written per bf16 logit, where two sweeps (losses.hip) move 6. A CU has 512 KB of
-// registers and 160 KB of LDS: a row of 262,144 bf16 logits is 512 KB, of which 1024 threads hold 22 16-byte slots each in
-// registers (88 of the 128 that 16 wavefronts leave a thread) and 9 in LDS; what is beyond is read a second time. A row's
-// slots are all requested before the first is used, so the whole row is in flight at once.
+// registers and 160 KB of LDS: a row of 262,144 bf16 logits is 512 KB, of which 1024 threads hold 22 16-byte slots each
+// in registers (88 of the 128 that 16 wavefronts leave a thread) and 9 in LDS; what is beyond is read a second time. A
+// row's slots are all requested before the first is used, so the whole row is in flight at once.
+//
+// Measured (policy, all rows counting): 8192 rows of 262,144 bf16 logits 1690-1760 us (4.9-5.1 TB/s: one row per CU,
+// whose read and sum, 28 us, and write follow each other), of 131,072 770 us (5.6), of 32,000 165-195 us (5.4-6.4,
+// several rows per CU), 8192 rows of 50,021 fp32 logits 600 us (5.5).
 #include "loss_common.h"
 
 namespace me {
@@ -27,7 +31,7 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *g
     constexpr int N = kVec<T>;
     constexpr bool kDist = kOp == kDistill, kWeighted = kOp >= kPolicy;
     constexpr int kWaves = kThreads / 64;
-    constexpr bool kKeepExp = sizeof(T) == 4;  // fp32 slots take the exponentials in place: the gradient needs no second one
+    constexpr bool kKeepExp = sizeof(T) == 4;  // fp32 slots take the exponentials in place: none for the gradient
     __shared__ Raw<T> held[kLds > 0 ? kLds : 1][kThreads];
     __shared__ __attribute__((aligned(16))) uint8_t entry_space[kDist ? kPassTop * kEntryBytes : 16];
     constexpr bool kBits = kRest && kLds == 0;
@@ -35,7 +39,8 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *g
     __shared__ float sums[kWaves];
     const int64_t r = blockIdx.x;
     const int32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int32_t vocab = a.logits.vocab, whole = vocab / N, slots = (whole + kThreads - 1) / kThreads, rest = vocab - N * whole;
+    const int32_t vocab = a.logits.vocab, whole = vocab / N, rest = vocab - N * whole;
+    const int32_t slots = (whole + kThreads - 1) / kThreads;
     T *g = static_cast<T *>(grad) + r * vocab;
     if (kWeighted ? constant(a.weights.weight + r) == 0.0f : a.tokens.token(r, vocab) < 0) {
         if (grad != nullptr) {
@@ -57,9 +62,10 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *g
     }
     const T *x = static_cast<const T *>(a.logits.x) + a.logits.offset(r);
 
-    // All loads of the row are issued before the first is used, and none of them under a condition: a slot past the row's
-    // end loads the last unit again. (Loads return in the order of their issue; after one that may or may not have been
-    // issued the compiler can only wait for all.) The entries of a row come before its logits for the same reason.
+    // All loads of the row are issued before the first is used, and none of them under a condition: a slot past the
+    // row's end loads the last unit again. (Loads return in the order of their issue; after one that may or may not
+    // have been issued the compiler can only wait for all.) The entries of a row come before its logits for the same
+    // reason, and its other few values through the scalar cache.
     constexpr int kPer = kDist ? (kPassTop + kThreads - 1) / kThreads : 1;  // entries of a thread
     const Entries e = entries_at(entry_space, a.top);
     int32_t entry_id[kPer];
@@ -96,10 +102,10 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *g
         else if constexpr (kOp == kPreference) sampled.ref_logp = constant(a.ref_logps + r);
     }
     const Guess guess = guess_of(xt, a.k);
-    const int32_t t_slot = kDist || t >= N * whole ? -1 : (t / N) / kThreads, t_thread = kDist ? -1 : (t / N) % kThreads;
+    const int32_t t_slot = kDist || t >= N * whole ? -1 : t / N / kThreads, t_thread = kDist ? -1 : t / N % kThreads;
 
-    // Where entries are to be left out of the sum: a bit for each token, or where the LDS is taken by logits, a mark for each
-    // slot of a wavefront that holds one (few do: such rows are long).
+    // Where entries are to be left out of the sum: a bit for each token, or where the LDS is taken by logits, a mark for
+    // each slot of a wavefront that holds one (few do: such rows are long).
     uint64_t marks = 0;
     if constexpr (kBits) {
         for (int32_t i = tid; i < (vocab + 31) / 32; i += kThreads) left_out[i] = 0;
@@ -362,13 +368,15 @@ template <typename T, int kThreads, int kRegs, int kLds, bool kStream = false>
 void launch_pass_of(Op op, const RowArgs &a, void *grad, hipStream_t s) {
     const unsigned n = static_cast<unsigned>(a.logits.n);
     if constexpr (kThreads <= 256) {  // (kForwardUnits)
-        if (op == kLogps) return pass_kernel<T, kThreads, kRegs, kLds, kStream, kLogps, false><<<n, kThreads, 0, s>>>(a, nullptr);
+        if (op == kLogps)
+            return pass_kernel<T, kThreads, kRegs, kLds, kStream, kLogps, false><<<n, kThreads, 0, s>>>(a, nullptr);
         if (op == kPreference)
             return pass_kernel<T, kThreads, kRegs, kLds, kStream, kPreference, false><<<n, kThreads, 0, s>>>(a, nullptr);
     }
     if (op == kPolicy) pass_kernel<T, kThreads, kRegs, kLds, kStream, kPolicy, false><<<n, kThreads, 0, s>>>(a, grad);
-    else if constexpr (kRegs <= 16 || kLds > 0) {  // (registers for the other tokens as a class are there in these only)
-        if (a.teacher_lse != nullptr) pass_kernel<T, kThreads, kRegs, kLds, kStream, kDistill, true><<<n, kThreads, 0, s>>>(a, grad);
+    else if constexpr (kRegs <= 16 || kLds > 0) {  // (with 22 slots in registers alone, leaving entries out spills)
+        if (a.teacher_lse != nullptr)
+            pass_kernel<T, kThreads, kRegs, kLds, kStream, kDistill, true><<<n, kThreads, 0, s>>>(a, grad);
         else pass_kernel<T, kThreads, kRegs, kLds, kStream, kDistill, false><<<n, kThreads, 0, s>>>(a, grad);
     } else pass_kernel<T, kThreads, kRegs, kLds, kStream, kDistill, false><<<n, kThreads, 0, s>>>(a, grad);
 }
@@ -387,12 +395,12 @@ void launch_pass(Op op, const RowArgs &a, void *grad, bool stream_rows, hipStrea
 
 }  // namespace
 
-// Rows from which one read wins, measured as kernel times (policy / distillation with 64 entries and the rest class, two
-// sweeps over one read): at 32,768 units (262,144 bf16 logits) 64 rows 0.79 / 0.76, 128 rows 1.06 / 0.90, 256 rows 1.19 /
-// 1.11; 8192 units 32 rows 1.01 / 0.95, 64 rows 1.18 / 1.02; 4000 units 16 rows 0.85 / 1.01, 32 rows 1.16; 1000 units 16
-// rows 1.03 / 1.10; 125 units 8 rows 1.08. Without a gradient there is nothing to read twice, and the parts of many
-// workgroups read faster than a CU's one row (8192 rows of 262,144: 500 us against 615); short rows keep their kernel there,
-// for fewer launches.
+// Rows from which one read wins, measured as kernel times (policy / distillation with 64 entries and the rest class,
+// two sweeps over one read): at 32,768 units (262,144 bf16 logits) 64 rows 0.79 / 0.76, 128 rows 1.06 / 0.90, 256 rows
+// 1.19 / 1.11; 8192 units 32 rows 1.01 / 0.95, 64 rows 1.18 / 1.02; 4000 units 16 rows 0.85 / 1.01, 32 rows 1.16; 1000
+// units 16 rows 1.03 / 1.10; 125 units 8 rows 1.08. Without a gradient there is nothing to read twice, and the parts of
+// many workgroups read faster than a CU's one row (8192 rows of 262,144: 500 us against 615); rows of up to 4096 units
+// take one read there too, for its fewer launches (4000 units: 256 rows 20.8 us against 14.6, 8192 rows 103 against 109).
 bool takes_row_pass(int64_t n, int64_t vocab, int dtype, int64_t top, bool with_grad) {
     if (n == 0 || vocab < 64 || top > kPassTop) return false;
     const int64_t units = vocab / (dtype == ME_BF16 ? 8 : 4);

@@ -24,8 +24,10 @@ using namespace loss;
 
 namespace {
 
-// The weight of a row: 1 over the rows that count (kMean), 1 (kSum), or 1 over the row's sequence's counting rows and the
-// sequences that have any (kSequence); 0 for a row that does not count. One workgroup: it runs beside the rows' own ones.
+// The weight of a row: 1 over the rows that count (kMean), 1 (kSum), or 1 over the row's sequence's counting rows
+// and the sequences that have any (kSequence); 0 for a row that does not count. Made by one workgroup, bound by the
+// latency of its loads, hence eight of them in flight per thread: 5.6 us alone for 8192 rows, 7.7 for 3885 by
+// sequences.
 template <typename I>
 __device__ int64_t count_rows(const WeightArgs &a) {
     const bool of_ids = a.ids != nullptr;
@@ -119,8 +121,11 @@ struct StatsArgs {
     int ids64;
 };
 
-// (m, s) of one part of a row, of all tokens but the row's own, per workgroup: bound by the bytes of the logits. Four 16-byte loads per thread are in
-// flight before the first is used. The workgroup past the last part makes the rows' weights meanwhile.
+// (m, s) of one part of a row per workgroup, of all its tokens but the row's own (or but the teacher's entries). Bound
+// by the bytes of the logits: the rows of 8 x 511 with a target, 1.6 GB of bf16 logits, take 231 us, 7.0 TB/s (a device
+// copy of 4 GB moves 4.9, a fill 6.8). For that the loads go past the caches (262 us otherwise), four 16-byte ones per
+// thread are in flight, and a logit costs one multiply-add, one exponential and one addition (Guess). The workgroup
+// past the last part makes the rows' weights meanwhile.
 template <typename T, int kThreads, bool kLeaveOut>
 __global__ __launch_bounds__(kThreads) void stats_kernel(const StatsArgs a) {
     const int64_t parts = a.logits.n * a.splits;
@@ -155,8 +160,9 @@ __global__ __launch_bounds__(kThreads) void stats_kernel(const StatsArgs a) {
     }
     const Guess guess = guess_of(near, a.k);
     constexpr int N = kVec<T>;
-    // v: the unit of unit number `first` + lane of this part, whose logits the sum leaves out where they are entries' or the
-    // row's own token's (which token_terms adds). Only the wavefront that holds the token looks at single lanes for it.
+    // v: unit `first` + lane of this part, whose logits the sum leaves out where they are entries' or the row's own
+    // token's (which token_terms adds). Only the wavefront that holds the token looks at single lanes for it (every
+    // lane at every unit: 380 us instead of 231).
     const int32_t lane = tid & 63;
     const auto leave_out = [&](float (&v)[N], int32_t first) {
         if constexpr (kLeaveOut) {
@@ -239,14 +245,16 @@ __global__ __launch_bounds__(kThreads) void stats_kernel(const StatsArgs a) {
     if (tid == 0) a.part[blockIdx.x] = acc;
 }
 
-// A wavefront per row: joins the parts' (m, s), then the loss's own few values.
+// A wavefront per row: joins the parts' (m, s), then the loss's own few values. A chain of a few dependent loads per
+// row, whatever its length: 2.5 us for one row, 4.7 for 4088, 8.7 for 8286.
 template <Op kOp, bool kBf16>
 __global__ __launch_bounds__(kOp == kDistill ? 256 : 1024) void row_kernel(const RowArgs a) {
     constexpr int kWaves = kOp == kDistill ? 4 : 16;
-    extern __shared__ __attribute__((aligned(16))) uint8_t entry_space[];  // distillation: kEntryBytes * top per wavefront
+    extern __shared__ __attribute__((aligned(16))) uint8_t entry_space[];  // distillation: its entries per wavefront
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kWaves;
     RowSums sums;
-    for (int64_t r = static_cast<int64_t>(blockIdx.x) * kWaves + wave; r < a.logits.n; r += static_cast<int64_t>(gridDim.x) * kWaves) {
+    for (int64_t r = static_cast<int64_t>(blockIdx.x) * kWaves + wave; r < a.logits.n; r += step) {
         const int32_t t = kOp == kDistill ? 0 : a.tokens.token(r, a.logits.vocab);
         const float weight = kOp >= kPolicy ? row_weight(a.weights, r) : 1.0f;
         if (t < 0 || (kOp >= kPolicy && weight == 0.0f)) {
@@ -296,7 +304,8 @@ __global__ __launch_bounds__(kOp == kDistill ? 256 : 1024) void row_kernel(const
     }
     if constexpr (kOp >= kPolicy) {
         __shared__ double slots[kWaves];
-        const double loss = block_sum(sums.loss, slots), kl = block_sum(sums.kl, slots), clipped = block_sum(sums.clipped, slots);
+        const double loss = block_sum(sums.loss, slots), kl = block_sum(sums.kl, slots);
+        const double clipped = block_sum(sums.clipped, slots);
         if (threadIdx.x == 0) {
             if (gridDim.x > 1) {
                 a.sums[3 * blockIdx.x] = loss;
@@ -317,7 +326,9 @@ __global__ __launch_bounds__(kOp == kDistill ? 256 : 1024) void row_kernel(const
 // The weights alone, before a kernel that needs them.
 __global__ __launch_bounds__(1024) void weights_kernel(const WeightArgs a) { make_weights(a); }
 
-// The teacher's entries of every row for the one-read kernel, a wavefront per row; the last workgroup makes the weights.
+// The teacher's entries of every row for the one-read kernel, a wavefront per row; the last workgroup makes the
+// weights. Apart from that kernel because there a row's chain of ids, logits at them and their sums would be waited
+// for by a whole CU (about 17 us of a row's 75 there; all of 4096 rows of 64 entries take 19 us here).
 template <bool kBf16>
 __global__ __launch_bounds__(256) void entries_kernel(const RowArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint8_t entry_space[];
@@ -455,7 +466,8 @@ __global__ __launch_bounds__(1024) void pair_kernel(const PairArgs a) {
     __shared__ double slots[16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
     double sum = 0;
-    for (int64_t p = static_cast<int64_t>(blockIdx.x) * waves + wave; p < a.pairs; p += static_cast<int64_t>(gridDim.x) * waves) {
+    const int64_t step = static_cast<int64_t>(gridDim.x) * waves;
+    for (int64_t p = static_cast<int64_t>(blockIdx.x) * waves + wave; p < a.pairs; p += step) {
         const double loss = pair_terms(a, p);
         if (lane == 0) sum += loss;
     }
@@ -485,8 +497,10 @@ struct GradArgs {
     int ids64, done_for_one;
 };
 
-// One part of a row per workgroup: streams the logits once more and writes the gradient; a copy's bytes, and bound
-// by them. Rows whose factor is 0 are filled without being read.
+// One part of a row: streams the logits once more and writes the gradient. A copy's bytes, and bound by them: 3.5 GB
+// read and 4.3 written (8286 rows of 262,144 bf16 logits, 6640 that count) take 1300 us, 6.0 TB/s, where a device
+// copy of 4 GB moves 4.9 (grad_split_of has what the parts' size does to it). Rows whose factor is 0 are filled without
+// being read.
 template <typename T, int kThreads, bool kStream>
 __device__ __forceinline__ void grad_part(const GradArgs &a, float up, int64_t row, int32_t part) {
     constexpr int N = kVec<T>;
@@ -579,9 +593,9 @@ Split split_of(int64_t n, int64_t vocab) {
     return {static_cast<int32_t>(ceil_div(vocab, span)), static_cast<int32_t>(span)};
 }
 
-// Parts of a row for the gradient, which nothing has to join: 16 KB, so that the workgroups that run at one time read and
-// write within 32 MB (8286 rows of 262,144 bf16 logits: parts of 64 KB 1430 us, 32 KB 1390, 16 KB 1310, 8 KB 1550, where starting
-// the workgroups begins to count).
+// Parts of a row for the gradient, which nothing has to join: 16 KB, so that the workgroups that run at one time read
+// and write within 32 MB (8286 rows of 262,144 bf16 logits: parts of 64 KB 1430 us, 32 KB 1390, 16 KB 1310, 8 KB 1550,
+// where starting the workgroups begins to count; for reading alone the parts' size makes no difference).
 Split grad_split_of(int64_t n, int64_t vocab, int dtype) {
     const int32_t most = dtype == ME_BF16 ? 8192 : 4096;
     Split s = split_of(n, vocab);
@@ -628,26 +642,38 @@ Space carve(void *base, int64_t n, int64_t vocab, int64_t pairs, int64_t top = 0
     return w;
 }
 
+int check_vocab(const char *what, int64_t vocab) {
+    constexpr int64_t kMost = int64_t{kMaxSpan} * kMaxSplits;
+    ME_CHECK_ARG(vocab >= 1 && vocab <= kMost, "%s: vocab must be in 1..%d", what, static_cast<int>(kMost));
+    return ME_OK;
+}
+
 // rows_per_batch past the rows there are makes one batch of them; one that is not positive stays 0 for the check.
-Logits logits_of(const void *x, int64_t n, int64_t rows_per_batch, int64_t batch_stride, int64_t row_stride, int64_t vocab) {
-    const uint32_t per = rows_per_batch < 1 ? 0u : static_cast<uint32_t>(rows_per_batch < INT32_MAX ? rows_per_batch : INT32_MAX);
-    return {x, n, per, batch_stride, row_stride, static_cast<int32_t>(vocab)};
+Logits logits_of(const void *x, int64_t n, int64_t rows_per_batch, int64_t batch_stride, int64_t row_stride,
+                 int64_t vocab) {
+    const int64_t per = rows_per_batch < 1 ? 0 : rows_per_batch < INT32_MAX ? rows_per_batch : INT32_MAX;
+    return {x, n, static_cast<uint32_t>(per), batch_stride, row_stride, static_cast<int32_t>(vocab)};
 }
 
 int check_logits(const char *what, const Logits &l, int dtype) {
     ME_CHECK_ARG(dtype == ME_BF16 || dtype == ME_F32, "%s: logits must be bf16 or fp32", what);
     ME_CHECK_ARG(l.n >= 0 && l.n <= INT32_MAX, "%s: n out of range", what);
-    ME_CHECK_ARG(l.vocab >= 1 && l.vocab <= kMaxSpan * kMaxSplits, "%s: vocab must be in 1..%d", what, kMaxSpan * kMaxSplits);
     ME_CHECK_ARG(l.n == 0 || l.x != nullptr, "%s: logits are null", what);
     ME_CHECK_ARG(l.rows_per_batch >= 1, "%s: rows_per_batch must be positive", what);
     ME_CHECK_ARG(l.row_stride >= 0 && l.batch_stride >= 0, "%s: negative strides", what);
     const Split s = split_of(l.n, l.vocab);
-    ME_CHECK_ARG(l.n * s.splits < INT32_MAX && l.n * grad_split_of(l.n, l.vocab, dtype).splits < INT32_MAX, "%s: too many rows", what);
+    const Split g = grad_split_of(l.n, l.vocab, dtype);
+    ME_CHECK_ARG(l.n * s.splits < INT32_MAX && l.n * g.splits < INT32_MAX, "%s: too many rows", what);
     return ME_OK;
 }
 
 int check_temperature(const char *what, double t) {
     ME_CHECK_ARG(t >= 1e-6 && t <= 1e6, "%s: temperature must be in 1e-6..1e6", what);
+    return ME_OK;
+}
+
+int check_row_stats(const char *what, const float *row_stats) {
+    ME_CHECK_ARG(reinterpret_cast<uint64_t>(row_stats) % 16 == 0, "%s: row_stats must be 16-byte aligned", what);
     return ME_OK;
 }
 
@@ -712,8 +738,8 @@ void launch_rows(const RowArgs &a, int dtype, hipStream_t s) {
 
 template <typename T, int kThreads>
 void launch_grad_of(const GradArgs &a, bool stream_out, hipStream_t s) {
-    // a workgroup per part; where most likely nothing is left to do, no more than fill the GPU twice (65,536 workgroups that
-    // end at once take 15 us, 4096 take 3)
+    // a workgroup per part; where most likely nothing is left to do, no more than fill the GPU twice (65,536 workgroups
+    // that end at once take 15 us, 4096 take 4)
     const int64_t parts = a.logits.n * a.splits;
     const unsigned blocks = static_cast<unsigned>(a.done_for_one && parts > 4096 ? 4096 : parts);
     if (stream_out) grad_kernel<T, kThreads, true><<<blocks, kThreads, 0, s>>>(a);
@@ -733,6 +759,10 @@ void launch_grad(const GradArgs &a, int dtype, hipStream_t s) {
 }
 
 int check_space(const char *what, const Space &w, const void *workspace, size_t bytes) {
+    if (reinterpret_cast<uint64_t>(workspace) % 16 != 0) {
+        set_error("%s: the workspace is not 16-byte aligned", what);
+        return ME_ERR_WORKSPACE;
+    }
     if (workspace == nullptr || bytes < w.bytes) {
         set_error("%s: workspace of %zu bytes, %zu needed", what, workspace == nullptr ? size_t{0} : bytes, w.bytes);
         return ME_ERR_WORKSPACE;
@@ -749,7 +779,7 @@ extern "C" int me_loss_workspace_size(int64_t n, int64_t vocab, int64_t pairs, i
     ME_CHECK_ARG(bytes != nullptr, "me_loss_workspace_size: bytes is null");
     ME_CHECK_ARG(n >= 0 && n <= INT32_MAX && pairs >= 0 && pairs <= INT32_MAX && top >= 0 && top <= kMaxTop,
                  "me_loss_workspace_size: size out of range");
-    ME_CHECK_ARG(vocab >= 1 && vocab <= kMaxSpan * kMaxSplits, "me_loss_workspace_size: vocab must be in 1..%d", kMaxSpan * kMaxSplits);
+    ME_TRY(check_vocab("me_loss_workspace_size", vocab));
     *bytes = carve(nullptr, n, vocab, pairs, top).bytes;
     return ME_OK;
 }
@@ -759,12 +789,13 @@ extern "C" int me_token_logps(const void *logits, int dtype, int64_t n, int64_t 
                               int64_t ignore_index, double temperature, float *logps, float *row_stats,
                               void *workspace, size_t workspace_bytes, void *stream) {
     const char *what = "me_token_logps";
-    ME_CHECK_ARG(vocab >= 1 && vocab <= kMaxSpan * kMaxSplits, "%s: vocab must be in 1..%d", what, kMaxSpan * kMaxSplits);
+    ME_TRY(check_vocab(what, vocab));
     const Logits l = logits_of(logits, n, rows_per_batch, batch_stride, row_stride, vocab);
     ME_TRY(check_logits(what, l, dtype));
     ME_TRY(check_temperature(what, temperature));
     ME_TRY(check_tokens(what, targets, targets_dtype, n));
     ME_CHECK_ARG(n == 0 || logps != nullptr, "%s: logps is null", what);
+    ME_TRY(check_row_stats(what, row_stats));
     if (n == 0) return ME_OK;
     const Space w = carve(workspace, n, vocab, 0);
     ME_TRY(check_space(what, w, workspace, workspace_bytes));
@@ -799,13 +830,14 @@ extern "C" int me_token_logps_backward(const void *logits, int dtype, int64_t n,
                                        const float *coef, double coef_scale, const float *upstream, int done_for_one,
                                        void *grad, void *stream) {
     const char *what = "me_token_logps_backward";
-    ME_CHECK_ARG(vocab >= 1 && vocab <= kMaxSpan * kMaxSplits, "%s: vocab must be in 1..%d", what, kMaxSpan * kMaxSplits);
+    ME_TRY(check_vocab(what, vocab));
     const Logits l = logits_of(logits, n, rows_per_batch, batch_stride, row_stride, vocab);
     ME_TRY(check_logits(what, l, dtype));
     ME_TRY(check_temperature(what, temperature));
     ME_TRY(check_tokens(what, targets, targets_dtype, n));
     ME_CHECK_ARG(n == 0 || (row_stats != nullptr && coef != nullptr && grad != nullptr), "%s: null pointer", what);
     ME_CHECK_ARG(!done_for_one || upstream != nullptr, "%s: done_for_one needs upstream", what);
+    ME_TRY(check_row_stats(what, row_stats));
     const Split sp = grad_split_of(n, vocab, dtype);
     GradArgs g = {};
     g.logits = l;
@@ -830,7 +862,7 @@ extern "C" int me_preference(const void *logits, int dtype, int64_t n, int64_t v
                              float *loss, float *chosen, float *rejected, float *row_stats, float *coef,
                              void *workspace, size_t workspace_bytes, void *stream) {
     const char *what = "me_preference";
-    ME_CHECK_ARG(vocab >= 1 && vocab <= kMaxSpan * kMaxSplits, "%s: vocab must be in 1..%d", what, kMaxSpan * kMaxSplits);
+    ME_TRY(check_vocab(what, vocab));
     const Logits l = logits_of(logits, n, rows_per_batch, batch_stride, row_stride, vocab);
     ME_TRY(check_logits(what, l, dtype));
     ME_TRY(check_tokens(what, targets, targets_dtype, n));
@@ -839,8 +871,10 @@ extern "C" int me_preference(const void *logits, int dtype, int64_t n, int64_t v
     ME_CHECK_ARG(kind >= kSigmoid && kind <= kHinge, "%s: unknown loss kind", what);
     ME_CHECK_ARG(beta > 0 && beta <= 1e6, "%s: beta must be positive", what);
     ME_CHECK_ARG(smoothing >= 0 && smoothing <= 1, "%s: smoothing must be in 0..1", what);
+    ME_TRY(check_row_stats(what, row_stats));
     ME_CHECK_ARG(loss != nullptr && (pairs == 0 || (chosen != nullptr && rejected != nullptr)), "%s: null output", what);
-    ME_CHECK_ARG(n == 0 || (ref_logps != nullptr && (coef != nullptr) == (row_stats != nullptr)), "%s: null pointer", what);
+    ME_CHECK_ARG(n == 0 || ref_logps != nullptr, "%s: ref_logps is null", what);
+    ME_CHECK_ARG((coef != nullptr) == (row_stats != nullptr), "%s: row_stats and coef go together", what);
     const Space w = carve(workspace, n, vocab, pairs);
     ME_TRY(check_space(what, w, workspace, workspace_bytes));
     const hipStream_t s = as_stream(stream);
@@ -904,7 +938,7 @@ extern "C" int me_policy(const void *logits, int dtype, int64_t n, int64_t vocab
                          double scale, int reduction, float *loss, float *logps, float *out_stats, float *row_stats,
                          float *coef, void *grad, void *workspace, size_t workspace_bytes, void *stream) {
     const char *what = "me_policy";
-    ME_CHECK_ARG(vocab >= 1 && vocab <= kMaxSpan * kMaxSplits, "%s: vocab must be in 1..%d", what, kMaxSpan * kMaxSplits);
+    ME_TRY(check_vocab(what, vocab));
     const Logits l = logits_of(logits, n, rows_per_batch, batch_stride, row_stride, vocab);
     ME_TRY(check_logits(what, l, dtype));
     ME_TRY(check_temperature(what, temperature));
@@ -913,6 +947,7 @@ extern "C" int me_policy(const void *logits, int dtype, int64_t n, int64_t vocab
     ME_CHECK_ARG(clip_low >= 0 && clip_high >= 0, "%s: clip bounds must not be negative", what);
     ME_CHECK_ARG(reduction >= kMean && reduction <= kSequence, "%s: unknown reduction", what);
     ME_CHECK_ARG(loss != nullptr && out_stats != nullptr, "%s: null output", what);
+    ME_TRY(check_row_stats(what, row_stats));
     ME_CHECK_ARG(n == 0 || (old_logps != nullptr && advantages != nullptr && logps != nullptr && coef != nullptr),
                  "%s: null pointer", what);
     ME_CHECK_ARG(grad == nullptr || n == 0 || row_stats != nullptr, "%s: grad needs row_stats", what);
@@ -992,7 +1027,7 @@ extern "C" int me_distill(const void *logits, int dtype, int64_t n, int64_t voca
                           float *row_stats, float *coef, float *fix, void *grad, void *workspace,
                           size_t workspace_bytes, void *stream) {
     const char *what = "me_distill";
-    ME_CHECK_ARG(vocab >= 1 && vocab <= kMaxSpan * kMaxSplits, "%s: vocab must be in 1..%d", what, kMaxSpan * kMaxSplits);
+    ME_TRY(check_vocab(what, vocab));
     const Logits l = logits_of(logits, n, rows_per_batch, batch_stride, row_stride, vocab);
     ME_TRY(check_logits(what, l, dtype));
     ME_TRY(check_temperature(what, temperature));
@@ -1002,6 +1037,7 @@ extern "C" int me_distill(const void *logits, int dtype, int64_t n, int64_t voca
     ME_CHECK_ARG(teacher_lse == nullptr || top < vocab, "%s: entries for every token leave no rest", what);
     ME_CHECK_ARG(reduction == kMean || reduction == kSum, "%s: unknown reduction", what);
     ME_CHECK_ARG(loss != nullptr, "%s: null output", what);
+    ME_TRY(check_row_stats(what, row_stats));
     ME_CHECK_ARG(n == 0 || (teacher_ids != nullptr && teacher != nullptr && row_stats != nullptr && coef != nullptr &&
                             fix != nullptr), "%s: null pointer", what);
     const Space w = carve(workspace, n, vocab, 0, top);
@@ -1088,7 +1124,7 @@ extern "C" int me_distill_backward(const void *logits, int dtype, int64_t n, int
                                    int64_t top, double temperature, const float *row_stats, const float *coef,
                                    const float *fix, const float *upstream, int done_for_one, void *grad, void *stream) {
     const char *what = "me_distill_backward";
-    ME_CHECK_ARG(vocab >= 1 && vocab <= kMaxSpan * kMaxSplits, "%s: vocab must be in 1..%d", what, kMaxSpan * kMaxSplits);
+    ME_TRY(check_vocab(what, vocab));
     const Logits l = logits_of(logits, n, rows_per_batch, batch_stride, row_stride, vocab);
     ME_TRY(check_logits(what, l, dtype));
     ME_TRY(check_temperature(what, temperature));
@@ -1097,6 +1133,7 @@ extern "C" int me_distill_backward(const void *logits, int dtype, int64_t n, int
     ME_CHECK_ARG(n == 0 || (teacher_ids != nullptr && row_stats != nullptr && coef != nullptr && fix != nullptr &&
                             grad != nullptr), "%s: null pointer", what);
     ME_CHECK_ARG(!done_for_one || upstream != nullptr, "%s: done_for_one needs upstream", what);
+    ME_TRY(check_row_stats(what, row_stats));
     const Split sp = grad_split_of(n, vocab, dtype);
     GradArgs g = {};
     g.logits = l;

@@ -141,7 +141,8 @@ class _TokenLogps(torch.autograd.Function):
         logits, targets, stats = ctx.saved_tensors  # looks whether they are still as they were
         if ctx.run is not None:
             return ctx.run(_upstream(grad)), None, None
-        return loss_ops.token_logps_backward(logits.detach(), targets, stats, _upstream(grad), *ctx.consts), None, None
+        grad = loss_ops.token_logps_backward(logits.detach(), targets, stats, _upstream(grad), *ctx.consts)
+        return grad, None, None
 
 
 def token_logps(logits, targets, temperature=1.0, ignore_index=IGNORE_INDEX):
@@ -178,8 +179,8 @@ class _Preference(torch.autograd.Function):
         logits, targets, saved = ctx.saved_tensors
         if ctx.run is not None:
             return ctx.run(_upstream(upstream)), None, None
-        return loss_ops.saved_token_backward(logits.detach(), targets, saved, _upstream(upstream), ctx.ignore_index,
-                                             1.0), None, None
+        grad = loss_ops.saved_token_backward(logits.detach(), targets, saved, _upstream(upstream), ctx.ignore_index, 1.0)
+        return grad, None, None
 
 
 def preference_loss(logits, targets, ref_logps, cu_seqlens=None, beta=0.1, loss_type="sigmoid",
@@ -240,7 +241,8 @@ class _Policy(torch.autograd.Function):
         run, ctx.run = ctx.run, None  # its gradient is handed out once
         if run is not None:
             return run(_upstream(upstream)), None, None
-        return loss_ops.saved_token_backward(logits.detach(), targets, saved, _upstream(upstream), *ctx.consts), None, None
+        grad = loss_ops.saved_token_backward(logits.detach(), targets, saved, _upstream(upstream), *ctx.consts)
+        return grad, None, None
 
 
 def policy_loss(logits, targets, old_logps, advantages, ref_logps=None, cu_seqlens=None, clip_low=0.2,
@@ -303,7 +305,8 @@ class _Distill(torch.autograd.Function):
         run, ctx.run = ctx.run, None
         if run is not None:
             return run(_upstream(upstream)), None, None
-        return loss_ops.distill_backward(logits.detach(), teacher_ids, saved, _upstream(upstream), ctx.temperature), None, None
+        grad = loss_ops.distill_backward(logits.detach(), teacher_ids, saved, _upstream(upstream), ctx.temperature)
+        return grad, None, None
 
 
 def distill_loss(logits, teacher_ids, teacher_logits, teacher_lse=None, mask=None, temperature=1.0, scale=1.0,

@@ -597,3 +597,25 @@ def test_tokens_that_are_nearly_certain_keep_their_digits(dtype, vocab):
     _close(logps, want, REL * want.detach().abs(), "policy logps")
     ratio = torch.exp(want.detach() - old.double().cpu())
     _close(grad, -want_grad * ratio[:, None] / n, (2 * REL + HALF_ULP[dtype]) * (want_grad * ratio[:, None] / n).abs(), "policy grad")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("temperature", [1e-6, 1e-3, 1e6])
+def test_extreme_temperatures(dtype, temperature):
+    # z is x / temperature: up to 3e7, where only ties and near ties share any weight; or nearly 0, where all tokens do
+    n, vocab = 9, 2051
+    x, hot = _logits(n, vocab, dtype, 4)
+    x[:3] += 500.0
+    targets = hot.clone()
+    targets[::3] = 7
+    x[1, 11] = x[1, hot[1]]
+    leaf = x.double().requires_grad_()
+    want = ref64.token_logps(leaf, targets, temperature)
+    want_grad, = torch.autograd.grad(want.sum(), leaf)
+    xg = x.to(DEV).requires_grad_()
+    got = losses.token_logps(xg, targets.to(DEV), temperature=temperature)
+    grad, = torch.autograd.grad(got.sum(), xg)
+    _close(got, want, REL + 3e-7 * want.detach().abs(), "logps")
+    # a probability's error is that of its exponent z: its two roundings, relative to |z| where it still is a probability (< 90)
+    tol = _grad_tol(torch.ones(n).double() / temperature, _probs(x.double(), temperature), targets, dtype, want_grad)
+    _close(grad, want_grad, tol + 1e-37 / temperature, "grad")
