@@ -301,7 +301,6 @@ __global__ __launch_bounds__(kThreads) void pass_kernel(const RowArgs a, void *g
 
     // ---- gradient
     if (grad == nullptr) return;
-    if (grad == nullptr) return;
     if (!guessed) {
         for (int32_t j = tid; j < vocab; j += kThreads)
             store1(g + j, !kDist && j == t ? at_token : factor * exp2_of(load1(x + j), ref, a.k));

@@ -139,8 +139,9 @@ class _TokenLogps(torch.autograd.Function):
     @_no_second_derivatives
     def backward(ctx, grad):
         logits, targets, stats = ctx.saved_tensors  # looks whether they are still as they were
-        if ctx.run is not None:
-            return ctx.run(_upstream(grad)), None, None
+        run, ctx.run = ctx.run, None  # so that a loss that is kept does not keep the logits
+        if run is not None:
+            return run(_upstream(grad)), None, None
         grad = loss_ops.token_logps_backward(logits.detach(), targets, stats, _upstream(grad), *ctx.consts)
         return grad, None, None
 
@@ -177,8 +178,9 @@ class _Preference(torch.autograd.Function):
         if upstream is None:
             return None, None, None
         logits, targets, saved = ctx.saved_tensors
-        if ctx.run is not None:
-            return ctx.run(_upstream(upstream)), None, None
+        run, ctx.run = ctx.run, None
+        if run is not None:
+            return run(_upstream(upstream)), None, None
         grad = loss_ops.saved_token_backward(logits.detach(), targets, saved, _upstream(upstream), ctx.ignore_index, 1.0)
         return grad, None, None
 

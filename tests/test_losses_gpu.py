@@ -484,6 +484,22 @@ def test_upstream_gradients_and_repeated_backwards(name, vocab, dtype):
     _close(both, 2 * single.double().cpu(), 1e-6 * single.double().abs().cpu() + 1e-12, "twice")
 
 
+@pytest.mark.parametrize("name", ["logps", "preference", "policy", "distill"])
+def test_a_kept_loss_holds_no_logits_after_its_backward(name):
+    x = torch.randn(6, 50, generator=_gen(8)).to(DEV).requires_grad_()
+    f = _losses_of(x)[name]
+    wide = torch.zeros(6, 1 << 20, device=DEV)  # 24 MB; columns past the 50 make no difference to what is held
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    y = torch.cat([x, wide], dim=1)
+    loss = f(y)
+    grad, = torch.autograd.grad(loss, x)
+    assert torch.isfinite(grad).all()
+    del y, grad
+    assert torch.cuda.memory_allocated() - before < 1 << 20  # the loss and its graph alone
+    assert torch.isfinite(loss)
+
+
 @pytest.mark.parametrize("name", ["logps", "preference", "policy", "distill", "distill_rest"])
 def test_same_bits_every_time_and_on_another_stream(name):
     x = (torch.randn(6, 40_001, generator=_gen(8)) * 2).bfloat16().to(DEV)
