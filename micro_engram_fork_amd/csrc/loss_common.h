@@ -471,7 +471,7 @@ static __device__ void distill_entries(const RowArgs &a, int64_t r, int64_t off,
             }
         }
         p = id >= 0 ? p / norm : 0.0f;
-        e.p[i] = first ? p : -p;
+        e.p[i] = first ? fabsf(p) : -fabsf(p);  // a NaN may have come with a sign of its own
     }
     wave_lds_order();
 }

@@ -708,7 +708,8 @@ int check_seqs(const char *what, const void *offsets, int dtype, int64_t n_seqs,
     if (offsets != nullptr) {
         ME_CHECK_ARG(dtype == ME_I32 || dtype == ME_I64, "%s: sequence offsets must be int32 or int64", what);
     } else {
-        ME_CHECK_ARG(length >= 0 && n_seqs * length == n, "%s: the sequences do not hold the rows", what);
+        ME_CHECK_ARG(length >= 0 && length <= INT32_MAX && n_seqs * length == n,
+                     "%s: the sequences do not hold the rows", what);
     }
     return ME_OK;
 }

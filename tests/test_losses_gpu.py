@@ -419,6 +419,22 @@ def test_distill_entries_that_hold_nearly_everything():
     _close(grad, want_grad, 3 * REL * want_grad.abs() + REL * 0.5 * torch.softmax(x.double(), -1) + 1e-7, "grad")
 
 
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("bits", [0x7fc00000, -0x400000], ids=["nan", "negative nan"])
+@pytest.mark.parametrize("n,vocab", [(6, 50), (6, 640), (2, 9000)])  # in two sweeps, in one read, in parts
+def test_distill_of_a_teacher_without_a_value_is_none(n, vocab, bits, rest):
+    x = torch.randn(n, vocab, generator=_gen(9)).to(DEV).requires_grad_()
+    ids, teacher = _teacher(n, vocab, 5, 9)
+    lse = (teacher.logsumexp(1) + 0.2).to(DEV) if rest else None
+    teacher[1, 2] = torch.tensor(bits, dtype=torch.int32).view(torch.float32)
+    ids, teacher = ids.to(DEV), teacher.to(DEV)
+    loss = losses.distill_loss(x, ids, teacher, teacher_lse=lse)
+    grad, = torch.autograd.grad(loss, x)
+    assert bool(loss.isnan()) and bool(grad[1, ids[1, 2]].isnan()) and bool(grad[0].isfinite().all())
+    with torch.no_grad():
+        assert bool(losses.distill_loss(x, ids, teacher, teacher_lse=lse).isnan())
+
+
 # ----------------------------------------------------------------------- autograd and the device
 def _losses_of(x, seed=3):
     """name -> function of logits [6, vocab] giving a scalar."""
