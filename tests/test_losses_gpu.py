@@ -296,6 +296,18 @@ def test_policy(dtype, reduction, reference, per_seq, packed, b, t, vocab):
     _close(again[2], stats, 4 * REL, "stats without gradients")
 
 
+def test_policy_advantages_of_as_many_sequences_as_tokens():
+    x, hot = (v.to(DEV) for v in _logits(3, 77, torch.float32, 8))
+    old = losses.token_logps(x, hot)
+    adv = torch.tensor([1.0, 2.0, 4.0], device=DEV)
+    cu = torch.tensor([0, 0, 1, 3], device=DEV)  # the first sequence is empty, the last has two tokens
+    of_tokens = losses.policy_loss(x, hot, old, adv, cu_seqlens=cu, reduction="sum")[0]
+    of_seqs = losses.policy_loss(x, hot, old, adv[:, None], cu_seqlens=cu, reduction="sum")[0]
+    # ratios of 1 up to the rounding of the log-probabilities: REL each, by advantages up to 4
+    assert float(of_tokens) == pytest.approx(-7.0, abs=12 * REL)
+    assert float(of_seqs) == pytest.approx(-10.0, abs=12 * REL)
+
+
 def test_policy_rows_of_no_sequence_and_empty_batches():
     x, hot = _logits(9, 77, torch.float32, 8)
     old = ref64.token_logps(x.double(), hot).float().to(DEV)
