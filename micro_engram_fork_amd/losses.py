@@ -261,8 +261,9 @@ def policy_loss(logits, targets, old_logps, advantages, ref_logps=None, cu_seqle
     tokens whose ratio was clipped.
 
     advantages: of targets' shape, or one for each sequence: [sequences], or [sequences, 1], which is never taken
-    for values of the tokens where a packed batch has as many sequences (some of them empty) as tokens. Sequences
-    as in preference_loss (a 1-D batch without cu_seqlens is one sequence)."""
+    for values of the tokens where a packed 1-D batch has as many sequences (some of them empty) as tokens, or
+    [*targets.shape[:-1], 1] where these are as many. Sequences as in preference_loss (a 1-D batch without
+    cu_seqlens is one sequence)."""
     _check_targets(logits, targets)
     how = _choice(_POLICY_REDUCTIONS, reduction, "reduction")
     clip_low = _check_number(clip_low, "clip_low")
@@ -276,7 +277,8 @@ def policy_loss(logits, targets, old_logps, advantages, ref_logps=None, cu_seqle
     old = _per_row(old_logps, targets.shape, "old_logps")
     ref = None if ref_logps is None else _per_row(ref_logps, targets.shape, "ref_logps")
     per_seq = advantages.shape != targets.shape
-    if per_seq and tuple(advantages.shape) not in ((n_seqs,), (n_seqs, 1), (*targets.shape[:-1], 1)):
+    if per_seq and (advantages.numel() != n_seqs or tuple(advantages.shape) not in
+                    ((n_seqs,), (n_seqs, 1), (*targets.shape[:-1], 1))):  # (the last of as many sequences as rows of targets)
         raise ValueError(f"[micro_engram] advantages {tuple(advantages.shape)} are neither the rows' "
                          f"{tuple(targets.shape)} nor one for each of {n_seqs} sequences")
     adv = _per_row(advantages, advantages.shape, "advantages")
