@@ -126,7 +126,7 @@ class _TokenLogps(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, args):
         ctx.run = None
-        if loss_ops.is_plain(logits, targets):
+        if loss_ops.is_plain(logits, targets, *args):
             (logps, stats), held = loss_ops.run_token_logps(logits.detach(), targets, *args, True)
             ctx.run = loss_ops.LogpsBackward(held, args[1], stats)
         else:
@@ -140,7 +140,7 @@ class _TokenLogps(torch.autograd.Function):
     def backward(ctx, grad):
         logits, targets, stats = ctx.saved_tensors  # looks whether they are still as they were
         run, ctx.run = ctx.run, None  # so that a loss that is kept does not keep the logits
-        if run is not None:
+        if run is not None and loss_ops.is_plain(grad):
             return run(_upstream(grad)), None, None
         grad = loss_ops.token_logps_backward(logits.detach(), targets, stats, _upstream(grad), *ctx.consts)
         return grad, None, None
@@ -161,7 +161,7 @@ class _Preference(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, args):
         ctx.run = None
-        if loss_ops.is_plain(logits, targets):
+        if loss_ops.is_plain(logits, targets, *args):
             (loss, chosen, rejected, saved), held = loss_ops.run_preference(logits.detach(), targets, *args, True)
             ctx.run = loss_ops.token_backward(held, 1.0, saved)
         else:
@@ -179,7 +179,7 @@ class _Preference(torch.autograd.Function):
             return None, None, None
         logits, targets, saved = ctx.saved_tensors
         run, ctx.run = ctx.run, None
-        if run is not None:
+        if run is not None and loss_ops.is_plain(upstream):
             return run(_upstream(upstream)), None, None
         grad = loss_ops.saved_token_backward(logits.detach(), targets, saved, _upstream(upstream), ctx.ignore_index, 1.0)
         return grad, None, None
@@ -224,7 +224,7 @@ class _Policy(torch.autograd.Function):
     def forward(ctx, logits, targets, args):
         ctx.consts = args[-1], args[-4]  # ignore_index, temperature
         ctx.run = None
-        if loss_ops.is_plain(logits, targets):
+        if loss_ops.is_plain(logits, targets, *args):
             (loss, logps, out_stats, saved, grad), held = loss_ops.run_policy(logits.detach(), targets, *args, True)
             ctx.run = loss_ops.token_backward(held, args[-4], saved, grad)
         else:  # traced: the gradient is the backward's, nothing is written in place
@@ -241,7 +241,7 @@ class _Policy(torch.autograd.Function):
             return None, None, None
         logits, targets, saved = ctx.saved_tensors
         run, ctx.run = ctx.run, None  # its gradient is handed out once
-        if run is not None:
+        if run is not None and loss_ops.is_plain(upstream):
             return run(_upstream(upstream)), None, None
         grad = loss_ops.saved_token_backward(logits.detach(), targets, saved, _upstream(upstream), *ctx.consts)
         return grad, None, None
@@ -295,7 +295,7 @@ class _Distill(torch.autograd.Function):
     def forward(ctx, logits, teacher_ids, args):
         ctx.temperature = args[3]
         ctx.run = None
-        if loss_ops.is_plain(logits, teacher_ids):
+        if loss_ops.is_plain(logits, teacher_ids, *args):
             (loss, saved, grad), held = loss_ops.run_distill(logits.detach(), teacher_ids, *args, True)
             ctx.run = loss_ops.distill_backward_of(held, ctx.temperature, saved, grad)
         else:
@@ -308,7 +308,7 @@ class _Distill(torch.autograd.Function):
     def backward(ctx, upstream):
         logits, teacher_ids, saved = ctx.saved_tensors
         run, ctx.run = ctx.run, None
-        if run is not None:
+        if run is not None and loss_ops.is_plain(upstream):
             return run(_upstream(upstream)), None, None
         grad = loss_ops.distill_backward(logits.detach(), teacher_ids, saved, _upstream(upstream), ctx.temperature)
         return grad, None, None

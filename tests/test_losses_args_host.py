@@ -3,7 +3,7 @@ refused, shapes that do reach the GPU's own check."""
 import pytest
 import torch
 
-from micro_engram_fork_amd import losses
+from micro_engram_fork_amd import loss_ops, losses
 
 
 def _policy(shape, advantages, sequences=None):
@@ -32,3 +32,93 @@ def test_advantages_of_another_number_of_sequences_are_refused(shape, advantages
 def test_advantages_of_the_tokens_or_the_sequences_pass(shape, advantages, sequences):
     with pytest.raises(RuntimeError, match="only on the GPU"):
         _policy(shape, advantages, sequences)
+
+
+class _Reached(Exception):
+    pass
+
+
+class _Wrapped(torch.Tensor):
+    """A tensor subclass without memory of its own (as sharded or quantised tensors are), which ends a call at the
+    first of this library's ops that it reaches."""
+
+    @staticmethod
+    def __new__(cls, inner):
+        return torch.Tensor._make_wrapper_subclass(cls, inner.shape, dtype=inner.dtype, device=inner.device)
+
+    def __init__(self, inner):
+        self.inner = inner
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        if func.namespace == "micro_engram_amd":
+            raise _Reached(func.name())
+        res = func(*(a.inner if isinstance(a, cls) else a for a in args), **(kwargs or {}))
+        return cls(res) if isinstance(res, torch.Tensor) else res
+
+
+def _loss_with(name, wrapped, grad):
+    """The loss with its argument `wrapped` as such a subclass."""
+    rows, vocab = (2, 3), 11
+    args = dict(logits=torch.zeros(*rows, vocab, requires_grad=grad))
+    if name == "distill_loss":
+        args.update(teacher_ids=torch.zeros(*rows, 2, dtype=torch.long), teacher_logits=torch.zeros(*rows, 2),
+                    teacher_lse=torch.zeros(rows), mask=torch.ones(rows, dtype=torch.bool))
+    else:
+        args["targets"] = torch.zeros(rows, dtype=torch.long)
+    if name == "preference_loss":
+        args.update(ref_logps=torch.zeros(rows), cu_seqlens=torch.tensor([0, 3, 6]))
+    if name == "policy_loss":
+        args.update(old_logps=torch.zeros(rows), advantages=torch.zeros(2), ref_logps=torch.zeros(rows),
+                    cu_seqlens=torch.tensor([0, 3, 6]))
+    args[wrapped] = _Wrapped(args[wrapped])
+    return getattr(losses, name)(**args)
+
+
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("name,wrapped", [
+    ("token_logps", "targets"), ("preference_loss", "targets"), ("preference_loss", "ref_logps"), ("preference_loss", "cu_seqlens"),
+    ("policy_loss", "old_logps"), ("policy_loss", "advantages"), ("policy_loss", "ref_logps"), ("policy_loss", "cu_seqlens"),
+    ("distill_loss", "teacher_ids"), ("distill_loss", "teacher_logits"), ("distill_loss", "teacher_lse"), ("distill_loss", "mask"),
+])
+def test_tensor_subclasses_in_any_argument_reach_the_op(name, wrapped, grad):
+    # not the kernels with the subclass's own address, which is none: an optional argument would count as not given
+    with pytest.raises(_Reached, match="micro_engram_amd::" + name.replace("_loss", "")):
+        _loss_with(name, wrapped, grad)
+
+
+@pytest.fixture
+def entry_calls(monkeypatch):
+    """The losses without their kernels: names of the library's entry points in the order of their calls."""
+    names = []
+    monkeypatch.setattr(loss_ops, "call", lambda name, *args: names.append(name))
+    monkeypatch.setattr(loss_ops, "require_gpu", lambda *tensors: torch.device("cpu"))
+    monkeypatch.setattr(loss_ops, "stream_of", lambda device: 0)
+    monkeypatch.setattr(loss_ops, "workspace_bytes", lambda *sizes: 256)
+    return names
+
+
+def _plain_loss(name, logits):
+    rows = logits.shape[:-1]
+    targets, values = torch.zeros(rows, dtype=torch.long), torch.zeros(rows)
+    if name == "token_logps":
+        return losses.token_logps(logits, targets)
+    if name == "preference_loss":
+        return losses.preference_loss(logits, targets, values)[0]
+    if name == "policy_loss":
+        return losses.policy_loss(logits, targets, values, values)[0]
+    return losses.distill_loss(logits, targets[..., None], values[..., None])
+
+
+NAMES = ["token_logps", "preference_loss", "policy_loss", "distill_loss"]
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_an_upstream_gradient_of_a_subclass_reaches_the_op(entry_calls, name):
+    logits = torch.zeros(2, 3, 11, requires_grad=True)
+    loss = _plain_loss(name, logits)
+    with pytest.raises(_Reached, match="backward"):
+        torch.autograd.grad(loss, logits, _Wrapped(torch.full(loss.shape, 3.0)))
+    assert len(entry_calls) == 1
+    torch.autograd.grad(_plain_loss(name, logits), logits, torch.full(loss.shape, 3.0))
+    assert len(entry_calls) == 3 and entry_calls[2].endswith("_backward")

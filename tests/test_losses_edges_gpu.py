@@ -1,0 +1,72 @@
+"""The losses over logits where a call is out of the ordinary: tensor subclasses among the arguments."""
+import pytest
+import torch
+
+from micro_engram_fork_amd import losses
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+ROWS, VOCAB = (2, 3), 77
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+class _Wrapped(torch.Tensor):
+    """A subclass that holds another tensor and hands every op that tensor."""
+
+    @staticmethod
+    def __new__(cls, inner):
+        return torch.Tensor._make_wrapper_subclass(cls, inner.shape, dtype=inner.dtype, device=inner.device)
+
+    def __init__(self, inner):
+        self.inner = inner
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        res = func(*(a.inner if isinstance(a, cls) else a for a in args), **(kwargs or {}))
+        # values made from a wrapped one are wrapped, results of this library's ops plain
+        return cls(res) if func.namespace == "aten" and isinstance(res, torch.Tensor) else res
+
+
+def _arguments():
+    """name -> (function, its arguments but the logits)."""
+    values = lambda seed, *shape: torch.randn(*shape, generator=_gen(seed)).to(DEV)  # noqa: E731
+    targets = torch.randint(0, VOCAB, ROWS, generator=_gen(1)).to(DEV)
+    ids = torch.stack([torch.randperm(VOCAB, generator=_gen(k))[:4] for k in range(6)]).view(*ROWS, 4).to(DEV)
+    teacher = values(2, *ROWS, 4)
+    cu = torch.tensor([0, 2, 6], device=DEV)
+    return {
+        "token_logps": (losses.token_logps, dict(targets=targets)),
+        "preference": (losses.preference_loss, dict(targets=targets, ref_logps=values(3, *ROWS) - 4, cu_seqlens=cu)),
+        "policy": (losses.policy_loss, dict(targets=targets, old_logps=values(4, *ROWS) - 4, advantages=values(5, 2),
+                                            ref_logps=values(6, *ROWS) - 4, cu_seqlens=cu, kl_coef=0.3)),
+        "distill": (losses.distill_loss, dict(teacher_ids=ids, teacher_logits=teacher, teacher_lse=teacher.logsumexp(-1) + 0.3,
+                                              mask=torch.tensor([[True, True, False], [True, False, True]], device=DEV))),
+    }
+
+
+def _first(out):
+    return out[0] if isinstance(out, tuple) else out
+
+
+@pytest.mark.parametrize("name,wrapped", [
+    ("token_logps", "targets"), ("preference", "ref_logps"), ("preference", "cu_seqlens"), ("policy", "old_logps"),
+    ("policy", "advantages"), ("policy", "ref_logps"), ("policy", "cu_seqlens"), ("distill", "teacher_logits"),
+    ("distill", "teacher_lse"), ("distill", "mask"), ("distill", "upstream"), ("policy", "upstream"), ("preference", "upstream"),
+    ("token_logps", "upstream")])
+def test_subclasses_give_the_values_of_what_they_hold(name, wrapped):
+    fn, args = _arguments()[name]
+    x = torch.randn(*ROWS, VOCAB, generator=_gen(9)).to(DEV).requires_grad_()
+    want = _first(fn(x, **args))
+    upstream = torch.full_like(want, 3.0)
+    want_grad, = torch.autograd.grad(want, x, upstream)
+    if wrapped == "upstream":
+        upstream = _Wrapped(upstream)
+    else:
+        args[wrapped] = _Wrapped(args[wrapped])
+    got = _first(fn(x, **args))
+    grad, = torch.autograd.grad(got, x, upstream)
+    # the same kernels on the same values
+    assert torch.equal(got, want) and torch.equal(grad, want_grad)
