@@ -19,7 +19,9 @@ fp64 inside, whatever the logits are.
 distill_loss and policy_loss know a row's gradient as soon as they have read the row, so with
 gradients they write it in the forward and keep it for the backward, for an upstream gradient of 1.
 The backward looks (on the device) whether that held, and computes the gradient again from the
-logits if not: give a factor such as 1 / accumulation steps as `scale`, where it costs nothing.
+logits if not: give a factor such as 1 / accumulation steps as `scale`, where it costs nothing. Under
+hooks on saved tensors (torch.autograd.graph.save_on_cpu, non-reentrant checkpointing) nothing is kept
+that does not pass through the hooks, and the gradient is written in the backward.
 """
 import functools
 import math
@@ -121,12 +123,17 @@ def _wants_grad(logits):
 # ------------------------------------------------------------------------- log-probabilities
 # The Functions take everything but their first two tensors as one tuple: apply() costs host time for each argument,
 # and a small batch's training step is bound by the rate at which the host issues it. For plain tensors the
-# backward's call is made ready in the forward (ctx.run, used once: a second backward makes its own).
+# backward's call is made ready in the forward (ctx.run, used once: a second backward makes its own). It holds the
+# logits and for two of the losses the gradient, so it is not made where hooks on saved tensors are to have these.
+def _makes_ready(*values):
+    return loss_ops.is_plain(*values) and torch._C._autograd._top_saved_tensors_default_hooks(False) is None
+
+
 class _TokenLogps(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, args):
         ctx.run = None
-        if loss_ops.is_plain(logits, targets, *args):
+        if _makes_ready(logits, targets, *args):
             (logps, stats), held = loss_ops.run_token_logps(logits.detach(), targets, *args, True)
             ctx.run = loss_ops.LogpsBackward(held, args[1], stats)
         else:
@@ -161,7 +168,7 @@ class _Preference(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, args):
         ctx.run = None
-        if loss_ops.is_plain(logits, targets, *args):
+        if _makes_ready(logits, targets, *args):
             (loss, chosen, rejected, saved), held = loss_ops.run_preference(logits.detach(), targets, *args, True)
             ctx.run = loss_ops.token_backward(held, 1.0, saved)
         else:
@@ -224,10 +231,10 @@ class _Policy(torch.autograd.Function):
     def forward(ctx, logits, targets, args):
         ctx.consts = args[-1], args[-4]  # ignore_index, temperature
         ctx.run = None
-        if loss_ops.is_plain(logits, targets, *args):
+        if _makes_ready(logits, targets, *args):
             (loss, logps, out_stats, saved, grad), held = loss_ops.run_policy(logits.detach(), targets, *args, True)
             ctx.run = loss_ops.token_backward(held, args[-4], saved, grad)
-        else:  # traced: the gradient is the backward's, nothing is written in place
+        else:  # the gradient is the backward's, nothing is written in place
             loss, logps, out_stats, saved = loss_ops.policy(logits.detach(), targets, *args, False)
         ctx.save_for_backward(logits, targets, saved)
         ctx.mark_non_differentiable(logps, out_stats)
@@ -295,7 +302,7 @@ class _Distill(torch.autograd.Function):
     def forward(ctx, logits, teacher_ids, args):
         ctx.temperature = args[3]
         ctx.run = None
-        if loss_ops.is_plain(logits, teacher_ids, *args):
+        if _makes_ready(logits, teacher_ids, *args):
             (loss, saved, grad), held = loss_ops.run_distill(logits.detach(), teacher_ids, *args, True)
             ctx.run = loss_ops.distill_backward_of(held, ctx.temperature, saved, grad)
         else:

@@ -122,3 +122,22 @@ def test_an_upstream_gradient_of_a_subclass_reaches_the_op(entry_calls, name):
     assert len(entry_calls) == 1
     torch.autograd.grad(_plain_loss(name, logits), logits, torch.full(loss.shape, 3.0))
     assert len(entry_calls) == 3 and entry_calls[2].endswith("_backward")
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_saved_tensor_hooks_get_all_that_a_backward_needs(entry_calls, name):
+    # hooks that move saved tensors off the GPU, or make them again, find the logits nowhere else in the graph
+    packed, logits = [], torch.zeros(2, 3, 11, requires_grad=True)
+
+    def pack(t):
+        packed.append(t.shape)
+        return t.clone()
+
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t):
+        loss = _plain_loss(name, logits * 1)
+    assert torch.Size((2, 3, 11)) in packed
+    assert loss.grad_fn.run is None  # the prepared call would hold them
+    torch.autograd.grad(loss, logits, torch.ones(loss.shape))
+    assert len(entry_calls) == 2 and entry_calls[1].endswith("_backward")
+    loss = _plain_loss(name, logits * 1)
+    assert loss.grad_fn.run is not None

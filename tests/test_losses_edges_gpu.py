@@ -1,6 +1,8 @@
-"""The losses over logits where a call is out of the ordinary: tensor subclasses among the arguments."""
+"""The losses over logits where a call is out of the ordinary: tensor subclasses among the arguments, hooks on what a
+backward keeps."""
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from micro_engram_fork_amd import losses
 
@@ -70,3 +72,37 @@ def test_subclasses_give_the_values_of_what_they_hold(name, wrapped):
     grad, = torch.autograd.grad(got, x, upstream)
     # the same kernels on the same values
     assert torch.equal(got, want) and torch.equal(grad, want_grad)
+
+
+# ------------------------------------------------------------------------------- saved tensors
+WIDE = 1 << 20  # columns added to the logits, 24 MB in all
+
+
+def _close(a, b):
+    """Gradients of one row kernel and of two sweeps: probabilities off by 1.5e-5 of themselves in each."""
+    torch.testing.assert_close(a, b, rtol=6e-5, atol=1e-9)
+
+
+@pytest.mark.parametrize("name", ["token_logps", "preference", "policy", "distill"])
+@pytest.mark.parametrize("way", ["save_on_cpu", "checkpoint"])
+def test_what_saved_tensor_hooks_take_is_not_held_beside(name, way):
+    fn, args = _arguments()[name]
+    x = torch.randn(*ROWS, VOCAB, generator=_gen(9)).to(DEV).requires_grad_()
+    wide = torch.full((*ROWS, WIDE), -1e4, device=DEV)
+
+    def value(z):
+        return _first(fn(torch.cat([z, wide], dim=-1), **args))
+
+    plain = value(x)
+    want, = torch.autograd.grad(plain.sum(), x)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    if way == "save_on_cpu":
+        with torch.autograd.graph.save_on_cpu():
+            loss = value(x)
+    else:
+        loss = torch.utils.checkpoint.checkpoint(value, x, use_reentrant=False)
+    assert torch.cuda.memory_allocated() - before < 1 << 20  # the graph alone
+    grad, = torch.autograd.grad(loss.sum(), x)
+    assert torch.allclose(loss, plain, rtol=1e-5, atol=1e-6)
+    _close(grad, want)
