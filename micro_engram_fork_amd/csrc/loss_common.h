@@ -339,8 +339,16 @@ __device__ __forceinline__ float row_logit(const Logits &l, int64_t off, int32_t
     return bf16 ? load1(static_cast<const uint16_t *>(l.x) + off + j) : load1(static_cast<const float *>(l.x) + off + j);
 }
 
-// exp(d) - 1 - d without the cancellation of small d
-__device__ __forceinline__ float exp_excess(float d) { return expm1f(d) - d; }
+// exp(d) - 1 - d: for small d, where d is nearly all of exp(d) - 1, by its series (the first term left out is 5e-8 of the
+// sum at 0.5); infinite for an infinite d.
+__device__ __forceinline__ float exp_excess(float d) {
+    if (fabsf(d) < 0.5f) {
+        const float tail = 1.0f + d * (1.0f / 3) * (1.0f + d * (1.0f / 4) * (1.0f + d * (1.0f / 5) * (1.0f + d * (1.0f / 6) *
+                           (1.0f + d * (1.0f / 7) * (1.0f + d * (1.0f / 8))))));
+        return 0.5f * d * d * tail;
+    }
+    return fabsf(d) == kInf ? kInf : expm1f(d) - d;
+}
 
 // A row's token against all others. `others` is the (m, s) of these alone, so that a log-probability near 0 and the
 // 1 - q of the gradient there keep their digits: log(1 + u) for the others' weight u over the token's.

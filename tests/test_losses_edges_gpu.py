@@ -1,5 +1,7 @@
 """The losses over logits where a call is out of the ordinary: tensor subclasses among the arguments, hooks on what a
 backward keeps."""
+import math
+
 import pytest
 import torch
 import torch.utils.checkpoint
@@ -106,3 +108,38 @@ def test_what_saved_tensor_hooks_take_is_not_held_beside(name, way):
     grad, = torch.autograd.grad(loss.sum(), x)
     assert torch.allclose(loss, plain, rtol=1e-5, atol=1e-6)
     _close(grad, want)
+
+
+# -------------------------------------------------------------------------------------- policy
+ROUTES = [(3, 7), (6, 640), (2, 9000)]  # rows and vocabulary: two sweeps, one read, rows in parts
+
+
+def _sampled(n, vocab):
+    """Logits that want gradients, targets, their log-probabilities as the losses give them."""
+    x = torch.randn(n, vocab, generator=_gen(2)).to(DEV).requires_grad_()
+    targets = torch.randint(0, vocab, (n,), generator=_gen(3)).to(DEV)
+    return x, targets, losses.token_logps(x.detach(), targets)
+
+
+@pytest.mark.parametrize("d", [1e-6, 1e-4, 3e-3, 0.02, 0.24, 0.26, 0.49, 0.51, 1.0, 5.0, 40.0])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_policy_kl_of_small_differences_keeps_its_digits(d, sign):
+    # one token in all: its log-probability is 0 exactly, the difference the reference's. The value is a series of a few
+    # terms or a difference that loses at most two bits: 1e-6 of itself
+    ref = torch.tensor([sign * d], device=DEV)
+    x = torch.randn(1, 1, generator=_gen(1)).to(DEV)
+    loss, logps, stats = losses.policy_loss(x, torch.zeros(1, dtype=torch.long, device=DEV), torch.zeros(1, device=DEV),
+                                            torch.zeros(1, device=DEV), ref_logps=ref, kl_coef=1.0)
+    d = float(ref)
+    want = math.expm1(d) - d if abs(d) > 1e-2 else sum(d ** k / math.factorial(k) for k in range(2, 9))
+    assert float(logps) == 0.0
+    assert float(stats[0]) == pytest.approx(want, rel=1e-6) and float(loss) == pytest.approx(want, rel=1e-6)
+
+
+@pytest.mark.parametrize("n,vocab", ROUTES)
+def test_policy_kl_of_a_token_ruled_out_is_infinite(n, vocab):
+    x, targets, old = _sampled(n, vocab)
+    x.data[1, targets[1]] = -float("inf")
+    for kl_coef in (0.0, 0.1):
+        stats = losses.policy_loss(x.detach(), targets, old, torch.ones(n, device=DEV), ref_logps=old, kl_coef=kl_coef)[2]
+        assert float(stats[0]) == float("inf")
