@@ -394,8 +394,10 @@ __device__ __forceinline__ void policy_terms(const RowArgs &a, const Sampled &v,
     if (a.ref_logps != nullptr) {
         const float d = v.ref_logp - logp;
         kl = exp_excess(d);
-        loss += a.kl_coef * kl;
-        slope -= a.kl_coef * expm1f(d);
+        if (a.kl_coef != 0.0f) {  // a coefficient of 0 makes no term of a value past fp32 either
+            loss += a.kl_coef * kl;
+            slope -= a.kl_coef * expm1f(d);
+        }
     }
 }
 

@@ -264,8 +264,8 @@ def policy_loss(logits, targets, old_logps, advantages, ref_logps=None, cu_seqle
 
     times `scale`, reduced by "token" (mean over counted tokens), "sequence" (mean over sequences with a
     counted token of their means) or "sum". Log-probabilities (fp32, targets' shape) and stats carry no
-    gradient; stats [2] are the means over counted tokens of the KL term (0 without ref_logps) and of the
-    tokens whose ratio was clipped.
+    gradient; stats [2] are the means over counted tokens of exp(d) - d - 1 (0 without ref_logps; with a kl_coef
+    of 0 ref_logps is for this alone) and of the tokens whose ratio was clipped.
 
     advantages: of targets' shape, or one for each sequence: [sequences], or [sequences, 1], which is never taken
     for values of the tokens where a packed 1-D batch has as many sequences (some of them empty) as tokens, or

@@ -143,3 +143,24 @@ def test_policy_kl_of_a_token_ruled_out_is_infinite(n, vocab):
     for kl_coef in (0.0, 0.1):
         stats = losses.policy_loss(x.detach(), targets, old, torch.ones(n, device=DEV), ref_logps=old, kl_coef=kl_coef)[2]
         assert float(stats[0]) == float("inf")
+
+
+@pytest.mark.parametrize("n,vocab", ROUTES)
+@pytest.mark.parametrize("far", ["reference", "logit"])
+def test_policy_with_the_kl_as_a_statistic_alone(n, vocab, far):
+    # kl_coef 0: no KL term, also where its value is past fp32
+    x, targets, old = _sampled(n, vocab)
+    ref = old.clone()
+    if far == "reference":
+        ref[1] += 100.0
+    else:  # a token that has been ruled out since it was sampled
+        x.data[1, targets[1]] = -float("inf")
+    adv = torch.tensor([2.0, 0.5, -1.0, 1.0, 1.0, 3.0], device=DEV)[:n]
+    want, _, _ = losses.policy_loss(x, targets, old, adv)
+    want_grad, = torch.autograd.grad(want, x)
+    loss, _, stats = losses.policy_loss(x, targets, old, adv, ref_logps=ref, kl_coef=0.0)
+    grad, = torch.autograd.grad(loss, x)
+    assert bool(want.isfinite()) and torch.equal(loss, want) and torch.equal(grad, want_grad)
+    assert float(stats[0]) == float("inf")
+    with torch.no_grad():
+        assert bool(losses.policy_loss(x, targets, old, adv, ref_logps=ref)[0].isfinite())
