@@ -386,7 +386,9 @@ __device__ __forceinline__ void policy_terms(const RowArgs &a, const Sampled &v,
                                              float &kl, bool &clipped) {
     const float ratio = expf(logp - v.old_logp);
     const float held = fminf(fmaxf(ratio, 1.0f - a.clip_low), 1.0f + a.clip_high);
-    const float free_term = ratio * v.advantage, held_term = held * v.advantage;
+    // an advantage of 0 makes no term of a ratio past fp32 either (a NaN stays one)
+    const float free_term = v.advantage == 0.0f && ratio == kInf ? 0.0f : ratio * v.advantage;
+    const float held_term = held * v.advantage;
     clipped = free_term > held_term;
     loss = -(clipped ? held_term : free_term);
     slope = clipped ? 0.0f : -free_term;

@@ -164,3 +164,21 @@ def test_policy_with_the_kl_as_a_statistic_alone(n, vocab, far):
     assert float(stats[0]) == float("inf")
     with torch.no_grad():
         assert bool(losses.policy_loss(x, targets, old, adv, ref_logps=ref)[0].isfinite())
+
+
+@pytest.mark.parametrize("n,vocab", ROUTES)
+def test_policy_of_an_advantage_of_zero(n, vocab):
+    # its term is 0 at any ratio, also one past fp32; a ratio that is NaN stays NaN
+    x, targets, old = _sampled(n, vocab)
+    old[1] = -200.0
+    adv = torch.ones(n, device=DEV)
+    adv[1] = 0.0
+    loss, _, stats = losses.policy_loss(x, targets, old, adv, reduction="sum")
+    grad, = torch.autograd.grad(loss, x)
+    # ratios of 1 up to the rounding of log-probabilities in other orders of the sum
+    assert float(loss) == pytest.approx(1.0 - n, abs=(n - 1) * 1.5e-5)
+    assert int(grad[1].count_nonzero()) == 0 and bool(grad.isfinite().all()) and float(stats[1]) == 0.0
+    with torch.no_grad():
+        assert float(losses.policy_loss(x, targets, old, adv, reduction="sum")[0]) == pytest.approx(1.0 - n, abs=(n - 1) * 1.5e-5)
+    old[1] = float("nan")
+    assert bool(losses.policy_loss(x, targets, old, adv)[0].isnan())
