@@ -402,7 +402,8 @@ struct PairArgs {
     float *chosen, *rejected, *loss;
     double *sums;          // [pairs]
     int64_t pairs;
-    float beta, smoothing;
+    double beta;
+    float smoothing;
     int32_t vocab;
     int kind, normalized;
 };
@@ -411,11 +412,12 @@ struct PairArgs {
 __device__ __forceinline__ float softplus_neg(float x) { return fmaxf(-x, 0.0f) + log1pf(expf(-fabsf(x))); }
 
 // One pair by one wavefront: both sequences' sums, the loss, and the factors of their rows' gradients. Returns the loss.
-// Eight rows per lane are requested at a time: the sums are bound by the loads' latency.
+// Eight rows per lane are requested at a time: the sums are bound by the loads' latency. The sums and their difference,
+// where two large values nearly cancel, are in fp64; what is rounded to fp32 is the difference.
 __device__ double pair_terms(const PairArgs &a, int64_t p) {
     constexpr int kFlight = 8;
     const int lane = threadIdx.x & 63;
-    float d[2];
+    double d[2];
     int64_t from[2], to[2];
     float inv_len[2];
     for (int side = 0; side < 2; ++side) {
@@ -442,24 +444,26 @@ __device__ double pair_terms(const PairArgs &a, int64_t p) {
         }
         sum = wave_sum(sum);
         count = wave_sum(count);
-        inv_len[side] = a.normalized ? 1.0f / static_cast<float>(count > 0 ? count : 1) : 1.0f;
-        d[side] = static_cast<float>(sum * inv_len[side]);
+        const double length = a.normalized && count > 0 ? static_cast<double>(count) : 1.0;
+        inv_len[side] = static_cast<float>(1.0 / length);
+        d[side] = sum / length;
     }
-    const float h = d[0] - d[1], x = a.beta * h;
+    const double h = d[0] - d[1];
+    const float beta = static_cast<float>(a.beta), x = static_cast<float>(a.beta * h);
     float loss, slope;
     if (a.kind == kSigmoid) {
         loss = (1.0f - a.smoothing) * softplus_neg(x) + a.smoothing * softplus_neg(-x);
         // 1 / (1 + e^-x) - (1 - smoothing), each side's small part kept: sigma(x) - 1 = -sigma(-x)
         const float up = 1.0f / (1.0f + expf(-x)), down = 1.0f / (1.0f + expf(x));
-        slope = a.beta * (a.smoothing * up - (1.0f - a.smoothing) * down);
+        slope = beta * (a.smoothing * up - (1.0f - a.smoothing) * down);
     } else if (a.kind == kIpo) {
-        const float e = h - 0.5f / a.beta;
+        const float e = static_cast<float>(h - 0.5 / a.beta);
         loss = e * e;
         slope = 2.0f * e;
     } else {
         loss = fmaxf(1.0f - x, 0.0f);
         if (x != x) loss = x;
-        slope = x < 1.0f ? -a.beta : 0.0f;
+        slope = x < 1.0f ? -beta : 0.0f;
     }
     slope /= static_cast<float>(a.pairs);
     for (int side = 0; a.coef != nullptr && side < 2; ++side) {
@@ -475,8 +479,8 @@ __device__ double pair_terms(const PairArgs &a, int64_t p) {
         }
     }
     if (lane == 0) {
-        a.chosen[p] = a.beta * d[0];
-        a.rejected[p] = a.beta * d[1];
+        a.chosen[p] = static_cast<float>(a.beta * d[0]);
+        a.rejected[p] = static_cast<float>(a.beta * d[1]);
     }
     return loss;
 }
@@ -936,7 +940,7 @@ extern "C" int me_preference(const void *logits, int dtype, int64_t n, int64_t v
     p.loss = loss;
     p.sums = w.sums;
     p.pairs = pairs;
-    p.beta = static_cast<float>(beta);
+    p.beta = beta;
     p.smoothing = static_cast<float>(smoothing);
     p.vocab = l.vocab;
     p.kind = kind;

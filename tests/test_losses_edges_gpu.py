@@ -182,3 +182,33 @@ def test_policy_of_an_advantage_of_zero(n, vocab):
         assert float(losses.policy_loss(x, targets, old, adv, reduction="sum")[0]) == pytest.approx(1.0 - n, abs=(n - 1) * 1.5e-5)
     old[1] = float("nan")
     assert bool(losses.policy_loss(x, targets, old, adv)[0].isnan())
+
+
+# ---------------------------------------------------------------------------------- preference
+def _pair_of_sums(chosen, rejected, normalized, kind, beta):
+    """preference_loss of two sequences whose differences to the reference are given (one token in all: log-probabilities
+    of 0 exactly), and its 64-bit value."""
+    ref = -torch.tensor([*chosen, *rejected], dtype=torch.float32)
+    n = len(ref)
+    cu = torch.tensor([0, len(chosen), n], device=DEV)
+    got = losses.preference_loss(torch.zeros(n, 1, device=DEV), torch.zeros(n, dtype=torch.long, device=DEV), ref.to(DEV),
+                                 cu_seqlens=cu, beta=beta, loss_type=kind, length_normalized=normalized)
+    d = [float((-part.double()).sum()) / (len(part) if normalized else 1) for part in ref.split([len(chosen), len(rejected)])]
+    h = d[0] - d[1]
+    want = {"sigmoid": math.log1p(math.exp(-abs(beta * h))) + max(-beta * h, 0.0), "ipo": (h - 0.5 / beta) ** 2,
+            "hinge": max(0.0, 1 - beta * h)}[kind]
+    return got, want, d
+
+
+@pytest.mark.parametrize("kind", ["sigmoid", "ipo", "hinge"])
+@pytest.mark.parametrize("normalized", [False, True])
+def test_preference_of_long_answers_far_from_the_reference(kind, normalized):
+    # sums of about 5000 (means of about 1) that differ by little: h keeps the digits that each has past fp32
+    g = _gen(4)
+    base = torch.rand(5000, generator=g) + 0.5
+    chosen, rejected = (base + 1e-4).tolist(), base[torch.randperm(5000, generator=g)].tolist()
+    beta = 0.5 if not normalized else 50.0
+    got, want, d = _pair_of_sums(chosen, rejected, normalized, kind, beta)
+    # h is exact up to its own rounding; a few roundings of fp32 follow
+    assert float(got[0]) == pytest.approx(want, rel=1e-6)
+    assert float(got[1]) == pytest.approx(beta * d[0], rel=3e-7) and float(got[2]) == pytest.approx(beta * d[1], rel=3e-7)
