@@ -452,7 +452,9 @@ __device__ double pair_terms(const PairArgs &a, int64_t p) {
     const float beta = static_cast<float>(a.beta), x = static_cast<float>(a.beta * h);
     float loss, slope;
     if (a.kind == kSigmoid) {
-        loss = (1.0f - a.smoothing) * softplus_neg(x) + a.smoothing * softplus_neg(-x);
+        // a share of 0 makes no term of an infinite value (a sequence with a token that is ruled out)
+        loss = a.smoothing < 1.0f ? (1.0f - a.smoothing) * softplus_neg(x) : 0.0f;
+        if (a.smoothing > 0.0f) loss += a.smoothing * softplus_neg(-x);
         // 1 / (1 + e^-x) - (1 - smoothing), each side's small part kept: sigma(x) - 1 = -sigma(-x)
         const float up = 1.0f / (1.0f + expf(-x)), down = 1.0f / (1.0f + expf(x));
         slope = beta * (a.smoothing * up - (1.0f - a.smoothing) * down);

@@ -212,3 +212,26 @@ def test_preference_of_long_answers_far_from_the_reference(kind, normalized):
     # h is exact up to its own rounding; a few roundings of fp32 follow
     assert float(got[0]) == pytest.approx(want, rel=1e-6)
     assert float(got[1]) == pytest.approx(beta * d[0], rel=3e-7) and float(got[2]) == pytest.approx(beta * d[1], rel=3e-7)
+
+
+@pytest.mark.parametrize("smoothing", [0.0, 1.0])
+@pytest.mark.parametrize("side", [0, 1])
+def test_preference_of_an_answer_that_cannot_be(side, smoothing):
+    # a token of it is ruled out: its sum is minus infinity. The sigmoid loss is 0 where that is as it should be, and
+    # infinite where not, whose gradient is that of an ordinary lost pair
+    n, vocab = 6, 50
+    x = torch.randn(n, vocab, generator=_gen(5))
+    targets = torch.arange(n)
+    x[3 * side + 1, targets[3 * side + 1]] = -float("inf")
+    xg = x.to(DEV).requires_grad_()
+    loss, chosen, rejected = losses.preference_loss(xg, targets.to(DEV), torch.zeros(n, device=DEV),
+                                                    cu_seqlens=torch.tensor([0, 3, 6], device=DEV), beta=0.5, label_smoothing=smoothing)
+    grad, = torch.autograd.grad(loss, xg)
+    assert float((chosen, rejected)[side]) == -float("inf") and bool((chosen, rejected)[1 - side].isfinite().all())
+    wanted = side == (1 if smoothing == 0.0 else 0)  # the answer that should lose
+    assert float(loss) == (0.0 if wanted else float("inf"))
+    assert bool(grad.isfinite().all())
+    q = torch.softmax(x.double(), -1)
+    c = torch.tensor([1.0, -1.0]).repeat_interleave(3)[:, None] * (0.5 if smoothing else -0.5)
+    want = c * (torch.nn.functional.one_hot(targets, vocab) - q) * (0.0 if wanted else 1.0)
+    torch.testing.assert_close(grad.double().cpu(), want, rtol=3e-5, atol=1e-9)
