@@ -4,6 +4,7 @@ fake implementation for tracing, no host synchronisation. losses.py is the surfa
 """
 import ctypes
 import functools
+import math
 from typing import List, Optional
 
 import torch
@@ -35,11 +36,12 @@ def row_layout(logits):
     n = logits.numel() // vocab if vocab else 0
     rows = logits
     if lead > 2:
+        flat = math.prod(logits.shape[:-2]), logits.shape[-2], vocab
         try:
-            rows = logits.view(-1, logits.shape[-2], vocab)
+            rows = logits.view(flat)
         except RuntimeError:
             logits = logits.contiguous()
-            rows = logits.view(-1, logits.shape[-2], vocab)
+            rows = logits.view(flat)
     if lead == 0:
         per, batch_stride, row_stride = 1, 0, 0
     elif lead == 1:

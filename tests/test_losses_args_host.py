@@ -141,3 +141,16 @@ def test_saved_tensor_hooks_get_all_that_a_backward_needs(entry_calls, name):
     assert len(entry_calls) == 2 and entry_calls[1].endswith("_backward")
     loss = _plain_loss(name, logits * 1)
     assert loss.grad_fn.run is not None
+
+
+@pytest.mark.parametrize("shape", [(2, 3, 0, 10), (2, 0, 3, 10), (0, 2, 3, 10), (2, 2, 0, 3, 10), (2, 0, 10), (0, 10)])
+def test_row_layout_of_no_rows(shape):
+    logits, args = loss_ops.row_layout(torch.zeros(shape))
+    assert logits.shape == shape and args[2:5] == (0, 10, max(1, shape[-2]))
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_logits_of_no_rows_in_many_dims(entry_calls, name):
+    logits = torch.zeros(2, 3, 0, 10, requires_grad=True)
+    loss = _plain_loss(name, logits)
+    assert torch.autograd.grad(loss, logits, torch.ones(loss.shape))[0].shape == logits.shape

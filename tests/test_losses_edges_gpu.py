@@ -235,3 +235,18 @@ def test_preference_of_an_answer_that_cannot_be(side, smoothing):
     c = torch.tensor([1.0, -1.0]).repeat_interleave(3)[:, None] * (0.5 if smoothing else -0.5)
     want = c * (torch.nn.functional.one_hot(targets, vocab) - q) * (0.0 if wanted else 1.0)
     torch.testing.assert_close(grad.double().cpu(), want, rtol=3e-5, atol=1e-9)
+
+
+# -------------------------------------------------------------------------------------- no rows
+@pytest.mark.parametrize("shape", [(2, 3, 0, 10), (2, 0, 3, 10)])
+def test_no_rows_in_many_dims(shape):
+    x = torch.zeros(shape, device=DEV, requires_grad=True)
+    targets, rows = torch.zeros(shape[:-1], dtype=torch.long, device=DEV), torch.zeros(shape[:-1], device=DEV)
+    pairs = math.prod(shape[:-2]) // 2
+    out = losses.token_logps(x, targets)
+    assert out.shape == targets.shape and torch.autograd.grad(out.sum(), x)[0].shape == x.shape
+    loss, chosen, _ = losses.preference_loss(x, targets, rows)
+    assert float(loss.detach()) == pytest.approx(math.log(2) if pairs else 0.0) and chosen.tolist() == [0.0] * pairs
+    assert torch.autograd.grad(loss, x)[0].shape == x.shape
+    for loss in (losses.policy_loss(x, targets, rows, rows)[0], losses.distill_loss(x, targets[..., None], rows[..., None])):
+        assert float(loss.detach()) == 0 and torch.autograd.grad(loss, x)[0].shape == x.shape
