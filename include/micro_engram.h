@@ -531,6 +531,9 @@ int me_mask_media(const void *ids, int ids_dtype, int64_t n, int64_t width, int6
  *   logits      [n, vocab] of dtype (ME_BF16 / ME_F32): row r starts at element
  *               (r / rows_per_batch) * batch_stride + (r % rows_per_batch) * row_stride, its
  *               values next to each other; rows may start at any element. vocab <= 2,097,152.
+ *   n           A launch holds fewer than 2^32 threads, and a call that would need more is
+ *               refused: rows of up to 2048 tokens take 64 each, longer ones 256 for each 8192
+ *               (ME_F32: 4096; where no gradient is wanted 32,768) tokens begun.
  *   targets     [n] token ids of targets_dtype (ME_I32 / ME_I64). A row whose target is
  *               ignore_index or outside [0, vocab) does not count: it is not read, its values
  *               are 0 and its gradient is zeros.

@@ -681,15 +681,21 @@ Logits logits_of(const void *x, int64_t n, int64_t rows_per_batch, int64_t batch
     return {x, n, static_cast<uint32_t>(per), batch_stride, row_stride, static_cast<int32_t>(vocab)};
 }
 
-int check_logits(const char *what, const Logits &l, int dtype) {
+// Rows of up to kShort tokens take workgroups of one wavefront in both sweeps, longer ones of four.
+constexpr int64_t kShort = 2048;
+
+// with_grad: the call writes the gradient, or leaves what it is made from.
+int check_logits(const char *what, const Logits &l, int dtype, bool with_grad) {
     ME_CHECK_ARG(dtype == ME_BF16 || dtype == ME_F32, "%s: logits must be bf16 or fp32", what);
     ME_CHECK_ARG(l.n >= 0 && l.n <= INT32_MAX, "%s: n out of range", what);
     ME_CHECK_ARG(l.n == 0 || l.x != nullptr, "%s: logits are null", what);
     ME_CHECK_ARG(l.rows_per_batch >= 1, "%s: rows_per_batch must be positive", what);
     ME_CHECK_ARG(l.row_stride >= 0 && l.batch_stride >= 0, "%s: negative strides", what);
-    const Split s = split_of(l.n, l.vocab);
-    const Split g = grad_split_of(l.n, l.vocab, dtype);
-    ME_CHECK_ARG(l.n * s.splits < INT32_MAX && l.n * g.splits < INT32_MAX, "%s: too many rows", what);
+    // A launch of 2^32 threads or more is cut to what its count's lower 32 bits say, without an error. The sweeps have
+    // the most: the one-read kernels have no more threads for a row than the gradient's parts, nor without a gradient
+    // than the sums' parts. (16 workgroups: the one of the weights, the last of the entries.)
+    const Split s = with_grad ? grad_split_of(l.n, l.vocab, dtype) : split_of(l.n, l.vocab);
+    ME_CHECK_ARG((l.n * s.splits + 16) * (l.vocab <= kShort ? 64 : 256) <= int64_t{UINT32_MAX}, "%s: too many rows", what);
     return ME_OK;
 }
 
@@ -729,7 +735,7 @@ void launch_stats_of(const StatsArgs &a, bool left_out, hipStream_t s) {
 }
 
 void launch_stats(StatsArgs a, int dtype, bool left_out, hipStream_t s) {
-    const bool small = a.logits.vocab <= 2048;
+    const bool small = a.logits.vocab <= kShort;
     if (small && a.weights.counted != nullptr && a.logits.n > 1024) {  // too many for a workgroup of one wavefront
         weights_kernel<<<1, 1024, 0, s>>>(a.weights);
         a.weights.counted = nullptr;
@@ -775,7 +781,7 @@ void launch_grad_of(const GradArgs &a, bool stream_out, hipStream_t s) {
 
 void launch_grad(const GradArgs &a, int dtype, hipStream_t s) {
     if (a.logits.n == 0) return;
-    const bool small = a.logits.vocab <= 2048, out = streams(a.logits, a.grad, dtype);
+    const bool small = a.logits.vocab <= kShort, out = streams(a.logits, a.grad, dtype);
     if (dtype == ME_BF16) {
         if (small) launch_grad_of<uint16_t, 64>(a, out, s);
         else launch_grad_of<uint16_t, 256>(a, out, s);
@@ -818,7 +824,7 @@ extern "C" int me_token_logps(const void *logits, int dtype, int64_t n, int64_t 
     const char *what = "me_token_logps";
     ME_TRY(check_vocab(what, vocab));
     const Logits l = logits_of(logits, n, rows_per_batch, batch_stride, row_stride, vocab);
-    ME_TRY(check_logits(what, l, dtype));
+    ME_TRY(check_logits(what, l, dtype, row_stats != nullptr));
     ME_TRY(check_temperature(what, temperature));
     ME_TRY(check_tokens(what, targets, targets_dtype, n));
     ME_CHECK_ARG(n == 0 || logps != nullptr, "%s: logps is null", what);
@@ -859,7 +865,7 @@ extern "C" int me_token_logps_backward(const void *logits, int dtype, int64_t n,
     const char *what = "me_token_logps_backward";
     ME_TRY(check_vocab(what, vocab));
     const Logits l = logits_of(logits, n, rows_per_batch, batch_stride, row_stride, vocab);
-    ME_TRY(check_logits(what, l, dtype));
+    ME_TRY(check_logits(what, l, dtype, true));
     ME_TRY(check_temperature(what, temperature));
     ME_TRY(check_tokens(what, targets, targets_dtype, n));
     ME_CHECK_ARG(n == 0 || (row_stats != nullptr && coef != nullptr && grad != nullptr), "%s: null pointer", what);
@@ -891,7 +897,7 @@ extern "C" int me_preference(const void *logits, int dtype, int64_t n, int64_t v
     const char *what = "me_preference";
     ME_TRY(check_vocab(what, vocab));
     const Logits l = logits_of(logits, n, rows_per_batch, batch_stride, row_stride, vocab);
-    ME_TRY(check_logits(what, l, dtype));
+    ME_TRY(check_logits(what, l, dtype, row_stats != nullptr));
     ME_TRY(check_tokens(what, targets, targets_dtype, n));
     ME_CHECK_ARG(pairs >= 0 && pairs < INT32_MAX / 2, "%s: pairs out of range", what);
     ME_TRY(check_seqs(what, seq_offsets, offsets_dtype, 2 * pairs, seq_len, n));
@@ -967,7 +973,7 @@ extern "C" int me_policy(const void *logits, int dtype, int64_t n, int64_t vocab
     const char *what = "me_policy";
     ME_TRY(check_vocab(what, vocab));
     const Logits l = logits_of(logits, n, rows_per_batch, batch_stride, row_stride, vocab);
-    ME_TRY(check_logits(what, l, dtype));
+    ME_TRY(check_logits(what, l, dtype, grad != nullptr));
     ME_TRY(check_temperature(what, temperature));
     ME_TRY(check_tokens(what, targets, targets_dtype, n));
     ME_TRY(check_seqs(what, seq_offsets, offsets_dtype, n_seqs, seq_len, n));
@@ -1056,7 +1062,7 @@ extern "C" int me_distill(const void *logits, int dtype, int64_t n, int64_t voca
     const char *what = "me_distill";
     ME_TRY(check_vocab(what, vocab));
     const Logits l = logits_of(logits, n, rows_per_batch, batch_stride, row_stride, vocab);
-    ME_TRY(check_logits(what, l, dtype));
+    ME_TRY(check_logits(what, l, dtype, grad != nullptr));
     ME_TRY(check_temperature(what, temperature));
     ME_CHECK_ARG(ids_dtype == ME_I32 || ids_dtype == ME_I64, "%s: teacher ids must be int32 or int64", what);
     ME_CHECK_ARG(teacher_dtype == ME_BF16 || teacher_dtype == ME_F32, "%s: teacher logits must be bf16 or fp32", what);
@@ -1153,7 +1159,7 @@ extern "C" int me_distill_backward(const void *logits, int dtype, int64_t n, int
     const char *what = "me_distill_backward";
     ME_TRY(check_vocab(what, vocab));
     const Logits l = logits_of(logits, n, rows_per_batch, batch_stride, row_stride, vocab);
-    ME_TRY(check_logits(what, l, dtype));
+    ME_TRY(check_logits(what, l, dtype, true));
     ME_TRY(check_temperature(what, temperature));
     ME_CHECK_ARG(ids_dtype == ME_I32 || ids_dtype == ME_I64, "%s: teacher ids must be int32 or int64", what);
     ME_CHECK_ARG(top >= 1 && top <= kMaxTop, "%s: top must be in 1..%d", what, kMaxTop);

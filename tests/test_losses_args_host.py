@@ -3,7 +3,7 @@ refused, shapes that do reach the GPU's own check."""
 import pytest
 import torch
 
-from micro_engram_fork_amd import loss_ops, losses
+from micro_engram_fork_amd import _lib, loss_ops, losses
 
 
 def _policy(shape, advantages, sequences=None):
@@ -154,3 +154,27 @@ def test_logits_of_no_rows_in_many_dims(entry_calls, name):
     logits = torch.zeros(2, 3, 0, 10, requires_grad=True)
     loss = _plain_loss(name, logits)
     assert torch.autograd.grad(loss, logits, torch.ones(loss.shape))[0].shape == logits.shape
+
+
+def _entry_args(name, n, vocab, dtype):
+    """Arguments of entry point `name` for n rows, with addresses that no refused call reads."""
+    at, logits, targets = 64, (64, dtype, n, vocab, n, 0, vocab), (64, _lib.ME_I64, -100)
+    space = (at, 1 << 62, None)
+    return {
+        "me_token_logps": (*logits, *targets, 1.0, at, at, *space),
+        "me_token_logps_backward": (*logits, *targets, 1.0, at, at, 1.0, None, 0, at, None),
+        "me_preference": (*logits, *targets, at, at, _lib.ME_I64, 1, 0, 0, 0.1, 0.0, 0, at, at, at, at, at, *space),
+        "me_policy": (*logits, *targets, at, at, 0, None, None, 0, 1, n, 0.2, 0.2, 0.0, 1.0, 1.0, 0, at, at, at, at, at, at, *space),
+        "me_distill": (*logits, at, _lib.ME_I64, at, _lib.ME_F32, 1, None, None, 1.0, 1.0, 0, at, at, at, at, at, *space),
+        "me_distill_backward": (*logits, at, _lib.ME_I64, 1, 1.0, at, at, at, None, 0, at, None),
+    }[name]
+
+
+@pytest.mark.parametrize("name", ["me_token_logps", "me_token_logps_backward", "me_preference", "me_policy", "me_distill",
+                                  "me_distill_backward"])
+@pytest.mark.parametrize("n,vocab,dtype", [((1 << 26) - 16, 64, _lib.ME_BF16), ((1 << 24) - 16, 4096, _lib.ME_F32),
+                                           (1 << 23, 8200, _lib.ME_BF16), ((1 << 31) - 1, 2, _lib.ME_BF16)])
+def test_rows_past_what_a_launch_holds_are_refused(name, n, vocab, dtype):
+    # a launch of 2^32 threads runs only those past the 32 bits that count them, without an error
+    with pytest.raises(_lib.EngramLibError, match="too many rows"):
+        _lib.call(name, *_entry_args(name, n, vocab, dtype))

@@ -6,7 +6,7 @@ import pytest
 import torch
 import torch.utils.checkpoint
 
-from micro_engram_fork_amd import losses
+from micro_engram_fork_amd import _lib, losses
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -250,3 +250,36 @@ def test_no_rows_in_many_dims(shape):
     assert torch.autograd.grad(loss, x)[0].shape == x.shape
     for loss in (losses.policy_loss(x, targets, rows, rows)[0], losses.distill_loss(x, targets[..., None], rows[..., None])):
         assert float(loss.detach()) == 0 and torch.autograd.grad(loss, x)[0].shape == x.shape
+
+
+# ------------------------------------------------------------------------------------ most rows
+MOST_SHORT = (2 ** 32 - 1) // 64 - 16  # rows of up to 2048 tokens that a launch holds
+
+
+def test_as_many_rows_as_a_launch_holds():
+    # one row in memory, expanded; targets that differ at both ends and in the middle
+    n, vocab = MOST_SHORT, 8
+    row = torch.randn(vocab, generator=_gen(6)).bfloat16().to(DEV)
+    targets = torch.zeros(n, dtype=torch.int32, device=DEV)
+    for r in (0, n // 2, n - 1):
+        targets[r] = 5
+    x = row.expand(n, vocab).requires_grad_()
+    out = losses.token_logps(x, targets)
+    grad, = torch.autograd.grad(out, x, torch.ones(n, device=DEV))
+    want = torch.log_softmax(row.double(), -1)
+    for t, count in ((5, 3), (0, n - 3)):
+        here = targets == t
+        value = out[here]
+        assert int(here.sum()) == count and bool((value == value[0]).all())
+        assert float(value[0]) == pytest.approx(float(want[t]), abs=1.5e-5)
+        rows = grad[here]
+        assert bool((rows == rows[0]).all())
+        g = torch.nn.functional.one_hot(torch.tensor(t), vocab).to(DEV) - want.exp()
+        torch.testing.assert_close(rows[0].double(), g, rtol=2.0 ** -8, atol=1.5e-5)
+
+
+def test_more_rows_are_refused():
+    n, vocab = MOST_SHORT + 1, 8
+    x = torch.zeros(vocab, device=DEV).expand(n, vocab)
+    with pytest.raises(_lib.EngramLibError, match="too many rows"):
+        losses.token_logps(x, torch.zeros(n, dtype=torch.int32, device=DEV))
