@@ -283,3 +283,56 @@ def test_more_rows_are_refused():
     x = torch.zeros(vocab, device=DEV).expand(n, vocab)
     with pytest.raises(_lib.EngramLibError, match="too many rows"):
         losses.token_logps(x, torch.zeros(n, dtype=torch.int32, device=DEV))
+
+
+# -------------------------------------------------------------------------------- distillation
+# one width of each kernel that keeps rows, as (dtype, vocabulary): 64, 256, 512 and 1024 threads, 22 units in
+# registers, with LDS, with a second read
+DISTILL_WIDTHS = [(torch.bfloat16, v) for v in (64, 1000, 8201, 40_001, 70_003, 140_001, 262_144, 300_007)] + \
+                 [(torch.float32, v) for v in (64, 4099, 16_391, 40_003, 70_001, 131_072)]
+
+
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("dtype,vocab", DISTILL_WIDTHS)
+def test_distillation_loss_of_each_row_width(dtype, vocab, rest):
+    rows, top, temp, scale = 260, 5 if vocab < 100 else 70, 1.5, 0.5
+    g = torch.Generator(device=DEV).manual_seed(vocab)
+    x = torch.randn(rows, vocab, generator=g, device=DEV) * 2
+    start = torch.randint(0, vocab, (rows, 1), generator=g, device=DEV)
+    ids = (start + torch.randint(1, vocab // top + 1, (rows, top), generator=g, device=DEV).cumsum(1)) % vocab
+    x.scatter_(1, ids[:, :1], math.log(vocab) + 1.0)
+    x = x.to(dtype)
+    ids[3, 2:4] = ids[3, 0]  # entries of one token
+    ids[4, 1:] = -1
+    ids[5] = -1              # does not count
+    mask = torch.ones(rows, dtype=torch.bool, device=DEV)
+    mask[30:60:2] = False
+    x[9, ids[9, 0]] = -float("inf")  # a token that the teacher wants and the student rules out
+    teacher = (torch.randn(rows, top, generator=g, device=DEV) * 2 + 10).to(dtype)
+    use = ids >= 0
+    t64 = torch.where(use, teacher.double() / temp, -float("inf"))
+    lse = (t64.logsumexp(1) + 0.1 + 0.2 * torch.rand(rows, generator=g, device=DEV)).nan_to_num(0, 0, 0).float() if rest else None
+    ok = mask & use.any(1)
+    # the definition in 64 bits, a token's entries added up
+    p_entry = torch.where(use, (t64 - (t64.logsumexp(1, keepdim=True) if lse is None else lse[:, None].double())).exp(), 0.0)
+    p = torch.zeros(rows, vocab, dtype=torch.float64, device=DEV).scatter_add_(1, ids.clamp(min=0), p_entry)
+    where = torch.zeros(rows, vocab, device=DEV).scatter_add_(1, ids.clamp(min=0), use.float()) > 0
+    logq = torch.log_softmax(x.double() / temp, -1)
+    each = torch.where(p > 0, p * (p.clamp(min=1e-300).log() - logq), 0.0).sum(1)
+    size = torch.where(p > 0, p * logq.abs(), 0.0).sum(1)
+    if rest:
+        left, other = 1 - p.sum(1), torch.where(where, -float("inf"), logq).logsumexp(1)
+        each, size = each + left * (left.log() - other), size + left * (left.log() - other).abs()
+    xg = x.clone().requires_grad_()
+
+    def loss(counting):
+        return losses.distill_loss(xg, ids, teacher, teacher_lse=lse, mask=counting, temperature=temp, scale=scale)
+
+    assert float(loss(mask)) == float("inf")
+    mask[9] = ok[9] = False
+    want = float(scale * temp ** 2 * each[ok].mean())
+    # log q and log p are off by 1.5e-5 each, with the rest class its logarithm too, and by the rounding of themselves
+    tol = scale * temp ** 2 * (3 * 1.5e-5 + 4e-7 * float(size[ok].mean())) + 1e-6 * abs(want)
+    assert float(loss(mask)) == pytest.approx(want, abs=tol)
+    with torch.no_grad():
+        assert float(loss(mask)) == pytest.approx(want, abs=tol)
