@@ -336,3 +336,99 @@ def test_distillation_loss_of_each_row_width(dtype, vocab, rest):
     assert float(loss(mask)) == pytest.approx(want, abs=tol)
     with torch.no_grad():
         assert float(loss(mask)) == pytest.approx(want, abs=tol)
+
+
+# ------------------------------------------------------------------------------------ many rows
+MANY = 70_001
+
+
+def _many(vocab):
+    """Rows of a small vocabulary on the GPU with targets, a few that do not count, and their log-probabilities in 64 bits."""
+    g = torch.Generator(device=DEV).manual_seed(vocab)
+    x = torch.randn(MANY, vocab, generator=g, device=DEV) * 2
+    targets = torch.randint(0, vocab, (MANY,), generator=g, device=DEV)
+    targets[torch.rand(MANY, generator=g, device=DEV) < 0.2] = -100
+    ok = targets >= 0
+    now = torch.log_softmax(x.double(), -1).gather(1, targets.clamp(min=0)[:, None]).squeeze(1)
+    return x, targets, ok, torch.where(ok, now, 0.0), g
+
+
+def _row_grad(x, targets, coef):
+    g = -coef[:, None] * torch.softmax(x.double(), -1)
+    return g.scatter_add(1, targets.clamp(min=0)[:, None], coef[:, None])
+
+
+def _close_rows(grad, want, coef):
+    tol = 6e-5 * coef.abs()[:, None] + 2.0 ** -23 * want.abs() + 1e-37
+    assert bool(((grad.double() - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("vocab", [9, 70])  # two sweeps, one read
+@pytest.mark.parametrize("reduction", ["token", "sequence"])
+def test_policy_of_many_rows_in_sequences_of_all_lengths(vocab, reduction):
+    x, targets, ok, now, g = _many(vocab)
+    cu = torch.tensor([0, 1, 1, 40_000, 40_003, 69_000, 70_000], device=DEV)  # the last row is of no sequence
+    seqs = len(cu) - 1
+    seq = torch.bucketize(torch.arange(MANY, device=DEV), cu[1:], right=True)
+    adv = torch.randn(seqs, generator=g, device=DEV)
+    old = (now - 0.1 * torch.rand(MANY, generator=g, device=DEV)).float()
+    counts = ok & (seq < seqs)
+    lengths = torch.zeros(seqs + 1, dtype=torch.float64, device=DEV).index_add(0, seq, counts.double())[:seqs]
+    weight = counts.double() / counts.sum()
+    if reduction == "sequence":
+        weight = counts / lengths.clamp(min=1)[seq.clamp(max=seqs - 1)] / (lengths > 0).sum()
+    adv_rows = adv.double()[seq.clamp(max=seqs - 1)]
+    ratio = torch.exp(now - old.double())  # 1 to 1.11: inside the bounds
+    xg = x.clone().requires_grad_()
+    loss, logps, stats = losses.policy_loss(xg, targets, old, adv[:, None], cu_seqlens=cu, reduction=reduction)
+    grad, = torch.autograd.grad(loss, xg)
+    want = -(ratio * adv_rows * weight).sum()
+    # a ratio has the error of its log-probability, 1.5e-5, and the roundings of itself and of a weight
+    size = float((ratio * adv_rows.abs() * weight).sum())
+    assert float(loss) == pytest.approx(float(want), abs=2e-5 * size)
+    assert bool(((logps.double() - now).abs()[counts] <= 1.5e-5 + 1e-6 * now.abs()[counts]).all())
+    coef = -ratio * adv_rows * weight
+    _close_rows(grad, _row_grad(x, targets, coef), coef)
+    assert int(grad[~counts].count_nonzero()) == 0 and stats.tolist() == [0.0, 0.0]
+
+
+@pytest.mark.parametrize("vocab", [9, 70])
+def test_distillation_of_many_rows(vocab):
+    x, targets, _, _, g = _many(vocab)
+    mask = targets >= 0
+    ids = torch.randint(0, vocab, (MANY, 1), generator=g, device=DEV)
+    xg = x.clone().requires_grad_()
+    loss = losses.distill_loss(xg, ids, torch.zeros(MANY, 1, device=DEV), mask=mask)
+    grad, = torch.autograd.grad(loss, xg)
+    # one entry has all of the teacher: minus its log-probability
+    each = -torch.log_softmax(x.double(), -1).gather(1, ids).squeeze(1)
+    want = each[mask].mean()
+    assert float(loss) == pytest.approx(float(want), abs=2 * 1.5e-5 + 1e-6 * float(want))
+    coef = -mask.double() / mask.sum()
+    _close_rows(grad, _row_grad(x, ids.squeeze(1), coef), coef)
+
+
+@pytest.mark.parametrize("vocab", [9, 70])
+def test_preference_of_many_pairs(vocab):
+    x, targets, ok, now, g = _many(vocab)
+    pairs = 10_000
+    cuts = torch.sort(torch.randint(0, MANY, (2 * pairs - 1,), generator=g, device=DEV)).values
+    cu = torch.cat([torch.tensor([0], device=DEV), cuts, torch.tensor([MANY], device=DEV)])
+    ref = (now + 0.1 * torch.randn(MANY, generator=g, device=DEV)).float()
+    seq = torch.bucketize(torch.arange(MANY, device=DEV), cu[1:], right=True)
+    d = torch.zeros(2 * pairs, dtype=torch.float64, device=DEV).index_add(0, seq, torch.where(ok, now - ref.double(), 0.0))
+    longest = int(torch.bincount(seq).max())
+    xg = x.clone().requires_grad_()
+    loss, chosen, rejected = losses.preference_loss(xg, targets, ref, cu_seqlens=cu, beta=0.5)
+    grad, = torch.autograd.grad(loss, xg)
+    h = d[:pairs] - d[pairs:]
+    off = 1.5e-5 * longest + 3e-7 * float(d.abs().max())  # log-probabilities off by 1.5e-5 each
+    assert float(loss) == pytest.approx(float(torch.nn.functional.softplus(-0.5 * h).mean()), abs=2 * 0.5 * off)
+    got = torch.cat([chosen, rejected]).double()
+    assert bool(((got - 0.5 * d).abs() <= 0.5 * off).all())
+    slope = -0.5 * torch.sigmoid(-0.5 * h) / pairs
+    coef = torch.where(ok, torch.cat([slope, -slope])[seq], 0.0)
+    want = _row_grad(x, targets, coef)
+    # the factor's derivative by h is at most 1/4 of 0.5^2 / pairs
+    tol = 6e-5 * coef.abs()[:, None] + 2 * off * 0.0625 / pairs + 2.0 ** -23 * want.abs()
+    assert bool(((grad.double() - want).abs() <= tol).all()) and int(grad[~ok].count_nonzero()) == 0
