@@ -981,8 +981,9 @@ extern "C" int me_policy(const void *logits, int dtype, int64_t n, int64_t vocab
     ME_CHECK_ARG(reduction >= kMean && reduction <= kSequence, "%s: unknown reduction", what);
     ME_CHECK_ARG(loss != nullptr && out_stats != nullptr, "%s: null output", what);
     ME_TRY(check_row_stats(what, row_stats));
-    ME_CHECK_ARG(n == 0 || (old_logps != nullptr && advantages != nullptr && logps != nullptr && coef != nullptr),
-                 "%s: null pointer", what);
+    const bool none = n == 0 || (adv_per_seq && n_seqs == 0);  // advantages of nothing have no address
+    ME_CHECK_ARG(none || advantages != nullptr, "%s: advantages are null", what);
+    ME_CHECK_ARG(n == 0 || (old_logps != nullptr && logps != nullptr && coef != nullptr), "%s: null pointer", what);
     ME_CHECK_ARG(grad == nullptr || n == 0 || row_stats != nullptr, "%s: grad needs row_stats", what);
     const Space w = carve(workspace, n, vocab, 0);
     ME_TRY(check_space(what, w, workspace, workspace_bytes));

@@ -432,3 +432,15 @@ def test_preference_of_many_pairs(vocab):
     # the factor's derivative by h is at most 1/4 of 0.5^2 / pairs
     tol = 6e-5 * coef.abs()[:, None] + 2 * off * 0.0625 / pairs + 2.0 ** -23 * want.abs()
     assert bool(((grad.double() - want).abs() <= tol).all()) and int(grad[~ok].count_nonzero()) == 0
+
+
+def test_policy_of_no_sequences():
+    # rows, but no sequence that holds one, and so no advantage either
+    x = torch.randn(5, 33, generator=_gen(7)).to(DEV).requires_grad_()
+    rows, targets = torch.zeros(5, device=DEV), torch.zeros(5, dtype=torch.long, device=DEV)
+    for reduction in ("token", "sequence", "sum"):
+        loss, logps, stats = losses.policy_loss(x, targets, rows, torch.zeros(0, device=DEV), reduction=reduction,
+                                                cu_seqlens=torch.zeros(1, dtype=torch.long, device=DEV))
+        grad, = torch.autograd.grad(loss, x)
+        assert float(loss.detach()) == 0 and logps.tolist() == [0.0] * 5 and stats.tolist() == [0.0, 0.0]
+        assert int(grad.count_nonzero()) == 0
