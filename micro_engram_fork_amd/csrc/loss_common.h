@@ -184,6 +184,9 @@ struct MaxSum {
     float m, s;
 };
 
+// one logit; a NaN is put in s, as m goes through fmaxf, which drops it
+__device__ __forceinline__ MaxSum pair_of(float x) { return {x, x == x ? 1.0f : x}; }
+
 // exp2((x - m) k); v_exp_f32 is within one unit in the last place and takes minus infinity to 0
 __device__ __forceinline__ float exp2_of(float x, float m, float k) { return __builtin_amdgcn_exp2f((x - m) * k); }
 
@@ -364,7 +367,7 @@ __device__ __forceinline__ TokenTerms token_terms(float xt, MaxSum others, float
     else v.logp = -log1pf(others.s * expf(d));
     if (xt == kInf) v.logp = __builtin_nanf("");  // infinity over infinity
     v.rest = -expm1f(v.logp);
-    v.all = join(others, {xt, 1.0f}, k);
+    v.all = join(others, pair_of(xt), k);
     return v;
 }
 
@@ -499,7 +502,7 @@ static __device__ float distill_finish(const RowArgs &a, int64_t r, MaxSum seen,
     if (rest) {
         MaxSum mine = {-kInf, 0.0f};
         for (int32_t i = lane; i < a.top; i += 64)
-            if (e.id[i] >= 0 && !__builtin_signbitf(e.p[i])) mine = join(mine, {e.x[i], 1.0f}, a.k);
+            if (e.id[i] >= 0 && !__builtin_signbitf(e.p[i])) mine = join(mine, pair_of(e.x[i]), a.k);
         all = join(seen, wave_join(mine, a.k), a.k);
     }
     const float log_s = logf(all.s), inv_s = 1.0f / all.s;

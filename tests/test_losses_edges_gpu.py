@@ -444,3 +444,26 @@ def test_policy_of_no_sequences():
         grad, = torch.autograd.grad(loss, x)
         assert float(loss.detach()) == 0 and logps.tolist() == [0.0] * 5 and stats.tolist() == [0.0, 0.0]
         assert int(grad.count_nonzero()) == 0
+
+
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n,vocab", ROUTES)
+def test_distillation_of_a_logit_that_is_none(n, vocab, dtype, rest):
+    # among the teacher's entries or the other tokens: the row has no loss, whatever the entry's own probability
+    top = min(5, vocab - 1)
+    ids = torch.stack([torch.randperm(vocab, generator=_gen(k))[:top] for k in range(n)]).to(DEV)
+    teacher = torch.randn(n, top, generator=_gen(8)).to(DEV)
+    teacher[:, 1] = -200.0  # an entry of probability 0
+    lse = teacher.logsumexp(-1) + 0.3 if rest else None
+    base = torch.randn(n, vocab, generator=_gen(9)).to(dtype).to(DEV)
+    others = [j for j in range(vocab) if j not in ids[1].tolist()]
+    for token in (int(ids[1, 0]), int(ids[1, 1]), int(ids[1, top - 1]), others[0], others[-1]):
+        x = base.clone()
+        x[1, token] = float("nan")
+        xg = x.requires_grad_()
+        loss = losses.distill_loss(xg, ids, teacher, teacher_lse=lse)
+        grad, = torch.autograd.grad(loss, xg)
+        assert bool(loss.isnan()) and bool(grad[1].isnan().any()) and bool(grad[0].isfinite().all()), token
+        with torch.no_grad():
+            assert bool(losses.distill_loss(xg, ids, teacher, teacher_lse=lse).isnan())
