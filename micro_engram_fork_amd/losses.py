@@ -125,15 +125,16 @@ def _wants_grad(logits):
 # and a small batch's training step is bound by the rate at which the host issues it. For plain tensors the
 # backward's call is made ready in the forward (ctx.run, used once: a second backward makes its own). It holds the
 # logits and for two of the losses the gradient, so it is not made where hooks on saved tensors are to have these.
-def _makes_ready(*values):
-    return loss_ops.is_plain(*values) and torch._C._autograd._top_saved_tensors_default_hooks(False) is None
+def _makes_ready(*tensors):
+    """tensors: all that the call takes, those that were not given as None."""
+    return loss_ops.is_plain(*tensors) and torch._C._autograd._top_saved_tensors_default_hooks(False) is None
 
 
 class _TokenLogps(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, args):
         ctx.run = None
-        if _makes_ready(logits, targets, *args):
+        if _makes_ready(logits, targets):
             (logps, stats), held = loss_ops.run_token_logps(logits.detach(), targets, *args, True)
             ctx.run = loss_ops.LogpsBackward(held, args[1], stats)
         else:
@@ -147,7 +148,7 @@ class _TokenLogps(torch.autograd.Function):
     def backward(ctx, grad):
         logits, targets, stats = ctx.saved_tensors  # looks whether they are still as they were
         run, ctx.run = ctx.run, None  # so that a loss that is kept does not keep the logits
-        if run is not None and loss_ops.is_plain(grad):
+        if run is not None and type(grad) is torch.Tensor:  # subclasses go through the op
             return run(_upstream(grad)), None, None
         grad = loss_ops.token_logps_backward(logits.detach(), targets, stats, _upstream(grad), *ctx.consts)
         return grad, None, None
@@ -168,7 +169,7 @@ class _Preference(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, args):
         ctx.run = None
-        if _makes_ready(logits, targets, *args):
+        if _makes_ready(logits, targets, *args[:2]):  # ref_logps, cu_seqlens
             (loss, chosen, rejected, saved), held = loss_ops.run_preference(logits.detach(), targets, *args, True)
             ctx.run = loss_ops.token_backward(held, 1.0, saved)
         else:
@@ -186,7 +187,7 @@ class _Preference(torch.autograd.Function):
             return None, None, None
         logits, targets, saved = ctx.saved_tensors
         run, ctx.run = ctx.run, None
-        if run is not None and loss_ops.is_plain(upstream):
+        if run is not None and type(upstream) is torch.Tensor:
             return run(_upstream(upstream)), None, None
         grad = loss_ops.saved_token_backward(logits.detach(), targets, saved, _upstream(upstream), ctx.ignore_index, 1.0)
         return grad, None, None
@@ -231,7 +232,7 @@ class _Policy(torch.autograd.Function):
     def forward(ctx, logits, targets, args):
         ctx.consts = args[-1], args[-4]  # ignore_index, temperature
         ctx.run = None
-        if _makes_ready(logits, targets, *args):
+        if _makes_ready(logits, targets, *args[:2], *args[3:5]):  # old_logps, advantages, ref_logps, cu_seqlens
             (loss, logps, out_stats, saved, grad), held = loss_ops.run_policy(logits.detach(), targets, *args, True)
             ctx.run = loss_ops.token_backward(held, args[-4], saved, grad)
         else:  # the gradient is the backward's, nothing is written in place
@@ -248,7 +249,7 @@ class _Policy(torch.autograd.Function):
             return None, None, None
         logits, targets, saved = ctx.saved_tensors
         run, ctx.run = ctx.run, None  # its gradient is handed out once
-        if run is not None and loss_ops.is_plain(upstream):
+        if run is not None and type(upstream) is torch.Tensor:
             return run(_upstream(upstream)), None, None
         grad = loss_ops.saved_token_backward(logits.detach(), targets, saved, _upstream(upstream), *ctx.consts)
         return grad, None, None
@@ -302,7 +303,7 @@ class _Distill(torch.autograd.Function):
     def forward(ctx, logits, teacher_ids, args):
         ctx.temperature = args[3]
         ctx.run = None
-        if _makes_ready(logits, teacher_ids, *args):
+        if _makes_ready(logits, teacher_ids, *args[:3]):  # teacher_logits, teacher_lse, mask
             (loss, saved, grad), held = loss_ops.run_distill(logits.detach(), teacher_ids, *args, True)
             ctx.run = loss_ops.distill_backward_of(held, ctx.temperature, saved, grad)
         else:
@@ -315,7 +316,7 @@ class _Distill(torch.autograd.Function):
     def backward(ctx, upstream):
         logits, teacher_ids, saved = ctx.saved_tensors
         run, ctx.run = ctx.run, None
-        if run is not None and loss_ops.is_plain(upstream):
+        if run is not None and type(upstream) is torch.Tensor:
             return run(_upstream(upstream)), None, None
         grad = loss_ops.distill_backward(logits.detach(), teacher_ids, saved, _upstream(upstream), ctx.temperature)
         return grad, None, None
