@@ -544,8 +544,9 @@ int me_mask_media(const void *ids, int ids_dtype, int64_t n, int64_t width, int6
  *               grad already holds the gradient for an upstream of 1, and nothing is written
  *               if it is 1.
  *   sequences   seq_offsets [n_seqs + 1] of offsets_dtype (rows seq_offsets[s] up to
- *               seq_offsets[s + 1]; clamped to 0..n; rows of no sequence do not count), or
- *               NULL: n_seqs sequences of seq_len rows each
+ *               seq_offsets[s + 1], ascending; clamped to 0..n; rows of no sequence do not
+ *               count), or NULL: n_seqs sequences of seq_len rows each. Offsets that descend
+ *               make sequences overlap, and values of the rows they share that are not defined.
  *   workspace   me_loss_workspace_size(n, vocab, pairs or 0, top or 0) bytes, 16-byte aligned
  */
 #define ME_REDUCE_MEAN 0     /* over the rows that count */

@@ -3,12 +3,13 @@
 //
 // Bound by HBM: 2 bytes read and 2 written per bf16 logit, where two sweeps (losses.hip) move 6. A CU has 512 KB of
 // registers and 160 KB of LDS: a row of 262,144 bf16 logits is 512 KB, of which 1024 threads hold 22 16-byte slots each
-// in registers (88 of the 128 that 16 wavefronts leave a thread) and 9 in LDS; what is beyond is read a second time. A
-// row's slots are all requested before the first is used, so the whole row is in flight at once.
+// in registers (88 of the 128 that 16 wavefronts leave a thread: all are taken, and up to 4 values are in scratch) and 9
+// in LDS; what is beyond is read a second time. A row's slots are all requested before the first is used, so the whole
+// row is in flight at once.
 //
-// Measured (policy, all rows counting): 8192 rows of 262,144 bf16 logits 1690-1760 us (4.9-5.1 TB/s: one row per CU,
-// whose read and sum, 28 us, and write follow each other), of 131,072 770 us (5.6), of 32,000 165-195 us (5.4-6.4,
-// several rows per CU), 8192 rows of 50,021 fp32 logits 600 us (5.5).
+// Measured (policy, all rows counting): 8192 rows of 262,144 bf16 logits 1690-1920 us (4.5-5.1 TB/s: one row per CU,
+// whose read and sum, 28 us, and write follow each other), of 131,072 775 us (5.5), of 32,000 165-205 us (5.1-6.4,
+// several rows per CU), 8192 rows of 50,021 fp32 logits 610 us (5.4).
 #include "loss_common.h"
 
 namespace me {
@@ -373,7 +374,9 @@ void launch_pass_of(Op op, const RowArgs &a, void *grad, hipStream_t s) {
             return pass_kernel<T, kThreads, kRegs, kLds, kStream, kPreference, false><<<n, kThreads, 0, s>>>(a, nullptr);
     }
     if (op == kPolicy) pass_kernel<T, kThreads, kRegs, kLds, kStream, kPolicy, false><<<n, kThreads, 0, s>>>(a, grad);
-    else if constexpr (kRegs <= 16 || kLds > 0) {  // (with 22 slots in registers alone, leaving entries out spills)
+    else if constexpr (kRegs <= 16 || kLds > 0) {
+        // (with 22 slots in registers alone, leaving entries out spills 32 registers, fp32 54; the variants of 1024
+        // threads that are launched spill 4 at most)
         if (a.teacher_lse != nullptr)
             pass_kernel<T, kThreads, kRegs, kLds, kStream, kDistill, true><<<n, kThreads, 0, s>>>(a, grad);
         else pass_kernel<T, kThreads, kRegs, kLds, kStream, kDistill, false><<<n, kThreads, 0, s>>>(a, grad);

@@ -26,8 +26,8 @@ namespace {
 
 // The weight of a row: 1 over the rows that count (kMean), 1 (kSum), or 1 over the row's sequence's counting rows
 // and the sequences that have any (kSequence); 0 for a row that does not count. Made by one workgroup, bound by the
-// latency of its loads, hence eight of them in flight per thread: 5.6 us alone for 8192 rows, 7.7 for 3885 by
-// sequences.
+// latency of its loads, hence eight of them in flight per thread: 5.7-6.1 us alone for 8192 rows, 7.6-8.7 for 3885
+// in 5 sequences, a wavefront each.
 template <typename I>
 __device__ int64_t count_rows(const WeightArgs &a) {
     const bool of_ids = a.ids != nullptr;
@@ -125,7 +125,8 @@ struct StatsArgs {
 // by the bytes of the logits: the rows of 8 x 511 with a target, 1.6 GB of bf16 logits, take 231 us, 7.0 TB/s (a device
 // copy of 4 GB moves 4.9, a fill 6.8). For that the loads go past the caches (262 us otherwise), four 16-byte ones
 // (fp32: eight) per thread are in flight, and a logit costs one multiply-add, one exponential and one addition (Guess).
-// The workgroup past the last part makes the rows' weights meanwhile.
+// The workgroup past the last part makes the rows' weights: beside the others where all are resident at one time (2048
+// of 256 threads), behind them in larger grids.
 template <typename T, int kThreads, bool kLeaveOut>
 __global__ __launch_bounds__(kThreads) void stats_kernel(const StatsArgs a) {
     const int64_t parts = a.logits.n * a.splits;
@@ -246,7 +247,7 @@ __global__ __launch_bounds__(kThreads) void stats_kernel(const StatsArgs a) {
 }
 
 // A wavefront per row: joins the parts' (m, s), then the loss's own few values. A chain of a few dependent loads per
-// row, whatever its length: 2.5 us for one row, 4.7 for 4088, 8.7 for 8286.
+// row, whatever its length: 3.1 us for one row, 5.4-5.6 for 4088, 8.2-8.6 for 8286.
 template <Op kOp, bool kBf16>
 __global__ __launch_bounds__(kOp == kDistill ? 256 : 1024) void row_kernel(const RowArgs a) {
     constexpr int kWaves = kOp == kDistill ? 4 : 16;
@@ -353,7 +354,7 @@ __global__ __launch_bounds__(256) void entries_kernel(const RowArgs a) {
 }
 
 // Adds the workgroups' or rows' sums in a fixed order. One workgroup, bound by the latency of its loads: with four rows
-// in flight per thread three sums of 8192 rows take 7.0 us, one after the other 12.2.
+// in flight per thread three sums of 8192 rows take 6.7-7.0 us, one after the other 12.2.
 template <int kParts>
 __global__ __launch_bounds__(1024) void total_kernel(const double *sums, int64_t count, const float *counted, float scale,
                                                     float *loss, float *out_stats) {
@@ -772,7 +773,8 @@ void launch_rows(const RowArgs &a, int dtype, hipStream_t s) {
 template <typename T, int kThreads>
 void launch_grad_of(const GradArgs &a, bool stream_out, hipStream_t s) {
     // a workgroup per part; where most likely nothing is left to do, no more than fill the GPU twice (65,536 workgroups
-    // that end at once take 15 us, 4096 take 4)
+    // that end at once take 15 us, 4096 take 4; where something is, they take 1450 us for 8192 rows of 262,144 of which
+    // a fifth do not count)
     const int64_t parts = a.logits.n * a.splits;
     const unsigned blocks = static_cast<unsigned>(a.done_for_one && parts > 4096 ? 4096 : parts);
     if (stream_out) grad_kernel<T, kThreads, true><<<blocks, kThreads, 0, s>>>(a);

@@ -200,8 +200,8 @@ def preference_loss(logits, targets, ref_logps, cu_seqlens=None, beta=0.1, loss_
     (log-probability - ref_logps), or their mean with length_normalized; the rewards are beta D and
     carry no gradient.
 
-    Sequences are the rows of `targets`' last dim, or with cu_seqlens [sequences + 1] the rows packed back
-    to back; the first half of them are the chosen answers, the second half the rejected ones in the same
+    Sequences are the rows of `targets`' last dim, or with cu_seqlens [sequences + 1] (ascending) the rows packed
+    back to back; the first half of them are the chosen answers, the second half the rejected ones in the same
     order. ref_logps: the reference's log-probabilities of the same targets (token_logps), token by token:
     differences of single tokens lose nothing, where those of whole sequences' sums would.
 
@@ -285,8 +285,9 @@ def policy_loss(logits, targets, old_logps, advantages, ref_logps=None, cu_seqle
     old = _per_row(old_logps, targets.shape, "old_logps")
     ref = None if ref_logps is None else _per_row(ref_logps, targets.shape, "ref_logps")
     per_seq = advantages.shape != targets.shape
+    # one for each of targets.shape[:-1] only where these are all sequences: cu_seqlens may name more than they hold
     if per_seq and (advantages.numel() != n_seqs or tuple(advantages.shape) not in
-                    ((n_seqs,), (n_seqs, 1), (*targets.shape[:-1], 1))):  # (the last of as many sequences as rows of targets)
+                    ((n_seqs,), (n_seqs, 1), (*targets.shape[:-1], 1))):
         raise ValueError(f"[micro_engram] advantages {tuple(advantages.shape)} are neither the rows' "
                          f"{tuple(targets.shape)} nor one for each of {n_seqs} sequences")
     adv = _per_row(advantages, advantages.shape, "advantages")
