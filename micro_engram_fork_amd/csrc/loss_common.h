@@ -10,7 +10,6 @@ namespace me {
 namespace loss {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kInf = __builtin_huge_valf();
 constexpr int kMaxSplits = 64;      // parts of a row whose (m, s) one wavefront joins, a lane each
 constexpr int kMaxSpan = 32768;     // logits of one part
