@@ -1,5 +1,6 @@
 """The losses over logits where a call is out of the ordinary: tensor subclasses among the arguments, hooks on what a
-backward keeps."""
+backward keeps, values past fp32 and NaN, sums that nearly cancel, no rows, as many rows as a launch holds and batches of
+many; and the distillation loss at each width of the kernels that keep a row."""
 import math
 
 import pytest
