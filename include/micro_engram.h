@@ -477,6 +477,33 @@ int me_sparse_adam(int32_t n_tables, void *const *params, void *const *exp_avgs,
                    int stochastic_rounding, uint64_t seed, void *stream);
 
 /*
+ * me_adamw -- one AdamW step of n_tensors dense tensors: what torch.optim.AdamW does for the engram's
+ * projections and scales in the reference's trainer (state layout micro_engram/optim.py:47-63).
+ *
+ *   m = beta1 m + (1 - beta1) g        v = beta2 v + (1 - beta2) g^2
+ *   p = (1 - lr weight_decay) p - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ *
+ *   HOST arrays [n_tensors]: params (device, param_dtype), grads (device, grad_dtype), exp_avgs and
+ *   exp_avg_sqs (device; state_bits 32: fp32, 8: e4m3 and e5m2 bytes), numels, stream_ids (distinct per
+ *   tensor: selects its rounding noise). Tensors may start at any multiple of their element size.
+ *   exp_avg_scales, exp_avg_sq_scales  state_bits 8: device [ceil(numel / 128)] E8M0 bytes, the power of
+ *               two that 128 values share; else NULL
+ *   steps       HOST [n_tensors]: the step counts t after this step; or NULL and
+ *   device_steps  HOST array of device fp32 scalars, which the call increments first (replays of a
+ *               captured call then count on)
+ * bf16 weights are rounded stochastically when stochastic_rounding != 0, 8-bit moments always; an
+ * exp_avg_sq over zero stays over zero. The noise of the eight values from 8 k on is Philox4x32-10 keyed by seed
+ * with counter (k low, k high, t, stream_id), 16 bits each: r for the weight, r rotated by eight bits for
+ * exp_avg, 65535 - r for exp_avg_sq. Moments that are not finite become NaN.
+ */
+int me_adamw(int32_t n_tensors, void *const *params, const void *const *grads, void *const *exp_avgs,
+             void *const *exp_avg_sqs, void *const *exp_avg_scales, void *const *exp_avg_sq_scales,
+             const int64_t *numels, const double *steps, float *const *device_steps,
+             const int32_t *stream_ids, int param_dtype, int grad_dtype, int state_bits, double lr,
+             double beta1, double beta2, double eps, double weight_decay, int stochastic_rounding,
+             uint64_t seed, void *stream);
+
+/*
  * me_stochastic_bf16 -- fp32 -> bf16 with stochastic rounding (micro_engram/optim.py:33-44):
  * the 16-bit noise is added to the fp32 bit pattern below the kept bits, then the low 16 bits
  * are dropped; inf and NaN convert as usual. Element i takes the me_sparse_adam noise of

@@ -66,6 +66,8 @@ SIGNATURES = {
     "me_sparse_adam": [c_i32, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_int, c_ptr, c_ptr, c_ptr, c_i32, c_int,
                        c_int, c_int, c_int, c_double, c_double, c_double, c_double, c_double,
                        c_int, ctypes.c_uint64, c_ptr],
+    "me_adamw": [c_i32, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_int, c_int, c_int,
+                 c_double, c_double, c_double, c_double, c_double, c_int, ctypes.c_uint64, c_ptr],
     "me_clip_scale": [c_ptr, c_int, c_i64, c_ptr, c_double, c_ptr],
     "me_stochastic_bf16": [c_ptr, c_i64, c_ptr, ctypes.c_uint64, ctypes.c_uint32, ctypes.c_uint32,
                            c_ptr],
@@ -143,6 +145,10 @@ def i32_array(values):
 
 def i64_array(values):
     return (c_i64 * len(values))(*values)
+
+
+def f64_array(values):
+    return (c_double * len(values))(*values)
 
 
 def ptr_array(values):

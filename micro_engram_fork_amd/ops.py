@@ -13,7 +13,7 @@ from typing import List, Optional, Sequence
 import torch
 
 from . import _lib
-from ._lib import ME_BF16, ME_F32, ME_I32, ME_I64, ME_U8, call, i32_array, i64_array, ptr_array
+from ._lib import ME_BF16, ME_F32, ME_I32, ME_I64, ME_U8, call, f64_array, i32_array, i64_array, ptr_array
 
 _DTYPES = {torch.int32: ME_I32, torch.int64: ME_I64, torch.float32: ME_F32,
            torch.bfloat16: ME_BF16, torch.bool: ME_U8, torch.uint8: ME_U8}
@@ -1009,6 +1009,27 @@ def sparse_adam_launch(dev, param_ptrs, exp_avg_ptrs, exp_avg_sq_ptrs, n, dim, d
          int(bool(rowwise)), sq_dtype, int(bool(lazy)), float(lr), float(betas[0]), float(betas[1]),
          float(eps), float(weight_decay), int(bool(stochastic_rounding)), int(seed) & ((1 << 64) - 1),
          stream_of(dev))
+
+
+def call_on(dev, name, *args):
+    """call(name, *args, stream): on dev's current stream, with dev the current device (the default stream's
+    handle is that of whichever device is current)."""
+    index = dev.index
+    if index is None or index == torch._C._cuda_getDevice():
+        call(name, *args, stream_of(dev))
+    else:
+        with torch.cuda.device(index):
+            call(name, *args, stream_of(dev))
+
+
+def adamw_launch(dev, n, arrays, grads, numels, steps, device_steps, stream_ids, dtype, grad_dtype, state_bits, *, lr,
+                 betas, eps, weight_decay, stochastic_rounding, seed):
+    """One AdamW step of n tensors from pointer arrays (ctypes) that a caller has checked: arrays are those of the
+    parameters, exp_avg, exp_avg_sq and, for 8-bit moments, their scales (else None)."""
+    params, exp_avgs, exp_avg_sqs, scales, sq_scales = arrays
+    call_on(dev, "me_adamw", n, params, grads, exp_avgs, exp_avg_sqs, scales, sq_scales, numels, steps, device_steps,
+            stream_ids, dtype, grad_dtype, state_bits, float(lr), float(betas[0]), float(betas[1]), float(eps),
+            float(weight_decay), int(bool(stochastic_rounding)), int(seed) & ((1 << 64) - 1))
 
 
 def stochastic_bf16(x, seed, step=0, stream_id=0):

@@ -12,7 +12,12 @@ parameter group with the same layout in one launch. bf16 weights and moments are
 with stochastic rounding whose noise comes from a counter-based generator (Philox4x32-10 keyed
 by `seed`, the table's step and the element's position) instead of torch.randint: the same
 rounding distribution, reproducible for a given seed.
+
+DenseAdamW is plain AdamW for everything else that is trained (the engrams' projections and scales, a
+decoder's weights): all tensors of a group in one launch per 42 of them, moments in fp32 or in 8 bits.
 """
+import math
+
 import torch
 
 from . import ops
@@ -64,7 +69,81 @@ class SparseBatch:
         return batch, ks
 
 
-class LazyAdamW(torch.optim.Optimizer):
+class _DirectOptimizer(torch.optim.Optimizer):
+    """What the optimizers here share: step counters of a group in one buffer, and step and zero_grad
+    without torch.optim's profiler ranges. A subclass has _step(closure=None)."""
+
+    def _advance_steps(self, gi, group, live):
+        """Adds 1 to the step counter of every live parameter and returns the new values. The
+        counters are CPU tensors, as torch.optim.AdamW keeps them; those of a group are views
+        into one buffer of the group (adopted on first sight, and again after anything put a
+        tensor of its own in their place, e.g. load_state_dict), so the usual step -- every
+        parameter live -- is one add and one host read."""
+        bufs = self.__dict__.setdefault("_step_bufs", {})
+        params = group["params"]
+        entry = bufs.get(gi)
+        if entry is None or entry[2] != tuple(id(p) for p in params):
+            buf = torch.zeros(len(params), dtype=torch.float32)
+            entry = bufs[gi] = (buf, [buf[i] for i in range(len(params))], tuple(id(p) for p in params))
+        buf, views, _ = entry
+        if len(live) == len(params) and all(a is b for a, b in zip(live, params)):
+            states = [self.state[p] for p in params]
+            for i, st in enumerate(states):
+                if st["step"] is not views[i]:
+                    step = st["step"]
+                    if step.device.type != "cpu" or step.numel() != 1:
+                        step = step.detach().reshape(()).cpu()
+                    views[i].copy_(step.float())
+                    st["step"] = views[i]
+            buf.add_(1)
+            return buf.tolist()
+        counters = [self.state[p]["step"] for p in live]
+        for c in counters:
+            c.add_(1)
+        return [float(c) for c in counters]
+
+    def step(self, *args, **kwargs):
+        """One step (closure: optional, as torch.optim's). torch.optim wraps an optimizer's step
+        in a profiler range and its step hooks; that range is a dispatched op (~25 us of host
+        time per step, paid with no profiler running, on a training step bound by its host's
+        issue rate), so this optimizer runs the hooks itself, with the same order and return
+        rules, and opens the range only while the autograd profiler is on."""
+        if torch.autograd.profiler._is_profiler_enabled:
+            with torch.autograd.profiler.record_function(f"Optimizer.step#{type(self).__name__}.step"):
+                return self._hooked_step(args, kwargs)
+        return self._hooked_step(args, kwargs)
+
+    step.hooked = True  # torch.optim.Optimizer leaves a step marked so unwrapped
+
+    def _hooked_step(self, args, kwargs):
+        from torch.optim.optimizer import _global_optimizer_post_hooks, _global_optimizer_pre_hooks
+
+        for pre_hook in (*_global_optimizer_pre_hooks.values(), *self._optimizer_step_pre_hooks.values()):
+            result = pre_hook(self, args, kwargs)
+            if result is not None:
+                if isinstance(result, tuple) and len(result) == 2:
+                    args, kwargs = result
+                else:
+                    raise RuntimeError(f"optimizer step pre-hooks must return None or a tuple of "
+                                       f"(new_args, new_kwargs), but got {result}.")
+        out = self._step(*args, **kwargs)
+        self._optimizer_step_code()
+        for post_hook in (*self._optimizer_step_post_hooks.values(), *_global_optimizer_post_hooks.values()):
+            post_hook(self, args, kwargs)
+        return out
+
+    def zero_grad(self, set_to_none=True):
+        """torch.optim's zero_grad; with set_to_none (the default) without its profiler range
+        (opened only while the autograd profiler is on, as for step)."""
+        if not set_to_none or torch.autograd.profiler._is_profiler_enabled:
+            return super().zero_grad(set_to_none)
+        for group in self.param_groups:
+            for p in group["params"]:
+                if p.grad is not None:
+                    p.grad = None
+
+
+class LazyAdamW(_DirectOptimizer):
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, lazy=False,
                  rowwise=False, stochastic_rounding=True, seed=None):
         """stochastic_rounding: bf16 weights and states are written back with stochastic rounding
@@ -156,35 +235,6 @@ class LazyAdamW(torch.optim.Optimizer):
         plan = plans[gi] = {"key": key, "members": members, "batches": list(batches.values())}
         return plan
 
-    def _advance_steps(self, gi, group, live):
-        """Adds 1 to the step counter of every live parameter and returns the new values. The
-        counters are CPU tensors, as torch.optim.AdamW keeps them; those of a group are views
-        into one buffer of the group (adopted on first sight, and again after anything put a
-        tensor of its own in their place, e.g. load_state_dict), so the usual step -- every
-        parameter live -- is one add and one host read."""
-        bufs = self.__dict__.setdefault("_step_bufs", {})
-        params = group["params"]
-        entry = bufs.get(gi)
-        if entry is None or entry[2] != tuple(id(p) for p in params):
-            buf = torch.zeros(len(params), dtype=torch.float32)
-            entry = bufs[gi] = (buf, [buf[i] for i in range(len(params))], tuple(id(p) for p in params))
-        buf, views, _ = entry
-        if len(live) == len(params) and all(a is b for a, b in zip(live, params)):
-            states = [self.state[p] for p in params]
-            for i, st in enumerate(states):
-                if st["step"] is not views[i]:
-                    step = st["step"]
-                    if step.device.type != "cpu" or step.numel() != 1:
-                        step = step.detach().reshape(()).cpu()
-                    views[i].copy_(step.float())
-                    st["step"] = views[i]
-            buf.add_(1)
-            return buf.tolist()
-        counters = [self.state[p]["step"] for p in live]
-        for c in counters:
-            c.add_(1)
-        return [float(c) for c in counters]
-
     @staticmethod
     def _batch_pointers(b, live, step_of):
         """The launch's row / gradient pointer arrays straight from a SparseBatch when every
@@ -207,46 +257,6 @@ class LazyAdamW(torch.optim.Optimizer):
         rb, gb = rows.data_ptr(), sums.data_ptr()
         return ([rows, sums], [rb + bnd[k] * 8 for k in ks], [gb + bnd[k] * dim * 4 for k in ks],
                 [bnd[k + 1] - bnd[k] for k in ks], [int(step_of[i]) for i in b["pos"]])
-
-    def step(self, *args, **kwargs):
-        """One step (closure: optional, as torch.optim's). torch.optim wraps an optimizer's step
-        in a profiler range and its step hooks; that range is a dispatched op (~25 us of host
-        time per step, paid with no profiler running, on a training step bound by its host's
-        issue rate), so this optimizer runs the hooks itself, with the same order and return
-        rules, and opens the range only while the autograd profiler is on."""
-        if torch.autograd.profiler._is_profiler_enabled:
-            with torch.autograd.profiler.record_function(f"Optimizer.step#{type(self).__name__}.step"):
-                return self._hooked_step(args, kwargs)
-        return self._hooked_step(args, kwargs)
-
-    step.hooked = True  # torch.optim.Optimizer leaves a step marked so unwrapped
-
-    def _hooked_step(self, args, kwargs):
-        from torch.optim.optimizer import _global_optimizer_post_hooks, _global_optimizer_pre_hooks
-
-        for pre_hook in (*_global_optimizer_pre_hooks.values(), *self._optimizer_step_pre_hooks.values()):
-            result = pre_hook(self, args, kwargs)
-            if result is not None:
-                if isinstance(result, tuple) and len(result) == 2:
-                    args, kwargs = result
-                else:
-                    raise RuntimeError(f"optimizer step pre-hooks must return None or a tuple of "
-                                       f"(new_args, new_kwargs), but got {result}.")
-        out = self._step(*args, **kwargs)
-        self._optimizer_step_code()
-        for post_hook in (*self._optimizer_step_post_hooks.values(), *_global_optimizer_post_hooks.values()):
-            post_hook(self, args, kwargs)
-        return out
-
-    def zero_grad(self, set_to_none=True):
-        """torch.optim's zero_grad; with set_to_none (the default) without its profiler range
-        (opened only while the autograd profiler is on, as for step)."""
-        if not set_to_none or torch.autograd.profiler._is_profiler_enabled:
-            return super().zero_grad(set_to_none)
-        for group in self.param_groups:
-            for p in group["params"]:
-                if p.grad is not None:
-                    p.grad = None
 
     @torch.no_grad()
     def prepare_step(self):
@@ -370,5 +380,219 @@ class LazyAdamW(torch.optim.Optimizer):
                 # the kernel wrote through raw pointers: move the version counters as torch's
                 # own in-place ops would (autograd's saved-tensor checks and caches keyed on
                 # them then see the update) (p itself: p.data has a version counter of its own)
+                torch.autograd.graph.increment_version(b["written"])
+        return loss
+
+
+class DenseAdamW(_DirectOptimizer):
+    """AdamW (torch.optim.AdamW's formula) over many dense tensors at once.
+
+        opt = DenseAdamW(model.parameters(), lr=1e-4, weight_decay=0.1, state_bits=8)
+        loss.backward(); opt.step(); opt.zero_grad()
+
+    Parameters are bf16 or fp32, contiguous, on a GPU; gradients p.grad, or p.fp32_grad in its place where that is
+    set: an fp32 tensor of p's shape in which a program sums several backwards (torch lets a bf16 p.grad be bf16
+    only). A parameter with neither stays as it is. bf16 weights are written back with stochastic rounding
+    (stochastic_rounding=False: to nearest).
+
+    state_bits 32: exp_avg and exp_avg_sq are fp32, whatever the parameter is. 8: exp_avg is float8_e4m3fn and
+    exp_avg_sq float8_e5m2, each with one float8_e8m0fnu scale (exp_avg_scale, exp_avg_sq_scale) for every 128
+    values in memory order; a moment is value * scale. They are always rounded stochastically: to nearest, a second
+    moment would not move, as its changes are far smaller than its steps. A value that is not finite makes its own
+    moments NaN, not its neighbours'.
+
+    The rounding noise is a function of (seed, step count, position of the parameter in the optimizer, place in the
+    parameter); seed None draws one from torch's default generator.
+
+    capturable: step counts live on the GPU and the step may be captured in a graph, with the hyperparameters and
+    gradient tensors of the capture; the states have to exist by then (one step outside, or load_state_dict).
+    Without it a step under capture is refused, since replays would repeat one step count."""
+
+    BLOCK = 128  # values per scale of 8-bit moments
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32,
+                 stochastic_rounding=True, seed=None, capturable=False):
+        if state_bits not in (32, 8):
+            raise ValueError(f"[micro_engram] DenseAdamW: state_bits of {state_bits!r}: 32 or 8")
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
+                                      stochastic_rounding=stochastic_rounding, capturable=capturable))
+        self.seed = int(torch.randint(0, 2**62, (1,)).item()) if seed is None else int(seed)
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        try:
+            self._check_group(self.param_groups[-1])
+        except Exception:
+            del self.param_groups[-1]
+            raise
+
+    @staticmethod
+    def _check_group(group):
+        for name, low, high in (("lr", 0.0, math.inf), ("eps", 0.0, math.inf), ("weight_decay", 0.0, math.inf)):
+            if not low <= float(group[name]) < high:
+                raise ValueError(f"[micro_engram] DenseAdamW: {name} of {group[name]} is out of range")
+        if len(group["betas"]) != 2 or not all(0.0 <= float(b) < 1.0 for b in group["betas"]):
+            raise ValueError(f"[micro_engram] DenseAdamW: betas of {group['betas']} are out of range")
+        if group["state_bits"] not in (32, 8):
+            raise ValueError(f"[micro_engram] DenseAdamW: state_bits of {group['state_bits']!r}: 32 or 8")
+        for p in group["params"]:
+            if p.dtype not in (torch.bfloat16, torch.float32):
+                raise TypeError(f"[micro_engram] DenseAdamW: parameters must be bf16 or fp32, got {p.dtype}")
+
+    @staticmethod
+    def init_state(state, p, group):
+        """Fresh state of p."""
+        state["step"] = torch.zeros((), dtype=torch.float32, device=p.device if group["capturable"] else "cpu")
+        for name, kind in (("exp_avg", torch.float8_e4m3fn), ("exp_avg_sq", torch.float8_e5m2)):
+            if group["state_bits"] == 32:
+                state[name] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+                continue
+            state[name] = torch.zeros(p.shape, dtype=torch.uint8, device=p.device).view(kind)
+            blocks = -(-p.numel() // DenseAdamW.BLOCK)
+            state[name + "_scale"] = torch.zeros(blocks, dtype=torch.uint8, device=p.device).view(torch.float8_e8m0fnu)
+
+    def load_state_dict(self, state_dict):
+        """torch.optim's load, which casts floating states to their parameter's dtype: the moments are put back as they
+        were saved."""
+        saved = state_dict["state"]
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        super().load_state_dict(state_dict)
+        for group in self.param_groups:
+            self._check_group(group)
+        for i, (p, group) in zip(ids, [(p, g) for g in self.param_groups for p in g["params"]]):
+            for name, value in saved.get(i, {}).items():
+                if name == "step":
+                    where = p.device if group["capturable"] else "cpu"
+                    value = torch.as_tensor(value, dtype=torch.float32).detach().reshape(())
+                    self.state[p][name] = value.to(device=where, copy=True)
+                elif torch.is_tensor(value):
+                    self.state[p][name] = value.detach().to(device=p.device, copy=True).contiguous()
+        self._plans = {}
+
+    _STATES = ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")
+
+    def _plan(self, gi, group, live):
+        """As LazyAdamW's launch plan: the pointer arrays of group gi's launches that stay put between steps, per
+        (device, parameter dtype, gradient dtype), kept while parameters, their storage and their states are
+        the same tensors. live: [(parameter, gradient, gradient dtype)]."""
+        plans = self.__dict__.setdefault("_plans", {})
+        plan = plans.get(gi)
+        eight = group["state_bits"] == 8
+        names = self._STATES[:4 if eight else 2]
+        if plan is not None and len(plan["members"]) == len(live):
+            for (p, _, kind), (q, ptr, n, was, states) in zip(live, plan["members"]):
+                s = self.state[p]
+                if p is not q or p.data_ptr() != ptr or p.numel() != n or kind is not was or any(
+                        s.get(k) is not t for k, t in zip(names, states)):
+                    break
+            else:
+                if plan["eight"] == eight:
+                    return plan
+        index = {id(p): i for i, p in enumerate(p for g in self.param_groups for p in g["params"])}
+        members, batches = [], {}
+        for i, (p, g, kind) in enumerate(live):
+            state = self.state[p]
+            states = tuple(state.get(k) for k in names)
+            self._check_state(p, states, eight)
+            members.append((p, p.data_ptr(), p.numel(), kind, states))
+            b = batches.setdefault((p.device, p.dtype, kind), {"pos": [], "ptr": [[] for _ in range(5)], "n": [], "ids": [],
+                                                               "written": []})
+            b["pos"].append(i)
+            for at, t in zip(b["ptr"], (p, *states)):
+                at.append(t.data_ptr())
+            b["n"].append(p.numel())
+            b["ids"].append(index[id(p)])
+            b["written"] += [p, *states]
+        for (device, dtype, kind), b in batches.items():
+            b.update(device=device, dtype=ops.dtype_code(torch.empty(0, dtype=dtype)),
+                     grad_dtype=ops.dtype_code(torch.empty(0, dtype=kind)),
+                     arrays=[ops.ptr_array(x) if x else None for x in b["ptr"]], n=ops.i64_array(b["n"]),
+                     ids=ops.i32_array(b["ids"]))
+        plan = plans[gi] = {"members": members, "batches": list(batches.values()), "eight": eight}
+        return plan
+
+    def _check_state(self, p, states, eight):
+        ops.require_gpu(p, *states)
+        if not p.is_contiguous() or not all(t is not None and t.is_contiguous() for t in states):
+            raise ValueError("[micro_engram] DenseAdamW: parameters and their state must be contiguous")
+        kinds = (torch.float8_e4m3fn, torch.float8_e5m2) if eight else (torch.float32, torch.float32)
+        if any(t.shape != p.shape or t.dtype is not k for t, k in zip(states, kinds)) or any(
+                t.numel() != -(-p.numel() // self.BLOCK) or t.dtype is not torch.float8_e8m0fnu for t in states[2:]):
+            raise ValueError("[micro_engram] DenseAdamW: optimizer state does not match its parameter")
+
+    @staticmethod
+    def _gradient(p):
+        """(p's gradient, its dtype) as the kernel reads it."""
+        g = getattr(p, "fp32_grad", None)
+        if g is None:
+            g = p.grad
+            if g.is_sparse or g.layout is not torch.strided:
+                raise ValueError("[micro_engram] DenseAdamW: gradients must be dense (rows of tables: LazyAdamW)")
+        elif g.dtype is not torch.float32:
+            raise TypeError(f"[micro_engram] DenseAdamW: fp32_grad must be fp32, got {g.dtype}")
+        if g.shape != p.shape or g.device != p.device:
+            raise ValueError("[micro_engram] DenseAdamW: a gradient must have its parameter's shape and device")
+        if not g.is_contiguous():
+            g = g.contiguous()
+        return g, g.dtype
+
+    def zero_grad(self, set_to_none=True):
+        super().zero_grad(set_to_none)
+        for group in self.param_groups:
+            for p in group["params"]:
+                g = getattr(p, "fp32_grad", None)
+                if g is not None:
+                    if set_to_none:
+                        p.fp32_grad = None
+                    else:
+                        g.zero_()
+
+    @torch.no_grad()
+    def _step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for gi, group in enumerate(self.param_groups):
+            live = []
+            for p in group["params"]:
+                if getattr(p, "sparse_grad", None) is not None:
+                    raise ValueError("[micro_engram] DenseAdamW: sparse row gradients need LazyAdamW")
+                if p.grad is not None or getattr(p, "fp32_grad", None) is not None:
+                    live.append((p, *self._gradient(p)))
+            if not live:
+                continue
+            if not all(p.is_cuda for p, _, _ in live):
+                ops.require_gpu(*(p for p, _, _ in live))
+            capturable = bool(group["capturable"])
+            if torch.cuda.is_current_stream_capturing() and (
+                    not capturable or not all(self.state[p] for p, _, _ in live)):
+                raise RuntimeError("[micro_engram] DenseAdamW: a step under graph capture needs capturable=True and "
+                                   "states that exist already")
+            for p, _, _ in live:
+                if not self.state[p]:
+                    self.init_state(self.state[p], p, group)
+            plan = self._plan(gi, group, live)
+            if capturable:
+                counts = None
+                for p, _, _ in live:
+                    step = self.state[p]["step"]
+                    if step.device != p.device or step.dtype is not torch.float32 or step.numel() != 1:
+                        raise ValueError("[micro_engram] DenseAdamW: capturable step counts are fp32 scalars on the GPU")
+            else:
+                counts = self._advance_steps(gi, group, [p for p, _, _ in live])
+            for b in plan["batches"]:
+                pos, arrays = b["pos"], b["arrays"]
+                grads = ops.ptr_array([live[i][1].data_ptr() for i in pos])
+                steps = device_steps = None
+                if counts is not None:
+                    steps = ops.f64_array([counts[i] for i in pos])
+                else:
+                    device_steps = ops.ptr_array([self.state[live[i][0]]["step"].data_ptr() for i in pos])
+                ops.adamw_launch(b["device"], len(pos), arrays, grads, b["n"], steps, device_steps, b["ids"], b["dtype"],
+                                 b["grad_dtype"], group["state_bits"], lr=group["lr"], betas=group["betas"],
+                                 eps=group["eps"], weight_decay=group["weight_decay"],
+                                 stochastic_rounding=group["stochastic_rounding"], seed=self.seed)
+                # written through raw pointers: as LazyAdamW
                 torch.autograd.graph.increment_version(b["written"])
         return loss
