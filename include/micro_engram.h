@@ -671,6 +671,60 @@ int me_distill_backward(const void *logits, int dtype, int64_t n, int64_t vocab,
                         const float *row_stats, const float *coef, const float *fix,
                         const float *upstream, int done_for_one, void *grad, void *stream);
 
+/* ---- losses over a decoder's head, without its logits ------------------------------------
+ * The reference trains with a cross-entropy in pieces of its logits (micro_engram/train/head.py:85-165);
+ * here the logits z = hidden weight^T / temperature exist a tile at a time. Common arguments:
+ *
+ *   hidden      [n, dim] of dtype (ME_BF16 / ME_F32), laid out as logits' rows above; dim <= 65536,
+ *               n <= 2^24
+ *   weight      [vocab, dim] of the same dtype, rows w_stride (>= dim) elements apart; vocab <= 2^21.
+ *               bf16 rows that start at multiples of 16 bytes are read where they lie, others and
+ *               fp32 ones are laid out a piece at a time
+ *   targets, ignore_index, temperature  as above; nothing of a row that does not count is read
+ *   saved       [16 + 4 n] 4-byte elements (16-byte aligned): what the backward needs
+ *   workspace   me_head_workspace_size bytes for the same n, vocab, dim, dtype, weight and w_stride, with
+ *               backward != 0 for me_head_backward; 16-byte aligned
+ * bf16 products accumulate in fp32; fp32 ones are made of bf16 parts that add up to the operands, with
+ * the accuracy of fp32 products.
+ */
+int me_head_workspace_size(int64_t n, int64_t vocab, int64_t dim, int dtype, const void *weight,
+                           int64_t w_stride, int backward, size_t *bytes);
+
+/*
+ * me_head_logps -- logps[r] = log softmax(z[r])[targets[r]], fp32; 0 where a row does not count.
+ */
+int me_head_logps(const void *hidden, int dtype, int64_t n, int64_t dim, int64_t rows_per_batch,
+                  int64_t batch_stride, int64_t row_stride, const void *weight, int64_t vocab,
+                  int64_t w_stride, const void *targets, int targets_dtype, int64_t ignore_index,
+                  double temperature, float *logps, void *saved, void *workspace,
+                  size_t workspace_bytes, void *stream);
+
+/*
+ * me_head_ce -- loss = scale * sum (or mean) over the rows that count of
+ *   lse - (1 - smoothing) z[target] - smoothing / vocab sum_j z[j] + z_loss lse^2,
+ * lse the log of the sum of exp(z). No such rows: 0.
+ */
+int me_head_ce(const void *hidden, int dtype, int64_t n, int64_t dim, int64_t rows_per_batch,
+               int64_t batch_stride, int64_t row_stride, const void *weight, int64_t vocab,
+               int64_t w_stride, const void *targets, int targets_dtype, int64_t ignore_index,
+               double temperature, double smoothing, double z_loss, double scale, int reduction,
+               float *loss, void *saved, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * me_head_backward -- gradients of me_head_logps (upstream_per_row != 0: upstream [n] fp32, the
+ * log-probabilities' gradient; scale 1) or of me_head_ce (upstream: device scalar; its other
+ * arguments as given there), with what that call left in saved.
+ *   grad_hidden  nullable, [n, dim] contiguous, zeros in rows that do not count
+ *   grad_weight  nullable, [vocab, dim] contiguous; both of dtype and 16-byte aligned
+ */
+int me_head_backward(const void *hidden, int dtype, int64_t n, int64_t dim, int64_t rows_per_batch,
+                     int64_t batch_stride, int64_t row_stride, const void *weight, int64_t vocab,
+                     int64_t w_stride, const void *targets, int targets_dtype, int64_t ignore_index,
+                     double temperature, const float *upstream, int upstream_per_row,
+                     double smoothing, double z_loss, double scale, int reduction,
+                     const void *saved, void *grad_hidden, void *grad_weight, void *workspace,
+                     size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -29,7 +29,7 @@ import math
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import loss_ops
+from . import head_ops, loss_ops
 from ._lib import (ME_PAIR_HINGE, ME_PAIR_IPO, ME_PAIR_SIGMOID, ME_REDUCE_MEAN, ME_REDUCE_SEQUENCE,
                    ME_REDUCE_SUM)
 
@@ -364,3 +364,74 @@ def distill_loss(logits, teacher_ids, teacher_logits, teacher_lse=None, mask=Non
     if _wants_grad(logits):
         return _Distill.apply(logits, teacher_ids, args)
     return loss_ops.distill(logits.detach(), teacher_ids, *args, False)[0]
+
+
+# ------------------------------------------------------------------------- from the head, without logits
+def _check_head(hidden, weight, targets):
+    if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1] or not weight.numel():
+        raise ValueError(f"[micro_engram] hidden {tuple(hidden.shape)} and weight {tuple(weight.shape)} must be [..., dim] "
+                         "and [vocab, dim]")
+    if hidden.dtype not in (torch.bfloat16, torch.float32) or weight.dtype is not hidden.dtype:
+        raise TypeError(f"[micro_engram] hidden and weight must both be bf16 or both fp32, got {hidden.dtype} and {weight.dtype}")
+    if targets.shape != hidden.shape[:-1]:
+        raise ValueError(f"[micro_engram] targets {tuple(targets.shape)} do not match the hidden states' rows "
+                         f"{tuple(hidden.shape[:-1])}")
+    if targets.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"[micro_engram] targets must be int32 or int64, got {targets.dtype}")
+
+
+class _HeadLoss(torch.autograd.Function):
+    """args: (op, ignore_index, temperature, and for head_ce smoothing, z_loss, scale, reduction)."""
+
+    @staticmethod
+    def forward(ctx, hidden, weight, targets, args):
+        out, saved = args[0](hidden.detach(), weight.detach(), targets, *args[1:])
+        ctx.save_for_backward(hidden, weight, targets, saved)
+        ctx.consts = args[1:]
+        return out
+
+    @staticmethod
+    @_no_second_derivatives
+    def backward(ctx, upstream):
+        hidden, weight, targets, saved = ctx.saved_tensors
+        need = ctx.needs_input_grad[:2]
+        per_row = len(ctx.consts) == 2
+        ignore_index, temperature, *rest = ctx.consts if not per_row else (*ctx.consts, 0.0, 0.0, 1.0, ME_REDUCE_SUM)
+        grads = iter(head_ops.head_backward(hidden.detach(), weight.detach(), targets, saved, _upstream(upstream), ignore_index,
+                                            temperature, per_row, *rest, *need))
+        return next(grads) if need[0] else None, next(grads) if need[1] else None, None, None
+
+
+def _head_loss(op, hidden, weight, targets, *args):
+    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+        return _HeadLoss.apply(hidden, weight, targets, (op, *args))
+    return op(hidden.detach(), weight.detach(), targets, *args)[0]
+
+
+def head_token_logps(hidden, weight, targets, temperature=1.0, ignore_index=IGNORE_INDEX):
+    """token_logps(hidden @ weight.T, targets) without the logits: log softmax(hidden weight^T / temperature) at `targets`
+    (hidden's shape without its last dim), fp32, 0 where a row does not count. Differentiable in hidden and weight.
+
+    hidden [..., dim] are the states after the decoder's last norm, weight [vocab, dim] its head, both bf16 or both fp32.
+    Memory is that of a piece of the logits' gradient (512 MiB at most for up to 131,072 rows in bf16), whatever the
+    vocabulary. Rows that do not count cost nothing and are not read."""
+    _check_head(hidden, weight, targets)
+    return _head_loss(head_ops.head_logps, hidden, weight, targets, int(ignore_index), _check_temperature(temperature))
+
+
+def head_cross_entropy(hidden, weight, targets, temperature=1.0, label_smoothing=0.0, z_loss=0.0, scale=1.0,
+                       reduction="mean", ignore_index=IGNORE_INDEX):
+    """The cross entropy of the decoder's next tokens from hidden states and head, without the logits: `scale` times the
+    mean (or "sum") over the rows that count of
+
+        lse - (1 - s) z[target] - s mean(z) + z_loss lse^2,   z = hidden weight^T / temperature,  lse = log sum exp(z)
+
+    with s the label_smoothing. Arguments and memory as head_token_logps; differentiable in hidden and weight. No
+    row that counts gives 0 and gradients of zeros."""
+    _check_head(hidden, weight, targets)
+    how = _choice(_DISTILL_REDUCTIONS, reduction, "reduction")
+    smoothing = _check_number(label_smoothing, "label_smoothing", 0.0, 1.0)
+    z_loss = _check_number(z_loss, "z_loss", 0.0, 1e6)
+    scale = _check_number(scale, "scale", -1e30, 1e30)
+    return _head_loss(head_ops.head_ce, hidden, weight, targets, int(ignore_index), _check_temperature(temperature), smoothing,
+                      z_loss, scale, how)

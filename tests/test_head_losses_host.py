@@ -1,0 +1,62 @@
+"""What the losses over a decoder's head refuse, and the shapes that tracing sees."""
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+from micro_engram_fork_amd import _lib, head_ops, losses
+
+CALLS = [losses.head_cross_entropy, losses.head_token_logps]
+
+
+def _args(rows=(2, 3), vocab=11, dim=8, dtype=torch.bfloat16):
+    return torch.zeros(*rows, dim, dtype=dtype), torch.zeros(vocab, dim, dtype=dtype), torch.zeros(rows, dtype=torch.long)
+
+
+@pytest.mark.parametrize("call", CALLS)
+def test_shapes_and_types(call):
+    hidden, weight, targets = _args()
+    for bad in ((hidden[..., :7], weight, targets), (hidden, weight[0], targets), (hidden, weight[:0], targets),
+                (hidden, weight[None], targets), (hidden, weight, targets[:, :2]), (hidden, weight, targets[..., None])):
+        with pytest.raises(ValueError, match="micro_engram"):
+            call(*bad)
+    for bad in ((hidden.float(), weight, targets), (hidden, weight.float(), targets), (hidden.half(), weight.half(), targets),
+                (hidden.double(), weight.double(), targets), (hidden, weight, targets.float()), (hidden, weight, targets.to(torch.int16))):
+        with pytest.raises(TypeError, match="micro_engram"):
+            call(*bad)
+    with pytest.raises(ValueError, match="temperature"):
+        call(*_args(), temperature=0.0)
+    with pytest.raises(RuntimeError, match="only on the GPU"):
+        call(*_args())
+
+
+@pytest.mark.parametrize("bad", [dict(label_smoothing=-0.1), dict(label_smoothing=1.1), dict(z_loss=-1.0), dict(z_loss=float("nan")),
+                                 dict(scale=float("inf")), dict(reduction="none"), dict(reduction="sequence"), dict(temperature=float("nan"))])
+def test_options(bad):
+    with pytest.raises(ValueError, match="micro_engram"):
+        losses.head_cross_entropy(*_args(), **bad)
+
+
+def test_c_entry_checks():
+    """The C entry refuses what its kernels do not hold, before any launch."""
+    p = 4096  # an address that is not read
+
+    def logps(dtype=_lib.ME_BF16, n=4, dim=8, vocab=11, stride=8, tdtype=_lib.ME_I64, temperature=1.0, size=1 << 40, ws=p, saved=p):
+        _lib.call("me_head_logps", p, dtype, n, dim, max(n, 1), 0, dim, p, vocab, stride, p, tdtype, -100, temperature, p, saved, ws, size, None)
+    for bad in (dict(dtype=_lib.ME_I32), dict(n=-1), dict(n=1 << 25), dict(dim=0), dict(dim=65537), dict(vocab=0), dict(vocab=1 << 22),
+                dict(stride=7), dict(stride=1 << 23), dict(tdtype=_lib.ME_F32), dict(temperature=0.0), dict(temperature=float("nan")),
+                dict(size=16), dict(ws=None), dict(saved=None), dict(ws=p + 8)):
+        with pytest.raises(_lib.EngramLibError):
+            logps(**bad)
+
+
+def test_fake_shapes():
+    with FakeTensorMode():
+        hidden, weight, targets = (x.cuda() if False else x for x in _args())
+        out, saved = head_ops.head_logps(hidden, weight, targets, -100, 1.0)
+        assert out.shape == (2, 3) and out.dtype is torch.float32
+        loss, saved = head_ops.head_ce(hidden, weight, targets, -100, 1.0, 0.0, 0.0, 1.0, 0)
+        assert loss.shape == () and saved.shape == (16 + 4 * 6,)
+        both = head_ops.head_backward(hidden, weight, targets, saved, loss, -100, 1.0, False, 0.0, 0.0, 1.0, 0, True, True)
+        assert [g.shape for g in both] == [hidden.shape, weight.shape] and both[1].dtype is torch.bfloat16
+        one, = head_ops.head_backward(hidden, weight, targets, saved, loss, -100, 1.0, False, 0.0, 0.0, 1.0, 0, False, True)
+        assert one.shape == weight.shape
