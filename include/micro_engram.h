@@ -682,13 +682,19 @@ int me_distill_backward(const void *logits, int dtype, int64_t n, int64_t vocab,
  *               fp32 ones are laid out a piece at a time
  *   targets, ignore_index, temperature  as above; nothing of a row that does not count is read
  *   saved       [16 + 4 n] 4-byte elements (16-byte aligned): what the backward needs
- *   workspace   me_head_workspace_size bytes for the same n, vocab, dim, dtype, weight and w_stride, with
- *               backward != 0 for me_head_backward; 16-byte aligned
+ *   unit        nullable, [me_head_unit_size] fp32 (16-byte aligned): where the gradient of hidden
+ *               alone is wanted, the forward leaves there what the backward only has to scale. A
+ *               size of 0: the call is too small for that to pay (unit may still be given, n times
+ *               dim rounded up to 4 values)
+ *   workspace   me_head_workspace_size bytes for the same n, vocab, dim, dtype, weight and w_stride, with pass
+ *               0 for a forward, 1 for me_head_backward (without unit, which needs none), 2 for a
+ *               forward with unit; 16-byte aligned
  * bf16 products accumulate in fp32; fp32 ones are made of bf16 parts that add up to the operands, with
  * the accuracy of fp32 products.
  */
 int me_head_workspace_size(int64_t n, int64_t vocab, int64_t dim, int dtype, const void *weight,
-                           int64_t w_stride, int backward, size_t *bytes);
+                           int64_t w_stride, int pass, size_t *bytes);
+int me_head_unit_size(int64_t n, int64_t vocab, int64_t dim, int dtype, int64_t *elements);
 
 /*
  * me_head_logps -- logps[r] = log softmax(z[r])[targets[r]], fp32; 0 where a row does not count.
@@ -696,7 +702,7 @@ int me_head_workspace_size(int64_t n, int64_t vocab, int64_t dim, int dtype, con
 int me_head_logps(const void *hidden, int dtype, int64_t n, int64_t dim, int64_t rows_per_batch,
                   int64_t batch_stride, int64_t row_stride, const void *weight, int64_t vocab,
                   int64_t w_stride, const void *targets, int targets_dtype, int64_t ignore_index,
-                  double temperature, float *logps, void *saved, void *workspace,
+                  double temperature, float *logps, void *saved, float *unit, void *workspace,
                   size_t workspace_bytes, void *stream);
 
 /*
@@ -708,12 +714,14 @@ int me_head_ce(const void *hidden, int dtype, int64_t n, int64_t dim, int64_t ro
                int64_t batch_stride, int64_t row_stride, const void *weight, int64_t vocab,
                int64_t w_stride, const void *targets, int targets_dtype, int64_t ignore_index,
                double temperature, double smoothing, double z_loss, double scale, int reduction,
-               float *loss, void *saved, void *workspace, size_t workspace_bytes, void *stream);
+               float *loss, void *saved, float *unit, void *workspace, size_t workspace_bytes,
+               void *stream);
 
 /*
  * me_head_backward -- gradients of me_head_logps (upstream_per_row != 0: upstream [n] fp32, the
  * log-probabilities' gradient; scale 1) or of me_head_ce (upstream: device scalar; its other
  * arguments as given there), with what that call left in saved.
+ *   unit         as the forward left it, or NULL; with it grad_weight is NULL
  *   grad_hidden  nullable, [n, dim] contiguous, zeros in rows that do not count
  *   grad_weight  nullable, [vocab, dim] contiguous; both of dtype and 16-byte aligned
  */
@@ -722,8 +730,8 @@ int me_head_backward(const void *hidden, int dtype, int64_t n, int64_t dim, int6
                      int64_t w_stride, const void *targets, int targets_dtype, int64_t ignore_index,
                      double temperature, const float *upstream, int upstream_per_row,
                      double smoothing, double z_loss, double scale, int reduction,
-                     const void *saved, void *grad_hidden, void *grad_weight, void *workspace,
-                     size_t workspace_bytes, void *stream);
+                     const void *saved, const float *unit, void *grad_hidden, void *grad_weight,
+                     void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -142,6 +142,41 @@ __global__ __launch_bounds__(256) void layout_kernel(const Layout a) {
 // ---- epilogues -----------------------------------------------------------------------------------------------
 // acc[x][y][4 g + e] is row row0 + 32 y + (lane & 31), column col0 + 32 x + 8 g + 4 (lane >> 5) + e of the tile.
 
+// Four values of row lane & 31 at column col of a staged block of 32 rows, bf16 or in parts that add up to them
+template <int NPARTS, int SX>
+__device__ __forceinline__ void stage4(float (&v)[4], uint8_t *stage, int col, int lane) {
+    constexpr int kPitch = 64 * SX + 16;
+#pragma unroll
+    for (int p = 0; p < NPARTS; ++p) {
+        uint32_t w[2];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint16_t b = float_to_bf16_bits_rne(v[e]);
+            reinterpret_cast<uint16_t *>(w)[e] = b;
+            if (p + 1 < NPARTS) {
+                v[e] -= bf16_bits_to_float(b);
+                if (p == 0 && !(__builtin_fabsf(v[e]) < __builtin_inff())) v[e] = 0.f;  // not finite: the first part alone
+            }
+        }
+        *reinterpret_cast<uint2 *>(stage + (p * 32 + (lane & 31)) * kPitch + col * 2) = make_uint2(w[0], w[1]);
+    }
+}
+
+// A staged block as 16-byte chunks of rows r0 .. of [rows][ld], from column c0 on
+template <int NPARTS, int SX>
+__device__ __forceinline__ void store_rows(const uint8_t *stage, uint8_t *out, int64_t ld, int64_t part, int64_t r0, int64_t rows, int64_t c0,
+                                           int lane) {
+    constexpr int kPitch = 64 * SX + 16, kChunks = 4 * SX;
+#pragma unroll
+    for (int p = 0; p < NPARTS; ++p)
+#pragma unroll 4
+        for (int it = 0; it < 32 * kChunks / 64; ++it) {
+            const int ch = it * 64 + lane, r = ch / kChunks, cc = ch % kChunks;
+            const u32x4_v v = *reinterpret_cast<const u32x4_v *>(stage + (p * 32 + r) * kPitch + cc * 16);
+            if (r0 + r < rows && c0 + cc * 8 < ld) *as_global(reinterpret_cast<u32x4_v *>(out + p * part + ((r0 + r) * ld + c0 + cc * 8) * 2)) = v;
+        }
+}
+
 // Statistics of a tile's rows over a wave's columns, in units of log2: their maximum and sum without the target,
 // the target's own value, and where wanted the plain sum of the values.
 struct StatsEpilogue {
@@ -216,6 +251,80 @@ struct StatsEpilogue {
     }
 };
 
+// The exponentials of a tile's logits, 2^(z - ref) by row and zero at the target, bf16 or in three parts, as rows of a
+// piece, and their sums over a wave's columns
+template <int NPARTS>
+struct ExpEpilogue {
+    const int32_t *tgt;
+    const float *ref;        // by row, log2
+    float *part, *sum;       // by (column part, row), as StatsEpilogue
+    float *at_target;
+    int64_t part_stride, row_stride;
+    uint8_t *out;
+    int64_t ld, out_part;
+    int64_t first, vocab;
+    float k;
+
+    template <bool AGPR, int SX, int SY>
+    __device__ __forceinline__ void run(const floatx16 (&acc)[SX][SY], const Tile &t, int row0, int col0, uint8_t *lds, int lane) const {
+        const int64_t c0 = t.s0 + col0;
+        const int there = static_cast<int>(max(min(vocab - c0, int64_t{32 * SX}), int64_t{0}));
+        const int64_t part_at = (first + c0) / (32 * SX);
+        constexpr int kPitch = 64 * SX + 16, kPlaces = NPARTS == 1 ? 2 : 1;
+#pragma unroll
+        for (int y = 0; y < SY; ++y) {
+            uint8_t *stage = lds + ((threadIdx.x >> 6) * kPlaces + (y % kPlaces)) * (NPARTS * 32 * kPitch);
+            const int64_t row = t.r0 + row0 + 32 * y + (lane & 31);
+            const bool ok = row < t.rows;
+            const float shift = ok ? ref[row] : 0.f;
+            const int64_t off = ok ? tgt[row] - (first + c0) : -1;
+            const int mine = off >= 0 && off < there ? static_cast<int>(off) : -1;
+            float s, total = 0.f;
+            // three parts: one way through it, or the code outgrows what the compiler unrolls; the K loop is six times as long
+            if (NPARTS > 1 || there < 32 * SX || __any(mine >= 0))
+                s = stage_rows<AGPR, true, SX, SY>(acc, y, row, shift, mine, there, total, stage, lane);
+            else
+                s = stage_rows<AGPR, false, SX, SY>(acc, y, row, shift, mine, there, total, stage, lane);
+            s += __shfl_xor(s, 32);
+            total += __shfl_xor(total, 32);
+            if (ok && lane < 32) {
+                part[part_at * part_stride + row * row_stride] = s;
+                if (sum != nullptr) sum[part_at * part_stride + row * row_stride] = total * k;
+            }
+            store_rows<NPARTS, SX>(stage, out, ld, out_part, t.r0 + row0 + 32 * y, t.rows, c0, lane);
+        }
+    }
+
+    template <bool AGPR, bool SOME, int SX, int SY>
+    __device__ __forceinline__ float stage_rows(const floatx16 (&acc)[SX][SY], int y, int64_t row, float shift, int mine, int there,
+                                                float &total, uint8_t *stage, int lane) const {
+        const int half4 = 4 * (lane >> 5);
+        float s = 0.f;
+#pragma unroll
+        for (int x = 0; x < SX; ++x)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float z = acc_read<AGPR>(acc[x][y], 4 * q + e);
+                    v[e] = __builtin_amdgcn_exp2f(fmaf(z, k, -shift));
+                    if constexpr (SOME) {
+                        const int col = 32 * x + 8 * q + half4 + e;
+                        if (col == mine) at_target[row] = z * k;
+                        if (col == mine || col >= there) v[e] = 0.f;
+                        total += col < there ? z : 0.f;
+                    } else {
+                        total += z;
+                    }
+                    s += v[e];
+                }
+                stage4<NPARTS, SX>(v, stage, 32 * x + 8 * q + half4, lane);
+            }
+        return s;
+    }
+};
+
 struct RowGrad {
     float lse2, ca, cb, gt;
 };
@@ -235,7 +344,6 @@ struct GradEpilogue {
         const int64_t c0 = t.s0 + col0;
         const int there = static_cast<int>(max(min(vocab - c0, int64_t{32 * SX}), int64_t{0}));
         constexpr int kPitch = 64 * SX + 16;  // staged row (bytes)
-        constexpr int kChunks = 4 * SX;
 #pragma unroll
         for (int y = 0; y < SY; ++y) {
             // 32 rows at a time through LDS, where a wave has two places in turn (with three parts one: a wave's
@@ -252,47 +360,29 @@ struct GradEpilogue {
                 stage_rows<AGPR, true, SX, SY>(acc, y, g, mine, there, stage, lane);
             else
                 stage_rows<AGPR, false, SX, SY>(acc, y, g, mine, there, stage, lane);
-#pragma unroll
-            for (int p = 0; p < NPARTS; ++p)
-#pragma unroll 4
-                for (int it = 0; it < 32 * kChunks / 64; ++it) {
-                    const int ch = it * 64 + lane, r = ch / kChunks, cc = ch % kChunks;
-                    const int64_t rg = t.r0 + row0 + 32 * y + r, cg = c0 + cc * 8;
-                    const u32x4_v v = *reinterpret_cast<const u32x4_v *>(stage + (p * 32 + r) * kPitch + cc * 16);
-                    if (rg < t.rows && cg < ld) *as_global(reinterpret_cast<u32x4_v *>(out + p * part + (rg * ld + cg) * 2)) = v;
-                }
+            store_rows<NPARTS, SX>(stage, out, ld, part, t.r0 + row0 + 32 * y, t.rows, c0, lane);
         }
     }
 
     template <bool AGPR, bool SOME, int SX, int SY>
     __device__ __forceinline__ void stage_rows(const floatx16 (&acc)[SX][SY], int y, const RowGrad &g, int mine, int there, uint8_t *stage,
                                                int lane) const {
-        constexpr int kPitch = 64 * SX + 16;
         const int half4 = 4 * (lane >> 5);
 #pragma unroll
         for (int x = 0; x < SX; ++x)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                uint32_t w[NPARTS][2];
+                float v[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    float v = fmaf(__builtin_amdgcn_exp2f(fmaf(acc_read<AGPR>(acc[x][y], 4 * q + e), k, -g.lse2)), g.ca, -g.cb);
+                    v[e] = fmaf(__builtin_amdgcn_exp2f(fmaf(acc_read<AGPR>(acc[x][y], 4 * q + e), k, -g.lse2)), g.ca, -g.cb);
                     if constexpr (SOME) {
                         const int col = 32 * x + 8 * q + half4 + e;
-                        if (col == mine) v = g.gt;
-                        if (col >= there) v = 0.f;  // past the vocabulary: nothing for the products with W and h
-                    }
-#pragma unroll
-                    for (int p = 0; p < NPARTS; ++p) {
-                        const uint16_t b = float_to_bf16_bits_rne(v);
-                        reinterpret_cast<uint16_t *>(w[p])[e] = b;
-                        v -= bf16_bits_to_float(b);
-                        if (p == 0 && NPARTS > 1 && !(__builtin_fabsf(v) < __builtin_inff())) v = 0.f;  // not finite: the first part alone
+                        if (col == mine) v[e] = g.gt;
+                        if (col >= there) v[e] = 0.f;  // past the vocabulary: nothing for the products with W and h
                     }
                 }
-#pragma unroll
-                for (int p = 0; p < NPARTS; ++p)
-                    *reinterpret_cast<uint2 *>(stage + (p * 32 + (lane & 31)) * kPitch + (32 * x + 8 * q + half4) * 2) = make_uint2(w[p][0], w[p][1]);
+                stage4<NPARTS, SX>(v, stage, 32 * x + 8 * q + half4, lane);
             }
     }
 };
@@ -345,26 +435,19 @@ struct WeightEpilogue {
 #pragma unroll
         for (int y = 0; y < SY; ++y) {
             if (!F32 && whole) {
-                constexpr int kPitch = 64 * SX + 16, kChunks = 4 * SX;
+                constexpr int kPitch = 64 * SX + 16;
                 static_assert(8 * 32 * kPitch <= kRingBytes, "the stage fits the ring");
                 uint8_t *stage = lds + ((threadIdx.x >> 6) * 2 + (y & 1)) * (32 * kPitch);
 #pragma unroll
                 for (int x = 0; x < SX; ++x)
 #pragma unroll
                     for (int g = 0; g < 4; ++g) {
-                        uint32_t w[2];
+                        float v[4];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            reinterpret_cast<uint16_t *>(w)[e] = float_to_bf16_bits_rne(acc_read<AGPR>(acc[x][y], 4 * g + e));
-                        *reinterpret_cast<uint2 *>(stage + (lane & 31) * kPitch + (32 * x + 8 * g + half4) * 2) = make_uint2(w[0], w[1]);
+                        for (int e = 0; e < 4; ++e) v[e] = acc_read<AGPR>(acc[x][y], 4 * g + e);
+                        stage4<1, SX>(v, stage, 32 * x + 8 * g + half4, lane);
                     }
-#pragma unroll 4
-                for (int it = 0; it < 32 * kChunks / 64; ++it) {
-                    const int ch = it * 64 + lane, r = ch / kChunks, cc = ch % kChunks;
-                    const int64_t rg = t.r0 + row0 + 32 * y + r, cg = t.s0 + col0 + cc * 8;
-                    const u32x4_v v = *reinterpret_cast<const u32x4_v *>(stage + r * kPitch + cc * 16);
-                    if (rg < t.rows && cg < dim) *as_global(reinterpret_cast<u32x4_v *>(out + (rg * dim + cg) * 2)) = v;
-                }
+                store_rows<1, SX>(stage, out, dim, 0, t.r0 + row0 + 32 * y, t.rows, t.s0 + col0, lane);
                 continue;
             }
             const int64_t row = t.r0 + row0 + 32 * y + (lane & 31);
@@ -398,10 +481,12 @@ struct WeightEpilogue {
 struct FinishArgs {
     const float2 *part;
     const float *sum, *at_target;
+    const float *exps, *ref;  // in place of part: sums of 2^(z - ref), and ref by row
     int64_t part_stride, row_stride;
     int parts;
     int64_t n, vocab;
     Saved s;
+    const int32_t *count, *which;  // rows, and the counted rows that they are; null: those themselves
     float *logps;        // by source row, or null
     float *row_loss;     // by counted row, or null
     float smoothing, z_loss;
@@ -417,24 +502,30 @@ __device__ __forceinline__ Sum2 join(Sum2 a, Sum2 b) {
     return {m, a.s * __builtin_amdgcn_exp2f(a.m - shift) + b.s * __builtin_amdgcn_exp2f(b.m - shift)};
 }
 
-// A row's parts joined: WIDE 256 threads per row (few rows), else 64 rows by four threads each
+// A row's parts joined: WIDE 256 threads per row (few rows), else 16 rows by 16 threads each
 template <bool WIDE>
 __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs a) {
-    constexpr int kSlices = WIDE ? 256 : 4;
+    constexpr int kRows = WIDE ? 1 : 16, kSlices = 256 / kRows, kLast = WIDE ? 4 : 16;
     __shared__ Sum2 s_all[WIDE ? 4 : 256];
     __shared__ double s_sum[WIDE ? 4 : 256];
-    const int tid = threadIdx.x, slice = WIDE ? tid : tid >> 6;
-    const int64_t r = WIDE ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * 64 + (tid & 63);
-    const int64_t count = *a.s.count;
-    if (WIDE ? r >= count : static_cast<int64_t>(blockIdx.x) * 64 >= count) return;
+    const int tid = threadIdx.x, slice = tid / kRows;
+    const int64_t r = static_cast<int64_t>(blockIdx.x) * kRows + tid % kRows;
+    const int64_t count = a.count ? *a.count : *a.s.count;
+    if (static_cast<int64_t>(blockIdx.x) * kRows >= count) return;
     Sum2 all = {-__builtin_inff(), 0.f};
     double sum = 0.0;
     if (r < count) {
-        for (int p = slice; p < a.parts; p += kSlices) {
-            const float2 x = a.part[p * a.part_stride + r * a.row_stride];
-            all = join(all, {x.x, x.y});
-            if (a.sum) sum += a.sum[p * a.part_stride + r * a.row_stride];
+        if (a.exps) {
+            all.m = a.ref[r];
+            for (int p = slice; p < a.parts; p += kSlices) all.s += a.exps[p * a.part_stride + r * a.row_stride];
+        } else {
+            for (int p = slice; p < a.parts; p += kSlices) {
+                const float2 x = a.part[p * a.part_stride + r * a.row_stride];
+                all = join(all, {x.x, x.y});
+            }
         }
+        if (a.sum)
+            for (int p = slice; p < a.parts; p += kSlices) sum += a.sum[p * a.part_stride + r * a.row_stride];
     }
     if constexpr (WIDE) {
 #pragma unroll
@@ -447,11 +538,9 @@ __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs a) {
         s_all[tid] = all, s_sum[tid] = sum;
     }
     __syncthreads();
-    if (WIDE ? tid != 0 : (tid >= 64 || r >= count)) return;
-    constexpr int kStep = WIDE ? 1 : 64;
+    if (tid >= kRows || r >= count) return;
     all = s_all[tid], sum = s_sum[tid];
-#pragma unroll
-    for (int i = 1; i < 4; ++i) all = join(all, s_all[tid + i * kStep]), sum += s_sum[tid + i * kStep];
+    for (int i = 1; i < kLast; ++i) all = join(all, s_all[tid + i * kRows]), sum += s_sum[tid + i * kRows];
     // d: how far the others' sum is over the target, log2
     const float zt = a.at_target[r], rest = all.m + log2f(all.s);
     const float d = rest - zt;
@@ -459,14 +548,15 @@ __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs a) {
     const float nll = static_cast<float>(kLn2) * fmaxf(d, 0.f) + more;
     const float others = d > 0.f ? 1.f / (1.f + e) : e / (1.f + e);
     const float lse2 = (d > 0.f ? rest : zt) + more * kLog2e;
-    a.s.lse2[r] = lse2;
-    a.s.others[r] = d != d ? d : others;
-    if (a.logps) a.logps[a.s.rows[r]] = -nll;
+    const int64_t c = a.which ? a.which[r] : r;
+    a.s.lse2[c] = lse2;
+    a.s.others[c] = d != d ? d : others;
+    if (a.logps) a.logps[a.s.rows[c]] = -nll;
     if (a.row_loss) {
         const float lse = static_cast<float>(kLn2) * lse2;
         float loss = nll + a.z_loss * lse * lse;
         if (a.smoothing != 0.f) loss += a.smoothing * static_cast<float>(kLn2 * (zt - sum / static_cast<double>(a.vocab)));
-        a.row_loss[r] = loss;
+        a.row_loss[c] = loss;
     }
 }
 
@@ -522,6 +612,33 @@ __global__ __launch_bounds__(256) void coef_kernel(const CoefArgs a) {
     a.grad[r] = g;
 }
 
+// Four values of a row of the hidden states' gradient
+template <bool F32>
+__device__ __forceinline__ void store4(void *out, int64_t at, int64_t c, int64_t dim, const f32x4_v &v) {
+    if constexpr (F32) {
+        float *o = static_cast<float *>(out) + at + c;
+        if (dim % 4 == 0) {
+            *as_global(reinterpret_cast<f32x4_v *>(o)) = v;
+            return;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (c + e < dim) o[e] = v[e];
+    } else {
+        uint16_t *o = static_cast<uint16_t *>(out) + at + c;
+        uint16_t b[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) b[e] = float_to_bf16_bits_rne(v[e]);
+        if (dim % 4 == 0) {
+            *as_global(reinterpret_cast<u32x2_v *>(o)) = u32x2_v{b[0] | (static_cast<uint32_t>(b[1]) << 16), b[2] | (static_cast<uint32_t>(b[3]) << 16)};
+            return;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (c + e < dim) o[e] = b[e];
+    }
+}
+
 // Gradient of the hidden states, source rows in their order: the splits' sums, or zeros
 template <bool F32>
 __global__ __launch_bounds__(256) void hidden_kernel(const float *sums, int64_t ld, int64_t split_stride, int splits, const int32_t *place,
@@ -533,25 +650,187 @@ __global__ __launch_bounds__(256) void hidden_kernel(const float *sums, int64_t 
         f32x4_v v = {0.f, 0.f, 0.f, 0.f};
         if (r >= 0)
             for (int s = 0; s < splits; ++s) v += *as_global(reinterpret_cast<const f32x4_v *>(sums + s * split_stride + r * ld + c));
+        store4<F32>(out, i * dim, c, dim, v);
+    }
+}
+
+// ---- the hidden states' gradient from the forward's exponentials ---------------------------------------------------
+// Where the head takes no gradient, the forward's tiles of logits are worth a second use: their exponentials
+// 2^(z - ref), with ref the target's logit, go through the product with W as they are, and the row's sum, known when all
+// pieces are through, scales the result: D = a sum_{j != t} q_j w_j + (a q_t - 1) w_t, the gradient of a loss of
+// upstream 1 before the factors that rows share; the target's term in fp32. The backward only scales D. ref is no
+// maximum: a row whose sum passes 2^100 (its loss is over some 69) or is not finite is made again by the plain way
+// (statistics, then gradient), in launches that find no row otherwise.
+template <bool F32>
+__global__ __launch_bounds__(256) void ref_kernel(const Layout h, const void *weight, int64_t w_stride, const int32_t *tgt, float k, float *ref) {
+    const int64_t r = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    if (r >= *h.count) return;
+    const int lane = threadIdx.x & 63;
+    const int64_t from = h.rows[r], at = from / h.per_batch * h.batch_stride + from % h.per_batch * h.row_stride;
+    const int64_t w = tgt[r] * w_stride;
+    float sum = 0.f;
+    for (int64_t c = lane; c < h.dim; c += 64) {
+        if constexpr (F32)
+            sum += static_cast<const float *>(h.src)[at + c] * static_cast<const float *>(weight)[w + c];
+        else
+            sum += bf16_bits_to_float(static_cast<const uint16_t *>(h.src)[at + c]) * bf16_bits_to_float(static_cast<const uint16_t *>(weight)[w + c]);
+    }
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (c + e < dim) {
-                if constexpr (F32)
-                    static_cast<float *>(out)[i * dim + c + e] = v[e];
-                else
-                    static_cast<uint16_t *>(out)[i * dim + c + e] = float_to_bf16_bits_rne(v[e]);
+    for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+    sum *= k;
+    if (lane == 0) ref[r] = __builtin_fabsf(sum) < __builtin_inff() ? sum : 0.f;
+}
+
+// Rows to make again, in order, with their targets. One workgroup.
+struct RedoArgs {
+    Saved s;
+    const float *ref;
+    const int32_t *tgt;
+    int32_t *count, *rows, *tgt2;
+};
+
+__global__ __launch_bounds__(kIndexThreads) void redo_kernel(const RedoArgs a) {
+    __shared__ int sums[kIndexThreads / 64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int n = *a.s.count;
+    int at = 0;
+    for (int i0 = 0; i0 < n; i0 += kIndexThreads) {
+        const int i = i0 + tid;
+        // the row's sum is 2^(lse2 - ref), at least about 1, as the target is one of its terms; NaN is bad too
+        const float over = i < n ? a.s.lse2[i] - a.ref[i] : 0.f;
+        const bool bad = !(over > -1.f && over < 100.f);
+        const uint64_t mask = __ballot(bad);
+        if (lane == 0) sums[wave] = __popcll(mask);
+        __syncthreads();
+        int before = at, all = 0;
+        for (int w = 0; w < kIndexThreads / 64; ++w) {
+            before += w < wave ? sums[w] : 0;
+            all += sums[w];
+        }
+        if (bad) {
+            const int r = before + __popcll(mask & ((uint64_t{1} << lane) - 1));
+            a.rows[r] = i;
+            a.tgt2[r] = a.tgt[i];
+        }
+        at += all;
+        __syncthreads();
+    }
+    if (tid == 0) *a.count = at;
+}
+
+// Gradient of z itself for the rows that are made again: a q, nothing at the target
+__global__ __launch_bounds__(256) void redo_coef_kernel(Saved s, const int32_t *count, const int32_t *rows, float z_loss, RowGrad *grad) {
+    const int r = static_cast<int>(blockIdx.x) * 256 + static_cast<int>(threadIdx.x);
+    if (r >= *count) return;
+    const float lse2 = s.lse2[rows[r]];
+    grad[r] = {lse2, 1.f + 2.f * z_loss * static_cast<float>(kLn2) * lse2, 0.f, 0.f};
+}
+
+// Sums of the head's columns, which a smoothed target's gradient takes in: chunks of rows, then over the chunks
+constexpr int kColumnRows = 512;
+
+template <bool F32>
+__global__ __launch_bounds__(256) void column_kernel(const void *weight, int64_t w_stride, int64_t vocab, int64_t dim, float *part) {
+    const int64_t c = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (c >= dim) return;
+    const int64_t v0 = static_cast<int64_t>(blockIdx.y) * kColumnRows, v1 = min(vocab, v0 + kColumnRows);
+    float sum = 0.f;
+#pragma unroll 8
+    for (int64_t v = v0; v < v1; ++v)
+        sum += F32 ? static_cast<const float *>(weight)[v * w_stride + c] : bf16_bits_to_float(static_cast<const uint16_t *>(weight)[v * w_stride + c]);
+    part[blockIdx.y * dim + c] = sum;
+}
+
+__global__ __launch_bounds__(256) void column_total_kernel(const float *part, int chunks, int64_t dim, float *out) {
+    const int64_t c = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (c >= dim) return;
+    double sum = 0.0;
+    for (int i = 0; i < chunks; ++i) sum += static_cast<double>(part[i * dim + c]);
+    out[c] = static_cast<float>(sum);
+}
+
+struct UnitArgs {
+    const float *sums;
+    int64_t ld, split_stride;
+    int splits;
+    Saved s;
+    const int32_t *count, *which;  // as FinishArgs
+    const int32_t *tgt;            // by row of sums
+    const float *ref;              // null: sums are of a q
+    const void *weight;
+    int64_t w_stride, dim, n;
+    float z_loss, smoothing;
+    const float *columns;          // sums of the head's columns, null without smoothing
+    double vocab;
+    float *unit;                   // [counted rows][dim rounded up to 4]
+};
+
+template <bool F32>
+__global__ __launch_bounds__(256) void unit_kernel(const UnitArgs a) {
+    const int64_t units = ceil_div(a.dim, 4);
+    const int64_t count = a.count ? *a.count : *a.s.count;
+    for (int64_t u = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; u < count * units; u += static_cast<int64_t>(gridDim.x) * 256) {
+        const int64_t r = u / units, c = (u - r * units) * 4;
+        const int64_t at = a.which ? a.which[r] : r;
+        const float lse2 = a.s.lse2[at];
+        const float more = 2.f * a.z_loss * static_cast<float>(kLn2) * lse2;
+        const float own = more - (1.f + more) * a.s.others[at] + a.smoothing;
+        const float each = a.columns ? static_cast<float>(a.smoothing / a.vocab) : 0.f;
+        const float scale = a.ref ? (1.f + more) * __builtin_amdgcn_exp2f(a.ref[r] - lse2) : 1.f;
+        f32x4_v v = {0.f, 0.f, 0.f, 0.f};
+        for (int s = 0; s < a.splits; ++s) v += *as_global(reinterpret_cast<const f32x4_v *>(a.sums + s * a.split_stride + r * a.ld + c));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float w = 0.f, all = 0.f;
+            if (c + e < a.dim) {
+                if (a.columns) all = each * a.columns[c + e];
+                const int64_t i = a.tgt[r] * a.w_stride + c + e;
+                w = F32 ? static_cast<const float *>(a.weight)[i] : bf16_bits_to_float(static_cast<const uint16_t *>(a.weight)[i]);
             }
+            v[e] = fmaf(v[e], scale, fmaf(own, w, -all));
+        }
+        *as_global(reinterpret_cast<f32x4_v *>(a.unit + at * units * 4 + c)) = v;
+    }
+}
+
+// The backward where the forward left D
+struct ScaleArgs {
+    const float *unit;
+    const int32_t *count, *place;
+    const float *upstream;
+    int per_row, mean;
+    double scale;  // of the loss, over T
+    int64_t n, dim;
+    void *out;
+};
+
+template <bool F32>
+__global__ __launch_bounds__(256) void scale_kernel(const ScaleArgs a) {
+    const int64_t units = ceil_div(a.dim, 4);
+    const double all = a.per_row ? -a.scale : static_cast<double>(*a.upstream) * a.scale / (a.mean ? max(*a.count, 1) : 1);
+    for (int64_t u = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; u < a.n * units; u += static_cast<int64_t>(gridDim.x) * 256) {
+        const int64_t i = u / units, c = (u - i * units) * 4;
+        const int64_t r = a.place[i];
+        f32x4_v v = {0.f, 0.f, 0.f, 0.f};
+        if (r >= 0) {
+            const float f = static_cast<float>(a.per_row ? all * static_cast<double>(a.upstream[i]) : all);
+            v = *as_global(reinterpret_cast<const f32x4_v *>(a.unit + r * units * 4 + c)) * f;
+        }
+        store4<F32>(a.out, i * a.dim, c, a.dim, v);
     }
 }
 
 // ---- plan: sizes and places in the workspace ---------------------------------------------------------------------
+enum Pass { kStats, kBackward, kLeavesUnit };  // the forward alone, the backward, the forward that leaves D
+
 struct Plan {
-    int64_t n, vocab, dim, ld;  // ld: dim rounded up to whole slabs
-    bool f32, few, copy_w;      // copy_w: the head is laid out piece by piece
-    int np;                     // parts of an operand
-    int64_t piece;              // columns of the vocabulary at a time
-    int splits;                 // of the product with W
+    int64_t n, rows, vocab, dim, ld;  // rows: n rounded up, at least 64; ld: dim rounded up to whole slabs
+    bool f32, few, copy_w;            // copy_w: the head is laid out piece by piece
+    int np;                           // parts of an operand
+    int64_t piece;                    // columns of the vocabulary at a time
+    int splits;                       // of the product with W
     int64_t h, tgt, part, sum, at_target, row_loss, w, g, grad, acc;  // workspace offsets
+    int64_t ref, redo, h2, tgt2, columns, column_part;
     int64_t bytes;
 };
 
@@ -569,17 +848,17 @@ int splits_of(int64_t tiles, int64_t at_once, int64_t slabs) {
     return best;
 }
 
-Plan plan_of(int64_t n, int64_t vocab, int64_t dim, int dtype, const void *weight, int64_t w_stride, bool backward) {
+Plan plan_of(int64_t n, int64_t vocab, int64_t dim, int dtype, const void *weight, int64_t w_stride, Pass pass) {
     Plan p{};
     p.n = n, p.vocab = vocab, p.dim = dim, p.ld = round_up(dim, kSlabK);
     p.f32 = dtype == ME_F32;
     p.np = p.f32 ? 3 : 1;
     p.few = n <= kFew;
     p.copy_w = p.f32 || w_stride % 8 != 0 || reinterpret_cast<uintptr_t>(weight) % 16 != 0;
+    const int64_t rows = p.rows = round_up(std::max<int64_t>(n, 1), 64);
     int64_t piece = round_up(vocab, kTile);
-    const int64_t rows = round_up(std::max<int64_t>(n, 1), 64);
     if (p.copy_w) piece = std::min(piece, std::max<int64_t>(kPieceBytes / (p.ld * 2 * p.np) / 2048 * 2048, 2048));
-    if (backward) piece = std::min(piece, std::max<int64_t>(kPieceBytes / (rows * 2 * p.np) / 2048 * 2048, 2048));
+    if (pass != kStats) piece = std::min(piece, std::max<int64_t>(kPieceBytes / (rows * 2 * p.np) / 2048 * 2048, 2048));
     // a launch holds fewer than 2^32 threads
     p.piece = std::min(piece, std::max<int64_t>((int64_t{1} << 23) / ceil_div(rows, p.few ? 64 : kTile) * kTile / 2048 * 2048, 2048));
     int64_t at = 0;
@@ -590,21 +869,38 @@ Plan plan_of(int64_t n, int64_t vocab, int64_t dim, int dtype, const void *weigh
     };
     p.h = take(rows * p.ld * 2 * p.np);
     p.tgt = take(n * 4);
+    p.grad = take(n * static_cast<int64_t>(sizeof(RowGrad)));
     if (p.copy_w) p.w = take(p.piece * p.ld * 2 * p.np);
-    if (!backward) {
+    if (pass != kBackward) {
         const int64_t parts = ceil_div(vocab, p.few ? 64 : 128) + 4;
         p.part = take(parts * rows * 8);
         p.sum = take(parts * rows * 4);
         p.at_target = take(n * 4);
         p.row_loss = take(n * 4);
-    } else {
+    }
+    if (pass != kStats) {
         p.g = take(rows * p.piece * 2 * p.np);
-        p.grad = take(n * static_cast<int64_t>(sizeof(RowGrad)));
         p.splits = splits_of(ceil_div(n, p.few ? 64 : kTile) * ceil_div(dim, kTile), p.few ? 512 : 256, p.piece / kSlabK);
         p.acc = take(p.splits * rows * p.ld * 4);
     }
+    if (pass == kLeavesUnit) {
+        p.ref = take(n * 4);
+        p.redo = take((kHeader + n) * 4);
+        p.h2 = take(rows * p.ld * 2 * p.np);
+        p.tgt2 = take(n * 4);
+        p.columns = take(dim * 4);
+        p.column_part = take(ceil_div(vocab, kColumnRows) * dim * 4);
+    }
     p.bytes = at;
     return p;
+}
+
+// Whether a forward for the hidden states' gradient alone leaves D. It saves the backward one of three products (few
+// rows: one of three reads of the head) and costs some ten launches more.
+bool leaves_unit(int64_t n, int64_t vocab, int64_t dim, int dtype) {
+    const double product = 2.0 * static_cast<double>(n) * vocab * dim * (dtype == ME_F32 ? 6 : 1) / 1.2e15;
+    const double read = static_cast<double>(vocab) * dim * (dtype == ME_F32 ? 6 : 2) / 5e12;
+    return std::max(product, read) > 50e-6;
 }
 
 struct Call {
@@ -626,13 +922,17 @@ void lay_out(bool f32, const Layout &l, hipStream_t s) {
         hipLaunchKernelGGL(layout_kernel<false>, dim3(blocks), dim3(256), 0, s, l);
 }
 
-int64_t h_part(const Plan &p) { return round_up(std::max<int64_t>(p.n, 1), 64) * p.ld * 2; }
+int64_t h_part(const Plan &p) { return p.rows * p.ld * 2; }
 
-void lay_out_hidden(const Plan &p, const Call &c) {
-    lay_out(p.f32, Layout{c.hidden, c.per_batch, c.batch_stride, c.row_stride, c.s.rows, c.s.count, p.n, p.dim, p.ld, h_part(p), c.ws + p.h}, c.stream);
+Layout hidden_layout(const Plan &p, const Call &c) {
+    return {c.hidden, c.per_batch, c.batch_stride, c.row_stride, c.s.rows, c.s.count, p.n, p.dim, p.ld, h_part(p), c.ws + p.h};
 }
 
-Operand hidden_operand(const Plan &p, const Call &c) { return {c.ws + p.h, p.ld, h_part(p)}; }
+// Rows of a product: the hidden states laid out, with how many there are and their targets
+struct Rows {
+    uint8_t *h;
+    const int32_t *count, *tgt;
+};
 
 // The head from row v0 on, `width` rows of it
 Operand weight_operand(const Plan &p, const Call &c, int64_t v0, int64_t width) {
@@ -656,57 +956,171 @@ void multiply_few(const Gemm &g, const Epilogue &e, hipStream_t s) {
     hipLaunchKernelGGL((few_kernel<B_KC, kTS, kRing, SEGS, Epilogue>), grid, dim3(kThreads), 0, s, g, e);
 }
 
-// logits of a piece: hidden [counted rows] x head rows
+// logits of a piece: rows x head rows
 template <int SEGS, class Epilogue>
-void logits_of(const Plan &p, const Call &c, const Operand &w, int64_t width, const Epilogue &e) {
-    Gemm g{hidden_operand(p, c), w, p.n, width, p.dim, c.s.count, 0, 8, 1};
+void logits_of(const Plan &p, const Call &c, const Rows &rows, const Operand &w, int64_t width, const Epilogue &e) {
+    const Gemm g{{rows.h, p.ld, h_part(p)}, w, p.n, width, p.dim, rows.count, 0, 8, 1};
     if (p.few)
         multiply_few<true, SEGS>(g, e, c.stream);
     else
         multiply_large<true, true, SEGS>(g, e, c.stream);
 }
 
-int forward(const Plan &p, const Call &c, double temperature, float *logps, float *loss, double smoothing, double z_loss, double scale, int mean) {
-    int32_t *tgt = reinterpret_cast<int32_t *>(c.ws + p.tgt);
-    if (c.tdtype == ME_I64)
-        hipLaunchKernelGGL(index_kernel<int64_t>, dim3(1), dim3(kIndexThreads), 0, c.stream, static_cast<const int64_t *>(c.targets), p.n, c.ignore, p.vocab, c.s, tgt);
+// product of a piece of the logits' gradient (or exponentials) with the head, onto the sums
+void times_head(const Plan &p, const Call &c, const Rows &rows, const Operand &w, int64_t v0, int64_t width) {
+    const Gemm g{{c.ws + p.g, p.piece, p.rows * p.piece * 2}, w, p.n, p.dim, width, rows.count, 0, 8, p.splits};
+    const AccumulateEpilogue e{reinterpret_cast<float *>(c.ws + p.acc), p.ld, p.rows * p.ld, v0 > 0};
+    if (p.few)
+        p.f32 ? multiply_few<false, 6>(g, e, c.stream) : multiply_few<false, 1>(g, e, c.stream);
     else
-        hipLaunchKernelGGL(index_kernel<int32_t>, dim3(1), dim3(kIndexThreads), 0, c.stream, static_cast<const int32_t *>(c.targets), p.n, c.ignore, p.vocab, c.s, tgt);
-    FinishArgs f{};
-    if (p.n > 0) {
-        lay_out_hidden(p, c);
-        const int cols = p.few ? 64 : 128;
-        const int64_t rows = round_up(p.n, 64);
-        StatsEpilogue e{};
-        e.tgt = tgt;
-        e.part = reinterpret_cast<float2 *>(c.ws + p.part);
-        e.sum = smoothing != 0.0 ? reinterpret_cast<float *>(c.ws + p.sum) : nullptr;
-        e.at_target = reinterpret_cast<float *>(c.ws + p.at_target);
-        const int parts = static_cast<int>(ceil_div(p.vocab, cols));
-        e.part_stride = p.few ? 1 : rows;
-        e.row_stride = p.few ? parts + 4 : 1;
-        e.k = static_cast<float>(1.44269504088896340736 / temperature);
+        p.f32 ? multiply_large<true, false, 6>(g, e, c.stream) : multiply_large<true, false, 1>(g, e, c.stream);
+}
+
+void gradient_of(const Plan &p, const Call &c, const Rows &rows, const Operand &w, int64_t v0, int64_t width, const RowGrad *grad, float k) {
+    const int64_t part = p.rows * p.piece * 2;
+    if (p.f32)
+        logits_of<6>(p, c, rows, w, width, GradEpilogue<3>{rows.tgt, grad, c.ws + p.g, p.piece, part, v0, width, k});
+    else
+        logits_of<1>(p, c, rows, w, width, GradEpilogue<1>{rows.tgt, grad, c.ws + p.g, p.piece, part, v0, width, k});
+}
+
+void finish(const Plan &p, const FinishArgs &f, hipStream_t s) {
+    if (p.few)
+        hipLaunchKernelGGL(finish_kernel<true>, dim3(static_cast<unsigned>(p.n)), dim3(256), 0, s, f);
+    else
+        hipLaunchKernelGGL(finish_kernel<false>, dim3(static_cast<unsigned>(ceil_div(p.n, 16))), dim3(256), 0, s, f);
+}
+
+struct Loss {
+    double temperature, smoothing, z_loss, scale;
+    int mean;
+    float *logps, *loss;  // one of them
+    float *unit;          // D, or null
+};
+
+unsigned row_blocks(int64_t n) { return static_cast<unsigned>(std::max<int64_t>(ceil_div(n, 256), 1)); }
+
+// D from the sums of the products with the head
+void unit_of(const Plan &p, const Call &c, const Loss &l, const Rows &rows, const int32_t *which, const float *ref) {
+    UnitArgs u{};
+    u.sums = reinterpret_cast<const float *>(c.ws + p.acc);
+    u.ld = p.ld, u.split_stride = p.rows * p.ld, u.splits = p.splits;
+    u.s = c.s, u.count = rows.count, u.which = which, u.tgt = rows.tgt, u.ref = ref;
+    u.weight = c.weight, u.w_stride = c.w_stride, u.dim = p.dim, u.n = p.n;
+    u.z_loss = static_cast<float>(l.z_loss), u.smoothing = static_cast<float>(l.smoothing);
+    u.columns = l.smoothing != 0.0 ? reinterpret_cast<const float *>(c.ws + p.columns) : nullptr;
+    u.vocab = static_cast<double>(p.vocab);
+    u.unit = l.unit;
+    const unsigned blocks = blocks_for(p.n * ceil_div(p.dim, 4));
+    if (p.f32)
+        hipLaunchKernelGGL(unit_kernel<true>, dim3(blocks), dim3(256), 0, c.stream, u);
+    else
+        hipLaunchKernelGGL(unit_kernel<false>, dim3(blocks), dim3(256), 0, c.stream, u);
+}
+
+void forward_rows(const Plan &p, const Call &c, const Loss &l) {
+    hipStream_t s = c.stream;
+    const Rows rows{c.ws + p.h, c.s.count, reinterpret_cast<int32_t *>(c.ws + p.tgt)};
+    const Layout h = hidden_layout(p, c);
+    lay_out(p.f32, h, s);
+    const int cols = p.few ? 64 : 128;
+    const int parts = static_cast<int>(ceil_div(p.vocab, cols));
+    const float k = static_cast<float>(1.44269504088896340736 / l.temperature);
+    float *at_target = reinterpret_cast<float *>(c.ws + p.at_target);
+
+    StatsEpilogue e{};
+    e.tgt = rows.tgt;
+    e.part = reinterpret_cast<float2 *>(c.ws + p.part);
+    e.sum = l.smoothing != 0.0 ? reinterpret_cast<float *>(c.ws + p.sum) : nullptr;
+    e.at_target = at_target;
+    e.part_stride = p.few ? 1 : p.rows;
+    e.row_stride = p.few ? parts + 4 : 1;
+    e.k = k;
+    auto stats = [&](const Rows &of) {
+        e.tgt = of.tgt;
         for (int64_t v0 = 0; v0 < p.vocab; v0 += p.piece) {
             const int64_t width = std::min(p.piece, p.vocab - v0);
             e.first = v0, e.vocab = width;
             const Operand w = weight_operand(p, c, v0, width);
             if (p.f32)
-                logits_of<6>(p, c, w, width, e);
+                logits_of<6>(p, c, of, w, width, e);
             else
-                logits_of<1>(p, c, w, width, e);
+                logits_of<1>(p, c, of, w, width, e);
         }
-        f.part = e.part, f.sum = e.sum, f.at_target = e.at_target, f.part_stride = e.part_stride, f.row_stride = e.row_stride, f.parts = parts;
-        f.n = p.n, f.vocab = p.vocab, f.s = c.s, f.logps = logps;
-        f.row_loss = loss ? reinterpret_cast<float *>(c.ws + p.row_loss) : nullptr;
-        f.smoothing = static_cast<float>(smoothing), f.z_loss = static_cast<float>(z_loss);
-        if (p.few)
-            hipLaunchKernelGGL(finish_kernel<true>, dim3(static_cast<unsigned>(p.n)), dim3(256), 0, c.stream, f);
-        else
-            hipLaunchKernelGGL(finish_kernel<false>, dim3(static_cast<unsigned>(ceil_div(p.n, 64))), dim3(256), 0, c.stream, f);
-        if (logps)
-            hipLaunchKernelGGL(uncounted_logps_kernel, dim3(static_cast<unsigned>(ceil_div(p.n, 256))), dim3(256), 0, c.stream, c.s.place, p.n, logps);
+    };
+    FinishArgs f{};
+    f.part = e.part, f.sum = e.sum, f.at_target = at_target, f.part_stride = e.part_stride, f.row_stride = e.row_stride, f.parts = parts;
+    f.n = p.n, f.vocab = p.vocab, f.s = c.s, f.logps = l.logps;
+    f.row_loss = l.loss ? reinterpret_cast<float *>(c.ws + p.row_loss) : nullptr;
+    f.smoothing = static_cast<float>(l.smoothing), f.z_loss = static_cast<float>(l.z_loss);
+    if (!l.unit) {
+        stats(rows);
+        finish(p, f, s);
+        return;
     }
-    if (loss) hipLaunchKernelGGL(total_kernel, dim3(1), dim3(1024), 0, c.stream, reinterpret_cast<const float *>(c.ws + p.row_loss), c.s.count, scale, mean, loss);
+    float *ref = reinterpret_cast<float *>(c.ws + p.ref);
+    const unsigned waves = static_cast<unsigned>(ceil_div(p.n, 4));
+    if (p.f32)
+        hipLaunchKernelGGL(ref_kernel<true>, dim3(waves), dim3(256), 0, s, h, c.weight, c.w_stride, rows.tgt, k, ref);
+    else
+        hipLaunchKernelGGL(ref_kernel<false>, dim3(waves), dim3(256), 0, s, h, c.weight, c.w_stride, rows.tgt, k, ref);
+    if (l.smoothing != 0.0) {
+        const dim3 grid(static_cast<unsigned>(ceil_div(p.dim, 256)), static_cast<unsigned>(ceil_div(p.vocab, kColumnRows)));
+        float *part = reinterpret_cast<float *>(c.ws + p.column_part);
+        if (p.f32)
+            hipLaunchKernelGGL(column_kernel<true>, grid, dim3(256), 0, s, c.weight, c.w_stride, p.vocab, p.dim, part);
+        else
+            hipLaunchKernelGGL(column_kernel<false>, grid, dim3(256), 0, s, c.weight, c.w_stride, p.vocab, p.dim, part);
+        hipLaunchKernelGGL(column_total_kernel, dim3(grid.x), dim3(256), 0, s, part, static_cast<int>(grid.y), p.dim, reinterpret_cast<float *>(c.ws + p.columns));
+    }
+    float *exps = reinterpret_cast<float *>(c.ws + p.part);
+    const int64_t out_part = p.rows * p.piece * 2;
+    for (int64_t v0 = 0; v0 < p.vocab; v0 += p.piece) {
+        const int64_t width = std::min(p.piece, p.vocab - v0);
+        const Operand w = weight_operand(p, c, v0, width);
+        if (p.f32)
+            logits_of<6>(p, c, rows, w, width, ExpEpilogue<3>{rows.tgt, ref, exps, e.sum, at_target, e.part_stride, e.row_stride, c.ws + p.g, p.piece, out_part, v0, width, k});
+        else
+            logits_of<1>(p, c, rows, w, width, ExpEpilogue<1>{rows.tgt, ref, exps, e.sum, at_target, e.part_stride, e.row_stride, c.ws + p.g, p.piece, out_part, v0, width, k});
+        times_head(p, c, rows, w, v0, width);
+    }
+    f.exps = exps, f.ref = ref;
+    finish(p, f, s);
+    unit_of(p, c, l, rows, nullptr, ref);
+
+    // rows that ref was too far from
+    int32_t *redo = reinterpret_cast<int32_t *>(c.ws + p.redo);
+    int32_t *tgt2 = reinterpret_cast<int32_t *>(c.ws + p.tgt2);
+    RowGrad *grad = reinterpret_cast<RowGrad *>(c.ws + p.grad);
+    const Rows again{c.ws + p.h2, redo, tgt2};
+    hipLaunchKernelGGL(redo_kernel, dim3(1), dim3(kIndexThreads), 0, s, RedoArgs{c.s, ref, rows.tgt, redo, redo + kHeader, tgt2});
+    for (int part = 0; part < p.np; ++part)
+        lay_out(false, Layout{c.ws + p.h + part * h_part(p), std::max<int64_t>(p.n, 1), 0, p.ld, redo + kHeader, redo, p.n, p.ld, p.ld, 0, again.h + part * h_part(p)}, s);
+    stats(again);
+    f.exps = nullptr, f.ref = nullptr, f.count = redo, f.which = redo + kHeader;
+    finish(p, f, s);
+    hipLaunchKernelGGL(redo_coef_kernel, dim3(row_blocks(p.n)), dim3(256), 0, s, c.s, redo, redo + kHeader, f.z_loss, grad);
+    for (int64_t v0 = 0; v0 < p.vocab; v0 += p.piece) {
+        const int64_t width = std::min(p.piece, p.vocab - v0);
+        const Operand w = weight_operand(p, c, v0, width);
+        gradient_of(p, c, again, w, v0, width, grad, k);
+        times_head(p, c, again, w, v0, width);
+    }
+    unit_of(p, c, l, again, redo + kHeader, nullptr);
+}
+
+int forward(const Plan &p, const Call &c, const Loss &l) {
+    int32_t *tgt = reinterpret_cast<int32_t *>(c.ws + p.tgt);
+    hipStream_t s = c.stream;
+    if (c.tdtype == ME_I64)
+        hipLaunchKernelGGL(index_kernel<int64_t>, dim3(1), dim3(kIndexThreads), 0, s, static_cast<const int64_t *>(c.targets), p.n, c.ignore, p.vocab, c.s, tgt);
+    else
+        hipLaunchKernelGGL(index_kernel<int32_t>, dim3(1), dim3(kIndexThreads), 0, s, static_cast<const int32_t *>(c.targets), p.n, c.ignore, p.vocab, c.s, tgt);
+    if (p.n > 0) {
+        forward_rows(p, c, l);
+        if (l.logps) hipLaunchKernelGGL(uncounted_logps_kernel, dim3(row_blocks(p.n)), dim3(256), 0, s, c.s.place, p.n, l.logps);
+    }
+    if (l.loss) hipLaunchKernelGGL(total_kernel, dim3(1), dim3(1024), 0, s, reinterpret_cast<const float *>(c.ws + p.row_loss), c.s.count, l.scale, l.mean, l.loss);
     return check_launch("me_head");
 }
 
@@ -731,107 +1145,117 @@ int check_call(const void *hidden, int dtype, int64_t n, int64_t dim, int64_t pe
 
 using namespace me;
 
-extern "C" int me_head_workspace_size(int64_t n, int64_t vocab, int64_t dim, int dtype, const void *weight, int64_t w_stride, int backward,
+extern "C" int me_head_workspace_size(int64_t n, int64_t vocab, int64_t dim, int dtype, const void *weight, int64_t w_stride, int pass,
                                       size_t *bytes) {
-    ME_CHECK_ARG(bytes && n >= 0 && vocab >= 1 && dim >= 1, "bad sizes");
-    *bytes = static_cast<size_t>(plan_of(n, vocab, dim, dtype, weight, w_stride, backward != 0).bytes);
+    ME_CHECK_ARG(bytes && n >= 0 && vocab >= 1 && dim >= 1 && pass >= 0 && pass <= 2, "bad sizes");
+    *bytes = static_cast<size_t>(plan_of(n, vocab, dim, dtype, weight, w_stride, static_cast<Pass>(pass)).bytes);
+    return ME_OK;
+}
+
+extern "C" int me_head_unit_size(int64_t n, int64_t vocab, int64_t dim, int dtype, int64_t *elements) {
+    ME_CHECK_ARG(elements && n >= 0 && vocab >= 1 && dim >= 1, "bad sizes");
+    *elements = n > 0 && leaves_unit(n, vocab, dim, dtype) ? n * ceil_div(dim, 4) * 4 : 0;
     return ME_OK;
 }
 
 extern "C" int me_head_logps(const void *hidden, int dtype, int64_t n, int64_t dim, int64_t rows_per_batch, int64_t batch_stride,
                              int64_t row_stride, const void *weight, int64_t vocab, int64_t w_stride, const void *targets, int targets_dtype,
-                             int64_t ignore_index, double temperature, float *logps, void *saved, void *workspace, size_t workspace_bytes,
-                             void *stream) {
+                             int64_t ignore_index, double temperature, float *logps, void *saved, float *unit, void *workspace,
+                             size_t workspace_bytes, void *stream) {
     const int rc = check_call(hidden, dtype, n, dim, rows_per_batch, weight, vocab, w_stride, targets, targets_dtype, temperature, saved, workspace);
     if (rc != ME_OK) return rc;
-    const Plan p = plan_of(n, vocab, dim, dtype, weight, w_stride, false);
+    const Plan p = plan_of(n, vocab, dim, dtype, weight, w_stride, unit ? kLeavesUnit : kStats);
     ME_CHECK_ARG(workspace_bytes >= static_cast<size_t>(p.bytes), "workspace of %zu bytes, %lld are needed", workspace_bytes, static_cast<long long>(p.bytes));
     ME_CHECK_ARG(n == 0 || logps, "logps is needed");
+    ME_CHECK_ARG(reinterpret_cast<uintptr_t>(unit) % 16 == 0, "unit must be 16-byte aligned");
     const Call c{hidden, weight, targets, rows_per_batch, batch_stride, row_stride, w_stride, ignore_index, targets_dtype,
                  static_cast<uint8_t *>(workspace), saved_of(saved, n), as_stream(stream)};
-    return forward(p, c, temperature, logps, nullptr, 0.0, 0.0, 1.0, 0);
+    return forward(p, c, Loss{temperature, 0.0, 0.0, 1.0, 0, logps, nullptr, unit});
 }
 
 extern "C" int me_head_ce(const void *hidden, int dtype, int64_t n, int64_t dim, int64_t rows_per_batch, int64_t batch_stride,
                           int64_t row_stride, const void *weight, int64_t vocab, int64_t w_stride, const void *targets, int targets_dtype,
                           int64_t ignore_index, double temperature, double smoothing, double z_loss, double scale, int reduction, float *loss,
-                          void *saved, void *workspace, size_t workspace_bytes, void *stream) {
+                          void *saved, float *unit, void *workspace, size_t workspace_bytes, void *stream) {
     const int rc = check_call(hidden, dtype, n, dim, rows_per_batch, weight, vocab, w_stride, targets, targets_dtype, temperature, saved, workspace);
     if (rc != ME_OK) return rc;
     ME_CHECK_ARG(reduction == ME_REDUCE_MEAN || reduction == ME_REDUCE_SUM, "reduction must be mean or sum");
     ME_CHECK_ARG(loss, "loss is needed");
-    const Plan p = plan_of(n, vocab, dim, dtype, weight, w_stride, false);
+    ME_CHECK_ARG(reinterpret_cast<uintptr_t>(unit) % 16 == 0, "unit must be 16-byte aligned");
+    const Plan p = plan_of(n, vocab, dim, dtype, weight, w_stride, unit ? kLeavesUnit : kStats);
     ME_CHECK_ARG(workspace_bytes >= static_cast<size_t>(p.bytes), "workspace of %zu bytes, %lld are needed", workspace_bytes, static_cast<long long>(p.bytes));
     const Call c{hidden, weight, targets, rows_per_batch, batch_stride, row_stride, w_stride, ignore_index, targets_dtype,
                  static_cast<uint8_t *>(workspace), saved_of(saved, n), as_stream(stream)};
-    return forward(p, c, temperature, nullptr, loss, smoothing, z_loss, scale, reduction == ME_REDUCE_MEAN);
+    return forward(p, c, Loss{temperature, smoothing, z_loss, scale, reduction == ME_REDUCE_MEAN, nullptr, loss, unit});
 }
 
 extern "C" int me_head_backward(const void *hidden, int dtype, int64_t n, int64_t dim, int64_t rows_per_batch, int64_t batch_stride,
                                 int64_t row_stride, const void *weight, int64_t vocab, int64_t w_stride, const void *targets,
                                 int targets_dtype, int64_t ignore_index, double temperature, const float *upstream, int upstream_per_row,
-                                double smoothing, double z_loss, double scale, int reduction, const void *saved, void *grad_hidden,
-                                void *grad_weight, void *workspace, size_t workspace_bytes, void *stream) {
-    const int rc = check_call(hidden, dtype, n, dim, rows_per_batch, weight, vocab, w_stride, targets, targets_dtype, temperature, saved, workspace);
+                                double smoothing, double z_loss, double scale, int reduction, const void *saved, const float *unit,
+                                void *grad_hidden, void *grad_weight, void *workspace, size_t workspace_bytes, void *stream) {
+    const int rc = check_call(hidden, dtype, n, dim, rows_per_batch, weight, vocab, w_stride, targets, targets_dtype, temperature, saved,
+                              unit ? saved : workspace);
     if (rc != ME_OK) return rc;
     ME_CHECK_ARG(upstream || (n == 0 && upstream_per_row), "upstream is needed");
-    const Plan p = plan_of(n, vocab, dim, dtype, weight, w_stride, true);
-    ME_CHECK_ARG(workspace_bytes >= static_cast<size_t>(p.bytes), "workspace of %zu bytes, %lld are needed", workspace_bytes, static_cast<long long>(p.bytes));
     ME_CHECK_ARG(reinterpret_cast<uintptr_t>(grad_hidden) % 16 == 0 && reinterpret_cast<uintptr_t>(grad_weight) % 16 == 0, "gradients must be 16-byte aligned");
+    ME_CHECK_ARG(!unit || !grad_weight, "unit is for the hidden states' gradient alone");
     if (!grad_hidden && !grad_weight) return ME_OK;
+    const Saved saved_rows = saved_of(const_cast<void *>(saved), n);
+    const bool f32 = dtype == ME_F32;
+    if (unit) {
+        if (n == 0) return ME_OK;
+        const ScaleArgs a{unit, saved_rows.count, saved_rows.place, upstream, upstream_per_row != 0, reduction == ME_REDUCE_MEAN, scale / temperature, n, dim, grad_hidden};
+        const unsigned blocks = blocks_for(n * ceil_div(dim, 4));
+        if (f32)
+            hipLaunchKernelGGL(scale_kernel<true>, dim3(blocks), dim3(256), 0, as_stream(stream), a);
+        else
+            hipLaunchKernelGGL(scale_kernel<false>, dim3(blocks), dim3(256), 0, as_stream(stream), a);
+        return check_launch("me_head_backward");
+    }
+    const Plan p = plan_of(n, vocab, dim, dtype, weight, w_stride, kBackward);
+    ME_CHECK_ARG(workspace_bytes >= static_cast<size_t>(p.bytes), "workspace of %zu bytes, %lld are needed", workspace_bytes, static_cast<long long>(p.bytes));
     const Call c{hidden, weight, targets, rows_per_batch, batch_stride, row_stride, w_stride, ignore_index, targets_dtype,
-                 static_cast<uint8_t *>(workspace), saved_of(const_cast<void *>(saved), n), as_stream(stream)};
+                 static_cast<uint8_t *>(workspace), saved_rows, as_stream(stream)};
     hipStream_t s = c.stream;
     int32_t *tgt = reinterpret_cast<int32_t *>(c.ws + p.tgt);
+    const Rows rows{c.ws + p.h, c.s.count, tgt};
     RowGrad *grad = reinterpret_cast<RowGrad *>(c.ws + p.grad);
-    const unsigned row_blocks = static_cast<unsigned>(std::max<int64_t>(ceil_div(n, 256), 1));
     if (n > 0) {
+        const dim3 blocks(row_blocks(n));
         if (targets_dtype == ME_I64)
-            hipLaunchKernelGGL(targets_kernel<int64_t>, dim3(row_blocks), dim3(256), 0, s, static_cast<const int64_t *>(targets), n, c.s.rows, c.s.count, tgt);
+            hipLaunchKernelGGL(targets_kernel<int64_t>, blocks, dim3(256), 0, s, static_cast<const int64_t *>(targets), n, c.s.rows, c.s.count, tgt);
         else
-            hipLaunchKernelGGL(targets_kernel<int32_t>, dim3(row_blocks), dim3(256), 0, s, static_cast<const int32_t *>(targets), n, c.s.rows, c.s.count, tgt);
-        CoefArgs k{c.s, n, upstream, upstream_per_row != 0, reduction == ME_REDUCE_MEAN, scale / temperature, static_cast<float>(smoothing),
-                   static_cast<float>(z_loss), static_cast<double>(vocab), grad};
-        hipLaunchKernelGGL(coef_kernel, dim3(row_blocks), dim3(256), 0, s, k);
-        lay_out_hidden(p, c);
+            hipLaunchKernelGGL(targets_kernel<int32_t>, blocks, dim3(256), 0, s, static_cast<const int32_t *>(targets), n, c.s.rows, c.s.count, tgt);
+        const CoefArgs k{c.s, n, upstream, upstream_per_row != 0, reduction == ME_REDUCE_MEAN, scale / temperature, static_cast<float>(smoothing),
+                         static_cast<float>(z_loss), static_cast<double>(vocab), grad};
+        hipLaunchKernelGGL(coef_kernel, blocks, dim3(256), 0, s, k);
+        lay_out(p.f32, hidden_layout(p, c), s);
     }
-    const int64_t rows = round_up(std::max<int64_t>(n, 1), 64);
-    const int64_t g_part = rows * p.piece * 2;
-    float *acc = reinterpret_cast<float *>(c.ws + p.acc);
     const float k = static_cast<float>(1.44269504088896340736 / temperature);
     for (int64_t v0 = 0; v0 < vocab; v0 += p.piece) {
         const int64_t width = std::min(p.piece, vocab - v0);
-        const Operand dz{c.ws + p.g, p.piece, g_part};
         if (n > 0) {
             const Operand w = weight_operand(p, c, v0, width);
-            if (p.f32)
-                logits_of<6>(p, c, w, width, GradEpilogue<3>{tgt, grad, c.ws + p.g, p.piece, g_part, v0, width, k});
-            else
-                logits_of<1>(p, c, w, width, GradEpilogue<1>{tgt, grad, c.ws + p.g, p.piece, g_part, v0, width, k});
-            if (grad_hidden) {
-                const Gemm g{dz, w, n, dim, width, c.s.count, 0, 8, p.splits};
-                const AccumulateEpilogue e{acc, p.ld, rows * p.ld, v0 > 0};
-                if (p.few)
-                    p.f32 ? multiply_few<false, 6>(g, e, s) : multiply_few<false, 1>(g, e, s);
-                else
-                    p.f32 ? multiply_large<true, false, 6>(g, e, s) : multiply_large<true, false, 1>(g, e, s);
-            }
+            gradient_of(p, c, rows, w, v0, width, grad, k);
+            if (grad_hidden) times_head(p, c, rows, w, v0, width);
         }
         if (grad_weight) {
-            const Gemm g{dz, hidden_operand(p, c), width, dim, n, c.s.count, 1, 8, 1};
-            uint8_t *out = static_cast<uint8_t *>(grad_weight) + v0 * dim * (p.f32 ? 4 : 2);
-            if (p.f32)
+            const Gemm g{{c.ws + p.g, p.piece, p.rows * p.piece * 2}, {c.ws + p.h, p.ld, h_part(p)}, width, dim, n, c.s.count, 1, 8, 1};
+            uint8_t *out = static_cast<uint8_t *>(grad_weight) + v0 * dim * (f32 ? 4 : 2);
+            if (f32)
                 multiply_large<false, false, 6>(g, WeightEpilogue<true>{out, dim}, s);
             else
                 multiply_large<false, false, 1>(g, WeightEpilogue<false>{out, dim}, s);
         }
     }
     if (grad_hidden && n > 0) {
+        const float *acc = reinterpret_cast<const float *>(c.ws + p.acc);
         const unsigned blocks = blocks_for(n * ceil_div(dim, 4));
-        if (p.f32)
-            hipLaunchKernelGGL(hidden_kernel<true>, dim3(blocks), dim3(256), 0, s, acc, p.ld, rows * p.ld, p.splits, c.s.place, n, dim, grad_hidden);
+        if (f32)
+            hipLaunchKernelGGL(hidden_kernel<true>, dim3(blocks), dim3(256), 0, s, acc, p.ld, p.rows * p.ld, p.splits, c.s.place, n, dim, grad_hidden);
         else
-            hipLaunchKernelGGL(hidden_kernel<false>, dim3(blocks), dim3(256), 0, s, acc, p.ld, rows * p.ld, p.splits, c.s.place, n, dim, grad_hidden);
+            hipLaunchKernelGGL(hidden_kernel<false>, dim3(blocks), dim3(256), 0, s, acc, p.ld, p.rows * p.ld, p.splits, c.s.place, n, dim, grad_hidden);
     }
     return check_launch("me_head_backward");
 }

@@ -2,13 +2,16 @@
 loss_ops.py. losses.py is the surface for users.
 """
 import ctypes
-from typing import List
+import functools
+from typing import List, Optional
 
 import torch
 
 from ._lib import call
 from .loss_ops import _targets, row_layout
-from .ops import _custom_op, call_on, dtype_code, require_gpu
+from .ops import _custom_op, _p, call_on, dtype_code, require_gpu
+
+_FORWARD, _BACKWARD, _FORWARD_UNIT = 0, 1, 2
 
 
 def weight_layout(weight):
@@ -27,71 +30,88 @@ def _operands(hidden, weight, targets, ignore_index):
     return (hidden, weight, targets), (*rows, *head, *toks)
 
 
-def _workspace(hidden, weight, head, n, backward):
+def _workspace(hidden, operands, which):
     """(buffer, address, size)."""
     size = ctypes.c_size_t(0)
-    call("me_head_workspace_size", n, head[1], weight.shape[1], dtype_code(weight), head[0], head[2], backward, ctypes.byref(size))
+    call("me_head_workspace_size", operands[2], operands[8], operands[3], operands[1], operands[7], operands[9], which, ctypes.byref(size))
     ws = torch.empty(size.value, dtype=torch.uint8, device=hidden.device)
     return ws, ws.data_ptr(), ws.numel()
 
 
-def _forward(name, hidden, weight, targets, ignore_index, out, args):
+@functools.lru_cache(maxsize=256)
+def unit_elements(n, vocab, dim, dtype):
+    """Size of what a forward leaves for the gradient of hidden alone; 0: nothing."""
+    size = ctypes.c_int64(0)
+    call("me_head_unit_size", n, vocab, dim, dtype, ctypes.byref(size))
+    return size.value
+
+
+def _unit_size(hidden, weight, targets):
+    return unit_elements(targets.numel(), weight.shape[0], weight.shape[1], dtype_code(weight))
+
+
+def _forward(name, hidden, weight, targets, ignore_index, with_unit, out, args):
     dev = require_gpu(hidden, weight, targets)
     held, operands = _operands(hidden, weight, targets, ignore_index)
-    n = operands[2]
-    saved = torch.empty(16 + 4 * n, dtype=torch.float32, device=dev)
-    ws, ptr, size = _workspace(held[0], held[1], operands[7:10], n, 0)
-    call_on(dev, name, *operands, *args, out.data_ptr(), saved.data_ptr(), ptr, size)
-    return [out, saved]
+    saved = torch.empty(16 + 4 * operands[2], dtype=torch.float32, device=dev)
+    size = _unit_size(hidden, weight, targets) if with_unit else 0
+    unit = torch.empty(size, dtype=torch.float32, device=dev) if size else None
+    ws, ptr, size = _workspace(held[0], operands, _FORWARD if unit is None else _FORWARD_UNIT)
+    call_on(dev, name, *operands, *args, out.data_ptr(), saved.data_ptr(), _p(unit), ptr, size)
+    return [out, saved] if unit is None else [out, saved, unit]
+
+
+def _fake_forward(hidden, weight, targets, with_unit, shape):
+    res = [hidden.new_empty(shape, dtype=torch.float32), hidden.new_empty((16 + 4 * targets.numel(),), dtype=torch.float32)]
+    size = _unit_size(hidden, weight, targets) if with_unit else 0
+    return [*res, hidden.new_empty((size,), dtype=torch.float32)] if size else res
 
 
 @_custom_op("head_logps")
 def head_logps(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, ignore_index: int,
-               temperature: float) -> List[torch.Tensor]:
-    """[log-probabilities fp32 of targets' shape, saved (what the backward needs)]."""
+               temperature: float, with_unit: bool) -> List[torch.Tensor]:
+    """[log-probabilities fp32 of targets' shape, saved (what the backward needs)], and where with_unit and the size pays
+    unit, from which the backward of hidden alone only scales."""
     out = torch.empty(targets.shape, dtype=torch.float32, device=targets.device)
-    return _forward("me_head_logps", hidden, weight, targets, ignore_index, out, (temperature,))
+    return _forward("me_head_logps", hidden, weight, targets, ignore_index, with_unit, out, (temperature,))
 
 
 @head_logps.register_fake
-def _(hidden, weight, targets, ignore_index, temperature):
-    return [hidden.new_empty(targets.shape, dtype=torch.float32),
-            hidden.new_empty((16 + 4 * targets.numel(),), dtype=torch.float32)]
+def _(hidden, weight, targets, ignore_index, temperature, with_unit):
+    return _fake_forward(hidden, weight, targets, with_unit, targets.shape)
 
 
 @_custom_op("head_ce")
 def head_ce(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, ignore_index: int, temperature: float,
-            smoothing: float, z_loss: float, scale: float, reduction: int) -> List[torch.Tensor]:
-    """[loss fp32, saved]."""
+            smoothing: float, z_loss: float, scale: float, reduction: int, with_unit: bool) -> List[torch.Tensor]:
+    """[loss fp32, saved], and unit as of head_logps."""
     out = torch.empty((), dtype=torch.float32, device=targets.device)
-    return _forward("me_head_ce", hidden, weight, targets, ignore_index, out,
+    return _forward("me_head_ce", hidden, weight, targets, ignore_index, with_unit, out,
                     (temperature, smoothing, z_loss, scale, reduction))
 
 
 @head_ce.register_fake
-def _(hidden, weight, targets, ignore_index, temperature, smoothing, z_loss, scale, reduction):
-    return [hidden.new_empty((), dtype=torch.float32), hidden.new_empty((16 + 4 * targets.numel(),), dtype=torch.float32)]
+def _(hidden, weight, targets, ignore_index, temperature, smoothing, z_loss, scale, reduction, with_unit):
+    return _fake_forward(hidden, weight, targets, with_unit, ())
 
 
 @_custom_op("head_backward")
 def head_backward(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, saved: torch.Tensor,
-                  upstream: torch.Tensor, ignore_index: int, temperature: float, per_row: bool, smoothing: float,
-                  z_loss: float, scale: float, reduction: int, need_hidden: bool, need_weight: bool) -> List[torch.Tensor]:
+                  unit: Optional[torch.Tensor], upstream: torch.Tensor, ignore_index: int, temperature: float, per_row: bool,
+                  smoothing: float, z_loss: float, scale: float, reduction: int, need_hidden: bool,
+                  need_weight: bool) -> List[torch.Tensor]:
     """The gradients that are needed, of hidden and of weight. upstream: fp32, one (head_ce) or per row (head_logps)."""
-    dev = require_gpu(hidden, weight, targets, saved, upstream)
+    dev = require_gpu(hidden, weight, targets, saved, unit, upstream)
     held, operands = _operands(hidden, weight, targets, ignore_index)
-    n = operands[2]
     grad_hidden = torch.empty(hidden.shape, dtype=hidden.dtype, device=dev) if need_hidden else None
     grad_weight = torch.empty(weight.shape, dtype=weight.dtype, device=dev) if need_weight else None
-    ws, ptr, size = _workspace(held[0], held[1], operands[7:10], n, 1)
-    grads = [g for g in (grad_hidden, grad_weight) if g is not None]
+    ws, ptr, size = _workspace(held[0], operands, _BACKWARD) if unit is None else (None, None, 0)
     call_on(dev, "me_head_backward", *operands, temperature, upstream.data_ptr(), int(per_row), smoothing, z_loss, scale,
-            reduction, saved.data_ptr(), grad_hidden.data_ptr() if need_hidden else None,
-            grad_weight.data_ptr() if need_weight else None, ptr, size)
-    return grads
+            reduction, saved.data_ptr(), _p(unit), _p(grad_hidden), _p(grad_weight), ptr, size)
+    return [g for g in (grad_hidden, grad_weight) if g is not None]
 
 
 @head_backward.register_fake
-def _(hidden, weight, targets, saved, upstream, ignore_index, temperature, per_row, smoothing, z_loss, scale, reduction,
-      need_hidden, need_weight):
+def _(hidden, weight, targets, saved, unit, upstream, ignore_index, temperature, per_row, smoothing, z_loss, scale,
+      reduction, need_hidden, need_weight):
     return [x.new_empty(x.shape) for x, need in ((hidden, need_hidden), (weight, need_weight)) if need]

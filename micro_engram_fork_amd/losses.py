@@ -385,27 +385,27 @@ class _HeadLoss(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, hidden, weight, targets, args):
-        out, saved = args[0](hidden.detach(), weight.detach(), targets, *args[1:])
-        ctx.save_for_backward(hidden, weight, targets, saved)
+        out, *kept = args[0](hidden.detach(), weight.detach(), targets, *args[1:], not weight.requires_grad)
+        ctx.save_for_backward(hidden, weight, targets, *kept)
         ctx.consts = args[1:]
         return out
 
     @staticmethod
     @_no_second_derivatives
     def backward(ctx, upstream):
-        hidden, weight, targets, saved = ctx.saved_tensors
+        hidden, weight, targets, saved, *unit = ctx.saved_tensors
         need = ctx.needs_input_grad[:2]
         per_row = len(ctx.consts) == 2
         ignore_index, temperature, *rest = ctx.consts if not per_row else (*ctx.consts, 0.0, 0.0, 1.0, ME_REDUCE_SUM)
-        grads = iter(head_ops.head_backward(hidden.detach(), weight.detach(), targets, saved, _upstream(upstream), ignore_index,
-                                            temperature, per_row, *rest, *need))
+        grads = iter(head_ops.head_backward(hidden.detach(), weight.detach(), targets, saved, unit[0] if unit else None,
+                                            _upstream(upstream), ignore_index, temperature, per_row, *rest, *need))
         return next(grads) if need[0] else None, next(grads) if need[1] else None, None, None
 
 
 def _head_loss(op, hidden, weight, targets, *args):
     if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
         return _HeadLoss.apply(hidden, weight, targets, (op, *args))
-    return op(hidden.detach(), weight.detach(), targets, *args)[0]
+    return op(hidden.detach(), weight.detach(), targets, *args, False)[0]
 
 
 def head_token_logps(hidden, weight, targets, temperature=1.0, ignore_index=IGNORE_INDEX):

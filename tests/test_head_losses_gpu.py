@@ -323,3 +323,139 @@ def test_compiled():
     g, = torch.autograd.grad(f(h), h)
     want, = torch.autograd.grad(losses.head_cross_entropy(h * 2, weight, targets), h)
     assert torch.equal(g, want)
+
+
+# ---- the hidden states' gradient alone, from the forward's exponentials ------------------------------------------
+@pytest.fixture
+def leaves_unit(monkeypatch):
+    """Calls of any size take that way, not those alone that are large enough for it to pay."""
+    from micro_engram_fork_amd import head_ops
+    monkeypatch.setattr(head_ops, "unit_elements", lambda n, vocab, dim, dtype: n * -(-dim // 4) * 4)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("n,vocab,dim", SIZES)
+def test_hidden_alone_at_the_ends_of_tiles(n, vocab, dim, dtype, leaves_unit):
+    _check_hidden_alone(*_inputs(n, vocab, dim, dtype))
+
+
+LARGE = [(130, 40_001, 264, BF16), (700, 33_000, 1_024, BF16), (70, 33_000, 1_000, FP32), (300, 20_001, 520, FP32), (3, 70_000, 2_048, BF16),
+         (9_000, 40_000, 64, BF16)]
+
+
+def _check_hidden_alone(hidden, weight, targets, upstream=None, label_smoothing=0.0, reduction="mean", **kw):
+    """Both losses and their gradients of hidden, where these leave what the backward scales."""
+    h = hidden.detach().requires_grad_()
+    loss = losses.head_cross_entropy(h, weight, targets, label_smoothing=label_smoothing, reduction=reduction, **kw)
+    want = ref.head(hidden, weight, targets, hidden.dtype, smoothing=label_smoothing, mean=reduction == "mean", **kw)
+    _close(loss, want["loss"], "loss")
+    _close(torch.autograd.grad(loss, h)[0], want["hidden"], "hidden of the loss")
+    up = torch.randn(targets.shape, device=DEV, generator=torch.Generator(device=DEV).manual_seed(9))
+    kw.pop("z_loss", None), kw.pop("scale", None)
+    logps = losses.head_token_logps(h, weight, targets, **kw)
+    want = ref.head(hidden, weight, targets, hidden.dtype, upstream=up, **kw)
+    _close(logps, want["logps"], "logps")
+    _close(torch.autograd.grad(logps, h, up)[0], want["hidden"], "hidden of logps")
+
+
+@pytest.mark.parametrize("n,vocab,dim,dtype", LARGE)
+def test_hidden_alone(n, vocab, dim, dtype, leaves_unit):
+    _check_hidden_alone(*_inputs(n, vocab, dim, dtype))
+
+
+@pytest.mark.parametrize("n", [100, 300])
+@pytest.mark.parametrize("kw", [dict(label_smoothing=0.1), dict(z_loss=1e-2, temperature=0.5), dict(reduction="sum", scale=-2.5, ignore_index=7),
+                                dict(label_smoothing=0.3, z_loss=1e-3, temperature=1.7, scale=0.01)])
+def test_hidden_alone_options(kw, n, leaves_unit):
+    hidden, weight, targets = _inputs(n, 40_000, 1_024, BF16)
+    targets[1] = 7
+    _check_hidden_alone(hidden, weight, targets, **kw)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("n", [40, 300])
+def test_hidden_alone_of_unlikely_targets(n, dtype, leaves_unit):
+    """Rows whose target is so unlikely that exponentials around it would overflow, between ordinary ones, and rows
+    that are not finite: each as it should be, and the others untouched by them."""
+    hidden, weight, targets = _inputs(n, 33_000, 1_024, dtype, masked=0.3)
+    some = torch.arange(n, device=DEV) % 7 == 3
+    hidden[some] *= 60.0
+    _check_hidden_alone(hidden, weight, targets)
+    _check_hidden_alone(hidden * 30, weight, targets)
+    h = hidden.clone()
+    h[5, 1], targets[5] = float("nan"), 3
+    h[6, 2], targets[6] = float("inf"), 4
+    h.requires_grad_()
+    logps = losses.head_token_logps(h, weight, targets)
+    assert bool(torch.isnan(logps[5])) and bool(torch.isnan(logps[6]))
+    up = torch.ones_like(logps)
+    g, = torch.autograd.grad(logps, h, up)
+    clean = torch.ones(n, dtype=torch.bool, device=DEV)
+    clean[5] = clean[6] = False
+    want = ref.head(hidden, weight, torch.where(clean, targets, -100), dtype, upstream=up)
+    assert bool(torch.isnan(g[5]).any()) and bool(torch.isnan(g[6]).any())
+    assert bool(((g.double() - want["hidden"][0]).abs() <= want["hidden"][1])[clean].all())
+
+
+def test_hidden_alone_strides_and_odd_heads(leaves_unit):
+    hidden, weight, _ = _inputs(400, 40_000, 1_000, BF16)
+    targets = torch.randint(0, 39_990, (2, 199), device=DEV)
+    view = hidden.view(2, 200, 1_000)[:, :-1, 1:]
+    odd = weight[5:39_995, 1:]
+    h = view.detach().requires_grad_()
+    logps = losses.head_token_logps(h, odd, targets)
+    up = torch.randn(targets.shape, device=DEV)
+    want = ref.head(view.reshape(-1, 999), odd, targets.reshape(-1), BF16, upstream=up.reshape(-1))
+    _close(logps, want["logps"])
+    _close(torch.autograd.grad(logps, h, up)[0], want["hidden"])
+
+
+@pytest.mark.parametrize("n", [100, 300])
+def test_hidden_alone_without_counted_rows(n, leaves_unit):
+    hidden, weight, targets = _inputs(n, 40_000, 1_024, BF16)
+    h = hidden.fill_(float("nan")).requires_grad_()
+    loss = losses.head_cross_entropy(h, weight, torch.full_like(targets, -100))
+    assert float(loss.detach()) == 0 and not torch.autograd.grad(loss, h)[0].any()
+
+
+def test_hidden_alone_captured_and_twice(leaves_unit):
+    hidden, weight, targets = _inputs(300, 40_000, 1_024, BF16)
+    h = hidden.requires_grad_()
+
+    def step():
+        loss = losses.head_cross_entropy(h, weight, targets, label_smoothing=0.1)
+        return [loss, *torch.autograd.grad(loss, h, retain_graph=True), *torch.autograd.grad(3 * loss, h)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for k in range(4):
+        new = _inputs(300, 40_000, 1_024, BF16, seed=30 + k, masked=0.25 * k)
+        with torch.no_grad():
+            h.copy_(new[0] * (60 if k == 2 else 1)), weight.copy_(new[1]), targets.copy_(new[2])
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [x.detach().clone() for x in captured]
+        want = [x.detach() for x in step()]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), k
+
+
+def test_hidden_alone_under_saved_tensor_hooks(leaves_unit):
+    hidden, weight, targets = _inputs(300, 40_000, 1_024, BF16)
+    h = hidden.requires_grad_()
+    want, = torch.autograd.grad(losses.head_cross_entropy(h, weight, targets), h)
+    with torch.autograd.graph.save_on_cpu():
+        loss = losses.head_cross_entropy(h, weight, targets)
+    assert torch.equal(torch.autograd.grad(loss, h)[0], want)
+
+
+def test_large_calls_for_hidden_alone_take_that_way():
+    from micro_engram_fork_amd import head_ops
+    hidden, weight, targets = _inputs(700, 33_000, 2_048, BF16)
+    assert head_ops._unit_size(hidden, weight, targets) == 700 * 2_048
+    _check_hidden_alone(hidden, weight, targets)

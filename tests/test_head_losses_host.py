@@ -41,7 +41,7 @@ def test_c_entry_checks():
     p = 4096  # an address that is not read
 
     def logps(dtype=_lib.ME_BF16, n=4, dim=8, vocab=11, stride=8, tdtype=_lib.ME_I64, temperature=1.0, size=1 << 40, ws=p, saved=p):
-        _lib.call("me_head_logps", p, dtype, n, dim, max(n, 1), 0, dim, p, vocab, stride, p, tdtype, -100, temperature, p, saved, ws, size, None)
+        _lib.call("me_head_logps", p, dtype, n, dim, max(n, 1), 0, dim, p, vocab, stride, p, tdtype, -100, temperature, p, saved, None, ws, size, None)
     for bad in (dict(dtype=_lib.ME_I32), dict(n=-1), dict(n=1 << 25), dict(dim=0), dict(dim=65537), dict(vocab=0), dict(vocab=1 << 22),
                 dict(stride=7), dict(stride=1 << 23), dict(tdtype=_lib.ME_F32), dict(temperature=0.0), dict(temperature=float("nan")),
                 dict(size=16), dict(ws=None), dict(saved=None), dict(ws=p + 8)):
@@ -51,12 +51,23 @@ def test_c_entry_checks():
 
 def test_fake_shapes():
     with FakeTensorMode():
-        hidden, weight, targets = (x.cuda() if False else x for x in _args())
-        out, saved = head_ops.head_logps(hidden, weight, targets, -100, 1.0)
+        hidden, weight, targets = _args()
+        out, saved = head_ops.head_logps(hidden, weight, targets, -100, 1.0, False)
         assert out.shape == (2, 3) and out.dtype is torch.float32
-        loss, saved = head_ops.head_ce(hidden, weight, targets, -100, 1.0, 0.0, 0.0, 1.0, 0)
+        loss, saved = head_ops.head_ce(hidden, weight, targets, -100, 1.0, 0.0, 0.0, 1.0, 0, False)
         assert loss.shape == () and saved.shape == (16 + 4 * 6,)
-        both = head_ops.head_backward(hidden, weight, targets, saved, loss, -100, 1.0, False, 0.0, 0.0, 1.0, 0, True, True)
+        both = head_ops.head_backward(hidden, weight, targets, saved, None, loss, -100, 1.0, False, 0.0, 0.0, 1.0, 0, True, True)
         assert [g.shape for g in both] == [hidden.shape, weight.shape] and both[1].dtype is torch.bfloat16
-        one, = head_ops.head_backward(hidden, weight, targets, saved, loss, -100, 1.0, False, 0.0, 0.0, 1.0, 0, False, True)
+        one, = head_ops.head_backward(hidden, weight, targets, saved, None, loss, -100, 1.0, False, 0.0, 0.0, 1.0, 0, False, True)
         assert one.shape == weight.shape
+
+
+def test_what_a_forward_leaves_for_the_gradient_of_hidden_alone():
+    """Nothing for small calls; fp32 values of every row, in whole fours, for those worth it."""
+    assert head_ops.unit_elements(64, 300, 64, _lib.ME_BF16) == 0
+    assert head_ops.unit_elements(0, 262_144, 5_376, _lib.ME_BF16) == 0
+    assert head_ops.unit_elements(3, 262_144, 5_375, _lib.ME_BF16) == 3 * 5_376
+    with FakeTensorMode():
+        hidden, weight, targets = _args(rows=(4096,), vocab=32_000, dim=1_024)
+        _, saved, unit = head_ops.head_ce(hidden, weight, targets, -100, 1.0, 0.0, 0.0, 1.0, 0, True)
+        assert unit.shape == (4096 * 1024,) and unit.dtype is torch.float32
