@@ -477,6 +477,183 @@ struct WeightEpilogue {
     }
 };
 
+// A maximum and the sum of 2^(x - maximum)
+struct Sum2 {
+    float m, s;
+};
+
+__device__ __forceinline__ Sum2 join(Sum2 a, Sum2 b) {
+    const float m = fmaxf(a.m, b.m);
+    const float shift = m == -__builtin_inff() ? 0.f : m;
+    return {m, a.s * __builtin_amdgcn_exp2f(a.m - shift) + b.s * __builtin_amdgcn_exp2f(b.m - shift)};
+}
+
+// ---- a few rows: one read of the head by plain products ----------------------------------------------------------
+// Up to kVectorRows rows of a forward alone: a workgroup holds them in LDS in fp32, its waves take head rows
+// two at a time, each lane 16 bytes of a row at a stride of a KiB, and the 64 partial sums are added across the wave.
+// Nothing is laid out first (fp32 parts would be read and written three times over) and the rows are found by every
+// workgroup for itself: two launches for a sampled token's log-probability. Lane l keeps the logits of
+// the wave's l-th head row of each 64, and statistics are taken of 64 at a time.
+constexpr int kVectorRows = 8;
+constexpr int kVectorLds = 64 * 1024;
+constexpr int kVectorGroups = 2048;
+
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+
+struct VectorArgs {
+    Layout h;
+    const float *weight;
+    int64_t w_stride, vocab;
+    const void *targets;
+    int t64;
+    int64_t ignore;
+    Saved s;
+    float2 *part;   // [rows][workgroups]
+    float *sum;     // likewise, or null
+    float *at_target;
+    float k;
+};
+
+struct Chunk {  // 16 bytes of a row
+    float v[4];
+    __device__ __forceinline__ void load(const float *row, int64_t c, int64_t dim) {
+        const auto at = as_global(row + c);
+        if (c + 4 <= dim) {
+            const f32x4_any x = *(gmem_ptr<const f32x4_any>)(at);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = x[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = c + j < dim ? at[j] : 0.f;
+        }
+    }
+};
+
+template <int CTRL>
+__device__ __forceinline__ float dpp_add(float x) {
+    return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, false));
+}
+
+__device__ __forceinline__ float wave_sum(float x) {
+    x = dpp_add<0xb1>(x);   // quad_perm [1, 0, 3, 2]
+    x = dpp_add<0x4e>(x);   // quad_perm [2, 3, 0, 1]
+    x = dpp_add<0x141>(x);  // row_half_mirror
+    x = dpp_add<0x140>(x);  // row_mirror
+    x += __shfl_xor(x, 16);
+    return x + __shfl_xor(x, 32);
+}
+
+template <int N>
+__global__ __launch_bounds__(256) void vector_kernel(const VectorArgs a) {
+    extern __shared__ __attribute__((aligned(16))) float s_h[];  // [N][pitch]
+    __shared__ int s_tgt[N], s_from[N], s_count;
+    __shared__ float2 s_part[4][N];
+    __shared__ float s_sum[4][N];
+    constexpr int kValues = 4, kStep = 64 * kValues;
+    constexpr int kUnroll = N >= 8 ? 1 : N >= 4 ? 2 : 4;  // loads in flight against registers
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int64_t pitch = ceil_div(a.h.dim, int64_t{kStep}) * kStep;
+    if (tid < 64) {
+        const int n = static_cast<int>(a.h.n);
+        int64_t t = -1;
+        if (lane < n) t = a.t64 ? static_cast<const int64_t *>(a.targets)[lane] : static_cast<const int32_t *>(a.targets)[lane];
+        const bool ok = lane < n && t != a.ignore && t >= 0 && t < a.vocab;
+        const uint64_t mask = __ballot(ok);
+        const int r = __popcll(mask & ((uint64_t{1} << lane) - 1));
+        if (ok) s_tgt[r] = static_cast<int>(t), s_from[r] = lane;
+        if (lane == 0) s_count = __popcll(mask);
+        if (blockIdx.x == 0) {  // for the launches that follow
+            if (lane < n) a.s.place[lane] = ok ? r : -1;
+            if (ok) a.s.rows[r] = lane;
+            if (lane == 0) *a.s.count = __popcll(mask);
+        }
+    }
+    __syncthreads();
+    const int count = s_count;
+    if (count == 0) return;
+    for (int64_t u = tid; u < N * pitch; u += 256) {
+        const int r = static_cast<int>(u / pitch);
+        const int64_t c = u - r * pitch;
+        float x = 0.f;
+        if (r < count && c < a.h.dim) {
+            const int64_t from = s_from[r], at = from / a.h.per_batch * a.h.batch_stride + from % a.h.per_batch * a.h.row_stride + c;
+            x = static_cast<const float *>(a.h.src)[at];
+        }
+        s_h[u] = x;
+    }
+    __syncthreads();
+
+    float m[N], s[N], sum[N], z[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) m[i] = -__builtin_inff(), s[i] = 0.f, sum[i] = 0.f, z[i] = -__builtin_inff();
+    auto take = [&]() {  // the statistics of this lane's logits so far
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float top = fmaxf(m[i], z[i]);
+            const float shift = top == -__builtin_inff() ? 0.f : top;
+            s[i] = s[i] * __builtin_amdgcn_exp2f(m[i] - shift) + __builtin_amdgcn_exp2f(z[i] - shift);
+            m[i] = top;
+            z[i] = -__builtin_inff();
+        }
+    };
+    const int64_t waves = static_cast<int64_t>(gridDim.x) * 4;
+    int slot = 0;
+    for (int64_t j = (static_cast<int64_t>(blockIdx.x) * 4 + wave) * 2; j < a.vocab; j += waves * 2) {
+        const int64_t j1 = min(j + 1, a.vocab - 1);
+        const float *w0 = a.weight + j * a.w_stride, *w1 = a.weight + j1 * a.w_stride;
+        float acc[2][N] = {};
+#pragma unroll kUnroll
+        for (int64_t c = lane * kValues; c < a.h.dim; c += kStep) {
+            Chunk x0, x1;
+            x0.load(w0, c, a.h.dim);
+            x1.load(w1, c, a.h.dim);
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+#pragma unroll
+                for (int e = 0; e < kValues; ++e) {
+                    const float h = s_h[i * pitch + c + e];
+                    acc[0][i] = fmaf(x0.v[e], h, acc[0][i]);
+                    acc[1][i] = fmaf(x1.v[e], h, acc[1][i]);
+                }
+        }
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const int64_t col = j + b;
+            if (col < a.vocab) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const float v = wave_sum(acc[b][i]) * a.k;
+                    if (lane == slot) {
+                        sum[i] += v;
+                        if (i < count && col == s_tgt[i])
+                            a.at_target[i] = v;
+                        else
+                            z[i] = v;
+                    }
+                }
+                if (++slot == 64) take(), slot = 0;
+            }
+        }
+    }
+    take();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        Sum2 all = {m[i], s[i]};
+#pragma unroll
+        for (int d = 32; d; d >>= 1) all = join(all, {__shfl_xor(all.m, d), __shfl_xor(all.s, d)});
+        const float total = wave_sum(sum[i]);
+        if (lane == 0) s_part[wave][i] = make_float2(all.m, all.s), s_sum[wave][i] = total;
+    }
+    __syncthreads();
+    if (tid < N && tid < count) {
+        Sum2 all = {s_part[0][tid].x, s_part[0][tid].y};
+        float total = s_sum[0][tid];
+        for (int w = 1; w < 4; ++w) all = join(all, {s_part[w][tid].x, s_part[w][tid].y}), total += s_sum[w][tid];
+        a.part[static_cast<int64_t>(tid) * gridDim.x + blockIdx.x] = make_float2(all.m, all.s);
+        if (a.sum) a.sum[static_cast<int64_t>(tid) * gridDim.x + blockIdx.x] = total;
+    }
+}
+
 // ---- rows' results ---------------------------------------------------------------------------------------------
 struct FinishArgs {
     const float2 *part;
@@ -490,17 +667,8 @@ struct FinishArgs {
     float *logps;        // by source row, or null
     float *row_loss;     // by counted row, or null
     float smoothing, z_loss;
+    int by_source;       // WIDE: a workgroup per source row, which writes the logps of those that do not count too
 };
-
-struct Sum2 {
-    float m, s;
-};
-
-__device__ __forceinline__ Sum2 join(Sum2 a, Sum2 b) {
-    const float m = fmaxf(a.m, b.m);
-    const float shift = m == -__builtin_inff() ? 0.f : m;
-    return {m, a.s * __builtin_amdgcn_exp2f(a.m - shift) + b.s * __builtin_amdgcn_exp2f(b.m - shift)};
-}
 
 // A row's parts joined: WIDE 256 threads per row (few rows), else 16 rows by 16 threads each
 template <bool WIDE>
@@ -509,9 +677,20 @@ __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs a) {
     __shared__ Sum2 s_all[WIDE ? 4 : 256];
     __shared__ double s_sum[WIDE ? 4 : 256];
     const int tid = threadIdx.x, slice = tid / kRows;
-    const int64_t r = static_cast<int64_t>(blockIdx.x) * kRows + tid % kRows;
+    int64_t r = static_cast<int64_t>(blockIdx.x) * kRows + tid % kRows;
     const int64_t count = a.count ? *a.count : *a.s.count;
-    if (static_cast<int64_t>(blockIdx.x) * kRows >= count) return;
+    if constexpr (WIDE) {
+        if (a.by_source) {
+            r = a.s.place[blockIdx.x];
+            if (r < 0) {
+                if (tid == 0 && a.logps) a.logps[blockIdx.x] = 0.f;
+                return;
+            }
+        }
+        if (r >= count) return;
+    } else {
+        if (static_cast<int64_t>(blockIdx.x) * kRows >= count) return;
+    }
     Sum2 all = {-__builtin_inff(), 0.f};
     double sum = 0.0;
     if (r < count) {
@@ -872,7 +1051,7 @@ Plan plan_of(int64_t n, int64_t vocab, int64_t dim, int dtype, const void *weigh
     p.grad = take(n * static_cast<int64_t>(sizeof(RowGrad)));
     if (p.copy_w) p.w = take(p.piece * p.ld * 2 * p.np);
     if (pass != kBackward) {
-        const int64_t parts = ceil_div(vocab, p.few ? 64 : 128) + 4;
+        const int64_t parts = std::max<int64_t>(ceil_div(vocab, p.few ? 64 : 128) + 4, n <= kVectorRows ? kVectorGroups : 0);
         p.part = take(parts * rows * 8);
         p.sum = take(parts * rows * 4);
         p.at_target = take(n * 4);
@@ -1109,9 +1288,54 @@ void forward_rows(const Plan &p, const Call &c, const Loss &l) {
     unit_of(p, c, l, again, redo + kHeader, nullptr);
 }
 
+void vector_rows(const VectorArgs &a, int rows, unsigned groups, size_t lds, hipStream_t s) {
+    if (rows == 1)
+        hipLaunchKernelGGL(vector_kernel<1>, dim3(groups), dim3(256), lds, s, a);
+    else if (rows == 2)
+        hipLaunchKernelGGL(vector_kernel<2>, dim3(groups), dim3(256), lds, s, a);
+    else if (rows == 4)
+        hipLaunchKernelGGL(vector_kernel<4>, dim3(groups), dim3(256), lds, s, a);
+    else
+        hipLaunchKernelGGL(vector_kernel<8>, dim3(groups), dim3(256), lds, s, a);
+}
+
+// Whether a forward goes the way of few rows by plain products, and the LDS it takes for its rows. fp32 alone: bf16 rows
+// read the head once on the matrix cores as well, at 5.9 TB/s (262,144 x 5376, 1 to 16 rows, 480 us; by plain
+// products 718 for one row, 810 for two).
+bool takes_vectors(const Plan &p, int &rows, size_t &lds) {
+    rows = p.n <= 1 ? 1 : p.n <= 2 ? 2 : p.n <= 4 ? 4 : 8;
+    lds = static_cast<size_t>(rows) * round_up(p.dim, 256) * 4;
+    return p.f32 && p.n >= 1 && p.n <= kVectorRows && lds <= kVectorLds;
+}
+
+void forward_vectors(const Plan &p, const Call &c, const Loss &l, int rows, size_t lds) {
+    const unsigned groups = static_cast<unsigned>(std::min<int64_t>(ceil_div(p.vocab, 8), kVectorGroups));
+    VectorArgs a{};
+    a.h = hidden_layout(p, c);
+    a.weight = static_cast<const float *>(c.weight), a.w_stride = c.w_stride, a.vocab = p.vocab, a.targets = c.targets, a.t64 = c.tdtype == ME_I64, a.ignore = c.ignore, a.s = c.s;
+    a.part = reinterpret_cast<float2 *>(c.ws + p.part);
+    a.sum = l.smoothing != 0.0 ? reinterpret_cast<float *>(c.ws + p.sum) : nullptr;
+    a.at_target = reinterpret_cast<float *>(c.ws + p.at_target);
+    a.k = static_cast<float>(1.44269504088896340736 / l.temperature);
+    vector_rows(a, rows, groups, lds, c.stream);
+    FinishArgs f{};
+    f.part = a.part, f.sum = a.sum, f.at_target = a.at_target, f.part_stride = 1, f.row_stride = groups, f.parts = static_cast<int>(groups);
+    f.n = p.n, f.vocab = p.vocab, f.s = c.s, f.logps = l.logps, f.by_source = 1;
+    f.row_loss = l.loss ? reinterpret_cast<float *>(c.ws + p.row_loss) : nullptr;
+    f.smoothing = static_cast<float>(l.smoothing), f.z_loss = static_cast<float>(l.z_loss);
+    hipLaunchKernelGGL(finish_kernel<true>, dim3(static_cast<unsigned>(p.n)), dim3(256), 0, c.stream, f);
+}
+
 int forward(const Plan &p, const Call &c, const Loss &l) {
     int32_t *tgt = reinterpret_cast<int32_t *>(c.ws + p.tgt);
     hipStream_t s = c.stream;
+    int rows;
+    size_t lds;
+    if (!l.unit && takes_vectors(p, rows, lds)) {
+        forward_vectors(p, c, l, rows, lds);
+        if (l.loss) hipLaunchKernelGGL(total_kernel, dim3(1), dim3(1024), 0, s, reinterpret_cast<const float *>(c.ws + p.row_loss), c.s.count, l.scale, l.mean, l.loss);
+        return check_launch("me_head");
+    }
     if (c.tdtype == ME_I64)
         hipLaunchKernelGGL(index_kernel<int64_t>, dim3(1), dim3(kIndexThreads), 0, s, static_cast<const int64_t *>(c.targets), p.n, c.ignore, p.vocab, c.s, tgt);
     else
