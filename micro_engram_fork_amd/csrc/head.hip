@@ -29,7 +29,8 @@ using namespace head;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr double kLn2 = 0.69314718055994530942;
 constexpr int64_t kFew = 128;                            // rows up to which the 64-row tiles are taken
-constexpr int64_t kPieceBytes = int64_t{512} << 20;      // of a piece's gradient, and of a piece of laid-out weights
+constexpr int64_t kPieceBytes = int64_t{1} << 30;        // of a piece's gradient, and of a piece of laid-out weights
+constexpr int kSplits = 3, kMostSplits = 16;             // of the product with W
 constexpr int kHeader = 16;                              // ints before the rows in `saved`: the number of them
 
 // What the forward leaves for the backward: counted rows, and by counted row its source, log2-sum and o; by source
@@ -654,6 +655,23 @@ __global__ __launch_bounds__(256) void vector_kernel(const VectorArgs a) {
     }
 }
 
+// Sums of the products with the head: [split][rows][ld], in as many splits as the product took for the rows
+struct Sums {
+    float *at;
+    int64_t ld, split_stride;
+    int tile_rows, col_tiles, most;
+    int cost;
+
+    __device__ __forceinline__ int splits(int64_t rows) const {
+        return most == 1 || rows == 0 ? 1 : splits_for(static_cast<int>(ceil_div(rows, tile_rows)) * col_tiles, most, cost);
+    }
+    __device__ __forceinline__ f32x4_v row4(int64_t row, int64_t c, int splits) const {
+        f32x4_v v = {0.f, 0.f, 0.f, 0.f};
+        for (int s = 0; s < splits; ++s) v += *as_global(reinterpret_cast<const f32x4_v *>(at + s * split_stride + row * ld + c));
+        return v;
+    }
+};
+
 // ---- rows' results ---------------------------------------------------------------------------------------------
 struct FinishArgs {
     const float2 *part;
@@ -820,16 +838,13 @@ __device__ __forceinline__ void store4(void *out, int64_t at, int64_t c, int64_t
 
 // Gradient of the hidden states, source rows in their order: the splits' sums, or zeros
 template <bool F32>
-__global__ __launch_bounds__(256) void hidden_kernel(const float *sums, int64_t ld, int64_t split_stride, int splits, const int32_t *place,
-                                                     int64_t n, int64_t dim, void *out) {
+__global__ __launch_bounds__(256) void hidden_kernel(const Sums sums, const int32_t *place, const int32_t *count, int64_t n, int64_t dim, void *out) {
     const int64_t units = ceil_div(dim, 4);
+    const int splits = sums.splits(*count);
     for (int64_t u = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; u < n * units; u += static_cast<int64_t>(gridDim.x) * 256) {
         const int64_t i = u / units, c = (u - i * units) * 4;
         const int64_t r = place[i];
-        f32x4_v v = {0.f, 0.f, 0.f, 0.f};
-        if (r >= 0)
-            for (int s = 0; s < splits; ++s) v += *as_global(reinterpret_cast<const f32x4_v *>(sums + s * split_stride + r * ld + c));
-        store4<F32>(out, i * dim, c, dim, v);
+        store4<F32>(out, i * dim, c, dim, r >= 0 ? sums.row4(r, c, splits) : f32x4_v{0.f, 0.f, 0.f, 0.f});
     }
 }
 
@@ -929,9 +944,7 @@ __global__ __launch_bounds__(256) void column_total_kernel(const float *part, in
 }
 
 struct UnitArgs {
-    const float *sums;
-    int64_t ld, split_stride;
-    int splits;
+    Sums sums;
     Saved s;
     const int32_t *count, *which;  // as FinishArgs
     const int32_t *tgt;            // by row of sums
@@ -948,6 +961,7 @@ template <bool F32>
 __global__ __launch_bounds__(256) void unit_kernel(const UnitArgs a) {
     const int64_t units = ceil_div(a.dim, 4);
     const int64_t count = a.count ? *a.count : *a.s.count;
+    const int splits = a.sums.splits(count);
     for (int64_t u = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; u < count * units; u += static_cast<int64_t>(gridDim.x) * 256) {
         const int64_t r = u / units, c = (u - r * units) * 4;
         const int64_t at = a.which ? a.which[r] : r;
@@ -956,8 +970,7 @@ __global__ __launch_bounds__(256) void unit_kernel(const UnitArgs a) {
         const float own = more - (1.f + more) * a.s.others[at] + a.smoothing;
         const float each = a.columns ? static_cast<float>(a.smoothing / a.vocab) : 0.f;
         const float scale = a.ref ? (1.f + more) * __builtin_amdgcn_exp2f(a.ref[r] - lse2) : 1.f;
-        f32x4_v v = {0.f, 0.f, 0.f, 0.f};
-        for (int s = 0; s < a.splits; ++s) v += *as_global(reinterpret_cast<const f32x4_v *>(a.sums + s * a.split_stride + r * a.ld + c));
+        f32x4_v v = a.sums.row4(r, c, splits);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             float w = 0.f, all = 0.f;
@@ -1007,25 +1020,14 @@ struct Plan {
     bool f32, few, copy_w;            // copy_w: the head is laid out piece by piece
     int np;                           // parts of an operand
     int64_t piece;                    // columns of the vocabulary at a time
-    int splits;                       // of the product with W
+    int splits;                       // of the product with W, at most
+    int split_cost;
     int64_t h, tgt, part, sum, at_target, row_loss, w, g, grad, acc;  // workspace offsets
     int64_t ref, redo, h2, tgt2, columns, column_part;
     int64_t bytes;
 };
 
 int64_t round_up(int64_t x, int64_t to) { return ceil_div(x, to) * to; }
-
-// Splits of the reduction over a piece so that the last round of tiles is as full as it gets; each costs a pass over
-// the sums.
-int splits_of(int64_t tiles, int64_t at_once, int64_t slabs) {
-    int best = 1;
-    double least = 1e30;
-    for (int s = 1; s <= 16 && s <= std::max<int64_t>(1, slabs / 8); ++s) {
-        const double cost = static_cast<double>(ceil_div(tiles * s, at_once)) / s + 0.01 * s;
-        if (cost < least - 1e-9) least = cost, best = s;
-    }
-    return best;
-}
 
 Plan plan_of(int64_t n, int64_t vocab, int64_t dim, int dtype, const void *weight, int64_t w_stride, Pass pass) {
     Plan p{};
@@ -1059,7 +1061,11 @@ Plan plan_of(int64_t n, int64_t vocab, int64_t dim, int dtype, const void *weigh
     }
     if (pass != kStats) {
         p.g = take(rows * p.piece * 2 * p.np);
-        p.splits = splits_of(ceil_div(n, p.few ? 64 : kTile) * ceil_div(dim, kTile), p.few ? 512 : 256, p.piece / kSlabK);
+        // at least eight slabs each; parts of few tiles are as many as fill the chip, those of many at most kSplits
+        const int64_t tiles = ceil_div(rows, p.few ? 64 : kTile) * ceil_div(dim, kTile);
+        p.splits = static_cast<int>(std::max<int64_t>(std::min<int64_t>({std::max<int64_t>(256 / tiles, kSplits), kMostSplits, p.piece / kSlabK / 8}), 1));
+        // reading and writing the sums at 4.8 TB/s against a piece's products at 1.25 PFLOP/s
+        p.split_cost = static_cast<int>(4096 * (8.0 / 4.8e12) / (2.0 * static_cast<double>(p.piece) * (p.f32 ? 6 : 1) / 1.25e15)) + 1;
         p.acc = take(p.splits * rows * p.ld * 4);
     }
     if (pass == kLeavesUnit) {
@@ -1138,7 +1144,7 @@ void multiply_few(const Gemm &g, const Epilogue &e, hipStream_t s) {
 // logits of a piece: rows x head rows
 template <int SEGS, class Epilogue>
 void logits_of(const Plan &p, const Call &c, const Rows &rows, const Operand &w, int64_t width, const Epilogue &e) {
-    const Gemm g{{rows.h, p.ld, h_part(p)}, w, p.n, width, p.dim, rows.count, 0, 8, 1};
+    const Gemm g{{rows.h, p.ld, h_part(p)}, w, p.n, width, p.dim, rows.count, 0, 8, 1, 0};
     if (p.few)
         multiply_few<true, SEGS>(g, e, c.stream);
     else
@@ -1147,12 +1153,16 @@ void logits_of(const Plan &p, const Call &c, const Rows &rows, const Operand &w,
 
 // product of a piece of the logits' gradient (or exponentials) with the head, onto the sums
 void times_head(const Plan &p, const Call &c, const Rows &rows, const Operand &w, int64_t v0, int64_t width) {
-    const Gemm g{{c.ws + p.g, p.piece, p.rows * p.piece * 2}, w, p.n, p.dim, width, rows.count, 0, 8, p.splits};
+    const Gemm g{{c.ws + p.g, p.piece, p.rows * p.piece * 2}, w, p.n, p.dim, width, rows.count, 0, 8, p.splits, p.split_cost};
     const AccumulateEpilogue e{reinterpret_cast<float *>(c.ws + p.acc), p.ld, p.rows * p.ld, v0 > 0};
     if (p.few)
         p.f32 ? multiply_few<false, 6>(g, e, c.stream) : multiply_few<false, 1>(g, e, c.stream);
     else
         p.f32 ? multiply_large<true, false, 6>(g, e, c.stream) : multiply_large<true, false, 1>(g, e, c.stream);
+}
+
+Sums sums_of(const Plan &p, const Call &c) {
+    return {reinterpret_cast<float *>(c.ws + p.acc), p.ld, p.rows * p.ld, p.few ? 64 : kTile, static_cast<int>(ceil_div(p.dim, kTile)), p.splits, p.split_cost};
 }
 
 void gradient_of(const Plan &p, const Call &c, const Rows &rows, const Operand &w, int64_t v0, int64_t width, const RowGrad *grad, float k) {
@@ -1182,8 +1192,7 @@ unsigned row_blocks(int64_t n) { return static_cast<unsigned>(std::max<int64_t>(
 // D from the sums of the products with the head
 void unit_of(const Plan &p, const Call &c, const Loss &l, const Rows &rows, const int32_t *which, const float *ref) {
     UnitArgs u{};
-    u.sums = reinterpret_cast<const float *>(c.ws + p.acc);
-    u.ld = p.ld, u.split_stride = p.rows * p.ld, u.splits = p.splits;
+    u.sums = sums_of(p, c);
     u.s = c.s, u.count = rows.count, u.which = which, u.tgt = rows.tgt, u.ref = ref;
     u.weight = c.weight, u.w_stride = c.w_stride, u.dim = p.dim, u.n = p.n;
     u.z_loss = static_cast<float>(l.z_loss), u.smoothing = static_cast<float>(l.smoothing);
@@ -1465,7 +1474,7 @@ extern "C" int me_head_backward(const void *hidden, int dtype, int64_t n, int64_
             if (grad_hidden) times_head(p, c, rows, w, v0, width);
         }
         if (grad_weight) {
-            const Gemm g{{c.ws + p.g, p.piece, p.rows * p.piece * 2}, {c.ws + p.h, p.ld, h_part(p)}, width, dim, n, c.s.count, 1, 8, 1};
+            const Gemm g{{c.ws + p.g, p.piece, p.rows * p.piece * 2}, {c.ws + p.h, p.ld, h_part(p)}, width, dim, n, c.s.count, 1, 8, 1, 0};
             uint8_t *out = static_cast<uint8_t *>(grad_weight) + v0 * dim * (f32 ? 4 : 2);
             if (f32)
                 multiply_large<false, false, 6>(g, WeightEpilogue<true>{out, dim}, s);
@@ -1474,12 +1483,11 @@ extern "C" int me_head_backward(const void *hidden, int dtype, int64_t n, int64_
         }
     }
     if (grad_hidden && n > 0) {
-        const float *acc = reinterpret_cast<const float *>(c.ws + p.acc);
         const unsigned blocks = blocks_for(n * ceil_div(dim, 4));
         if (f32)
-            hipLaunchKernelGGL(hidden_kernel<true>, dim3(blocks), dim3(256), 0, s, acc, p.ld, p.rows * p.ld, p.splits, c.s.place, n, dim, grad_hidden);
+            hipLaunchKernelGGL(hidden_kernel<true>, dim3(blocks), dim3(256), 0, s, sums_of(p, c), c.s.place, c.s.count, n, dim, grad_hidden);
         else
-            hipLaunchKernelGGL(hidden_kernel<false>, dim3(blocks), dim3(256), 0, s, acc, p.ld, p.rows * p.ld, p.splits, c.s.place, n, dim, grad_hidden);
+            hipLaunchKernelGGL(hidden_kernel<false>, dim3(blocks), dim3(256), 0, s, sums_of(p, c), c.s.place, c.s.count, n, dim, grad_hidden);
     }
     return check_launch("me_head_backward");
 }

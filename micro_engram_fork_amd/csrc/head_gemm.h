@@ -49,8 +49,25 @@ struct Gemm {
     const int32_t *count;  // null, or rows that there are: of R (reduce_rows 0) or of K (1)
     int count_is_k;
     int group;             // column tiles that follow one another before the next row tile
-    int splits;            // parts of the reduction, each with an output of its own
+    int most_splits;       // parts of the reduction, each with an output of its own: up to so many (splits_for)
+    int split_cost;        // of splits_for
 };
+
+// Parts of the reduction that tiles of C take so that the last round of workgroups is as full as it gets. Each
+// costs `cost` / 4096 of the product's own time (its sums are read and written once more). The rows may be
+// known to the device alone, so this is decided there, by whoever writes the parts and whoever adds them: in
+// integers, so that all of them come to the same.
+__device__ inline int splits_for(int tiles, int most, int cost) {
+    constexpr int64_t kCus = 256;
+    int best = 1;
+    int64_t least = int64_t{1} << 62;
+    for (int s = 1; s <= most; ++s) {
+        const int64_t all = static_cast<int64_t>(tiles) * s;
+        const int64_t time = (all + kCus - 1) / kCus * kCus * 4096 / all + static_cast<int64_t>(cost) * s;
+        if (time < least) least = time, best = s;
+    }
+    return best;
+}
 
 // segment -> parts of A and B: (0,0) (0,1) (1,0) (0,2) (1,1) (2,0)
 __device__ __forceinline__ int part_a(int seg) { return (0x910 >> (2 * seg)) & 3; }
@@ -151,7 +168,10 @@ __device__ __forceinline__ bool tile_of(const Gemm &a, int tr, int ts, Tile &t) 
             rows = min(rows, n);
     }
     const int n_rt = static_cast<int>(ceil_div(rows, tr)), n_st = static_cast<int>(ceil_div(a.S, ts));
-    const int per_split = n_rt * n_st, total = per_split * a.splits;
+    const int per_split = n_rt * n_st;
+    if (per_split == 0) return false;
+    const int splits = a.most_splits == 1 ? 1 : splits_for(per_split, a.most_splits, a.split_cost);
+    const int total = per_split * splits;
     const int per_xcd = (total + kXcds - 1) / kXcds;
     const int slot = static_cast<int>(blockIdx.x) / kXcds;
     int i = static_cast<int>(blockIdx.x) % kXcds * per_xcd + slot;
@@ -168,8 +188,8 @@ __device__ __forceinline__ bool tile_of(const Gemm &a, int tr, int ts, Tile &t) 
     t.s0 = static_cast<int64_t>(t.st) * ts;
     t.rows = rows;
     const int64_t slabs = ceil_div(k, int64_t{kSlabK});
-    t.k0 = slabs * t.split / a.splits * kSlabK;
-    t.k1 = min(k, slabs * (t.split + 1) / a.splits * kSlabK);
+    t.k0 = slabs * t.split / splits * kSlabK;
+    t.k1 = min(k, slabs * (t.split + 1) / splits * kSlabK);
     return true;
 }
 
@@ -188,7 +208,8 @@ struct Loader {
     uint32_t off[LOADS];
     bool even_out, odd_out;  // this lane's chunk of an even / odd load is past K in the last slab
 
-    __device__ __forceinline__ void init(const Operand &o, int64_t first, int64_t there, int64_t k, int wave, int lane) {
+    // rows / columns from `first` on up to `there`; k values from k0 on up to k
+    __device__ __forceinline__ void init(const Operand &o, int64_t first, int64_t there, int64_t k0, int64_t k, int wave, int lane) {
         pitch = o.ld * 2;
         part = o.part;
         K = k;
@@ -196,7 +217,7 @@ struct Loader {
             base = reinterpret_cast<uint64_t>(o.base) + static_cast<uint64_t>(first * pitch);
             const int64_t rows = min(there - first, static_cast<int64_t>(DIM));
             range = static_cast<uint32_t>(rows * pitch);
-            const int valid = static_cast<int>(k - (k - 1) / kSlabK * kSlabK);  // k values of the last slab
+            const int valid = k > k0 ? static_cast<int>(k - (k - 1) / kSlabK * kSlabK) : 0;  // k values of the last slab
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) {
                 const int row = (wave * LOADS + i) * 8 + (lane >> 3);
@@ -263,8 +284,8 @@ __global__ __launch_bounds__(kThreads, 1) void large_kernel(const Gemm a, const 
 
     Loader<A_KC, kTile, kDma> la;
     Loader<B_KC, kTile, kDma> lb;
-    la.init(a.a, t.r0, A_KC ? t.rows : a.R, t.k1, wave, lane);
-    lb.init(a.b, t.s0, a.S, t.k1, wave, lane);
+    la.init(a.a, t.r0, A_KC ? t.rows : a.R, t.k0, t.k1, wave, lane);
+    lb.init(a.b, t.s0, a.S, t.k0, t.k1, wave, lane);
     const uint32_t w0 = __builtin_amdgcn_readfirstlane(lds_addr(ring) + static_cast<uint32_t>(wave) * (kDma * 1024u));
     auto issue_a = [&](int sl, int i) {
         const int seg = SEGS == 1 ? 0 : sl / spq;
@@ -420,8 +441,8 @@ __global__ __launch_bounds__(kThreads) void few_kernel(const Gemm a, const Epilo
     const int slabs = spq * SEGS;
     Loader<true, kTR, kDmaA> la;
     Loader<B_KC, TS, kDmaB> lb;
-    la.init(a.a, t.r0, t.rows, t.k1, wave, lane);
-    lb.init(a.b, t.s0, a.S, t.k1, wave, lane);
+    la.init(a.a, t.r0, t.rows, t.k0, t.k1, wave, lane);
+    lb.init(a.b, t.s0, a.S, t.k0, t.k1, wave, lane);
     const uint32_t w0 = __builtin_amdgcn_readfirstlane(lds_addr(ring));
     auto issue = [&](int sl) {
         const int seg = SEGS == 1 ? 0 : sl / spq;
@@ -485,7 +506,7 @@ __global__ __launch_bounds__(kThreads) void few_kernel(const Gemm a, const Epilo
 
 // Workgroups that hold every tile at the largest count
 inline int64_t workgroups(const Gemm &a, int tr, int ts) {
-    return ceil_div(ceil_div(a.R, tr) * ceil_div(a.S, ts) * a.splits, kXcds) * kXcds;
+    return ceil_div(ceil_div(a.R, tr) * ceil_div(a.S, ts) * a.most_splits, kXcds) * kXcds;
 }
 
 }  // namespace head
