@@ -86,9 +86,10 @@ class _DirectOptimizer(torch.optim.Optimizer):
             buf = torch.zeros(len(params), dtype=torch.float32)
             entry = bufs[gi] = (buf, [buf[i] for i in range(len(params))], tuple(id(p) for p in params))
         buf, views, _ = entry
-        if len(live) == len(params) and all(a is b for a, b in zip(live, params)):
-            states = [self.state[p] for p in params]
-            for i, st in enumerate(states):
+        if len(live) == len(params) and (live is params or all(a is b for a, b in zip(live, params))):
+            state = self.state
+            for i, p in enumerate(params):
+                st = state[p]
                 if st["step"] is not views[i]:
                     step = st["step"]
                     if step.device.type != "cpu" or step.numel() != 1:
@@ -471,30 +472,49 @@ class DenseAdamW(_DirectOptimizer):
 
     _STATES = ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")
 
+    def _same(self, plan, group):
+        """(parameters with a gradient, their gradients) if `plan` still holds: the same parameters at the same places have
+        one, their states are the same tensors, and the gradients' types are the same and such as the kernel reads as
+        they are. None otherwise. (The usual step; each check here is made for each tensor, so they are the
+        cheapest that will do.)"""
+        params, members = group["params"], plan["members"]
+        if len(params) != plan["of"] or plan["settings"] != (group["state_bits"], bool(group["capturable"])):
+            return None
+        if plan["idle"]:
+            for i, q in plan["idle"]:
+                p = params[i]
+                if p is not q or p.grad is not None or p.__dict__.get("fp32_grad") is not None or p.__dict__.get("sparse_grad") is not None:
+                    return None
+            params = [params[i] for i in plan["at"]]
+        state, grads = self.state, []
+        for p, (q, ptr, n, kind, st, m, v, ms, vs) in zip(params, members):
+            own = p.__dict__
+            g = own.get("fp32_grad")
+            if g is None:
+                g = p.grad
+                if g is None or g.is_sparse:
+                    return None
+            elif g.shape != p.shape or g.device != p.device:
+                return None
+            if (p is not q or g.dtype is not kind or not g.is_contiguous() or state.get(p) is not st or st.get("exp_avg") is not m
+                    or st.get("exp_avg_sq") is not v or st.get("exp_avg_scale") is not ms or st.get("exp_avg_sq_scale") is not vs
+                    or p.data_ptr() != ptr or p.numel() != n or own.get("sparse_grad") is not None):
+                return None
+            grads.append(g)
+        return params, grads
+
     def _plan(self, gi, group, live):
         """As LazyAdamW's launch plan: the pointer arrays of group gi's launches that stay put between steps, per
-        (device, parameter dtype, gradient dtype), kept while parameters, their storage and their states are
-        the same tensors. live: [(parameter, gradient, gradient dtype)]."""
-        plans = self.__dict__.setdefault("_plans", {})
-        plan = plans.get(gi)
+        (device, parameter dtype, gradient dtype). live: [(parameter, gradient, gradient dtype)]."""
         eight = group["state_bits"] == 8
         names = self._STATES[:4 if eight else 2]
-        if plan is not None and len(plan["members"]) == len(live):
-            for (p, _, kind), (q, ptr, n, was, states) in zip(live, plan["members"]):
-                s = self.state[p]
-                if p is not q or p.data_ptr() != ptr or p.numel() != n or kind is not was or any(
-                        s.get(k) is not t for k, t in zip(names, states)):
-                    break
-            else:
-                if plan["eight"] == eight:
-                    return plan
         index = {id(p): i for i, p in enumerate(p for g in self.param_groups for p in g["params"])}
         members, batches = [], {}
         for i, (p, g, kind) in enumerate(live):
             state = self.state[p]
             states = tuple(state.get(k) for k in names)
             self._check_state(p, states, eight)
-            members.append((p, p.data_ptr(), p.numel(), kind, states))
+            members.append((p, p.data_ptr(), p.numel(), kind, state, *(state.get(k) for k in self._STATES)))
             b = batches.setdefault((p.device, p.dtype, kind), {"pos": [], "ptr": [[] for _ in range(5)], "n": [], "ids": [],
                                                                "written": []})
             b["pos"].append(i)
@@ -508,7 +528,12 @@ class DenseAdamW(_DirectOptimizer):
                      grad_dtype=ops.dtype_code(torch.empty(0, dtype=kind)),
                      arrays=[ops.ptr_array(x) if x else None for x in b["ptr"]], n=ops.i64_array(b["n"]),
                      ids=ops.i32_array(b["ids"]))
-        plan = plans[gi] = {"members": members, "batches": list(batches.values()), "eight": eight}
+        params, ids = group["params"], {id(p) for p, _, _ in live}
+        plan = {"members": members, "batches": list(batches.values()), "of": len(params),
+                "settings": (group["state_bits"], bool(group["capturable"])),
+                "at": [i for i, p in enumerate(params) if id(p) in ids],
+                "idle": [(i, p) for i, p in enumerate(params) if id(p) not in ids]}
+        self.__dict__.setdefault("_plans", {})[gi] = plan
         return plan
 
     def _check_state(self, p, states, eight):
@@ -553,46 +578,58 @@ class DenseAdamW(_DirectOptimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        plans = self.__dict__.setdefault("_plans", {})
         for gi, group in enumerate(self.param_groups):
-            live = []
-            for p in group["params"]:
-                if getattr(p, "sparse_grad", None) is not None:
-                    raise ValueError("[micro_engram] DenseAdamW: sparse row gradients need LazyAdamW")
-                if p.grad is not None or getattr(p, "fp32_grad", None) is not None:
-                    live.append((p, *self._gradient(p)))
-            if not live:
-                continue
-            if not all(p.is_cuda for p, _, _ in live):
-                ops.require_gpu(*(p for p, _, _ in live))
+            plan = plans.get(gi)
+            same = self._same(plan, group) if plan is not None else None
+            if same is not None:
+                params, grads = same
+            else:
+                live = self._live(group)
+                if not live:
+                    continue
+                params, grads = [p for p, _, _ in live], [g for _, g, _ in live]
             capturable = bool(group["capturable"])
-            if torch.cuda.is_current_stream_capturing() and (
-                    not capturable or not all(self.state[p] for p, _, _ in live)):
+            if torch.cuda.is_current_stream_capturing() and (not capturable or not all(self.state.get(p) for p in params)):
                 raise RuntimeError("[micro_engram] DenseAdamW: a step under graph capture needs capturable=True and "
                                    "states that exist already")
-            for p, _, _ in live:
-                if not self.state[p]:
-                    self.init_state(self.state[p], p, group)
-            plan = self._plan(gi, group, live)
+            if same is None:
+                for p in params:
+                    if not self.state[p]:
+                        self.init_state(self.state[p], p, group)
+                plan = self._plan(gi, group, live)
             if capturable:
                 counts = None
-                for p, _, _ in live:
+                for p in params:
                     step = self.state[p]["step"]
                     if step.device != p.device or step.dtype is not torch.float32 or step.numel() != 1:
                         raise ValueError("[micro_engram] DenseAdamW: capturable step counts are fp32 scalars on the GPU")
             else:
-                counts = self._advance_steps(gi, group, [p for p, _, _ in live])
+                counts = self._advance_steps(gi, group, params)
             for b in plan["batches"]:
-                pos, arrays = b["pos"], b["arrays"]
-                grads = ops.ptr_array([live[i][1].data_ptr() for i in pos])
+                pos = b["pos"]
+                pointers = ops.ptr_array([grads[i].data_ptr() for i in pos])
                 steps = device_steps = None
                 if counts is not None:
-                    steps = ops.f64_array([counts[i] for i in pos])
+                    steps = ops.f64_array(counts if len(pos) == len(counts) else [counts[i] for i in pos])
                 else:
-                    device_steps = ops.ptr_array([self.state[live[i][0]]["step"].data_ptr() for i in pos])
-                ops.adamw_launch(b["device"], len(pos), arrays, grads, b["n"], steps, device_steps, b["ids"], b["dtype"],
+                    device_steps = ops.ptr_array([self.state[params[i]]["step"].data_ptr() for i in pos])
+                ops.adamw_launch(b["device"], len(pos), b["arrays"], pointers, b["n"], steps, device_steps, b["ids"], b["dtype"],
                                  b["grad_dtype"], group["state_bits"], lr=group["lr"], betas=group["betas"],
                                  eps=group["eps"], weight_decay=group["weight_decay"],
                                  stochastic_rounding=group["stochastic_rounding"], seed=self.seed)
                 # written through raw pointers: as LazyAdamW
                 torch.autograd.graph.increment_version(b["written"])
         return loss
+
+    def _live(self, group):
+        """[(parameter, gradient, gradient dtype)] of the parameters that have one."""
+        live = []
+        for p in group["params"]:
+            if getattr(p, "sparse_grad", None) is not None:
+                raise ValueError("[micro_engram] DenseAdamW: sparse row gradients need LazyAdamW")
+            if p.grad is not None or getattr(p, "fp32_grad", None) is not None:
+                live.append((p, *self._gradient(p)))
+        if not all(p.is_cuda for p, _, _ in live):
+            ops.require_gpu(*(p for p, _, _ in live))
+        return live

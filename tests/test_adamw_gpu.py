@@ -329,3 +329,61 @@ def test_groups_and_fp32_grad():
     was = a.detach().clone()
     opt.step()
     assert torch.equal(a, was)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_what_changes_between_steps_is_noticed(bits):
+    """Each of these ends the reuse of what the step before prepared: every step is as one from scratch."""
+    params = _tensors([300, 129, 50], torch.bfloat16, torch.bfloat16)
+    opt = DenseAdamW(params, state_bits=bits, seed=SEED, **HYPER)
+    counts = [0, 0, 0]
+
+    def step():
+        live = [k for k, p in enumerate(params) if p.grad is not None or getattr(p, "fp32_grad", None) is not None]
+        before = {k: _before(opt, [params[k]], bits)[0] for k in live}
+        held = [p.detach().clone() for p in params]
+        opt.step()
+        for k, p in enumerate(params):
+            if k not in live:
+                assert torch.equal(p, held[k])
+                continue
+            counts[k] += 1
+            assert float(opt.state[p]["step"]) == counts[k]
+            _check_one(opt, p, before[k], counts[k], bits, k)
+    step(), step()
+    params[1].grad = None                                              # one rests
+    step(), step()
+    params[1].grad = torch.randn_like(params[1])                       # and comes back, another rests
+    params[0].grad = None
+    step()
+    params[0].fp32_grad = torch.randn(params[0].shape, device=DEV)     # a wide gradient
+    step(), step()
+    params[0].fp32_grad = params[0].fp32_grad[::1].clone()             # another tensor
+    step()
+    params[2].data = torch.randn(50, device=DEV).bfloat16()            # another place
+    step()
+    s = opt.state[params[2]]
+    s["exp_avg"] = s["exp_avg"].clone()                                # other states
+    step()
+    opt.state[params[2]] = dict(s)
+    step()
+    s["step"].fill_(99.0)                                              # no longer the parameter's own
+    opt.state[params[1]]["step"] = torch.tensor(7.0)                   # another count
+    counts[1] = 7
+    opt.state[params[2]]["step"] = torch.tensor(float(counts[2]))
+    step()
+    params[1].grad = torch.randn(129 * 2, device=DEV).bfloat16()[::2]  # strides
+    step()
+    opt.param_groups[0]["lr"] = HYPER["lr"]
+    opt.add_param_group({"params": [torch.nn.Parameter(torch.zeros(3, device=DEV))]})
+    step()
+
+
+def _check_one(opt, p, before, t, bits, stream):
+    """_check_step of one parameter with the noise of its place."""
+    noise = ref.noise
+    try:
+        ref.noise = lambda n, seed, step, _: noise(n, seed, step, stream)
+        _check_step(opt, [p], [before], t, bits)
+    finally:
+        ref.noise = noise
