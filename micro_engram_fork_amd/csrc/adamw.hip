@@ -34,8 +34,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kPer = 8;                      // values per thread and round
-constexpr int kRounds = 2;                   // rounds per workgroup
-constexpr int kChunk = kThreads * kPer * kRounds;
+constexpr int kChunk = kThreads * kPer;       // values per workgroup: two or four rounds each took 3-8 % longer
 constexpr int kTensors = 42;                 // tensors per launch (kernel arguments stay under 4 KiB)
 constexpr int kBlock = 128;                  // values per scale of 8-bit moments
 constexpr int64_t kMostChunks = int64_t{1} << 23;
@@ -243,86 +242,77 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(const Args a) {
         step_size = static_cast<float>(a.lr / -expm1(s * a.log_beta1));
         inv_sqrt_bc2 = static_cast<float>(1.0 / sqrt(-expm1(s * a.log_beta2)));
     }
-    float p[kRounds][kPer], g[kRounds][kPer], m[kRounds][kPer], v[kRounds][kPer];
-    u32x2_v mc[kRounds], vc[kRounds];
-    uint32_t ms[kRounds], vs[kRounds];
-    int64_t at[kRounds];
-    int left[kRounds];
+    float p[kPer], g[kPer], m[kPer], v[kPer];
+    u32x2_v mc, vc;
+    uint32_t ms, vs;
+    const int64_t at = base + static_cast<int64_t>(threadIdx.x) * kPer;
+    const int left = static_cast<int>(min(max(n - at, int64_t{0}), int64_t{kPer}));
+    load8<P16>(t.p, at, left, p);
+    load8<G16>(t.g, at, left, g);
+    if constexpr (EIGHT) {
+        mc = load8_codes(t.m, at, left);
+        vc = load8_codes(t.v, at, left);
+        ms = left > 0 ? as_global(t.m_scale)[at / kBlock] : 0;
+        vs = left > 0 ? as_global(t.v_scale)[at / kBlock] : 0;
+    } else {
+        load8<false>(t.m, at, left, m);
+        load8<false>(t.v, at, left, v);
+    }
+    uint32_t noise[kPer];
+    const bool draws = EIGHT || (P16 && a.sr);
+    if (draws) {
+        const uint64_t group = static_cast<uint64_t>(at) / kPer;
+        const uint4 w = philox4x32_10(make_uint4(static_cast<uint32_t>(group), static_cast<uint32_t>(group >> 32), step, t.stream),
+                                      make_uint2(static_cast<uint32_t>(a.seed), static_cast<uint32_t>(a.seed >> 32)));
+        const uint32_t words[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int r = 0; r < kRounds; ++r) {
-        at[r] = base + (r * kThreads + static_cast<int>(threadIdx.x)) * kPer;
-        left[r] = static_cast<int>(min(max(n - at[r], int64_t{0}), int64_t{kPer}));
-        load8<P16>(t.p, at[r], left[r], p[r]);
-        load8<G16>(t.g, at[r], left[r], g[r]);
-        if constexpr (EIGHT) {
-            mc[r] = load8_codes(t.m, at[r], left[r]);
-            vc[r] = load8_codes(t.v, at[r], left[r]);
-            ms[r] = left[r] > 0 ? as_global(t.m_scale)[at[r] / kBlock] : 0;
-            vs[r] = left[r] > 0 ? as_global(t.v_scale)[at[r] / kBlock] : 0;
-        } else {
-            load8<false>(t.m, at[r], left[r], m[r]);
-            load8<false>(t.v, at[r], left[r], v[r]);
-        }
+        for (int j = 0; j < kPer; ++j) noise[j] = (words[j >> 1] >> (16 * (j & 1))) & 0xffffu;
+    }
+    if constexpr (EIGHT) {
+        decode8<false>(mc, scale_of(ms), m);
+        decode8<true>(vc, scale_of(vs), v);
     }
 #pragma unroll
-    for (int r = 0; r < kRounds; ++r) {
-        uint32_t noise[kPer];
-        const bool draws = EIGHT || (P16 && a.sr);
-        if (draws) {
-            const uint64_t group = static_cast<uint64_t>(at[r]) / kPer;
-            const uint4 w = philox4x32_10(make_uint4(static_cast<uint32_t>(group), static_cast<uint32_t>(group >> 32), step, t.stream),
-                                          make_uint2(static_cast<uint32_t>(a.seed), static_cast<uint32_t>(a.seed >> 32)));
-            const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+    for (int j = 0; j < kPer; ++j) {
+        m[j] = a.beta1 * m[j] + a.rest1 * g[j];
+        v[j] = a.beta2 * v[j] + a.rest2 * (g[j] * g[j]);
+        // 1 ulp each: far below the rounding of p, of which the quotient is at most a few lr
+        const float denom = __builtin_amdgcn_sqrtf(v[j]) * inv_sqrt_bc2 + a.eps;
+        p[j] = a.decay * p[j] - step_size * (m[j] * __builtin_amdgcn_rcpf(denom));
+    }
+    if constexpr (P16) {
+        uint32_t w[4];
 #pragma unroll
-            for (int j = 0; j < kPer; ++j) noise[j] = (words[j >> 1] >> (16 * (j & 1))) & 0xffffu;
+        for (int j = 0; j < 4; ++j) {
+            uint32_t half[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                half[h] = a.sr ? stochastic_bf16_bits(p[2 * j + h], noise[2 * j + h])
+                               : float_to_bf16_bits_rne(p[2 * j + h]);
+            w[j] = half[0] | (half[1] << 16);
         }
-        if constexpr (EIGHT) {
-            decode8<false>(mc[r], scale_of(ms[r]), m[r]);
-            decode8<true>(vc[r], scale_of(vs[r]), v[r]);
-        }
+        store8_bf16(t.p, at, left, w);
+    } else {
+        store8_f32(t.p, at, left, p);
+    }
+    if constexpr (EIGHT) {
+        uint32_t turned[kPer], opposite[kPer];
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
-            m[r][j] = a.beta1 * m[r][j] + a.rest1 * g[r][j];
-            v[r][j] = a.beta2 * v[r][j] + a.rest2 * (g[r][j] * g[r][j]);
-            // 1 ulp each: far below the rounding of p, of which the quotient is at most a few lr
-            const float denom = __builtin_amdgcn_sqrtf(v[r][j]) * inv_sqrt_bc2 + a.eps;
-            p[r][j] = a.decay * p[r][j] - step_size * (m[r][j] * __builtin_amdgcn_rcpf(denom));
+            turned[j] = ((noise[j] << 8) | (noise[j] >> 8)) & 0xffffu;
+            opposite[j] = 0xffffu - noise[j];
         }
-        if constexpr (P16) {
-            uint32_t w[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                uint32_t half[2];
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    half[h] = a.sr ? stochastic_bf16_bits(p[r][2 * j + h], noise[2 * j + h])
-                                   : float_to_bf16_bits_rne(p[r][2 * j + h]);
-                w[j] = half[0] | (half[1] << 16);
-            }
-            store8_bf16(t.p, at[r], left[r], w);
-        } else {
-            store8_f32(t.p, at[r], left[r], p[r]);
-        }
-        if constexpr (EIGHT) {
-            uint32_t turned[kPer], opposite[kPer];
-#pragma unroll
-            for (int j = 0; j < kPer; ++j) {
-                turned[j] = ((noise[j] << 8) | (noise[j] >> 8)) & 0xffffu;
-                opposite[j] = 0xffffu - noise[j];
-            }
-            uint32_t scale;
-            const bool leads = left[r] > 0 && (threadIdx.x & 15) == 0;
-            store8_codes(t.m, at[r], left[r], encode8<false>(m[r], turned, scale));
-            if (leads) as_global(t.m_scale)[at[r] / kBlock] = static_cast<uint8_t>(scale);
-            store8_codes(t.v, at[r], left[r], encode8<true>(v[r], opposite, scale));
-            if (leads) as_global(t.v_scale)[at[r] / kBlock] = static_cast<uint8_t>(scale);
-        } else {
-            store8_f32(t.m, at[r], left[r], m[r]);
-            store8_f32(t.v, at[r], left[r], v[r]);
-        }
+        uint32_t scale;
+        const bool leads = left > 0 && (threadIdx.x & 15) == 0;
+        store8_codes(t.m, at, left, encode8<false>(m, turned, scale));
+        if (leads) as_global(t.m_scale)[at / kBlock] = static_cast<uint8_t>(scale);
+        store8_codes(t.v, at, left, encode8<true>(v, opposite, scale));
+        if (leads) as_global(t.v_scale)[at / kBlock] = static_cast<uint8_t>(scale);
+    } else {
+        store8_f32(t.m, at, left, m);
+        store8_f32(t.v, at, left, v);
     }
 }
-
 // step counts kept on the device, one more each
 struct CountArgs {
     float *at[256];
@@ -361,7 +351,7 @@ extern "C" int me_adamw(int32_t n_tensors, void *const *params, const void *cons
     ME_CHECK_ARG(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1, "betas must be in [0, 1)");
     for (int k = 0; k < n_tensors; ++k) {
         ME_CHECK_ARG(numels[k] >= 0, "tensor %d: negative size", k);
-        ME_CHECK_ARG(ceil_div(numels[k], kChunk) <= kMostChunks, "tensor %d: more than 2^35 values", k);
+        ME_CHECK_ARG(ceil_div(numels[k], kChunk) <= kMostChunks, "tensor %d: more than 2^34 values", k);
         ME_CHECK_ARG(device_steps ? device_steps[k] != nullptr : steps[k] >= 1, "tensor %d: step must be >= 1", k);
         if (numels[k] == 0) continue;
         ME_CHECK_ARG(params[k] && grads[k] && exp_avgs[k] && exp_avg_sqs[k], "tensor %d: null tensor pointer", k);

@@ -87,13 +87,30 @@ __global__ __launch_bounds__(256) void targets_kernel(const T *targets, int64_t 
 }
 
 // ---- operands as the products read them: [rows][ld] bf16, ld a multiple of 64, zeros past dim; fp32 in three parts -----
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));        // pieces of rows that may start
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));     // at any element
+
 struct Layout {
     const void *src;
     int64_t per_batch, batch_stride, row_stride;  // row r: (r / per_batch) * batch_stride + (r % per_batch) * row_stride
     const int32_t *rows, *count;                  // sources of the rows and how many there are; null: as they are
     int64_t n, dim, ld, part;                     // part: bytes
     uint8_t *dst;
+    const int32_t *gate;                          // a count; 0: nothing is laid out. Null: none
 };
+
+// Eight values of a row of fp32 from c on, zeros from dim on
+__device__ __forceinline__ void load8(const float *row, int64_t c, int64_t dim, float (&x)[8]) {
+    const auto at = as_global(row + c);
+    if (c + 8 <= dim) {
+        const f32x4_any a = *(gmem_ptr<const f32x4_any>)(at), b = *(gmem_ptr<const f32x4_any>)(at + 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = a[j], x[4 + j] = b[j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = c + j < dim ? at[j] : 0.f;
+    }
+}
 
 // x as three bf16 that add up to it: each the nearest bf16 of what remains. What is not finite stands in the
 // first part alone.
@@ -107,6 +124,7 @@ __device__ __forceinline__ void split3(float x, uint16_t (&p)[3]) {
 
 template <bool F32>
 __global__ __launch_bounds__(256) void layout_kernel(const Layout a) {
+    if (a.gate != nullptr && *a.gate == 0) return;
     const int64_t units = a.ld / 8;
     const int64_t n = a.count ? min(a.n, static_cast<int64_t>(*a.count)) : a.n;
     for (int64_t u = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; u < n * units; u += static_cast<int64_t>(gridDim.x) * 256) {
@@ -116,17 +134,18 @@ __global__ __launch_bounds__(256) void layout_kernel(const Layout a) {
         uint32_t w[3][4] = {};
         uint16_t(&h)[3][8] = reinterpret_cast<uint16_t(&)[3][8]>(w);
         if constexpr (F32) {
-            const float *src = static_cast<const float *>(a.src) + at;
+            float x[8];
+            load8(static_cast<const float *>(a.src) + (at - c), c, a.dim, x);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 uint16_t p[3];
-                split3(c + j < a.dim ? src[j] : 0.f, p);
+                split3(x[j], p);
                 h[0][j] = p[0], h[1][j] = p[1], h[2][j] = p[2];
             }
         } else {
             const uint16_t *src = static_cast<const uint16_t *>(a.src) + at;
-            if (c + 8 <= a.dim && reinterpret_cast<uintptr_t>(src) % 16 == 0) {
-                const u32x4_v x = *as_global(reinterpret_cast<const u32x4_v *>(src));
+            if (c + 8 <= a.dim) {
+                const u32x4_any x = *(gmem_ptr<const u32x4_any>)(as_global(src));
 #pragma unroll
                 for (int j = 0; j < 4; ++j) w[0][j] = x[j];
             } else {
@@ -139,6 +158,80 @@ __global__ __launch_bounds__(256) void layout_kernel(const Layout a) {
             *as_global(reinterpret_cast<u32x4_v *>(a.dst + p * a.part + (r * a.ld + c) * 2)) = u32x4_v{w[p][0], w[p][1], w[p][2], w[p][3]};
     }
 }
+
+// fp32 rows in two fp16 parts over a power of two by row, which goes to `scale` (what the parts are multiplied by to
+// give the value). A wave per row. Of what is not finite, the first part alone.
+__global__ __launch_bounds__(256) void layout16_kernel(const Layout a, float *scale) {
+    if (a.gate != nullptr && *a.gate == 0) return;
+    const int lane = threadIdx.x & 63;
+    const int64_t n = a.count ? min(a.n, static_cast<int64_t>(*a.count)) : a.n;
+    constexpr int kKept = 4;  // pieces of 512 values that stay in registers; further ones are read again
+    for (int64_t r = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6); r < n; r += static_cast<int64_t>(gridDim.x) * 4) {
+        const int64_t from = a.rows ? a.rows[r] : r;
+        const float *src = static_cast<const float *>(a.src) + (from / a.per_batch * a.batch_stride + from % a.per_batch * a.row_stride);
+        float kept[kKept][8];
+        uint32_t most = 0;
+        auto look = [&](const float (&x)[8]) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t b = __float_as_uint(x[j]) & 0x7fffffffu;
+                most = max(most, b < 0x7f800000u ? b : 0u);
+            }
+        };
+#pragma unroll
+        for (int i = 0; i < kKept; ++i)
+            if (i * 512 < a.dim) {
+                load8(src, i * 512 + lane * 8, a.dim, kept[i]);
+                look(kept[i]);
+            }
+        for (int64_t c = kKept * 512 + lane * 8; c < a.dim; c += 512) {
+            float x[8];
+            load8(src, c, a.dim, x);
+            look(x);
+        }
+#pragma unroll
+        for (int d = 32; d; d >>= 1) most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), d)));
+        // the largest below 2^15; the power and its inverse are normal fp32 numbers
+        const int up = min(max(14 - (static_cast<int>(most >> 23) - 127), -112), 126);
+        const float times = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
+        if (lane == 0) scale[r] = __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
+        auto put = [&](const float (&v)[8], int64_t c) {
+            if (c >= a.ld) return;
+            halfx8 hi, lo;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float x = v[j] * times;
+                hi[j] = static_cast<_Float16>(x);
+                const float rest = x - static_cast<float>(hi[j]);
+                lo[j] = static_cast<_Float16>(__builtin_fabsf(rest) < __builtin_inff() ? rest : 0.f);
+            }
+            *as_global(reinterpret_cast<halfx8 *>(a.dst + (r * a.ld + c) * 2)) = hi;
+            *as_global(reinterpret_cast<halfx8 *>(a.dst + a.part + (r * a.ld + c) * 2)) = lo;
+        };
+#pragma unroll
+        for (int i = 0; i < kKept; ++i)
+            if (i * 512 < a.dim) put(kept[i], i * 512 + lane * 8);
+        for (int64_t c = kKept * 512 + lane * 8; c < a.ld; c += 512) {
+            float x[8];
+            load8(src, c, a.dim, x);
+            put(x, c);
+        }
+    }
+}
+
+// What rows and columns of a product of fp16 parts are multiplied by; null: nothing
+struct Scales {
+    const float *row, *col;  // by counted row; by column of the piece, readable up to whole tiles
+
+    __device__ __forceinline__ float of_row(int64_t r, bool ok) const { return row != nullptr && ok ? row[r] : 1.f; }
+    template <bool SCALED>
+    __device__ __forceinline__ f32x4_v of_cols(int64_t c) const {
+        if constexpr (SCALED)
+            return *as_global(reinterpret_cast<const f32x4_v *>(col + c));
+        else
+            return f32x4_v{1.f, 1.f, 1.f, 1.f};
+    }
+};
 
 // ---- epilogues -----------------------------------------------------------------------------------------------
 // acc[x][y][4 g + e] is row row0 + 32 y + (lane & 31), column col0 + 32 x + 8 g + 4 (lane >> 5) + e of the tile.
@@ -180,8 +273,10 @@ __device__ __forceinline__ void store_rows(const uint8_t *stage, uint8_t *out, i
 
 // Statistics of a tile's rows over a wave's columns, in units of log2: their maximum and sum without the target,
 // the target's own value, and where wanted the plain sum of the values.
+template <bool SCALED>
 struct StatsEpilogue {
     const int32_t *tgt;
+    Scales scales;
     float2 *part;            // by (column part, row): part * part_stride + row * row_stride
     float *sum;              // likewise, or null
     float *at_target;        // by row
@@ -200,54 +295,63 @@ struct StatsEpilogue {
             const bool ok = row < t.rows;
             const int64_t off = ok ? tgt[row] - (first + c0) : -1;
             const int mine = off >= 0 && off < there ? static_cast<int>(off) : -1;
+            const float kr = k * scales.of_row(row, ok);
             // few waves hold a target of their rows, or the vocabulary's end
             if (there < 32 * SX || __any(mine >= 0))
-                row_part<AGPR, true, SX, SY>(acc, y, row, ok, mine, there, part_at, lane);
+                row_part<AGPR, true, SX, SY>(acc, y, row, kr, c0, ok, mine, there, part_at, lane);
             else
-                row_part<AGPR, false, SX, SY>(acc, y, row, ok, mine, there, part_at, lane);
+                row_part<AGPR, false, SX, SY>(acc, y, row, kr, c0, ok, mine, there, part_at, lane);
         }
     }
 
     template <bool AGPR, bool SOME, int SX, int SY>
-    __device__ __forceinline__ void row_part(const floatx16 (&acc)[SX][SY], int y, int64_t row, bool ok, int mine, int there, int64_t part_at,
-                                             int lane) const {
+    __device__ __forceinline__ void row_part(const floatx16 (&acc)[SX][SY], int y, int64_t row, float kr, int64_t c0, bool ok, int mine,
+                                             int there, int64_t part_at, int lane) const {
         const int half4 = 4 * (lane >> 5);
         float m = -__builtin_inff(), total = 0.f;
 #pragma unroll
         for (int x = 0; x < SX; ++x)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                float v = acc_read<AGPR>(acc[x][y], e);
-                if constexpr (SOME) {
-                    const int col = 32 * x + 8 * (e >> 2) + half4 + (e & 3);
-                    total += col < there ? v : 0.f;
-                    if (col == mine) at_target[row] = v * k;
-                    if (col == mine || col >= there) v = -__builtin_inff();
-                } else {
-                    total += v;
+            for (int q = 0; q < 4; ++q) {
+                const f32x4_v cs = scales.of_cols<SCALED>(c0 + 32 * x + 8 * q + half4);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float v = acc_read<AGPR>(acc[x][y], 4 * q + e) * cs[e];
+                    if constexpr (SOME) {
+                        const int col = 32 * x + 8 * q + half4 + e;
+                        total += col < there ? v : 0.f;
+                        if (col == mine) at_target[row] = v * kr;
+                        if (col == mine || col >= there) v = -__builtin_inff();
+                    } else {
+                        total += v;
+                    }
+                    m = fmaxf(m, v);
                 }
-                m = fmaxf(m, v);
             }
-        m = fmaxf(m, __shfl_xor(m, 32)) * k;
+        m = fmaxf(m, __shfl_xor(m, 32)) * kr;
         const float shift = m == -__builtin_inff() ? 0.f : m;
         float s = 0.f;
         if constexpr (SOME) asm volatile("" : "+v"(mine), "+s"(there));  // compared anew: 64 lane masks are not kept
 #pragma unroll
         for (int x = 0; x < SX; ++x)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                float v = acc_read<AGPR>(acc[x][y], e);
-                if constexpr (SOME) {
-                    const int col = 32 * x + 8 * (e >> 2) + half4 + (e & 3);
-                    if (col == mine || col >= there) v = -__builtin_inff();
+            for (int q = 0; q < 4; ++q) {
+                const f32x4_v cs = scales.of_cols<SCALED>(c0 + 32 * x + 8 * q + half4);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float v = acc_read<AGPR>(acc[x][y], 4 * q + e) * cs[e];
+                    if constexpr (SOME) {
+                        const int col = 32 * x + 8 * q + half4 + e;
+                        if (col == mine || col >= there) v = -__builtin_inff();
+                    }
+                    s += __builtin_amdgcn_exp2f(fmaf(v, kr, -shift));
                 }
-                s += __builtin_amdgcn_exp2f(fmaf(v, k, -shift));
             }
         s += __shfl_xor(s, 32);
         total += __shfl_xor(total, 32);
         if (ok && lane < 32) {
             part[part_at * part_stride + row * row_stride] = make_float2(m, s);
-            if (sum != nullptr) sum[part_at * part_stride + row * row_stride] = total * k;
+            if (sum != nullptr) sum[part_at * part_stride + row * row_stride] = total * kr;
         }
     }
 };
@@ -257,6 +361,7 @@ struct StatsEpilogue {
 template <int NPARTS>
 struct ExpEpilogue {
     const int32_t *tgt;
+    Scales scales;
     const float *ref;        // by row, log2
     float *part, *sum;       // by (column part, row), as StatsEpilogue
     float *at_target;
@@ -281,24 +386,25 @@ struct ExpEpilogue {
             const int64_t off = ok ? tgt[row] - (first + c0) : -1;
             const int mine = off >= 0 && off < there ? static_cast<int>(off) : -1;
             float s, total = 0.f;
-            // three parts: one way through it, or the code outgrows what the compiler unrolls; the K loop is six times as long
+            const float kr = k * scales.of_row(row, ok);
+            // three parts: one way through it, or the code outgrows what the compiler unrolls; the K loop is three times as long
             if (NPARTS > 1 || there < 32 * SX || __any(mine >= 0))
-                s = stage_rows<AGPR, true, SX, SY>(acc, y, row, shift, mine, there, total, stage, lane);
+                s = stage_rows<AGPR, true, SX, SY>(acc, y, row, kr, c0, shift, mine, there, total, stage, lane);
             else
-                s = stage_rows<AGPR, false, SX, SY>(acc, y, row, shift, mine, there, total, stage, lane);
+                s = stage_rows<AGPR, false, SX, SY>(acc, y, row, kr, c0, shift, mine, there, total, stage, lane);
             s += __shfl_xor(s, 32);
             total += __shfl_xor(total, 32);
             if (ok && lane < 32) {
                 part[part_at * part_stride + row * row_stride] = s;
-                if (sum != nullptr) sum[part_at * part_stride + row * row_stride] = total * k;
+                if (sum != nullptr) sum[part_at * part_stride + row * row_stride] = total * kr;
             }
             store_rows<NPARTS, SX>(stage, out, ld, out_part, t.r0 + row0 + 32 * y, t.rows, c0, lane);
         }
     }
 
     template <bool AGPR, bool SOME, int SX, int SY>
-    __device__ __forceinline__ float stage_rows(const floatx16 (&acc)[SX][SY], int y, int64_t row, float shift, int mine, int there,
-                                                float &total, uint8_t *stage, int lane) const {
+    __device__ __forceinline__ float stage_rows(const floatx16 (&acc)[SX][SY], int y, int64_t row, float kr, int64_t c0, float shift, int mine,
+                                                int there, float &total, uint8_t *stage, int lane) const {
         const int half4 = 4 * (lane >> 5);
         float s = 0.f;
 #pragma unroll
@@ -306,13 +412,14 @@ struct ExpEpilogue {
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 float v[4];
+                const f32x4_v cs = scales.of_cols<(NPARTS > 1)>(c0 + 32 * x + 8 * q + half4);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float z = acc_read<AGPR>(acc[x][y], 4 * q + e);
-                    v[e] = __builtin_amdgcn_exp2f(fmaf(z, k, -shift));
+                    const float z = acc_read<AGPR>(acc[x][y], 4 * q + e) * cs[e];
+                    v[e] = __builtin_amdgcn_exp2f(fmaf(z, kr, -shift));
                     if constexpr (SOME) {
                         const int col = 32 * x + 8 * q + half4 + e;
-                        if (col == mine) at_target[row] = z * k;
+                        if (col == mine) at_target[row] = z * kr;
                         if (col == mine || col >= there) v[e] = 0.f;
                         total += col < there ? z : 0.f;
                     } else {
@@ -334,6 +441,7 @@ struct RowGrad {
 template <int NPARTS>
 struct GradEpilogue {
     const int32_t *tgt;
+    Scales scales;
     const RowGrad *grad;
     uint8_t *out;          // [rows][ld] of each part
     int64_t ld, part;      // ld: columns of the piece, a multiple of 64; part: bytes
@@ -357,26 +465,28 @@ struct GradEpilogue {
             const RowGrad g = ok ? grad[row] : RowGrad{0.f, 0.f, 0.f, 0.f};
             const int64_t off = ok ? tgt[row] - (first + c0) : -1;
             const int mine = off >= 0 && off < there ? static_cast<int>(off) : -1;
-            if (there < 32 * SX || __any(mine >= 0))
-                stage_rows<AGPR, true, SX, SY>(acc, y, g, mine, there, stage, lane);
+            const float kr = k * scales.of_row(row, ok);
+            if (NPARTS > 1 || there < 32 * SX || __any(mine >= 0))
+                stage_rows<AGPR, true, SX, SY>(acc, y, g, kr, c0, mine, there, stage, lane);
             else
-                stage_rows<AGPR, false, SX, SY>(acc, y, g, mine, there, stage, lane);
+                stage_rows<AGPR, false, SX, SY>(acc, y, g, kr, c0, mine, there, stage, lane);
             store_rows<NPARTS, SX>(stage, out, ld, part, t.r0 + row0 + 32 * y, t.rows, c0, lane);
         }
     }
 
     template <bool AGPR, bool SOME, int SX, int SY>
-    __device__ __forceinline__ void stage_rows(const floatx16 (&acc)[SX][SY], int y, const RowGrad &g, int mine, int there, uint8_t *stage,
-                                               int lane) const {
+    __device__ __forceinline__ void stage_rows(const floatx16 (&acc)[SX][SY], int y, const RowGrad &g, float kr, int64_t c0, int mine,
+                                               int there, uint8_t *stage, int lane) const {
         const int half4 = 4 * (lane >> 5);
 #pragma unroll
         for (int x = 0; x < SX; ++x)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 float v[4];
+                const f32x4_v cs = scales.of_cols<(NPARTS > 1)>(c0 + 32 * x + 8 * q + half4);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    v[e] = fmaf(__builtin_amdgcn_exp2f(fmaf(acc_read<AGPR>(acc[x][y], 4 * q + e), k, -g.lse2)), g.ca, -g.cb);
+                    v[e] = fmaf(__builtin_amdgcn_exp2f(fmaf(acc_read<AGPR>(acc[x][y], 4 * q + e) * cs[e], kr, -g.lse2)), g.ca, -g.cb);
                     if constexpr (SOME) {
                         const int col = 32 * x + 8 * q + half4 + e;
                         if (col == mine) v[e] = g.gt;
@@ -498,8 +608,6 @@ __device__ __forceinline__ Sum2 join(Sum2 a, Sum2 b) {
 constexpr int kVectorRows = 8;
 constexpr int kVectorLds = 64 * 1024;
 constexpr int kVectorGroups = 2048;
-
-typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 
 struct VectorArgs {
     Layout h;
@@ -881,6 +989,8 @@ struct RedoArgs {
     const float *ref;
     const int32_t *tgt;
     int32_t *count, *rows, *tgt2;
+    const float *scale;  // of the rows' parts, or null
+    float *scale2;
 };
 
 __global__ __launch_bounds__(kIndexThreads) void redo_kernel(const RedoArgs a) {
@@ -905,6 +1015,7 @@ __global__ __launch_bounds__(kIndexThreads) void redo_kernel(const RedoArgs a) {
             const int r = before + __popcll(mask & ((uint64_t{1} << lane) - 1));
             a.rows[r] = i;
             a.tgt2[r] = a.tgt[i];
+            if (a.scale) a.scale2[r] = a.scale[i];
         }
         at += all;
         __syncthreads();
@@ -1018,12 +1129,13 @@ enum Pass { kStats, kBackward, kLeavesUnit };  // the forward alone, the backwar
 struct Plan {
     int64_t n, rows, vocab, dim, ld;  // rows: n rounded up, at least 64; ld: dim rounded up to whole slabs
     bool f32, few, copy_w;            // copy_w: the head is laid out piece by piece
-    int np;                           // parts of an operand
+    int np, nz;                       // parts of an operand: of a product with the gradient, of the logits
     int64_t piece;                    // columns of the vocabulary at a time
     int splits;                       // of the product with W, at most
     int split_cost;
     int64_t h, tgt, part, sum, at_target, row_loss, w, g, grad, acc;  // workspace offsets
     int64_t ref, redo, h2, tgt2, columns, column_part;
+    int64_t z, wz, row_scale, col_scale, row_scale2;  // fp32: hidden states and head in fp16 parts, and their scales
     int64_t bytes;
 };
 
@@ -1034,6 +1146,7 @@ Plan plan_of(int64_t n, int64_t vocab, int64_t dim, int dtype, const void *weigh
     p.n = n, p.vocab = vocab, p.dim = dim, p.ld = round_up(dim, kSlabK);
     p.f32 = dtype == ME_F32;
     p.np = p.f32 ? 3 : 1;
+    p.nz = p.f32 ? 2 : 1;
     p.few = n <= kFew;
     p.copy_w = p.f32 || w_stride % 8 != 0 || reinterpret_cast<uintptr_t>(weight) % 16 != 0;
     const int64_t rows = p.rows = round_up(std::max<int64_t>(n, 1), 64);
@@ -1048,10 +1161,18 @@ Plan plan_of(int64_t n, int64_t vocab, int64_t dim, int dtype, const void *weigh
         at += round_up(bytes, 256);
         return here;
     };
-    p.h = take(rows * p.ld * 2 * p.np);
     p.tgt = take(n * 4);
     p.grad = take(n * static_cast<int64_t>(sizeof(RowGrad)));
-    if (p.copy_w) p.w = take(p.piece * p.ld * 2 * p.np);
+    p.z = take(rows * p.ld * 2 * p.nz);
+    p.h = p.z;
+    if (p.copy_w) p.wz = take(p.piece * p.ld * 2 * p.nz);
+    p.w = p.wz;
+    if (p.f32) {
+        p.row_scale = take(n * 4);
+        p.col_scale = take((p.piece + kTile) * 4);
+        if (pass == kBackward) p.h = take(rows * p.ld * 2 * p.np);
+        if (pass != kStats) p.w = take(p.piece * p.ld * 2 * p.np);
+    }
     if (pass != kBackward) {
         const int64_t parts = std::max<int64_t>(ceil_div(vocab, p.few ? 64 : 128) + 4, n <= kVectorRows ? kVectorGroups : 0);
         p.part = take(parts * rows * 8);
@@ -1071,8 +1192,9 @@ Plan plan_of(int64_t n, int64_t vocab, int64_t dim, int dtype, const void *weigh
     if (pass == kLeavesUnit) {
         p.ref = take(n * 4);
         p.redo = take((kHeader + n) * 4);
-        p.h2 = take(rows * p.ld * 2 * p.np);
+        p.h2 = take(rows * p.ld * 2 * p.nz);
         p.tgt2 = take(n * 4);
+        if (p.f32) p.row_scale2 = take(n * 4);
         p.columns = take(dim * 4);
         p.column_part = take(ceil_div(vocab, kColumnRows) * dim * 4);
     }
@@ -1109,23 +1231,52 @@ void lay_out(bool f32, const Layout &l, hipStream_t s) {
 
 int64_t h_part(const Plan &p) { return p.rows * p.ld * 2; }
 
-Layout hidden_layout(const Plan &p, const Call &c) {
-    return {c.hidden, c.per_batch, c.batch_stride, c.row_stride, c.s.rows, c.s.count, p.n, p.dim, p.ld, h_part(p), c.ws + p.h};
+Layout hidden_layout(const Plan &p, const Call &c, int64_t to) {
+    return {c.hidden, c.per_batch, c.batch_stride, c.row_stride, c.s.rows, c.s.count, p.n, p.dim, p.ld, h_part(p), c.ws + to};
 }
 
-// Rows of a product: the hidden states laid out, with how many there are and their targets
+void lay_out16(const Layout &l, float *scale, hipStream_t s) {
+    const unsigned blocks = static_cast<unsigned>(std::min<int64_t>(std::max<int64_t>(ceil_div(l.n, 4), 1), 16384));
+    hipLaunchKernelGGL(layout16_kernel, dim3(blocks), dim3(256), 0, s, l, scale);
+}
+
+// Rows of a product: the hidden states laid out for the logits, with how many there are, their targets and, of
+// fp16 parts, their scales
 struct Rows {
     uint8_t *h;
     const int32_t *count, *tgt;
+    const float *scale;
 };
 
-// The head from row v0 on, `width` rows of it
-Operand weight_operand(const Plan &p, const Call &c, int64_t v0, int64_t width) {
+Rows lay_out_rows(const Plan &p, const Call &c) {
+    float *scale = p.f32 ? reinterpret_cast<float *>(c.ws + p.row_scale) : nullptr;
+    if (p.f32)
+        lay_out16(hidden_layout(p, c, p.z), scale, c.stream);
+    else
+        lay_out(false, hidden_layout(p, c, p.z), c.stream);
+    return {c.ws + p.z, c.s.count, reinterpret_cast<const int32_t *>(c.ws + p.tgt), scale};
+}
+
+// The head from row v0 on, `width` rows of it, for the logits and for the product with their gradient
+struct Head {
+    Operand logits, product;
+    const float *scale;  // of the logits' columns
+};
+
+Head head_of(const Plan &p, const Call &c, int64_t v0, int64_t width, bool for_product, const int32_t *gate = nullptr) {
     const uint8_t *from = static_cast<const uint8_t *>(c.weight) + v0 * c.w_stride * (p.f32 ? 4 : 2);
-    if (!p.copy_w) return {from, c.w_stride, 0};
+    if (!p.copy_w) return {{from, c.w_stride, 0}, {from, c.w_stride, 0}, nullptr};
     const int64_t part = p.piece * p.ld * 2;
-    lay_out(p.f32, Layout{from, width, 0, c.w_stride, nullptr, nullptr, width, p.dim, p.ld, part, c.ws + p.w}, c.stream);
-    return {c.ws + p.w, p.ld, part};
+    Layout l{from, width, 0, c.w_stride, nullptr, nullptr, width, p.dim, p.ld, part, c.ws + p.wz, gate};
+    float *scale = p.f32 ? reinterpret_cast<float *>(c.ws + p.col_scale) : nullptr;
+    if (p.f32) {
+        lay_out16(l, scale, c.stream);
+        l.dst = c.ws + p.w;
+        if (for_product) lay_out(true, l, c.stream);
+    } else {
+        lay_out(false, l, c.stream);
+    }
+    return {{c.ws + p.wz, p.ld, part}, {c.ws + p.w, p.ld, part}, scale};
 }
 
 template <bool A_KC, bool B_KC, int SEGS, class Epilogue>
@@ -1143,8 +1294,8 @@ void multiply_few(const Gemm &g, const Epilogue &e, hipStream_t s) {
 
 // logits of a piece: rows x head rows
 template <int SEGS, class Epilogue>
-void logits_of(const Plan &p, const Call &c, const Rows &rows, const Operand &w, int64_t width, const Epilogue &e) {
-    const Gemm g{{rows.h, p.ld, h_part(p)}, w, p.n, width, p.dim, rows.count, 0, 8, 1, 0};
+void logits_of(const Plan &p, const Call &c, const Rows &rows, const Head &w, int64_t width, const Epilogue &e) {
+    const Gemm g{{rows.h, p.ld, h_part(p)}, w.logits, p.n, width, p.dim, rows.count, 0, 8, 1, 0};
     if (p.few)
         multiply_few<true, SEGS>(g, e, c.stream);
     else
@@ -1152,8 +1303,8 @@ void logits_of(const Plan &p, const Call &c, const Rows &rows, const Operand &w,
 }
 
 // product of a piece of the logits' gradient (or exponentials) with the head, onto the sums
-void times_head(const Plan &p, const Call &c, const Rows &rows, const Operand &w, int64_t v0, int64_t width) {
-    const Gemm g{{c.ws + p.g, p.piece, p.rows * p.piece * 2}, w, p.n, p.dim, width, rows.count, 0, 8, p.splits, p.split_cost};
+void times_head(const Plan &p, const Call &c, const Rows &rows, const Head &w, int64_t v0, int64_t width) {
+    const Gemm g{{c.ws + p.g, p.piece, p.rows * p.piece * 2}, w.product, p.n, p.dim, width, rows.count, 0, 8, p.splits, p.split_cost};
     const AccumulateEpilogue e{reinterpret_cast<float *>(c.ws + p.acc), p.ld, p.rows * p.ld, v0 > 0};
     if (p.few)
         p.f32 ? multiply_few<false, 6>(g, e, c.stream) : multiply_few<false, 1>(g, e, c.stream);
@@ -1165,12 +1316,13 @@ Sums sums_of(const Plan &p, const Call &c) {
     return {reinterpret_cast<float *>(c.ws + p.acc), p.ld, p.rows * p.ld, p.few ? 64 : kTile, static_cast<int>(ceil_div(p.dim, kTile)), p.splits, p.split_cost};
 }
 
-void gradient_of(const Plan &p, const Call &c, const Rows &rows, const Operand &w, int64_t v0, int64_t width, const RowGrad *grad, float k) {
+void gradient_of(const Plan &p, const Call &c, const Rows &rows, const Head &w, int64_t v0, int64_t width, const RowGrad *grad, float k) {
     const int64_t part = p.rows * p.piece * 2;
+    const Scales scales{rows.scale, w.scale};
     if (p.f32)
-        logits_of<6>(p, c, rows, w, width, GradEpilogue<3>{rows.tgt, grad, c.ws + p.g, p.piece, part, v0, width, k});
+        logits_of<3>(p, c, rows, w, width, GradEpilogue<3>{rows.tgt, scales, grad, c.ws + p.g, p.piece, part, v0, width, k});
     else
-        logits_of<1>(p, c, rows, w, width, GradEpilogue<1>{rows.tgt, grad, c.ws + p.g, p.piece, part, v0, width, k});
+        logits_of<1>(p, c, rows, w, width, GradEpilogue<1>{rows.tgt, scales, grad, c.ws + p.g, p.piece, part, v0, width, k});
 }
 
 void finish(const Plan &p, const FinishArgs &f, hipStream_t s) {
@@ -1206,70 +1358,60 @@ void unit_of(const Plan &p, const Call &c, const Loss &l, const Rows &rows, cons
         hipLaunchKernelGGL(unit_kernel<false>, dim3(blocks), dim3(256), 0, c.stream, u);
 }
 
+// Statistics of the rows' logits, piece by piece
+template <bool F32>
+void stats_of(const Plan &p, const Call &c, const Rows &rows, StatsEpilogue<F32> e, const int32_t *gate = nullptr) {
+    e.tgt = rows.tgt;
+    for (int64_t v0 = 0; v0 < p.vocab; v0 += p.piece) {
+        const int64_t width = std::min(p.piece, p.vocab - v0);
+        const Head w = head_of(p, c, v0, width, false, gate);
+        e.first = v0, e.vocab = width, e.scales = {rows.scale, w.scale};
+        logits_of<F32 ? 3 : 1>(p, c, rows, w, width, e);
+    }
+}
+
+template <bool F32>
 void forward_rows(const Plan &p, const Call &c, const Loss &l) {
     hipStream_t s = c.stream;
-    const Rows rows{c.ws + p.h, c.s.count, reinterpret_cast<int32_t *>(c.ws + p.tgt)};
-    const Layout h = hidden_layout(p, c);
-    lay_out(p.f32, h, s);
+    const Rows rows = lay_out_rows(p, c);
     const int cols = p.few ? 64 : 128;
     const int parts = static_cast<int>(ceil_div(p.vocab, cols));
     const float k = static_cast<float>(1.44269504088896340736 / l.temperature);
     float *at_target = reinterpret_cast<float *>(c.ws + p.at_target);
 
-    StatsEpilogue e{};
-    e.tgt = rows.tgt;
+    StatsEpilogue<F32> e{};
     e.part = reinterpret_cast<float2 *>(c.ws + p.part);
     e.sum = l.smoothing != 0.0 ? reinterpret_cast<float *>(c.ws + p.sum) : nullptr;
     e.at_target = at_target;
     e.part_stride = p.few ? 1 : p.rows;
     e.row_stride = p.few ? parts + 4 : 1;
     e.k = k;
-    auto stats = [&](const Rows &of) {
-        e.tgt = of.tgt;
-        for (int64_t v0 = 0; v0 < p.vocab; v0 += p.piece) {
-            const int64_t width = std::min(p.piece, p.vocab - v0);
-            e.first = v0, e.vocab = width;
-            const Operand w = weight_operand(p, c, v0, width);
-            if (p.f32)
-                logits_of<6>(p, c, of, w, width, e);
-            else
-                logits_of<1>(p, c, of, w, width, e);
-        }
-    };
     FinishArgs f{};
     f.part = e.part, f.sum = e.sum, f.at_target = at_target, f.part_stride = e.part_stride, f.row_stride = e.row_stride, f.parts = parts;
     f.n = p.n, f.vocab = p.vocab, f.s = c.s, f.logps = l.logps;
     f.row_loss = l.loss ? reinterpret_cast<float *>(c.ws + p.row_loss) : nullptr;
     f.smoothing = static_cast<float>(l.smoothing), f.z_loss = static_cast<float>(l.z_loss);
     if (!l.unit) {
-        stats(rows);
+        stats_of<F32>(p, c, rows, e);
         finish(p, f, s);
         return;
     }
     float *ref = reinterpret_cast<float *>(c.ws + p.ref);
-    const unsigned waves = static_cast<unsigned>(ceil_div(p.n, 4));
-    if (p.f32)
-        hipLaunchKernelGGL(ref_kernel<true>, dim3(waves), dim3(256), 0, s, h, c.weight, c.w_stride, rows.tgt, k, ref);
-    else
-        hipLaunchKernelGGL(ref_kernel<false>, dim3(waves), dim3(256), 0, s, h, c.weight, c.w_stride, rows.tgt, k, ref);
+    hipLaunchKernelGGL(ref_kernel<F32>, dim3(static_cast<unsigned>(ceil_div(p.n, 4))), dim3(256), 0, s, hidden_layout(p, c, p.z), c.weight, c.w_stride,
+                       rows.tgt, k, ref);
     if (l.smoothing != 0.0) {
         const dim3 grid(static_cast<unsigned>(ceil_div(p.dim, 256)), static_cast<unsigned>(ceil_div(p.vocab, kColumnRows)));
         float *part = reinterpret_cast<float *>(c.ws + p.column_part);
-        if (p.f32)
-            hipLaunchKernelGGL(column_kernel<true>, grid, dim3(256), 0, s, c.weight, c.w_stride, p.vocab, p.dim, part);
-        else
-            hipLaunchKernelGGL(column_kernel<false>, grid, dim3(256), 0, s, c.weight, c.w_stride, p.vocab, p.dim, part);
+        hipLaunchKernelGGL(column_kernel<F32>, grid, dim3(256), 0, s, c.weight, c.w_stride, p.vocab, p.dim, part);
         hipLaunchKernelGGL(column_total_kernel, dim3(grid.x), dim3(256), 0, s, part, static_cast<int>(grid.y), p.dim, reinterpret_cast<float *>(c.ws + p.columns));
     }
     float *exps = reinterpret_cast<float *>(c.ws + p.part);
-    const int64_t out_part = p.rows * p.piece * 2;
     for (int64_t v0 = 0; v0 < p.vocab; v0 += p.piece) {
         const int64_t width = std::min(p.piece, p.vocab - v0);
-        const Operand w = weight_operand(p, c, v0, width);
-        if (p.f32)
-            logits_of<6>(p, c, rows, w, width, ExpEpilogue<3>{rows.tgt, ref, exps, e.sum, at_target, e.part_stride, e.row_stride, c.ws + p.g, p.piece, out_part, v0, width, k});
-        else
-            logits_of<1>(p, c, rows, w, width, ExpEpilogue<1>{rows.tgt, ref, exps, e.sum, at_target, e.part_stride, e.row_stride, c.ws + p.g, p.piece, out_part, v0, width, k});
+        const Head w = head_of(p, c, v0, width, true);
+        const ExpEpilogue<F32 ? 3 : 1> exp{rows.tgt, {rows.scale, w.scale}, ref, exps, e.sum, at_target, e.part_stride, e.row_stride,
+                                           c.ws + p.g, p.piece, p.rows * p.piece * 2, v0, width, k};
+        logits_of<F32 ? 3 : 1>(p, c, rows, w, width, exp);
         times_head(p, c, rows, w, v0, width);
     }
     f.exps = exps, f.ref = ref;
@@ -1279,18 +1421,19 @@ void forward_rows(const Plan &p, const Call &c, const Loss &l) {
     // rows that ref was too far from
     int32_t *redo = reinterpret_cast<int32_t *>(c.ws + p.redo);
     int32_t *tgt2 = reinterpret_cast<int32_t *>(c.ws + p.tgt2);
+    float *scale2 = F32 ? reinterpret_cast<float *>(c.ws + p.row_scale2) : nullptr;
     RowGrad *grad = reinterpret_cast<RowGrad *>(c.ws + p.grad);
-    const Rows again{c.ws + p.h2, redo, tgt2};
-    hipLaunchKernelGGL(redo_kernel, dim3(1), dim3(kIndexThreads), 0, s, RedoArgs{c.s, ref, rows.tgt, redo, redo + kHeader, tgt2});
-    for (int part = 0; part < p.np; ++part)
-        lay_out(false, Layout{c.ws + p.h + part * h_part(p), std::max<int64_t>(p.n, 1), 0, p.ld, redo + kHeader, redo, p.n, p.ld, p.ld, 0, again.h + part * h_part(p)}, s);
-    stats(again);
+    const Rows again{c.ws + p.h2, redo, tgt2, scale2};
+    hipLaunchKernelGGL(redo_kernel, dim3(1), dim3(kIndexThreads), 0, s, RedoArgs{c.s, ref, rows.tgt, redo, redo + kHeader, tgt2, rows.scale, scale2});
+    for (int part = 0; part < p.nz; ++part)
+        lay_out(false, Layout{rows.h + part * h_part(p), p.n, 0, p.ld, redo + kHeader, redo, p.n, p.ld, p.ld, 0, again.h + part * h_part(p)}, s);
+    stats_of<F32>(p, c, again, e, redo);
     f.exps = nullptr, f.ref = nullptr, f.count = redo, f.which = redo + kHeader;
     finish(p, f, s);
     hipLaunchKernelGGL(redo_coef_kernel, dim3(row_blocks(p.n)), dim3(256), 0, s, c.s, redo, redo + kHeader, f.z_loss, grad);
     for (int64_t v0 = 0; v0 < p.vocab; v0 += p.piece) {
         const int64_t width = std::min(p.piece, p.vocab - v0);
-        const Operand w = weight_operand(p, c, v0, width);
+        const Head w = head_of(p, c, v0, width, true, redo);
         gradient_of(p, c, again, w, v0, width, grad, k);
         times_head(p, c, again, w, v0, width);
     }
@@ -1320,7 +1463,7 @@ bool takes_vectors(const Plan &p, int &rows, size_t &lds) {
 void forward_vectors(const Plan &p, const Call &c, const Loss &l, int rows, size_t lds) {
     const unsigned groups = static_cast<unsigned>(std::min<int64_t>(ceil_div(p.vocab, 8), kVectorGroups));
     VectorArgs a{};
-    a.h = hidden_layout(p, c);
+    a.h = hidden_layout(p, c, p.z);
     a.weight = static_cast<const float *>(c.weight), a.w_stride = c.w_stride, a.vocab = p.vocab, a.targets = c.targets, a.t64 = c.tdtype == ME_I64, a.ignore = c.ignore, a.s = c.s;
     a.part = reinterpret_cast<float2 *>(c.ws + p.part);
     a.sum = l.smoothing != 0.0 ? reinterpret_cast<float *>(c.ws + p.sum) : nullptr;
@@ -1350,7 +1493,7 @@ int forward(const Plan &p, const Call &c, const Loss &l) {
     else
         hipLaunchKernelGGL(index_kernel<int32_t>, dim3(1), dim3(kIndexThreads), 0, s, static_cast<const int32_t *>(c.targets), p.n, c.ignore, p.vocab, c.s, tgt);
     if (p.n > 0) {
-        forward_rows(p, c, l);
+        p.f32 ? forward_rows<true>(p, c, l) : forward_rows<false>(p, c, l);
         if (l.logps) hipLaunchKernelGGL(uncounted_logps_kernel, dim3(row_blocks(p.n)), dim3(256), 0, s, c.s.place, p.n, l.logps);
     }
     if (l.loss) hipLaunchKernelGGL(total_kernel, dim3(1), dim3(1024), 0, s, reinterpret_cast<const float *>(c.ws + p.row_loss), c.s.count, l.scale, l.mean, l.loss);
@@ -1452,7 +1595,7 @@ extern "C" int me_head_backward(const void *hidden, int dtype, int64_t n, int64_
                  static_cast<uint8_t *>(workspace), saved_rows, as_stream(stream)};
     hipStream_t s = c.stream;
     int32_t *tgt = reinterpret_cast<int32_t *>(c.ws + p.tgt);
-    const Rows rows{c.ws + p.h, c.s.count, tgt};
+    Rows rows{};
     RowGrad *grad = reinterpret_cast<RowGrad *>(c.ws + p.grad);
     if (n > 0) {
         const dim3 blocks(row_blocks(n));
@@ -1463,13 +1606,14 @@ extern "C" int me_head_backward(const void *hidden, int dtype, int64_t n, int64_
         const CoefArgs k{c.s, n, upstream, upstream_per_row != 0, reduction == ME_REDUCE_MEAN, scale / temperature, static_cast<float>(smoothing),
                          static_cast<float>(z_loss), static_cast<double>(vocab), grad};
         hipLaunchKernelGGL(coef_kernel, blocks, dim3(256), 0, s, k);
-        lay_out(p.f32, hidden_layout(p, c), s);
+        rows = lay_out_rows(p, c);
+        if (f32 && grad_weight) lay_out(true, hidden_layout(p, c, p.h), s);
     }
     const float k = static_cast<float>(1.44269504088896340736 / temperature);
     for (int64_t v0 = 0; v0 < vocab; v0 += p.piece) {
         const int64_t width = std::min(p.piece, vocab - v0);
         if (n > 0) {
-            const Operand w = weight_operand(p, c, v0, width);
+            const Head w = head_of(p, c, v0, width, grad_hidden != nullptr);
             gradient_of(p, c, rows, w, v0, width, grad, k);
             if (grad_hidden) times_head(p, c, rows, w, v0, width);
         }

@@ -12,9 +12,14 @@
 //                   which transpose 4 x 16 blocks on the way (see rc_lane_off)
 // A 32x32x16 MFMA operand holds, in lane l, the 8 k values 16 ks + 8 (l >> 5) .. + 7 of row / column l & 31.
 //
-// fp32 operands come as three bf16 parts each that add up to them exactly; the six products of parts that are not
-// below 2^-26 of the whole are accumulated, as segments of one reduction (SEGS 6): A's part stride and
-// B's lead from one part to the next.
+// fp32 operands come in parts, whose products are segments of one reduction; A's part stride and B's lead from one
+// part to the next:
+//   SEGS 6  three bf16 parts that add up to the value exactly; six of their nine products, the others are below
+//           2^-26 of the whole. Keeps every value's digits, whatever the values around it.
+//   SEGS 3  two fp16 parts of the value over a power of two by row that puts the row's largest below 2^15; three of
+//           their four products, the fourth is below 2^-22 of the whole, its root mean square 2^-25. Half the
+//           matrix time; a value's parts hold it to 2^-22 of itself, or 2^-40 of its row's largest where that
+//           is more. That is as exact as fp32 for logits, whose error counts against those of their row.
 #pragma once
 
 #include "me_common.h"
@@ -33,6 +38,7 @@ constexpr uint32_t kOff = 0xffffffffu;           // a load offset past every buf
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef int int32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) bf16x4 lds_bf16x4;
@@ -40,7 +46,7 @@ typedef __attribute__((address_space(3))) bf16x4 lds_bf16x4;
 struct Operand {
     const uint8_t *base;
     int64_t ld;     // elements from one row (k-row) to the next
-    int64_t part;   // bytes from one part to the next (SEGS 6)
+    int64_t part;   // bytes from one part to the next
 };
 
 struct Gemm {
@@ -69,9 +75,17 @@ __device__ inline int splits_for(int tiles, int most, int cost) {
     return best;
 }
 
-// segment -> parts of A and B: (0,0) (0,1) (1,0) (0,2) (1,1) (2,0)
+// segment -> parts of A and B: (0,0) (0,1) (1,0) and for SEGS 6 on to (0,2) (1,1) (2,0)
 __device__ __forceinline__ int part_a(int seg) { return (0x910 >> (2 * seg)) & 3; }
 __device__ __forceinline__ int part_b(int seg) { return (0x184 >> (2 * seg)) & 3; }
+
+template <int SEGS>
+__device__ __forceinline__ floatx16 multiply(const bf16x8 &x, const bf16x8 &y, const floatx16 &acc) {
+    if constexpr (SEGS == 3)
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(halfx8, x), __builtin_bit_cast(halfx8, y), acc, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, acc, 0, 0, 0);
+}
 
 __device__ __forceinline__ int32x4 buffer_rsrc(uint64_t base, uint32_t bytes) {
     int32x4 r;
@@ -358,8 +372,7 @@ __global__ __launch_bounds__(kThreads, 1) void large_kernel(const Gemm a, const 
     for (int q = 0; q < kParts; ++q) load_part(unit_a(0), unit_b(0), 0, f0, part_of(q));
 
     auto mfma = [&](const Frag &f, int i) {
-        acc[i / kSub][i % kSub] =
-            __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.s[i / kSub], f.r[i % kSub], acc[i / kSub][i % kSub], 0, 0, 0);
+        acc[i / kSub][i % kSub] = multiply<SEGS>(f.s[i / kSub], f.r[i % kSub], acc[i / kSub][i % kSub]);
         __builtin_amdgcn_sched_barrier(0);
     };
     // Slab s, four k-steps: each k-step's MFMAs run while the next one's fragments are read. k-steps 0 and 1
@@ -497,7 +510,7 @@ __global__ __launch_bounds__(kThreads) void few_kernel(const Gemm a, const Epilo
             for (int x = 0; x < kBS; ++x)
 #pragma unroll
                 for (int y = 0; y < kBR; ++y)
-                    acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fs[x], fr[y], acc[x][y], 0, 0, 0);
+                    acc[x][y] = multiply<SEGS>(fs[x], fr[y], acc[x][y]);
         }
     }
     __syncthreads();
