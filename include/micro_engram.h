@@ -682,15 +682,15 @@ int me_distill_backward(const void *logits, int dtype, int64_t n, int64_t vocab,
  *               fp32 ones are laid out a piece at a time
  *   targets, ignore_index, temperature  as above; nothing of a row that does not count is read
  *   saved       [16 + 4 n] 4-byte elements (16-byte aligned): what the backward needs
- *   unit        nullable, [me_head_unit_size] fp32 (16-byte aligned): where the gradient of hidden
- *               alone is wanted, the forward leaves there what the backward only has to scale. A
+ *   unit        nullable, [me_head_unit_size] fp32 (16-byte aligned), ME_BF16 alone: where the
+ *               gradient of hidden alone is wanted, the forward leaves there what the backward only has to scale. A
  *               size of 0: the call is too small for that to pay (unit may still be given, n times
  *               dim rounded up to 4 values)
  *   workspace   me_head_workspace_size bytes for the same n, vocab, dim, dtype, weight and w_stride, with pass
  *               0 for a forward, 1 for me_head_backward (without unit, which needs none), 2 for a
  *               forward with unit; 16-byte aligned
- * bf16 products accumulate in fp32; fp32 ones are made of bf16 parts that add up to the operands, with
- * the accuracy of fp32 products.
+ * bf16 products accumulate in fp32; fp32 ones are made of bf16 or fp16 parts of the operands, with the
+ * accuracy of fp32 products.
  */
 int me_head_workspace_size(int64_t n, int64_t vocab, int64_t dim, int dtype, const void *weight,
                            int64_t w_stride, int pass, size_t *bytes);

@@ -160,9 +160,10 @@ __global__ __launch_bounds__(256) void layout_kernel(const Layout a) {
 }
 
 // fp32 rows in two fp16 parts over a power of two by row, which goes to `scale` (what the parts are multiplied by to
-// give the value). A wave per row. Of what is not finite, the first part alone.
-__global__ __launch_bounds__(256) void layout16_kernel(const Layout a, float *scale) {
-    if (a.gate != nullptr && *a.gate == 0) return;
+// give the value), and the largest of these, where wanted, to `largest`. A wave per row. Of what is not finite, the
+// first part alone.
+__global__ __launch_bounds__(256) void layout16_kernel(const Layout a, float *scale, uint32_t *largest) {
+    uint32_t widest = 0;
     const int lane = threadIdx.x & 63;
     const int64_t n = a.count ? min(a.n, static_cast<int64_t>(*a.count)) : a.n;
     constexpr int kKept = 4;  // pieces of 512 values that stay in registers; further ones are read again
@@ -194,7 +195,9 @@ __global__ __launch_bounds__(256) void layout16_kernel(const Layout a, float *sc
         // the largest below 2^15; the power and its inverse are normal fp32 numbers
         const int up = min(max(14 - (static_cast<int>(most >> 23) - 127), -112), 126);
         const float times = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
-        if (lane == 0) scale[r] = __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
+        const uint32_t down = static_cast<uint32_t>(127 - up) << 23;
+        widest = max(widest, down);
+        if (lane == 0) scale[r] = __uint_as_float(down);
         auto put = [&](const float (&v)[8], int64_t c) {
             if (c >= a.ld) return;
             halfx8 hi, lo;
@@ -217,6 +220,7 @@ __global__ __launch_bounds__(256) void layout16_kernel(const Layout a, float *sc
             put(x, c);
         }
     }
+    if (largest != nullptr && lane == 0) atomicMax(largest, widest);  // a maximum: the same in any order
 }
 
 // What rows and columns of a product of fp16 parts are multiplied by; null: nothing
@@ -254,6 +258,22 @@ __device__ __forceinline__ void stage4(float (&v)[4], uint8_t *stage, int col, i
         }
         *reinterpret_cast<uint2 *>(stage + (p * 32 + (lane & 31)) * kPitch + col * 2) = make_uint2(w[0], w[1]);
     }
+}
+
+// Likewise in two fp16 parts
+template <int SX>
+__device__ __forceinline__ void stage4_half(const float (&v)[4], uint8_t *stage, int col, int lane) {
+    constexpr int kPitch = 64 * SX + 16;
+    typedef _Float16 halfx4 __attribute__((ext_vector_type(4)));
+    halfx4 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        hi[e] = static_cast<_Float16>(v[e]);
+        const float rest = v[e] - static_cast<float>(hi[e]);
+        lo[e] = static_cast<_Float16>(__builtin_fabsf(rest) < __builtin_inff() ? rest : 0.f);
+    }
+    *reinterpret_cast<halfx4 *>(stage + (lane & 31) * kPitch + col * 2) = hi;
+    *reinterpret_cast<halfx4 *>(stage + (32 + (lane & 31)) * kPitch + col * 2) = lo;
 }
 
 // A staged block as 16-byte chunks of rows r0 .. of [rows][ld], from column c0 on
@@ -356,18 +376,16 @@ struct StatsEpilogue {
     }
 };
 
-// The exponentials of a tile's logits, 2^(z - ref) by row and zero at the target, bf16 or in three parts, as rows of a
-// piece, and their sums over a wave's columns
-template <int NPARTS>
+// The exponentials of a tile's logits, 2^(z - ref) by row and zero at the target, in bf16 as rows of a piece, and their
+// sums over a wave's columns
 struct ExpEpilogue {
     const int32_t *tgt;
-    Scales scales;
     const float *ref;        // by row, log2
     float *part, *sum;       // by (column part, row), as StatsEpilogue
     float *at_target;
     int64_t part_stride, row_stride;
     uint8_t *out;
-    int64_t ld, out_part;
+    int64_t ld;
     int64_t first, vocab;
     float k;
 
@@ -376,35 +394,33 @@ struct ExpEpilogue {
         const int64_t c0 = t.s0 + col0;
         const int there = static_cast<int>(max(min(vocab - c0, int64_t{32 * SX}), int64_t{0}));
         const int64_t part_at = (first + c0) / (32 * SX);
-        constexpr int kPitch = 64 * SX + 16, kPlaces = NPARTS == 1 ? 2 : 1;
+        constexpr int kPitch = 64 * SX + 16;
 #pragma unroll
         for (int y = 0; y < SY; ++y) {
-            uint8_t *stage = lds + ((threadIdx.x >> 6) * kPlaces + (y % kPlaces)) * (NPARTS * 32 * kPitch);
+            uint8_t *stage = lds + ((threadIdx.x >> 6) * 2 + (y & 1)) * (32 * kPitch);
             const int64_t row = t.r0 + row0 + 32 * y + (lane & 31);
             const bool ok = row < t.rows;
             const float shift = ok ? ref[row] : 0.f;
             const int64_t off = ok ? tgt[row] - (first + c0) : -1;
             const int mine = off >= 0 && off < there ? static_cast<int>(off) : -1;
             float s, total = 0.f;
-            const float kr = k * scales.of_row(row, ok);
-            // three parts: one way through it, or the code outgrows what the compiler unrolls; the K loop is three times as long
-            if (NPARTS > 1 || there < 32 * SX || __any(mine >= 0))
-                s = stage_rows<AGPR, true, SX, SY>(acc, y, row, kr, c0, shift, mine, there, total, stage, lane);
+            if (there < 32 * SX || __any(mine >= 0))
+                s = stage_rows<AGPR, true, SX, SY>(acc, y, row, shift, mine, there, total, stage, lane);
             else
-                s = stage_rows<AGPR, false, SX, SY>(acc, y, row, kr, c0, shift, mine, there, total, stage, lane);
+                s = stage_rows<AGPR, false, SX, SY>(acc, y, row, shift, mine, there, total, stage, lane);
             s += __shfl_xor(s, 32);
             total += __shfl_xor(total, 32);
             if (ok && lane < 32) {
                 part[part_at * part_stride + row * row_stride] = s;
-                if (sum != nullptr) sum[part_at * part_stride + row * row_stride] = total * kr;
+                if (sum != nullptr) sum[part_at * part_stride + row * row_stride] = total * k;
             }
-            store_rows<NPARTS, SX>(stage, out, ld, out_part, t.r0 + row0 + 32 * y, t.rows, c0, lane);
+            store_rows<1, SX>(stage, out, ld, 0, t.r0 + row0 + 32 * y, t.rows, c0, lane);
         }
     }
 
     template <bool AGPR, bool SOME, int SX, int SY>
-    __device__ __forceinline__ float stage_rows(const floatx16 (&acc)[SX][SY], int y, int64_t row, float kr, int64_t c0, float shift, int mine,
-                                                int there, float &total, uint8_t *stage, int lane) const {
+    __device__ __forceinline__ float stage_rows(const floatx16 (&acc)[SX][SY], int y, int64_t row, float shift, int mine, int there, float &total,
+                                                uint8_t *stage, int lane) const {
         const int half4 = 4 * (lane >> 5);
         float s = 0.f;
 #pragma unroll
@@ -412,14 +428,13 @@ struct ExpEpilogue {
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 float v[4];
-                const f32x4_v cs = scales.of_cols<(NPARTS > 1)>(c0 + 32 * x + 8 * q + half4);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float z = acc_read<AGPR>(acc[x][y], 4 * q + e) * cs[e];
-                    v[e] = __builtin_amdgcn_exp2f(fmaf(z, kr, -shift));
+                    const float z = acc_read<AGPR>(acc[x][y], 4 * q + e);
+                    v[e] = __builtin_amdgcn_exp2f(fmaf(z, k, -shift));
                     if constexpr (SOME) {
                         const int col = 32 * x + 8 * q + half4 + e;
-                        if (col == mine) at_target[row] = z * kr;
+                        if (col == mine) at_target[row] = z * k;
                         if (col == mine || col >= there) v[e] = 0.f;
                         total += col < there ? z : 0.f;
                     } else {
@@ -427,7 +442,7 @@ struct ExpEpilogue {
                     }
                     s += v[e];
                 }
-                stage4<NPARTS, SX>(v, stage, 32 * x + 8 * q + half4, lane);
+                stage4<1, SX>(v, stage, 32 * x + 8 * q + half4, lane);
             }
         return s;
     }
@@ -437,45 +452,68 @@ struct RowGrad {
     float lse2, ca, cb, gt;
 };
 
-// The logits' gradient of a tile, bf16 or in three parts, as rows of a piece
-template <int NPARTS>
+// Power of two that puts a row's gradient times the columns' scales into fp16's range: the largest below 2^15. row: a
+// bound of the row's values, largest: of the scales (a power of two)
+__device__ __forceinline__ int row_power(float row, uint32_t largest) {
+    const int e = static_cast<int>(__float_as_uint(row) >> 23) - 127 + static_cast<int>(largest >> 23) - 127;
+    return min(max(14 - e, -126), 126);
+}
+
+__device__ __forceinline__ float power_of(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
+
+// The logits' gradient of a tile as rows of a piece: bf16 for bf16 operands; for fp32 ones three bf16 parts where the
+// head's gradient is wanted, and two fp16 parts, times the columns' scales and the row's power, where the hidden
+// states' is
+template <bool F32>
 struct GradEpilogue {
     const int32_t *tgt;
     Scales scales;
     const RowGrad *grad;
-    uint8_t *out;          // [rows][ld] of each part
-    int64_t ld, part;      // ld: columns of the piece, a multiple of 64; part: bytes
-    int64_t first, vocab;  // first column of the piece, columns that there are
+    const float *bound;       // of each row's values (F32)
+    const uint32_t *largest;  // of the columns' scales (F32)
+    uint8_t *out, *half;      // [rows][ld] of each part; null: not wanted
+    int64_t ld, part;         // ld: columns of the piece, a multiple of 64; part: bytes
+    int64_t first, vocab;     // first column of the piece, columns that there are
     float k;
 
     template <bool AGPR, int SX, int SY>
     __device__ __forceinline__ void run(const floatx16 (&acc)[SX][SY], const Tile &t, int row0, int col0, uint8_t *lds, int lane) const {
+        if constexpr (F32) {
+            if (half != nullptr) rows_of<AGPR, true, SX, SY>(acc, t, row0, col0, lds, lane);
+            if (out == nullptr) return;
+        }
+        rows_of<AGPR, false, SX, SY>(acc, t, row0, col0, lds, lane);
+    }
+
+    template <bool AGPR, bool HALF, int SX, int SY>
+    __device__ __forceinline__ void rows_of(const floatx16 (&acc)[SX][SY], const Tile &t, int row0, int col0, uint8_t *lds, int lane) const {
         const int64_t c0 = t.s0 + col0;
         const int there = static_cast<int>(max(min(vocab - c0, int64_t{32 * SX}), int64_t{0}));
-        constexpr int kPitch = 64 * SX + 16;  // staged row (bytes)
+        constexpr int kParts = !F32 ? 1 : HALF ? 2 : 3;
+        // 32 rows at a time through LDS, where a wave has two places in turn (with parts one: a wave's LDS
+        // accesses keep their order)
+        constexpr int kPitch = 64 * SX + 16, kPlaces = F32 ? 1 : 2;
+        static_assert(4 * kPlaces * kParts * 32 * kPitch <= (SX == 4 ? kRingBytes : 3 * kUnit), "the stage fits the ring");
 #pragma unroll
         for (int y = 0; y < SY; ++y) {
-            // 32 rows at a time through LDS, where a wave has two places in turn (with three parts one: a wave's
-            // LDS accesses keep their order)
-            constexpr int kPlaces = NPARTS == 1 ? 2 : 1;
-            static_assert(4 * kPlaces * NPARTS * 32 * kPitch <= (SX == 4 ? kRingBytes : 3 * kUnit), "the stage fits the ring");
-            uint8_t *stage = lds + ((threadIdx.x >> 6) * kPlaces + (y % kPlaces)) * (NPARTS * 32 * kPitch);
+            uint8_t *stage = lds + ((threadIdx.x >> 6) * kPlaces + (y % kPlaces)) * (kParts * 32 * kPitch);
             const int64_t row = t.r0 + row0 + 32 * y + (lane & 31);
             const bool ok = row < t.rows;
-            const RowGrad g = ok ? grad[row] : RowGrad{0.f, 0.f, 0.f, 0.f};
+            RowGrad g = ok ? grad[row] : RowGrad{0.f, 0.f, 0.f, 0.f};
             const int64_t off = ok ? tgt[row] - (first + c0) : -1;
             const int mine = off >= 0 && off < there ? static_cast<int>(off) : -1;
             const float kr = k * scales.of_row(row, ok);
-            if (NPARTS > 1 || there < 32 * SX || __any(mine >= 0))
-                stage_rows<AGPR, true, SX, SY>(acc, y, g, kr, c0, mine, there, stage, lane);
+            const float up = HALF && ok ? power_of(row_power(bound[row], *largest)) : 1.f;
+            if (F32 || there < 32 * SX || __any(mine >= 0))
+                stage_rows<AGPR, HALF, true, SX, SY>(acc, y, g, kr, up, c0, mine, there, stage, lane);
             else
-                stage_rows<AGPR, false, SX, SY>(acc, y, g, kr, c0, mine, there, stage, lane);
-            store_rows<NPARTS, SX>(stage, out, ld, part, t.r0 + row0 + 32 * y, t.rows, c0, lane);
+                stage_rows<AGPR, HALF, false, SX, SY>(acc, y, g, kr, up, c0, mine, there, stage, lane);
+            store_rows<kParts, SX>(stage, HALF ? half : out, ld, part, t.r0 + row0 + 32 * y, t.rows, c0, lane);
         }
     }
 
-    template <bool AGPR, bool SOME, int SX, int SY>
-    __device__ __forceinline__ void stage_rows(const floatx16 (&acc)[SX][SY], int y, const RowGrad &g, float kr, int64_t c0, int mine,
+    template <bool AGPR, bool HALF, bool SOME, int SX, int SY>
+    __device__ __forceinline__ void stage_rows(const floatx16 (&acc)[SX][SY], int y, const RowGrad &g, float kr, float up, int64_t c0, int mine,
                                                int there, uint8_t *stage, int lane) const {
         const int half4 = 4 * (lane >> 5);
 #pragma unroll
@@ -483,7 +521,7 @@ struct GradEpilogue {
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 float v[4];
-                const f32x4_v cs = scales.of_cols<(NPARTS > 1)>(c0 + 32 * x + 8 * q + half4);
+                const f32x4_v cs = scales.of_cols<F32>(c0 + 32 * x + 8 * q + half4);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     v[e] = fmaf(__builtin_amdgcn_exp2f(fmaf(acc_read<AGPR>(acc[x][y], 4 * q + e) * cs[e], kr, -g.lse2)), g.ca, -g.cb);
@@ -492,8 +530,12 @@ struct GradEpilogue {
                         if (col == mine) v[e] = g.gt;
                         if (col >= there) v[e] = 0.f;  // past the vocabulary: nothing for the products with W and h
                     }
+                    if constexpr (HALF) v[e] *= up * (!SOME || 32 * x + 8 * q + half4 + e < there ? cs[e] : 0.f);
                 }
-                stage4<NPARTS, SX>(v, stage, 32 * x + 8 * q + half4, lane);
+                if constexpr (HALF)
+                    stage4_half<SX>(v, stage, 32 * x + 8 * q + half4, lane);
+                else
+                    stage4<F32 ? 3 : 1, SX>(v, stage, 32 * x + 8 * q + half4, lane);
             }
     }
 };
@@ -503,6 +545,8 @@ struct AccumulateEpilogue {
     float *out;
     int64_t ld, split_stride;  // ld: a multiple of 4
     int add;
+    const float *bound;        // of fp16 parts: what the rows' powers come from, else null
+    const uint32_t *largest;
 
     template <bool AGPR, int SX, int SY>
     __device__ __forceinline__ void run(const floatx16 (&acc)[SX][SY], const Tile &t, int row0, int col0, uint8_t *, int lane) const {
@@ -512,6 +556,7 @@ struct AccumulateEpilogue {
         for (int y = 0; y < SY; ++y) {
             const int64_t row = t.r0 + row0 + 32 * y + (lane & 31);
             if (row >= t.rows) continue;
+            const float down = bound != nullptr ? power_of(-row_power(bound[row], *largest)) : 1.f;
 #pragma unroll
             for (int x = 0; x < SX; ++x) {
                 const int64_t col = t.s0 + col0 + 32 * x + half4;
@@ -525,7 +570,7 @@ struct AccumulateEpilogue {
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) v[g][e] += acc_read<AGPR>(acc[x][y], 4 * g + e);
+                    for (int e = 0; e < 4; ++e) v[g][e] = fmaf(acc_read<AGPR>(acc[x][y], 4 * g + e), down, v[g][e]);
                     if (col + 8 * g < ld) at[2 * g] = v[g];
                 }
             }
@@ -895,9 +940,14 @@ struct CoefArgs {
     float smoothing, z_loss;
     double vocab;
     RowGrad *grad;
+    float *bound;           // of each row's values, or null
+    uint32_t *largest;      // set to 0, `pieces` of them
+    int pieces;
 };
 
 __global__ __launch_bounds__(256) void coef_kernel(const CoefArgs a) {
+    if (blockIdx.x == 0)
+        for (int i = static_cast<int>(threadIdx.x); i < a.pieces; i += 256) a.largest[i] = 0;
     const int64_t r = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
     const int64_t count = *a.s.count;
     if (r >= a.n || r >= count) return;
@@ -915,6 +965,8 @@ __global__ __launch_bounds__(256) void coef_kernel(const CoefArgs a) {
         g.gt = static_cast<float>(c * (more - (1.0 + more) * o + e - e / a.vocab));
     }
     a.grad[r] = g;
+    // a token's probability is at most that of all but the target
+    if (a.bound) a.bound[r] = fmaxf(fabsf(g.ca) * (1.0001f * o) + fabsf(g.cb), fabsf(g.gt));
 }
 
 // Four values of a row of the hidden states' gradient
@@ -963,20 +1015,15 @@ __global__ __launch_bounds__(256) void hidden_kernel(const Sums sums, const int3
 // upstream 1 before the factors that rows share; the target's term in fp32. The backward only scales D. ref is no
 // maximum: a row whose sum passes 2^100 (its loss is over some 69) or is not finite is made again by the plain way
 // (statistics, then gradient), in launches that find no row otherwise.
-template <bool F32>
-__global__ __launch_bounds__(256) void ref_kernel(const Layout h, const void *weight, int64_t w_stride, const int32_t *tgt, float k, float *ref) {
+__global__ __launch_bounds__(256) void ref_kernel(const Layout h, const uint16_t *weight, int64_t w_stride, const int32_t *tgt, float k, float *ref) {
     const int64_t r = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
     if (r >= *h.count) return;
     const int lane = threadIdx.x & 63;
     const int64_t from = h.rows[r], at = from / h.per_batch * h.batch_stride + from % h.per_batch * h.row_stride;
     const int64_t w = tgt[r] * w_stride;
     float sum = 0.f;
-    for (int64_t c = lane; c < h.dim; c += 64) {
-        if constexpr (F32)
-            sum += static_cast<const float *>(h.src)[at + c] * static_cast<const float *>(weight)[w + c];
-        else
-            sum += bf16_bits_to_float(static_cast<const uint16_t *>(h.src)[at + c]) * bf16_bits_to_float(static_cast<const uint16_t *>(weight)[w + c]);
-    }
+    for (int64_t c = lane; c < h.dim; c += 64)
+        sum += bf16_bits_to_float(static_cast<const uint16_t *>(h.src)[at + c]) * bf16_bits_to_float(weight[w + c]);
 #pragma unroll
     for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
     sum *= k;
@@ -989,8 +1036,6 @@ struct RedoArgs {
     const float *ref;
     const int32_t *tgt;
     int32_t *count, *rows, *tgt2;
-    const float *scale;  // of the rows' parts, or null
-    float *scale2;
 };
 
 __global__ __launch_bounds__(kIndexThreads) void redo_kernel(const RedoArgs a) {
@@ -1015,7 +1060,6 @@ __global__ __launch_bounds__(kIndexThreads) void redo_kernel(const RedoArgs a) {
             const int r = before + __popcll(mask & ((uint64_t{1} << lane) - 1));
             a.rows[r] = i;
             a.tgt2[r] = a.tgt[i];
-            if (a.scale) a.scale2[r] = a.scale[i];
         }
         at += all;
         __syncthreads();
@@ -1034,15 +1078,14 @@ __global__ __launch_bounds__(256) void redo_coef_kernel(Saved s, const int32_t *
 // Sums of the head's columns, which a smoothed target's gradient takes in: chunks of rows, then over the chunks
 constexpr int kColumnRows = 512;
 
-template <bool F32>
-__global__ __launch_bounds__(256) void column_kernel(const void *weight, int64_t w_stride, int64_t vocab, int64_t dim, float *part) {
+__global__ __launch_bounds__(256) void column_kernel(const uint16_t *weight, int64_t w_stride, int64_t vocab, int64_t dim, float *part) {
     const int64_t c = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
     if (c >= dim) return;
     const int64_t v0 = static_cast<int64_t>(blockIdx.y) * kColumnRows, v1 = min(vocab, v0 + kColumnRows);
     float sum = 0.f;
 #pragma unroll 8
     for (int64_t v = v0; v < v1; ++v)
-        sum += F32 ? static_cast<const float *>(weight)[v * w_stride + c] : bf16_bits_to_float(static_cast<const uint16_t *>(weight)[v * w_stride + c]);
+        sum += bf16_bits_to_float(weight[v * w_stride + c]);
     part[blockIdx.y * dim + c] = sum;
 }
 
@@ -1060,7 +1103,7 @@ struct UnitArgs {
     const int32_t *count, *which;  // as FinishArgs
     const int32_t *tgt;            // by row of sums
     const float *ref;              // null: sums are of a q
-    const void *weight;
+    const uint16_t *weight;
     int64_t w_stride, dim, n;
     float z_loss, smoothing;
     const float *columns;          // sums of the head's columns, null without smoothing
@@ -1068,7 +1111,6 @@ struct UnitArgs {
     float *unit;                   // [counted rows][dim rounded up to 4]
 };
 
-template <bool F32>
 __global__ __launch_bounds__(256) void unit_kernel(const UnitArgs a) {
     const int64_t units = ceil_div(a.dim, 4);
     const int64_t count = a.count ? *a.count : *a.s.count;
@@ -1087,8 +1129,7 @@ __global__ __launch_bounds__(256) void unit_kernel(const UnitArgs a) {
             float w = 0.f, all = 0.f;
             if (c + e < a.dim) {
                 if (a.columns) all = each * a.columns[c + e];
-                const int64_t i = a.tgt[r] * a.w_stride + c + e;
-                w = F32 ? static_cast<const float *>(a.weight)[i] : bf16_bits_to_float(static_cast<const uint16_t *>(a.weight)[i]);
+                w = bf16_bits_to_float(a.weight[a.tgt[r] * a.w_stride + c + e]);
             }
             v[e] = fmaf(v[e], scale, fmaf(own, w, -all));
         }
@@ -1107,7 +1148,6 @@ struct ScaleArgs {
     void *out;
 };
 
-template <bool F32>
 __global__ __launch_bounds__(256) void scale_kernel(const ScaleArgs a) {
     const int64_t units = ceil_div(a.dim, 4);
     const double all = a.per_row ? -a.scale : static_cast<double>(*a.upstream) * a.scale / (a.mean ? max(*a.count, 1) : 1);
@@ -1119,7 +1159,7 @@ __global__ __launch_bounds__(256) void scale_kernel(const ScaleArgs a) {
             const float f = static_cast<float>(a.per_row ? all * static_cast<double>(a.upstream[i]) : all);
             v = *as_global(reinterpret_cast<const f32x4_v *>(a.unit + r * units * 4 + c)) * f;
         }
-        store4<F32>(a.out, i * a.dim, c, a.dim, v);
+        store4<false>(a.out, i * a.dim, c, a.dim, v);
     }
 }
 
@@ -1129,13 +1169,14 @@ enum Pass { kStats, kBackward, kLeavesUnit };  // the forward alone, the backwar
 struct Plan {
     int64_t n, rows, vocab, dim, ld;  // rows: n rounded up, at least 64; ld: dim rounded up to whole slabs
     bool f32, few, copy_w;            // copy_w: the head is laid out piece by piece
-    int np, nz;                       // parts of an operand: of a product with the gradient, of the logits
+    int np, nz;                       // parts of an operand: of the head's gradient; of the logits and the hidden states' gradient
     int64_t piece;                    // columns of the vocabulary at a time
     int splits;                       // of the product with W, at most
     int split_cost;
-    int64_t h, tgt, part, sum, at_target, row_loss, w, g, grad, acc;  // workspace offsets
+    int64_t h, tgt, part, sum, at_target, row_loss, g, grad, acc;  // workspace offsets
     int64_t ref, redo, h2, tgt2, columns, column_part;
-    int64_t z, wz, row_scale, col_scale, row_scale2;  // fp32: hidden states and head in fp16 parts, and their scales
+    int64_t z, wz, row_scale, col_scale;  // operands of the logits; fp32: fp16 parts, and their scales
+    int64_t half, bound, largest;         // fp32: the gradient in fp16 parts, its rows' bounds, the scales' largest by piece
     int64_t bytes;
 };
 
@@ -1151,8 +1192,8 @@ Plan plan_of(int64_t n, int64_t vocab, int64_t dim, int dtype, const void *weigh
     p.copy_w = p.f32 || w_stride % 8 != 0 || reinterpret_cast<uintptr_t>(weight) % 16 != 0;
     const int64_t rows = p.rows = round_up(std::max<int64_t>(n, 1), 64);
     int64_t piece = round_up(vocab, kTile);
-    if (p.copy_w) piece = std::min(piece, std::max<int64_t>(kPieceBytes / (p.ld * 2 * p.np) / 2048 * 2048, 2048));
-    if (pass != kStats) piece = std::min(piece, std::max<int64_t>(kPieceBytes / (rows * 2 * p.np) / 2048 * 2048, 2048));
+    if (p.copy_w) piece = std::min(piece, std::max<int64_t>(kPieceBytes / (p.ld * 2 * p.nz) / 2048 * 2048, 2048));
+    if (pass != kStats) piece = std::min(piece, std::max<int64_t>(kPieceBytes / (rows * (p.f32 ? 10 : 2)) / 2048 * 2048, 2048));
     // a launch holds fewer than 2^32 threads
     p.piece = std::min(piece, std::max<int64_t>((int64_t{1} << 23) / ceil_div(rows, p.few ? 64 : kTile) * kTile / 2048 * 2048, 2048));
     int64_t at = 0;
@@ -1166,12 +1207,15 @@ Plan plan_of(int64_t n, int64_t vocab, int64_t dim, int dtype, const void *weigh
     p.z = take(rows * p.ld * 2 * p.nz);
     p.h = p.z;
     if (p.copy_w) p.wz = take(p.piece * p.ld * 2 * p.nz);
-    p.w = p.wz;
     if (p.f32) {
         p.row_scale = take(n * 4);
         p.col_scale = take((p.piece + kTile) * 4);
-        if (pass == kBackward) p.h = take(rows * p.ld * 2 * p.np);
-        if (pass != kStats) p.w = take(p.piece * p.ld * 2 * p.np);
+        if (pass == kBackward) {
+            p.h = take(rows * p.ld * 2 * p.np);
+            p.half = take(rows * p.piece * 2 * p.nz);
+            p.bound = take(n * 4);
+            p.largest = take(ceil_div(vocab, p.piece) * 4);
+        }
     }
     if (pass != kBackward) {
         const int64_t parts = std::max<int64_t>(ceil_div(vocab, p.few ? 64 : 128) + 4, n <= kVectorRows ? kVectorGroups : 0);
@@ -1186,15 +1230,14 @@ Plan plan_of(int64_t n, int64_t vocab, int64_t dim, int dtype, const void *weigh
         const int64_t tiles = ceil_div(rows, p.few ? 64 : kTile) * ceil_div(dim, kTile);
         p.splits = static_cast<int>(std::max<int64_t>(std::min<int64_t>({std::max<int64_t>(256 / tiles, kSplits), kMostSplits, p.piece / kSlabK / 8}), 1));
         // reading and writing the sums at 4.8 TB/s against a piece's products at 1.25 PFLOP/s
-        p.split_cost = static_cast<int>(4096 * (8.0 / 4.8e12) / (2.0 * static_cast<double>(p.piece) * (p.f32 ? 6 : 1) / 1.25e15)) + 1;
+        p.split_cost = static_cast<int>(4096 * (8.0 / 4.8e12) / (2.0 * static_cast<double>(p.piece) * (p.f32 ? 3 : 1) / 1.25e15)) + 1;
         p.acc = take(p.splits * rows * p.ld * 4);
     }
     if (pass == kLeavesUnit) {
         p.ref = take(n * 4);
         p.redo = take((kHeader + n) * 4);
-        p.h2 = take(rows * p.ld * 2 * p.nz);
+        p.h2 = take(rows * p.ld * 2);
         p.tgt2 = take(n * 4);
-        if (p.f32) p.row_scale2 = take(n * 4);
         p.columns = take(dim * 4);
         p.column_part = take(ceil_div(vocab, kColumnRows) * dim * 4);
     }
@@ -1202,12 +1245,12 @@ Plan plan_of(int64_t n, int64_t vocab, int64_t dim, int dtype, const void *weigh
     return p;
 }
 
-// Whether a forward for the hidden states' gradient alone leaves D. It saves the backward one of three products (few
-// rows: one of three reads of the head) and costs some ten launches more.
+// Whether a forward for the hidden states' gradient alone leaves D: bf16, where it saves the backward one of three
+// products (few rows: one of three reads of the head) and that is worth some ten launches more. (fp32: the
+// exponentials would need six products with the head, where the gradient, whose size is known, needs three.)
 bool leaves_unit(int64_t n, int64_t vocab, int64_t dim, int dtype) {
-    const double product = 2.0 * static_cast<double>(n) * vocab * dim * (dtype == ME_F32 ? 6 : 1) / 1.2e15;
-    const double read = static_cast<double>(vocab) * dim * (dtype == ME_F32 ? 6 : 2) / 5e12;
-    return std::max(product, read) > 50e-6;
+    const double product = 2.0 * static_cast<double>(n) * vocab * dim / 1.2e15, read = 2.0 * static_cast<double>(vocab) * dim / 5e12;
+    return dtype == ME_BF16 && std::max(product, read) > 50e-6;
 }
 
 struct Call {
@@ -1235,9 +1278,9 @@ Layout hidden_layout(const Plan &p, const Call &c, int64_t to) {
     return {c.hidden, c.per_batch, c.batch_stride, c.row_stride, c.s.rows, c.s.count, p.n, p.dim, p.ld, h_part(p), c.ws + to};
 }
 
-void lay_out16(const Layout &l, float *scale, hipStream_t s) {
-    const unsigned blocks = static_cast<unsigned>(std::min<int64_t>(std::max<int64_t>(ceil_div(l.n, 4), 1), 16384));
-    hipLaunchKernelGGL(layout16_kernel, dim3(blocks), dim3(256), 0, s, l, scale);
+void lay_out16(const Layout &l, float *scale, uint32_t *largest, hipStream_t s) {
+    const unsigned blocks = static_cast<unsigned>(std::min<int64_t>(std::max<int64_t>(ceil_div(l.n, 4), 1), 2048));
+    hipLaunchKernelGGL(layout16_kernel, dim3(blocks), dim3(256), 0, s, l, scale, largest);
 }
 
 // Rows of a product: the hidden states laid out for the logits, with how many there are, their targets and, of
@@ -1251,32 +1294,29 @@ struct Rows {
 Rows lay_out_rows(const Plan &p, const Call &c) {
     float *scale = p.f32 ? reinterpret_cast<float *>(c.ws + p.row_scale) : nullptr;
     if (p.f32)
-        lay_out16(hidden_layout(p, c, p.z), scale, c.stream);
+        lay_out16(hidden_layout(p, c, p.z), scale, nullptr, c.stream);
     else
         lay_out(false, hidden_layout(p, c, p.z), c.stream);
     return {c.ws + p.z, c.s.count, reinterpret_cast<const int32_t *>(c.ws + p.tgt), scale};
 }
 
-// The head from row v0 on, `width` rows of it, for the logits and for the product with their gradient
+// The head from row v0 on, `width` rows of it
 struct Head {
-    Operand logits, product;
-    const float *scale;  // of the logits' columns
+    Operand w;
+    const float *scale;  // of fp16 parts, by row
 };
 
-Head head_of(const Plan &p, const Call &c, int64_t v0, int64_t width, bool for_product, const int32_t *gate = nullptr) {
+Head head_of(const Plan &p, const Call &c, int64_t v0, int64_t width, uint32_t *largest = nullptr, const int32_t *gate = nullptr) {
     const uint8_t *from = static_cast<const uint8_t *>(c.weight) + v0 * c.w_stride * (p.f32 ? 4 : 2);
-    if (!p.copy_w) return {{from, c.w_stride, 0}, {from, c.w_stride, 0}, nullptr};
+    if (!p.copy_w) return {{from, c.w_stride, 0}, nullptr};
     const int64_t part = p.piece * p.ld * 2;
-    Layout l{from, width, 0, c.w_stride, nullptr, nullptr, width, p.dim, p.ld, part, c.ws + p.wz, gate};
+    const Layout l{from, width, 0, c.w_stride, nullptr, nullptr, width, p.dim, p.ld, part, c.ws + p.wz, gate};
     float *scale = p.f32 ? reinterpret_cast<float *>(c.ws + p.col_scale) : nullptr;
-    if (p.f32) {
-        lay_out16(l, scale, c.stream);
-        l.dst = c.ws + p.w;
-        if (for_product) lay_out(true, l, c.stream);
-    } else {
+    if (p.f32)
+        lay_out16(l, scale, largest, c.stream);
+    else
         lay_out(false, l, c.stream);
-    }
-    return {{c.ws + p.wz, p.ld, part}, {c.ws + p.w, p.ld, part}, scale};
+    return {{c.ws + p.wz, p.ld, part}, scale};
 }
 
 template <bool A_KC, bool B_KC, int SEGS, class Epilogue>
@@ -1295,7 +1335,7 @@ void multiply_few(const Gemm &g, const Epilogue &e, hipStream_t s) {
 // logits of a piece: rows x head rows
 template <int SEGS, class Epilogue>
 void logits_of(const Plan &p, const Call &c, const Rows &rows, const Head &w, int64_t width, const Epilogue &e) {
-    const Gemm g{{rows.h, p.ld, h_part(p)}, w.logits, p.n, width, p.dim, rows.count, 0, 8, 1, 0};
+    const Gemm g{{rows.h, p.ld, h_part(p)}, w.w, p.n, width, p.dim, rows.count, 0, 8, 1, 0};
     if (p.few)
         multiply_few<true, SEGS>(g, e, c.stream);
     else
@@ -1303,26 +1343,29 @@ void logits_of(const Plan &p, const Call &c, const Rows &rows, const Head &w, in
 }
 
 // product of a piece of the logits' gradient (or exponentials) with the head, onto the sums
-void times_head(const Plan &p, const Call &c, const Rows &rows, const Head &w, int64_t v0, int64_t width) {
-    const Gemm g{{c.ws + p.g, p.piece, p.rows * p.piece * 2}, w.product, p.n, p.dim, width, rows.count, 0, 8, p.splits, p.split_cost};
-    const AccumulateEpilogue e{reinterpret_cast<float *>(c.ws + p.acc), p.ld, p.rows * p.ld, v0 > 0};
+void times_head(const Plan &p, const Call &c, const Rows &rows, const Head &w, int64_t v0, int64_t width, const uint32_t *largest = nullptr) {
+    const Operand dz{c.ws + (p.f32 ? p.half : p.g), p.piece, p.rows * p.piece * 2};
+    const Gemm g{dz, w.w, p.n, p.dim, width, rows.count, 0, 8, p.splits, p.split_cost};
+    const AccumulateEpilogue e{reinterpret_cast<float *>(c.ws + p.acc), p.ld, p.rows * p.ld, v0 > 0,
+                               p.f32 ? reinterpret_cast<const float *>(c.ws + p.bound) : nullptr, largest};
     if (p.few)
-        p.f32 ? multiply_few<false, 6>(g, e, c.stream) : multiply_few<false, 1>(g, e, c.stream);
+        p.f32 ? multiply_few<false, 3>(g, e, c.stream) : multiply_few<false, 1>(g, e, c.stream);
     else
-        p.f32 ? multiply_large<true, false, 6>(g, e, c.stream) : multiply_large<true, false, 1>(g, e, c.stream);
+        p.f32 ? multiply_large<true, false, 3>(g, e, c.stream) : multiply_large<true, false, 1>(g, e, c.stream);
 }
 
 Sums sums_of(const Plan &p, const Call &c) {
     return {reinterpret_cast<float *>(c.ws + p.acc), p.ld, p.rows * p.ld, p.few ? 64 : kTile, static_cast<int>(ceil_div(p.dim, kTile)), p.splits, p.split_cost};
 }
 
-void gradient_of(const Plan &p, const Call &c, const Rows &rows, const Head &w, int64_t v0, int64_t width, const RowGrad *grad, float k) {
-    const int64_t part = p.rows * p.piece * 2;
-    const Scales scales{rows.scale, w.scale};
-    if (p.f32)
-        logits_of<3>(p, c, rows, w, width, GradEpilogue<3>{rows.tgt, scales, grad, c.ws + p.g, p.piece, part, v0, width, k});
-    else
-        logits_of<1>(p, c, rows, w, width, GradEpilogue<1>{rows.tgt, scales, grad, c.ws + p.g, p.piece, part, v0, width, k});
+// gradient of the logits of a piece, for the products that follow
+template <bool F32>
+void gradient_of(const Plan &p, const Call &c, const Rows &rows, const Head &w, int64_t v0, int64_t width, const RowGrad *grad, float k,
+                 const uint32_t *largest, bool for_hidden, bool for_weight) {
+    const GradEpilogue<F32> e{rows.tgt, {rows.scale, w.scale}, grad, F32 ? reinterpret_cast<const float *>(c.ws + p.bound) : nullptr, largest,
+                              !F32 || for_weight ? c.ws + p.g : nullptr, F32 && for_hidden ? c.ws + p.half : nullptr, p.piece,
+                              p.rows * p.piece * 2, v0, width, k};
+    logits_of<F32 ? 3 : 1>(p, c, rows, w, width, e);
 }
 
 void finish(const Plan &p, const FinishArgs &f, hipStream_t s) {
@@ -1346,16 +1389,12 @@ void unit_of(const Plan &p, const Call &c, const Loss &l, const Rows &rows, cons
     UnitArgs u{};
     u.sums = sums_of(p, c);
     u.s = c.s, u.count = rows.count, u.which = which, u.tgt = rows.tgt, u.ref = ref;
-    u.weight = c.weight, u.w_stride = c.w_stride, u.dim = p.dim, u.n = p.n;
+    u.weight = static_cast<const uint16_t *>(c.weight), u.w_stride = c.w_stride, u.dim = p.dim, u.n = p.n;
     u.z_loss = static_cast<float>(l.z_loss), u.smoothing = static_cast<float>(l.smoothing);
     u.columns = l.smoothing != 0.0 ? reinterpret_cast<const float *>(c.ws + p.columns) : nullptr;
     u.vocab = static_cast<double>(p.vocab);
     u.unit = l.unit;
-    const unsigned blocks = blocks_for(p.n * ceil_div(p.dim, 4));
-    if (p.f32)
-        hipLaunchKernelGGL(unit_kernel<true>, dim3(blocks), dim3(256), 0, c.stream, u);
-    else
-        hipLaunchKernelGGL(unit_kernel<false>, dim3(blocks), dim3(256), 0, c.stream, u);
+    hipLaunchKernelGGL(unit_kernel, dim3(blocks_for(p.n * ceil_div(p.dim, 4))), dim3(256), 0, c.stream, u);
 }
 
 // Statistics of the rows' logits, piece by piece
@@ -1364,7 +1403,7 @@ void stats_of(const Plan &p, const Call &c, const Rows &rows, StatsEpilogue<F32>
     e.tgt = rows.tgt;
     for (int64_t v0 = 0; v0 < p.vocab; v0 += p.piece) {
         const int64_t width = std::min(p.piece, p.vocab - v0);
-        const Head w = head_of(p, c, v0, width, false, gate);
+        const Head w = head_of(p, c, v0, width, nullptr, gate);
         e.first = v0, e.vocab = width, e.scales = {rows.scale, w.scale};
         logits_of<F32 ? 3 : 1>(p, c, rows, w, width, e);
     }
@@ -1391,27 +1430,26 @@ void forward_rows(const Plan &p, const Call &c, const Loss &l) {
     f.n = p.n, f.vocab = p.vocab, f.s = c.s, f.logps = l.logps;
     f.row_loss = l.loss ? reinterpret_cast<float *>(c.ws + p.row_loss) : nullptr;
     f.smoothing = static_cast<float>(l.smoothing), f.z_loss = static_cast<float>(l.z_loss);
-    if (!l.unit) {
+    if (F32 || !l.unit) {
         stats_of<F32>(p, c, rows, e);
         finish(p, f, s);
         return;
     }
+    const uint16_t *weight = static_cast<const uint16_t *>(c.weight);
     float *ref = reinterpret_cast<float *>(c.ws + p.ref);
-    hipLaunchKernelGGL(ref_kernel<F32>, dim3(static_cast<unsigned>(ceil_div(p.n, 4))), dim3(256), 0, s, hidden_layout(p, c, p.z), c.weight, c.w_stride,
+    hipLaunchKernelGGL(ref_kernel, dim3(static_cast<unsigned>(ceil_div(p.n, 4))), dim3(256), 0, s, hidden_layout(p, c, p.z), weight, c.w_stride,
                        rows.tgt, k, ref);
     if (l.smoothing != 0.0) {
         const dim3 grid(static_cast<unsigned>(ceil_div(p.dim, 256)), static_cast<unsigned>(ceil_div(p.vocab, kColumnRows)));
         float *part = reinterpret_cast<float *>(c.ws + p.column_part);
-        hipLaunchKernelGGL(column_kernel<F32>, grid, dim3(256), 0, s, c.weight, c.w_stride, p.vocab, p.dim, part);
+        hipLaunchKernelGGL(column_kernel, grid, dim3(256), 0, s, weight, c.w_stride, p.vocab, p.dim, part);
         hipLaunchKernelGGL(column_total_kernel, dim3(grid.x), dim3(256), 0, s, part, static_cast<int>(grid.y), p.dim, reinterpret_cast<float *>(c.ws + p.columns));
     }
     float *exps = reinterpret_cast<float *>(c.ws + p.part);
     for (int64_t v0 = 0; v0 < p.vocab; v0 += p.piece) {
         const int64_t width = std::min(p.piece, p.vocab - v0);
-        const Head w = head_of(p, c, v0, width, true);
-        const ExpEpilogue<F32 ? 3 : 1> exp{rows.tgt, {rows.scale, w.scale}, ref, exps, e.sum, at_target, e.part_stride, e.row_stride,
-                                           c.ws + p.g, p.piece, p.rows * p.piece * 2, v0, width, k};
-        logits_of<F32 ? 3 : 1>(p, c, rows, w, width, exp);
+        const Head w = head_of(p, c, v0, width);
+        logits_of<1>(p, c, rows, w, width, ExpEpilogue{rows.tgt, ref, exps, e.sum, at_target, e.part_stride, e.row_stride, c.ws + p.g, p.piece, v0, width, k});
         times_head(p, c, rows, w, v0, width);
     }
     f.exps = exps, f.ref = ref;
@@ -1421,20 +1459,18 @@ void forward_rows(const Plan &p, const Call &c, const Loss &l) {
     // rows that ref was too far from
     int32_t *redo = reinterpret_cast<int32_t *>(c.ws + p.redo);
     int32_t *tgt2 = reinterpret_cast<int32_t *>(c.ws + p.tgt2);
-    float *scale2 = F32 ? reinterpret_cast<float *>(c.ws + p.row_scale2) : nullptr;
     RowGrad *grad = reinterpret_cast<RowGrad *>(c.ws + p.grad);
-    const Rows again{c.ws + p.h2, redo, tgt2, scale2};
-    hipLaunchKernelGGL(redo_kernel, dim3(1), dim3(kIndexThreads), 0, s, RedoArgs{c.s, ref, rows.tgt, redo, redo + kHeader, tgt2, rows.scale, scale2});
-    for (int part = 0; part < p.nz; ++part)
-        lay_out(false, Layout{rows.h + part * h_part(p), p.n, 0, p.ld, redo + kHeader, redo, p.n, p.ld, p.ld, 0, again.h + part * h_part(p)}, s);
+    const Rows again{c.ws + p.h2, redo, tgt2, nullptr};
+    hipLaunchKernelGGL(redo_kernel, dim3(1), dim3(kIndexThreads), 0, s, RedoArgs{c.s, ref, rows.tgt, redo, redo + kHeader, tgt2});
+    lay_out(false, Layout{rows.h, p.n, 0, p.ld, redo + kHeader, redo, p.n, p.ld, p.ld, 0, again.h}, s);
     stats_of<F32>(p, c, again, e, redo);
     f.exps = nullptr, f.ref = nullptr, f.count = redo, f.which = redo + kHeader;
     finish(p, f, s);
     hipLaunchKernelGGL(redo_coef_kernel, dim3(row_blocks(p.n)), dim3(256), 0, s, c.s, redo, redo + kHeader, f.z_loss, grad);
     for (int64_t v0 = 0; v0 < p.vocab; v0 += p.piece) {
         const int64_t width = std::min(p.piece, p.vocab - v0);
-        const Head w = head_of(p, c, v0, width, true, redo);
-        gradient_of(p, c, again, w, v0, width, grad, k);
+        const Head w = head_of(p, c, v0, width, nullptr, redo);
+        gradient_of<false>(p, c, again, w, v0, width, grad, k, nullptr, true, false);
         times_head(p, c, again, w, v0, width);
     }
     unit_of(p, c, l, again, redo + kHeader, nullptr);
@@ -1543,7 +1579,7 @@ extern "C" int me_head_logps(const void *hidden, int dtype, int64_t n, int64_t d
     const Plan p = plan_of(n, vocab, dim, dtype, weight, w_stride, unit ? kLeavesUnit : kStats);
     ME_CHECK_ARG(workspace_bytes >= static_cast<size_t>(p.bytes), "workspace of %zu bytes, %lld are needed", workspace_bytes, static_cast<long long>(p.bytes));
     ME_CHECK_ARG(n == 0 || logps, "logps is needed");
-    ME_CHECK_ARG(reinterpret_cast<uintptr_t>(unit) % 16 == 0, "unit must be 16-byte aligned");
+    ME_CHECK_ARG(reinterpret_cast<uintptr_t>(unit) % 16 == 0 && (!unit || dtype == ME_BF16), "unit must be 16-byte aligned, and is for bf16");
     const Call c{hidden, weight, targets, rows_per_batch, batch_stride, row_stride, w_stride, ignore_index, targets_dtype,
                  static_cast<uint8_t *>(workspace), saved_of(saved, n), as_stream(stream)};
     return forward(p, c, Loss{temperature, 0.0, 0.0, 1.0, 0, logps, nullptr, unit});
@@ -1557,7 +1593,7 @@ extern "C" int me_head_ce(const void *hidden, int dtype, int64_t n, int64_t dim,
     if (rc != ME_OK) return rc;
     ME_CHECK_ARG(reduction == ME_REDUCE_MEAN || reduction == ME_REDUCE_SUM, "reduction must be mean or sum");
     ME_CHECK_ARG(loss, "loss is needed");
-    ME_CHECK_ARG(reinterpret_cast<uintptr_t>(unit) % 16 == 0, "unit must be 16-byte aligned");
+    ME_CHECK_ARG(reinterpret_cast<uintptr_t>(unit) % 16 == 0 && (!unit || dtype == ME_BF16), "unit must be 16-byte aligned, and is for bf16");
     const Plan p = plan_of(n, vocab, dim, dtype, weight, w_stride, unit ? kLeavesUnit : kStats);
     ME_CHECK_ARG(workspace_bytes >= static_cast<size_t>(p.bytes), "workspace of %zu bytes, %lld are needed", workspace_bytes, static_cast<long long>(p.bytes));
     const Call c{hidden, weight, targets, rows_per_batch, batch_stride, row_stride, w_stride, ignore_index, targets_dtype,
@@ -1575,18 +1611,14 @@ extern "C" int me_head_backward(const void *hidden, int dtype, int64_t n, int64_
     if (rc != ME_OK) return rc;
     ME_CHECK_ARG(upstream || (n == 0 && upstream_per_row), "upstream is needed");
     ME_CHECK_ARG(reinterpret_cast<uintptr_t>(grad_hidden) % 16 == 0 && reinterpret_cast<uintptr_t>(grad_weight) % 16 == 0, "gradients must be 16-byte aligned");
-    ME_CHECK_ARG(!unit || !grad_weight, "unit is for the hidden states' gradient alone");
+    ME_CHECK_ARG(!unit || (dtype == ME_BF16 && !grad_weight), "unit is for bf16 and the hidden states' gradient alone");
     if (!grad_hidden && !grad_weight) return ME_OK;
     const Saved saved_rows = saved_of(const_cast<void *>(saved), n);
     const bool f32 = dtype == ME_F32;
     if (unit) {
         if (n == 0) return ME_OK;
         const ScaleArgs a{unit, saved_rows.count, saved_rows.place, upstream, upstream_per_row != 0, reduction == ME_REDUCE_MEAN, scale / temperature, n, dim, grad_hidden};
-        const unsigned blocks = blocks_for(n * ceil_div(dim, 4));
-        if (f32)
-            hipLaunchKernelGGL(scale_kernel<true>, dim3(blocks), dim3(256), 0, as_stream(stream), a);
-        else
-            hipLaunchKernelGGL(scale_kernel<false>, dim3(blocks), dim3(256), 0, as_stream(stream), a);
+        hipLaunchKernelGGL(scale_kernel, dim3(blocks_for(n * ceil_div(dim, 4))), dim3(256), 0, as_stream(stream), a);
         return check_launch("me_head_backward");
     }
     const Plan p = plan_of(n, vocab, dim, dtype, weight, w_stride, kBackward);
@@ -1595,6 +1627,7 @@ extern "C" int me_head_backward(const void *hidden, int dtype, int64_t n, int64_
                  static_cast<uint8_t *>(workspace), saved_rows, as_stream(stream)};
     hipStream_t s = c.stream;
     int32_t *tgt = reinterpret_cast<int32_t *>(c.ws + p.tgt);
+    uint32_t *largest = f32 ? reinterpret_cast<uint32_t *>(c.ws + p.largest) : nullptr;
     Rows rows{};
     RowGrad *grad = reinterpret_cast<RowGrad *>(c.ws + p.grad);
     if (n > 0) {
@@ -1604,7 +1637,8 @@ extern "C" int me_head_backward(const void *hidden, int dtype, int64_t n, int64_
         else
             hipLaunchKernelGGL(targets_kernel<int32_t>, blocks, dim3(256), 0, s, static_cast<const int32_t *>(targets), n, c.s.rows, c.s.count, tgt);
         const CoefArgs k{c.s, n, upstream, upstream_per_row != 0, reduction == ME_REDUCE_MEAN, scale / temperature, static_cast<float>(smoothing),
-                         static_cast<float>(z_loss), static_cast<double>(vocab), grad};
+                         static_cast<float>(z_loss), static_cast<double>(vocab), grad, f32 ? reinterpret_cast<float *>(c.ws + p.bound) : nullptr,
+                         largest, f32 ? static_cast<int>(ceil_div(vocab, p.piece)) : 0};
         hipLaunchKernelGGL(coef_kernel, blocks, dim3(256), 0, s, k);
         rows = lay_out_rows(p, c);
         if (f32 && grad_weight) lay_out(true, hidden_layout(p, c, p.h), s);
@@ -1613,9 +1647,12 @@ extern "C" int me_head_backward(const void *hidden, int dtype, int64_t n, int64_
     for (int64_t v0 = 0; v0 < vocab; v0 += p.piece) {
         const int64_t width = std::min(p.piece, vocab - v0);
         if (n > 0) {
-            const Head w = head_of(p, c, v0, width, grad_hidden != nullptr);
-            gradient_of(p, c, rows, w, v0, width, grad, k);
-            if (grad_hidden) times_head(p, c, rows, w, v0, width);
+            uint32_t *widest = f32 ? largest + v0 / p.piece : nullptr;
+            const Head w = head_of(p, c, v0, width, widest);
+            const bool for_hidden = grad_hidden != nullptr, for_weight = grad_weight != nullptr;
+            f32 ? gradient_of<true>(p, c, rows, w, v0, width, grad, k, widest, for_hidden, for_weight)
+                : gradient_of<false>(p, c, rows, w, v0, width, grad, k, widest, for_hidden, for_weight);
+            if (grad_hidden) times_head(p, c, rows, w, v0, width, widest);
         }
         if (grad_weight) {
             const Gemm g{{c.ws + p.g, p.piece, p.rows * p.piece * 2}, {c.ws + p.h, p.ld, h_part(p)}, width, dim, n, c.s.count, 1, 8, 1, 0};

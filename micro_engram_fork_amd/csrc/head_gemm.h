@@ -19,7 +19,9 @@
 //   SEGS 3  two fp16 parts of the value over a power of two by row that puts the row's largest below 2^15; three of
 //           their four products, the fourth is below 2^-22 of the whole, its root mean square 2^-25. Half the
 //           matrix time; a value's parts hold it to 2^-22 of itself, or 2^-40 of its row's largest where that
-//           is more. That is as exact as fp32 for logits, whose error counts against those of their row.
+//           is more. That is as exact as fp32 where errors count against the rest of a row's sum: for logits, and for
+//           the gradient of the hidden states. The gradient of the head has rows of its own for tokens of any
+//           probability, down to products that fp16 could not tell from zero: six products.
 #pragma once
 
 #include "me_common.h"

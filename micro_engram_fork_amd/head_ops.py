@@ -7,7 +7,7 @@ from typing import List, Optional
 
 import torch
 
-from ._lib import call
+from ._lib import ME_BF16, call
 from .loss_ops import _targets, row_layout
 from .ops import _custom_op, _p, call_on, dtype_code, require_gpu
 
@@ -40,7 +40,9 @@ def _workspace(hidden, operands, which):
 
 @functools.lru_cache(maxsize=256)
 def unit_elements(n, vocab, dim, dtype):
-    """Size of what a forward leaves for the gradient of hidden alone; 0: nothing."""
+    """Size of what a forward leaves for the gradient of hidden alone; 0: nothing, as always of fp32."""
+    if dtype != ME_BF16:
+        return 0
     size = ctypes.c_int64(0)
     call("me_head_unit_size", n, vocab, dim, dtype, ctypes.byref(size))
     return size.value
