@@ -30,11 +30,18 @@ def _operands(hidden, weight, targets, ignore_index):
     return (hidden, weight, targets), (*rows, *head, *toks)
 
 
-def _workspace(hidden, operands, which):
-    """(buffer, address, size)."""
+@functools.lru_cache(maxsize=256)
+def workspace_bytes(n, vocab, dim, dtype, misaligned, w_stride, which):
+    """misaligned: the weight's address modulo 16."""
     size = ctypes.c_size_t(0)
-    call("me_head_workspace_size", operands[2], operands[8], operands[3], operands[1], operands[7], operands[9], which, ctypes.byref(size))
-    ws = torch.empty(size.value, dtype=torch.uint8, device=hidden.device)
+    call("me_head_workspace_size", n, vocab, dim, dtype, misaligned, w_stride, which, ctypes.byref(size))
+    return size.value
+
+
+def _workspace(operands, dev, which):
+    """(buffer, address, size)."""
+    _, dtype, n, dim, _, _, _, weight, vocab, w_stride = operands[:10]
+    ws = torch.empty(workspace_bytes(n, vocab, dim, dtype, weight % 16, w_stride, which), dtype=torch.uint8, device=dev)
     return ws, ws.data_ptr(), ws.numel()
 
 
@@ -53,14 +60,42 @@ def _unit_size(hidden, weight, targets):
 
 
 def _forward(name, hidden, weight, targets, ignore_index, with_unit, out, args):
+    """([out, saved] and unit where the call leaves one, the operands' arguments with the tensors that hold them)."""
     dev = require_gpu(hidden, weight, targets)
     held, operands = _operands(hidden, weight, targets, ignore_index)
     saved = torch.empty(16 + 4 * operands[2], dtype=torch.float32, device=dev)
-    size = _unit_size(hidden, weight, targets) if with_unit else 0
+    size = unit_elements(operands[2], operands[8], operands[3], operands[1]) if with_unit else 0
     unit = torch.empty(size, dtype=torch.float32, device=dev) if size else None
-    ws, ptr, size = _workspace(held[0], operands, _FORWARD if unit is None else _FORWARD_UNIT)
+    ws, ptr, size = _workspace(operands, dev, _FORWARD if unit is None else _FORWARD_UNIT)
     call_on(dev, name, *operands, *args, out.data_ptr(), saved.data_ptr(), _p(unit), ptr, size)
-    return [out, saved] if unit is None else [out, saved, unit]
+    return [out, saved] if unit is None else [out, saved, unit], (held, operands)
+
+
+class Backward:
+    """The backward's call, made ready in the forward: as loss_ops.Backward. kept: what the forward gave beside its result;
+    consts: the arguments of head_backward from the temperature to the reduction."""
+    __slots__ = ("held", "operands", "saved", "unit", "consts")
+
+    def __init__(self, held, kept, consts):
+        (self.held, self.operands), self.consts = held, consts
+        self.saved, self.unit = kept[0], kept[1] if len(kept) > 1 else None
+
+    def __call__(self, upstream, need_hidden, need_weight):
+        hidden, weight, _ = self.held
+        return _backward(hidden.shape, weight.shape, self.operands, hidden, self.saved, self.unit, upstream, self.consts,
+                         need_hidden, need_weight)
+
+
+def _backward(hidden_shape, weight_shape, operands, like, saved, unit, upstream, consts, need_hidden, need_weight):
+    """(gradient of hidden or None, gradient of weight or None)."""
+    dev, dtype = like.device, like.dtype
+    grad_hidden = torch.empty(hidden_shape, dtype=dtype, device=dev) if need_hidden else None
+    grad_weight = torch.empty(weight_shape, dtype=dtype, device=dev) if need_weight else None
+    ws, ptr, size = _workspace(operands, dev, _BACKWARD) if unit is None else (None, None, 0)
+    temperature, per_row, smoothing, z_loss, scale, reduction = consts
+    call_on(dev, "me_head_backward", *operands, temperature, upstream.data_ptr(), int(per_row), smoothing, z_loss, scale,
+            reduction, saved.data_ptr(), _p(unit), _p(grad_hidden), _p(grad_weight), ptr, size)
+    return grad_hidden, grad_weight
 
 
 def _fake_forward(hidden, weight, targets, with_unit, shape):
@@ -69,13 +104,17 @@ def _fake_forward(hidden, weight, targets, with_unit, shape):
     return [*res, hidden.new_empty((size,), dtype=torch.float32)] if size else res
 
 
+def run_head_logps(hidden, weight, targets, ignore_index, temperature, with_unit):
+    out = torch.empty(targets.shape, dtype=torch.float32, device=targets.device)
+    return _forward("me_head_logps", hidden, weight, targets, ignore_index, with_unit, out, (temperature,))
+
+
 @_custom_op("head_logps")
 def head_logps(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, ignore_index: int,
                temperature: float, with_unit: bool) -> List[torch.Tensor]:
     """[log-probabilities fp32 of targets' shape, saved (what the backward needs)], and where with_unit and the size pays
     unit, from which the backward of hidden alone only scales."""
-    out = torch.empty(targets.shape, dtype=torch.float32, device=targets.device)
-    return _forward("me_head_logps", hidden, weight, targets, ignore_index, with_unit, out, (temperature,))
+    return run_head_logps(hidden, weight, targets, ignore_index, temperature, with_unit)[0]
 
 
 @head_logps.register_fake
@@ -83,13 +122,17 @@ def _(hidden, weight, targets, ignore_index, temperature, with_unit):
     return _fake_forward(hidden, weight, targets, with_unit, targets.shape)
 
 
+def run_head_ce(hidden, weight, targets, ignore_index, temperature, smoothing, z_loss, scale, reduction, with_unit):
+    out = torch.empty((), dtype=torch.float32, device=targets.device)
+    return _forward("me_head_ce", hidden, weight, targets, ignore_index, with_unit, out,
+                    (temperature, smoothing, z_loss, scale, reduction))
+
+
 @_custom_op("head_ce")
 def head_ce(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, ignore_index: int, temperature: float,
             smoothing: float, z_loss: float, scale: float, reduction: int, with_unit: bool) -> List[torch.Tensor]:
     """[loss fp32, saved], and unit as of head_logps."""
-    out = torch.empty((), dtype=torch.float32, device=targets.device)
-    return _forward("me_head_ce", hidden, weight, targets, ignore_index, with_unit, out,
-                    (temperature, smoothing, z_loss, scale, reduction))
+    return run_head_ce(hidden, weight, targets, ignore_index, temperature, smoothing, z_loss, scale, reduction, with_unit)[0]
 
 
 @head_ce.register_fake
@@ -103,14 +146,12 @@ def head_backward(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Ten
                   smoothing: float, z_loss: float, scale: float, reduction: int, need_hidden: bool,
                   need_weight: bool) -> List[torch.Tensor]:
     """The gradients that are needed, of hidden and of weight. upstream: fp32, one (head_ce) or per row (head_logps)."""
-    dev = require_gpu(hidden, weight, targets, saved, unit, upstream)
-    held, operands = _operands(hidden, weight, targets, ignore_index)
-    grad_hidden = torch.empty(hidden.shape, dtype=hidden.dtype, device=dev) if need_hidden else None
-    grad_weight = torch.empty(weight.shape, dtype=weight.dtype, device=dev) if need_weight else None
-    ws, ptr, size = _workspace(held[0], operands, _BACKWARD) if unit is None else (None, None, 0)
-    call_on(dev, "me_head_backward", *operands, temperature, upstream.data_ptr(), int(per_row), smoothing, z_loss, scale,
-            reduction, saved.data_ptr(), _p(unit), _p(grad_hidden), _p(grad_weight), ptr, size)
-    return [g for g in (grad_hidden, grad_weight) if g is not None]
+    require_gpu(hidden, weight, targets, saved, unit, upstream)
+    _, operands = held = _operands(hidden, weight, targets, ignore_index)
+    grads = _backward(hidden.shape, weight.shape, operands, hidden, saved, unit, upstream,
+                      (temperature, per_row, smoothing, z_loss, scale, reduction), need_hidden, need_weight)
+    del held  # the operands are addresses in these
+    return [g for g in grads if g is not None]
 
 
 @head_backward.register_fake

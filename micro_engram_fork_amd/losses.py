@@ -381,31 +381,44 @@ def _check_head(hidden, weight, targets):
 
 
 class _HeadLoss(torch.autograd.Function):
-    """args: (op, ignore_index, temperature, and for head_ce smoothing, z_loss, scale, reduction)."""
+    """kind: (the op, its plain run, whether upstream is per row). args: ignore_index, temperature, and for the cross
+    entropy smoothing, z_loss, scale, reduction."""
 
     @staticmethod
-    def forward(ctx, hidden, weight, targets, args):
-        out, *kept = args[0](hidden.detach(), weight.detach(), targets, *args[1:], not weight.requires_grad)
+    def forward(ctx, hidden, weight, targets, kind, args):
+        op, run, per_row = kind
+        ctx.consts = args[1], per_row, *(args[2:] or (0.0, 0.0, 1.0, ME_REDUCE_SUM))
+        ctx.ignore_index, ctx.run = args[0], None
+        with_unit = not weight.requires_grad
+        if _makes_ready(hidden, weight, targets):
+            (out, *kept), held = run(hidden.detach(), weight.detach(), targets, *args, with_unit)
+            ctx.run = head_ops.Backward(held, kept, ctx.consts)
+        else:
+            out, *kept = op(hidden.detach(), weight.detach(), targets, *args, with_unit)
         ctx.save_for_backward(hidden, weight, targets, *kept)
-        ctx.consts = args[1:]
         return out
 
     @staticmethod
     @_no_second_derivatives
     def backward(ctx, upstream):
-        hidden, weight, targets, saved, *unit = ctx.saved_tensors
+        hidden, weight, targets, saved, *unit = ctx.saved_tensors  # looks whether they are still as they were
         need = ctx.needs_input_grad[:2]
-        per_row = len(ctx.consts) == 2
-        ignore_index, temperature, *rest = ctx.consts if not per_row else (*ctx.consts, 0.0, 0.0, 1.0, ME_REDUCE_SUM)
+        run, ctx.run = ctx.run, None
+        if run is not None and type(upstream) is torch.Tensor:
+            return *run(_upstream(upstream), *need), None, None, None
         grads = iter(head_ops.head_backward(hidden.detach(), weight.detach(), targets, saved, unit[0] if unit else None,
-                                            _upstream(upstream), ignore_index, temperature, per_row, *rest, *need))
-        return next(grads) if need[0] else None, next(grads) if need[1] else None, None, None
+                                            _upstream(upstream), ctx.ignore_index, *ctx.consts, *need))
+        return next(grads) if need[0] else None, next(grads) if need[1] else None, None, None, None
 
 
-def _head_loss(op, hidden, weight, targets, *args):
+_HEAD_LOGPS = head_ops.head_logps, head_ops.run_head_logps, True
+_HEAD_CE = head_ops.head_ce, head_ops.run_head_ce, False
+
+
+def _head_loss(kind, hidden, weight, targets, *args):
     if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
-        return _HeadLoss.apply(hidden, weight, targets, (op, *args))
-    return op(hidden.detach(), weight.detach(), targets, *args, False)[0]
+        return _HeadLoss.apply(hidden, weight, targets, kind, args)
+    return kind[0](hidden.detach(), weight.detach(), targets, *args, False)[0]
 
 
 def head_token_logps(hidden, weight, targets, temperature=1.0, ignore_index=IGNORE_INDEX):
@@ -416,7 +429,7 @@ def head_token_logps(hidden, weight, targets, temperature=1.0, ignore_index=IGNO
     Memory is that of a piece of the logits' gradient (512 MiB at most for up to 131,072 rows in bf16), whatever the
     vocabulary. Rows that do not count cost nothing and are not read."""
     _check_head(hidden, weight, targets)
-    return _head_loss(head_ops.head_logps, hidden, weight, targets, int(ignore_index), _check_temperature(temperature))
+    return _head_loss(_HEAD_LOGPS, hidden, weight, targets, int(ignore_index), _check_temperature(temperature))
 
 
 def head_cross_entropy(hidden, weight, targets, temperature=1.0, label_smoothing=0.0, z_loss=0.0, scale=1.0,
@@ -433,5 +446,5 @@ def head_cross_entropy(hidden, weight, targets, temperature=1.0, label_smoothing
     smoothing = _check_number(label_smoothing, "label_smoothing", 0.0, 1.0)
     z_loss = _check_number(z_loss, "z_loss", 0.0, 1e6)
     scale = _check_number(scale, "scale", -1e30, 1e30)
-    return _head_loss(head_ops.head_ce, hidden, weight, targets, int(ignore_index), _check_temperature(temperature), smoothing,
+    return _head_loss(_HEAD_CE, hidden, weight, targets, int(ignore_index), _check_temperature(temperature), smoothing,
                       z_loss, scale, how)
