@@ -28,7 +28,11 @@ using namespace head;
 
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr double kLn2 = 0.69314718055994530942;
-constexpr int64_t kFew = 128;                            // rows up to which the 64-row tiles are taken
+// Rows up to which the 64-row tiles are taken, and twice as many where 256-row tiles would leave CUs without one and a
+// tile's K loop is short. us, 64-row / 256-row tiles, log-probabilities alone: 262,144 x 5376, 129 rows 898 / 646, 96 rows
+// 699 / (129 rows') 646; 32,000 x 1024, 129 to 256 rows 42-44 / 57-59; 32,000 x 4096, 256 rows 109 / 112 and with
+// the hidden states' gradient 262 / 248
+constexpr int64_t kFew = 128;
 constexpr int64_t kPieceBytes = int64_t{1} << 30;        // of a piece's gradient, and of a piece of laid-out weights
 constexpr int kSplits = 3, kMostSplits = 16;             // of the product with W
 constexpr int kHeader = 16;                              // ints before the rows in `saved`: the number of them
@@ -1188,7 +1192,7 @@ Plan plan_of(int64_t n, int64_t vocab, int64_t dim, int dtype, const void *weigh
     p.f32 = dtype == ME_F32;
     p.np = p.f32 ? 3 : 1;
     p.nz = p.f32 ? 2 : 1;
-    p.few = n <= kFew;
+    p.few = n <= kFew || (n <= 2 * kFew && vocab <= 65536 && dim <= 2048);
     p.copy_w = p.f32 || w_stride % 8 != 0 || reinterpret_cast<uintptr_t>(weight) % 16 != 0;
     const int64_t rows = p.rows = round_up(std::max<int64_t>(n, 1), 64);
     int64_t piece = round_up(vocab, kTile);
