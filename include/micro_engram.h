@@ -681,7 +681,7 @@ int me_distill_backward(const void *logits, int dtype, int64_t n, int64_t vocab,
  *               bf16 rows that start at multiples of 16 bytes are read where they lie, others and
  *               fp32 ones are laid out a piece at a time
  *   targets, ignore_index, temperature  as above; nothing of a row that does not count is read
- *   saved       [16 + 4 n] 4-byte elements (16-byte aligned): what the backward needs
+ *   saved       [16 + 5 n] 4-byte elements (16-byte aligned): what the backward needs
  *   unit        nullable, [me_head_unit_size] fp32 (16-byte aligned), ME_BF16 alone: where the
  *               gradient of hidden alone is wanted, the forward leaves there what the backward only has to scale. A
  *               size of 0: the call is too small for that to pay (unit may still be given, n times

@@ -37,26 +37,26 @@ constexpr int64_t kPieceBytes = int64_t{1} << 30;        // of a piece's gradien
 constexpr int kSplits = 3, kMostSplits = 16;             // of the product with W
 constexpr int kHeader = 16;                              // ints before the rows in `saved`: the number of them
 
-// What the forward leaves for the backward: counted rows, and by counted row its source, log2-sum and o; by source
-// row its place among the counted ones.
+// What the forward leaves for the backward: the number of counted rows, and by counted row its source, target,
+// log2-sum and o; by source row its place among the counted ones.
 struct Saved {
-    int32_t *count, *rows, *place;
+    int32_t *count, *rows, *place, *tgt;
     float *lse2, *others;
 };
 
 Saved saved_of(void *p, int64_t n) {
     int32_t *i = static_cast<int32_t *>(p);
     float *f = static_cast<float *>(p);
-    return {i, i + kHeader, i + kHeader + n, f + kHeader + 2 * n, f + kHeader + 3 * n};
+    return {i, i + kHeader, i + kHeader + n, i + kHeader + 2 * n, f + kHeader + 3 * n, f + kHeader + 4 * n};
 }
 
 // ---- rows that count -------------------------------------------------------------------------------------------
-// One workgroup: rows[r] = source of the r-th counted row, place[i] = r or -1, tgt[r] its target.
+// One workgroup: rows[r] = source of the r-th counted row, tgt[r] its target, place[i] = r or -1.
 constexpr int kIndexThreads = 1024;
 
 template <typename T>
 __global__ __launch_bounds__(kIndexThreads) void index_kernel(const T *targets, int64_t n, int64_t ignore, int64_t vocab,
-                                                              Saved s, int32_t *tgt) {
+                                                              Saved s) {
     __shared__ int sums[kIndexThreads / 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int at = 0;
@@ -76,7 +76,7 @@ __global__ __launch_bounds__(kIndexThreads) void index_kernel(const T *targets, 
         if (i < n) s.place[i] = ok ? r : -1;
         if (ok) {
             s.rows[r] = static_cast<int32_t>(i);
-            tgt[r] = static_cast<int32_t>(t);
+            s.tgt[r] = static_cast<int32_t>(t);
         }
         at += all;
         __syncthreads();
@@ -84,11 +84,46 @@ __global__ __launch_bounds__(kIndexThreads) void index_kernel(const T *targets, 
     if (tid == 0) *s.count = at;
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void targets_kernel(const T *targets, int64_t n, const int32_t *rows, const int32_t *count, int32_t *tgt) {
-    const int64_t r = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-    if (r < n && r < *count) tgt[r] = static_cast<int32_t>(targets[rows[r]]);
-}
+// ---- what the gradient of a row's logits is made of ---------------------------------------------------------------
+// dz_j = ca 2^(z_j - lse2) - cb, gt at the target, z in units of log2
+struct RowGrad {
+    float lse2, ca, cb, gt;
+};
+
+struct Coefs {
+    Saved s;
+    const float *upstream;  // by source row (per_row) or one
+    int per_row, mean;
+    double scale;           // of the loss, over T
+    float smoothing, z_loss;
+    double vocab;
+    RowGrad *grad;          // null: none of this is wanted
+    float *bound;           // of each row's values, or null
+    uint32_t *largest;      // set to 0, `pieces` of them
+    int pieces;
+
+    __device__ __forceinline__ void row(int64_t r, int64_t count) const {
+        const float lse2 = s.lse2[r], o = s.others[r];
+        RowGrad g;
+        g.lse2 = lse2;
+        if (per_row) {  // log-probabilities: -upstream times the loss -log q
+            const float c = static_cast<float>(-static_cast<double>(upstream[s.rows[r]]) * scale);
+            g.ca = c, g.cb = 0.f, g.gt = -c * o;
+        } else {
+            const double c = static_cast<double>(*upstream) * scale / (mean ? static_cast<double>(max(count, int64_t{1})) : 1.0);
+            const double more = 2.0 * z_loss * kLn2 * lse2, e = smoothing;
+            g.ca = static_cast<float>(c * (1.0 + more));
+            g.cb = static_cast<float>(c * e / vocab);
+            g.gt = static_cast<float>(c * (more - (1.0 + more) * o + e - e / vocab));
+        }
+        grad[r] = g;
+        // a token's probability is at most that of all but the target
+        if (bound) bound[r] = fmaxf(fabsf(g.ca) * (1.0001f * o) + fabsf(g.cb), fabsf(g.gt));
+    }
+    __device__ __forceinline__ void clear(int64_t thread) const {
+        if (thread < pieces) largest[thread] = 0;
+    }
+};
 
 // ---- operands as the products read them: [rows][ld] bf16, ld a multiple of 64, zeros past dim; fp32 in three parts -----
 typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));        // pieces of rows that may start
@@ -126,13 +161,15 @@ __device__ __forceinline__ void split3(float x, uint16_t (&p)[3]) {
     p[2] = float_to_bf16_bits_rne(rest - bf16_bits_to_float(p[1]));
 }
 
+// k: of the rows' gradients, which the first of a row's threads makes on the way (the row layout of a backward)
 template <bool F32>
-__global__ __launch_bounds__(256) void layout_kernel(const Layout a) {
+__global__ __launch_bounds__(256) void layout_kernel(const Layout a, const Coefs k) {
     if (a.gate != nullptr && *a.gate == 0) return;
     const int64_t units = a.ld / 8;
     const int64_t n = a.count ? min(a.n, static_cast<int64_t>(*a.count)) : a.n;
     for (int64_t u = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; u < n * units; u += static_cast<int64_t>(gridDim.x) * 256) {
         const int64_t r = u / units, c = (u - r * units) * 8;
+        if (k.grad != nullptr && c == 0) k.row(r, n);
         const int64_t from = a.rows ? a.rows[r] : r;
         const int64_t at = from / a.per_batch * a.batch_stride + from % a.per_batch * a.row_stride + c;
         uint32_t w[3][4] = {};
@@ -166,8 +203,9 @@ __global__ __launch_bounds__(256) void layout_kernel(const Layout a) {
 // fp32 rows in two fp16 parts over a power of two by row, which goes to `scale` (what the parts are multiplied by to
 // give the value), and the largest of these, where wanted, to `largest`. A wave per row. Of what is not finite, the
 // first part alone.
-__global__ __launch_bounds__(256) void layout16_kernel(const Layout a, float *scale, uint32_t *largest) {
+__global__ __launch_bounds__(256) void layout16_kernel(const Layout a, float *scale, uint32_t *largest, const Coefs k) {
     uint32_t widest = 0;
+    if (k.grad != nullptr) k.clear(static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x);
     const int lane = threadIdx.x & 63;
     const int64_t n = a.count ? min(a.n, static_cast<int64_t>(*a.count)) : a.n;
     constexpr int kKept = 4;  // pieces of 512 values that stay in registers; further ones are read again
@@ -201,7 +239,10 @@ __global__ __launch_bounds__(256) void layout16_kernel(const Layout a, float *sc
         const float times = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
         const uint32_t down = static_cast<uint32_t>(127 - up) << 23;
         widest = max(widest, down);
-        if (lane == 0) scale[r] = __uint_as_float(down);
+        if (lane == 0) {
+            scale[r] = __uint_as_float(down);
+            if (k.grad != nullptr) k.row(r, n);
+        }
         auto put = [&](const float (&v)[8], int64_t c) {
             if (c >= a.ld) return;
             halfx8 hi, lo;
@@ -450,10 +491,6 @@ struct ExpEpilogue {
             }
         return s;
     }
-};
-
-struct RowGrad {
-    float lse2, ca, cb, gt;
 };
 
 // Power of two that puts a row's gradient times the columns' scales into fp16's range: the largest below 2^15. row: a
@@ -722,7 +759,7 @@ __global__ __launch_bounds__(256) void vector_kernel(const VectorArgs a) {
         if (lane == 0) s_count = __popcll(mask);
         if (blockIdx.x == 0) {  // for the launches that follow
             if (lane < n) a.s.place[lane] = ok ? r : -1;
-            if (ok) a.s.rows[r] = lane;
+            if (ok) a.s.rows[r] = lane, a.s.tgt[r] = static_cast<int>(t);
             if (lane == 0) *a.s.count = __popcll(mask);
         }
     }
@@ -842,7 +879,7 @@ struct FinishArgs {
     float *logps;        // by source row, or null
     float *row_loss;     // by counted row, or null
     float smoothing, z_loss;
-    int by_source;       // WIDE: a workgroup per source row, which writes the logps of those that do not count too
+    int uncounted;       // the logps of source rows that do not count are written too: zeros
 };
 
 // A row's parts joined: WIDE 256 threads per row (few rows), else 16 rows by 16 threads each
@@ -852,20 +889,10 @@ __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs a) {
     __shared__ Sum2 s_all[WIDE ? 4 : 256];
     __shared__ double s_sum[WIDE ? 4 : 256];
     const int tid = threadIdx.x, slice = tid / kRows;
-    int64_t r = static_cast<int64_t>(blockIdx.x) * kRows + tid % kRows;
+    const int64_t r = static_cast<int64_t>(blockIdx.x) * kRows + tid % kRows;
     const int64_t count = a.count ? *a.count : *a.s.count;
-    if constexpr (WIDE) {
-        if (a.by_source) {
-            r = a.s.place[blockIdx.x];
-            if (r < 0) {
-                if (tid == 0 && a.logps) a.logps[blockIdx.x] = 0.f;
-                return;
-            }
-        }
-        if (r >= count) return;
-    } else {
-        if (static_cast<int64_t>(blockIdx.x) * kRows >= count) return;
-    }
+    if (a.uncounted && a.logps && tid < kRows && r < a.n && a.s.place[r] < 0) a.logps[r] = 0.f;
+    if (static_cast<int64_t>(blockIdx.x) * kRows >= count) return;
     Sum2 all = {-__builtin_inff(), 0.f};
     double sum = 0.0;
     if (r < count) {
@@ -914,11 +941,6 @@ __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs a) {
     }
 }
 
-__global__ __launch_bounds__(256) void uncounted_logps_kernel(const int32_t *place, int64_t n, float *logps) {
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-    if (i < n && place[i] < 0) logps[i] = 0.f;
-}
-
 __global__ __launch_bounds__(1024) void total_kernel(const float *row_loss, const int32_t *count, double scale, int mean, float *loss) {
     __shared__ double s[16];
     const int n = *count;
@@ -933,44 +955,6 @@ __global__ __launch_bounds__(1024) void total_kernel(const float *row_loss, cons
         for (int i = 0; i < 16; ++i) sum += s[i];
         *loss = static_cast<float>(sum * scale / (mean ? max(n, 1) : 1));
     }
-}
-
-struct CoefArgs {
-    Saved s;
-    int64_t n;
-    const float *upstream;  // by source row (per_row) or one
-    int per_row, mean;
-    double scale;           // of the loss, over T
-    float smoothing, z_loss;
-    double vocab;
-    RowGrad *grad;
-    float *bound;           // of each row's values, or null
-    uint32_t *largest;      // set to 0, `pieces` of them
-    int pieces;
-};
-
-__global__ __launch_bounds__(256) void coef_kernel(const CoefArgs a) {
-    if (blockIdx.x == 0)
-        for (int i = static_cast<int>(threadIdx.x); i < a.pieces; i += 256) a.largest[i] = 0;
-    const int64_t r = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-    const int64_t count = *a.s.count;
-    if (r >= a.n || r >= count) return;
-    const float lse2 = a.s.lse2[r], o = a.s.others[r];
-    RowGrad g;
-    g.lse2 = lse2;
-    if (a.per_row) {  // log-probabilities: -upstream times the loss -log q
-        const float c = static_cast<float>(-static_cast<double>(a.upstream[a.s.rows[r]]) * a.scale);
-        g.ca = c, g.cb = 0.f, g.gt = -c * o;
-    } else {
-        const double c = static_cast<double>(*a.upstream) * a.scale / (a.mean ? static_cast<double>(max(count, int64_t{1})) : 1.0);
-        const double more = 2.0 * a.z_loss * kLn2 * lse2, e = a.smoothing;
-        g.ca = static_cast<float>(c * (1.0 + more));
-        g.cb = static_cast<float>(c * e / a.vocab);
-        g.gt = static_cast<float>(c * (more - (1.0 + more) * o + e - e / a.vocab));
-    }
-    a.grad[r] = g;
-    // a token's probability is at most that of all but the target
-    if (a.bound) a.bound[r] = fmaxf(fabsf(g.ca) * (1.0001f * o) + fabsf(g.cb), fabsf(g.gt));
 }
 
 // Four values of a row of the hidden states' gradient
@@ -1177,7 +1161,7 @@ struct Plan {
     int64_t piece;                    // columns of the vocabulary at a time
     int splits;                       // of the product with W, at most
     int split_cost;
-    int64_t h, tgt, part, sum, at_target, row_loss, g, grad, acc;  // workspace offsets
+    int64_t h, part, sum, at_target, row_loss, g, grad, acc;  // workspace offsets
     int64_t ref, redo, h2, tgt2, columns, column_part;
     int64_t z, wz, row_scale, col_scale;  // operands of the logits; fp32: fp16 parts, and their scales
     int64_t half, bound, largest;         // fp32: the gradient in fp16 parts, its rows' bounds, the scales' largest by piece
@@ -1206,7 +1190,6 @@ Plan plan_of(int64_t n, int64_t vocab, int64_t dim, int dtype, const void *weigh
         at += round_up(bytes, 256);
         return here;
     };
-    p.tgt = take(n * 4);
     p.grad = take(n * static_cast<int64_t>(sizeof(RowGrad)));
     p.z = take(rows * p.ld * 2 * p.nz);
     p.h = p.z;
@@ -1268,12 +1251,12 @@ struct Call {
 
 unsigned blocks_for(int64_t units) { return static_cast<unsigned>(std::min<int64_t>(std::max<int64_t>(ceil_div(units, 256), 1), 16384)); }
 
-void lay_out(bool f32, const Layout &l, hipStream_t s) {
+void lay_out(bool f32, const Layout &l, hipStream_t s, const Coefs &k = Coefs{}) {
     const unsigned blocks = blocks_for(l.n * (l.ld / 8));
     if (f32)
-        hipLaunchKernelGGL(layout_kernel<true>, dim3(blocks), dim3(256), 0, s, l);
+        hipLaunchKernelGGL(layout_kernel<true>, dim3(blocks), dim3(256), 0, s, l, k);
     else
-        hipLaunchKernelGGL(layout_kernel<false>, dim3(blocks), dim3(256), 0, s, l);
+        hipLaunchKernelGGL(layout_kernel<false>, dim3(blocks), dim3(256), 0, s, l, k);
 }
 
 int64_t h_part(const Plan &p) { return p.rows * p.ld * 2; }
@@ -1282,9 +1265,10 @@ Layout hidden_layout(const Plan &p, const Call &c, int64_t to) {
     return {c.hidden, c.per_batch, c.batch_stride, c.row_stride, c.s.rows, c.s.count, p.n, p.dim, p.ld, h_part(p), c.ws + to};
 }
 
-void lay_out16(const Layout &l, float *scale, uint32_t *largest, hipStream_t s) {
-    const unsigned blocks = static_cast<unsigned>(std::min<int64_t>(std::max<int64_t>(ceil_div(l.n, 4), 1), 2048));
-    hipLaunchKernelGGL(layout16_kernel, dim3(blocks), dim3(256), 0, s, l, scale, largest);
+void lay_out16(const Layout &l, float *scale, uint32_t *largest, hipStream_t s, const Coefs &k = Coefs{}) {
+    // a thread for each piece's largest scale among them (pieces of 2048 columns or more: at most 1024)
+    const unsigned blocks = static_cast<unsigned>(std::min<int64_t>(std::max<int64_t>({ceil_div(l.n, 4), 1, k.grad ? 4 : 1}), 2048));
+    hipLaunchKernelGGL(layout16_kernel, dim3(blocks), dim3(256), 0, s, l, scale, largest, k);
 }
 
 // Rows of a product: the hidden states laid out for the logits, with how many there are, their targets and, of
@@ -1295,13 +1279,13 @@ struct Rows {
     const float *scale;
 };
 
-Rows lay_out_rows(const Plan &p, const Call &c) {
+Rows lay_out_rows(const Plan &p, const Call &c, const Coefs &k = Coefs{}) {
     float *scale = p.f32 ? reinterpret_cast<float *>(c.ws + p.row_scale) : nullptr;
     if (p.f32)
-        lay_out16(hidden_layout(p, c, p.z), scale, nullptr, c.stream);
+        lay_out16(hidden_layout(p, c, p.z), scale, nullptr, c.stream, k);
     else
-        lay_out(false, hidden_layout(p, c, p.z), c.stream);
-    return {c.ws + p.z, c.s.count, reinterpret_cast<const int32_t *>(c.ws + p.tgt), scale};
+        lay_out(false, hidden_layout(p, c, p.z), c.stream, k);
+    return {c.ws + p.z, c.s.count, c.s.tgt, scale};
 }
 
 // The head from row v0 on, `width` rows of it
@@ -1431,7 +1415,7 @@ void forward_rows(const Plan &p, const Call &c, const Loss &l) {
     e.k = k;
     FinishArgs f{};
     f.part = e.part, f.sum = e.sum, f.at_target = at_target, f.part_stride = e.part_stride, f.row_stride = e.row_stride, f.parts = parts;
-    f.n = p.n, f.vocab = p.vocab, f.s = c.s, f.logps = l.logps;
+    f.n = p.n, f.vocab = p.vocab, f.s = c.s, f.logps = l.logps, f.uncounted = 1;
     f.row_loss = l.loss ? reinterpret_cast<float *>(c.ws + p.row_loss) : nullptr;
     f.smoothing = static_cast<float>(l.smoothing), f.z_loss = static_cast<float>(l.z_loss);
     if (F32 || !l.unit) {
@@ -1468,7 +1452,7 @@ void forward_rows(const Plan &p, const Call &c, const Loss &l) {
     hipLaunchKernelGGL(redo_kernel, dim3(1), dim3(kIndexThreads), 0, s, RedoArgs{c.s, ref, rows.tgt, redo, redo + kHeader, tgt2});
     lay_out(false, Layout{rows.h, p.n, 0, p.ld, redo + kHeader, redo, p.n, p.ld, p.ld, 0, again.h}, s);
     stats_of<F32>(p, c, again, e, redo);
-    f.exps = nullptr, f.ref = nullptr, f.count = redo, f.which = redo + kHeader;
+    f.uncounted = 0, f.exps = nullptr, f.ref = nullptr, f.count = redo, f.which = redo + kHeader;
     finish(p, f, s);
     hipLaunchKernelGGL(redo_coef_kernel, dim3(row_blocks(p.n)), dim3(256), 0, s, c.s, redo, redo + kHeader, f.z_loss, grad);
     for (int64_t v0 = 0; v0 < p.vocab; v0 += p.piece) {
@@ -1512,14 +1496,13 @@ void forward_vectors(const Plan &p, const Call &c, const Loss &l, int rows, size
     vector_rows(a, rows, groups, lds, c.stream);
     FinishArgs f{};
     f.part = a.part, f.sum = a.sum, f.at_target = a.at_target, f.part_stride = 1, f.row_stride = groups, f.parts = static_cast<int>(groups);
-    f.n = p.n, f.vocab = p.vocab, f.s = c.s, f.logps = l.logps, f.by_source = 1;
+    f.n = p.n, f.vocab = p.vocab, f.s = c.s, f.logps = l.logps, f.uncounted = 1;
     f.row_loss = l.loss ? reinterpret_cast<float *>(c.ws + p.row_loss) : nullptr;
     f.smoothing = static_cast<float>(l.smoothing), f.z_loss = static_cast<float>(l.z_loss);
     hipLaunchKernelGGL(finish_kernel<true>, dim3(static_cast<unsigned>(p.n)), dim3(256), 0, c.stream, f);
 }
 
 int forward(const Plan &p, const Call &c, const Loss &l) {
-    int32_t *tgt = reinterpret_cast<int32_t *>(c.ws + p.tgt);
     hipStream_t s = c.stream;
     int rows;
     size_t lds;
@@ -1529,12 +1512,11 @@ int forward(const Plan &p, const Call &c, const Loss &l) {
         return check_launch("me_head");
     }
     if (c.tdtype == ME_I64)
-        hipLaunchKernelGGL(index_kernel<int64_t>, dim3(1), dim3(kIndexThreads), 0, s, static_cast<const int64_t *>(c.targets), p.n, c.ignore, p.vocab, c.s, tgt);
+        hipLaunchKernelGGL(index_kernel<int64_t>, dim3(1), dim3(kIndexThreads), 0, s, static_cast<const int64_t *>(c.targets), p.n, c.ignore, p.vocab, c.s);
     else
-        hipLaunchKernelGGL(index_kernel<int32_t>, dim3(1), dim3(kIndexThreads), 0, s, static_cast<const int32_t *>(c.targets), p.n, c.ignore, p.vocab, c.s, tgt);
+        hipLaunchKernelGGL(index_kernel<int32_t>, dim3(1), dim3(kIndexThreads), 0, s, static_cast<const int32_t *>(c.targets), p.n, c.ignore, p.vocab, c.s);
     if (p.n > 0) {
         p.f32 ? forward_rows<true>(p, c, l) : forward_rows<false>(p, c, l);
-        if (l.logps) hipLaunchKernelGGL(uncounted_logps_kernel, dim3(row_blocks(p.n)), dim3(256), 0, s, c.s.place, p.n, l.logps);
     }
     if (l.loss) hipLaunchKernelGGL(total_kernel, dim3(1), dim3(1024), 0, s, reinterpret_cast<const float *>(c.ws + p.row_loss), c.s.count, l.scale, l.mean, l.loss);
     return check_launch("me_head");
@@ -1630,21 +1612,14 @@ extern "C" int me_head_backward(const void *hidden, int dtype, int64_t n, int64_
     const Call c{hidden, weight, targets, rows_per_batch, batch_stride, row_stride, w_stride, ignore_index, targets_dtype,
                  static_cast<uint8_t *>(workspace), saved_rows, as_stream(stream)};
     hipStream_t s = c.stream;
-    int32_t *tgt = reinterpret_cast<int32_t *>(c.ws + p.tgt);
     uint32_t *largest = f32 ? reinterpret_cast<uint32_t *>(c.ws + p.largest) : nullptr;
-    Rows rows{};
     RowGrad *grad = reinterpret_cast<RowGrad *>(c.ws + p.grad);
+    Rows rows{};
     if (n > 0) {
-        const dim3 blocks(row_blocks(n));
-        if (targets_dtype == ME_I64)
-            hipLaunchKernelGGL(targets_kernel<int64_t>, blocks, dim3(256), 0, s, static_cast<const int64_t *>(targets), n, c.s.rows, c.s.count, tgt);
-        else
-            hipLaunchKernelGGL(targets_kernel<int32_t>, blocks, dim3(256), 0, s, static_cast<const int32_t *>(targets), n, c.s.rows, c.s.count, tgt);
-        const CoefArgs k{c.s, n, upstream, upstream_per_row != 0, reduction == ME_REDUCE_MEAN, scale / temperature, static_cast<float>(smoothing),
-                         static_cast<float>(z_loss), static_cast<double>(vocab), grad, f32 ? reinterpret_cast<float *>(c.ws + p.bound) : nullptr,
-                         largest, f32 ? static_cast<int>(ceil_div(vocab, p.piece)) : 0};
-        hipLaunchKernelGGL(coef_kernel, blocks, dim3(256), 0, s, k);
-        rows = lay_out_rows(p, c);
+        const Coefs coefs{c.s, upstream, upstream_per_row != 0, reduction == ME_REDUCE_MEAN, scale / temperature, static_cast<float>(smoothing),
+                          static_cast<float>(z_loss), static_cast<double>(vocab), grad, f32 ? reinterpret_cast<float *>(c.ws + p.bound) : nullptr,
+                          largest, f32 ? static_cast<int>(ceil_div(vocab, p.piece)) : 0};
+        rows = lay_out_rows(p, c, coefs);
         if (f32 && grad_weight) lay_out(true, hidden_layout(p, c, p.h), s);
     }
     const float k = static_cast<float>(1.44269504088896340736 / temperature);

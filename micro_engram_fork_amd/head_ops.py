@@ -63,7 +63,7 @@ def _forward(name, hidden, weight, targets, ignore_index, with_unit, out, args):
     """([out, saved] and unit where the call leaves one, the operands' arguments with the tensors that hold them)."""
     dev = require_gpu(hidden, weight, targets)
     held, operands = _operands(hidden, weight, targets, ignore_index)
-    saved = torch.empty(16 + 4 * operands[2], dtype=torch.float32, device=dev)
+    saved = torch.empty(16 + 5 * operands[2], dtype=torch.float32, device=dev)
     size = unit_elements(operands[2], operands[8], operands[3], operands[1]) if with_unit else 0
     unit = torch.empty(size, dtype=torch.float32, device=dev) if size else None
     ws, ptr, size = _workspace(operands, dev, _FORWARD if unit is None else _FORWARD_UNIT)
@@ -99,7 +99,7 @@ def _backward(hidden_shape, weight_shape, operands, like, saved, unit, upstream,
 
 
 def _fake_forward(hidden, weight, targets, with_unit, shape):
-    res = [hidden.new_empty(shape, dtype=torch.float32), hidden.new_empty((16 + 4 * targets.numel(),), dtype=torch.float32)]
+    res = [hidden.new_empty(shape, dtype=torch.float32), hidden.new_empty((16 + 5 * targets.numel(),), dtype=torch.float32)]
     size = _unit_size(hidden, weight, targets) if with_unit else 0
     return [*res, hidden.new_empty((size,), dtype=torch.float32)] if size else res
 

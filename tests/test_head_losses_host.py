@@ -55,7 +55,7 @@ def test_fake_shapes():
         out, saved = head_ops.head_logps(hidden, weight, targets, -100, 1.0, False)
         assert out.shape == (2, 3) and out.dtype is torch.float32
         loss, saved = head_ops.head_ce(hidden, weight, targets, -100, 1.0, 0.0, 0.0, 1.0, 0, False)
-        assert loss.shape == () and saved.shape == (16 + 4 * 6,)
+        assert loss.shape == () and saved.shape == (16 + 5 * 6,)
         both = head_ops.head_backward(hidden, weight, targets, saved, None, loss, -100, 1.0, False, 0.0, 0.0, 1.0, 0, True, True)
         assert [g.shape for g in both] == [hidden.shape, weight.shape] and both[1].dtype is torch.bfloat16
         one, = head_ops.head_backward(hidden, weight, targets, saved, None, loss, -100, 1.0, False, 0.0, 0.0, 1.0, 0, False, True)
