@@ -676,7 +676,7 @@ int me_distill_backward(const void *logits, int dtype, int64_t n, int64_t vocab,
  * here the logits z = hidden weight^T / temperature exist a tile at a time. Common arguments:
  *
  *   hidden      [n, dim] of dtype (ME_BF16 / ME_F32), laid out as logits' rows above; dim <= 65536,
- *               n <= 2^24
+ *               n <= 2^24, n dim <= 2^38
  *   weight      [vocab, dim] of the same dtype, rows w_stride (>= dim) elements apart; vocab <= 2^21.
  *               bf16 rows that start at multiples of 16 bytes are read where they lie, others and
  *               fp32 ones are laid out a piece at a time
@@ -688,12 +688,12 @@ int me_distill_backward(const void *logits, int dtype, int64_t n, int64_t vocab,
  *               dim rounded up to 4 values)
  *   workspace   me_head_workspace_size bytes for the same n, vocab, dim, dtype, weight and w_stride, with pass
  *               0 for a forward, 1 for me_head_backward (without unit, which needs none), 2 for a
- *               forward with unit; 16-byte aligned
+ *               forward with unit, and smoothed != 0 for a forward with smoothing; 16-byte aligned
  * bf16 products accumulate in fp32; fp32 ones are made of bf16 or fp16 parts of the operands, with the
  * accuracy of fp32 products.
  */
 int me_head_workspace_size(int64_t n, int64_t vocab, int64_t dim, int dtype, const void *weight,
-                           int64_t w_stride, int pass, size_t *bytes);
+                           int64_t w_stride, int pass, int smoothed, size_t *bytes);
 int me_head_unit_size(int64_t n, int64_t vocab, int64_t dim, int dtype, int64_t *elements);
 
 /*

@@ -1170,7 +1170,7 @@ struct Plan {
 
 int64_t round_up(int64_t x, int64_t to) { return ceil_div(x, to) * to; }
 
-Plan plan_of(int64_t n, int64_t vocab, int64_t dim, int dtype, const void *weight, int64_t w_stride, Pass pass) {
+Plan plan_of(int64_t n, int64_t vocab, int64_t dim, int dtype, const void *weight, int64_t w_stride, Pass pass, bool smoothed) {
     Plan p{};
     p.n = n, p.vocab = vocab, p.dim = dim, p.ld = round_up(dim, kSlabK);
     p.f32 = dtype == ME_F32;
@@ -1207,7 +1207,7 @@ Plan plan_of(int64_t n, int64_t vocab, int64_t dim, int dtype, const void *weigh
     if (pass != kBackward) {
         const int64_t parts = std::max<int64_t>(ceil_div(vocab, p.few ? 64 : 128) + 4, n <= kVectorRows ? kVectorGroups : 0);
         p.part = take(parts * rows * 8);
-        p.sum = take(parts * rows * 4);
+        if (smoothed) p.sum = take(parts * rows * 4);
         p.at_target = take(n * 4);
         p.row_loss = take(n * 4);
     }
@@ -1225,8 +1225,10 @@ Plan plan_of(int64_t n, int64_t vocab, int64_t dim, int dtype, const void *weigh
         p.redo = take((kHeader + n) * 4);
         p.h2 = take(rows * p.ld * 2);
         p.tgt2 = take(n * 4);
-        p.columns = take(dim * 4);
-        p.column_part = take(ceil_div(vocab, kColumnRows) * dim * 4);
+        if (smoothed) {
+            p.columns = take(dim * 4);
+            p.column_part = take(ceil_div(vocab, kColumnRows) * dim * 4);
+        }
     }
     p.bytes = at;
     return p;
@@ -1528,7 +1530,7 @@ int check_call(const void *hidden, int dtype, int64_t n, int64_t dim, int64_t pe
     ME_CHECK_ARG(tdtype == ME_I32 || tdtype == ME_I64, "targets must be int32/int64");
     ME_CHECK_ARG(n >= 0 && n <= (int64_t{1} << 24), "n must be in 0..2^24");
     ME_CHECK_ARG(dim >= 1 && dim <= 65536, "dim must be in 1..65536");
-    ME_CHECK_ARG(ceil_div(n, 256) * ceil_div(dim, 256) <= (int64_t{1} << 23), "n times dim must be at most 2^39");
+    ME_CHECK_ARG(ceil_div(n, 256) * ceil_div(dim, 256) <= (int64_t{1} << 22), "n times dim must be at most 2^38");
     ME_CHECK_ARG(vocab >= 1 && vocab <= (int64_t{1} << 21), "vocab must be in 1..2^21");
     ME_CHECK_ARG(w_stride >= dim && w_stride <= (int64_t{1} << 22), "weight rows must be dim or more elements apart, at most 2^22");
     ME_CHECK_ARG(n == 0 || (hidden && targets && per_batch >= 1), "hidden and targets are needed");
@@ -1544,9 +1546,9 @@ int check_call(const void *hidden, int dtype, int64_t n, int64_t dim, int64_t pe
 using namespace me;
 
 extern "C" int me_head_workspace_size(int64_t n, int64_t vocab, int64_t dim, int dtype, const void *weight, int64_t w_stride, int pass,
-                                      size_t *bytes) {
+                                      int smoothed, size_t *bytes) {
     ME_CHECK_ARG(bytes && n >= 0 && vocab >= 1 && dim >= 1 && pass >= 0 && pass <= 2, "bad sizes");
-    *bytes = static_cast<size_t>(plan_of(n, vocab, dim, dtype, weight, w_stride, static_cast<Pass>(pass)).bytes);
+    *bytes = static_cast<size_t>(plan_of(n, vocab, dim, dtype, weight, w_stride, static_cast<Pass>(pass), smoothed != 0).bytes);
     return ME_OK;
 }
 
@@ -1562,7 +1564,7 @@ extern "C" int me_head_logps(const void *hidden, int dtype, int64_t n, int64_t d
                              size_t workspace_bytes, void *stream) {
     const int rc = check_call(hidden, dtype, n, dim, rows_per_batch, weight, vocab, w_stride, targets, targets_dtype, temperature, saved, workspace);
     if (rc != ME_OK) return rc;
-    const Plan p = plan_of(n, vocab, dim, dtype, weight, w_stride, unit ? kLeavesUnit : kStats);
+    const Plan p = plan_of(n, vocab, dim, dtype, weight, w_stride, unit ? kLeavesUnit : kStats, false);
     ME_CHECK_ARG(workspace_bytes >= static_cast<size_t>(p.bytes), "workspace of %zu bytes, %lld are needed", workspace_bytes, static_cast<long long>(p.bytes));
     ME_CHECK_ARG(n == 0 || logps, "logps is needed");
     ME_CHECK_ARG(reinterpret_cast<uintptr_t>(unit) % 16 == 0 && (!unit || dtype == ME_BF16), "unit must be 16-byte aligned, and is for bf16");
@@ -1580,7 +1582,7 @@ extern "C" int me_head_ce(const void *hidden, int dtype, int64_t n, int64_t dim,
     ME_CHECK_ARG(reduction == ME_REDUCE_MEAN || reduction == ME_REDUCE_SUM, "reduction must be mean or sum");
     ME_CHECK_ARG(loss, "loss is needed");
     ME_CHECK_ARG(reinterpret_cast<uintptr_t>(unit) % 16 == 0 && (!unit || dtype == ME_BF16), "unit must be 16-byte aligned, and is for bf16");
-    const Plan p = plan_of(n, vocab, dim, dtype, weight, w_stride, unit ? kLeavesUnit : kStats);
+    const Plan p = plan_of(n, vocab, dim, dtype, weight, w_stride, unit ? kLeavesUnit : kStats, smoothing != 0.0);
     ME_CHECK_ARG(workspace_bytes >= static_cast<size_t>(p.bytes), "workspace of %zu bytes, %lld are needed", workspace_bytes, static_cast<long long>(p.bytes));
     const Call c{hidden, weight, targets, rows_per_batch, batch_stride, row_stride, w_stride, ignore_index, targets_dtype,
                  static_cast<uint8_t *>(workspace), saved_of(saved, n), as_stream(stream)};
@@ -1607,7 +1609,7 @@ extern "C" int me_head_backward(const void *hidden, int dtype, int64_t n, int64_
         hipLaunchKernelGGL(scale_kernel, dim3(blocks_for(n * ceil_div(dim, 4))), dim3(256), 0, as_stream(stream), a);
         return check_launch("me_head_backward");
     }
-    const Plan p = plan_of(n, vocab, dim, dtype, weight, w_stride, kBackward);
+    const Plan p = plan_of(n, vocab, dim, dtype, weight, w_stride, kBackward, false);
     ME_CHECK_ARG(workspace_bytes >= static_cast<size_t>(p.bytes), "workspace of %zu bytes, %lld are needed", workspace_bytes, static_cast<long long>(p.bytes));
     const Call c{hidden, weight, targets, rows_per_batch, batch_stride, row_stride, w_stride, ignore_index, targets_dtype,
                  static_cast<uint8_t *>(workspace), saved_rows, as_stream(stream)};

@@ -31,17 +31,17 @@ def _operands(hidden, weight, targets, ignore_index):
 
 
 @functools.lru_cache(maxsize=256)
-def workspace_bytes(n, vocab, dim, dtype, misaligned, w_stride, which):
+def workspace_bytes(n, vocab, dim, dtype, misaligned, w_stride, which, smoothed):
     """misaligned: the weight's address modulo 16."""
     size = ctypes.c_size_t(0)
-    call("me_head_workspace_size", n, vocab, dim, dtype, misaligned, w_stride, which, ctypes.byref(size))
+    call("me_head_workspace_size", n, vocab, dim, dtype, misaligned, w_stride, which, smoothed, ctypes.byref(size))
     return size.value
 
 
-def _workspace(operands, dev, which):
+def _workspace(operands, dev, which, smoothed=False):
     """(buffer, address, size)."""
     _, dtype, n, dim, _, _, _, weight, vocab, w_stride = operands[:10]
-    ws = torch.empty(workspace_bytes(n, vocab, dim, dtype, weight % 16, w_stride, which), dtype=torch.uint8, device=dev)
+    ws = torch.empty(workspace_bytes(n, vocab, dim, dtype, weight % 16, w_stride, which, smoothed), dtype=torch.uint8, device=dev)
     return ws, ws.data_ptr(), ws.numel()
 
 
@@ -66,7 +66,8 @@ def _forward(name, hidden, weight, targets, ignore_index, with_unit, out, args):
     saved = torch.empty(16 + 5 * operands[2], dtype=torch.float32, device=dev)
     size = unit_elements(operands[2], operands[8], operands[3], operands[1]) if with_unit else 0
     unit = torch.empty(size, dtype=torch.float32, device=dev) if size else None
-    ws, ptr, size = _workspace(operands, dev, _FORWARD if unit is None else _FORWARD_UNIT)
+    smoothed = len(args) > 1 and args[1] != 0.0
+    ws, ptr, size = _workspace(operands, dev, _FORWARD if unit is None else _FORWARD_UNIT, smoothed)
     call_on(dev, name, *operands, *args, out.data_ptr(), saved.data_ptr(), _p(unit), ptr, size)
     return [out, saved] if unit is None else [out, saved, unit], (held, operands)
 

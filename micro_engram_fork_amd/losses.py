@@ -426,8 +426,11 @@ def head_token_logps(hidden, weight, targets, temperature=1.0, ignore_index=IGNO
     (hidden's shape without its last dim), fp32, 0 where a row does not count. Differentiable in hidden and weight.
 
     hidden [..., dim] are the states after the decoder's last norm, weight [vocab, dim] its head, both bf16 or both fp32.
-    Memory is that of a piece of the logits' gradient (512 MiB at most for up to 131,072 rows in bf16), whatever the
-    vocabulary. Rows that do not count cost nothing and are not read."""
+    Memory, during a call: statistics of a 32nd of the bf16 logits' size, and with gradients a piece of the logits' gradient
+    (at most 1 GiB up to 262,144 bf16 rows). Heads in fp32, or whose bf16 rows do not start at multiples of 16 bytes, are
+    laid out a piece at a time as well (again at most 1 GiB). Rows that do not count cost nothing and are not read.
+    For the gradient of bf16 hidden states alone (a frozen head), larger calls make it in the forward, which saves one of
+    three products, and keep it for the backward in fp32 before its upstream factors."""
     _check_head(hidden, weight, targets)
     return _head_loss(_HEAD_LOGPS, hidden, weight, targets, int(ignore_index), _check_temperature(temperature))
 

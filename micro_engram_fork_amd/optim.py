@@ -415,9 +415,20 @@ class DenseAdamW(_DirectOptimizer):
                  stochastic_rounding=True, seed=None, capturable=False):
         if state_bits not in (32, 8):
             raise ValueError(f"[micro_engram] DenseAdamW: state_bits of {state_bits!r}: 32 or 8")
+        seed = int(torch.randint(0, 2**62, (1,)).item()) if seed is None else int(seed)
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
-                                      stochastic_rounding=stochastic_rounding, capturable=capturable))
-        self.seed = int(torch.randint(0, 2**62, (1,)).item()) if seed is None else int(seed)
+                                      stochastic_rounding=stochastic_rounding, seed=seed, capturable=capturable))
+
+    @property
+    def seed(self):
+        """Key of the rounding noise (a setting of the groups, so that it is saved and loaded with them)."""
+        return self.param_groups[0]["seed"]
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        for group in self.param_groups:  # of another AdamW, or of an older state
+            for name, value in self.defaults.items():
+                group.setdefault(name, value)
 
     def add_param_group(self, param_group):
         super().add_param_group(param_group)
@@ -436,6 +447,8 @@ class DenseAdamW(_DirectOptimizer):
             raise ValueError(f"[micro_engram] DenseAdamW: betas of {group['betas']} are out of range")
         if group["state_bits"] not in (32, 8):
             raise ValueError(f"[micro_engram] DenseAdamW: state_bits of {group['state_bits']!r}: 32 or 8")
+        if len({id(p) for p in group["params"]}) != len(group["params"]):
+            raise ValueError("[micro_engram] DenseAdamW: a parameter is there twice")
         for p in group["params"]:
             if p.dtype not in (torch.bfloat16, torch.float32):
                 raise TypeError(f"[micro_engram] DenseAdamW: parameters must be bf16 or fp32, got {p.dtype}")
@@ -454,7 +467,7 @@ class DenseAdamW(_DirectOptimizer):
 
     def load_state_dict(self, state_dict):
         """torch.optim's load, which casts floating states to their parameter's dtype: the moments are put back as they
-        were saved."""
+        were saved (for state_bits 32 in fp32: torch.optim.AdamW's own may be bf16)."""
         saved = state_dict["state"]
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         super().load_state_dict(state_dict)
@@ -467,7 +480,8 @@ class DenseAdamW(_DirectOptimizer):
                     value = torch.as_tensor(value, dtype=torch.float32).detach().reshape(())
                     self.state[p][name] = value.to(device=where, copy=True)
                 elif torch.is_tensor(value):
-                    self.state[p][name] = value.detach().to(device=p.device, copy=True).contiguous()
+                    kind = torch.float32 if group["state_bits"] == 32 and value.is_floating_point() else value.dtype
+                    self.state[p][name] = value.detach().to(device=p.device, dtype=kind, copy=True).contiguous()
         self._plans = {}
 
     _STATES = ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")
@@ -487,7 +501,7 @@ class DenseAdamW(_DirectOptimizer):
                     return None
             params = [params[i] for i in plan["at"]]
         state, grads = self.state, []
-        for p, (q, ptr, n, kind, st, m, v, ms, vs) in zip(params, members):
+        for p, (q, ptr, n, dtype, kind, st, m, v, ms, vs) in zip(params, members):
             own = p.__dict__
             g = own.get("fp32_grad")
             if g is None:
@@ -498,7 +512,7 @@ class DenseAdamW(_DirectOptimizer):
                 return None
             if (p is not q or g.dtype is not kind or not g.is_contiguous() or state.get(p) is not st or st.get("exp_avg") is not m
                     or st.get("exp_avg_sq") is not v or st.get("exp_avg_scale") is not ms or st.get("exp_avg_sq_scale") is not vs
-                    or p.data_ptr() != ptr or p.numel() != n or own.get("sparse_grad") is not None):
+                    or p.data_ptr() != ptr or p.numel() != n or p.dtype is not dtype or own.get("sparse_grad") is not None):
                 return None
             grads.append(g)
         return params, grads
@@ -514,7 +528,7 @@ class DenseAdamW(_DirectOptimizer):
             state = self.state[p]
             states = tuple(state.get(k) for k in names)
             self._check_state(p, states, eight)
-            members.append((p, p.data_ptr(), p.numel(), kind, state, *(state.get(k) for k in self._STATES)))
+            members.append((p, p.data_ptr(), p.numel(), p.dtype, kind, state, *(state.get(k) for k in self._STATES)))
             b = batches.setdefault((p.device, p.dtype, kind), {"pos": [], "ptr": [[] for _ in range(5)], "n": [], "ids": [],
                                                                "written": []})
             b["pos"].append(i)
@@ -617,7 +631,7 @@ class DenseAdamW(_DirectOptimizer):
                 ops.adamw_launch(b["device"], len(pos), b["arrays"], pointers, b["n"], steps, device_steps, b["ids"], b["dtype"],
                                  b["grad_dtype"], group["state_bits"], lr=group["lr"], betas=group["betas"],
                                  eps=group["eps"], weight_decay=group["weight_decay"],
-                                 stochastic_rounding=group["stochastic_rounding"], seed=self.seed)
+                                 stochastic_rounding=group["stochastic_rounding"], seed=group["seed"])
                 # written through raw pointers: as LazyAdamW
                 torch.autograd.graph.increment_version(b["written"])
         return loss

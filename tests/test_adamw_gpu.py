@@ -387,3 +387,18 @@ def _check_one(opt, p, before, t, bits, stream):
         _check_step(opt, [p], [before], t, bits)
     finally:
         ref.noise = noise
+
+
+def test_the_state_of_torchs_adamw_goes_on():
+    """bf16 parameters whose moments torch keeps in bf16: they go on in fp32 from there."""
+    p = torch.nn.Parameter(torch.randn(700, device=DEV).bfloat16())
+    p.grad = torch.randn(700, device=DEV).bfloat16()
+    torchs = torch.optim.AdamW([p], **HYPER)
+    torchs.step()
+    opt = DenseAdamW([p], seed=SEED)
+    opt.load_state_dict(torchs.state_dict())
+    assert opt.state[p]["exp_avg"].dtype is torch.float32
+    assert torch.equal(opt.state[p]["exp_avg"], torchs.state[p]["exp_avg"].float())
+    before = _before(opt, [p], 32)
+    opt.step()
+    _check_step(opt, [p], before, 2, 32)

@@ -74,3 +74,25 @@ def test_philox_known_answer():
     ones = np.full((1, 4), 0xFFFFFFFF, dtype=np.uint64)
     out = ref.philox(ones, (0xFFFFFFFF, 0xFFFFFFFF))[0]
     assert [int(x) for x in out] == [0x408F276D, 0x41C83B0E, 0xA20BC7C6, 0x6D5451FD]
+
+
+def test_a_parameter_twice():
+    p = _param()
+    with pytest.raises(ValueError, match="twice"):
+        with pytest.warns(UserWarning):
+            DenseAdamW([p, p])
+
+
+def test_copies_and_older_states_have_every_setting():
+    import copy
+    import pickle
+    opt = DenseAdamW([_param()], state_bits=8, seed=11)
+    for other in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        assert other.seed == 11 and other.param_groups[0]["state_bits"] == 8
+    state = torch.optim.AdamW([_param()], lr=0.25).state_dict()
+    opt.load_state_dict(state)
+    group = opt.param_groups[0]
+    assert group["lr"] == 0.25 and group["seed"] == 11 and group["state_bits"] == 8
+    saved = DenseAdamW([_param()], seed=5).state_dict()
+    opt.load_state_dict(saved)
+    assert opt.seed == 5 and opt.param_groups[0]["state_bits"] == 32

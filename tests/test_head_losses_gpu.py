@@ -459,3 +459,36 @@ def test_large_calls_for_hidden_alone_take_that_way():
     hidden, weight, targets = _inputs(700, 33_000, 2_048, BF16)
     assert head_ops._unit_size(hidden, weight, targets) == 700 * 2_048
     _check_hidden_alone(hidden, weight, targets)
+
+
+@pytest.mark.parametrize("alone", [False, True])
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("n", [12, 140])
+def test_gradients_of_likely_targets(n, dtype, alone, leaves_unit):
+    """Rows whose target carries all but 1e-3 to 1e-9: their gradients, as small as that, keep their digits (the reference's
+    bound is relative to the others' weight)."""
+    dim, vocab = 128, 700
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    weight = (torch.randn(vocab, dim, device=DEV, generator=gen) / 8).to(dtype)
+    targets = torch.randint(0, vocab, (n,), device=DEV, generator=gen)
+    row = weight[targets].float()
+    hidden = (row / row.square().sum(1, keepdim=True) * torch.linspace(14, 27, n, device=DEV)[:, None]).to(dtype)
+    h, w = hidden.requires_grad_(), weight.requires_grad_(not alone)
+    logps = losses.head_token_logps(h, w, targets)
+    up = torch.rand(n, device=DEV, generator=gen) + 0.5
+    grads = torch.autograd.grad(logps, (h,) if alone else (h, w), up)
+    want = ref.head(hidden.detach(), weight.detach(), targets, dtype, upstream=up)
+    assert float(want["hidden"][0].abs().amax(1).min()) < 1e-8
+    _close(grads[0], want["hidden"], "hidden")
+    if not alone:
+        _close(grads[1], want["weight"], "weight")
+
+
+def test_heads_of_rows_of_very_different_sizes():
+    """fp32 rows of the head from 1e-6 to 1e3 of the others: each is a part of the sums as it should be."""
+    hidden, weight, targets = _inputs(150, 600, 128, FP32)
+    weight *= torch.logspace(-6, 3, 600, device=DEV)[torch.randperm(600, device=DEV)][:, None]
+    hidden /= 300
+    _check_logps(hidden, weight, targets)
+    hidden *= torch.logspace(-4, 1, 150, device=DEV)[:, None]
+    _check_logps(hidden, weight, targets)

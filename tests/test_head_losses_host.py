@@ -71,3 +71,36 @@ def test_what_a_forward_leaves_for_the_gradient_of_hidden_alone():
         hidden, weight, targets = _args(rows=(4096,), vocab=32_000, dim=1_024)
         _, saved, unit = head_ops.head_ce(hidden, weight, targets, -100, 1.0, 0.0, 0.0, 1.0, 0, True)
         assert unit.shape == (4096 * 1024,) and unit.dtype is torch.float32
+
+
+class _Reached(Exception):
+    pass
+
+
+class _Wrapped(torch.Tensor):
+    """A tensor subclass without memory of its own, which ends a call at the first of this library's ops that it reaches."""
+
+    @staticmethod
+    def __new__(cls, inner):
+        return torch.Tensor._make_wrapper_subclass(cls, inner.shape, dtype=inner.dtype, device=inner.device)
+
+    def __init__(self, inner):
+        self.inner = inner
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        if func.namespace == "micro_engram_amd":
+            raise _Reached(func.name())
+        res = func(*(a.inner if isinstance(a, cls) else a for a in args), **(kwargs or {}))
+        return cls(res) if isinstance(res, torch.Tensor) else res
+
+
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("which", [0, 1, 2])
+@pytest.mark.parametrize("call", CALLS)
+def test_tensor_subclasses_go_through_the_ops(call, which, grad):
+    args = list(_args())
+    args[0].requires_grad_(grad)
+    args[which] = _Wrapped(args[which])
+    with pytest.raises(_Reached):
+        call(*args)
