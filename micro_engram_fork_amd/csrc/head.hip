@@ -28,10 +28,7 @@ using namespace head;
 
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr double kLn2 = 0.69314718055994530942;
-// Rows up to which the 64-row tiles are taken, and twice as many where 256-row tiles would leave CUs without one and a
-// tile's K loop is short. us, 64-row / 256-row tiles, log-probabilities alone: 262,144 x 5376, 129 rows 898 / 646, 96 rows
-// 699 / (129 rows') 646; 32,000 x 1024, 129 to 256 rows 42-44 / 57-59; 32,000 x 4096, 256 rows 109 / 112 and with
-// the hidden states' gradient 262 / 248
+// Rows up to which the tiles of few rows are taken (takes_few)
 constexpr int64_t kFew = 128;
 constexpr int64_t kPieceBytes = int64_t{1} << 30;        // of a piece's gradient, and of a piece of laid-out weights
 constexpr int kSplits = 3, kMostSplits = 16;             // of the product with W
@@ -1010,8 +1007,19 @@ __global__ __launch_bounds__(256) void ref_kernel(const Layout h, const uint16_t
     const int64_t from = h.rows[r], at = from / h.per_batch * h.batch_stride + from % h.per_batch * h.row_stride;
     const int64_t w = tgt[r] * w_stride;
     float sum = 0.f;
-    for (int64_t c = lane; c < h.dim; c += 64)
-        sum += bf16_bits_to_float(static_cast<const uint16_t *>(h.src)[at + c]) * bf16_bits_to_float(weight[w + c]);
+    const auto x = as_global(static_cast<const uint16_t *>(h.src) + at), y = as_global(weight + w);
+    for (int64_t c = lane * 8; c < h.dim; c += 512) {
+        if (c + 8 <= h.dim) {
+            const u32x4_any a = *(gmem_ptr<const u32x4_any>)(x + c), b = *(gmem_ptr<const u32x4_any>)(y + c);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                sum = fmaf(__uint_as_float(a[j] << 16), __uint_as_float(b[j] << 16), sum);
+                sum = fmaf(__uint_as_float(a[j] & 0xffff0000u), __uint_as_float(b[j] & 0xffff0000u), sum);
+            }
+        } else {
+            for (int64_t i = c; i < h.dim; ++i) sum += bf16_bits_to_float(x[i]) * bf16_bits_to_float(y[i]);
+        }
+    }
 #pragma unroll
     for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
     sum *= k;
@@ -1157,6 +1165,7 @@ enum Pass { kStats, kBackward, kLeavesUnit };  // the forward alone, the backwar
 struct Plan {
     int64_t n, rows, vocab, dim, ld;  // rows: n rounded up, at least 64; ld: dim rounded up to whole slabs
     bool f32, few, copy_w;            // copy_w: the head is laid out piece by piece
+    int tile;                         // rows of a tile
     int np, nz;                       // parts of an operand: of the head's gradient; of the logits and the hidden states' gradient
     int64_t piece;                    // columns of the vocabulary at a time
     int splits;                       // of the product with W, at most
@@ -1170,20 +1179,35 @@ struct Plan {
 
 int64_t round_up(int64_t x, int64_t to) { return ceil_div(x, to) * to; }
 
+// Whether the tiles of few rows are taken, and of 64 rows or 128. Up to 128 rows always: the read of the head is what they
+// wait for. More where 64-row tiles all find a place at once, so larger ones would leave CUs without work, and up to
+// twice as many where 256-row tiles would and a tile's K loop is short. us, few / 256-row tiles, log-probabilities
+// alone unless said otherwise:
+//   262,144 x 5376   129 rows 898 (64-row tiles) / 646; 128 rows 547 (128-row tiles, 658 with 64)
+//   32,000 x 1024    129 rows 37 / 57, 256 rows 38 / 59, 384 rows 59 / 60
+//   32,000 x 2048    256 rows 53 / -, 384 rows 88 / 81;  32,000 x 4096, 256 rows, with the hidden states' gradient 262 / 248
+//   5,000 x 512      512 rows 27 / 46
+bool takes_few(int64_t n, int64_t vocab, int64_t dim) {
+    return n <= kFew || ceil_div(n, 64) * ceil_div(vocab, kTile) <= 256 || (n <= 2 * kFew && vocab <= 65536 && dim <= 2048);
+}
+
+int few_rows(int64_t n, int64_t vocab) { return n <= 64 || ceil_div(n, 64) * ceil_div(vocab, kTile) <= 256 ? 64 : 128; }
+
 Plan plan_of(int64_t n, int64_t vocab, int64_t dim, int dtype, const void *weight, int64_t w_stride, Pass pass, bool smoothed) {
     Plan p{};
     p.n = n, p.vocab = vocab, p.dim = dim, p.ld = round_up(dim, kSlabK);
     p.f32 = dtype == ME_F32;
     p.np = p.f32 ? 3 : 1;
     p.nz = p.f32 ? 2 : 1;
-    p.few = n <= kFew || (n <= 2 * kFew && vocab <= 65536 && dim <= 2048);
+    p.few = takes_few(n, vocab, dim);
     p.copy_w = p.f32 || w_stride % 8 != 0 || reinterpret_cast<uintptr_t>(weight) % 16 != 0;
+    p.tile = p.few ? few_rows(n, vocab) : kTile;
     const int64_t rows = p.rows = round_up(std::max<int64_t>(n, 1), 64);
     int64_t piece = round_up(vocab, kTile);
     if (p.copy_w) piece = std::min(piece, std::max<int64_t>(kPieceBytes / (p.ld * 2 * p.nz) / 2048 * 2048, 2048));
     if (pass != kStats) piece = std::min(piece, std::max<int64_t>(kPieceBytes / (rows * (p.f32 ? 10 : 2)) / 2048 * 2048, 2048));
     // a launch holds fewer than 2^32 threads
-    p.piece = std::min(piece, std::max<int64_t>((int64_t{1} << 23) / ceil_div(rows, p.few ? 64 : kTile) * kTile / 2048 * 2048, 2048));
+    p.piece = std::min(piece, std::max<int64_t>((int64_t{1} << 23) / ceil_div(rows, p.tile) * kTile / 2048 * 2048, 2048));
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
         const int64_t here = at;
@@ -1214,7 +1238,7 @@ Plan plan_of(int64_t n, int64_t vocab, int64_t dim, int dtype, const void *weigh
     if (pass != kStats) {
         p.g = take(rows * p.piece * 2 * p.np);
         // at least eight slabs each; parts of few tiles are as many as fill the chip, those of many at most kSplits
-        const int64_t tiles = ceil_div(rows, p.few ? 64 : kTile) * ceil_div(dim, kTile);
+        const int64_t tiles = ceil_div(rows, p.tile) * ceil_div(dim, kTile);
         p.splits = static_cast<int>(std::max<int64_t>(std::min<int64_t>({std::max<int64_t>(256 / tiles, kSplits), kMostSplits, p.piece / kSlabK / 8}), 1));
         // reading and writing the sums at 4.8 TB/s against a piece's products at 1.25 PFLOP/s
         p.split_cost = static_cast<int>(4096 * (8.0 / 4.8e12) / (2.0 * static_cast<double>(p.piece) * (p.f32 ? 3 : 1) / 1.25e15)) + 1;
@@ -1316,10 +1340,13 @@ void multiply_large(const Gemm &g, const Epilogue &e, hipStream_t s) {
 }
 
 template <bool B_KC, int SEGS, class Epilogue>
-void multiply_few(const Gemm &g, const Epilogue &e, hipStream_t s) {
-    constexpr int kTS = 256, kRing = 3;
-    const dim3 grid(static_cast<unsigned>(workgroups(g, 64, kTS)));
-    hipLaunchKernelGGL((few_kernel<B_KC, kTS, kRing, SEGS, Epilogue>), grid, dim3(kThreads), 0, s, g, e);
+void multiply_few(int tile, const Gemm &g, const Epilogue &e, hipStream_t s) {
+    constexpr int kRing = 3;
+    const dim3 grid(static_cast<unsigned>(workgroups(g, tile, kTile)));
+    if (tile == 64)
+        hipLaunchKernelGGL((few_kernel<B_KC, 2, kTile, kRing, SEGS, Epilogue>), grid, dim3(kThreads), 0, s, g, e);
+    else
+        hipLaunchKernelGGL((few_kernel<B_KC, 4, kTile, kRing, SEGS, Epilogue>), grid, dim3(kThreads), 0, s, g, e);
 }
 
 // logits of a piece: rows x head rows
@@ -1327,7 +1354,7 @@ template <int SEGS, class Epilogue>
 void logits_of(const Plan &p, const Call &c, const Rows &rows, const Head &w, int64_t width, const Epilogue &e) {
     const Gemm g{{rows.h, p.ld, h_part(p)}, w.w, p.n, width, p.dim, rows.count, 0, 8, 1, 0};
     if (p.few)
-        multiply_few<true, SEGS>(g, e, c.stream);
+        multiply_few<true, SEGS>(p.tile, g, e, c.stream);
     else
         multiply_large<true, true, SEGS>(g, e, c.stream);
 }
@@ -1339,13 +1366,13 @@ void times_head(const Plan &p, const Call &c, const Rows &rows, const Head &w, i
     const AccumulateEpilogue e{reinterpret_cast<float *>(c.ws + p.acc), p.ld, p.rows * p.ld, v0 > 0,
                                p.f32 ? reinterpret_cast<const float *>(c.ws + p.bound) : nullptr, largest};
     if (p.few)
-        p.f32 ? multiply_few<false, 3>(g, e, c.stream) : multiply_few<false, 1>(g, e, c.stream);
+        p.f32 ? multiply_few<false, 3>(p.tile, g, e, c.stream) : multiply_few<false, 1>(p.tile, g, e, c.stream);
     else
         p.f32 ? multiply_large<true, false, 3>(g, e, c.stream) : multiply_large<true, false, 1>(g, e, c.stream);
 }
 
 Sums sums_of(const Plan &p, const Call &c) {
-    return {reinterpret_cast<float *>(c.ws + p.acc), p.ld, p.rows * p.ld, p.few ? 64 : kTile, static_cast<int>(ceil_div(p.dim, kTile)), p.splits, p.split_cost};
+    return {reinterpret_cast<float *>(c.ws + p.acc), p.ld, p.rows * p.ld, p.tile, static_cast<int>(ceil_div(p.dim, kTile)), p.splits, p.split_cost};
 }
 
 // gradient of the logits of a piece, for the products that follow

@@ -434,14 +434,14 @@ __global__ __launch_bounds__(kThreads, 1) void large_kernel(const Gemm a, const 
     epi.template run<true, kSub, kSub>(acc, t, wr * 128, ws * 128, ring, lane);
 }
 
-// ---- 64 x TS tiles for few rows: TS 128 or 256 --------------------------------------------------------------
+// ---- 64 or 128 x 256 tiles for few rows ---------------------------------------------------------------------
 // The product of a few rows is bound by the one read of its other operand. Four waves next to each other over
-// the columns, 64 rows each; whole slabs in a ring of RING slots, RING - 1 in flight while one is consumed, one
-// barrier per slab; two workgroups share a CU.
-template <bool B_KC, int TS, int RING, int SEGS, class Epilogue>
+// the columns, all 32 BR rows each; whole slabs in a ring of RING slots, RING - 1 in flight while one is consumed, one
+// barrier per slab; one workgroup per CU, 64 or 96 KB of loads in flight.
+template <bool B_KC, int BR, int TS, int RING, int SEGS, class Epilogue>
 __global__ __launch_bounds__(kThreads) void few_kernel(const Gemm a, const Epilogue epi) {
-    constexpr int kTR = 64;
-    constexpr int kBS = TS / 128, kBR = 2;                 // 32-wide subtiles of a wave
+    constexpr int kTR = 32 * BR;
+    constexpr int kBS = TS / 128, kBR = BR;                // 32-wide subtiles of a wave
     constexpr int kUnitA = kTR * kSlabBytes;
     constexpr int kSlot = (kTR + TS) * kSlabBytes;
     constexpr int kDmaA = kTR / 32, kDmaB = TS / 32;       // 1 KiB loads per wave and slab
