@@ -678,23 +678,27 @@ int me_distill_backward(const void *logits, int dtype, int64_t n, int64_t vocab,
  *   hidden      [n, dim] of dtype (ME_BF16 / ME_F32), laid out as logits' rows above; dim <= 65536,
  *               n <= 2^24, n dim <= 2^38
  *   weight      [vocab, dim] of the same dtype, rows w_stride (>= dim) elements apart; vocab <= 2^21.
- *               bf16 rows that start at multiples of 16 bytes are read where they lie, others and
- *               fp32 ones are laid out a piece at a time
+ *               bf16 rows of a multiple of 8 elements that start at multiples of 16 bytes are read
+ *               where they lie, and so are fp32 ones of few rows of hidden (me_head_unit_size); others are
+ *               laid out a piece at a time
  *   targets, ignore_index, temperature  as above; nothing of a row that does not count is read
  *   saved       [16 + 5 n] 4-byte elements (16-byte aligned): what the backward needs
- *   unit        nullable, [me_head_unit_size] fp32 (16-byte aligned), ME_BF16 alone: where the
- *               gradient of hidden alone is wanted, the forward leaves there what the backward only has to scale. A
- *               size of 0: the call is too small for that to pay (unit may still be given, n times
- *               dim rounded up to 4 values)
+ *   unit        nullable, [me_head_unit_size] fp32 (16-byte aligned): what the forward leaves for the
+ *               backward. bf16: for the gradient of hidden alone (for_weight 0), what that only has to
+ *               scale; a size of 0: the call is too small for that to pay (unit may still be given, n
+ *               times dim rounded up to 4 values). fp32, up to 384 rows (1024 where vocab is small): the logits,
+ *               for any gradient; a size of 0: unit is NULL
  *   workspace   me_head_workspace_size bytes for the same n, vocab, dim, dtype, weight and w_stride, with pass
- *               0 for a forward, 1 for me_head_backward (without unit, which needs none), 2 for a
- *               forward with unit, and smoothed != 0 for a forward with smoothing; 16-byte aligned
+ *               0 for a forward, 1 for me_head_backward without unit, 2 for a forward with unit, 3 for
+ *               me_head_backward with it (bf16: none), and smoothed != 0 for a forward with
+ *               smoothing; 16-byte aligned
  * bf16 products accumulate in fp32; fp32 ones are made of bf16 or fp16 parts of the operands, with the
- * accuracy of fp32 products.
+ * accuracy of fp32 products, also where few rows' logits are kept.
  */
 int me_head_workspace_size(int64_t n, int64_t vocab, int64_t dim, int dtype, const void *weight,
                            int64_t w_stride, int pass, int smoothed, size_t *bytes);
-int me_head_unit_size(int64_t n, int64_t vocab, int64_t dim, int dtype, int64_t *elements);
+int me_head_unit_size(int64_t n, int64_t vocab, int64_t dim, int dtype, int for_weight,
+                      int64_t *elements);
 
 /*
  * me_head_logps -- logps[r] = log softmax(z[r])[targets[r]], fp32; 0 where a row does not count.
@@ -721,7 +725,7 @@ int me_head_ce(const void *hidden, int dtype, int64_t n, int64_t dim, int64_t ro
  * me_head_backward -- gradients of me_head_logps (upstream_per_row != 0: upstream [n] fp32, the
  * log-probabilities' gradient; scale 1) or of me_head_ce (upstream: device scalar; its other
  * arguments as given there), with what that call left in saved.
- *   unit         as the forward left it, or NULL; with it grad_weight is NULL
+ *   unit         as the forward left it, or NULL; with bf16's grad_weight is NULL
  *   grad_hidden  nullable, [n, dim] contiguous, zeros in rows that do not count
  *   grad_weight  nullable, [vocab, dim] contiguous; both of dtype and 16-byte aligned
  */

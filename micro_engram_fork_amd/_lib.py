@@ -89,7 +89,7 @@ SIGNATURES = {
     "me_distill_backward": [*_LOGITS, c_ptr, c_int, c_i64, c_double, c_ptr, c_ptr, c_ptr, c_ptr, c_int, c_ptr,
                             c_ptr],
     "me_head_workspace_size": [c_i64, c_i64, c_i64, c_int, c_ptr, c_i64, c_int, c_int, ctypes.POINTER(c_size)],
-    "me_head_unit_size": [c_i64, c_i64, c_i64, c_int, ctypes.POINTER(c_i64)],
+    "me_head_unit_size": [c_i64, c_i64, c_i64, c_int, c_int, ctypes.POINTER(c_i64)],
     "me_head_logps": [*_LOGITS, c_ptr, c_i64, c_i64, *_TARGETS, c_double, c_ptr, c_ptr, c_ptr, c_ptr, c_size, c_ptr],
     "me_head_ce": [*_LOGITS, c_ptr, c_i64, c_i64, *_TARGETS, c_double, c_double, c_double, c_double, c_int, c_ptr, c_ptr,
                    c_ptr, c_ptr, c_size, c_ptr],

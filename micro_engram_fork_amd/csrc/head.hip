@@ -32,6 +32,8 @@ constexpr double kLn2 = 0.69314718055994530942;
 constexpr int64_t kFew = 128;
 constexpr int64_t kPieceBytes = int64_t{1} << 30;        // of a piece's gradient, and of a piece of laid-out weights
 constexpr int kSplits = 3, kMostSplits = 16;             // of the product with W
+// Rows of fp32 up to which logits are kept (takes_kept)
+constexpr int64_t kKeptRows = 384, kKeptMost = 1024;
 constexpr int kHeader = 16;                              // ints before the rows in `saved`: the number of them
 
 // What the forward leaves for the backward: the number of counted rows, and by counted row its source, target,
@@ -99,7 +101,7 @@ struct Coefs {
     uint32_t *largest;      // set to 0, `pieces` of them
     int pieces;
 
-    __device__ __forceinline__ void row(int64_t r, int64_t count) const {
+    __device__ __forceinline__ RowGrad of(int64_t r, int64_t count) const {
         const float lse2 = s.lse2[r], o = s.others[r];
         RowGrad g;
         g.lse2 = lse2;
@@ -113,6 +115,11 @@ struct Coefs {
             g.cb = static_cast<float>(c * e / vocab);
             g.gt = static_cast<float>(c * (more - (1.0 + more) * o + e - e / vocab));
         }
+        return g;
+    }
+    __device__ __forceinline__ void row(int64_t r, int64_t count) const {
+        const RowGrad g = of(r, count);
+        const float o = s.others[r];
         grad[r] = g;
         // a token's probability is at most that of all but the target
         if (bound) bound[r] = fmaxf(fabsf(g.ca) * (1.0001f * o) + fabsf(g.cb), fabsf(g.gt));
@@ -683,7 +690,7 @@ __device__ __forceinline__ Sum2 join(Sum2 a, Sum2 b) {
 }
 
 // ---- a few rows: one read of the head by plain products ----------------------------------------------------------
-// Up to kVectorRows rows of a forward alone: a workgroup holds them in LDS in fp32, its waves take head rows
+// Up to kVectorRows rows: a workgroup holds them in LDS in fp32, its waves take head rows
 // two at a time, each lane 16 bytes of a row at a stride of a KiB, and the 64 partial sums are added across the wave.
 // Nothing is laid out first (fp32 parts would be read and written three times over) and the rows are found by every
 // workgroup for itself: two launches for a sampled token's log-probability. Lane l keeps the logits of
@@ -700,6 +707,8 @@ struct VectorArgs {
     int t64;
     int64_t ignore;
     Saved s;
+    float *logits;  // [rows][ld] for the backward, as of kept_kernel, or null
+    int64_t ld;
     float2 *part;   // [rows][workgroups]
     float *sum;     // likewise, or null
     float *at_target;
@@ -814,8 +823,9 @@ __global__ __launch_bounds__(256) void vector_kernel(const VectorArgs a) {
             if (col < a.vocab) {
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
-                    const float v = wave_sum(acc[b][i]) * a.k;
+                    const float raw = wave_sum(acc[b][i]), v = raw * a.k;
                     if (lane == slot) {
+                        if (a.logits != nullptr && i < count) a.logits[i * a.ld + col] = raw;
                         sum[i] += v;
                         if (i < count && col == s_tgt[i])
                             a.at_target[i] = v;
@@ -844,6 +854,227 @@ __global__ __launch_bounds__(256) void vector_kernel(const VectorArgs a) {
         a.part[static_cast<int64_t>(tid) * gridDim.x + blockIdx.x] = make_float2(all.m, all.s);
         if (a.sum) a.sum[static_cast<int64_t>(tid) * gridDim.x + blockIdx.x] = total;
     }
+}
+
+// ---- few rows of fp32: their logits are kept ----------------------------------------------------------------------
+// For few rows (takes_kept) the product with the head takes the head as it lies, once, and what it gives is small beside
+// the head: the logits stay, in fp32, for the backward. So a forward and the gradients of both operands read the head
+// twice and write its gradient, which nothing can do without. Bound by these up to some 30 rows; 262,144 x 5376 (5.6 GB), us:
+//   rows   logits   product with dz   outer product
+//     12     1024             1220            1361     5.5, 4.6 and 4.1 TB/s
+//     46     1214             1740            1993
+//    128     2330             2750            3100     beyond, by matrix and vector instructions that wait for each other
+// (laid out in parts instead: 12 rows 11,500 us in all, here 3370)
+constexpr int kKeptCols = 2048;  // logits of a workgroup: 8 of a thread
+
+struct KeptArgs {
+    const float *partial;    // [split][rows][ld], null: the logits are in place
+    float *logits;           // [counted rows][ld], times k not yet
+    int64_t ld, split_stride, vocab;
+    int tile_rows, col_tiles, most, cost;  // of the splits
+    Saved s;
+    float2 *part;            // by (row, workgroup of a row)
+    float *sum, *at_target;
+    float k;
+};
+
+// Adds the product's splits and takes the statistics that the tiles of other calls take as they leave the matrix cores
+__global__ __launch_bounds__(256) void kept_kernel(const KeptArgs a) {
+    __shared__ Sum2 s_all[4];
+    __shared__ float s_sum[4];
+    const int64_t r = blockIdx.y;
+    const int count = *a.s.count;
+    if (r >= count) return;
+    const int tid = threadIdx.x;
+    const int64_t target = a.s.tgt[r];
+    const int splits = a.partial == nullptr ? 0 : splits_for(static_cast<int>(ceil_div(count, a.tile_rows)) * a.col_tiles, a.most, a.cost);
+    float z[8], m = -__builtin_inff(), total = 0.f;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+        const int64_t c = static_cast<int64_t>(blockIdx.x) * kKeptCols + b * 1024 + tid * 4;
+        f32x4_v v = {0.f, 0.f, 0.f, 0.f};
+        if (c < a.ld) {
+            const auto at = as_global(reinterpret_cast<f32x4_v *>(a.logits + r * a.ld + c));
+            if (splits == 0) v = *at;
+            for (int i = 0; i < splits; ++i) v += *as_global(reinterpret_cast<const f32x4_v *>(a.partial + i * a.split_stride + r * a.ld + c));
+            if (splits > 0) *at = v;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const bool there = c + e < a.vocab;
+            const float x = v[e] * a.k;
+            total += there ? x : 0.f;
+            if (there && c + e == target) a.at_target[r] = x;
+            z[4 * b + e] = there && c + e != target ? v[e] : -__builtin_inff();
+            m = fmaxf(m, z[4 * b + e]);
+        }
+    }
+    m *= a.k;
+    const float shift = m == -__builtin_inff() ? 0.f : m;
+    Sum2 all = {m, 0.f};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) all.s += __builtin_amdgcn_exp2f(fmaf(z[i], a.k, -shift));
+#pragma unroll
+    for (int d = 32; d; d >>= 1) {
+        all = join(all, {__shfl_xor(all.m, d), __shfl_xor(all.s, d)});
+        total += __shfl_xor(total, d);
+    }
+    if ((tid & 63) == 0) s_all[tid >> 6] = all, s_sum[tid >> 6] = total;
+    __syncthreads();
+    if (tid) return;
+    for (int w = 1; w < 4; ++w) all = join(all, s_all[w]), total += s_sum[w];
+    const int64_t at = r * gridDim.x + blockIdx.x;
+    a.part[at] = make_float2(all.m, all.s);
+    if (a.sum) a.sum[at] = total;
+}
+
+// Sixteen rows' values of a column as the product of the head's gradient reads them: by block of 16 rows and column
+// three bf16 parts of 16 values each, 96 bytes
+constexpr int kOuterRows = 16, kOuterBytes = 3 * kOuterRows * 2;
+
+__device__ __forceinline__ void store_parts(uint8_t *to, const float (&x)[kOuterRows]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        floatx8 v;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = x[8 * h + i];
+        const Parts parts(v);
+#pragma unroll
+        for (int p = 0; p < 3; ++p) *as_global(reinterpret_cast<bf16x8 *>(to + p * kOuterRows * 2 + h * 16)) = parts.p[p];
+    }
+}
+
+// The logits' gradient from them: [counted rows][ld] for the product with the head, zeros past the vocabulary up
+// to whole chunks; and in parts for the product with the hidden states, zeros past the rows
+struct KeptGradArgs {
+    Coefs k;
+    const float *logits;
+    float *out;       // null: not wanted
+    uint8_t *parts;   // [block of rows][vocab], likewise
+    int64_t ld, vocab;
+    float scale;
+};
+
+__global__ __launch_bounds__(256) void kept_grad_kernel(const KeptGradArgs a) {
+    __shared__ RowGrad s_grad[kOuterRows];
+    __shared__ int s_tgt[kOuterRows];
+    const int64_t r0 = static_cast<int64_t>(blockIdx.y) * kOuterRows;
+    const int count = *a.k.s.count;
+    const int rows = static_cast<int>(min(count - r0, int64_t{kOuterRows}));
+    if (rows <= 0) return;
+    const int tid = threadIdx.x;
+    if (tid < rows) s_grad[tid] = a.k.of(r0 + tid, count), s_tgt[tid] = a.k.s.tgt[r0 + tid];
+    __syncthreads();
+    const int64_t c = static_cast<int64_t>(blockIdx.x) * 256 + tid;
+    if (c >= a.ld) return;
+    float v[kOuterRows];
+#pragma unroll
+    for (int r = 0; r < kOuterRows; ++r) v[r] = r < rows ? a.logits[(r0 + r) * a.ld + c] : 0.f;
+#pragma unroll
+    for (int r = 0; r < kOuterRows; ++r) {
+        if (r >= rows) break;
+        const RowGrad g = s_grad[r];
+        v[r] = fmaf(__builtin_amdgcn_exp2f(fmaf(v[r], a.scale, -g.lse2)), g.ca, -g.cb);
+        if (c == s_tgt[r]) v[r] = g.gt;
+        if (c >= a.vocab) v[r] = 0.f;
+        if (a.out != nullptr) a.out[(r0 + r) * a.ld + c] = v[r];
+    }
+    if (a.parts != nullptr && c < a.vocab) store_parts(a.parts + (blockIdx.y * a.vocab + c) * kOuterBytes, v);
+}
+
+// The hidden states in the same way: [block of rows][dim]
+__global__ __launch_bounds__(256) void hidden_parts_kernel(const Layout h, uint8_t *parts) {
+    const int64_t r0 = static_cast<int64_t>(blockIdx.y) * kOuterRows, c = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    const int count = *h.count;
+    if (r0 >= count || c >= h.dim) return;
+    float v[kOuterRows];
+#pragma unroll
+    for (int r = 0; r < kOuterRows; ++r) {
+        v[r] = 0.f;
+        if (r0 + r < count) {
+            const int64_t from = h.rows[r0 + r];
+            v[r] = static_cast<const float *>(h.src)[from / h.per_batch * h.batch_stride + from % h.per_batch * h.row_stride + c];
+        }
+    }
+    store_parts(parts + (blockIdx.y * h.dim + c) * kOuterBytes, v);
+}
+
+// The head's gradient from few rows: an outer product of short reduction, bound by the write of the result. Tiles of
+// 128 x 128, four waves of 64 x 64; a lane's fragment of a k-step is 16 bytes for each part, straight from L2 without
+// LDS, the next step's in flight. A lane's results are one column of the gradient: whole lines of 32 columns leave by each
+// store, wherever the rows start.
+struct OuterArgs {
+    const uint8_t *dz, *h;  // as above
+    const int32_t *count;
+    int64_t vocab, dim;
+    float *out;             // [vocab][dim]
+    int col_tiles;
+};
+
+__global__ __launch_bounds__(256, 2) void outer_kernel(const OuterArgs a) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    // each XCD takes a run of tiles, whose operands stay in its L2
+    const int tile = static_cast<int>(blockIdx.x % kXcds * (gridDim.x / kXcds) + blockIdx.x / kXcds);
+    const int64_t v0 = static_cast<int64_t>(tile / a.col_tiles) * 128 + (wave >> 1) * 64;
+    const int64_t d0 = static_cast<int64_t>(tile % a.col_tiles) * 128 + (wave & 1) * 64;
+    if (v0 >= a.vocab || d0 >= a.dim) return;
+    const int blocks = (*a.count + kOuterRows - 1) / kOuterRows;
+    uint32_t vo[2], ho[2];  // columns read: past the last one, the last
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+        const uint32_t half = static_cast<uint32_t>(lane >> 5) * 16u;
+        vo[x] = static_cast<uint32_t>(min(v0 + 32 * x + (lane & 31), a.vocab - 1)) * kOuterBytes + half;
+        ho[x] = static_cast<uint32_t>(min(d0 + 32 * x + (lane & 31), a.dim - 1)) * kOuterBytes + half;
+    }
+    floatx16 acc[2][2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[x][y][e] = 0.f;
+    struct Step {
+        Parts v[2], h[2];
+    };
+    auto load = [&](int b, Step &s) {
+        const uint8_t *dz = a.dz + b * a.vocab * kOuterBytes, *h = a.h + b * a.dim * kOuterBytes;
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int p = 0; p < 3; ++p) {
+                s.v[x].p[p] = *as_global(reinterpret_cast<const bf16x8 *>(dz + vo[x] + p * kOuterRows * 2));
+                s.h[x].p[p] = *as_global(reinterpret_cast<const bf16x8 *>(h + ho[x] + p * kOuterRows * 2));
+            }
+    };
+    auto step = [&](const Step &s) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) acc[x][y] = multiply(s.v[x], s.h[y], acc[x][y]);
+    };
+    Step s0, s1;
+    if (blocks > 0) load(0, s0);
+    for (int b = 0; b < blocks; b += 2) {
+        if (b + 1 < blocks) load(b + 1, s1);
+        step(s0);
+        if (b + 1 >= blocks) break;
+        if (b + 2 < blocks) load(b + 2, s0);
+        step(s1);
+    }
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int64_t v = v0 + 32 * x + 8 * g + 4 * (lane >> 5) + e;
+                if (v >= a.vocab) continue;
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    const int64_t d = d0 + 32 * y + (lane & 31);
+                    if (d < a.dim) as_global(a.out)[v * a.dim + d] = acc[x][y][4 * g + e];
+                }
+            }
 }
 
 // Sums of the products with the head: [split][rows][ld], in as many splits as the product took for the rows
@@ -1160,7 +1391,8 @@ __global__ __launch_bounds__(256) void scale_kernel(const ScaleArgs a) {
 }
 
 // ---- plan: sizes and places in the workspace ---------------------------------------------------------------------
-enum Pass { kStats, kBackward, kLeavesUnit };  // the forward alone, the backward, the forward that leaves D
+// the forward alone, the backward, the forward that leaves D or its logits, the backward that has them
+enum Pass { kStats, kBackward, kLeavesUnit, kHasUnit };
 
 struct Plan {
     int64_t n, rows, vocab, dim, ld;  // rows: n rounded up, at least 64; ld: dim rounded up to whole slabs
@@ -1179,6 +1411,10 @@ struct Plan {
 
 int64_t round_up(int64_t x, int64_t to) { return ceil_div(x, to) * to; }
 
+// Columns of an array whose rows are read a few hundred bytes at a time, many rows together: an odd number of lines, or the
+// rows' pieces would share few of the memory's channels (a vocabulary is often a multiple of a power of two)
+int64_t odd_lines(int64_t columns) { return (ceil_div(columns, 64) | 1) * 64; }
+
 // Whether the tiles of few rows are taken, and of 64 rows or 128. Up to 128 rows always: the read of the head is what they
 // wait for. More where 64-row tiles all find a place at once, so larger ones would leave CUs without work, and up to
 // twice as many where 256-row tiles would and a tile's K loop is short. us, few / 256-row tiles, log-probabilities
@@ -1187,8 +1423,71 @@ int64_t round_up(int64_t x, int64_t to) { return ceil_div(x, to) * to; }
 //   32,000 x 1024    129 rows 37 / 57, 256 rows 38 / 59, 384 rows 59 / 60
 //   32,000 x 2048    256 rows 53 / -, 384 rows 88 / 81;  32,000 x 4096, 256 rows, with the hidden states' gradient 262 / 248
 //   5,000 x 512      512 rows 27 / 46
-bool takes_few(int64_t n, int64_t vocab, int64_t dim) {
-    return n <= kFew || ceil_div(n, 64) * ceil_div(vocab, kTile) <= 256 || (n <= 2 * kFew && vocab <= 65536 && dim <= 2048);
+// fp32: where 64-row tiles all find a place at once.
+bool takes_few(int64_t n, int64_t vocab, int64_t dim, bool f32) {
+    return ceil_div(n, 64) * ceil_div(vocab, kTile) <= 256 || (!f32 && (n <= kFew || (n <= 2 * kFew && vocab <= 65536 && dim <= 2048)));
+}
+
+// Whether a call goes by kept logits (a forward alone too, in its workspace): few rows, and more of them where 256-row
+// tiles of parts would leave CUs without work. Parts / kept logits, us, the gradient of the hidden states:
+//   262,144 x 5376   257 rows 15,663 / 11,401, 384 rows 16,503 / 14,612, 512 rows 17,476 / 19,244
+//   32,000 x 1024    257 rows 512 / 328, 512 rows 547 / 510 (250 tiles), 768 rows 738 / 781
+//   10,113 x 5376    384 rows 862 / 612, 768 rows 1165 / 1116;  3,423 x 4608, 768 rows 557 / 471
+bool takes_kept(int64_t n, int64_t vocab, int dtype) {
+    return dtype == ME_F32 && n >= 1 && (n <= kKeptRows || (n <= kKeptMost && ceil_div(n, kTile) * ceil_div(vocab, kTile) <= 256));
+}
+
+int64_t kept_ld(int64_t vocab) { return odd_lines(vocab); }
+
+// Parts of a reduction over `slabs` slabs that `tiles` tiles take to fill the chip, at least four slabs each
+int most_splits(int64_t tiles, int64_t slabs) {
+    return static_cast<int>(std::max<int64_t>(std::min<int64_t>({std::max<int64_t>(256 / tiles, kSplits), 64, slabs / 4}), 1));
+}
+
+// What a call by kept logits needs
+struct KeptPlan {
+    int64_t n, vocab, dim, ld, h_ld, row_tiles;
+    int tile, piece;                       // rows of a tile; Loader's PIECE of the head
+    int logit_splits, logit_cost, splits, split_cost;
+    int64_t h, logits, partial, part, sum, at_target, row_loss, dz, acc, dz_parts, h_parts, bytes;
+};
+
+KeptPlan kept_plan_of(int64_t n, int64_t vocab, int64_t dim, const void *weight, int64_t w_stride, Pass pass, bool smoothed) {
+    KeptPlan p{};
+    p.n = n, p.vocab = vocab, p.dim = dim, p.ld = kept_ld(vocab), p.h_ld = round_up(dim, 32);
+    // the logits' tiles: two workgroups to a CU; the others': one
+    p.tile = pass != kHasUnit ? (n <= 32 ? 32 : 64) : static_cast<int>(round_up(ceil_div(n, ceil_div(n, 128)), 32));
+    p.row_tiles = ceil_div(n, p.tile);
+    p.piece = dim % 4 == 0 && w_stride % 4 == 0 && reinterpret_cast<uintptr_t>(weight) % 16 == 0 ? 16 : 4;
+    int64_t at = 0;
+    auto take = [&](int64_t bytes) {
+        const int64_t here = at;
+        at += round_up(bytes, 256);
+        return here;
+    };
+    if (pass != kHasUnit) {
+        const int64_t tiles = p.row_tiles * ceil_div(vocab, kTile);
+        // the sums' bytes against the head's
+        p.logit_splits = tiles > 512 ? 1 : most_splits(tiles, ceil_div(dim, 32));
+        p.logit_cost = static_cast<int>(4096 * 2 * n / dim) + 1;
+        p.h = take(n * p.h_ld * 4);
+        if (pass == kStats) p.logits = take(n * p.ld * 4);
+        if (p.logit_splits > 1) p.partial = take(p.logit_splits * n * p.ld * 4);
+        const int64_t parts = std::max<int64_t>(ceil_div(p.ld, kKeptCols), n <= kVectorRows ? kVectorGroups : 0);
+        p.part = take(parts * n * 8);
+        if (smoothed) p.sum = take(parts * n * 4);
+        p.at_target = take(n * 4);
+        p.row_loss = take(n * 4);
+    } else {
+        p.splits = most_splits(p.row_tiles * ceil_div(dim, kTile), ceil_div(vocab, 32));
+        p.split_cost = static_cast<int>(4096 * 2 * n / vocab) + 1;
+        p.dz = take(n * p.ld * 4);
+        p.acc = take(p.splits * n * p.h_ld * 4);
+        p.dz_parts = take(ceil_div(n, kOuterRows) * vocab * kOuterBytes);
+        p.h_parts = take(ceil_div(n, kOuterRows) * dim * kOuterBytes);
+    }
+    p.bytes = at;
+    return p;
 }
 
 int few_rows(int64_t n, int64_t vocab) { return n <= 64 || ceil_div(n, 64) * ceil_div(vocab, kTile) <= 256 ? 64 : 128; }
@@ -1199,8 +1498,8 @@ Plan plan_of(int64_t n, int64_t vocab, int64_t dim, int dtype, const void *weigh
     p.f32 = dtype == ME_F32;
     p.np = p.f32 ? 3 : 1;
     p.nz = p.f32 ? 2 : 1;
-    p.few = takes_few(n, vocab, dim);
-    p.copy_w = p.f32 || w_stride % 8 != 0 || reinterpret_cast<uintptr_t>(weight) % 16 != 0;
+    p.few = takes_few(n, vocab, dim, p.f32);
+    p.copy_w = p.f32 || dim % 8 != 0 || w_stride % 8 != 0 || reinterpret_cast<uintptr_t>(weight) % 16 != 0;
     p.tile = p.few ? few_rows(n, vocab) : kTile;
     const int64_t rows = p.rows = round_up(std::max<int64_t>(n, 1), 64);
     int64_t piece = round_up(vocab, kTile);
@@ -1341,12 +1640,35 @@ void multiply_large(const Gemm &g, const Epilogue &e, hipStream_t s) {
 
 template <bool B_KC, int SEGS, class Epilogue>
 void multiply_few(int tile, const Gemm &g, const Epilogue &e, hipStream_t s) {
-    constexpr int kRing = 3;
     const dim3 grid(static_cast<unsigned>(workgroups(g, tile, kTile)));
-    if (tile == 64)
-        hipLaunchKernelGGL((few_kernel<B_KC, 2, kTile, kRing, SEGS, Epilogue>), grid, dim3(kThreads), 0, s, g, e);
-    else
-        hipLaunchKernelGGL((few_kernel<B_KC, 4, kTile, kRing, SEGS, Epilogue>), grid, dim3(kThreads), 0, s, g, e);
+    if constexpr (SEGS == 1) {  // parts: 64 rows alone (takes_few)
+        if (tile == 128) {
+            hipLaunchKernelGGL((few_kernel<B_KC, 4, 1, 16, Epilogue>), grid, dim3(kThreads), 0, s, g, e);
+            return;
+        }
+    }
+    hipLaunchKernelGGL((few_kernel<B_KC, 2, SEGS, 16, Epilogue>), grid, dim3(kThreads), 0, s, g, e);
+}
+
+// fp32 as it lies
+template <bool B_KC, int PIECE>
+void multiply_kept(int tile, const Gemm &g, const AccumulateEpilogue &e, hipStream_t s) {
+    const dim3 grid(static_cast<unsigned>(workgroups(g, tile, kTile)));
+    if (tile == 32)
+        hipLaunchKernelGGL((few_kernel<B_KC, 1, 0, PIECE, AccumulateEpilogue>), grid, dim3(kThreads), 0, s, g, e);
+    else if (B_KC || tile == 64)
+        hipLaunchKernelGGL((few_kernel<B_KC, 2, 0, PIECE, AccumulateEpilogue>), grid, dim3(kThreads), 0, s, g, e);
+    else if constexpr (!B_KC) {
+        if (tile == 96)
+            hipLaunchKernelGGL((few_kernel<false, 3, 0, PIECE, AccumulateEpilogue>), grid, dim3(kThreads), 0, s, g, e);
+        else
+            hipLaunchKernelGGL((few_kernel<false, 4, 0, PIECE, AccumulateEpilogue>), grid, dim3(kThreads), 0, s, g, e);
+    }
+}
+
+template <bool B_KC>
+void multiply_kept(const KeptPlan &p, const Gemm &g, const AccumulateEpilogue &e, hipStream_t s) {
+    p.piece == 16 ? multiply_kept<B_KC, 16>(p.tile, g, e, s) : multiply_kept<B_KC, 4>(p.tile, g, e, s);
 }
 
 // logits of a piece: rows x head rows
@@ -1504,20 +1826,69 @@ void vector_rows(const VectorArgs &a, int rows, unsigned groups, size_t lds, hip
         hipLaunchKernelGGL(vector_kernel<8>, dim3(groups), dim3(256), lds, s, a);
 }
 
+void forward_kept(const KeptPlan &p, const Call &c, const Loss &l) {
+    hipStream_t s = c.stream;
+    // rows gathered and padded to whole slabs: copied as pairs of 16-bit values
+    const Layout rows{c.hidden, c.per_batch, 2 * c.batch_stride, 2 * c.row_stride, c.s.rows, c.s.count, p.n, 2 * p.dim, 2 * p.h_ld, 0, c.ws + p.h};
+    lay_out(false, rows, s);
+    float *logits = l.unit ? l.unit : reinterpret_cast<float *>(c.ws + p.logits);
+    float *partial = p.logit_splits > 1 ? reinterpret_cast<float *>(c.ws + p.partial) : nullptr;
+    const Gemm g{{c.ws + p.h, p.h_ld, 0}, {static_cast<const uint8_t *>(c.weight), c.w_stride, 0}, p.n, p.vocab, p.dim, c.s.count, 0, 8, p.logit_splits, p.logit_cost};
+    multiply_kept<true>(p, g, AccumulateEpilogue{partial ? partial : logits, p.ld, p.n * p.ld, 0, nullptr, nullptr}, s);
+    const int groups = static_cast<int>(ceil_div(p.ld, kKeptCols));
+    KeptArgs a{};
+    a.partial = partial, a.logits = logits, a.ld = p.ld, a.split_stride = p.n * p.ld, a.vocab = p.vocab;
+    a.tile_rows = p.tile, a.col_tiles = static_cast<int>(ceil_div(p.vocab, kTile)), a.most = p.logit_splits, a.cost = p.logit_cost;
+    a.s = c.s;
+    a.part = reinterpret_cast<float2 *>(c.ws + p.part);
+    a.sum = l.smoothing != 0.0 ? reinterpret_cast<float *>(c.ws + p.sum) : nullptr;
+    a.at_target = reinterpret_cast<float *>(c.ws + p.at_target);
+    a.k = static_cast<float>(1.44269504088896340736 / l.temperature);
+    hipLaunchKernelGGL(kept_kernel, dim3(static_cast<unsigned>(groups), static_cast<unsigned>(p.n)), dim3(256), 0, s, a);
+    FinishArgs f{};
+    f.part = a.part, f.sum = a.sum, f.at_target = a.at_target, f.part_stride = 1, f.row_stride = groups, f.parts = groups;
+    f.n = p.n, f.vocab = p.vocab, f.s = c.s, f.logps = l.logps, f.uncounted = 1;
+    f.row_loss = l.loss ? reinterpret_cast<float *>(c.ws + p.row_loss) : nullptr;
+    f.smoothing = static_cast<float>(l.smoothing), f.z_loss = static_cast<float>(l.z_loss);
+    hipLaunchKernelGGL(finish_kernel<true>, dim3(static_cast<unsigned>(p.n)), dim3(256), 0, s, f);
+}
+
+void backward_kept(const KeptPlan &p, const Call &c, const Coefs &k, const float *logits, double temperature, void *grad_hidden, void *grad_weight) {
+    hipStream_t s = c.stream;
+    float *dz = reinterpret_cast<float *>(c.ws + p.dz);
+    const unsigned row_blocks = static_cast<unsigned>(ceil_div(p.n, kOuterRows));
+    const KeptGradArgs a{k, logits, grad_hidden ? dz : nullptr, grad_weight ? c.ws + p.dz_parts : nullptr, p.ld, p.vocab, static_cast<float>(1.44269504088896340736 / temperature)};
+    hipLaunchKernelGGL(kept_grad_kernel, dim3(static_cast<unsigned>(ceil_div(p.ld, 256)), row_blocks), dim3(256), 0, s, a);
+    if (grad_hidden) {
+        const Gemm g{{c.ws + p.dz, p.ld, 0}, {static_cast<const uint8_t *>(c.weight), c.w_stride, 0}, p.n, p.dim, p.vocab, c.s.count, 0, 8, p.splits, p.split_cost};
+        float *acc = reinterpret_cast<float *>(c.ws + p.acc);
+        multiply_kept<false>(p, g, AccumulateEpilogue{acc, p.h_ld, p.n * p.h_ld, 0, nullptr, nullptr}, s);
+        const Sums sums{acc, p.h_ld, p.n * p.h_ld, p.tile, static_cast<int>(ceil_div(p.dim, kTile)), p.splits, p.split_cost};
+        hipLaunchKernelGGL(hidden_kernel<true>, dim3(blocks_for(p.n * ceil_div(p.dim, 4))), dim3(256), 0, s, sums, c.s.place, c.s.count, p.n, p.dim, grad_hidden);
+    }
+    if (grad_weight) {
+        const Layout h{c.hidden, c.per_batch, c.batch_stride, c.row_stride, c.s.rows, c.s.count, p.n, p.dim};
+        hipLaunchKernelGGL(hidden_parts_kernel, dim3(static_cast<unsigned>(ceil_div(p.dim, 256)), row_blocks), dim3(256), 0, s, h, c.ws + p.h_parts);
+        const OuterArgs o{c.ws + p.dz_parts, c.ws + p.h_parts, c.s.count, p.vocab, p.dim, static_cast<float *>(grad_weight), static_cast<int>(ceil_div(p.dim, 128))};
+        hipLaunchKernelGGL(outer_kernel, dim3(static_cast<unsigned>(round_up(o.col_tiles * ceil_div(p.vocab, 128), kXcds))), dim3(256), 0, s, o);
+    }
+}
+
 // Whether a forward goes the way of few rows by plain products, and the LDS it takes for its rows. fp32 alone: bf16 rows
 // read the head once on the matrix cores as well, at 5.9 TB/s (262,144 x 5376, 1 to 16 rows, 480 us; by plain
 // products 718 for one row, 810 for two).
-bool takes_vectors(const Plan &p, int &rows, size_t &lds) {
-    rows = p.n <= 1 ? 1 : p.n <= 2 ? 2 : p.n <= 4 ? 4 : 8;
-    lds = static_cast<size_t>(rows) * round_up(p.dim, 256) * 4;
-    return p.f32 && p.n >= 1 && p.n <= kVectorRows && lds <= kVectorLds;
+bool takes_vectors(int64_t n, int64_t dim, int &rows, size_t &lds) {
+    rows = n <= 1 ? 1 : n <= 2 ? 2 : n <= 4 ? 4 : 8;
+    lds = static_cast<size_t>(rows) * round_up(dim, 256) * 4;
+    return n <= kVectorRows && lds <= kVectorLds;
 }
 
-void forward_vectors(const Plan &p, const Call &c, const Loss &l, int rows, size_t lds) {
+void forward_vectors(const KeptPlan &p, const Call &c, const Loss &l, int rows, size_t lds) {
     const unsigned groups = static_cast<unsigned>(std::min<int64_t>(ceil_div(p.vocab, 8), kVectorGroups));
     VectorArgs a{};
-    a.h = hidden_layout(p, c, p.z);
+    a.h = {c.hidden, c.per_batch, c.batch_stride, c.row_stride, nullptr, nullptr, p.n, p.dim};
     a.weight = static_cast<const float *>(c.weight), a.w_stride = c.w_stride, a.vocab = p.vocab, a.targets = c.targets, a.t64 = c.tdtype == ME_I64, a.ignore = c.ignore, a.s = c.s;
+    a.logits = l.unit, a.ld = p.ld;
     a.part = reinterpret_cast<float2 *>(c.ws + p.part);
     a.sum = l.smoothing != 0.0 ? reinterpret_cast<float *>(c.ws + p.sum) : nullptr;
     a.at_target = reinterpret_cast<float *>(c.ws + p.at_target);
@@ -1531,23 +1902,33 @@ void forward_vectors(const Plan &p, const Call &c, const Loss &l, int rows, size
     hipLaunchKernelGGL(finish_kernel<true>, dim3(static_cast<unsigned>(p.n)), dim3(256), 0, c.stream, f);
 }
 
-int forward(const Plan &p, const Call &c, const Loss &l) {
+int forward(int64_t n, int64_t vocab, int64_t dim, int dtype, const Call &c, const Loss &l, size_t there) {
     hipStream_t s = c.stream;
+    const Pass pass = l.unit ? kLeavesUnit : kStats;
+    const bool smoothed = l.smoothing != 0.0, kept = takes_kept(n, vocab, dtype);
+    KeptPlan q{};
+    Plan p{};
+    if (kept)
+        q = kept_plan_of(n, vocab, dim, c.weight, c.w_stride, pass, smoothed);
+    else
+        p = plan_of(n, vocab, dim, dtype, c.weight, c.w_stride, pass, smoothed);
+    const int64_t needed = kept ? q.bytes : p.bytes, row_loss = kept ? q.row_loss : p.row_loss;
+    ME_CHECK_ARG(there >= static_cast<size_t>(needed), "workspace of %zu bytes, %lld are needed", there, static_cast<long long>(needed));
     int rows;
     size_t lds;
-    if (!l.unit && takes_vectors(p, rows, lds)) {
-        forward_vectors(p, c, l, rows, lds);
-        if (l.loss) hipLaunchKernelGGL(total_kernel, dim3(1), dim3(1024), 0, s, reinterpret_cast<const float *>(c.ws + p.row_loss), c.s.count, l.scale, l.mean, l.loss);
-        return check_launch("me_head");
+    if (kept && takes_vectors(n, dim, rows, lds)) {
+        forward_vectors(q, c, l, rows, lds);
+    } else {
+        if (c.tdtype == ME_I64)
+            hipLaunchKernelGGL(index_kernel<int64_t>, dim3(1), dim3(kIndexThreads), 0, s, static_cast<const int64_t *>(c.targets), n, c.ignore, vocab, c.s);
+        else
+            hipLaunchKernelGGL(index_kernel<int32_t>, dim3(1), dim3(kIndexThreads), 0, s, static_cast<const int32_t *>(c.targets), n, c.ignore, vocab, c.s);
+        if (kept)
+            forward_kept(q, c, l);
+        else if (n > 0)
+            p.f32 ? forward_rows<true>(p, c, l) : forward_rows<false>(p, c, l);
     }
-    if (c.tdtype == ME_I64)
-        hipLaunchKernelGGL(index_kernel<int64_t>, dim3(1), dim3(kIndexThreads), 0, s, static_cast<const int64_t *>(c.targets), p.n, c.ignore, p.vocab, c.s);
-    else
-        hipLaunchKernelGGL(index_kernel<int32_t>, dim3(1), dim3(kIndexThreads), 0, s, static_cast<const int32_t *>(c.targets), p.n, c.ignore, p.vocab, c.s);
-    if (p.n > 0) {
-        p.f32 ? forward_rows<true>(p, c, l) : forward_rows<false>(p, c, l);
-    }
-    if (l.loss) hipLaunchKernelGGL(total_kernel, dim3(1), dim3(1024), 0, s, reinterpret_cast<const float *>(c.ws + p.row_loss), c.s.count, l.scale, l.mean, l.loss);
+    if (l.loss) hipLaunchKernelGGL(total_kernel, dim3(1), dim3(1024), 0, s, reinterpret_cast<const float *>(c.ws + row_loss), c.s.count, l.scale, l.mean, l.loss);
     return check_launch("me_head");
 }
 
@@ -1574,14 +1955,21 @@ using namespace me;
 
 extern "C" int me_head_workspace_size(int64_t n, int64_t vocab, int64_t dim, int dtype, const void *weight, int64_t w_stride, int pass,
                                       int smoothed, size_t *bytes) {
-    ME_CHECK_ARG(bytes && n >= 0 && vocab >= 1 && dim >= 1 && pass >= 0 && pass <= 2, "bad sizes");
-    *bytes = static_cast<size_t>(plan_of(n, vocab, dim, dtype, weight, w_stride, static_cast<Pass>(pass), smoothed != 0).bytes);
+    ME_CHECK_ARG(bytes && n >= 0 && vocab >= 1 && dim >= 1 && pass >= kStats && pass <= kHasUnit, "bad sizes");
+    if (takes_kept(n, vocab, dtype) && pass != kBackward) {
+        *bytes = static_cast<size_t>(kept_plan_of(n, vocab, dim, weight, w_stride, static_cast<Pass>(pass), smoothed != 0).bytes);
+        return ME_OK;
+    }
+    *bytes = pass == kHasUnit ? 0 : static_cast<size_t>(plan_of(n, vocab, dim, dtype, weight, w_stride, static_cast<Pass>(pass), smoothed != 0).bytes);
     return ME_OK;
 }
 
-extern "C" int me_head_unit_size(int64_t n, int64_t vocab, int64_t dim, int dtype, int64_t *elements) {
+extern "C" int me_head_unit_size(int64_t n, int64_t vocab, int64_t dim, int dtype, int for_weight, int64_t *elements) {
     ME_CHECK_ARG(elements && n >= 0 && vocab >= 1 && dim >= 1, "bad sizes");
-    *elements = n > 0 && leaves_unit(n, vocab, dim, dtype) ? n * ceil_div(dim, 4) * 4 : 0;
+    if (takes_kept(n, vocab, dtype))
+        *elements = n * kept_ld(vocab);
+    else
+        *elements = n > 0 && !for_weight && leaves_unit(n, vocab, dim, dtype) ? n * ceil_div(dim, 4) * 4 : 0;
     return ME_OK;
 }
 
@@ -1591,13 +1979,11 @@ extern "C" int me_head_logps(const void *hidden, int dtype, int64_t n, int64_t d
                              size_t workspace_bytes, void *stream) {
     const int rc = check_call(hidden, dtype, n, dim, rows_per_batch, weight, vocab, w_stride, targets, targets_dtype, temperature, saved, workspace);
     if (rc != ME_OK) return rc;
-    const Plan p = plan_of(n, vocab, dim, dtype, weight, w_stride, unit ? kLeavesUnit : kStats, false);
-    ME_CHECK_ARG(workspace_bytes >= static_cast<size_t>(p.bytes), "workspace of %zu bytes, %lld are needed", workspace_bytes, static_cast<long long>(p.bytes));
     ME_CHECK_ARG(n == 0 || logps, "logps is needed");
-    ME_CHECK_ARG(reinterpret_cast<uintptr_t>(unit) % 16 == 0 && (!unit || dtype == ME_BF16), "unit must be 16-byte aligned, and is for bf16");
+    ME_CHECK_ARG(reinterpret_cast<uintptr_t>(unit) % 16 == 0 && (!unit || dtype == ME_BF16 || takes_kept(n, vocab, dtype)), "unit must be 16-byte aligned, and is for bf16 or few rows");
     const Call c{hidden, weight, targets, rows_per_batch, batch_stride, row_stride, w_stride, ignore_index, targets_dtype,
                  static_cast<uint8_t *>(workspace), saved_of(saved, n), as_stream(stream)};
-    return forward(p, c, Loss{temperature, 0.0, 0.0, 1.0, 0, logps, nullptr, unit});
+    return forward(n, vocab, dim, dtype, c, Loss{temperature, 0.0, 0.0, 1.0, 0, logps, nullptr, unit}, workspace_bytes);
 }
 
 extern "C" int me_head_ce(const void *hidden, int dtype, int64_t n, int64_t dim, int64_t rows_per_batch, int64_t batch_stride,
@@ -1608,12 +1994,10 @@ extern "C" int me_head_ce(const void *hidden, int dtype, int64_t n, int64_t dim,
     if (rc != ME_OK) return rc;
     ME_CHECK_ARG(reduction == ME_REDUCE_MEAN || reduction == ME_REDUCE_SUM, "reduction must be mean or sum");
     ME_CHECK_ARG(loss, "loss is needed");
-    ME_CHECK_ARG(reinterpret_cast<uintptr_t>(unit) % 16 == 0 && (!unit || dtype == ME_BF16), "unit must be 16-byte aligned, and is for bf16");
-    const Plan p = plan_of(n, vocab, dim, dtype, weight, w_stride, unit ? kLeavesUnit : kStats, smoothing != 0.0);
-    ME_CHECK_ARG(workspace_bytes >= static_cast<size_t>(p.bytes), "workspace of %zu bytes, %lld are needed", workspace_bytes, static_cast<long long>(p.bytes));
+    ME_CHECK_ARG(reinterpret_cast<uintptr_t>(unit) % 16 == 0 && (!unit || dtype == ME_BF16 || takes_kept(n, vocab, dtype)), "unit must be 16-byte aligned, and is for bf16 or few rows");
     const Call c{hidden, weight, targets, rows_per_batch, batch_stride, row_stride, w_stride, ignore_index, targets_dtype,
                  static_cast<uint8_t *>(workspace), saved_of(saved, n), as_stream(stream)};
-    return forward(p, c, Loss{temperature, smoothing, z_loss, scale, reduction == ME_REDUCE_MEAN, nullptr, loss, unit});
+    return forward(n, vocab, dim, dtype, c, Loss{temperature, smoothing, z_loss, scale, reduction == ME_REDUCE_MEAN, nullptr, loss, unit}, workspace_bytes);
 }
 
 extern "C" int me_head_backward(const void *hidden, int dtype, int64_t n, int64_t dim, int64_t rows_per_batch, int64_t batch_stride,
@@ -1622,14 +2006,24 @@ extern "C" int me_head_backward(const void *hidden, int dtype, int64_t n, int64_
                                 double smoothing, double z_loss, double scale, int reduction, const void *saved, const float *unit,
                                 void *grad_hidden, void *grad_weight, void *workspace, size_t workspace_bytes, void *stream) {
     const int rc = check_call(hidden, dtype, n, dim, rows_per_batch, weight, vocab, w_stride, targets, targets_dtype, temperature, saved,
-                              unit ? saved : workspace);
+                              unit && dtype == ME_BF16 ? saved : workspace);
     if (rc != ME_OK) return rc;
     ME_CHECK_ARG(upstream || (n == 0 && upstream_per_row), "upstream is needed");
     ME_CHECK_ARG(reinterpret_cast<uintptr_t>(grad_hidden) % 16 == 0 && reinterpret_cast<uintptr_t>(grad_weight) % 16 == 0, "gradients must be 16-byte aligned");
-    ME_CHECK_ARG(!unit || (dtype == ME_BF16 && !grad_weight), "unit is for bf16 and the hidden states' gradient alone");
+    ME_CHECK_ARG(!unit || (dtype == ME_BF16 && !grad_weight) || takes_kept(n, vocab, dtype), "unit is for the hidden states' gradient alone, or few rows of fp32");
     if (!grad_hidden && !grad_weight) return ME_OK;
     const Saved saved_rows = saved_of(const_cast<void *>(saved), n);
     const bool f32 = dtype == ME_F32;
+    if (unit && f32) {
+        const KeptPlan q = kept_plan_of(n, vocab, dim, weight, w_stride, kHasUnit, false);
+        ME_CHECK_ARG(workspace_bytes >= static_cast<size_t>(q.bytes), "workspace of %zu bytes, %lld are needed", workspace_bytes, static_cast<long long>(q.bytes));
+        const Call c{hidden, weight, targets, rows_per_batch, batch_stride, row_stride, w_stride, ignore_index, targets_dtype,
+                     static_cast<uint8_t *>(workspace), saved_rows, as_stream(stream)};
+        const Coefs coefs{saved_rows, upstream, upstream_per_row != 0, reduction == ME_REDUCE_MEAN, scale / temperature, static_cast<float>(smoothing),
+                          static_cast<float>(z_loss), static_cast<double>(vocab)};
+        backward_kept(q, c, coefs, unit, temperature, grad_hidden, grad_weight);
+        return check_launch("me_head_backward");
+    }
     if (unit) {
         if (n == 0) return ME_OK;
         const ScaleArgs a{unit, saved_rows.count, saved_rows.place, upstream, upstream_per_row != 0, reduction == ME_REDUCE_MEAN, scale / temperature, n, dim, grad_hidden};

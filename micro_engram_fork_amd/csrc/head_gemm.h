@@ -22,6 +22,10 @@
 //           is more. That is as exact as fp32 where errors count against the rest of a row's sum: for logits, and for
 //           the gradient of the hidden states. The gradient of the head has rows of its own for tokens of any
 //           probability, down to products that fp16 could not tell from zero: six products.
+// Few rows of fp32 (SEGS 0) are read as they lie instead, in 32-wide k-slabs, as laying out the other operand would
+// read and write what is otherwise read once; fragments are split into three bf16 parts in registers (Parts), the same six
+// products. (v_mfma_f32_32x32x2_f32 takes 2.7 times as long and was the bound from 40 rows on: 262,144 x 5376,
+// 46 rows 1661 us, 128 rows 2837.)
 #pragma once
 
 #include "me_common.h"
@@ -32,8 +36,12 @@ namespace me {
 namespace head {
 
 constexpr int kThreads = 256;
-constexpr int kSlabK = 64;
-constexpr int kSlabBytes = kSlabK * 2;
+constexpr int kSlabBytes = 128;                  // of a k-contiguous row
+constexpr int kSlabK = 64;                       // k values of a slab of 16-bit operands
+template <int SEGS>
+constexpr int kElement = SEGS == 0 ? 4 : 2;      // bytes
+template <int SEGS>
+constexpr int kSlab = kSlabBytes / kElement<SEGS>;
 constexpr int kXcds = 8;
 constexpr uint32_t kBufferConfig = 0x00020000u;  // raw buffer descriptor word 3 (gfx9 family)
 constexpr uint32_t kOff = 0xffffffffu;           // a load offset past every buffer: reads zeros
@@ -41,6 +49,8 @@ constexpr uint32_t kOff = 0xffffffffu;           // a load offset past every buf
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef float floatx8 __attribute__((ext_vector_type(8)));
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef int int32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) bf16x4 lds_bf16x4;
@@ -81,6 +91,28 @@ __device__ inline int splits_for(int tiles, int most, int cost) {
 __device__ __forceinline__ int part_a(int seg) { return (0x910 >> (2 * seg)) & 3; }
 __device__ __forceinline__ int part_b(int seg) { return (0x184 >> (2 * seg)) & 3; }
 
+// Eight k values of fp32 as three bf16 that add up to them, each the nearest of what remains. What is not finite, or
+// rounds to infinity (from 3.39e38 on), makes its products NaN.
+struct Parts {
+    bf16x8 p[3];
+
+    Parts() = default;
+    __device__ __forceinline__ explicit Parts(const floatx8 &x) {
+        p[0] = __builtin_convertvector(x, bf16x8);
+        const floatx8 r = x - __builtin_convertvector(p[0], floatx8);
+        p[1] = __builtin_convertvector(r, bf16x8);
+        p[2] = __builtin_convertvector(r - __builtin_convertvector(p[1], floatx8), bf16x8);
+    }
+};
+
+__device__ __forceinline__ floatx16 multiply(const Parts &x, const Parts &y, floatx16 acc) {
+#pragma unroll
+    for (int sum = 2; sum >= 0; --sum)  // small products first
+#pragma unroll
+        for (int i = 0; i <= sum; ++i) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x.p[i], y.p[sum - i], acc, 0, 0, 0);
+    return acc;
+}
+
 template <int SEGS>
 __device__ __forceinline__ floatx16 multiply(const bf16x8 &x, const bf16x8 &y, const floatx16 &acc) {
     if constexpr (SEGS == 3)
@@ -111,17 +143,25 @@ __device__ __forceinline__ void dma16(const int32x4 &rsrc, uint32_t lds_base, ui
                  : "memory");
 }
 
+// Likewise 64 x 4 bytes, from addresses that are multiples of 4
+__device__ __forceinline__ void dma4(const int32x4 &rsrc, uint32_t lds_base, uint32_t voffset, uint32_t soffset) {
+    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, %3 offen lds"
+                 :
+                 : "s"(lds_base), "v"(voffset), "s"(rsrc), "s"(soffset)
+                 : "memory");
+}
+
 template <int N>
 __device__ __forceinline__ void wait_vmcnt() {
     asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
 }
 
-// XOR swizzle (in 16-byte chunks) of k-row kr of a row-contiguous unit of COLS columns: the 4 k-rows x 4 chunks
-// that the 32 lanes of one LDS cycle read are on 16 distinct 16-byte bank groups
-template <int COLS>
+// XOR swizzle (in 16-byte chunks) of k-row kr of a row-contiguous unit. 16-bit: the 4 k-rows x 4 chunks that the 32
+// lanes of one LDS cycle read are on 16 distinct 16-byte bank groups. fp32: the two halves of a wave read k-rows eight
+// apart, of 32 columns each, on the two halves of the banks.
+template <int ELEMENT>
 __device__ __forceinline__ int rc_swizzle(int kr) {
-    static_assert(COLS == 64 || COLS == 128 || COLS == 256, "8, 16 or 32 chunks per k-row");
-    return COLS == 64 ? 4 * ((kr >> 1) & 1) : 4 * (kr & 3);
+    return ELEMENT == 4 ? 8 * ((kr >> 3) & 1) : 4 * (kr & 3);
 }
 
 // Two transpose reads make a fragment: 16-lane group g takes columns 16 (g & 1) .. + 15 of the 32-wide subtile and
@@ -129,10 +169,11 @@ __device__ __forceinline__ int rc_swizzle(int kr) {
 // .. + 3 and receives column i's four k values. k-step and half are constant byte offsets.
 template <int COLS>
 __device__ __forceinline__ uint32_t rc_lane_off(int col0, int lane) {
+    static_assert(COLS == 128 || COLS == 256, "16 or 32 chunks per k-row");
     const int i = lane & 15, g = lane >> 4;
     const int c = col0 + 16 * (g & 1) + 4 * (i & 3);
     const int kr = 8 * (g >> 1) + (i >> 2);
-    return static_cast<uint32_t>(kr * (2 * COLS) + (((c >> 3) ^ rc_swizzle<COLS>(kr)) << 4) + (c & 7) * 2);
+    return static_cast<uint32_t>(kr * (2 * COLS) + (((c >> 3) ^ rc_swizzle<2>(kr)) << 4) + (c & 7) * 2);
 }
 
 template <int COLS>
@@ -146,6 +187,14 @@ __device__ __forceinline__ bf16x8 rc_frag(const uint8_t *unit, int ks, uint32_t 
 __device__ __forceinline__ bf16x8 kc_frag(const uint8_t *unit, int ks, int row, int lane) {
     const int c = ((2 * ks + (lane >> 5)) ^ ((row >> 1) & 7)) << 4;
     return *reinterpret_cast<const bf16x8 *>(unit + row * kSlabBytes + c);
+}
+
+// fp32: 8 k values 16 ks + 8 (lane >> 5) .. + 7
+__device__ __forceinline__ floatx8 kc_frag_f32(const uint8_t *unit, int ks, int row, int lane) {
+    const int c = 4 * ks + 2 * (lane >> 5), x = (row >> 1) & 7;
+    const floatx4 lo = *reinterpret_cast<const floatx4 *>(unit + row * kSlabBytes + ((c ^ x) << 4));
+    const floatx4 hi = *reinterpret_cast<const floatx4 *>(unit + row * kSlabBytes + (((c + 1) ^ x) << 4));
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
 // Accumulator e of a tile. The large tiles' accumulators fill the AGPRs: read one by one, in the order of the
@@ -174,7 +223,7 @@ struct Tile {
 // Workgroup -> tile: each XCD takes a run of logical tiles; these go through `group` column tiles of
 // a row tile before the next row tile, so the tiles that an XCD's CUs work on at a time are a block whose rows and
 // columns share its L2. False: no tile (the device's count is short of the launch).
-__device__ __forceinline__ bool tile_of(const Gemm &a, int tr, int ts, Tile &t) {
+__device__ __forceinline__ bool tile_of(const Gemm &a, int tr, int ts, int slab, Tile &t) {
     int64_t rows = a.R, k = a.K;
     if (a.count != nullptr) {
         const int64_t n = *as_global(a.count);
@@ -203,71 +252,87 @@ __device__ __forceinline__ bool tile_of(const Gemm &a, int tr, int ts, Tile &t) 
     t.r0 = static_cast<int64_t>(t.rt) * tr;
     t.s0 = static_cast<int64_t>(t.st) * ts;
     t.rows = rows;
-    const int64_t slabs = ceil_div(k, int64_t{kSlabK});
-    t.k0 = slabs * t.split / splits * kSlabK;
-    t.k1 = min(k, slabs * (t.split + 1) / splits * kSlabK);
+    const int64_t slabs = ceil_div(k, static_cast<int64_t>(slab));
+    t.k0 = slabs * t.split / splits * slab;
+    t.k1 = min(k, slabs * (t.split + 1) / splits * slab);
     return true;
 }
 
-// The loads of one operand's slabs by a wave: LOADS of 1 KiB, fixed per-lane offsets.
-// k-contiguous: load i fills rows 8 (LOADS wave + i) + [0, 8), lane l row + l / 8 at physical chunk l % 8; the
-// slab's byte offset goes in soffset, and chunks past K in the last slab read zeros.
-// row-contiguous: load i fills 512 / COLS k-rows; the descriptor's base moves by the slab's k-rows and its size
+// The loads of one operand's slabs by a wave: LOADS of 1 KiB, fixed per-lane offsets, in pieces of 16 bytes a lane or of 4
+// (fp32 rows that start or end anywhere: four instructions for each KiB).
+// k-contiguous: load i fills rows 8 (LOADS wave + i) + [0, 8), the KiB's chunk c row + c / 8 at physical chunk c % 8;
+// the slab's byte offset goes in soffset, and pieces past K in the last slab read zeros.
+// row-contiguous: load i fills one or more k-rows; the descriptor's base moves by the slab's k-rows and its size
 // holds those that there are, so that k-rows past K read zeros with no per-lane work.
-template <bool KC, int DIM, int LOADS>
+template <bool KC, int DIM, int LOADS, int ELEMENT, int PIECE = 16>
 struct Loader {
+    static constexpr int kChunk = 16 / ELEMENT;             // values of a 16-byte chunk
+    static constexpr int kSlabValues = kSlabBytes / ELEMENT;
+    static constexpr int kSteps = 16 / PIECE;               // instructions of a KiB
+    static_assert(PIECE == 16 || (PIECE == 4 && ELEMENT == 4), "pieces of whole values");
     uint64_t base;     // of the tile (k-contiguous) or the operand (row-contiguous)
     int64_t pitch;     // bytes from row to row
     int64_t part;
     int64_t K;         // full reduction length of a segment's operand
     uint32_t range;    // k-contiguous: bytes of the tile's rows
-    uint32_t off[LOADS];
-    bool even_out, odd_out;  // this lane's chunk of an even / odd load is past K in the last slab
+    uint32_t off[LOADS * kSteps];
+    bool out[2 * kSteps];  // this lane's piece of an even / odd load is past K in the last slab
 
     // rows / columns from `first` on up to `there`; k values from k0 on up to k
     __device__ __forceinline__ void init(const Operand &o, int64_t first, int64_t there, int64_t k0, int64_t k, int wave, int lane) {
-        pitch = o.ld * 2;
+        pitch = o.ld * ELEMENT;
         part = o.part;
         K = k;
         if constexpr (KC) {
+            static_assert(LOADS % 2 == 0 || LOADS == 1 || LOADS == 3, "see out");
             base = reinterpret_cast<uint64_t>(o.base) + static_cast<uint64_t>(first * pitch);
             const int64_t rows = min(there - first, static_cast<int64_t>(DIM));
-            range = static_cast<uint32_t>(rows * pitch);
-            const int valid = k > k0 ? static_cast<int>(k - (k - 1) / kSlabK * kSlabK) : 0;  // k values of the last slab
+            range = static_cast<uint32_t>((rows - 1) * pitch + ceil_div(k, kChunk) * 16);
+            const int valid = k > k0 ? static_cast<int>(k - (k - 1) / kSlabValues * kSlabValues) : 0;  // k values of the last slab
 #pragma unroll
-            for (int i = 0; i < LOADS; ++i) {
-                const int row = (wave * LOADS + i) * 8 + (lane >> 3);
-                const uint32_t ch = static_cast<uint32_t>((lane & 7) ^ ((row >> 1) & 7));
-                off[i] = row < rows ? static_cast<uint32_t>(row * pitch) + ch * 16u : kOff;
-                const bool out = static_cast<int>(ch) * 8 >= valid;
-                if (i % 2 == 0)
-                    even_out = out;
-                else
-                    odd_out = out;
-            }
-            if constexpr (LOADS == 1) odd_out = even_out;
+            for (int i = 0; i < LOADS; ++i)
+#pragma unroll
+                for (int j = 0; j < kSteps; ++j) {
+                    const int at = (j * 64 + lane) * PIECE, row = (wave * LOADS + i) * 8 + at / kSlabBytes;
+                    const int ch = (at / 16 % 8) ^ ((row >> 1) & 7);
+                    off[i * kSteps + j] = row < rows ? static_cast<uint32_t>(row * pitch) + static_cast<uint32_t>(ch * 16 + at % 16) : kOff;
+                    out[i % 2 * kSteps + j] = ch * kChunk + at % 16 / ELEMENT >= valid;  // alike for all loads of i's parity
+                }
         } else {
             base = reinterpret_cast<uint64_t>(o.base);
-            constexpr int kChunks = DIM / 8, kRows = 64 / kChunks;
+            constexpr int kRowBytes = DIM * ELEMENT;
 #pragma unroll
-            for (int i = 0; i < LOADS; ++i) {
-                const int kr = (wave * LOADS + i) * kRows + lane / kChunks;
-                const int64_t col = first + 8 * ((lane % kChunks) ^ rc_swizzle<DIM>(kr));
-                off[i] = col < there ? static_cast<uint32_t>(kr * pitch + col * 2) : kOff;
-            }
+            for (int i = 0; i < LOADS; ++i)
+#pragma unroll
+                for (int j = 0; j < kSteps; ++j) {
+                    const int at = ((wave * LOADS + i) * 64 * kSteps + j * 64 + lane) * PIECE, kr = at / kRowBytes;
+                    const int64_t col = first + kChunk * ((at % kRowBytes / 16) ^ rc_swizzle<ELEMENT>(kr)) + at % 16 / ELEMENT;
+                    off[i * kSteps + j] = col < there ? static_cast<uint32_t>(kr * pitch + col * ELEMENT) : kOff;
+                }
         }
     }
 
     // load i of the slab at k0 of part p
     __device__ __forceinline__ void issue(int i, int64_t k0, int p, uint32_t lds) const {
         const uint64_t at = base + static_cast<uint64_t>(p * part);
+        int32x4 rsrc;
+        uint32_t soffset = 0;
+        bool last = false;
         if constexpr (KC) {
-            const bool last = k0 + kSlabK > K;
-            const bool out = last && ((i & 1) ? odd_out : even_out);
-            dma16(buffer_rsrc(at, range), lds, out ? kOff : off[i], static_cast<uint32_t>(k0 * 2));
+            last = k0 + kSlabValues > K;
+            rsrc = buffer_rsrc(at, range);
+            soffset = static_cast<uint32_t>(k0 * ELEMENT);
         } else {
-            const int64_t left = max(min(K - k0, int64_t{kSlabK}), int64_t{0});
-            dma16(buffer_rsrc(at + static_cast<uint64_t>(k0 * pitch), static_cast<uint32_t>(left * pitch)), lds, off[i], 0u);
+            const int64_t left = max(min(K - k0, int64_t{kSlabValues}), int64_t{0});
+            rsrc = buffer_rsrc(at + static_cast<uint64_t>(k0 * pitch), static_cast<uint32_t>(left * pitch));
+        }
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j) {
+            const uint32_t from = KC && last && out[i % 2 * kSteps + j] ? kOff : off[i * kSteps + j];
+            if constexpr (PIECE == 16)
+                dma16(rsrc, lds, from, soffset);
+            else
+                dma4(rsrc, lds + static_cast<uint32_t>(j) * 256u, from, soffset);
         }
     }
 };
@@ -290,7 +355,7 @@ __global__ __launch_bounds__(kThreads, 1) void large_kernel(const Gemm a, const 
     __shared__ __attribute__((aligned(16))) uint8_t ring[kRingBytes];
 
     Tile t;
-    if (!tile_of(a, kTile, kTile, t)) return;
+    if (!tile_of(a, kTile, kTile, kSlabK, t)) return;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wr = wave >> 1, ws = wave & 1;
@@ -298,8 +363,8 @@ __global__ __launch_bounds__(kThreads, 1) void large_kernel(const Gemm a, const 
     const int spq = max(static_cast<int>(ceil_div(t.k1 - t.k0, int64_t{kSlabK})), 1);
     const int slabs = spq * SEGS;
 
-    Loader<A_KC, kTile, kDma> la;
-    Loader<B_KC, kTile, kDma> lb;
+    Loader<A_KC, kTile, kDma, 2> la;
+    Loader<B_KC, kTile, kDma, 2> lb;
     la.init(a.a, t.r0, A_KC ? t.rows : a.R, t.k0, t.k1, wave, lane);
     lb.init(a.b, t.s0, a.S, t.k0, t.k1, wave, lane);
     const uint32_t w0 = __builtin_amdgcn_readfirstlane(lds_addr(ring) + static_cast<uint32_t>(wave) * (kDma * 1024u));
@@ -434,89 +499,116 @@ __global__ __launch_bounds__(kThreads, 1) void large_kernel(const Gemm a, const 
     epi.template run<true, kSub, kSub>(acc, t, wr * 128, ws * 128, ring, lane);
 }
 
-// ---- 64 or 128 x 256 tiles for few rows ---------------------------------------------------------------------
+// ---- 32 to 128 x 256 tiles for few rows ---------------------------------------------------------------------
 // The product of a few rows is bound by the one read of its other operand. Four waves next to each other over
-// the columns, all 32 BR rows each; whole slabs in a ring of RING slots, RING - 1 in flight while one is consumed, one
-// barrier per slab; one workgroup per CU, 64 or 96 KB of loads in flight.
-template <bool B_KC, int BR, int TS, int RING, int SEGS, class Epilogue>
+// the columns, all 32 BR rows each; whole slabs in a ring of three slots, two in flight while one is consumed, one
+// barrier per slab; one workgroup per CU, 64 to 96 KB of loads in flight. SEGS 0: fp32 as it lies, PIECE as of Loader;
+// k-contiguous heads then in two slots, for two workgroups per CU whose reads, splits and products take turns (46
+// rows, 262,144 x 5376: 1208 us, with three slots and one workgroup 1485; row-contiguous ones 1637 and 1556).
+template <bool B_KC, int BR, int SEGS, int PIECE, class Epilogue>
 __global__ __launch_bounds__(kThreads) void few_kernel(const Gemm a, const Epilogue epi) {
-    constexpr int kTR = 32 * BR;
-    constexpr int kBS = TS / 128, kBR = BR;                // 32-wide subtiles of a wave
+    constexpr int kTR = 32 * BR, kTS = 256, kRing = SEGS == 0 && B_KC ? 2 : 3, kEl = kElement<SEGS>, kStep = kSlab<SEGS>;
+    constexpr int kBS = kTS / 128;                         // 32-wide subtiles of a wave's columns
     constexpr int kUnitA = kTR * kSlabBytes;
-    constexpr int kSlot = (kTR + TS) * kSlabBytes;
-    constexpr int kDmaA = kTR / 32, kDmaB = TS / 32;       // 1 KiB loads per wave and slab
-    static_assert((RING - 2) * (kDmaA + kDmaB) <= 63 && RING >= 3, "vmcnt counts up to 63");
-    __shared__ __attribute__((aligned(16))) uint8_t ring[RING * kSlot];
+    constexpr int kSlot = (kTR + kTS) * kSlabBytes;
+    constexpr int kDmaA = kTR / 32, kDmaB = kTS / 32;      // 1 KiB loads per wave and slab
+    constexpr int kWait = (kRing - 2) * (kDmaA + kDmaB * (16 / PIECE));  // instructions of the slabs that may fly
+    static_assert(kWait <= 63, "vmcnt counts up to 63");
+    __shared__ __attribute__((aligned(16))) uint8_t ring[kRing * kSlot];
 
     Tile t;
-    if (!tile_of(a, kTR, TS, t)) return;
+    if (!tile_of(a, kTR, kTS, kStep, t)) return;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int spq = max(static_cast<int>(ceil_div(t.k1 - t.k0, int64_t{kSlabK})), 1);
-    const int slabs = spq * SEGS;
-    Loader<true, kTR, kDmaA> la;
-    Loader<B_KC, TS, kDmaB> lb;
+    const int spq = max(static_cast<int>(ceil_div(t.k1 - t.k0, static_cast<int64_t>(kStep))), 1);
+    const int slabs = spq * (SEGS == 0 ? 1 : SEGS);
+    Loader<true, kTR, kDmaA, kEl> la;
+    Loader<B_KC, kTS, kDmaB, kEl, PIECE> lb;
     la.init(a.a, t.r0, t.rows, t.k0, t.k1, wave, lane);
     lb.init(a.b, t.s0, a.S, t.k0, t.k1, wave, lane);
     const uint32_t w0 = __builtin_amdgcn_readfirstlane(lds_addr(ring));
     auto issue = [&](int sl) {
-        const int seg = SEGS == 1 ? 0 : sl / spq;
-        const int64_t k0 = t.k0 + static_cast<int64_t>(sl - seg * spq) * kSlabK;
-        uint32_t slot = w0 + static_cast<uint32_t>(sl % RING) * kSlot;
+        const int seg = SEGS <= 1 ? 0 : sl / spq;
+        const int64_t k0 = t.k0 + static_cast<int64_t>(sl - seg * spq) * kStep;
+        uint32_t slot = w0 + static_cast<uint32_t>(sl % kRing) * kSlot;
         asm volatile("" : "+s"(slot));
 #pragma unroll
-        for (int i = 0; i < kDmaA; ++i)
-            la.issue(i, k0, SEGS == 1 ? 0 : part_a(seg), slot + static_cast<uint32_t>(wave * kDmaA + i) * 1024u);
+        for (int i = 0; i < kDmaA; ++i) la.issue(i, k0, SEGS <= 1 ? 0 : part_a(seg), slot + static_cast<uint32_t>(wave * kDmaA + i) * 1024u);
 #pragma unroll
-        for (int i = 0; i < kDmaB; ++i)
-            lb.issue(i, k0, SEGS == 1 ? 0 : part_b(seg), slot + kUnitA + static_cast<uint32_t>(wave * kDmaB + i) * 1024u);
+        for (int i = 0; i < kDmaB; ++i) lb.issue(i, k0, SEGS <= 1 ? 0 : part_b(seg), slot + kUnitA + static_cast<uint32_t>(wave * kDmaB + i) * 1024u);
     };
     uint32_t soff[B_KC ? 1 : kBS];
     if constexpr (!B_KC) {
 #pragma unroll
-        for (int x = 0; x < kBS; ++x) soff[x] = rc_lane_off<TS>(wave * 32 * kBS + 32 * x, lane);
+        for (int x = 0; x < kBS; ++x) {
+            const int col = wave * 32 * kBS + 32 * x;
+            if constexpr (SEGS == 0)  // k-row 8 (lane >> 5) of a k-step, a lane's column
+                soff[x] = static_cast<uint32_t>(8 * (lane >> 5) * kTS * 4 + (((col >> 2) ^ rc_swizzle<4>(8 * (lane >> 5))) << 4) + (lane & 31) * 4);
+            else
+                soff[x] = rc_lane_off<kTS>(col, lane);
+        }
     }
-    floatx16 acc[kBS][kBR];
+    floatx16 acc[kBS][BR];
 #pragma unroll
     for (int x = 0; x < kBS; ++x)
 #pragma unroll
-        for (int y = 0; y < kBR; ++y)
+        for (int y = 0; y < BR; ++y)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[x][y][e] = 0.f;
 #pragma unroll
-    for (int sl = 0; sl < RING - 1; ++sl)
+    for (int sl = 0; sl < kRing - 1; ++sl)
         if (sl < slabs) issue(sl);
     for (int sl = 0; sl < slabs; ++sl) {
         // slab sl landed for this wave (later slabs may fly), then for every wave
-        if (sl + RING - 2 < slabs)
-            wait_vmcnt<(RING - 2) * (kDmaA + kDmaB)>();
+        if (sl + kRing - 2 < slabs)
+            wait_vmcnt<kWait>();
         else
             wait_vmcnt<0>();
         __syncthreads();
         // the slot of slab sl - 1 is free: every wave read it before this barrier
-        if (sl + RING - 1 < slabs) issue(sl + RING - 1);
-        const uint8_t *ua = ring + (sl % RING) * kSlot, *ub = ua + kUnitA;
+        if (sl + kRing - 1 < slabs) issue(sl + kRing - 1);
+        const uint8_t *ua = ring + (sl % kRing) * kSlot, *ub = ua + kUnitA;
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-            bf16x8 fs[kBS], fr[kBR];
+        for (int ks = 0; ks < kStep / 16; ++ks) {
+            if constexpr (SEGS == 0) {
+                auto take_b = [&](int x) {
+                    if constexpr (B_KC) {
+                        return kc_frag_f32(ub, ks, wave * 32 * kBS + 32 * x + (lane & 31), lane);
+                    } else {
+                        floatx8 f;
 #pragma unroll
-            for (int x = 0; x < kBS; ++x) {
-                if constexpr (B_KC)
-                    fs[x] = kc_frag(ub, ks, wave * 32 * kBS + 32 * x + (lane & 31), lane);
-                else
-                    fs[x] = rc_frag<TS>(ub, ks, soff[x]);
+                        for (int i = 0; i < 8; ++i) f[i] = *reinterpret_cast<const float *>(ub + soff[x] + (16 * ks + i) * kTS * 4);
+                        return f;
+                    }
+                };
+                const Parts fs[kBS] = {Parts(take_b(0)), Parts(take_b(1))};
+                static_assert(kBS == 2, "two subtiles");
+#pragma unroll
+                for (int y = 0; y < BR; ++y) {
+                    const Parts fr(kc_frag_f32(ua, ks, 32 * y + (lane & 31), lane));
+#pragma unroll
+                    for (int x = 0; x < kBS; ++x) acc[x][y] = multiply(fs[x], fr, acc[x][y]);
+                }
+            } else {
+                bf16x8 fs[kBS], fr[BR];
+#pragma unroll
+                for (int x = 0; x < kBS; ++x) {
+                    if constexpr (B_KC)
+                        fs[x] = kc_frag(ub, ks, wave * 32 * kBS + 32 * x + (lane & 31), lane);
+                    else
+                        fs[x] = rc_frag<kTS>(ub, ks, soff[x]);
+                }
+#pragma unroll
+                for (int y = 0; y < BR; ++y) fr[y] = kc_frag(ua, ks, 32 * y + (lane & 31), lane);
+#pragma unroll
+                for (int x = 0; x < kBS; ++x)
+#pragma unroll
+                    for (int y = 0; y < BR; ++y) acc[x][y] = multiply<SEGS>(fs[x], fr[y], acc[x][y]);
             }
-#pragma unroll
-            for (int y = 0; y < kBR; ++y) fr[y] = kc_frag(ua, ks, 32 * y + (lane & 31), lane);
-#pragma unroll
-            for (int x = 0; x < kBS; ++x)
-#pragma unroll
-                for (int y = 0; y < kBR; ++y)
-                    acc[x][y] = multiply<SEGS>(fs[x], fr[y], acc[x][y]);
         }
     }
     __syncthreads();
-    epi.template run<false, kBS, kBR>(acc, t, 0, wave * 32 * kBS, ring, lane);
+    epi.template run<false, kBS, BR>(acc, t, 0, wave * 32 * kBS, ring, lane);
 }
 
 // Workgroups that hold every tile at the largest count

@@ -7,11 +7,12 @@ from typing import List, Optional
 
 import torch
 
-from ._lib import ME_BF16, call
+from ._lib import call
 from .loss_ops import _targets, row_layout
 from .ops import _custom_op, _p, call_on, dtype_code, require_gpu
 
-_FORWARD, _BACKWARD, _FORWARD_UNIT = 0, 1, 2
+_FORWARD, _BACKWARD, _FORWARD_UNIT, _BACKWARD_UNIT = 0, 1, 2, 3
+NO_GRADIENT, OF_HIDDEN, OF_WEIGHT = 0, 1, 2  # what a forward may leave something for: hidden alone, weight as well
 
 
 def weight_layout(weight):
@@ -46,25 +47,21 @@ def _workspace(operands, dev, which, smoothed=False):
 
 
 @functools.lru_cache(maxsize=256)
-def unit_elements(n, vocab, dim, dtype):
-    """Size of what a forward leaves for the gradient of hidden alone; 0: nothing, as always of fp32."""
-    if dtype != ME_BF16:
+def unit_elements(n, vocab, dim, dtype, gradients):
+    """Size of what a forward leaves for these gradients; 0: nothing."""
+    if gradients == NO_GRADIENT:
         return 0
     size = ctypes.c_int64(0)
-    call("me_head_unit_size", n, vocab, dim, dtype, ctypes.byref(size))
+    call("me_head_unit_size", n, vocab, dim, dtype, int(gradients == OF_WEIGHT), ctypes.byref(size))
     return size.value
 
 
-def _unit_size(hidden, weight, targets):
-    return unit_elements(targets.numel(), weight.shape[0], weight.shape[1], dtype_code(weight))
-
-
-def _forward(name, hidden, weight, targets, ignore_index, with_unit, out, args):
+def _forward(name, hidden, weight, targets, ignore_index, gradients, out, args):
     """([out, saved] and unit where the call leaves one, the operands' arguments with the tensors that hold them)."""
     dev = require_gpu(hidden, weight, targets)
     held, operands = _operands(hidden, weight, targets, ignore_index)
     saved = torch.empty(16 + 5 * operands[2], dtype=torch.float32, device=dev)
-    size = unit_elements(operands[2], operands[8], operands[3], operands[1]) if with_unit else 0
+    size = unit_elements(operands[2], operands[8], operands[3], operands[1], gradients)
     unit = torch.empty(size, dtype=torch.float32, device=dev) if size else None
     smoothed = len(args) > 1 and args[1] != 0.0
     ws, ptr, size = _workspace(operands, dev, _FORWARD if unit is None else _FORWARD_UNIT, smoothed)
@@ -92,53 +89,53 @@ def _backward(hidden_shape, weight_shape, operands, like, saved, unit, upstream,
     dev, dtype = like.device, like.dtype
     grad_hidden = torch.empty(hidden_shape, dtype=dtype, device=dev) if need_hidden else None
     grad_weight = torch.empty(weight_shape, dtype=dtype, device=dev) if need_weight else None
-    ws, ptr, size = _workspace(operands, dev, _BACKWARD) if unit is None else (None, None, 0)
+    ws, ptr, size = _workspace(operands, dev, _BACKWARD if unit is None else _BACKWARD_UNIT)
     temperature, per_row, smoothing, z_loss, scale, reduction = consts
     call_on(dev, "me_head_backward", *operands, temperature, upstream.data_ptr(), int(per_row), smoothing, z_loss, scale,
             reduction, saved.data_ptr(), _p(unit), _p(grad_hidden), _p(grad_weight), ptr, size)
     return grad_hidden, grad_weight
 
 
-def _fake_forward(hidden, weight, targets, with_unit, shape):
+def _fake_forward(hidden, weight, targets, gradients, shape):
     res = [hidden.new_empty(shape, dtype=torch.float32), hidden.new_empty((16 + 5 * targets.numel(),), dtype=torch.float32)]
-    size = _unit_size(hidden, weight, targets) if with_unit else 0
+    size = unit_elements(targets.numel(), weight.shape[0], weight.shape[1], dtype_code(weight), gradients)
     return [*res, hidden.new_empty((size,), dtype=torch.float32)] if size else res
 
 
-def run_head_logps(hidden, weight, targets, ignore_index, temperature, with_unit):
+def run_head_logps(hidden, weight, targets, ignore_index, temperature, gradients):
     out = torch.empty(targets.shape, dtype=torch.float32, device=targets.device)
-    return _forward("me_head_logps", hidden, weight, targets, ignore_index, with_unit, out, (temperature,))
+    return _forward("me_head_logps", hidden, weight, targets, ignore_index, gradients, out, (temperature,))
 
 
 @_custom_op("head_logps")
 def head_logps(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, ignore_index: int,
-               temperature: float, with_unit: bool) -> List[torch.Tensor]:
-    """[log-probabilities fp32 of targets' shape, saved (what the backward needs)], and where with_unit and the size pays
-    unit, from which the backward of hidden alone only scales."""
-    return run_head_logps(hidden, weight, targets, ignore_index, temperature, with_unit)[0]
+               temperature: float, gradients: int) -> List[torch.Tensor]:
+    """[log-probabilities fp32 of targets' shape, saved (what the backward needs)], and where unit_elements says so unit: bf16,
+    what the backward of hidden alone only scales; few rows of fp32, their logits."""
+    return run_head_logps(hidden, weight, targets, ignore_index, temperature, gradients)[0]
 
 
 @head_logps.register_fake
-def _(hidden, weight, targets, ignore_index, temperature, with_unit):
-    return _fake_forward(hidden, weight, targets, with_unit, targets.shape)
+def _(hidden, weight, targets, ignore_index, temperature, gradients):
+    return _fake_forward(hidden, weight, targets, gradients, targets.shape)
 
 
-def run_head_ce(hidden, weight, targets, ignore_index, temperature, smoothing, z_loss, scale, reduction, with_unit):
+def run_head_ce(hidden, weight, targets, ignore_index, temperature, smoothing, z_loss, scale, reduction, gradients):
     out = torch.empty((), dtype=torch.float32, device=targets.device)
-    return _forward("me_head_ce", hidden, weight, targets, ignore_index, with_unit, out,
+    return _forward("me_head_ce", hidden, weight, targets, ignore_index, gradients, out,
                     (temperature, smoothing, z_loss, scale, reduction))
 
 
 @_custom_op("head_ce")
 def head_ce(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, ignore_index: int, temperature: float,
-            smoothing: float, z_loss: float, scale: float, reduction: int, with_unit: bool) -> List[torch.Tensor]:
+            smoothing: float, z_loss: float, scale: float, reduction: int, gradients: int) -> List[torch.Tensor]:
     """[loss fp32, saved], and unit as of head_logps."""
-    return run_head_ce(hidden, weight, targets, ignore_index, temperature, smoothing, z_loss, scale, reduction, with_unit)[0]
+    return run_head_ce(hidden, weight, targets, ignore_index, temperature, smoothing, z_loss, scale, reduction, gradients)[0]
 
 
 @head_ce.register_fake
-def _(hidden, weight, targets, ignore_index, temperature, smoothing, z_loss, scale, reduction, with_unit):
-    return _fake_forward(hidden, weight, targets, with_unit, ())
+def _(hidden, weight, targets, ignore_index, temperature, smoothing, z_loss, scale, reduction, gradients):
+    return _fake_forward(hidden, weight, targets, gradients, ())
 
 
 @_custom_op("head_backward")

@@ -389,12 +389,12 @@ class _HeadLoss(torch.autograd.Function):
         op, run, per_row = kind
         ctx.consts = args[1], per_row, *(args[2:] or (0.0, 0.0, 1.0, ME_REDUCE_SUM))
         ctx.ignore_index, ctx.run = args[0], None
-        with_unit = not weight.requires_grad
+        gradients = head_ops.OF_WEIGHT if weight.requires_grad else head_ops.OF_HIDDEN
         if _makes_ready(hidden, weight, targets):
-            (out, *kept), held = run(hidden.detach(), weight.detach(), targets, *args, with_unit)
+            (out, *kept), held = run(hidden.detach(), weight.detach(), targets, *args, gradients)
             ctx.run = head_ops.Backward(held, kept, ctx.consts)
         else:
-            out, *kept = op(hidden.detach(), weight.detach(), targets, *args, with_unit)
+            out, *kept = op(hidden.detach(), weight.detach(), targets, *args, gradients)
         ctx.save_for_backward(hidden, weight, targets, *kept)
         return out
 
@@ -418,7 +418,7 @@ _HEAD_CE = head_ops.head_ce, head_ops.run_head_ce, False
 def _head_loss(kind, hidden, weight, targets, *args):
     if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
         return _HeadLoss.apply(hidden, weight, targets, kind, args)
-    return kind[0](hidden.detach(), weight.detach(), targets, *args, False)[0]
+    return kind[0](hidden.detach(), weight.detach(), targets, *args, head_ops.NO_GRADIENT)[0]
 
 
 def head_token_logps(hidden, weight, targets, temperature=1.0, ignore_index=IGNORE_INDEX):
@@ -427,8 +427,9 @@ def head_token_logps(hidden, weight, targets, temperature=1.0, ignore_index=IGNO
 
     hidden [..., dim] are the states after the decoder's last norm, weight [vocab, dim] its head, both bf16 or both fp32.
     Memory, during a call: statistics of a 32nd of the bf16 logits' size, and with gradients a piece of the logits' gradient
-    (at most 1 GiB up to 262,144 bf16 rows). Heads in fp32, or whose bf16 rows do not start at multiples of 16 bytes, are
-    laid out a piece at a time as well (again at most 1 GiB). Rows that do not count cost nothing and are not read.
+    (at most 1 GiB up to 262,144 bf16 rows). Heads in fp32, or whose bf16 rows do not start and end at multiples of 16 bytes, are
+    laid out a piece at a time as well (again at most 1 GiB); but few rows in fp32 (up to 384, or 1,024 with a small vocabulary)
+    read the head as it lies and keep their logits for the backward, n x vocab in fp32. Rows that do not count cost nothing and are not read.
     For the gradient of bf16 hidden states alone (a frozen head), larger calls make it in the forward, which saves one of
     three products, and keep it for the backward in fp32 before its upstream factors."""
     _check_head(hidden, weight, targets)

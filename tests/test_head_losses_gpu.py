@@ -329,8 +329,11 @@ def test_compiled():
 @pytest.fixture
 def leaves_unit(monkeypatch):
     """Calls of any size take that way, not those alone that are large enough for it to pay."""
-    from micro_engram_fork_amd import head_ops
-    monkeypatch.setattr(head_ops, "unit_elements", lambda n, vocab, dim, dtype: n * -(-dim // 4) * 4 if dtype == head_ops.ME_BF16 else 0)
+    from micro_engram_fork_amd import _lib, head_ops
+    as_it_is = head_ops.unit_elements
+    monkeypatch.setattr(head_ops, "unit_elements", lambda n, vocab, dim, dtype, gradients:
+                        n * -(-dim // 4) * 4 if (dtype, gradients) == (_lib.ME_BF16, head_ops.OF_HIDDEN)
+                        else as_it_is(n, vocab, dim, dtype, gradients))
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP32])
@@ -455,9 +458,9 @@ def test_hidden_alone_under_saved_tensor_hooks(leaves_unit):
 
 
 def test_large_calls_for_hidden_alone_take_that_way():
-    from micro_engram_fork_amd import head_ops
+    from micro_engram_fork_amd import _lib, head_ops
     hidden, weight, targets = _inputs(700, 33_000, 2_048, BF16)
-    assert head_ops._unit_size(hidden, weight, targets) == 700 * 2_048
+    assert head_ops.unit_elements(700, 33_000, 2_048, _lib.ME_BF16, head_ops.OF_HIDDEN) == 700 * 2_048
     _check_hidden_alone(hidden, weight, targets)
 
 
@@ -492,3 +495,76 @@ def test_heads_of_rows_of_very_different_sizes():
     _check_logps(hidden, weight, targets)
     hidden *= torch.logspace(-4, 1, 150, device=DEV)[:, None]
     _check_logps(hidden, weight, targets)
+
+
+# ---- few rows of fp32, whose logits are kept ------------------------------------------------------------------------
+@pytest.mark.parametrize("n,vocab,dim", [(9, 1_000, 512), (31, 8_191, 100), (32, 20_001, 64), (33, 257, 1_023), (64, 3_000, 2_050), (90, 3_423, 1_000),
+                                         (96, 140_000, 36), (97, 511, 33), (128, 40_003, 260), (128, 700, 4_097), (2, 150_001, 129), (7, 600, 1_500),
+                                         (129, 5_000, 68), (193, 70_001, 40), (384, 3_001, 200), (1_000, 515, 77), (1_024, 16_000, 24)])
+def test_few_rows_of_fp32(n, vocab, dim):
+    """Tiles of 32 to 128 rows, one and more of them, splits of either reduction, heads whose rows start and end anywhere."""
+    _check_logps(*_inputs(n, vocab, dim, FP32))
+    _check_hidden_alone(*_inputs(n, vocab, dim, FP32, seed=1))
+
+
+@pytest.mark.parametrize("n", [5, 100])
+@pytest.mark.parametrize("kw", [dict(label_smoothing=0.1, z_loss=1e-2), dict(temperature=0.4, reduction="sum", scale=-2.0, upstream=0.3)])
+def test_few_rows_of_fp32_options(kw, n):
+    _check_ce(*_inputs(n, 5_001, 130, FP32), **kw)
+
+
+@pytest.mark.parametrize("n", [6, 77])
+def test_few_rows_of_fp32_twice_and_captured(n):
+    """A second backward finds the logits as they were; replays, with eager work between them, give the eager bits."""
+    hidden, weight, targets = _inputs(n, 3_001, 257, FP32)
+    h, w = hidden.requires_grad_(), weight.requires_grad_()
+    loss = losses.head_cross_entropy(h, w, targets)
+    want = torch.autograd.grad(loss, (h, w), retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(loss, (h, w)), want))
+    del loss
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        for _ in range(2):
+            torch.autograd.grad(losses.head_cross_entropy(h, w, targets), (h, w))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        got = torch.autograd.grad(losses.head_cross_entropy(h, w, targets), (h, w))
+    for _ in range(3):
+        for g in got:
+            g.zero_()
+        graph.replay()
+        torch.autograd.grad(losses.head_cross_entropy(h, w, targets), (h, w))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("n", [4, 60, 140])
+@pytest.mark.parametrize("dim", [64, 66, 67])
+def test_what_lies_between_rows_of_the_head_is_not_used(dim, n, dtype):
+    """Rows that are apart, of lengths that end inside of 16 bytes, with NaN between them and behind the last one's end."""
+    hidden, weight, targets = _inputs(n, 300, dim, dtype)
+    apart = torch.full((300, 72), float("nan"), device=DEV, dtype=dtype)
+    apart[:, :dim] = weight
+    _check_logps(hidden, apart[:, :dim], targets)
+    _check_hidden_alone(hidden, apart[:, :dim], targets)
+
+
+@pytest.mark.parametrize("n,vocab,dim", [(385, 70_001, 72), (1_025, 300, 129), (1_100, 2_049, 264), (1_500, 7_000, 65), (1_025, 9_000, 33_000)])
+def test_more_rows_of_fp32(n, vocab, dim):
+    """In parts: tiles of 64 rows and of 256, more than one piece of the head."""
+    _check_logps(*_inputs(n, vocab, dim, FP32))
+    _check_ce(*_inputs(n, vocab, dim, FP32, seed=1), label_smoothing=0.1, z_loss=1e-3)
+
+
+def test_few_rows_of_fp32_whose_forward_kept_nothing():
+    """The operators' own call: the logits are made again."""
+    from micro_engram_fork_amd import head_ops
+    hidden, weight, targets = _inputs(40, 700, 96, FP32)
+    up = torch.randn(40, device=DEV)
+    logps, saved = head_ops.head_logps(hidden, weight, targets, -100, 1.0, head_ops.NO_GRADIENT)
+    gh, gw = head_ops.head_backward(hidden, weight, targets, saved, None, up, -100, 1.0, True, 0.0, 0.0, 1.0, 0, True, True)
+    want = ref.head(hidden, weight, targets, FP32, upstream=up)
+    _close(gh, want["hidden"], "hidden")
+    _close(gw, want["weight"], "weight")

@@ -52,9 +52,9 @@ def test_c_entry_checks():
 def test_fake_shapes():
     with FakeTensorMode():
         hidden, weight, targets = _args()
-        out, saved = head_ops.head_logps(hidden, weight, targets, -100, 1.0, False)
+        out, saved = head_ops.head_logps(hidden, weight, targets, -100, 1.0, head_ops.NO_GRADIENT)
         assert out.shape == (2, 3) and out.dtype is torch.float32
-        loss, saved = head_ops.head_ce(hidden, weight, targets, -100, 1.0, 0.0, 0.0, 1.0, 0, False)
+        loss, saved = head_ops.head_ce(hidden, weight, targets, -100, 1.0, 0.0, 0.0, 1.0, 0, head_ops.NO_GRADIENT)
         assert loss.shape == () and saved.shape == (16 + 5 * 6,)
         both = head_ops.head_backward(hidden, weight, targets, saved, None, loss, -100, 1.0, False, 0.0, 0.0, 1.0, 0, True, True)
         assert [g.shape for g in both] == [hidden.shape, weight.shape] and both[1].dtype is torch.bfloat16
@@ -64,12 +64,21 @@ def test_fake_shapes():
 
 def test_what_a_forward_leaves_for_the_gradient_of_hidden_alone():
     """Nothing for small calls; fp32 values of every row, in whole fours, for those worth it."""
-    assert head_ops.unit_elements(64, 300, 64, _lib.ME_BF16) == 0
-    assert head_ops.unit_elements(0, 262_144, 5_376, _lib.ME_BF16) == 0
-    assert head_ops.unit_elements(3, 262_144, 5_375, _lib.ME_BF16) == 3 * 5_376
+    of = head_ops.OF_HIDDEN
+    assert head_ops.unit_elements(64, 300, 64, _lib.ME_BF16, of) == 0
+    assert head_ops.unit_elements(0, 262_144, 5_376, _lib.ME_BF16, of) == 0
+    assert head_ops.unit_elements(3, 262_144, 5_375, _lib.ME_BF16, of) == 3 * 5_376
+    assert head_ops.unit_elements(3, 262_144, 5_375, _lib.ME_BF16, head_ops.OF_WEIGHT) == 0
+    assert head_ops.unit_elements(3, 262_144, 5_375, _lib.ME_BF16, head_ops.NO_GRADIENT) == 0
+    for of in (head_ops.OF_HIDDEN, head_ops.OF_WEIGHT):  # few rows of fp32: their logits
+        assert head_ops.unit_elements(384, 262_144, 64, _lib.ME_F32, of) == 384 * (262_144 + 64)
+        assert head_ops.unit_elements(385, 262_144, 64, _lib.ME_F32, of) == 0
+        assert head_ops.unit_elements(1024, 301, 64, _lib.ME_F32, of) == 1024 * 320
+        assert head_ops.unit_elements(1025, 301, 64, _lib.ME_F32, of) == 0
+        assert head_ops.unit_elements(0, 301, 64, _lib.ME_F32, of) == 0
     with FakeTensorMode():
         hidden, weight, targets = _args(rows=(4096,), vocab=32_000, dim=1_024)
-        _, saved, unit = head_ops.head_ce(hidden, weight, targets, -100, 1.0, 0.0, 0.0, 1.0, 0, True)
+        _, saved, unit = head_ops.head_ce(hidden, weight, targets, -100, 1.0, 0.0, 0.0, 1.0, 0, head_ops.OF_HIDDEN)
         assert unit.shape == (4096 * 1024,) and unit.dtype is torch.float32
 
 
