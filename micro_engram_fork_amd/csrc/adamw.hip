@@ -5,7 +5,9 @@
 //   p' = (1 - lr wd) p - lr / (1 - b1^t) m' / (sqrt(v') / sqrt(1 - b2^t) + eps)
 //
 // HBM-bound: every value is read once and written once, 22 bytes a weight (bf16 weights and gradients,
-// fp32 moments), 28 (all fp32) or 10 (bf16, 8-bit moments). A thread takes eight values that lie together,
+// fp32 moments), 28 (all fp32) or 10 (bf16, 8-bit moments). Measured: 341 million weights in fp32 1750 us, 5.4 TB/s;
+// 929 million in bf16 with 8-bit moments 1906 us, 4.9 TB/s; 16.5 million in bf16 with fp32 ones 55 us in the
+// kernel, 6.6 TB/s with the 256 MB cache's help. (A 4 GB copy: 4.8 TB/s.) A thread takes eight values that lie together,
 // so that each tensor moves in 8- to 16-byte pieces and one Philox call gives the rounding noise of all
 // eight; the tensors of a launch stand in the kernel's arguments (no table to upload, graphs replay it), and a
 // workgroup finds its tensor with one load and a ballot over their first chunks.
@@ -33,8 +35,8 @@ namespace me {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kPer = 8;                      // values per thread and round
-constexpr int kChunk = kThreads * kPer;       // values per workgroup: two or four rounds each took 3-8 % longer
+constexpr int kPer = 8;                      // values per thread
+constexpr int kChunk = kThreads * kPer;       // values per workgroup; two or four times as many in rounds took 3-8 % longer
 constexpr int kTensors = 42;                 // tensors per launch (kernel arguments stay under 4 KiB)
 constexpr int kBlock = 128;                  // values per scale of 8-bit moments
 constexpr int64_t kMostChunks = int64_t{1} << 23;

@@ -22,6 +22,10 @@ The backward looks (on the device) whether that held, and computes the gradient 
 logits if not: give a factor such as 1 / accumulation steps as `scale`, where it costs nothing. Under
 hooks on saved tensors (torch.autograd.graph.save_on_cpu, non-reentrant checkpointing) nothing is kept
 that does not pass through the hooks, and the gradient is written in the backward.
+
+head_cross_entropy and head_token_logps start before the logits, from the decoder's hidden states and head
+(the reference takes the cross-entropy in pieces of its logits, micro_engram/train/head.py:85-165): logits exist a tile at a
+time, and the gradients are of hidden states and head.
 """
 import functools
 import math
