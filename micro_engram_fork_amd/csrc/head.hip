@@ -31,7 +31,7 @@ constexpr double kLn2 = 0.69314718055994530942;
 // Rows up to which the tiles of few rows are taken (takes_few)
 constexpr int64_t kFew = 128;
 constexpr int64_t kPieceBytes = int64_t{1} << 30;        // of a piece's gradient, and of a piece of laid-out weights
-constexpr int kSplits = 3, kMostSplits = 16;             // of the product with W
+constexpr int kSplits = 3;                               // of a product that fills the chip without
 // Rows of fp32 up to which logits are kept (takes_kept)
 constexpr int64_t kKeptRows = 384, kKeptMost = 1024;
 constexpr int kHeader = 16;                              // ints before the rows in `saved`: the number of them
@@ -1442,7 +1442,7 @@ int64_t kept_ld(int64_t vocab) { return odd_lines(vocab); }
 
 // Parts of a reduction over `slabs` slabs that `tiles` tiles take to fill the chip, at least four slabs each
 int most_splits(int64_t tiles, int64_t slabs) {
-    return static_cast<int>(std::max<int64_t>(std::min<int64_t>({std::max<int64_t>(256 / tiles, kSplits), 64, slabs / 4}), 1));
+    return static_cast<int>(std::max<int64_t>(std::min<int64_t>({std::max<int64_t>(256 / tiles, kSplits), kMostSplits, slabs / 4}), 1));
 }
 
 // What a call by kept logits needs
@@ -1470,7 +1470,7 @@ KeptPlan kept_plan_of(int64_t n, int64_t vocab, int64_t dim, const void *weight,
         const int64_t tiles = p.row_tiles * ceil_div(vocab, kTile);
         // the sums' bytes against the head's
         p.logit_splits = tiles > 512 ? 1 : most_splits(tiles, ceil_div(dim, 32));
-        p.logit_cost = static_cast<int>(4096 * 2 * n / dim) + 1;
+        p.logit_cost = static_cast<int>(std::min<int64_t>(4096 * 2 * n / dim + 1, kMostCost));
         p.h = take(n * p.h_ld * 4);
         if (pass == kStats) p.logits = take(n * p.ld * 4);
         if (p.logit_splits > 1) p.partial = take(p.logit_splits * n * p.ld * 4);
@@ -1481,7 +1481,7 @@ KeptPlan kept_plan_of(int64_t n, int64_t vocab, int64_t dim, const void *weight,
         p.row_loss = take(n * 4);
     } else {
         p.splits = most_splits(p.row_tiles * ceil_div(dim, kTile), ceil_div(vocab, 32));
-        p.split_cost = static_cast<int>(4096 * 2 * n / vocab) + 1;
+        p.split_cost = static_cast<int>(std::min<int64_t>(4096 * 2 * n / vocab + 1, kMostCost));
         p.dz = take(n * p.ld * 4);
         p.acc = take(p.splits * n * p.h_ld * 4);
         p.dz_parts = take(ceil_div(n, kOuterRows) * vocab * kOuterBytes);

@@ -71,20 +71,20 @@ struct Gemm {
     int split_cost;        // of splits_for
 };
 
-// Parts of the reduction that tiles of C take so that the last round of workgroups is as full as it gets. Each
-// costs `cost` / 4096 of the product's own time (its sums are read and written once more). The rows may be
-// known to the device alone, so this is decided there, by whoever writes the parts and whoever adds them: in
-// integers, so that all of them come to the same.
+// Parts of the reduction that tiles of C take so that the last round of workgroups is as full as it gets: the number of
+// them, up to `most`, that takes least time, where each costs `cost` / 4096 of the product's own (its sums are read
+// and written once more). The rows may be known to the device alone, so this is decided there, by whoever writes the
+// parts and whoever adds them: in integers, so that all of them come to the same; lane l tries l + 1 parts, as one after the
+// other took 5 us. Called by whole waves.
+constexpr int kMostSplits = 64, kMostCost = 1 << 18;
 __device__ inline int splits_for(int tiles, int most, int cost) {
-    constexpr int64_t kCus = 256;
-    int best = 1;
-    int64_t least = int64_t{1} << 62;
-    for (int s = 1; s <= most; ++s) {
-        const int64_t all = static_cast<int64_t>(tiles) * s;
-        const int64_t time = (all + kCus - 1) / kCus * kCus * 4096 / all + static_cast<int64_t>(cost) * s;
-        if (time < least) least = time, best = s;
-    }
-    return best;
+    const uint32_t s = static_cast<uint32_t>(threadIdx.x & 63) + 1, all = static_cast<uint32_t>(tiles) * s;
+    // rounds of the chip's 256 CUs against the work, times 4096; past 2^19 workgroups they hardly differ
+    const uint32_t time = (all < (1u << 19) ? (((all + 255) / 256) << 20) / all : 4096u) + static_cast<uint32_t>(cost) * s;
+    uint32_t best = s <= static_cast<uint32_t>(most) ? time * 64 + s - 1 : ~0u;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) best = min(best, static_cast<uint32_t>(__shfl_xor(static_cast<int>(best), d)));
+    return __builtin_amdgcn_readfirstlane(static_cast<int>(best & 63)) + 1;
 }
 
 // segment -> parts of A and B: (0,0) (0,1) (1,0) and for SEGS 6 on to (0,2) (1,1) (2,0)

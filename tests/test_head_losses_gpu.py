@@ -499,7 +499,7 @@ def test_heads_of_rows_of_very_different_sizes():
 
 # ---- few rows of fp32, whose logits are kept ------------------------------------------------------------------------
 @pytest.mark.parametrize("n,vocab,dim", [(9, 1_000, 512), (31, 8_191, 100), (32, 20_001, 64), (33, 257, 1_023), (64, 3_000, 2_050), (90, 3_423, 1_000),
-                                         (96, 140_000, 36), (97, 511, 33), (128, 40_003, 260), (128, 700, 4_097), (2, 150_001, 129), (7, 600, 1_500),
+                                         (96, 140_000, 36), (97, 511, 33), (128, 40_003, 260), (128, 700, 4_097), (2, 150_001, 129), (7, 600, 1_500), (8, 900, 2_300),
                                          (129, 5_000, 68), (193, 70_001, 40), (384, 3_001, 200), (1_000, 515, 77), (1_024, 16_000, 24)])
 def test_few_rows_of_fp32(n, vocab, dim):
     """Tiles of 32 to 128 rows, one and more of them, splits of either reduction, heads whose rows start and end anywhere."""
