@@ -443,6 +443,11 @@ class DenseAdamW(_DirectOptimizer):
         for name, low, high in (("lr", 0.0, math.inf), ("eps", 0.0, math.inf), ("weight_decay", 0.0, math.inf)):
             if not low <= float(group[name]) < high:
                 raise ValueError(f"[micro_engram] DenseAdamW: {name} of {group[name]} is out of range")
+        if 0.0 < float(group["eps"]) < 1.2e-38:  # a denominator has to have a reciprocal in fp32
+            raise ValueError(f"[micro_engram] DenseAdamW: eps of {group['eps']} is below fp32's normal numbers")
+        for name, plain in (("amsgrad", False), ("maximize", False), ("decoupled_weight_decay", True)):  # of another Adam's state
+            if bool(group.get(name, plain)) is not plain:
+                raise ValueError(f"[micro_engram] DenseAdamW: {name}={not plain} is not supported")
         if len(group["betas"]) != 2 or not all(0.0 <= float(b) < 1.0 for b in group["betas"]):
             raise ValueError(f"[micro_engram] DenseAdamW: betas of {group['betas']} are out of range")
         if group["state_bits"] not in (32, 8):
@@ -470,9 +475,9 @@ class DenseAdamW(_DirectOptimizer):
         were saved (for state_bits 32 in fp32: torch.optim.AdamW's own may be bf16)."""
         saved = state_dict["state"]
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        for group in state_dict["param_groups"]:
+            self._check_group({**self.defaults, **group, "params": []})
         super().load_state_dict(state_dict)
-        for group in self.param_groups:
-            self._check_group(group)
         for i, (p, group) in zip(ids, [(p, g) for g in self.param_groups for p in g["params"]]):
             for name, value in saved.get(i, {}).items():
                 if name == "step":

@@ -12,7 +12,7 @@ def _param(dtype=torch.float32):
     return p
 
 
-@pytest.mark.parametrize("bad", [dict(state_bits=16), dict(state_bits="8"), dict(lr=-1.0), dict(lr=float("nan")), dict(eps=-1e-8),
+@pytest.mark.parametrize("bad", [dict(state_bits=16), dict(state_bits="8"), dict(lr=-1.0), dict(lr=float("nan")), dict(eps=-1e-8), dict(eps=1e-40), dict(eps=1e-60),
                                  dict(betas=(1.0, 0.9)), dict(betas=(0.9, -0.1)), dict(betas=(0.9,)), dict(weight_decay=-1.0)])
 def test_hyperparameters(bad):
     with pytest.raises(ValueError, match="micro_engram"):
@@ -96,3 +96,19 @@ def test_copies_and_older_states_have_every_setting():
     saved = DenseAdamW([_param()], seed=5).state_dict()
     opt.load_state_dict(saved)
     assert opt.seed == 5 and opt.param_groups[0]["state_bits"] == 32
+
+
+@pytest.mark.parametrize("torchs", [lambda p: torch.optim.AdamW(p, amsgrad=True), lambda p: torch.optim.AdamW(p, maximize=True), torch.optim.Adam])
+def test_states_of_other_formulas_are_refused(torchs):
+    """And nothing of them is taken."""
+    p = _param()
+    state = torchs([p]).state_dict()
+    if torchs is torch.optim.Adam and "decoupled_weight_decay" not in state["param_groups"][0]:
+        pytest.skip("this torch's Adam does not say so")
+    opt = DenseAdamW([p], lr=0.25)
+    with pytest.raises(ValueError, match="not supported"):
+        opt.load_state_dict(state)
+    assert opt.param_groups[0]["lr"] == 0.25 and "amsgrad" not in opt.param_groups[0]
+    plain = torch.optim.AdamW([p], lr=0.5)
+    opt.load_state_dict(plain.state_dict())
+    assert opt.param_groups[0]["lr"] == 0.5
