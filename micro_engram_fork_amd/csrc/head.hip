@@ -1933,15 +1933,21 @@ int forward(int64_t n, int64_t vocab, int64_t dim, int dtype, const Call &c, con
     return check_launch("me_head");
 }
 
-int check_call(const void *hidden, int dtype, int64_t n, int64_t dim, int64_t per_batch, const void *weight, int64_t vocab, int64_t w_stride,
-               const void *targets, int tdtype, double temperature, const void *saved, const void *ws) {
-    ME_CHECK_ARG(dtype == ME_BF16 || dtype == ME_F32, "dtype must be bf16/fp32");
-    ME_CHECK_ARG(tdtype == ME_I32 || tdtype == ME_I64, "targets must be int32/int64");
+int check_sizes(int64_t n, int64_t vocab, int64_t dim, int64_t w_stride) {
     ME_CHECK_ARG(n >= 0 && n <= (int64_t{1} << 24), "n must be in 0..2^24");
     ME_CHECK_ARG(dim >= 1 && dim <= 65536, "dim must be in 1..65536");
     ME_CHECK_ARG(ceil_div(n, 256) * ceil_div(dim, 256) <= (int64_t{1} << 22), "n times dim must be at most 2^38");
     ME_CHECK_ARG(vocab >= 1 && vocab <= (int64_t{1} << 21), "vocab must be in 1..2^21");
     ME_CHECK_ARG(w_stride >= dim && w_stride <= (int64_t{1} << 22), "weight rows must be dim or more elements apart, at most 2^22");
+    return ME_OK;
+}
+
+int check_call(const void *hidden, int dtype, int64_t n, int64_t dim, int64_t per_batch, const void *weight, int64_t vocab, int64_t w_stride,
+               const void *targets, int tdtype, double temperature, const void *saved, const void *ws) {
+    ME_CHECK_ARG(dtype == ME_BF16 || dtype == ME_F32, "dtype must be bf16/fp32");
+    ME_CHECK_ARG(tdtype == ME_I32 || tdtype == ME_I64, "targets must be int32/int64");
+    const int rc = check_sizes(n, vocab, dim, w_stride);
+    if (rc != ME_OK) return rc;
     ME_CHECK_ARG(n == 0 || (hidden && targets && per_batch >= 1), "hidden and targets are needed");
     ME_CHECK_ARG(weight && saved && ws, "weight, saved and workspace are needed");
     ME_CHECK_ARG(reinterpret_cast<uintptr_t>(saved) % 16 == 0 && reinterpret_cast<uintptr_t>(ws) % 16 == 0, "saved and workspace must be 16-byte aligned");
@@ -1956,7 +1962,9 @@ using namespace me;
 
 extern "C" int me_head_workspace_size(int64_t n, int64_t vocab, int64_t dim, int dtype, const void *weight, int64_t w_stride, int pass,
                                       int smoothed, size_t *bytes) {
-    ME_CHECK_ARG(bytes && n >= 0 && vocab >= 1 && dim >= 1 && pass >= kStats && pass <= kHasUnit, "bad sizes");
+    ME_CHECK_ARG(bytes && pass >= kStats && pass <= kHasUnit, "bad pass");
+    const int rc = check_sizes(n, vocab, dim, w_stride);
+    if (rc != ME_OK) return rc;
     if (takes_kept(n, vocab, dtype) && pass != kBackward) {
         *bytes = static_cast<size_t>(kept_plan_of(n, vocab, dim, weight, w_stride, static_cast<Pass>(pass), smoothed != 0).bytes);
         return ME_OK;
@@ -1966,7 +1974,9 @@ extern "C" int me_head_workspace_size(int64_t n, int64_t vocab, int64_t dim, int
 }
 
 extern "C" int me_head_unit_size(int64_t n, int64_t vocab, int64_t dim, int dtype, int for_weight, int64_t *elements) {
-    ME_CHECK_ARG(elements && n >= 0 && vocab >= 1 && dim >= 1, "bad sizes");
+    ME_CHECK_ARG(elements, "elements is needed");
+    const int rc = check_sizes(n, vocab, dim, dim);
+    if (rc != ME_OK) return rc;
     if (takes_kept(n, vocab, dtype))
         *elements = n * kept_ld(vocab);
     else

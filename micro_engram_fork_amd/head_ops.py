@@ -98,7 +98,8 @@ def _backward(hidden_shape, weight_shape, operands, like, saved, unit, upstream,
 
 def _fake_forward(hidden, weight, targets, gradients, shape):
     res = [hidden.new_empty(shape, dtype=torch.float32), hidden.new_empty((16 + 5 * targets.numel(),), dtype=torch.float32)]
-    size = unit_elements(targets.numel(), weight.shape[0], weight.shape[1], dtype_code(weight), gradients)
+    # whole numbers: symbolic sizes are fixed here, as they decide how many tensors there are
+    size = unit_elements(int(targets.numel()), int(weight.shape[0]), int(weight.shape[1]), dtype_code(weight), gradients)
     return [*res, hidden.new_empty((size,), dtype=torch.float32)] if size else res
 
 

@@ -568,3 +568,17 @@ def test_few_rows_of_fp32_whose_forward_kept_nothing():
     want = ref.head(hidden, weight, targets, FP32, upstream=up)
     _close(gh, want["hidden"], "hidden")
     _close(gw, want["weight"], "weight")
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_compiled_for_any_number_of_rows(dtype):
+    hidden, weight, targets = _inputs(300, 700, 72, dtype)
+    h = hidden.requires_grad_()
+
+    @torch.compile(backend="aot_eager", dynamic=True)
+    def f(h, t):
+        return losses.head_cross_entropy(h * 2, weight, t)
+    for n in (300, 40, 17):
+        g, = torch.autograd.grad(f(h[:n], targets[:n]), h)
+        want, = torch.autograd.grad(losses.head_cross_entropy(h[:n] * 2, weight, targets[:n]), h)
+        assert torch.equal(g, want), n

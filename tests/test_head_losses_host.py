@@ -113,3 +113,12 @@ def test_tensor_subclasses_go_through_the_ops(call, which, grad):
     args[which] = _Wrapped(args[which])
     with pytest.raises(_Reached):
         call(*args)
+
+
+@pytest.mark.parametrize("n,vocab,dim,apart", [((1 << 24) + 1, 4, 8, 8), (4, (1 << 21) + 1, 8, 8), (4, 4, 65_537, 65_537), (1 << 24, 4, 32_768, 32_768),
+                                               (4, 4, 8, (1 << 22) + 8), (4, 4, 8, 7)])
+def test_sizes_past_the_limits(n, vocab, dim, apart):
+    """Refused when the workspace is asked for, before any is allocated."""
+    for dtype in (_lib.ME_F32, _lib.ME_BF16):
+        with pytest.raises(RuntimeError, match="must be"):
+            head_ops.workspace_bytes(n, vocab, dim, dtype, 0, apart, 0, False)
