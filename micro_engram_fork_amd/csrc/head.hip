@@ -15,7 +15,10 @@
 // A row's target is kept out of the sums, as in the losses over logits: the weight of the others, and with it the
 // loss and the gradient at the target, keeps its digits where the target is all but certain.
 // Statistics are fp32; the logits' gradient is rounded to bf16 once (fp32 operands: three parts, exact) before its
-// products: one rounding of 2^-9 per term where the sum itself is rounded so at its end.
+// products: one rounding per term where the sum itself is rounded so at its end. Many terms average out, but a row's target
+// carries as much as all its other tokens together: what the rounding leaves of it is added to the hidden states' gradient
+// in fp32 (hidden_kernel), and for few rows, whose product with h is bound by its result, the head's gradient takes
+// what the rounding leaves of every value as more rows of the reduction (takes_rest).
 #include "head_gemm.h"
 
 #include <algorithm>
@@ -139,6 +142,7 @@ struct Layout {
     const int32_t *rows, *count;                  // sources of the rows and how many there are; null: as they are
     int64_t n, dim, ld, part;                     // part: bytes
     uint8_t *dst;
+    int again;                                    // the rows once more behind the last one
     const int32_t *gate;                          // a count; 0: nothing is laid out. Null: none
 };
 
@@ -201,6 +205,7 @@ __global__ __launch_bounds__(256) void layout_kernel(const Layout a, const Coefs
 #pragma unroll
         for (int p = 0; p < (F32 ? 3 : 1); ++p)
             *as_global(reinterpret_cast<u32x4_v *>(a.dst + p * a.part + (r * a.ld + c) * 2)) = u32x4_v{w[p][0], w[p][1], w[p][2], w[p][3]};
+        if (!F32 && a.again) *as_global(reinterpret_cast<u32x4_v *>(a.dst + ((n + r) * a.ld + c) * 2)) = u32x4_v{w[0][0], w[0][1], w[0][2], w[0][3]};
     }
 }
 
@@ -506,11 +511,12 @@ __device__ __forceinline__ int row_power(float row, uint32_t largest) {
 
 __device__ __forceinline__ float power_of(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
 
-// The logits' gradient of a tile as rows of a piece: bf16 for bf16 operands; for fp32 ones three bf16 parts where the
-// head's gradient is wanted, and two fp16 parts, times the columns' scales and the row's power, where the hidden
-// states' is
-template <bool F32>
+// The logits' gradient of a tile as rows of a piece: bf16 for bf16 operands (PARTS 1), with what that leaves of them as
+// rows behind the last counted one (2); for fp32 ones three bf16 parts where the head's gradient is wanted, and two
+// fp16 parts, times the columns' scales and the row's power, where the hidden states' is (3)
+template <int PARTS>
 struct GradEpilogue {
+    static constexpr bool F32 = PARTS == 3;
     const int32_t *tgt;
     Scales scales;
     const RowGrad *grad;
@@ -534,10 +540,10 @@ struct GradEpilogue {
     __device__ __forceinline__ void rows_of(const floatx16 (&acc)[SX][SY], const Tile &t, int row0, int col0, uint8_t *lds, int lane) const {
         const int64_t c0 = t.s0 + col0;
         const int there = static_cast<int>(max(min(vocab - c0, int64_t{32 * SX}), int64_t{0}));
-        constexpr int kParts = !F32 ? 1 : HALF ? 2 : 3;
+        constexpr int kParts = HALF ? 2 : PARTS;
         // 32 rows at a time through LDS, where a wave has two places in turn (with parts one: a wave's LDS
         // accesses keep their order)
-        constexpr int kPitch = 64 * SX + 16, kPlaces = F32 ? 1 : 2;
+        constexpr int kPitch = 64 * SX + 16, kPlaces = PARTS > 1 ? 1 : 2;
         static_assert(4 * kPlaces * kParts * 32 * kPitch <= (SX == 4 ? kRingBytes : 3 * kUnit), "the stage fits the ring");
 #pragma unroll
         for (int y = 0; y < SY; ++y) {
@@ -553,7 +559,7 @@ struct GradEpilogue {
                 stage_rows<AGPR, HALF, true, SX, SY>(acc, y, g, kr, up, c0, mine, there, stage, lane);
             else
                 stage_rows<AGPR, HALF, false, SX, SY>(acc, y, g, kr, up, c0, mine, there, stage, lane);
-            store_rows<kParts, SX>(stage, HALF ? half : out, ld, part, t.r0 + row0 + 32 * y, t.rows, c0, lane);
+            store_rows<kParts, SX>(stage, HALF ? half : out, ld, PARTS == 2 ? t.rows * ld * 2 : part, t.r0 + row0 + 32 * y, t.rows, c0, lane);
         }
     }
 
@@ -580,7 +586,7 @@ struct GradEpilogue {
                 if constexpr (HALF)
                     stage4_half<SX>(v, stage, 32 * x + 8 * q + half4, lane);
                 else
-                    stage4<F32 ? 3 : 1, SX>(v, stage, 32 * x + 8 * q + half4, lane);
+                    stage4<PARTS, SX>(v, stage, 32 * x + 8 * q + half4, lane);
             }
     }
 };
@@ -1213,15 +1219,33 @@ __device__ __forceinline__ void store4(void *out, int64_t at, int64_t c, int64_t
     }
 }
 
+// What bf16 leaves of the logits' gradient at the rows' targets
+struct Rest {
+    const RowGrad *grad;
+    const int32_t *tgt;
+    const uint16_t *weight;
+    int64_t w_stride;
+};
+
 // Gradient of the hidden states, source rows in their order: the splits' sums, or zeros
 template <bool F32>
-__global__ __launch_bounds__(256) void hidden_kernel(const Sums sums, const int32_t *place, const int32_t *count, int64_t n, int64_t dim, void *out) {
+__global__ __launch_bounds__(256) void hidden_kernel(const Sums sums, const int32_t *place, const int32_t *count, int64_t n, int64_t dim, const Rest rest, void *out) {
     const int64_t units = ceil_div(dim, 4);
     const int splits = sums.splits(*count);
     for (int64_t u = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; u < n * units; u += static_cast<int64_t>(gridDim.x) * 256) {
         const int64_t i = u / units, c = (u - i * units) * 4;
         const int64_t r = place[i];
-        store4<F32>(out, i * dim, c, dim, r >= 0 ? sums.row4(r, c, splits) : f32x4_v{0.f, 0.f, 0.f, 0.f});
+        f32x4_v v = {0.f, 0.f, 0.f, 0.f};
+        if (r >= 0) {
+            v = sums.row4(r, c, splits);
+            if constexpr (!F32) {
+                const float left = rest.grad[r].gt - round_to_bf16(rest.grad[r].gt);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (c + e < dim) v[e] = fmaf(left, bf16_bits_to_float(rest.weight[rest.tgt[r] * rest.w_stride + c + e]), v[e]);
+            }
+        }
+        store4<F32>(out, i * dim, c, dim, v);
     }
 }
 
@@ -1399,6 +1423,7 @@ struct Plan {
     int64_t n, rows, vocab, dim, ld;  // rows: n rounded up, at least 64; ld: dim rounded up to whole slabs
     bool f32, few, copy_w;            // copy_w: the head is laid out piece by piece
     int tile;                         // rows of a tile
+    bool rest;                        // the gradient's rows twice: as bf16, and what that leaves
     int np, nz;                       // parts of an operand: of the head's gradient; of the logits and the hidden states' gradient
     int64_t piece;                    // columns of the vocabulary at a time
     int splits;                       // of the product with W, at most
@@ -1491,6 +1516,11 @@ KeptPlan kept_plan_of(int64_t n, int64_t vocab, int64_t dim, const void *weight,
     return p;
 }
 
+// Whether the head's gradient takes what bf16 leaves of the logits' gradient: few rows, where one value's rounding can
+// make most of a result's error (2 rows: up to 2.5 times that of rounding the result alone, 1.0 with it; 128 rows: 1.3 to
+// 1.5). The product is bound by the write of its result, and K of 128 or 256 makes no difference to it.
+bool takes_rest(int64_t n, bool f32) { return !f32 && n <= kFew; }
+
 int few_rows(int64_t n, int64_t vocab) { return n <= 64 || ceil_div(n, 64) * ceil_div(vocab, kTile) <= 256 ? 64 : 128; }
 
 Plan plan_of(int64_t n, int64_t vocab, int64_t dim, int dtype, const void *weight, int64_t w_stride, Pass pass, bool smoothed) {
@@ -1500,6 +1530,7 @@ Plan plan_of(int64_t n, int64_t vocab, int64_t dim, int dtype, const void *weigh
     p.np = p.f32 ? 3 : 1;
     p.nz = p.f32 ? 2 : 1;
     p.few = takes_few(n, vocab, dim, p.f32);
+    p.rest = pass == kBackward && takes_rest(n, p.f32);
     p.copy_w = p.f32 || dim % 8 != 0 || w_stride % 8 != 0 || reinterpret_cast<uintptr_t>(weight) % 16 != 0;
     p.tile = p.few ? few_rows(n, vocab) : kTile;
     const int64_t rows = p.rows = round_up(std::max<int64_t>(n, 1), 64);
@@ -1515,7 +1546,7 @@ Plan plan_of(int64_t n, int64_t vocab, int64_t dim, int dtype, const void *weigh
         return here;
     };
     p.grad = take(n * static_cast<int64_t>(sizeof(RowGrad)));
-    p.z = take(rows * p.ld * 2 * p.nz);
+    p.z = take(rows * p.ld * 2 * (p.rest ? 2 : p.nz));
     p.h = p.z;
     if (p.copy_w) p.wz = take(p.piece * p.ld * 2 * p.nz);
     if (p.f32) {
@@ -1536,7 +1567,7 @@ Plan plan_of(int64_t n, int64_t vocab, int64_t dim, int dtype, const void *weigh
         p.row_loss = take(n * 4);
     }
     if (pass != kStats) {
-        p.g = take(rows * p.piece * 2 * p.np);
+        p.g = take(rows * p.piece * 2 * (p.rest ? 2 : p.np));
         // at least eight slabs each; parts of few tiles are as many as fill the chip, those of many at most kSplits
         const int64_t tiles = ceil_div(rows, p.tile) * ceil_div(dim, kTile);
         p.splits = static_cast<int>(std::max<int64_t>(std::min<int64_t>({std::max<int64_t>(256 / tiles, kSplits), kMostSplits, p.piece / kSlabK / 8}), 1));
@@ -1588,7 +1619,7 @@ void lay_out(bool f32, const Layout &l, hipStream_t s, const Coefs &k = Coefs{})
 int64_t h_part(const Plan &p) { return p.rows * p.ld * 2; }
 
 Layout hidden_layout(const Plan &p, const Call &c, int64_t to) {
-    return {c.hidden, c.per_batch, c.batch_stride, c.row_stride, c.s.rows, c.s.count, p.n, p.dim, p.ld, h_part(p), c.ws + to};
+    return {c.hidden, c.per_batch, c.batch_stride, c.row_stride, c.s.rows, c.s.count, p.n, p.dim, p.ld, h_part(p), c.ws + to, p.rest};
 }
 
 void lay_out16(const Layout &l, float *scale, uint32_t *largest, hipStream_t s, const Coefs &k = Coefs{}) {
@@ -1624,7 +1655,7 @@ Head head_of(const Plan &p, const Call &c, int64_t v0, int64_t width, uint32_t *
     const uint8_t *from = static_cast<const uint8_t *>(c.weight) + v0 * c.w_stride * (p.f32 ? 4 : 2);
     if (!p.copy_w) return {{from, c.w_stride, 0}, nullptr};
     const int64_t part = p.piece * p.ld * 2;
-    const Layout l{from, width, 0, c.w_stride, nullptr, nullptr, width, p.dim, p.ld, part, c.ws + p.wz, gate};
+    const Layout l{from, width, 0, c.w_stride, nullptr, nullptr, width, p.dim, p.ld, part, c.ws + p.wz, 0, gate};
     float *scale = p.f32 ? reinterpret_cast<float *>(c.ws + p.col_scale) : nullptr;
     if (p.f32)
         lay_out16(l, scale, largest, c.stream);
@@ -1699,13 +1730,19 @@ Sums sums_of(const Plan &p, const Call &c) {
 }
 
 // gradient of the logits of a piece, for the products that follow
-template <bool F32>
+template <int PARTS>
 void gradient_of(const Plan &p, const Call &c, const Rows &rows, const Head &w, int64_t v0, int64_t width, const RowGrad *grad, float k,
                  const uint32_t *largest, bool for_hidden, bool for_weight) {
-    const GradEpilogue<F32> e{rows.tgt, {rows.scale, w.scale}, grad, F32 ? reinterpret_cast<const float *>(c.ws + p.bound) : nullptr, largest,
-                              !F32 || for_weight ? c.ws + p.g : nullptr, F32 && for_hidden ? c.ws + p.half : nullptr, p.piece,
-                              p.rows * p.piece * 2, v0, width, k};
-    logits_of<F32 ? 3 : 1>(p, c, rows, w, width, e);
+    constexpr bool kF32 = PARTS == 3;
+    const GradEpilogue<PARTS> e{rows.tgt, {rows.scale, w.scale}, grad, kF32 ? reinterpret_cast<const float *>(c.ws + p.bound) : nullptr, largest,
+                                !kF32 || for_weight ? c.ws + p.g : nullptr, kF32 && for_hidden ? c.ws + p.half : nullptr, p.piece,
+                                p.rows * p.piece * 2, v0, width, k};
+    if constexpr (PARTS == 2) {  // few rows
+        const Gemm g{{rows.h, p.ld, 0}, w.w, p.n, width, p.dim, rows.count, 0, 8, 1, 0};
+        multiply_few<true, 1>(p.tile, g, e, c.stream);
+    } else {
+        logits_of<PARTS>(p, c, rows, w, width, e);
+    }
 }
 
 void finish(const Plan &p, const FinishArgs &f, hipStream_t s) {
@@ -1802,7 +1839,7 @@ void forward_rows(const Plan &p, const Call &c, const Loss &l) {
     RowGrad *grad = reinterpret_cast<RowGrad *>(c.ws + p.grad);
     const Rows again{c.ws + p.h2, redo, tgt2, nullptr};
     hipLaunchKernelGGL(redo_kernel, dim3(1), dim3(kIndexThreads), 0, s, RedoArgs{c.s, ref, rows.tgt, redo, redo + kHeader, tgt2});
-    lay_out(false, Layout{rows.h, p.n, 0, p.ld, redo + kHeader, redo, p.n, p.ld, p.ld, 0, again.h}, s);
+    lay_out(false, Layout{rows.h, p.n, 0, p.ld, redo + kHeader, redo, p.n, p.ld, p.ld, 0, again.h, 0, nullptr}, s);
     stats_of<F32>(p, c, again, e, redo);
     f.uncounted = 0, f.exps = nullptr, f.ref = nullptr, f.count = redo, f.which = redo + kHeader;
     finish(p, f, s);
@@ -1810,7 +1847,7 @@ void forward_rows(const Plan &p, const Call &c, const Loss &l) {
     for (int64_t v0 = 0; v0 < p.vocab; v0 += p.piece) {
         const int64_t width = std::min(p.piece, p.vocab - v0);
         const Head w = head_of(p, c, v0, width, nullptr, redo);
-        gradient_of<false>(p, c, again, w, v0, width, grad, k, nullptr, true, false);
+        gradient_of<1>(p, c, again, w, v0, width, grad, k, nullptr, true, false);
         times_head(p, c, again, w, v0, width);
     }
     unit_of(p, c, l, again, redo + kHeader, nullptr);
@@ -1830,7 +1867,7 @@ void vector_rows(const VectorArgs &a, int rows, unsigned groups, size_t lds, hip
 void forward_kept(const KeptPlan &p, const Call &c, const Loss &l) {
     hipStream_t s = c.stream;
     // rows gathered and padded to whole slabs: copied as pairs of 16-bit values
-    const Layout rows{c.hidden, c.per_batch, 2 * c.batch_stride, 2 * c.row_stride, c.s.rows, c.s.count, p.n, 2 * p.dim, 2 * p.h_ld, 0, c.ws + p.h};
+    const Layout rows{c.hidden, c.per_batch, 2 * c.batch_stride, 2 * c.row_stride, c.s.rows, c.s.count, p.n, 2 * p.dim, 2 * p.h_ld, 0, c.ws + p.h, 0, nullptr};
     lay_out(false, rows, s);
     float *logits = l.unit ? l.unit : reinterpret_cast<float *>(c.ws + p.logits);
     float *partial = p.logit_splits > 1 ? reinterpret_cast<float *>(c.ws + p.partial) : nullptr;
@@ -1865,7 +1902,7 @@ void backward_kept(const KeptPlan &p, const Call &c, const Coefs &k, const float
         float *acc = reinterpret_cast<float *>(c.ws + p.acc);
         multiply_kept<false>(p, g, AccumulateEpilogue{acc, p.h_ld, p.n * p.h_ld, 0, nullptr, nullptr}, s);
         const Sums sums{acc, p.h_ld, p.n * p.h_ld, p.tile, static_cast<int>(ceil_div(p.dim, kTile)), p.splits, p.split_cost};
-        hipLaunchKernelGGL(hidden_kernel<true>, dim3(blocks_for(p.n * ceil_div(p.dim, 4))), dim3(256), 0, s, sums, c.s.place, c.s.count, p.n, p.dim, grad_hidden);
+        hipLaunchKernelGGL(hidden_kernel<true>, dim3(blocks_for(p.n * ceil_div(p.dim, 4))), dim3(256), 0, s, sums, c.s.place, c.s.count, p.n, p.dim, Rest{}, grad_hidden);
     }
     if (grad_weight) {
         const Layout h{c.hidden, c.per_batch, c.batch_stride, c.row_stride, c.s.rows, c.s.count, p.n, p.dim};
@@ -2063,12 +2100,17 @@ extern "C" int me_head_backward(const void *hidden, int dtype, int64_t n, int64_
             uint32_t *widest = f32 ? largest + v0 / p.piece : nullptr;
             const Head w = head_of(p, c, v0, width, widest);
             const bool for_hidden = grad_hidden != nullptr, for_weight = grad_weight != nullptr;
-            f32 ? gradient_of<true>(p, c, rows, w, v0, width, grad, k, widest, for_hidden, for_weight)
-                : gradient_of<false>(p, c, rows, w, v0, width, grad, k, widest, for_hidden, for_weight);
+            if (f32)
+                gradient_of<3>(p, c, rows, w, v0, width, grad, k, widest, for_hidden, for_weight);
+            else if (p.rest && for_weight)
+                gradient_of<2>(p, c, rows, w, v0, width, grad, k, widest, for_hidden, for_weight);
+            else
+                gradient_of<1>(p, c, rows, w, v0, width, grad, k, widest, for_hidden, for_weight);
             if (grad_hidden) times_head(p, c, rows, w, v0, width, widest);
         }
         if (grad_weight) {
-            const Gemm g{{c.ws + p.g, p.piece, p.rows * p.piece * 2}, {c.ws + p.h, p.ld, h_part(p)}, width, dim, n, c.s.count, 1, 8, 1, 0};
+            const int times = p.rest ? 2 : 1;
+            const Gemm g{{c.ws + p.g, p.piece, p.rows * p.piece * 2}, {c.ws + p.h, p.ld, h_part(p)}, width, dim, n * times, c.s.count, 1, 8, 1, 0, times};
             uint8_t *out = static_cast<uint8_t *>(grad_weight) + v0 * dim * (f32 ? 4 : 2);
             if (f32)
                 multiply_large<false, false, 6>(g, WeightEpilogue<true>{out, dim}, s);
@@ -2078,10 +2120,11 @@ extern "C" int me_head_backward(const void *hidden, int dtype, int64_t n, int64_
     }
     if (grad_hidden && n > 0) {
         const unsigned blocks = blocks_for(n * ceil_div(dim, 4));
+        const Rest rest{grad, rows.tgt, static_cast<const uint16_t *>(weight), w_stride};
         if (f32)
-            hipLaunchKernelGGL(hidden_kernel<true>, dim3(blocks), dim3(256), 0, s, sums_of(p, c), c.s.place, c.s.count, n, dim, grad_hidden);
+            hipLaunchKernelGGL(hidden_kernel<true>, dim3(blocks), dim3(256), 0, s, sums_of(p, c), c.s.place, c.s.count, n, dim, Rest{}, grad_hidden);
         else
-            hipLaunchKernelGGL(hidden_kernel<false>, dim3(blocks), dim3(256), 0, s, sums_of(p, c), c.s.place, c.s.count, n, dim, grad_hidden);
+            hipLaunchKernelGGL(hidden_kernel<false>, dim3(blocks), dim3(256), 0, s, sums_of(p, c), c.s.place, c.s.count, n, dim, rest, grad_hidden);
     }
     return check_launch("me_head_backward");
 }

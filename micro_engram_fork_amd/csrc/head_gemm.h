@@ -69,6 +69,7 @@ struct Gemm {
     int group;             // column tiles that follow one another before the next row tile
     int most_splits;       // parts of the reduction, each with an output of its own: up to so many (splits_for)
     int split_cost;        // of splits_for
+    int times = 1;         // rows of K for each that `count` counts
 };
 
 // Parts of the reduction that tiles of C take so that the last round of workgroups is as full as it gets: the number of
@@ -228,7 +229,7 @@ __device__ __forceinline__ bool tile_of(const Gemm &a, int tr, int ts, int slab,
     if (a.count != nullptr) {
         const int64_t n = *as_global(a.count);
         if (a.count_is_k)
-            k = min(k, n);
+            k = min(k, n * a.times);
         else
             rows = min(rows, n);
     }

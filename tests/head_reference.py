@@ -5,7 +5,8 @@ most 2^-24 of the sum of the products' sizes so far; fp32 operands as bf16 parts
 out under 2^-24): dz = (dim + 8) 2^-24 sum |h w| / T, three times that for fp32. Statistics are sums of positive
 terms in fp32: their logs are off by dz and by 2e-6 (fewer than 16 roundings in a row of each tree, exponentials of
 2 ulp). A value of the gradient dz_ij is off relatively by twice that (its exponent and its sum) and by 1e-6 of its
-roundings, to which bf16 adds 2^-8; its products with W or h are accumulated in fp32, and the result is
+roundings, to which bf16 adds 2^-8: not at a row's target for the gradient of the hidden states, and up to 128 rows
+(counted or not) only 2^-16 for that of the head; its products with W or h are accumulated in fp32, and the result is
 rounded to its type (half a step: 2^-8 or 2^-24). Exponentials and bf16 parts under 2^-126, the smallest normal number,
 may be taken as zeros: 2^-126 more for q, times the row's factor, and for the value of the gradient itself."""
 import torch
@@ -63,10 +64,13 @@ def head(hidden, weight, targets, dtype, temperature=1.0, ignore_index=-100, ups
     extra = (a - 1).abs() + (smoothing if upstream is None else 0.0) + b
     dg[rows, t] = a.abs() * (others * (2 * dmax + dlog + 1e-6)) + factor + 2.0 ** -22 * (extra + at.abs())
     half = 2.0 ** -24 if wide else 2.0 ** -8
-    g, dg = g * c[:, None], (dg + g.abs() * (2.0 ** -22 if wide else half)) * c.abs()[:, None]
+    rounded = {"hidden": g.abs() * half, "weight": g.abs() * (half if targets.shape[0] > 128 else half * half)}
+    rounded["hidden"][rows, t] = 0.0
+    g, dg = g * c[:, None], (dg + g.abs() * 2.0 ** -22) * c.abs()[:, None]
     dg = dg + 2.0 ** -126 * (1 + (a * c).abs()[:, None])
     for name, value, x, y, k in (("hidden", g @ w, g.abs(), w.abs(), vocab), ("weight", g.t() @ h, g.abs().t(), h.abs(), n)):
-        d = dg if name == "hidden" else dg.t()
+        d = dg if wide else dg + rounded[name] * c.abs()[:, None]
+        d = d if name == "hidden" else d.t()
         err = d @ y + (3 if wide else 1) * (k + 8) * 2.0 ** -24 * (x @ y) + half * (value.abs() + d @ y) + 2.0 ** -133
         out[name] = (full(value), full(err)) if name == "hidden" else (value, err)
     return out
