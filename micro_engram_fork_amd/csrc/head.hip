@@ -99,11 +99,15 @@ struct Coefs {
     double scale;           // of the loss, over T
     float smoothing, z_loss;
     double vocab;
+    float *factor;          // null, or takes what all rows share: theirs are then for an upstream of 1, loss a plain sum
     RowGrad *grad;          // null: none of this is wanted
     float *bound;           // of each row's values, or null
     uint32_t *largest;      // set to 0, `pieces` of them
     int pieces;
 
+    __device__ __forceinline__ double shared(int64_t count) const {
+        return static_cast<double>(*upstream) * scale / (mean ? static_cast<double>(max(count, int64_t{1})) : 1.0);
+    }
     __device__ __forceinline__ RowGrad of(int64_t r, int64_t count) const {
         const float lse2 = s.lse2[r], o = s.others[r];
         RowGrad g;
@@ -112,7 +116,7 @@ struct Coefs {
             const float c = static_cast<float>(-static_cast<double>(upstream[s.rows[r]]) * scale);
             g.ca = c, g.cb = 0.f, g.gt = -c * o;
         } else {
-            const double c = static_cast<double>(*upstream) * scale / (mean ? static_cast<double>(max(count, int64_t{1})) : 1.0);
+            const double c = factor != nullptr ? 1.0 : shared(count);
             const double more = 2.0 * z_loss * kLn2 * lse2, e = smoothing;
             g.ca = static_cast<float>(c * (1.0 + more));
             g.cb = static_cast<float>(c * e / vocab);
@@ -175,6 +179,7 @@ __global__ __launch_bounds__(256) void layout_kernel(const Layout a, const Coefs
     if (a.gate != nullptr && *a.gate == 0) return;
     const int64_t units = a.ld / 8;
     const int64_t n = a.count ? min(a.n, static_cast<int64_t>(*a.count)) : a.n;
+    if (k.factor != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *k.factor = static_cast<float>(k.shared(n));
     for (int64_t u = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; u < n * units; u += static_cast<int64_t>(gridDim.x) * 256) {
         const int64_t r = u / units, c = (u - r * units) * 8;
         if (k.grad != nullptr && c == 0) k.row(r, n);
@@ -634,11 +639,13 @@ template <bool F32>
 struct WeightEpilogue {
     uint8_t *out;
     int64_t dim;
+    const float *factor;  // of bf16: what all values are multiplied by, or null
 
     template <bool AGPR, int SX, int SY>
     __device__ __forceinline__ void run(const floatx16 (&acc)[SX][SY], const Tile &t, int row0, int col0, uint8_t *lds, int lane) const {
         const int half4 = 4 * (lane >> 5);
         const bool whole = dim % 8 == 0;  // rows of whole 16-byte chunks
+        const float f = !F32 && factor != nullptr ? *as_global(factor) : 1.f;
 #pragma unroll
         for (int y = 0; y < SY; ++y) {
             if (!F32 && whole) {
@@ -651,7 +658,7 @@ struct WeightEpilogue {
                     for (int g = 0; g < 4; ++g) {
                         float v[4];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) v[e] = acc_read<AGPR>(acc[x][y], 4 * g + e);
+                        for (int e = 0; e < 4; ++e) v[e] = acc_read<AGPR>(acc[x][y], 4 * g + e) * f;
                         stage4<1, SX>(v, stage, 32 * x + 8 * g + half4, lane);
                     }
                 store_rows<1, SX>(stage, out, dim, 0, t.r0 + row0 + 32 * y, t.rows, t.s0 + col0, lane);
@@ -665,7 +672,7 @@ struct WeightEpilogue {
                     const int64_t col = t.s0 + col0 + 32 * x + 8 * g + half4;
                     f32x4_v v;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = acc_read<AGPR>(acc[x][y], 4 * g + e);
+                    for (int e = 0; e < 4; ++e) v[e] = acc_read<AGPR>(acc[x][y], 4 * g + e) * f;
                     if (row >= t.rows) continue;
                     if (F32 && dim % 4 == 0) {
                         if (col < dim) *as_global(reinterpret_cast<f32x4_v *>(reinterpret_cast<float *>(out) + row * dim + col)) = v;
@@ -1159,7 +1166,7 @@ __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs a) {
     for (int i = 1; i < kLast; ++i) all = join(all, s_all[tid + i * kRows]), sum += s_sum[tid + i * kRows];
     // d: how far the others' sum is over the target, log2
     const float zt = a.at_target[r], rest = all.m + log2f(all.s);
-    const float d = rest - zt;
+    const float d = (all.m - zt) + log2f(all.s);  // the difference of two large values first: nothing is rounded
     const float e = exp2f(-fabsf(d)), more = log1pf(e);
     const float nll = static_cast<float>(kLn2) * fmaxf(d, 0.f) + more;
     const float others = d > 0.f ? 1.f / (1.f + e) : e / (1.f + e);
@@ -1225,6 +1232,7 @@ struct Rest {
     const int32_t *tgt;
     const uint16_t *weight;
     int64_t w_stride;
+    const float *factor;  // of the whole, or null
 };
 
 // Gradient of the hidden states, source rows in their order: the splits' sums, or zeros
@@ -1232,6 +1240,7 @@ template <bool F32>
 __global__ __launch_bounds__(256) void hidden_kernel(const Sums sums, const int32_t *place, const int32_t *count, int64_t n, int64_t dim, const Rest rest, void *out) {
     const int64_t units = ceil_div(dim, 4);
     const int splits = sums.splits(*count);
+    const float f = !F32 && rest.factor != nullptr ? *as_global(rest.factor) : 1.f;
     for (int64_t u = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; u < n * units; u += static_cast<int64_t>(gridDim.x) * 256) {
         const int64_t i = u / units, c = (u - i * units) * 4;
         const int64_t r = place[i];
@@ -1242,7 +1251,7 @@ __global__ __launch_bounds__(256) void hidden_kernel(const Sums sums, const int3
                 const float left = rest.grad[r].gt - round_to_bf16(rest.grad[r].gt);
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (c + e < dim) v[e] = fmaf(left, bf16_bits_to_float(rest.weight[rest.tgt[r] * rest.w_stride + c + e]), v[e]);
+                    if (c + e < dim) v[e] = f * fmaf(left, bf16_bits_to_float(rest.weight[rest.tgt[r] * rest.w_stride + c + e]), v[e]);
             }
         }
         store4<F32>(out, i * dim, c, dim, v);
@@ -1429,7 +1438,7 @@ struct Plan {
     int splits;                       // of the product with W, at most
     int split_cost;
     int64_t h, part, sum, at_target, row_loss, g, grad, acc;  // workspace offsets
-    int64_t ref, redo, h2, tgt2, columns, column_part;
+    int64_t ref, redo, h2, tgt2, columns, column_part, factor;
     int64_t z, wz, row_scale, col_scale;  // operands of the logits; fp32: fp16 parts, and their scales
     int64_t half, bound, largest;         // fp32: the gradient in fp16 parts, its rows' bounds, the scales' largest by piece
     int64_t bytes;
@@ -1546,6 +1555,7 @@ Plan plan_of(int64_t n, int64_t vocab, int64_t dim, int dtype, const void *weigh
         return here;
     };
     p.grad = take(n * static_cast<int64_t>(sizeof(RowGrad)));
+    p.factor = take(4);
     p.z = take(rows * p.ld * 2 * (p.rest ? 2 : p.nz));
     p.h = p.z;
     if (p.copy_w) p.wz = take(p.piece * p.ld * 2 * p.nz);
@@ -2086,9 +2096,12 @@ extern "C" int me_head_backward(const void *hidden, int dtype, int64_t n, int64_
     uint32_t *largest = f32 ? reinterpret_cast<uint32_t *>(c.ws + p.largest) : nullptr;
     RowGrad *grad = reinterpret_cast<RowGrad *>(c.ws + p.grad);
     Rows rows{};
+    // bf16: factors that all rows share come in after the products, so that a target of no probability is -1, which
+    // bf16 holds, and no small factor takes values out of its range
+    float *factor = !f32 && !upstream_per_row && n > 0 ? reinterpret_cast<float *>(c.ws + p.factor) : nullptr;
     if (n > 0) {
         const Coefs coefs{c.s, upstream, upstream_per_row != 0, reduction == ME_REDUCE_MEAN, scale / temperature, static_cast<float>(smoothing),
-                          static_cast<float>(z_loss), static_cast<double>(vocab), grad, f32 ? reinterpret_cast<float *>(c.ws + p.bound) : nullptr,
+                          static_cast<float>(z_loss), static_cast<double>(vocab), factor, grad, f32 ? reinterpret_cast<float *>(c.ws + p.bound) : nullptr,
                           largest, f32 ? static_cast<int>(ceil_div(vocab, p.piece)) : 0};
         rows = lay_out_rows(p, c, coefs);
         if (f32 && grad_weight) lay_out(true, hidden_layout(p, c, p.h), s);
@@ -2113,14 +2126,14 @@ extern "C" int me_head_backward(const void *hidden, int dtype, int64_t n, int64_
             const Gemm g{{c.ws + p.g, p.piece, p.rows * p.piece * 2}, {c.ws + p.h, p.ld, h_part(p)}, width, dim, n * times, c.s.count, 1, 8, 1, 0, times};
             uint8_t *out = static_cast<uint8_t *>(grad_weight) + v0 * dim * (f32 ? 4 : 2);
             if (f32)
-                multiply_large<false, false, 6>(g, WeightEpilogue<true>{out, dim}, s);
+                multiply_large<false, false, 6>(g, WeightEpilogue<true>{out, dim, nullptr}, s);
             else
-                multiply_large<false, false, 1>(g, WeightEpilogue<false>{out, dim}, s);
+                multiply_large<false, false, 1>(g, WeightEpilogue<false>{out, dim, factor}, s);
         }
     }
     if (grad_hidden && n > 0) {
         const unsigned blocks = blocks_for(n * ceil_div(dim, 4));
-        const Rest rest{grad, rows.tgt, static_cast<const uint16_t *>(weight), w_stride};
+        const Rest rest{grad, rows.tgt, static_cast<const uint16_t *>(weight), w_stride, factor};
         if (f32)
             hipLaunchKernelGGL(hidden_kernel<true>, dim3(blocks), dim3(256), 0, s, sums_of(p, c), c.s.place, c.s.count, n, dim, Rest{}, grad_hidden);
         else
