@@ -34,7 +34,7 @@ constexpr double kLn2 = 0.69314718055994530942;
 // Rows up to which the tiles of few rows are taken (takes_few)
 constexpr int64_t kFew = 128;
 constexpr int64_t kPieceBytes = int64_t{1} << 30;        // of a piece's gradient, and of a piece of laid-out weights
-constexpr int kSplits = 3;                               // of a product that fills the chip without
+constexpr int kSplits = 8;                               // of a product that fills the chip without
 // Rows of fp32 up to which logits are kept (takes_kept)
 constexpr int64_t kKeptRows = 384, kKeptMost = 1024;
 constexpr int kHeader = 16;                              // ints before the rows in `saved`: the number of them
@@ -1578,11 +1578,14 @@ Plan plan_of(int64_t n, int64_t vocab, int64_t dim, int dtype, const void *weigh
     }
     if (pass != kStats) {
         p.g = take(rows * p.piece * 2 * (p.rest ? 2 : p.np));
-        // at least eight slabs each; parts of few tiles are as many as fill the chip, those of many at most kSplits
+        // at least eight slabs each; parts of few tiles are as many as fill the chip, those of many up to kSplits as far as
+        // their sums take a piece's memory (2049 rows, 262,144 x 5376: 189 tiles in 4 parts are 2.95 rounds, in 3 2.2)
         const int64_t tiles = ceil_div(rows, p.tile) * ceil_div(dim, kTile);
-        p.splits = static_cast<int>(std::max<int64_t>(std::min<int64_t>({std::max<int64_t>(256 / tiles, kSplits), kMostSplits, p.piece / kSlabK / 8}), 1));
-        // reading and writing the sums at 4.8 TB/s against a piece's products at 1.25 PFLOP/s
-        p.split_cost = static_cast<int>(4096 * (8.0 / 4.8e12) / (2.0 * static_cast<double>(p.piece) * (p.f32 ? 3 : 1) / 1.25e15)) + 1;
+        const int64_t most = std::max<int64_t>(256 / tiles, std::min<int64_t>(kSplits, kPieceBytes / (rows * p.ld * 4)));
+        p.splits = static_cast<int>(std::max<int64_t>(std::min<int64_t>({most, kMostSplits, p.piece / kSlabK / 8}), 1));
+        // reading and writing the sums at 4.8 TB/s against a piece's products at 1.25 PFLOP/s; twice, as a round that is not full
+        // runs at a higher clock (5000 rows, 100,003 x 2048: 3616 us with 3 parts, 3701 with the 8 that once would choose)
+        p.split_cost = static_cast<int>(4096 * 2 * (8.0 / 4.8e12) / (2.0 * static_cast<double>(p.piece) * (p.f32 ? 3 : 1) / 1.25e15)) + 1;
         p.acc = take(p.splits * rows * p.ld * 4);
     }
     if (pass == kLeavesUnit) {
