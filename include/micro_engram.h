@@ -687,7 +687,7 @@ int me_distill_backward(const void *logits, int dtype, int64_t n, int64_t vocab,
  *               backward. bf16: for the gradient of hidden alone (for_weight 0), what that only has to
  *               scale; a size of 0: the call is too small for that to pay (unit may still be given, n
  *               times dim rounded up to 4 values). fp32, up to 384 rows (1024 where vocab is small): the logits,
- *               for any gradient; a size of 0: unit is NULL
+ *               for any gradient; more rows: the head as it was laid out, up to 1 GiB; a size of 0: unit is NULL
  *   workspace   me_head_workspace_size bytes for the same n, vocab, dim, dtype, weight and w_stride, with pass
  *               0 for a forward, 1 for me_head_backward without unit, 2 for a forward with unit, 3 for
  *               me_head_backward with it (bf16: none), and smoothed != 0 for a forward with

@@ -58,7 +58,7 @@ constexpr int kIndexThreads = 1024;
 
 template <typename T>
 __global__ __launch_bounds__(kIndexThreads) void index_kernel(const T *targets, int64_t n, int64_t ignore, int64_t vocab,
-                                                              Saved s) {
+                                                              Saved s, uint32_t *clear) {
     __shared__ int sums[kIndexThreads / 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int at = 0;
@@ -84,6 +84,7 @@ __global__ __launch_bounds__(kIndexThreads) void index_kernel(const T *targets, 
         __syncthreads();
     }
     if (tid == 0) *s.count = at;
+    if (tid == 0 && clear != nullptr) *clear = 0;
 }
 
 // ---- what the gradient of a row's logits is made of ---------------------------------------------------------------
@@ -1426,12 +1427,13 @@ __global__ __launch_bounds__(256) void scale_kernel(const ScaleArgs a) {
 
 // ---- plan: sizes and places in the workspace ---------------------------------------------------------------------
 // the forward alone, the backward, the forward that leaves D or its logits, the backward that has them
-enum Pass { kStats, kBackward, kLeavesUnit, kHasUnit };
+enum Pass { kStats, kBackward, kLeavesUnit, kHasUnit };  // (or, of fp32 in parts, the laid-out head)
 
 struct Plan {
     int64_t n, rows, vocab, dim, ld;  // rows: n rounded up, at least 64; ld: dim rounded up to whole slabs
     bool f32, few, copy_w;            // copy_w: the head is laid out piece by piece
     int tile;                         // rows of a tile
+    bool keeps;                       // the laid-out head is the forward's for the backward too (keeps_head)
     bool rest;                        // the gradient's rows twice: as bf16, and what that leaves
     int np, nz;                       // parts of an operand: of the head's gradient; of the logits and the hidden states' gradient
     int64_t piece;                    // columns of the vocabulary at a time
@@ -1532,8 +1534,29 @@ bool takes_rest(int64_t n, bool f32) { return !f32 && n <= kFew; }
 
 int few_rows(int64_t n, int64_t vocab) { return n <= 64 || ceil_div(n, 64) * ceil_div(vocab, kTile) <= 256 ? 64 : 128; }
 
+// Whether a forward in parts leaves the laid-out head for the backward: up to 1 GiB of it (32,000 x 1024: 77 us of a
+// step's 1160 with 1023 rows, 2150 with 2048)
+bool keeps_head(int64_t n, int64_t vocab, int64_t dim, int dtype) {
+    return dtype == ME_F32 && n >= 1 && !takes_kept(n, vocab, dtype) && vocab * round_up(dim, kSlabK) * 4 <= kPieceBytes;
+}
+
+// The head in parts, as long as it is, with its scales and the largest of these
+struct KeptHead {
+    uint8_t *parts;
+    float *scale;
+    uint32_t *largest;
+    int64_t part, elements;  // part: bytes; elements: 4 bytes each, of all of it
+};
+
+KeptHead kept_head_of(float *unit, int64_t vocab, int64_t dim) {
+    const int64_t ld = round_up(dim, kSlabK), scales = round_up(vocab, 4) + kTile;
+    return {reinterpret_cast<uint8_t *>(unit), unit + vocab * ld, reinterpret_cast<uint32_t *>(unit + vocab * ld + scales), vocab * ld * 2, vocab * ld + scales + 4};
+}
+
 Plan plan_of(int64_t n, int64_t vocab, int64_t dim, int dtype, const void *weight, int64_t w_stride, Pass pass, bool smoothed) {
     Plan p{};
+    p.keeps = dtype == ME_F32 && (pass == kLeavesUnit || pass == kHasUnit);
+    if (p.keeps) pass = pass == kLeavesUnit ? kStats : kBackward;
     p.n = n, p.vocab = vocab, p.dim = dim, p.ld = round_up(dim, kSlabK);
     p.f32 = dtype == ME_F32;
     p.np = p.f32 ? 3 : 1;
@@ -1544,7 +1567,7 @@ Plan plan_of(int64_t n, int64_t vocab, int64_t dim, int dtype, const void *weigh
     p.tile = p.few ? few_rows(n, vocab) : kTile;
     const int64_t rows = p.rows = round_up(std::max<int64_t>(n, 1), 64);
     int64_t piece = round_up(vocab, kTile);
-    if (p.copy_w) piece = std::min(piece, std::max<int64_t>(kPieceBytes / (p.ld * 2 * p.nz) / 2048 * 2048, 2048));
+    if (p.copy_w && !p.keeps) piece = std::min(piece, std::max<int64_t>(kPieceBytes / (p.ld * 2 * p.nz) / 2048 * 2048, 2048));
     if (pass != kStats) piece = std::min(piece, std::max<int64_t>(kPieceBytes / (rows * (p.f32 ? 10 : 2)) / 2048 * 2048, 2048));
     // a launch holds fewer than 2^32 threads
     p.piece = std::min(piece, std::max<int64_t>((int64_t{1} << 23) / ceil_div(rows, p.tile) * kTile / 2048 * 2048, 2048));
@@ -1558,15 +1581,15 @@ Plan plan_of(int64_t n, int64_t vocab, int64_t dim, int dtype, const void *weigh
     p.factor = take(4);
     p.z = take(rows * p.ld * 2 * (p.rest ? 2 : p.nz));
     p.h = p.z;
-    if (p.copy_w) p.wz = take(p.piece * p.ld * 2 * p.nz);
+    if (p.copy_w && !p.keeps) p.wz = take(p.piece * p.ld * 2 * p.nz);
     if (p.f32) {
         p.row_scale = take(n * 4);
-        p.col_scale = take((p.piece + kTile) * 4);
+        if (!p.keeps) p.col_scale = take((p.piece + kTile) * 4);
         if (pass == kBackward) {
             p.h = take(rows * p.ld * 2 * p.np);
             p.half = take(rows * p.piece * 2 * p.nz);
             p.bound = take(n * 4);
-            p.largest = take(ceil_div(vocab, p.piece) * 4);
+            if (!p.keeps) p.largest = take(ceil_div(vocab, p.piece) * 4);
         }
     }
     if (pass != kBackward) {
@@ -1617,6 +1640,8 @@ struct Call {
     uint8_t *ws;
     Saved s;
     hipStream_t stream;
+    float *unit = nullptr;  // the laid-out head
+    bool laid_out = false;  // and it is there already
 };
 
 unsigned blocks_for(int64_t units) { return static_cast<unsigned>(std::min<int64_t>(std::max<int64_t>(ceil_div(units, 256), 1), 16384)); }
@@ -1667,6 +1692,13 @@ struct Head {
 Head head_of(const Plan &p, const Call &c, int64_t v0, int64_t width, uint32_t *largest = nullptr, const int32_t *gate = nullptr) {
     const uint8_t *from = static_cast<const uint8_t *>(c.weight) + v0 * c.w_stride * (p.f32 ? 4 : 2);
     if (!p.copy_w) return {{from, c.w_stride, 0}, nullptr};
+    if (p.keeps) {
+        const KeptHead k = kept_head_of(c.unit, p.vocab, p.dim);
+        uint8_t *to = k.parts + v0 * p.ld * 2;
+        const Layout l{from, width, 0, c.w_stride, nullptr, nullptr, width, p.dim, p.ld, k.part, to, 0, nullptr};
+        if (!c.laid_out) lay_out16(l, k.scale + v0, k.largest, c.stream);
+        return {{to, p.ld, k.part}, k.scale + v0};
+    }
     const int64_t part = p.piece * p.ld * 2;
     const Layout l{from, width, 0, c.w_stride, nullptr, nullptr, width, p.dim, p.ld, part, c.ws + p.wz, 0, gate};
     float *scale = p.f32 ? reinterpret_cast<float *>(c.ws + p.col_scale) : nullptr;
@@ -1953,16 +1985,19 @@ void forward_vectors(const KeptPlan &p, const Call &c, const Loss &l, int rows, 
     hipLaunchKernelGGL(finish_kernel<true>, dim3(static_cast<unsigned>(p.n)), dim3(256), 0, c.stream, f);
 }
 
-int forward(int64_t n, int64_t vocab, int64_t dim, int dtype, const Call &c, const Loss &l, size_t there) {
-    hipStream_t s = c.stream;
+int forward(int64_t n, int64_t vocab, int64_t dim, int dtype, const Call &call, const Loss &l, size_t there) {
+    hipStream_t s = call.stream;
     const Pass pass = l.unit ? kLeavesUnit : kStats;
     const bool smoothed = l.smoothing != 0.0, kept = takes_kept(n, vocab, dtype);
     KeptPlan q{};
     Plan p{};
     if (kept)
-        q = kept_plan_of(n, vocab, dim, c.weight, c.w_stride, pass, smoothed);
+        q = kept_plan_of(n, vocab, dim, call.weight, call.w_stride, pass, smoothed);
     else
-        p = plan_of(n, vocab, dim, dtype, c.weight, c.w_stride, pass, smoothed);
+        p = plan_of(n, vocab, dim, dtype, call.weight, call.w_stride, pass, smoothed);
+    Call c = call;
+    uint32_t *clear = nullptr;
+    if (p.keeps) c.unit = l.unit, clear = kept_head_of(l.unit, vocab, dim).largest;
     const int64_t needed = kept ? q.bytes : p.bytes, row_loss = kept ? q.row_loss : p.row_loss;
     ME_CHECK_ARG(there >= static_cast<size_t>(needed), "workspace of %zu bytes, %lld are needed", there, static_cast<long long>(needed));
     int rows;
@@ -1971,9 +2006,9 @@ int forward(int64_t n, int64_t vocab, int64_t dim, int dtype, const Call &c, con
         forward_vectors(q, c, l, rows, lds);
     } else {
         if (c.tdtype == ME_I64)
-            hipLaunchKernelGGL(index_kernel<int64_t>, dim3(1), dim3(kIndexThreads), 0, s, static_cast<const int64_t *>(c.targets), n, c.ignore, vocab, c.s);
+            hipLaunchKernelGGL(index_kernel<int64_t>, dim3(1), dim3(kIndexThreads), 0, s, static_cast<const int64_t *>(c.targets), n, c.ignore, vocab, c.s, clear);
         else
-            hipLaunchKernelGGL(index_kernel<int32_t>, dim3(1), dim3(kIndexThreads), 0, s, static_cast<const int32_t *>(c.targets), n, c.ignore, vocab, c.s);
+            hipLaunchKernelGGL(index_kernel<int32_t>, dim3(1), dim3(kIndexThreads), 0, s, static_cast<const int32_t *>(c.targets), n, c.ignore, vocab, c.s, clear);
         if (kept)
             forward_kept(q, c, l);
         else if (n > 0)
@@ -2019,7 +2054,7 @@ extern "C" int me_head_workspace_size(int64_t n, int64_t vocab, int64_t dim, int
         *bytes = static_cast<size_t>(kept_plan_of(n, vocab, dim, weight, w_stride, static_cast<Pass>(pass), smoothed != 0).bytes);
         return ME_OK;
     }
-    *bytes = pass == kHasUnit ? 0 : static_cast<size_t>(plan_of(n, vocab, dim, dtype, weight, w_stride, static_cast<Pass>(pass), smoothed != 0).bytes);
+    *bytes = pass == kHasUnit && dtype != ME_F32 ? 0 : static_cast<size_t>(plan_of(n, vocab, dim, dtype, weight, w_stride, static_cast<Pass>(pass), smoothed != 0).bytes);
     return ME_OK;
 }
 
@@ -2029,6 +2064,8 @@ extern "C" int me_head_unit_size(int64_t n, int64_t vocab, int64_t dim, int dtyp
     if (rc != ME_OK) return rc;
     if (takes_kept(n, vocab, dtype))
         *elements = n * kept_ld(vocab);
+    else if (keeps_head(n, vocab, dim, dtype))
+        *elements = kept_head_of(nullptr, vocab, dim).elements;
     else
         *elements = n > 0 && !for_weight && leaves_unit(n, vocab, dim, dtype) ? n * ceil_div(dim, 4) * 4 : 0;
     return ME_OK;
@@ -2041,7 +2078,8 @@ extern "C" int me_head_logps(const void *hidden, int dtype, int64_t n, int64_t d
     const int rc = check_call(hidden, dtype, n, dim, rows_per_batch, weight, vocab, w_stride, targets, targets_dtype, temperature, saved, workspace);
     if (rc != ME_OK) return rc;
     ME_CHECK_ARG(n == 0 || logps, "logps is needed");
-    ME_CHECK_ARG(reinterpret_cast<uintptr_t>(unit) % 16 == 0 && (!unit || dtype == ME_BF16 || takes_kept(n, vocab, dtype)), "unit must be 16-byte aligned, and is for bf16 or few rows");
+    ME_CHECK_ARG(reinterpret_cast<uintptr_t>(unit) % 16 == 0 && (!unit || dtype == ME_BF16 || takes_kept(n, vocab, dtype) || keeps_head(n, vocab, dim, dtype)),
+                 "unit must be 16-byte aligned, and NULL where its size is 0 in fp32");
     const Call c{hidden, weight, targets, rows_per_batch, batch_stride, row_stride, w_stride, ignore_index, targets_dtype,
                  static_cast<uint8_t *>(workspace), saved_of(saved, n), as_stream(stream)};
     return forward(n, vocab, dim, dtype, c, Loss{temperature, 0.0, 0.0, 1.0, 0, logps, nullptr, unit}, workspace_bytes);
@@ -2055,7 +2093,8 @@ extern "C" int me_head_ce(const void *hidden, int dtype, int64_t n, int64_t dim,
     if (rc != ME_OK) return rc;
     ME_CHECK_ARG(reduction == ME_REDUCE_MEAN || reduction == ME_REDUCE_SUM, "reduction must be mean or sum");
     ME_CHECK_ARG(loss, "loss is needed");
-    ME_CHECK_ARG(reinterpret_cast<uintptr_t>(unit) % 16 == 0 && (!unit || dtype == ME_BF16 || takes_kept(n, vocab, dtype)), "unit must be 16-byte aligned, and is for bf16 or few rows");
+    ME_CHECK_ARG(reinterpret_cast<uintptr_t>(unit) % 16 == 0 && (!unit || dtype == ME_BF16 || takes_kept(n, vocab, dtype) || keeps_head(n, vocab, dim, dtype)),
+                 "unit must be 16-byte aligned, and NULL where its size is 0 in fp32");
     const Call c{hidden, weight, targets, rows_per_batch, batch_stride, row_stride, w_stride, ignore_index, targets_dtype,
                  static_cast<uint8_t *>(workspace), saved_of(saved, n), as_stream(stream)};
     return forward(n, vocab, dim, dtype, c, Loss{temperature, smoothing, z_loss, scale, reduction == ME_REDUCE_MEAN, nullptr, loss, unit}, workspace_bytes);
@@ -2071,11 +2110,12 @@ extern "C" int me_head_backward(const void *hidden, int dtype, int64_t n, int64_
     if (rc != ME_OK) return rc;
     ME_CHECK_ARG(upstream || (n == 0 && upstream_per_row), "upstream is needed");
     ME_CHECK_ARG(reinterpret_cast<uintptr_t>(grad_hidden) % 16 == 0 && reinterpret_cast<uintptr_t>(grad_weight) % 16 == 0, "gradients must be 16-byte aligned");
-    ME_CHECK_ARG(!unit || (dtype == ME_BF16 && !grad_weight) || takes_kept(n, vocab, dtype), "unit is for the hidden states' gradient alone, or few rows of fp32");
+    ME_CHECK_ARG(!unit || (dtype == ME_BF16 ? !grad_weight : takes_kept(n, vocab, dtype) || keeps_head(n, vocab, dim, dtype)),
+                 "unit is for the hidden states' gradient alone in bf16, and NULL where its size is 0 in fp32");
     if (!grad_hidden && !grad_weight) return ME_OK;
     const Saved saved_rows = saved_of(const_cast<void *>(saved), n);
     const bool f32 = dtype == ME_F32;
-    if (unit && f32) {
+    if (unit && takes_kept(n, vocab, dtype)) {
         const KeptPlan q = kept_plan_of(n, vocab, dim, weight, w_stride, kHasUnit, false);
         ME_CHECK_ARG(workspace_bytes >= static_cast<size_t>(q.bytes), "workspace of %zu bytes, %lld are needed", workspace_bytes, static_cast<long long>(q.bytes));
         const Call c{hidden, weight, targets, rows_per_batch, batch_stride, row_stride, w_stride, ignore_index, targets_dtype,
@@ -2085,18 +2125,18 @@ extern "C" int me_head_backward(const void *hidden, int dtype, int64_t n, int64_
         backward_kept(q, c, coefs, unit, temperature, grad_hidden, grad_weight);
         return check_launch("me_head_backward");
     }
-    if (unit) {
+    if (unit && !f32) {
         if (n == 0) return ME_OK;
         const ScaleArgs a{unit, saved_rows.count, saved_rows.place, upstream, upstream_per_row != 0, reduction == ME_REDUCE_MEAN, scale / temperature, n, dim, grad_hidden};
         hipLaunchKernelGGL(scale_kernel, dim3(blocks_for(n * ceil_div(dim, 4))), dim3(256), 0, as_stream(stream), a);
         return check_launch("me_head_backward");
     }
-    const Plan p = plan_of(n, vocab, dim, dtype, weight, w_stride, kBackward, false);
+    const Plan p = plan_of(n, vocab, dim, dtype, weight, w_stride, unit ? kHasUnit : kBackward, false);
     ME_CHECK_ARG(workspace_bytes >= static_cast<size_t>(p.bytes), "workspace of %zu bytes, %lld are needed", workspace_bytes, static_cast<long long>(p.bytes));
     const Call c{hidden, weight, targets, rows_per_batch, batch_stride, row_stride, w_stride, ignore_index, targets_dtype,
-                 static_cast<uint8_t *>(workspace), saved_rows, as_stream(stream)};
+                 static_cast<uint8_t *>(workspace), saved_rows, as_stream(stream), const_cast<float *>(unit), true};
     hipStream_t s = c.stream;
-    uint32_t *largest = f32 ? reinterpret_cast<uint32_t *>(c.ws + p.largest) : nullptr;
+    uint32_t *largest = f32 && !p.keeps ? reinterpret_cast<uint32_t *>(c.ws + p.largest) : nullptr;
     RowGrad *grad = reinterpret_cast<RowGrad *>(c.ws + p.grad);
     Rows rows{};
     // bf16: factors that all rows share come in after the products, so that a target of no probability is -1, which
@@ -2105,7 +2145,7 @@ extern "C" int me_head_backward(const void *hidden, int dtype, int64_t n, int64_
     if (n > 0) {
         const Coefs coefs{c.s, upstream, upstream_per_row != 0, reduction == ME_REDUCE_MEAN, scale / temperature, static_cast<float>(smoothing),
                           static_cast<float>(z_loss), static_cast<double>(vocab), factor, grad, f32 ? reinterpret_cast<float *>(c.ws + p.bound) : nullptr,
-                          largest, f32 ? static_cast<int>(ceil_div(vocab, p.piece)) : 0};
+                          largest, largest ? static_cast<int>(ceil_div(vocab, p.piece)) : 0};
         rows = lay_out_rows(p, c, coefs);
         if (f32 && grad_weight) lay_out(true, hidden_layout(p, c, p.h), s);
     }
@@ -2113,7 +2153,7 @@ extern "C" int me_head_backward(const void *hidden, int dtype, int64_t n, int64_
     for (int64_t v0 = 0; v0 < vocab; v0 += p.piece) {
         const int64_t width = std::min(p.piece, vocab - v0);
         if (n > 0) {
-            uint32_t *widest = f32 ? largest + v0 / p.piece : nullptr;
+            uint32_t *widest = p.keeps ? kept_head_of(c.unit, vocab, dim).largest : f32 ? largest + v0 / p.piece : nullptr;
             const Head w = head_of(p, c, v0, width, widest);
             const bool for_hidden = grad_hidden != nullptr, for_weight = grad_weight != nullptr;
             if (f32)

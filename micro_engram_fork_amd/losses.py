@@ -433,7 +433,8 @@ def head_token_logps(hidden, weight, targets, temperature=1.0, ignore_index=IGNO
     Memory, during a call: statistics of a 32nd of the bf16 logits' size, and with gradients a piece of the logits' gradient
     (at most 1 GiB up to 262,144 bf16 rows). Heads in fp32, or whose bf16 rows do not start and end at multiples of 16 bytes, are
     laid out a piece at a time as well (again at most 1 GiB); but few rows in fp32 (up to 384, or 1,024 with a small vocabulary)
-    read the head as it lies and keep their logits for the backward, n x vocab in fp32. Rows that do not count cost nothing and are not read.
+    read the head as it lies and keep their logits for the backward, n x vocab in fp32. For gradients in fp32 a laid-out head of
+    up to 1 GiB stays from the forward to the backward. Rows that do not count cost nothing and are not read.
     For the gradient of bf16 hidden states alone (a frozen head), larger calls make it in the forward, which saves one of
     three products, and keep it for the backward in fp32 before its upstream factors."""
     _check_head(hidden, weight, targets)

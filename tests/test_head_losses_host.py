@@ -72,9 +72,10 @@ def test_what_a_forward_leaves_for_the_gradient_of_hidden_alone():
     assert head_ops.unit_elements(3, 262_144, 5_375, _lib.ME_BF16, head_ops.NO_GRADIENT) == 0
     for of in (head_ops.OF_HIDDEN, head_ops.OF_WEIGHT):  # few rows of fp32: their logits
         assert head_ops.unit_elements(384, 262_144, 64, _lib.ME_F32, of) == 384 * (262_144 + 64)
-        assert head_ops.unit_elements(385, 262_144, 64, _lib.ME_F32, of) == 0
+        assert head_ops.unit_elements(385, 262_144, 64, _lib.ME_F32, of) == 262_144 * 64 + 262_144 + 256 + 4  # the head in parts
+        assert head_ops.unit_elements(385, 262_144, 1_025, _lib.ME_F32, of) == 0
         assert head_ops.unit_elements(1024, 301, 64, _lib.ME_F32, of) == 1024 * 320
-        assert head_ops.unit_elements(1025, 301, 64, _lib.ME_F32, of) == 0
+        assert head_ops.unit_elements(1025, 301, 64, _lib.ME_F32, of) == 301 * 64 + 304 + 256 + 4
         assert head_ops.unit_elements(0, 301, 64, _lib.ME_F32, of) == 0
     with FakeTensorMode():
         hidden, weight, targets = _args(rows=(4096,), vocab=32_000, dim=1_024)
