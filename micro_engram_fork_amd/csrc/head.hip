@@ -876,10 +876,10 @@ __global__ __launch_bounds__(256) void vector_kernel(const VectorArgs a) {
 // the head: the logits stay, in fp32, for the backward. So a forward and the gradients of both operands read the head
 // twice and write its gradient, which nothing can do without. Bound by these up to some 30 rows; 262,144 x 5376 (5.6 GB), us:
 //   rows   logits   product with dz   outer product
-//     12     1024             1220            1361     5.5, 4.6 and 4.1 TB/s
-//     46     1214             1740            1993
-//    128     2330             2750            3100     beyond, by matrix and vector instructions that wait for each other
-// (laid out in parts instead: 12 rows 11,500 us in all, here 3370)
+//     12     1028             1171            1344     5.5, 4.8 and 4.2 TB/s
+//     46     1209             1672            1978
+//    128     2294             2775            3057     beyond, by matrix and vector instructions that wait for each other
+// (laid out in parts instead: 12 rows 11,500 us in all, here 3270)
 constexpr int kKeptCols = 2048;  // logits of a workgroup: 8 of a thread
 
 struct KeptArgs {
