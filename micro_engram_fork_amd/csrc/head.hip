@@ -1122,6 +1122,7 @@ struct FinishArgs {
     float *logps;        // by source row, or null
     float *row_loss;     // by counted row, or null
     float smoothing, z_loss;
+    RowGrad *grad;       // of z itself, for rows that are made again: a q, nothing at the target; or null
     int uncounted;       // the logps of source rows that do not count are written too: zeros
 };
 
@@ -1176,6 +1177,7 @@ __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs a) {
     a.s.lse2[c] = lse2;
     a.s.others[c] = d != d ? d : others;
     if (a.logps) a.logps[a.s.rows[c]] = -nll;
+    if (a.grad) a.grad[r] = {lse2, 1.f + 2.f * a.z_loss * static_cast<float>(kLn2) * lse2, 0.f, 0.f};
     if (a.row_loss) {
         const float lse = static_cast<float>(kLn2) * lse2;
         float loss = nll + a.z_loss * lse * lse;
@@ -1327,14 +1329,6 @@ __global__ __launch_bounds__(kIndexThreads) void redo_kernel(const RedoArgs a) {
         __syncthreads();
     }
     if (tid == 0) *a.count = at;
-}
-
-// Gradient of z itself for the rows that are made again: a q, nothing at the target
-__global__ __launch_bounds__(256) void redo_coef_kernel(Saved s, const int32_t *count, const int32_t *rows, float z_loss, RowGrad *grad) {
-    const int r = static_cast<int>(blockIdx.x) * 256 + static_cast<int>(threadIdx.x);
-    if (r >= *count) return;
-    const float lse2 = s.lse2[rows[r]];
-    grad[r] = {lse2, 1.f + 2.f * z_loss * static_cast<float>(kLn2) * lse2, 0.f, 0.f};
 }
 
 // Sums of the head's columns, which a smoothed target's gradient takes in: chunks of rows, then over the chunks
@@ -1804,8 +1798,6 @@ struct Loss {
     float *unit;          // D, or null
 };
 
-unsigned row_blocks(int64_t n) { return static_cast<unsigned>(std::max<int64_t>(ceil_div(n, 256), 1)); }
-
 // D from the sums of the products with the head
 void unit_of(const Plan &p, const Call &c, const Loss &l, const Rows &rows, const int32_t *which, const float *ref) {
     UnitArgs u{};
@@ -1886,9 +1878,8 @@ void forward_rows(const Plan &p, const Call &c, const Loss &l) {
     hipLaunchKernelGGL(redo_kernel, dim3(1), dim3(kIndexThreads), 0, s, RedoArgs{c.s, ref, rows.tgt, redo, redo + kHeader, tgt2});
     lay_out(false, Layout{rows.h, p.n, 0, p.ld, redo + kHeader, redo, p.n, p.ld, p.ld, 0, again.h, 0, nullptr}, s);
     stats_of<F32>(p, c, again, e, redo);
-    f.uncounted = 0, f.exps = nullptr, f.ref = nullptr, f.count = redo, f.which = redo + kHeader;
+    f.uncounted = 0, f.exps = nullptr, f.ref = nullptr, f.count = redo, f.which = redo + kHeader, f.grad = grad;
     finish(p, f, s);
-    hipLaunchKernelGGL(redo_coef_kernel, dim3(row_blocks(p.n)), dim3(256), 0, s, c.s, redo, redo + kHeader, f.z_loss, grad);
     for (int64_t v0 = 0; v0 < p.vocab; v0 += p.piece) {
         const int64_t width = std::min(p.piece, p.vocab - v0);
         const Head w = head_of(p, c, v0, width, nullptr, redo);
