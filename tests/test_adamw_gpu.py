@@ -402,3 +402,19 @@ def test_the_state_of_torchs_adamw_goes_on():
     before = _before(opt, [p], 32)
     opt.step()
     _check_step(opt, [p], before, 2, 32)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_more_values_than_32_bits_count(bits):
+    """A first step moves each value with a gradient by the learning rate, against its sign, and no other."""
+    p = torch.nn.Parameter(torch.zeros(2_200_000_123, device="cuda", dtype=torch.bfloat16))
+    p.grad = torch.zeros_like(p)
+    at = torch.tensor([0, 4_095, 2_147_483_647, 2_147_483_648, 2_199_999_990, 2_200_000_122], device="cuda")
+    p.grad[at] = torch.tensor([1.0, -1.0, 2.0, -3.0, 1.0, -0.5], device="cuda", dtype=torch.bfloat16)
+    DenseAdamW([p], lr=2.0 ** -7, state_bits=bits, weight_decay=0.0, seed=1).step()
+    with torch.no_grad():
+        # m / (sqrt(v) + eps) is 1 but for eps / |g|, the quotient's roundings and that of the weight, 2^-7 at most
+        assert torch.allclose(p[at].float(), -(2.0 ** -7) * p.grad[at].float().sign(), rtol=2.0 ** -7 + 1e-6, atol=0.0)
+        assert int(p.count_nonzero()) == len(at)
+    del p
+    torch.cuda.empty_cache()

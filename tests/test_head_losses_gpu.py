@@ -582,3 +582,15 @@ def test_compiled_for_any_number_of_rows(dtype):
         g, = torch.autograd.grad(f(h[:n], targets[:n]), h)
         want, = torch.autograd.grad(losses.head_cross_entropy(h[:n] * 2, weight, targets[:n]), h)
         assert torch.equal(g, want), n
+
+
+def test_offsets_past_32_bits():
+    """Heads of more than 4 GiB, and their gradient: the last rows are where they belong."""
+    try:
+        _check_logps(*_inputs(12, 262_144, 4_200, FP32))
+        torch.cuda.empty_cache()
+        _check_hidden_alone(*_inputs(390, 262_144, 4_200, FP32))
+        torch.cuda.empty_cache()
+        _check_hidden_alone(*_inputs(70, 420_001, 5_376, BF16))
+    finally:
+        torch.cuda.empty_cache()
