@@ -550,7 +550,7 @@ struct GradEpilogue {
         // 32 rows at a time through LDS, where a wave has two places in turn (with parts one: a wave's LDS
         // accesses keep their order)
         constexpr int kPitch = 64 * SX + 16, kPlaces = PARTS > 1 ? 1 : 2;
-        static_assert(4 * kPlaces * kParts * 32 * kPitch <= (SX == 4 ? kRingBytes : 3 * kUnit), "the stage fits the ring");
+        static_assert(4 * kPlaces * kParts * 32 * kPitch <= (SX == 4 ? kRingBytes : SX == 2 ? 3 * kUnit : 2 * kUnit), "the stage fits the ring");
 #pragma unroll
         for (int y = 0; y < SY; ++y) {
             uint8_t *stage = lds + ((threadIdx.x >> 6) * kPlaces + (y % kPlaces)) * (kParts * 32 * kPitch);
@@ -1426,7 +1426,7 @@ enum Pass { kStats, kBackward, kLeavesUnit, kHasUnit };  // (or, of fp32 in part
 struct Plan {
     int64_t n, rows, vocab, dim, ld;  // rows: n rounded up, at least 64; ld: dim rounded up to whole slabs
     bool f32, few, copy_w;            // copy_w: the head is laid out piece by piece
-    int tile;                         // rows of a tile
+    int tile, cols;                   // rows of a tile, and columns of one of logits
     bool keeps;                       // the laid-out head is the forward's for the backward too (keeps_head)
     bool rest;                        // the gradient's rows twice: as bf16, and what that leaves
     int np, nz;                       // parts of an operand: of the head's gradient; of the logits and the hidden states' gradient
@@ -1547,6 +1547,9 @@ KeptHead kept_head_of(float *unit, int64_t vocab, int64_t dim) {
     return {reinterpret_cast<uint8_t *>(unit), unit + vocab * ld, reinterpret_cast<uint32_t *>(unit + vocab * ld + scales), vocab * ld * 2, vocab * ld + scales + 4};
 }
 
+// Columns of a wave's statistics
+int part_cols(const Plan &p) { return p.few ? p.cols / 4 : 128; }
+
 Plan plan_of(int64_t n, int64_t vocab, int64_t dim, int dtype, const void *weight, int64_t w_stride, Pass pass, bool smoothed) {
     Plan p{};
     p.keeps = dtype == ME_F32 && (pass == kLeavesUnit || pass == kHasUnit);
@@ -1559,6 +1562,9 @@ Plan plan_of(int64_t n, int64_t vocab, int64_t dim, int dtype, const void *weigh
     p.rest = pass == kBackward && takes_rest(n, p.f32);
     p.copy_w = p.f32 || dim % 8 != 0 || w_stride % 8 != 0 || reinterpret_cast<uintptr_t>(weight) % 16 != 0;
     p.tile = p.few ? few_rows(n, vocab) : kTile;
+    // tiles of 256 / 128 columns, us, log-probabilities or loss alone of 48 rows: 5,000 x 5376 68 / 50, 10,000 x 2048 38 / 30,
+    // 25,000 x 4096 57 / 45, 32,000 x 1024 29 / 29
+    p.cols = p.few && ceil_div(n, p.tile) * ceil_div(vocab, kTile) <= 128 ? 128 : kTile;
     const int64_t rows = p.rows = round_up(std::max<int64_t>(n, 1), 64);
     int64_t piece = round_up(vocab, kTile);
     if (p.copy_w && !p.keeps) piece = std::min(piece, std::max<int64_t>(kPieceBytes / (p.ld * 2 * p.nz) / 2048 * 2048, 2048));
@@ -1587,7 +1593,7 @@ Plan plan_of(int64_t n, int64_t vocab, int64_t dim, int dtype, const void *weigh
         }
     }
     if (pass != kBackward) {
-        const int64_t parts = std::max<int64_t>(ceil_div(vocab, p.few ? 64 : 128) + 4, n <= kVectorRows ? kVectorGroups : 0);
+        const int64_t parts = std::max<int64_t>(ceil_div(vocab, part_cols(p)) + 4, n <= kVectorRows ? kVectorGroups : 0);
         p.part = take(parts * rows * 8);
         if (smoothed) p.sum = take(parts * rows * 4);
         p.at_target = take(n * 4);
@@ -1709,16 +1715,22 @@ void multiply_large(const Gemm &g, const Epilogue &e, hipStream_t s) {
     hipLaunchKernelGGL((large_kernel<A_KC, B_KC, SEGS, Epilogue>), grid, dim3(kThreads), 0, s, g, e);
 }
 
-template <bool B_KC, int SEGS, class Epilogue>
+template <bool B_KC, int TS, int SEGS, class Epilogue>
 void multiply_few(int tile, const Gemm &g, const Epilogue &e, hipStream_t s) {
-    const dim3 grid(static_cast<unsigned>(workgroups(g, tile, kTile)));
+    const dim3 grid(static_cast<unsigned>(workgroups(g, tile, TS)));
     if constexpr (SEGS == 1) {  // parts: 64 rows alone (takes_few)
         if (tile == 128) {
-            hipLaunchKernelGGL((few_kernel<B_KC, 4, 1, 16, Epilogue>), grid, dim3(kThreads), 0, s, g, e);
+            hipLaunchKernelGGL((few_kernel<B_KC, 4, TS, 1, 16, Epilogue>), grid, dim3(kThreads), 0, s, g, e);
             return;
         }
     }
-    hipLaunchKernelGGL((few_kernel<B_KC, 2, SEGS, 16, Epilogue>), grid, dim3(kThreads), 0, s, g, e);
+    hipLaunchKernelGGL((few_kernel<B_KC, 2, TS, SEGS, 16, Epilogue>), grid, dim3(kThreads), 0, s, g, e);
+}
+
+// logits of few rows
+template <int SEGS, class Epilogue>
+void few_logits(const Plan &p, const Gemm &g, const Epilogue &e, hipStream_t s) {
+    p.cols == 128 ? multiply_few<true, 128, SEGS>(p.tile, g, e, s) : multiply_few<true, kTile, SEGS>(p.tile, g, e, s);
 }
 
 // fp32 as it lies
@@ -1726,14 +1738,14 @@ template <bool B_KC, int PIECE>
 void multiply_kept(int tile, const Gemm &g, const AccumulateEpilogue &e, hipStream_t s) {
     const dim3 grid(static_cast<unsigned>(workgroups(g, tile, kTile)));
     if (tile == 32)
-        hipLaunchKernelGGL((few_kernel<B_KC, 1, 0, PIECE, AccumulateEpilogue>), grid, dim3(kThreads), 0, s, g, e);
+        hipLaunchKernelGGL((few_kernel<B_KC, 1, kTile, 0, PIECE, AccumulateEpilogue>), grid, dim3(kThreads), 0, s, g, e);
     else if (B_KC || tile == 64)
-        hipLaunchKernelGGL((few_kernel<B_KC, 2, 0, PIECE, AccumulateEpilogue>), grid, dim3(kThreads), 0, s, g, e);
+        hipLaunchKernelGGL((few_kernel<B_KC, 2, kTile, 0, PIECE, AccumulateEpilogue>), grid, dim3(kThreads), 0, s, g, e);
     else if constexpr (!B_KC) {
         if (tile == 96)
-            hipLaunchKernelGGL((few_kernel<false, 3, 0, PIECE, AccumulateEpilogue>), grid, dim3(kThreads), 0, s, g, e);
+            hipLaunchKernelGGL((few_kernel<false, 3, kTile, 0, PIECE, AccumulateEpilogue>), grid, dim3(kThreads), 0, s, g, e);
         else
-            hipLaunchKernelGGL((few_kernel<false, 4, 0, PIECE, AccumulateEpilogue>), grid, dim3(kThreads), 0, s, g, e);
+            hipLaunchKernelGGL((few_kernel<false, 4, kTile, 0, PIECE, AccumulateEpilogue>), grid, dim3(kThreads), 0, s, g, e);
     }
 }
 
@@ -1747,7 +1759,7 @@ template <int SEGS, class Epilogue>
 void logits_of(const Plan &p, const Call &c, const Rows &rows, const Head &w, int64_t width, const Epilogue &e) {
     const Gemm g{{rows.h, p.ld, h_part(p)}, w.w, p.n, width, p.dim, rows.count, 0, 8, 1, 0};
     if (p.few)
-        multiply_few<true, SEGS>(p.tile, g, e, c.stream);
+        few_logits<SEGS>(p, g, e, c.stream);
     else
         multiply_large<true, true, SEGS>(g, e, c.stream);
 }
@@ -1759,7 +1771,7 @@ void times_head(const Plan &p, const Call &c, const Rows &rows, const Head &w, i
     const AccumulateEpilogue e{reinterpret_cast<float *>(c.ws + p.acc), p.ld, p.rows * p.ld, v0 > 0,
                                p.f32 ? reinterpret_cast<const float *>(c.ws + p.bound) : nullptr, largest};
     if (p.few)
-        p.f32 ? multiply_few<false, 3>(p.tile, g, e, c.stream) : multiply_few<false, 1>(p.tile, g, e, c.stream);
+        p.f32 ? multiply_few<false, kTile, 3>(p.tile, g, e, c.stream) : multiply_few<false, kTile, 1>(p.tile, g, e, c.stream);
     else
         p.f32 ? multiply_large<true, false, 3>(g, e, c.stream) : multiply_large<true, false, 1>(g, e, c.stream);
 }
@@ -1778,7 +1790,7 @@ void gradient_of(const Plan &p, const Call &c, const Rows &rows, const Head &w, 
                                 p.rows * p.piece * 2, v0, width, k};
     if constexpr (PARTS == 2) {  // few rows
         const Gemm g{{rows.h, p.ld, 0}, w.w, p.n, width, p.dim, rows.count, 0, 8, 1, 0};
-        multiply_few<true, 1>(p.tile, g, e, c.stream);
+        few_logits<1>(p, g, e, c.stream);
     } else {
         logits_of<PARTS>(p, c, rows, w, width, e);
     }
@@ -1827,7 +1839,7 @@ template <bool F32>
 void forward_rows(const Plan &p, const Call &c, const Loss &l) {
     hipStream_t s = c.stream;
     const Rows rows = lay_out_rows(p, c);
-    const int cols = p.few ? 64 : 128;
+    const int cols = part_cols(p);
     const int parts = static_cast<int>(ceil_div(p.vocab, cols));
     const float k = static_cast<float>(1.44269504088896340736 / l.temperature);
     float *at_target = reinterpret_cast<float *>(c.ws + p.at_target);

@@ -511,9 +511,10 @@ __global__ __launch_bounds__(kThreads, 1) void large_kernel(const Gemm a, const 
 // exponentials, 459 from the head's other side, 5.8 and 6.1 TB/s). SEGS 0: fp32 as it lies, PIECE as of Loader;
 // k-contiguous heads then in two slots, for two workgroups per CU whose reads, splits and products take turns (46
 // rows, 262,144 x 5376: 1208 us, with three slots and one workgroup 1485; row-contiguous ones 1637 and 1556).
-template <bool B_KC, int BR, int SEGS, int PIECE, class Epilogue>
+// TS: columns of a tile, 256 or, where that would leave CUs without one, 128.
+template <bool B_KC, int BR, int TS, int SEGS, int PIECE, class Epilogue>
 __global__ __launch_bounds__(kThreads) void few_kernel(const Gemm a, const Epilogue epi) {
-    constexpr int kTR = 32 * BR, kTS = 256, kRing = SEGS == 0 && B_KC ? 2 : 3, kEl = kElement<SEGS>, kStep = kSlab<SEGS>;
+    constexpr int kTR = 32 * BR, kTS = TS, kRing = SEGS == 0 && B_KC ? 2 : 3, kEl = kElement<SEGS>, kStep = kSlab<SEGS>;
     constexpr int kBS = kTS / 128;                         // 32-wide subtiles of a wave's columns
     constexpr int kUnitA = kTR * kSlabBytes;
     constexpr int kSlot = (kTR + kTS) * kSlabBytes;
@@ -587,8 +588,9 @@ __global__ __launch_bounds__(kThreads) void few_kernel(const Gemm a, const Epilo
                         return f;
                     }
                 };
-                const Parts fs[kBS] = {Parts(take_b(0)), Parts(take_b(1))};
-                static_assert(kBS == 2, "two subtiles");
+                Parts fs[kBS];
+#pragma unroll
+                for (int x = 0; x < kBS; ++x) fs[x] = Parts(take_b(x));
 #pragma unroll
                 for (int y = 0; y < BR; ++y) {
                     const Parts fr(kc_frag_f32(ua, ks, 32 * y + (lane & 31), lane));
